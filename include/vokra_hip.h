@@ -402,6 +402,131 @@ int vokra_hip_paged_attn_dev(vokra_hip_ctx_t *ctx, vokra_hip_kv_t *kv, size_t la
                              const int32_t *d_streams, const int32_t *d_lens, size_t max_len, size_t n_head_q,
                              const float *d_q, float scale, float *d_out);
 
+/* ---- block-scaled KV cache ------------------------------------------------- */
+
+/* A paged KV cache of sequences that share pages, held in 8 bits with one
+ * scale for each block of block_size tokens, head and side (K, V). No
+ * counterpart in the reference (its caches scale every 32 values and page by
+ * time over all streams, crates/vokra-core/src/cache/paged_quant.rs:152-545):
+ * here a page is one block of one sequence in every layer, so sequences fork
+ * without copying it and give it back on their own.
+ *
+ * A full block is rounded by its largest magnitude a = max |x| over its
+ * block_size x d_head values, in f32 operations rounded once, ties to even:
+ *   INT8: scale a / 127, values rint(x * (127 / a));
+ *   E4M3: scale a / 448, values e4m3(x * (448 / a)) (OCP, largest 448);
+ * a < 2^-100 holds zeros; a block with a value that is not finite reads as NaN
+ * throughout. The rows of the block that is not full yet are held as they came
+ * (f32). So each value is rounded once, and what the cache holds does not
+ * depend on how rows were split over steps. */
+typedef enum vokra_hip_bkv_codec_t { VOKRA_HIP_BKV_INT8 = 0, VOKRA_HIP_BKV_E4M3 = 1 } vokra_hip_bkv_codec_t;
+typedef struct vokra_hip_bkv vokra_hip_bkv_t;
+
+/* n_seq sequences (<= 65535) of up to max_time rows (<= 2^24), n_page pages
+ * (<= 2^26) for all of them, steps of up to max_rows new rows (<= 2^20).
+ * d_head 64 or 128 and block_size 16, 32 or 64 (else UNSUPPORTED_OP). Device
+ * memory: n_layer * n_head * (n_page * (2 * block_size * d_head + 8) + n_seq *
+ * 16 * block_size * d_head) bytes and some tables; 34 or 68 MB for split
+ * attention. Nothing is allocated by the _dev calls, so all of them can be
+ * captured into a graph. A cache belongs to its context's stream: calls on one
+ * cache run in the order in which they are made. */
+int vokra_hip_bkv_create(vokra_hip_ctx_t *ctx, size_t n_layer, size_t n_head, size_t d_head, size_t n_seq,
+                         size_t max_time, size_t block_size, size_t n_page, size_t max_rows, int codec,
+                         vokra_hip_bkv_t **out);
+void vokra_hip_bkv_destroy(vokra_hip_bkv_t *kv);
+/* Every sequence empty, every page free. */
+int vokra_hip_bkv_reset(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv);
+
+/* Begins a step: sequence seqs[i] takes counts[i] >= 0 rows from position
+ * starts[i] on, i < n <= 1024, and pages are taken for the blocks that become
+ * full. starts[i] is the sequence's length, or a lower position, which takes
+ * the sequence back to it first (drafted tokens that were not accepted): back
+ * to the first row of the block before the newest one (of the newest full
+ * block's end, for a forked sequence) at most. Pages that it gives up so are
+ * free for the next call. The rows of the step are packed: item i's are rows
+ * sum(counts[0..i-1]) and on of write's, attn's arrays.
+ * The first item that names no sequence, names one that an earlier item names,
+ * has a start or count out of range (INVALID_ARGUMENT), or finds too few free
+ * pages (KV_CACHE_EXHAUSTED) ends the step before it: earlier items stay,
+ * it and later ones are left as they were, and write and attn pass over their
+ * rows. Host arrays, synchronous; a step of more than max_rows rows is refused
+ * as a whole. */
+int vokra_hip_bkv_step(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t n, const int32_t *seqs,
+                       const int32_t *starts, const int32_t *counts);
+/* Device arrays, asynchronous; the outcome is read by bkv_status. n_rows bounds
+ * the sum of counts and max_count each of them (an item beyond either is
+ * INVALID_ARGUMENT); max_len, the longest sequence after the step, only sizes
+ * the attention's split. In a graph: a captured write or attn covers steps of
+ * at most the n, n_rows and max_count that the last step before its capture
+ * was given. */
+int vokra_hip_bkv_step_dev(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t n, size_t n_rows, size_t max_count,
+                           size_t max_len, const int32_t *d_seqs, const int32_t *d_starts, const int32_t *d_counts);
+/* Synchronizes; the outcome of the last step, fork, free, copy (on its
+ * destination cache) or compact, with the items that were done in *n_done
+ * (the pages moved, for compact; may be NULL). */
+int vokra_hip_bkv_status(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t *n_done);
+
+/* The step's rows of one layer, k and v [rows][n_head * d_head], into the
+ * cache. Every layer is written once a step, before that layer's attn. */
+int vokra_hip_bkv_write(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t layer, const float *k_rows,
+                        const float *v_rows);
+/* Device arrays (16-byte aligned), asynchronous. */
+int vokra_hip_bkv_write_dev(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t layer, const float *d_k,
+                            const float *d_v);
+/* Attention of the step's rows: the row at position p of its sequence attends
+ * to rows 0..p as the cache holds them,
+ *   out = softmax((q * scale) . K^T) . V,
+ * query head h with kv head h / (n_head_q / n_head); q, out [rows][n_head_q *
+ * d_head], n_head_q any multiple of n_head. f32 in and out: products of a query
+ * or a weight with 8-bit values run as two fp16 parts of the f32 operand (22
+ * bits), those with f32 rows in f32, sums in f32. Rows that the step does not
+ * reach are left as they are. One token a sequence, several (drafts) and long
+ * chunks of prompts take the same call. */
+int vokra_hip_bkv_attn(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t layer, size_t n_head_q, const float *q,
+                       float scale, float *out);
+/* Device arrays (16-byte aligned), asynchronous. */
+int vokra_hip_bkv_attn_dev(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t layer, size_t n_head_q,
+                           const float *d_q, float scale, float *d_out);
+/* Rows as the cache holds them: row (seqs[i], times[i]) of `layer` into
+ * k_out, v_out [n][n_head * d_head]; zeros where no row is held. */
+int vokra_hip_bkv_read(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t layer, size_t n, const int32_t *seqs,
+                       const int32_t *times, float *k_out, float *v_out);
+/* Device arrays (outputs 16-byte aligned), asynchronous. */
+int vokra_hip_bkv_read_dev(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t layer, size_t n, const int32_t *d_seqs,
+                           const int32_t *d_times, float *d_k, float *d_v);
+
+/* The four calls below end before the first item that fails, as a step does.
+ *
+ * fork: sequence dst[i] becomes what src[i] is. Full blocks are shared, the
+ * open block's rows are copied. dst[i] must be empty (freed), named once, and
+ * no source of the call's (INVALID_ARGUMENT). */
+int vokra_hip_bkv_fork(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t n, const int32_t *src, const int32_t *dst);
+int vokra_hip_bkv_fork_dev(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t n, const int32_t *d_src,
+                           const int32_t *d_dst);
+/* free: the sequences are empty again; a page goes back when the last sequence
+ * that holds it does. An empty sequence, or one named again, is no error. Ends
+ * the current step. */
+int vokra_hip_bkv_free(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t n, const int32_t *seqs);
+int vokra_hip_bkv_free_dev(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t n, const int32_t *d_seqs);
+/* copy: sequence dst[i] of dst_kv becomes a copy of src[i] of src_kv with pages
+ * of its own (from a prompt's cache to the one that serves it, or to a smaller
+ * or larger cache). The caches are of one context and agree in layers, heads,
+ * d_head, block_size and codec; dst as in fork, and KV_CACHE_EXHAUSTED where
+ * dst_kv has too few free pages. */
+int vokra_hip_bkv_copy(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *dst_kv, vokra_hip_bkv_t *src_kv, size_t n,
+                       const int32_t *src, const int32_t *dst);
+int vokra_hip_bkv_copy_dev(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *dst_kv, vokra_hip_bkv_t *src_kv, size_t n,
+                           const int32_t *d_src, const int32_t *d_dst);
+/* compact: the u pages in use become pages 0..u-1 (the k-th one at or above u
+ * moves to the k-th free one below u, in every layer). Contents, lengths and
+ * the current step stay. Asynchronous. */
+int vokra_hip_bkv_compact(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv);
+/* Rows that a sequence holds; free pages and pages in use; the page of a
+ * sequence's full block, -1 if there is none. Synchronous. */
+int vokra_hip_bkv_length(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t seq, size_t *length);
+int vokra_hip_bkv_pages(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t *free_pages, size_t *pages_in_use);
+int vokra_hip_bkv_page_of(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t seq, size_t block, long *page);
+
 /* out = a + b on device (residual connections; add_assign in the reference's
  * model code, crates/vokra-models/src/whisper/nn.rs). */
 int vokra_hip_add_f32_dev(vokra_hip_ctx_t *ctx, const float *d_a, const float *d_b, float *d_out, size_t n);

@@ -1,0 +1,711 @@
+// vk_bkv.hip — the block-scaled KV cache for gfx950: planning (pages, lengths,
+// steps), the write of rows, reading back, and the moving of pages.
+//
+// A page holds one block of bs tokens of one sequence, for every layer, head
+// and side (K, V), in 8 bits under one f32 scale per (layer, head, side):
+//   a = max |x| over the block (bs x hd values),
+//   int8: scale a / 127, value rint(x * (127 / a));
+//   e4m3: scale a / 448, value e4m3(x * (448 / a)),
+// each operation an f32 operation rounded once, ties to even. a < 2^-100 holds
+// zeros under scale 0 (127 / a would leave f32's range for the smallest a); a
+// block with a value that is not finite holds zeros under a NaN scale, so it
+// reads as NaN.
+//
+// Only a full block is rounded: the rows of the block that is still open stay
+// as they came (f32, in the ring of the sequence's last two blocks). So every
+// value is rounded once, by the largest value of its own block, and what the
+// cache holds does not depend on how the rows were split over calls; a page
+// never changes once it is written, so sequences may share it, and a fork
+// copies one row of the page table and the open block's rows.
+//
+// Planning is one workgroup (items are at most 1024, one thread each): checks,
+// prefix sums over the pages that the items take, pages from a bitmap (lowest
+// first, so the result does not depend on the order of earlier frees). The
+// first item that fails ends the call; the ones before it stay done.
+#include <algorithm>
+#include <climits>
+
+#include "../../include/vokra_hip.h"
+#include "vk_bkv.h"
+#include "vk_common.h"
+
+namespace vk {
+
+constexpr int BKV_TPB = 1024;
+
+// ---- workgroup prefix sums ----------------------------------------------------
+
+// Exclusive prefix sum over the 1024 threads; *total = the sum. red: 17 ints.
+__device__ __forceinline__ int bkv_scan(int v, int* red, int* total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o, VK_WAVE);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) red[wave] = x;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int s = 0;
+        for (int w = 0; w < BKV_TPB / 64; ++w) {
+            const int t = red[w];
+            red[w] = s;
+            s += t;
+        }
+        red[BKV_TPB / 64] = s;
+    }
+    __syncthreads();
+    *total = red[BKV_TPB / 64];
+    return red[wave] + x - v;
+}
+
+// The last index i in [0, n) with off[i] <= k (off ascending, off[0] = 0).
+__device__ __forceinline__ int bkv_find(const int* off, int n, int k) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (off[mid] <= k) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+// Takes the `want` lowest free pages (want <= free pages) into v.fresh,
+// ascending, and marks them used. Words from *hint on are searched, 1024 a
+// round; the caller has checked that enough are free.
+__device__ void bkv_take(const BkvView& v, int want, int* red) {
+    const int words = (v.n_page + 31) / 32;
+    int base = v.meta[BKV_HINT], got = 0, last = base;
+    while (got < want && base < words) {
+        const int w = base + (int)threadIdx.x;
+        uint32_t avail = w < words ? ~v.used[w] : 0u;
+        if (w == words - 1 && (v.n_page & 31)) avail &= (1u << (v.n_page & 31)) - 1u;
+        int total;
+        int at = got + bkv_scan(__popc(avail), red, &total);
+        uint32_t taken = 0;
+        while (avail && at < want) {
+            const int b = __ffs(avail) - 1;
+            v.fresh[at++] = w * 32 + b;
+            taken |= 1u << b;
+            avail &= avail - 1;
+        }
+        if (taken) v.used[w] |= taken;
+        got += total;
+        last = base;
+        base += BKV_TPB;
+    }
+    __syncthreads();
+    // every word before the last round's first is full now
+    if (threadIdx.x == 0 && want > 0) v.meta[BKV_HINT] = last;
+    __syncthreads();
+}
+
+// Drops one holder of a page; the last one frees it.
+__device__ __forceinline__ void bkv_drop(const BkvView& v, int page) {
+    if ((unsigned)page >= (unsigned)v.n_page) return;
+    if (atomicSub(&v.refs[page], 1) == 1) {
+        atomicAnd(&v.used[page >> 5], ~(1u << (page & 31)));
+        atomicAdd(&v.meta[BKV_FREE], 1);
+        atomicMin(&v.meta[BKV_HINT], page >> 5);
+    }
+}
+
+// ---- reset -------------------------------------------------------------------
+
+__global__ void vk_bkv_reset(BkvView v) {
+    const size_t i0 = (size_t)blockIdx.x * blockDim.x + threadIdx.x, step = (size_t)gridDim.x * blockDim.x;
+    for (size_t i = i0; i < (size_t)v.n_seq * v.max_blocks; i += step) v.table[i] = -1;
+    for (size_t i = i0; i < (size_t)v.n_seq; i += step) {
+        v.len[i] = 0;
+        v.floor_[i] = 0;
+        v.claim[i] = INT_MAX;
+    }
+    for (size_t i = i0; i < (size_t)v.n_page; i += step) v.refs[i] = 0;
+    for (size_t i = i0; i < (size_t)(v.n_page + 31) / 32; i += step) v.used[i] = 0;
+    if (i0 < BKV_META_INTS) v.meta[i0] = i0 == BKV_FREE ? v.n_page : 0;
+}
+
+__global__ void vk_bkv_fill(uint4* p, size_t n) {
+    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x)
+        p[i] = make_uint4(0, 0, 0, 0);
+}
+
+// ---- step --------------------------------------------------------------------
+
+// Every item names its sequence once: claim[seq] = the lowest item that names
+// it. The first barrier orders the clearing before the claims.
+__device__ __forceinline__ bool bkv_claim(const BkvView& v, int i, bool in_range, int seq) {
+    if (in_range) v.claim[seq] = INT_MAX;
+    __syncthreads();
+    if (in_range) atomicMin(&v.claim[seq], i);
+    __syncthreads();
+    return in_range && __hip_atomic_load(&v.claim[seq], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == i;
+}
+
+__global__ __launch_bounds__(BKV_TPB) void vk_bkv_step(BkvView v, int n, int n_rows, int max_count,
+                                                       const int* __restrict__ seqs, const int* __restrict__ starts,
+                                                       const int* __restrict__ counts) {
+    __shared__ int red[BKV_TPB / 64 + 1];
+    __shared__ int off[BKV_TPB];   // prefix of pages taken, then of write entries
+    __shared__ int s_start[BKV_TPB], s_seq[BKV_TPB];
+    __shared__ int s_bad, s_rows;
+    const int i = threadIdx.x;
+    if (i == 0) {
+        s_bad = n;
+        s_rows = 0;
+    }
+    const int seq = i < n ? seqs[i] : -1, start = i < n ? starts[i] : 0, count = i < n ? counts[i] : 0;
+    const bool in_range = i < n && (unsigned)seq < (unsigned)v.n_seq;
+    const bool mine = bkv_claim(v, i, in_range, seq);
+    const int len = in_range ? v.len[seq] : 0, fl = in_range ? v.floor_[seq] : 0;
+    bool ok = mine && count >= 0 && count <= max_count && start >= fl && start <= len &&
+              count <= v.max_time - start;
+    const int cnt = ok ? count : 0;
+    int rows;
+    const int row0 = bkv_scan(cnt, red, &rows);
+    if (row0 + cnt > n_rows) ok = false;
+    if (i < n && !ok) atomicMin(&s_bad, i);
+    __syncthreads();
+    const int bad = s_bad;
+    // pages: the blocks that are full after the step and reach into its rows
+    const int b0 = start / v.bs, b1 = ok ? (start + cnt) / v.bs : b0;
+    int need = ok && i < bad ? b1 - b0 : 0, total;
+    const int free_pages = v.meta[BKV_FREE];
+    int at = bkv_scan(need, red, &total);
+    __syncthreads();
+    if (i < bad && ok && need > 0 && at + need > free_pages) atomicMin(&s_bad, i);
+    __syncthreads();
+    const int done = s_bad;
+    if (i >= done) need = 0;
+    at = bkv_scan(need, red, &total);
+    off[i] = at;
+    s_start[i] = b0;
+    s_seq[i] = seq;
+    __syncthreads();
+    bkv_take(v, total, red);
+    // pages that a taken-back sequence held from its new start on
+    if (i < done) {
+        for (int b = b0; b < len / v.bs; ++b) {
+            bkv_drop(v, v.table[(size_t)seq * v.max_blocks + b]);
+            v.table[(size_t)seq * v.max_blocks + b] = -1;
+        }
+    }
+    __syncthreads();
+    for (int k = i; k < total; k += BKV_TPB) {
+        const int it = bkv_find(off, done, k);
+        const int page = v.fresh[k];
+        v.table[(size_t)s_seq[it] * v.max_blocks + s_start[it] + (k - off[it])] = page;
+        v.refs[page] = 1;
+    }
+    __syncthreads();
+    if (i < done) {
+        const int end = start + cnt, nb = (end + v.bs - 1) / v.bs;
+        v.len[seq] = end;
+        v.floor_[seq] = max(fl, (nb - 2) * v.bs);
+        BkvItem it;
+        it.seq = seq;
+        it.start = start;
+        it.count = cnt;
+        it.row0 = row0;
+        v.step[i] = it;
+    }
+    // the write's entries: every block that an item's rows reach
+    const int nblk = i < done && cnt > 0 ? (start + cnt - 1) / v.bs - b0 + 1 : 0;
+    int n_work;
+    const int w0 = bkv_scan(nblk, red, &n_work);
+    off[i] = w0;
+    if (i < done) atomicMax(&s_rows, row0 + cnt);  // rows of the items done
+    __syncthreads();
+    n_work = min(n_work, v.max_work);
+    for (int k = i; k < n_work; k += BKV_TPB) {
+        const int it = bkv_find(off, done, k);
+        v.work[k] = make_int2(it, s_start[it] + (k - off[it]));
+    }
+    if (i == 0) {
+        atomicSub(&v.meta[BKV_FREE], total);
+        v.meta[BKV_STATUS] = done == n ? VOKRA_HIP_OK
+                             : done < bad ? VOKRA_HIP_ERROR_KV_CACHE_EXHAUSTED
+                                          : VOKRA_HIP_ERROR_INVALID_ARGUMENT;
+        v.meta[BKV_DONE] = done;
+        v.meta[BKV_STEP_N] = done;
+        v.meta[BKV_STEP_ROWS] = s_rows;
+        v.meta[BKV_WORK_N] = n_work;
+    }
+}
+
+// ---- write -------------------------------------------------------------------
+
+// f32 -> e4m3 (OCP: 4 exponent bits, 3 mantissa bits, largest 448) with
+// round-to-nearest-even of |y| < 464; two values, low byte first.
+__device__ __forceinline__ uint32_t bkv_e4m3_pk(float a, float b) {
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu;
+}
+__device__ __forceinline__ float bkv_e4m3_f32(uint32_t byte) {
+    return __builtin_amdgcn_cvt_f32_fp8((int)byte, 0);
+}
+// The stored byte of y = x * (top / a): int8 values are stored with 128 added,
+// so that a byte is the low mantissa bits of an f16 in 1024 .. 1279.
+template <int CODEC>
+__device__ __forceinline__ uint32_t bkv_encode4(float a, float b, float c, float d) {
+    if constexpr (CODEC == BKV_INT8) {
+        const int ia = (int)rintf(a) + 128, ib = (int)rintf(b) + 128, ic = (int)rintf(c) + 128, id = (int)rintf(d) + 128;
+        return (uint32_t)ia | ((uint32_t)ib << 8) | ((uint32_t)ic << 16) | ((uint32_t)id << 24);
+    } else {
+        return bkv_e4m3_pk(a, b) | (bkv_e4m3_pk(c, d) << 16);
+    }
+}
+template <int CODEC>
+__device__ __forceinline__ float bkv_decode(uint32_t byte) {
+    if constexpr (CODEC == BKV_INT8) return (float)((int)byte - 128);
+    else return bkv_e4m3_f32(byte);
+}
+
+__device__ __forceinline__ size_t bkv_chunk(const BkvView& v, int layer, int page, int head) {
+    return (((size_t)layer * v.n_page + page) * v.n_head + head);
+}
+__device__ __forceinline__ float* bkv_ring(const BkvView& v, int layer, int seq, int side, int head) {
+    return v.ring + ((((size_t)layer * v.n_seq + seq) * 2 + side) * v.n_head + head) * (size_t)(2 * v.bs) * v.hd;
+}
+
+// One (item, block) entry, head and side: rounds the block if the step fills
+// it, and (the entry of the item's first block only) puts the rows of the
+// item's last two blocks into the ring. Only that workgroup reads ring rows
+// (those of the first block that earlier steps brought), before it writes any,
+// so no two workgroups meet there.
+template <int CODEC>
+__global__ __launch_bounds__(256) void vk_bkv_write(BkvView v, int layer, const float* __restrict__ k,
+                                                    const float* __restrict__ vv) {
+    extern __shared__ float tile[];  // [bs][hd]
+    __shared__ float red[4];
+    if ((int)blockIdx.x >= v.meta[BKV_WORK_N]) return;
+    const int2 e = v.work[blockIdx.x];
+    const BkvItem it = v.step[e.x];
+    const int head = blockIdx.y, side = blockIdx.z, hd = v.hd, bs = v.bs, block = e.y;
+    const float* in = (side ? vv : k) + (size_t)it.row0 * v.n_head * hd + (size_t)head * hd;
+    float* ring = bkv_ring(v, layer, it.seq, side, head);
+    const int end = it.start + it.count;
+    const bool full = (block + 1) * bs <= end;
+    if (full) {
+        float amax = 0.0f;
+        bool odd = false;  // a value that is not finite
+        for (int x = threadIdx.x * 4; x < bs * hd; x += 1024) {
+            const int t = block * bs + x / hd, d = x % hd;
+            const float4 r = t >= it.start ? *(const float4*)(in + (size_t)(t - it.start) * v.n_head * hd + d)
+                                           : *(const float4*)(ring + (size_t)(t % (2 * bs)) * hd + d);
+            *(float4*)(tile + x) = r;
+            const float m = fmaxf(fmaxf(fabsf(r.x), fabsf(r.y)), fmaxf(fabsf(r.z), fabsf(r.w)));
+            amax = fmaxf(amax, m);
+            odd |= !(fabsf(r.x) < INFINITY) | !(fabsf(r.y) < INFINITY) | !(fabsf(r.z) < INFINITY) |
+                   !(fabsf(r.w) < INFINITY);
+        }
+        if (odd) amax = INFINITY;
+        amax = vk_group_max<64>(amax);
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = amax;
+        __syncthreads();
+        amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        const float top = CODEC == BKV_INT8 ? 127.0f : 448.0f;
+        const bool holds = amax >= 0x1p-100f && amax < INFINITY;
+        const float inv = holds ? top / amax : 0.0f;
+        const float scale = holds ? amax / top : (amax < INFINITY ? 0.0f : __builtin_nanf(""));
+        const int page = v.table[(size_t)it.seq * v.max_blocks + block];
+        const size_t chunk = bkv_chunk(v, layer, page, head);
+        uint8_t* out = v.pool + chunk * 2 * bs * hd + (size_t)side * bs * hd;
+        if (threadIdx.x == 0) v.scales[chunk * 2 + side] = scale;
+        for (int x = threadIdx.x * 4; x < bs * hd; x += 1024) {  // x = byte offset: four consecutive bytes
+            const int ti = x / (16 * hd), r = x % (16 * hd), lane = (r >> 4) & 63, c = r >> 10, b = r & 15;
+            float y[4];
+            if (side == 0) {
+                const int t = ti * 16 + (lane & 15), d = c * 64 + (lane >> 4) * 16 + b;
+                for (int j = 0; j < 4; ++j) y[j] = tile[t * hd + d + j];
+            } else {
+                const int t = ti * 16 + (lane >> 4) * 4, d = c * 64 + (b >> 2) * 16 + (lane & 15);
+                for (int j = 0; j < 4; ++j) y[j] = tile[(t + j) * hd + d];
+            }
+            for (int j = 0; j < 4; ++j) y[j] = holds ? y[j] * inv : 0.0f;
+            *(uint32_t*)(out + x) = bkv_encode4<CODEC>(y[0], y[1], y[2], y[3]);
+        }
+    }
+    if (block != it.start / bs) return;
+    __syncthreads();
+    const int nb = (end + bs - 1) / bs, first = max(it.start, (nb - 2) * bs);
+    for (int x = threadIdx.x * 4; x < (end - first) * hd; x += 1024) {
+        const int t = first + x / hd, d = x % hd;
+        *(float4*)(ring + (size_t)(t % (2 * bs)) * hd + d) =
+            *(const float4*)(in + (size_t)(t - it.start) * v.n_head * hd + d);
+    }
+}
+
+// ---- read --------------------------------------------------------------------
+
+// Row r: the values held for (seqs[r], times[r]), zeros where nothing is held.
+template <int CODEC>
+__global__ __launch_bounds__(256) void vk_bkv_read(BkvView v, int layer, int n, const int* __restrict__ seqs,
+                                                   const int* __restrict__ times, float* __restrict__ k,
+                                                   float* __restrict__ vv) {
+    const int w4 = v.n_head * v.hd / 4;
+    const size_t total = (size_t)n * w4;
+    const int side = blockIdx.y;
+    float* out = side ? vv : k;
+    for (size_t g = (size_t)blockIdx.x * 256 + threadIdx.x; g < total; g += (size_t)gridDim.x * 256) {
+        const int r = (int)(g / w4), c = (int)(g % w4) * 4, head = c / v.hd, d = c % v.hd;
+        const int seq = seqs[r], t = times[r];
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if ((unsigned)seq < (unsigned)v.n_seq && t >= 0 && t < v.len[seq]) {
+            const int block = t / v.bs;
+            if (block < v.len[seq] / v.bs) {
+                const size_t chunk = bkv_chunk(v, layer, v.table[(size_t)seq * v.max_blocks + block], head);
+                const uint8_t* p = v.pool + chunk * 2 * v.bs * v.hd + (size_t)side * v.bs * v.hd +
+                                   (size_t)(t % v.bs / 16) * 16 * v.hd;
+                const float s = v.scales[chunk * 2 + side];
+                float q[4];
+                for (int j = 0; j < 4; ++j)
+                    q[j] = bkv_decode<CODEC>(p[side ? bkv_v_off(t & 15, d + j) : bkv_k_off(t & 15, d + j)]) * s;
+                y = make_float4(q[0], q[1], q[2], q[3]);
+            } else {
+                y = *(const float4*)(bkv_ring(v, layer, seq, side, head) + (size_t)(t % (2 * v.bs)) * v.hd + d);
+            }
+        }
+        *(float4*)(out + g * 4) = y;
+    }
+}
+
+// ---- fork, free, copy, compact -------------------------------------------------
+
+// The checks that a fork and a copy share: source and destination in range,
+// the destination empty, named once and no source of the call's.
+// A source that is some item's destination is refused (`same`: both ids are of
+// one cache).
+__device__ __forceinline__ bool bkv_pair_ok(const BkvView& dv, const BkvView& sv, bool same, int i, int n, int src,
+                                            int dst) {
+    const bool rs = i < n && (unsigned)src < (unsigned)sv.n_seq, rd = i < n && (unsigned)dst < (unsigned)dv.n_seq;
+    if (same && rs) dv.claim[src] = INT_MAX;
+    const bool mine = bkv_claim(dv, i, rd, dst);
+    bool ok = rs && mine && dv.len[dst] == 0;
+    if (same && ok)
+        ok = __hip_atomic_load(&dv.claim[src], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == INT_MAX;
+    return ok;
+}
+
+__global__ __launch_bounds__(BKV_TPB) void vk_bkv_fork_plan(BkvView v, int n, const int* __restrict__ srcs,
+                                                            const int* __restrict__ dsts) {
+    __shared__ int s_bad;
+    const int i = threadIdx.x;
+    if (i == 0) s_bad = n;
+    const int src = i < n ? srcs[i] : -1, dst = i < n ? dsts[i] : -1;
+    const bool ok = bkv_pair_ok(v, v, true, i, n, src, dst);
+    if (i < n && !ok) atomicMin(&s_bad, i);
+    __syncthreads();
+    const int done = s_bad;
+    if (i < done) {
+        BkvItem it;
+        it.seq = src;
+        it.start = dst;
+        it.count = v.len[src];
+        // the fork copies the open block's rows and none before it
+        it.row0 = max(v.floor_[src], it.count / v.bs * v.bs);
+        v.plan[i] = it;
+        v.len[dst] = it.count;
+        v.floor_[dst] = it.row0;
+    }
+    if (i == 0) {
+        v.meta[BKV_STATUS] = done == n ? VOKRA_HIP_OK : VOKRA_HIP_ERROR_INVALID_ARGUMENT;
+        v.meta[BKV_DONE] = done;
+        v.meta[BKV_PLAN_N] = done;
+    }
+}
+
+// blockIdx.x: item; blockIdx.y < n_layer: that layer's ring rows; else the table row.
+__global__ __launch_bounds__(256) void vk_bkv_fork_rows(BkvView v) {
+    if ((int)blockIdx.x >= v.meta[BKV_PLAN_N]) return;
+    const BkvItem it = v.plan[blockIdx.x];
+    const int layer = blockIdx.y;
+    if (layer == v.n_layer) {
+        for (int b = threadIdx.x; b < it.count / v.bs; b += 256) {
+            const int page = v.table[(size_t)it.seq * v.max_blocks + b];
+            v.table[(size_t)it.start * v.max_blocks + b] = page;
+            atomicAdd(&v.refs[page], 1);
+        }
+        return;
+    }
+    const int per = (it.count - it.row0) * v.hd, hs = 2 * v.n_head;
+    const float* src = bkv_ring(v, layer, it.seq, 0, 0);
+    float* dst = bkv_ring(v, layer, it.start, 0, 0);
+    for (int x = threadIdx.x * 4; x < per * hs; x += 1024) {
+        const int h = x / per, t = it.row0 + x % per / v.hd, d = x % v.hd;
+        const size_t o = ((size_t)h * 2 * v.bs + t % (2 * v.bs)) * v.hd + d;
+        *(float4*)(dst + o) = *(const float4*)(src + o);
+    }
+}
+
+__global__ __launch_bounds__(BKV_TPB) void vk_bkv_free_plan(BkvView v, int n, const int* __restrict__ seqs) {
+    __shared__ int s_bad;
+    const int i = threadIdx.x;
+    if (i == 0) s_bad = n;
+    const int seq = i < n ? seqs[i] : -1;
+    const bool in_range = i < n && (unsigned)seq < (unsigned)v.n_seq;
+    const bool mine = bkv_claim(v, i, in_range, seq);
+    if (i < n && !in_range) atomicMin(&s_bad, i);
+    __syncthreads();
+    const int done = s_bad;
+    if (i < done) {
+        BkvItem it;
+        it.seq = seq;
+        it.start = it.row0 = 0;
+        it.count = mine ? v.len[seq] : 0;  // a sequence named twice is freed once
+        v.plan[i] = it;
+        if (mine) {
+            v.len[seq] = 0;
+            v.floor_[seq] = 0;
+        }
+    }
+    if (i == 0) {
+        v.meta[BKV_STATUS] = done == n ? VOKRA_HIP_OK : VOKRA_HIP_ERROR_INVALID_ARGUMENT;
+        v.meta[BKV_DONE] = done;
+        v.meta[BKV_PLAN_N] = done;
+        v.meta[BKV_STEP_N] = v.meta[BKV_STEP_ROWS] = v.meta[BKV_WORK_N] = 0;  // a step ends with a free
+    }
+}
+
+__global__ __launch_bounds__(256) void vk_bkv_free_pages(BkvView v) {
+    if ((int)blockIdx.x >= v.meta[BKV_PLAN_N]) return;
+    const BkvItem it = v.plan[blockIdx.x];
+    for (int b = blockIdx.y * 256 + threadIdx.x; b < it.count / v.bs; b += 256 * gridDim.y) {
+        int* e = v.table + (size_t)it.seq * v.max_blocks + b;
+        bkv_drop(v, *e);
+        *e = -1;
+    }
+}
+
+__global__ __launch_bounds__(BKV_TPB) void vk_bkv_copy_plan(BkvView dv, BkvView sv, int same, int n,
+                                                            const int* __restrict__ srcs,
+                                                            const int* __restrict__ dsts) {
+    __shared__ int red[BKV_TPB / 64 + 1];
+    __shared__ int off[BKV_TPB], s_src[BKV_TPB], s_dst[BKV_TPB];
+    __shared__ int s_bad;
+    const int i = threadIdx.x;
+    if (i == 0) s_bad = n;
+    const int src = i < n ? srcs[i] : -1, dst = i < n ? dsts[i] : -1;
+    bool ok = bkv_pair_ok(dv, sv, same != 0, i, n, src, dst);
+    const int len = ok ? sv.len[src] : 0;
+    if (len > dv.max_time) ok = false;
+    if (i < n && !ok) atomicMin(&s_bad, i);
+    __syncthreads();
+    const int bad = s_bad;
+    int need = i < bad ? len / dv.bs : 0, total;
+    const int free_pages = dv.meta[BKV_FREE];
+    int at = bkv_scan(need, red, &total);
+    if (i < bad && need > 0 && at + need > free_pages) atomicMin(&s_bad, i);
+    __syncthreads();
+    const int done = s_bad;
+    if (i >= done) need = 0;
+    at = bkv_scan(need, red, &total);
+    off[i] = at;
+    s_src[i] = src;
+    s_dst[i] = dst;
+    __syncthreads();
+    bkv_take(dv, total, red);
+    for (int k = i; k < total; k += BKV_TPB) {
+        const int it = bkv_find(off, done, k), b = k - off[it], page = dv.fresh[k];
+        dv.table[(size_t)s_dst[it] * dv.max_blocks + b] = page;
+        dv.refs[page] = 1;
+        dv.moves[k] = make_int2(sv.table[(size_t)s_src[it] * sv.max_blocks + b], page);
+    }
+    if (i < done) {
+        BkvItem it;
+        it.seq = src;
+        it.start = dst;
+        it.count = len;
+        it.row0 = sv.floor_[src];
+        dv.plan[i] = it;
+        dv.len[dst] = len;
+        dv.floor_[dst] = it.row0;
+    }
+    if (i == 0) {
+        dv.meta[BKV_FREE] = free_pages - total;
+        dv.meta[BKV_STATUS] = done == n ? VOKRA_HIP_OK
+                              : done < bad ? VOKRA_HIP_ERROR_KV_CACHE_EXHAUSTED
+                                           : VOKRA_HIP_ERROR_INVALID_ARGUMENT;
+        dv.meta[BKV_DONE] = done;
+        dv.meta[BKV_PLAN_N] = done;
+        dv.meta[BKV_MOVE_N] = total;
+    }
+}
+
+// The moves' bytes and scales, every layer: runs of n_head * 2 * bs * hd bytes.
+__global__ __launch_bounds__(256) void vk_bkv_move_pages(BkvView dv, BkvView sv) {
+    const int n = dv.meta[BKV_MOVE_N];
+    const size_t run = (size_t)dv.n_head * 2 * dv.bs * dv.hd;
+    for (size_t e = blockIdx.x; e < (size_t)n * dv.n_layer; e += gridDim.x) {
+        const int layer = (int)(e / n);
+        const int2 m = dv.moves[e % n];
+        const size_t sp = (size_t)layer * sv.n_page + m.x, dp = (size_t)layer * dv.n_page + m.y;
+        const uint4* a = (const uint4*)(sv.pool + sp * run);
+        uint4* b = (uint4*)(dv.pool + dp * run);
+        for (size_t x = threadIdx.x; x < run / 16; x += 256) b[x] = a[x];
+        for (int x = threadIdx.x; x < 2 * dv.n_head; x += 256)
+            dv.scales[dp * 2 * dv.n_head + x] = sv.scales[sp * 2 * dv.n_head + x];
+    }
+}
+
+// The ring rows of copied sequences (all that a step may still go back to).
+__global__ __launch_bounds__(256) void vk_bkv_copy_rows(BkvView dv, BkvView sv) {
+    if ((int)blockIdx.x >= dv.meta[BKV_PLAN_N]) return;
+    const BkvItem it = dv.plan[blockIdx.x];
+    const int layer = blockIdx.y, per = (it.count - it.row0) * dv.hd, hs = 2 * dv.n_head;
+    const float* src = bkv_ring(sv, layer, it.seq, 0, 0);
+    float* dst = bkv_ring(dv, layer, it.start, 0, 0);
+    for (int x = threadIdx.x * 4; x < per * hs; x += 1024) {
+        const int h = x / per, t = it.row0 + x % per / dv.hd, d = x % dv.hd;
+        const size_t o = ((size_t)h * 2 * dv.bs + t % (2 * dv.bs)) * dv.hd + d;
+        *(float4*)(dst + o) = *(const float4*)(src + o);
+    }
+}
+
+// u pages are in use: the k-th one at or above u moves to the k-th free one
+// below u. v.fresh takes the free ones, v.moves the pairs.
+__global__ __launch_bounds__(BKV_TPB) void vk_bkv_compact_plan(BkvView v) {
+    __shared__ int red[BKV_TPB / 64 + 1];
+    const int u = v.n_page - v.meta[BKV_FREE], words = (v.n_page + 31) / 32;
+    int holes = 0, movers = 0;
+    for (int base = 0; base < words; base += BKV_TPB) {
+        const int w = base + (int)threadIdx.x;
+        const uint32_t bits = w < words ? v.used[w] : 0u;
+        // bits of pages below u
+        const int below = min(max(u - w * 32, 0), 32);
+        const uint32_t low = w < words ? (below == 32 ? ~0u : (1u << below) - 1u) : 0u;
+        uint32_t h = ~bits & low, m = bits & ~low;
+        int nh, nm;
+        int ah = holes + bkv_scan(__popc(h), red, &nh);
+        int am = movers + bkv_scan(__popc(m), red, &nm);
+        for (; h; h &= h - 1) v.fresh[ah++] = w * 32 + __ffs(h) - 1;
+        for (; m; m &= m - 1) v.moves[am++].x = w * 32 + __ffs(m) - 1;
+        holes += nh;
+        movers += nm;
+    }
+    __syncthreads();
+    for (int k = threadIdx.x; k < movers; k += BKV_TPB) {
+        const int from = v.moves[k].x, to = v.fresh[k];
+        v.moves[k].y = to;
+        v.remap[from] = to;
+        v.refs[to] = v.refs[from];
+        v.refs[from] = 0;
+    }
+    for (int w = threadIdx.x; w < words; w += BKV_TPB) {
+        const int below = min(max(u - w * 32, 0), 32);
+        v.used[w] = below == 32 ? ~0u : (1u << below) - 1u;
+    }
+    if (threadIdx.x == 0) {
+        v.meta[BKV_MOVE_N] = movers;
+        v.meta[BKV_HINT] = u / 32;
+        v.meta[BKV_STATUS] = VOKRA_HIP_OK;
+        v.meta[BKV_DONE] = movers;
+    }
+}
+
+// Table entries of moved pages, one sequence a workgroup.
+__global__ __launch_bounds__(256) void vk_bkv_compact_table(BkvView v) {
+    if (v.meta[BKV_MOVE_N] == 0) return;
+    const int u = v.n_page - v.meta[BKV_FREE];
+    for (int seq = blockIdx.x; seq < v.n_seq; seq += gridDim.x) {
+        const int nb = v.len[seq] / v.bs;
+        for (int b = threadIdx.x; b < nb; b += 256) {
+            int* e = v.table + (size_t)seq * v.max_blocks + b;
+            if (*e >= u) *e = v.remap[*e];
+        }
+    }
+}
+
+__global__ void vk_bkv_peek(BkvView v, int seq, int block, int* out) {
+    out[0] = v.len[seq];
+    out[1] = block < v.len[seq] / v.bs ? v.table[(size_t)seq * v.max_blocks + block] : -1;
+}
+
+// ---- launchers -----------------------------------------------------------------
+
+hipError_t launch_bkv_reset(hipStream_t s, const BkvView& v, bool clear_data) {
+    hipLaunchKernelGGL(vk_bkv_reset, dim3(256), dim3(256), 0, s, v);
+    if (clear_data) {
+        const size_t pages = (size_t)v.n_layer * v.n_page * v.n_head;
+        const size_t pool = pages * 2 * v.bs * v.hd;
+        const size_t ring = (size_t)v.n_layer * v.n_seq * 2 * v.n_head * 2 * v.bs * v.hd * sizeof(float);
+        hipLaunchKernelGGL(vk_bkv_fill, dim3(2048), dim3(256), 0, s, (uint4*)v.pool, pool / 16);
+        hipLaunchKernelGGL(vk_bkv_fill, dim3(2048), dim3(256), 0, s, (uint4*)v.ring, ring / 16);
+        // rounded up to 16 bytes by the allocation
+        hipLaunchKernelGGL(vk_bkv_fill, dim3(256), dim3(256), 0, s, (uint4*)v.scales, (pages * 8 + 15) / 16);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_bkv_step(hipStream_t s, const BkvView& v, int n, int n_rows, int max_count, const int* seqs,
+                           const int* starts, const int* counts) {
+    hipLaunchKernelGGL(vk_bkv_step, dim3(1), dim3(BKV_TPB), 0, s, v, n, n_rows, max_count, seqs, starts, counts);
+    return hipGetLastError();
+}
+
+hipError_t launch_bkv_write(hipStream_t s, const BkvView& v, int layer, int work_bound, const float* k,
+                            const float* vv) {
+    if (work_bound == 0) return hipSuccess;
+    const dim3 grid((unsigned)work_bound, (unsigned)v.n_head, 2);
+    const size_t lds = (size_t)v.bs * v.hd * sizeof(float);
+    if (v.codec == BKV_INT8)
+        hipLaunchKernelGGL(vk_bkv_write<BKV_INT8>, grid, dim3(256), lds, s, v, layer, k, vv);
+    else
+        hipLaunchKernelGGL(vk_bkv_write<BKV_E4M3>, grid, dim3(256), lds, s, v, layer, k, vv);
+    return hipGetLastError();
+}
+
+hipError_t launch_bkv_read(hipStream_t s, const BkvView& v, int layer, int n, const int* seqs, const int* times,
+                           float* k, float* vv) {
+    if (n == 0) return hipSuccess;
+    const size_t wgs = ((size_t)n * v.n_head * v.hd / 4 + 255) / 256;
+    const dim3 grid((unsigned)std::min<size_t>(wgs, 8192), 2);
+    if (v.codec == BKV_INT8)
+        hipLaunchKernelGGL(vk_bkv_read<BKV_INT8>, grid, dim3(256), 0, s, v, layer, n, seqs, times, k, vv);
+    else
+        hipLaunchKernelGGL(vk_bkv_read<BKV_E4M3>, grid, dim3(256), 0, s, v, layer, n, seqs, times, k, vv);
+    return hipGetLastError();
+}
+
+hipError_t launch_bkv_fork(hipStream_t s, const BkvView& v, int n, const int* src, const int* dst) {
+    hipLaunchKernelGGL(vk_bkv_fork_plan, dim3(1), dim3(BKV_TPB), 0, s, v, n, src, dst);
+    if (n) hipLaunchKernelGGL(vk_bkv_fork_rows, dim3((unsigned)n, (unsigned)v.n_layer + 1), dim3(256), 0, s, v);
+    return hipGetLastError();
+}
+
+hipError_t launch_bkv_free(hipStream_t s, const BkvView& v, int n, const int* seqs) {
+    hipLaunchKernelGGL(vk_bkv_free_plan, dim3(1), dim3(BKV_TPB), 0, s, v, n, seqs);
+    if (n) {
+        const unsigned y = (unsigned)std::min((v.max_blocks + 255) / 256, 64);
+        hipLaunchKernelGGL(vk_bkv_free_pages, dim3((unsigned)n, y), dim3(256), 0, s, v);
+    }
+    return hipGetLastError();
+}
+
+// Workgroups of the page moves: the number of moves is known on the device only.
+constexpr unsigned kMoveGrid = 2048;
+
+hipError_t launch_bkv_copy(hipStream_t s, const BkvView& dv, const BkvView& sv, int n, const int* src,
+                           const int* dst) {
+    hipLaunchKernelGGL(vk_bkv_copy_plan, dim3(1), dim3(BKV_TPB), 0, s, dv, sv, (int)(dv.meta == sv.meta), n, src, dst);
+    if (n) {
+        hipLaunchKernelGGL(vk_bkv_move_pages, dim3(kMoveGrid), dim3(256), 0, s, dv, sv);
+        hipLaunchKernelGGL(vk_bkv_copy_rows, dim3((unsigned)n, (unsigned)dv.n_layer), dim3(256), 0, s, dv, sv);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_bkv_compact(hipStream_t s, const BkvView& v) {
+    hipLaunchKernelGGL(vk_bkv_compact_plan, dim3(1), dim3(BKV_TPB), 0, s, v);
+    hipLaunchKernelGGL(vk_bkv_move_pages, dim3(kMoveGrid), dim3(256), 0, s, v, v);
+    hipLaunchKernelGGL(vk_bkv_compact_table, dim3((unsigned)std::min(v.n_seq, 1024)), dim3(256), 0, s, v);
+    return hipGetLastError();
+}
+
+hipError_t launch_bkv_peek(hipStream_t s, const BkvView& v, int seq, int block, int* out) {
+    hipLaunchKernelGGL(vk_bkv_peek, dim3(1), dim3(1), 0, s, v, seq, block, out);
+    return hipGetLastError();
+}
+
+}  // namespace vk

@@ -597,6 +597,7 @@ int check_paged_attn(const vokra_hip_kv* kv, size_t layer, size_t n, size_t hq) 
 // this file's entry points.
 namespace vk {
 hipStream_t ctx_stream(const vokra_hip_ctx* c) { return c->stream; }
+int ctx_device(const vokra_hip_ctx* c) { return c->device; }
 
 // Drains the context stream and turns a raised fp16-range flag of the
 // attention kernels into INVALID_ARGUMENT (the explicit failure of

@@ -78,6 +78,12 @@ class ActQuant(IntEnum):
     KQUANT = 2
 
 
+class KvCodec(IntEnum):
+    """8-bit values of the block-scaled cache (VOKRA_HIP_BKV_*)."""
+    INT8 = 0
+    E4M3 = 1
+
+
 class CrossPrecision(IntEnum):
     """Decoder cross-attention K/V reads (VOKRA_HIP_CROSS_*)."""
     F32 = 0
@@ -215,6 +221,29 @@ def _declare(L):
     L.vokra_hip_kv_set_free_order.argtypes = [P, P, i32p, sz]
     L.vokra_hip_paged_attn.argtypes = [P, P, sz, sz, i32p, i32p, sz, f32p, C.c_float, f32p]
     L.vokra_hip_paged_attn_dev.argtypes = [P, P, sz, sz, P, P, sz, sz, P, C.c_float, P]
+    L.vokra_hip_bkv_create.argtypes = [P, sz, sz, sz, sz, sz, sz, sz, sz, C.c_int, C.POINTER(P)]
+    L.vokra_hip_bkv_destroy.argtypes = [P]
+    L.vokra_hip_bkv_destroy.restype = None
+    L.vokra_hip_bkv_reset.argtypes = [P, P]
+    L.vokra_hip_bkv_step.argtypes = [P, P, sz, i32p, i32p, i32p]
+    L.vokra_hip_bkv_step_dev.argtypes = [P, P, sz, sz, sz, sz, P, P, P]
+    L.vokra_hip_bkv_status.argtypes = [P, P, C.POINTER(sz)]
+    L.vokra_hip_bkv_write.argtypes = [P, P, sz, f32p, f32p]
+    L.vokra_hip_bkv_write_dev.argtypes = [P, P, sz, P, P]
+    L.vokra_hip_bkv_attn.argtypes = [P, P, sz, sz, f32p, C.c_float, f32p]
+    L.vokra_hip_bkv_attn_dev.argtypes = [P, P, sz, sz, P, C.c_float, P]
+    L.vokra_hip_bkv_read.argtypes = [P, P, sz, sz, i32p, i32p, f32p, f32p]
+    L.vokra_hip_bkv_read_dev.argtypes = [P, P, sz, sz, P, P, P, P]
+    L.vokra_hip_bkv_fork.argtypes = [P, P, sz, i32p, i32p]
+    L.vokra_hip_bkv_fork_dev.argtypes = [P, P, sz, P, P]
+    L.vokra_hip_bkv_free.argtypes = [P, P, sz, i32p]
+    L.vokra_hip_bkv_free_dev.argtypes = [P, P, sz, P]
+    L.vokra_hip_bkv_copy.argtypes = [P, P, P, sz, i32p, i32p]
+    L.vokra_hip_bkv_copy_dev.argtypes = [P, P, P, sz, P, P]
+    L.vokra_hip_bkv_compact.argtypes = [P, P]
+    L.vokra_hip_bkv_length.argtypes = [P, P, sz, C.POINTER(sz)]
+    L.vokra_hip_bkv_pages.argtypes = [P, P, C.POINTER(sz), C.POINTER(sz)]
+    L.vokra_hip_bkv_page_of.argtypes = [P, P, sz, sz, C.POINTER(C.c_long)]
     L.vokra_hip_gemm_f32.argtypes = [P, sz, sz, sz, f32p, sz, f32p, sz, f32p, f32p, sz]
     L.vokra_hip_gemm_f32_dev.argtypes = [P, sz, sz, sz, P, P, C.c_int, P, P]
     L.vokra_hip_gemv_f32.argtypes = [P, sz, sz, f32p, sz, f32p, sz, f32p, f32p, sz]
@@ -664,6 +693,144 @@ class KvCache:
             pass
 
 
+class BlockKvCache:
+    """The block-scaled KV cache (vokra_hip_bkv_*): 8-bit pages of one sequence
+    each, one scale for each block of tokens, head and side. A step plans its
+    rows and pages; write and attn then take the step's packed rows, layer by
+    layer. The _dev forms take device buffers and do not synchronize."""
+
+    def __init__(self, ctx: "HipContext", n_layer, n_head, d_head, n_seq, max_time, block_size, n_page, max_rows,
+                 codec: KvCodec = KvCodec.INT8):
+        self._ctx = ctx
+        self.n_head, self.d_head = n_head, d_head
+        self._rows, self._max_rows = 0, max_rows  # rows of the current step
+        h = C.c_void_p()
+        _check(lib().vokra_hip_bkv_create(ctx._h, n_layer, n_head, d_head, n_seq, max_time, block_size, n_page,
+                                          max_rows, int(codec), C.byref(h)))
+        self._h = h
+
+    def _rows_arg(self, x, width):
+        x = _f32(x)
+        if x.size != self._rows * width:
+            raise InvalidArgument(f"block cache: {x.size} floats for a step of {self._rows} rows x {width}")
+        return x
+
+    @staticmethod
+    def _ids(*arrays):
+        out = [np.ascontiguousarray(a, np.int32).reshape(-1) for a in arrays]
+        if any(a.size != out[0].size for a in out):
+            raise InvalidArgument("block cache: item arrays differ in length")
+        return out
+
+    def step(self, seqs, starts, counts):
+        """Sequence seqs[i] takes counts[i] rows from starts[i] on (host arrays)."""
+        s, a, n = self._ids(seqs, starts, counts)
+        rows = int(np.maximum(n, 0).sum())
+        code = lib().vokra_hip_bkv_step(self._ctx._h, self._h, s.size, _ptr(s, C.c_int32), _ptr(a, C.c_int32),
+                                        _ptr(n, C.c_int32))
+        if rows <= self._max_rows and s.size <= 1024:  # else refused as a whole: the step before stays
+            self._rows = rows
+        _check(code)
+
+    def step_dev(self, n, n_rows, max_count, max_len, d_seqs, d_starts, d_counts):
+        _check(lib().vokra_hip_bkv_step_dev(self._ctx._h, self._h, n, n_rows, max_count, max_len, d_seqs.ptr,
+                                            d_starts.ptr, d_counts.ptr))
+        self._rows = int(n_rows)
+
+    def status(self):
+        """Items done by the last step, fork, free or copy; raises its error."""
+        n = C.c_size_t(0)
+        _check(lib().vokra_hip_bkv_status(self._ctx._h, self._h, C.byref(n)))
+        return n.value
+
+    def write(self, layer, k_rows, v_rows):
+        w = self.n_head * self.d_head
+        k, v = self._rows_arg(k_rows, w), self._rows_arg(v_rows, w)
+        _check(lib().vokra_hip_bkv_write(self._ctx._h, self._h, layer, _ptr(k, C.c_float), _ptr(v, C.c_float)))
+
+    def write_dev(self, layer, d_k, d_v):
+        _check(lib().vokra_hip_bkv_write_dev(self._ctx._h, self._h, layer, d_k.ptr, d_v.ptr))
+
+    def attn(self, layer, q, n_head_q, scale, out=None):
+        """Attention of the step's rows q [rows, n_head_q * d_head]; rows that the
+        step does not reach keep what `out` holds (zeros without one)."""
+        qv = self._rows_arg(q, n_head_q * self.d_head).reshape(self._rows, -1)
+        out = np.zeros_like(qv) if out is None else self._rows_arg(out, n_head_q * self.d_head).reshape(qv.shape)
+        _check(lib().vokra_hip_bkv_attn(self._ctx._h, self._h, layer, n_head_q, _ptr(qv, C.c_float),
+                                        C.c_float(scale), _ptr(out, C.c_float)))
+        return out
+
+    def attn_dev(self, layer, n_head_q, d_q, scale, d_out):
+        _check(lib().vokra_hip_bkv_attn_dev(self._ctx._h, self._h, layer, n_head_q, d_q.ptr, C.c_float(scale),
+                                            d_out.ptr))
+
+    def read(self, layer, seqs, times):
+        """(k, v) rows [n, n_head * d_head] as the cache holds them, zeros where none is."""
+        s, t = self._ids(seqs, times)
+        k = np.zeros((s.size, self.n_head * self.d_head), np.float32)
+        v = np.zeros_like(k)
+        _check(lib().vokra_hip_bkv_read(self._ctx._h, self._h, layer, s.size, _ptr(s, C.c_int32), _ptr(t, C.c_int32),
+                                        _ptr(k, C.c_float), _ptr(v, C.c_float)))
+        return k, v
+
+    def read_dev(self, layer, n, d_seqs, d_times, d_k, d_v):
+        _check(lib().vokra_hip_bkv_read_dev(self._ctx._h, self._h, layer, n, d_seqs.ptr, d_times.ptr, d_k.ptr,
+                                            d_v.ptr))
+
+    def fork(self, src, dst):
+        s, d = self._ids(src, dst)
+        _check(lib().vokra_hip_bkv_fork(self._ctx._h, self._h, s.size, _ptr(s, C.c_int32), _ptr(d, C.c_int32)))
+
+    def fork_dev(self, n, d_src, d_dst):
+        _check(lib().vokra_hip_bkv_fork_dev(self._ctx._h, self._h, n, d_src.ptr, d_dst.ptr))
+
+    def free(self, seqs):
+        s, = self._ids(seqs)
+        _check(lib().vokra_hip_bkv_free(self._ctx._h, self._h, s.size, _ptr(s, C.c_int32)))
+
+    def free_dev(self, n, d_seqs):
+        _check(lib().vokra_hip_bkv_free_dev(self._ctx._h, self._h, n, d_seqs.ptr))
+
+    def copy_from(self, src_cache, src, dst):
+        """Sequences src of src_cache (which may be this one), copied to dst of this cache."""
+        s, d = self._ids(src, dst)
+        _check(lib().vokra_hip_bkv_copy(self._ctx._h, self._h, src_cache._h, s.size, _ptr(s, C.c_int32),
+                                        _ptr(d, C.c_int32)))
+
+    def copy_from_dev(self, src_cache, n, d_src, d_dst):
+        _check(lib().vokra_hip_bkv_copy_dev(self._ctx._h, self._h, src_cache._h, n, d_src.ptr, d_dst.ptr))
+
+    def compact(self):
+        _check(lib().vokra_hip_bkv_compact(self._ctx._h, self._h))
+
+    def reset(self):
+        _check(lib().vokra_hip_bkv_reset(self._ctx._h, self._h))
+
+    def length(self, seq) -> int:
+        n = C.c_size_t(0)
+        _check(lib().vokra_hip_bkv_length(self._ctx._h, self._h, seq, C.byref(n)))
+        return n.value
+
+    def pages(self):
+        """(free pages, pages in use)"""
+        fr, used = C.c_size_t(0), C.c_size_t(0)
+        _check(lib().vokra_hip_bkv_pages(self._ctx._h, self._h, C.byref(fr), C.byref(used)))
+        return fr.value, used.value
+
+    def page_of(self, seq, block) -> int:
+        p = C.c_long(0)
+        _check(lib().vokra_hip_bkv_page_of(self._ctx._h, self._h, seq, block, C.byref(p)))
+        return p.value
+
+    def __del__(self):
+        try:
+            if getattr(self, "_h", None) and self._h.value and _ctx_alive(self):
+                lib().vokra_hip_bkv_destroy(self._h)
+                self._h = C.c_void_p()
+        except Exception:
+            pass
+
+
 class Encoder:
     """Device-resident pre-norm encoder (compute.rs:2775 encode_prenorm_encoder)."""
 
@@ -1034,6 +1201,10 @@ class HipContext:
 
     def kv_cache(self, n_layer, n_head, d_head, n_stream, max_time, block_size, mode=KvQuant.Q8_0) -> KvCache:
         return KvCache(self, n_layer, n_head, d_head, n_stream, max_time, block_size, mode)
+
+    def block_kv_cache(self, n_layer, n_head, d_head, n_seq, max_time, block_size, n_page, max_rows,
+                       codec=KvCodec.INT8) -> BlockKvCache:
+        return BlockKvCache(self, n_layer, n_head, d_head, n_seq, max_time, block_size, n_page, max_rows, codec)
 
     def qact(self, max_m: int, k: int) -> QAct:
         return QAct(self, max_m, k)
