@@ -527,6 +527,103 @@ int vokra_hip_bkv_length(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t seq, 
 int vokra_hip_bkv_pages(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t *free_pages, size_t *pages_in_use);
 int vokra_hip_bkv_page_of(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t seq, size_t block, long *page);
 
+/* ---- rotary plans and logits rules -------------------------------------------- */
+
+/* Rotary positions by a plan: the first rot_dim values of each head turn by
+ * pos * theta_j in pairs j < rot_dim / 2, x_a' = x_a cos - x_b sin, x_b' =
+ * x_a sin + x_b cos, the pair (a, b) being (j, j + rot_dim / 2) (HALF, the
+ * layout of vokra_hip_rope_f32) or (2j, 2j + 1) (INTERLEAVED); the others stay
+ * as they are. theta_j = base^(-2j / rot_dim), scaled for contexts longer than
+ * the trained orig_ctx:
+ *   LINEAR    theta_j / factor;
+ *   NTK       base * factor^(rot_dim / (rot_dim - 2)) in the place of base;
+ *   YARN      theta_j (1 - r_j) + r_j theta_j / factor with r_j rising from 0 to
+ *             1 between floor(d(beta_fast)) and ceil(d(beta_slow)), kept within
+ *             0 and rot_dim - 1, d(t) = rot_dim ln(orig_ctx / (2 pi t)) /
+ *             (2 ln base): pairs that make many turns over orig_ctx keep their
+ *             frequency;
+ *   BANDS     theta_j m_j + (1 - m_j) theta_j / factor with m_j = (t_j -
+ *             low_turns) / (high_turns - low_turns) within 0 and 1, t_j =
+ *             orig_ctx theta_j / 2 pi;
+ *   DIVISORS  theta_j / divisors[j] (rot_dim / 2 values).
+ * Turned values are multiplied by magnitude (0: 1, and 0.1 ln(factor) + 1 for
+ * YARN). The frequencies are formed in extended precision and the angle modulo
+ * a turn in 64-bit fixed point, so far positions lose nothing (the reference's
+ * rope_apply, crates/vokra-models/src/voxtral/text_decoder.rs:858-891, and
+ * vokra_hip_rope_f32 with it, take an f32 product of position and frequency).
+ * Zero in beta_fast, beta_slow, low_turns, high_turns: 32, 1, 1, 4. */
+typedef enum vokra_hip_rope_layout_t { VOKRA_HIP_ROPE_HALF = 0, VOKRA_HIP_ROPE_INTERLEAVED = 1 } vokra_hip_rope_layout_t;
+typedef enum vokra_hip_rope_scaling_t {
+    VOKRA_HIP_ROPE_NONE = 0,
+    VOKRA_HIP_ROPE_LINEAR = 1,
+    VOKRA_HIP_ROPE_NTK = 2,
+    VOKRA_HIP_ROPE_YARN = 3,
+    VOKRA_HIP_ROPE_BANDS = 4,
+    VOKRA_HIP_ROPE_DIVISORS = 5
+} vokra_hip_rope_scaling_t;
+typedef struct vokra_hip_rope_config {
+    size_t head_dim, rot_dim; /* rot_dim even, 2 .. head_dim */
+    int layout, scaling;
+    double base, factor; /* base > 1; factor >= 1 (not read by NONE and DIVISORS) */
+    size_t orig_ctx;     /* YARN and BANDS */
+    double beta_fast, beta_slow, low_turns, high_turns, magnitude;
+    const double *divisors;
+} vokra_hip_rope_config_t;
+typedef struct vokra_hip_rope vokra_hip_rope_t;
+int vokra_hip_rope_create(vokra_hip_ctx_t *ctx, const vokra_hip_rope_config_t *cfg, vokra_hip_rope_t **out);
+void vokra_hip_rope_destroy(vokra_hip_rope_t *rope);
+/* Row r of q [n_head_q heads] and k [n_head_k heads] at positions[r] (any
+ * int32), one launch; either may have no heads. Rows lie q_stride (and so on)
+ * floats apart, so q and k may be parts of one projection's rows. An output is
+ * its input (in place, the same stride) or does not overlap it. Device
+ * pointers, asynchronous; at most 2^32 values. */
+int vokra_hip_rope_apply_dev(vokra_hip_ctx_t *ctx, const vokra_hip_rope_t *rope, size_t rows,
+                             const int32_t *d_positions, size_t n_head_q, const float *d_q, size_t q_stride,
+                             float *d_q_out, size_t q_out_stride, size_t n_head_k, const float *d_k, size_t k_stride,
+                             float *d_k_out, size_t k_out_stride);
+/* Host arrays, synchronous; rows lie side by side. */
+int vokra_hip_rope_apply(vokra_hip_ctx_t *ctx, const vokra_hip_rope_t *rope, size_t rows, const int32_t *positions,
+                         size_t n_head_q, const float *q, float *q_out, size_t n_head_k, const float *k, float *k_out);
+
+/* The rules that logits pass before a token is chosen, and the greedy choice.
+ * No counterpart in the reference (its sampler takes the argmax of the logits
+ * as they are, crates/vokra-core/src/decode/sampler.rs:197-206). For token v of
+ * row r, standing n_v times in the row's history:
+ *   1. n_v > 0: x = x / repetition[r] if x > 0, else x * repetition[r];
+ *               then x = x - (presence[r] + frequency[r] * n_v);
+ *   2. v in the row's biases: x = x + bias (given several times: the last one);
+ *   3. bit v of the row's mask is 0: x = -inf;
+ * then next[r] = the lowest v with the largest x above -inf (a NaN is never
+ * chosen), -1 if there is none (a mask that leaves nothing).
+ * Lists are packed: row r's history is hist[hist_offsets[r] ..
+ * hist_offsets[r + 1] - 1], its biases likewise; token ids outside 0 .. vocab-1
+ * are passed over (padding). n_hist and n_bias are the lists' lengths, and no
+ * offset reads beyond them. repetition, presence, frequency: one value a row,
+ * NULL = 1, 0, 0. mask: word v / 32, bit v % 32 of a row, rows mask_stride
+ * words apart (0: one mask for all rows); NULL = every token is allowed. */
+typedef struct vokra_hip_logits_rules {
+    size_t n_hist;
+    const int32_t *hist, *hist_offsets;
+    const float *repetition, *presence, *frequency;
+    size_t n_bias;
+    const int32_t *bias_ids;
+    const float *bias;
+    const int32_t *bias_offsets;
+    const uint32_t *mask;
+    size_t mask_stride;
+} vokra_hip_logits_rules_t;
+/* logits and out [rows][vocab], rows `stride` floats apart in both; out may be
+ * logits (in place), or NULL: only next is wanted; next may be NULL. rows <=
+ * 65535, vocab <= 2^24. Device pointers (the struct itself in host memory),
+ * asynchronous; the first call with a next on a context allocates 1 MB, so one
+ * is made before a capture. */
+int vokra_hip_logits_rules_dev(vokra_hip_ctx_t *ctx, size_t rows, size_t vocab, size_t stride, const float *d_logits,
+                               const vokra_hip_logits_rules_t *rules, float *d_out, int32_t *d_next);
+/* Host arrays (rows side by side), synchronous; offsets out of order or range
+ * are INVALID_ARGUMENT. */
+int vokra_hip_logits_rules(vokra_hip_ctx_t *ctx, size_t rows, size_t vocab, const float *logits,
+                           const vokra_hip_logits_rules_t *rules, float *out, int32_t *next);
+
 /* out = a + b on device (residual connections; add_assign in the reference's
  * model code, crates/vokra-models/src/whisper/nn.rs). */
 int vokra_hip_add_f32_dev(vokra_hip_ctx_t *ctx, const float *d_a, const float *d_b, float *d_out, size_t n);

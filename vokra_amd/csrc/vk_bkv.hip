@@ -297,8 +297,8 @@ __global__ __launch_bounds__(256) void vk_bkv_write(BkvView v, int layer, const 
             *(float4*)(tile + x) = r;
             const float m = fmaxf(fmaxf(fabsf(r.x), fabsf(r.y)), fmaxf(fabsf(r.z), fabsf(r.w)));
             amax = fmaxf(amax, m);
-            odd |= !(fabsf(r.x) < INFINITY) | !(fabsf(r.y) < INFINITY) | !(fabsf(r.z) < INFINITY) |
-                   !(fabsf(r.w) < INFINITY);
+            odd = odd || !(fabsf(r.x) < INFINITY) || !(fabsf(r.y) < INFINITY) || !(fabsf(r.z) < INFINITY) ||
+                  !(fabsf(r.w) < INFINITY);
         }
         if (odd) amax = INFINITY;
         amax = vk_group_max<64>(amax);

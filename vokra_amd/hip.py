@@ -84,6 +84,22 @@ class KvCodec(IntEnum):
     E4M3 = 1
 
 
+class RopeLayout(IntEnum):
+    """Which values of a head turn together (VOKRA_HIP_ROPE_*)."""
+    HALF = 0
+    INTERLEAVED = 1
+
+
+class RopeScaling(IntEnum):
+    """How frequencies are scaled for long contexts (VOKRA_HIP_ROPE_*)."""
+    NONE = 0
+    LINEAR = 1
+    NTK = 2
+    YARN = 3
+    BANDS = 4
+    DIVISORS = 5
+
+
 class CrossPrecision(IntEnum):
     """Decoder cross-attention K/V reads (VOKRA_HIP_CROSS_*)."""
     F32 = 0
@@ -130,6 +146,22 @@ class VoxtralConfig(C.Structure):
 class WhisperLoadReport(C.Structure):
     """vokra_hip_whisper_load_report_t: Linear weights taken verbatim / packed at load."""
     _fields_ = [("verbatim", C.c_size_t), ("packed", C.c_size_t)]
+
+
+class RopeConfig(C.Structure):
+    """vokra_hip_rope_config_t"""
+    _fields_ = [("head_dim", C.c_size_t), ("rot_dim", C.c_size_t), ("layout", C.c_int), ("scaling", C.c_int),
+                ("base", C.c_double), ("factor", C.c_double), ("orig_ctx", C.c_size_t)] + \
+               [(n, C.c_double) for n in ("beta_fast", "beta_slow", "low_turns", "high_turns", "magnitude")] + \
+               [("divisors", C.POINTER(C.c_double))]
+
+
+class _LogitsRules(C.Structure):
+    """vokra_hip_logits_rules_t"""
+    _fields_ = [("n_hist", C.c_size_t), ("hist", C.c_void_p), ("hist_offsets", C.c_void_p),
+                ("repetition", C.c_void_p), ("presence", C.c_void_p), ("frequency", C.c_void_p),
+                ("n_bias", C.c_size_t), ("bias_ids", C.c_void_p), ("bias", C.c_void_p), ("bias_offsets", C.c_void_p),
+                ("mask", C.c_void_p), ("mask_stride", C.c_size_t)]
 
 
 class TextDecoderLayer(C.Structure):
@@ -244,6 +276,13 @@ def _declare(L):
     L.vokra_hip_bkv_length.argtypes = [P, P, sz, C.POINTER(sz)]
     L.vokra_hip_bkv_pages.argtypes = [P, P, C.POINTER(sz), C.POINTER(sz)]
     L.vokra_hip_bkv_page_of.argtypes = [P, P, sz, sz, C.POINTER(C.c_long)]
+    L.vokra_hip_rope_create.argtypes = [P, C.POINTER(RopeConfig), C.POINTER(P)]
+    L.vokra_hip_rope_destroy.argtypes = [P]
+    L.vokra_hip_rope_destroy.restype = None
+    L.vokra_hip_rope_apply_dev.argtypes = [P, P, sz, P, sz, P, sz, P, sz, sz, P, sz, P, sz]
+    L.vokra_hip_rope_apply.argtypes = [P, P, sz, i32p, sz, f32p, f32p, sz, f32p, f32p]
+    L.vokra_hip_logits_rules_dev.argtypes = [P, sz, sz, sz, P, C.POINTER(_LogitsRules), P, P]
+    L.vokra_hip_logits_rules.argtypes = [P, sz, sz, f32p, C.POINTER(_LogitsRules), f32p, i32p]
     L.vokra_hip_gemm_f32.argtypes = [P, sz, sz, sz, f32p, sz, f32p, sz, f32p, f32p, sz]
     L.vokra_hip_gemm_f32_dev.argtypes = [P, sz, sz, sz, P, P, C.c_int, P, P]
     L.vokra_hip_gemv_f32.argtypes = [P, sz, sz, f32p, sz, f32p, sz, f32p, f32p, sz]
@@ -831,6 +870,75 @@ class BlockKvCache:
             pass
 
 
+class RopePlan:
+    """Rotary positions by a plan (vokra_hip_rope_*): any even part of the head,
+    both pair layouts, frequencies scaled for long contexts."""
+
+    def __init__(self, ctx: "HipContext", head_dim, rot_dim, layout=RopeLayout.HALF, base=10000.0,
+                 scaling=RopeScaling.NONE, factor=1.0, orig_ctx=0, beta_fast=0.0, beta_slow=0.0, low_turns=0.0,
+                 high_turns=0.0, magnitude=0.0, divisors=None):
+        self._ctx, self.head_dim = ctx, int(head_dim)
+        div = None if divisors is None else np.ascontiguousarray(divisors, np.float64)
+        if div is not None and div.size != rot_dim // 2:
+            raise InvalidArgument(f"rope plan: {div.size} divisors for {rot_dim // 2} pairs")
+        cfg = RopeConfig(head_dim, rot_dim, int(layout), int(scaling), base, factor, orig_ctx, beta_fast, beta_slow,
+                         low_turns, high_turns, magnitude, _ptr(div, C.c_double))
+        h = C.c_void_p()
+        _check(lib().vokra_hip_rope_create(ctx._h, C.byref(cfg), C.byref(h)))
+        self._h = h
+
+    def apply_dev(self, rows, d_positions, n_head_q, d_q, d_q_out, n_head_k=0, d_k=None, d_k_out=None, q_stride=None,
+                  k_stride=None, q_out_stride=None, k_out_stride=None):
+        """Rows of q and k at positions[r]; an output may be its input. Strides in
+        floats; where not given, the heads' width, and in place the input's."""
+        def st(x, n):
+            return n * self.head_dim if x is None else x
+        if d_q_out is d_q and q_out_stride is None:
+            q_out_stride = q_stride
+        if d_k_out is d_k and k_out_stride is None:
+            k_out_stride = k_stride
+
+        def p(x):
+            return None if x is None else x.ptr
+        _check(lib().vokra_hip_rope_apply_dev(
+            self._ctx._h, self._h, rows, d_positions.ptr, n_head_q, p(d_q), st(q_stride, n_head_q), p(d_q_out),
+            st(q_out_stride, n_head_q), n_head_k, p(d_k), st(k_stride, n_head_k), p(d_k_out),
+            st(k_out_stride, n_head_k)))
+
+    def apply(self, positions, q=None, k=None):
+        """Host rows [n, heads * head_dim]; returns (q, k), None where none is given."""
+        pos = np.ascontiguousarray(positions, np.int32).reshape(-1)
+        args, outs = [], []
+        for x in (q, k):
+            x = None if x is None else _f32(x)
+            if x is not None and (x.size % (self.head_dim * max(pos.size, 1)) or (pos.size == 0 and x.size)):
+                raise InvalidArgument(f"rope plan: {x.size} values for {pos.size} rows of heads of {self.head_dim}")
+            out = None if x is None else np.empty_like(x)
+            heads = 0 if x is None or pos.size == 0 else x.size // pos.size // self.head_dim
+            args += [heads, _ptr(x, C.c_float), _ptr(out, C.c_float)]
+            outs.append(out)
+        _check(lib().vokra_hip_rope_apply(self._ctx._h, self._h, pos.size, _ptr(pos, C.c_int32), *args))
+        return tuple(outs)
+
+    def __del__(self):
+        try:
+            if getattr(self, "_h", None) and self._h.value and _ctx_alive(self):
+                lib().vokra_hip_rope_destroy(self._h)
+                self._h = C.c_void_p()
+        except Exception:
+            pass
+
+
+class LogitsRules:
+    """vokra_hip_logits_rules_t over device buffers, which it keeps."""
+
+    def __init__(self, n_hist=0, hist=None, hist_offsets=None, repetition=None, presence=None, frequency=None,
+                 n_bias=0, bias_ids=None, bias=None, bias_offsets=None, mask=None, mask_stride=0):
+        self._keep = (hist, hist_offsets, repetition, presence, frequency, bias_ids, bias, bias_offsets, mask)
+        p = [None if b is None else b.ptr for b in self._keep]
+        self._c = _LogitsRules(n_hist, *p[:5], n_bias, *p[5:], mask_stride)
+
+
 class Encoder:
     """Device-resident pre-norm encoder (compute.rs:2775 encode_prenorm_encoder)."""
 
@@ -1342,6 +1450,68 @@ class HipContext:
         one pass (decoder.rs:754-796 then sampler.rs:197-206); d_logits may be None."""
         _check(lib().vokra_hip_logits_argmax_dev(self._h, rows, vocab, d, d_x.ptr, d_emb.ptr,
                                                  None if d_logits is None else d_logits.ptr, d_next.ptr))
+
+    def logits_rules_dev(self, rows, vocab, d_logits, rules: LogitsRules, d_out, d_next, stride=None):
+        """Penalties, biases and masks on logits [rows, vocab] (rows `stride` floats
+        apart), then the greedy choice; d_out may be d_logits, or None, or d_next None."""
+        _check(lib().vokra_hip_logits_rules_dev(self._h, rows, vocab, vocab if stride is None else stride, d_logits.ptr,
+                                                C.byref(rules._c), None if d_out is None else d_out.ptr,
+                                                None if d_next is None else d_next.ptr))
+
+    def logits_rules(self, logits, history=None, repetition=None, presence=None, frequency=None, biases=None,
+                     mask=None):
+        """Host form: logits [rows, vocab]; history: one list of token ids a row;
+        repetition, presence, frequency: one value a row; biases: one list of
+        (id, value) a row; mask: bool [rows, vocab] or [vocab], True = allowed.
+        Returns (logits, next tokens, -1 where none is left)."""
+        x = _f32(logits)
+        rows, vocab = x.shape
+
+        def packed(lists, dtype):
+            if len(lists) != rows:
+                raise InvalidArgument(f"logits rules: {len(lists)} lists for {rows} rows")
+            off = np.concatenate([[0], np.cumsum([len(v) for v in lists])]).astype(np.int32)
+            return np.concatenate([np.asarray(v, dtype) for v in lists] + [np.zeros(0, dtype)]).astype(dtype), off
+        keep, c = [], _LogitsRules()
+
+        def bind(name, a):
+            keep.append(a)
+            setattr(c, name, a.ctypes.data)
+        if history is not None:
+            ids, off = packed(history, np.int32)
+            c.n_hist = ids.size
+            bind("hist", ids)
+            bind("hist_offsets", off)
+        for name, v in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+            if v is not None:
+                v = _f32(v).reshape(-1)
+                if v.size != rows:
+                    raise InvalidArgument(f"logits rules: {v.size} values of {name} for {rows} rows")
+                bind(name, v)
+        if biases is not None:
+            ids, off = packed([[i for i, _ in b] for b in biases], np.int32)
+            vals, _ = packed([[v for _, v in b] for b in biases], np.float32)
+            c.n_bias = ids.size
+            bind("bias_ids", ids)
+            bind("bias", vals)
+            bind("bias_offsets", off)
+        if mask is not None:
+            m = np.asarray(mask, bool)
+            if m.shape not in ((vocab,), (rows, vocab)):
+                raise InvalidArgument(f"logits rules: mask {m.shape} for logits {x.shape}")
+            words = -(-vocab // 32)
+            bits = np.zeros((m.size // vocab if vocab else 0, words * 32), np.uint8)
+            bits[:, :vocab] = m.reshape(-1, vocab)
+            bind("mask", np.ascontiguousarray(np.packbits(bits, axis=1, bitorder="little")).view(np.uint32))
+            c.mask_stride = words if m.ndim == 2 else 0
+        out, nxt = np.empty_like(x), np.empty(rows, np.int32)
+        _check(lib().vokra_hip_logits_rules(self._h, rows, vocab, _ptr(x, C.c_float), C.byref(c), _ptr(out, C.c_float),
+                                            _ptr(nxt, C.c_int32)))
+        return out, nxt
+
+    def rope_plan(self, head_dim, rot_dim, layout=RopeLayout.HALF, base=10000.0, scaling=RopeScaling.NONE, factor=1.0,
+                  orig_ctx=0, **more) -> RopePlan:
+        return RopePlan(self, head_dim, rot_dim, layout, base, scaling, factor, orig_ctx, **more)
 
     # ---- attention ----------------------------------------------------------
     def attn_f32(self, q, k, v, n_head_q: int, n_head_kv: int = None, scale: float = None,
