@@ -169,18 +169,28 @@ class Cache:
         out, tol = np.full(q.shape, np.nan), np.full(q.shape, np.nan)
         for s, a, n, r in self.plan:
             k, v = self.held(layer, s)
-            out[r:r + n], tol[r:r + n] = attention(q[r:r + n], k[:a + n], v[:a + n], a, scale)
+            reach = np.abs(np.asarray(v, np.float64)).max(2)  # [rows, kv heads], then of the row's block
+            for b in range(0, len(reach), self.bs):
+                reach[b:b + self.bs] = reach[b:b + self.bs].max(0)
+            out[r:r + n], tol[r:r + n] = attention(q[r:r + n], k[:a + n], v[:a + n], a, scale, reach)
         return out.reshape(len(q), -1), tol.reshape(len(q), -1)
 
 
-def attention(q, k, v, first, scale):
+def attention(q, k, v, first, scale, reach):
     """Causal attention of q [n, heads, hd] at positions first.. over k, v [t, kv_heads, hd]
     in 64 bits, and a bound on the error of a correct f32 evaluation:
     a score is a sum of hd products of operands held to 2^-22, scaled to base 2
     (a few more roundings), so it is off by at most ds = (2^-22 + (hd + 8) 2^-24)
     scale |q| . |k|; weights are then off by a factor e^(2 ds) and the roundings
     of exp2 and of their two-part form (2^-21 together); sums over t keys add
-    t 2^-24; all relative to sum p |v|."""
+    t 2^-24; all relative to sum p |v|.
+    Two fp16 parts hold their operand to 2^-22 down to the end of fp16's range
+    only. q's row is scaled so that its largest value is 2^14 at least, half of
+    fp16's smallest step is 2^-25: 2^-39 of that largest value for every
+    element, so ds grows by 2^-39 scale max|q| sum|k|. A weight w = p 2^e of the
+    largest 2^M = max p 2^e is held as 2^14 w 2^-M: off by 2^-39 2^M, times a
+    stored value of at most top (127 or 448) where 2^e top <= a, the largest
+    magnitude of the block (`reach`): 2^-39 max(p a) for each of the t keys."""
     n, heads, hd = q.shape
     k, v = np.asarray(k, np.float64), np.asarray(v, np.float64)
     rep = heads // k.shape[1]
@@ -195,5 +205,7 @@ def attention(q, k, v, first, scale):
             p /= p.sum()
             out[i, h] = p @ vh[:m]
             ds = (2.0 ** -22 + (hd + 8) * 2.0 ** -24) * abs(scale) * (np.abs(kh[:m]) @ np.abs(q[i, h])).max()
+            ds += 2.0 ** -39 * abs(scale) * np.abs(q[i, h]).max() * np.abs(kh[:m]).sum(1).max()
             tol[i, h] = (2 * ds + 2.0 ** -21 + (m + 8) * 2.0 ** -24) * (p @ np.abs(vh[:m])) + 1e-37
+            tol[i, h] += m * 2.0 ** -39 * (p * reach[:m, h // rep]).max()
     return out, tol
