@@ -9,7 +9,7 @@
 #include <stdint.h>
 
 constexpr int kBkvMaxItems = 1024;   // items of one call: one thread of the planning workgroup each
-constexpr int kBkvMaxParts = 4096;   // partial results of one split attention (tiles of 16 query rows)
+constexpr int kBkvParts = 1 << 18;  // query rows of which a split attention can hold a partial result
 
 // What planning kernels leave for the kernels of the same call or step.
 // meta (int32): see the BKV_ indices.
@@ -51,7 +51,7 @@ struct BkvView {
     int2* moves;     // [n_page] (source page, destination page) of a copy / compact
     int* remap;      // [n_page] new page of a moved page
     int* meta;
-    BkvItem* step;   // [kBkvMaxItems] the current step
+    BkvItem* step;   // [kBkvMaxItems] the current step, no rows in entries beyond it
     BkvItem* plan;   // [kBkvMaxItems] items of the current fork / free / copy
     int2* work;      // [max_work] (item, block) of the current step's write
     int n_layer, n_head, hd, n_seq, bs, n_page, max_blocks, max_time, codec, max_work;
@@ -86,8 +86,8 @@ hipError_t launch_bkv_compact(hipStream_t s, const BkvView& v);
 // out (2 ints): length of seq, page of block
 hipError_t launch_bkv_peek(hipStream_t s, const BkvView& v, int seq, int block, int* out);
 // Rows of the current step (n items, n_rows rows, at most max_count each, no
-// more than max_len rows held by any) against the cache; part: kBkvMaxParts *
-// 16 * (hd + 2) floats.
+// more than max_len rows held by any) against the cache; part: kBkvParts *
+// (hd + 2) floats.
 hipError_t launch_bkv_attn(hipStream_t s, const BkvView& v, int layer, int n, int n_rows, int max_count, int max_len,
                            int hq, const float* q, float scale, float* out, float* part);
 }  // namespace vk

@@ -124,6 +124,7 @@ __global__ void vk_bkv_reset(BkvView v) {
     }
     for (size_t i = i0; i < (size_t)v.n_page; i += step) v.refs[i] = 0;
     for (size_t i = i0; i < (size_t)(v.n_page + 31) / 32; i += step) v.used[i] = 0;
+    for (size_t i = i0; i < (size_t)kBkvMaxItems; i += step) v.step[i] = BkvItem{0, 0, 0, 0};
     if (i0 < BKV_META_INTS) v.meta[i0] = i0 == BKV_FREE ? v.n_page : 0;
 }
 
@@ -210,6 +211,8 @@ __global__ __launch_bounds__(BKV_TPB) void vk_bkv_step(BkvView v, int n, int n_r
         it.count = cnt;
         it.row0 = row0;
         v.step[i] = it;
+    } else {
+        v.step[i] = BkvItem{0, 0, 0, 0};  // no rows
     }
     // the write's entries: every block that an item's rows reach
     const int nblk = i < done && cnt > 0 ? (start + cnt - 1) / v.bs - b0 + 1 : 0;
@@ -460,6 +463,7 @@ __global__ __launch_bounds__(BKV_TPB) void vk_bkv_free_plan(BkvView v, int n, co
             v.floor_[seq] = 0;
         }
     }
+    v.step[i] = BkvItem{0, 0, 0, 0};
     if (i == 0) {
         v.meta[BKV_STATUS] = done == n ? VOKRA_HIP_OK : VOKRA_HIP_ERROR_INVALID_ARGUMENT;
         v.meta[BKV_DONE] = done;

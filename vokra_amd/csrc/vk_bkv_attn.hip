@@ -6,13 +6,16 @@
 // with k, v the values that the cache holds: 8-bit ones under their block's
 // scale, f32 rows in the open block.
 //
-// Columns: the count_i * G query rows of an item that read one kv head. A
-// workgroup takes up to 16 C of them over a range of keys; its four waves take
+// Columns: the count_i * G query rows of an item that read one kv head.
+// vk_bkv_attn takes up to 32 of them over a range of keys; its four waves take
 // the range's units of 32 keys in turn, each with an online softmax of its own,
-// and merge through LDS at the end: no barrier in the key loop. The 8-bit values
-// are exact in fp16, so a product is two fp16 matrix instructions, one for each
-// part of the f32 operand (22 bits): q in two parts under a power of two that
-// puts its row's largest value at 2^14, weights in two parts of 2^14 w.
+// and merge through LDS at the end: no barrier in the key loop.
+// vk_bkv_attn_chunk takes 128, 32 a wave, all waves over the same units, which
+// they widen to fp16 in LDS together (double buffered, one barrier a unit).
+// The 8-bit values are exact in fp16, so a product is two fp16 matrix
+// instructions, one for each part of the f32 operand (22 bits): q in two parts
+// under a power of two that puts its row's largest value at 2^14, weights in two
+// parts of 2^14 w.
 //   S^T [keys][columns] = K q^T: K's 16-byte loads are operand registers but for
 //     the widening (the pages hold tiles in that order);
 //   P's accumulator layout (4 consecutive keys a lane) is the operand layout of
@@ -43,9 +46,12 @@ struct BkvAttnArgs {
     size_t part_o;      // floats before the partial outputs
     float scale_log2;   // scale * log2(e)
     int layer, hq, g;   // g = hq / n_head
+    uint32_t g_inv, splits_inv;  // ceil(2^32 / g), ceil(2^32 / splits): see bkv_div
     int tile0;          // first column tile of this launch
-    int chunks;         // 0: one column tile an item (at most 16 C columns); 1: as many as its columns need
+    int tiles;          // column tiles of the call
+    int chunks;         // 0: one column tile an item; 1: as many as its columns need
     int splits;         // key ranges a column tile may have (grid)
+    int per;            // least units of a key range (chunks), 0: 8
     int cols;           // columns a slot has room for
 };
 
@@ -58,16 +64,22 @@ struct BkvTile {
     int keys;       // keys that its last row sees
     int full;       // keys in full blocks, no more than keys rounded up to a tile
     int units, per; // units of the 8-bit part, units a key range
-    int ranges;     // key ranges (at least one)
+    __device__ __forceinline__ bool one() const { return per >= units; }               // one key range
+    __device__ __forceinline__ bool beyond(int s) const { return s && s * per >= units; }  // no range s
+    __device__ __forceinline__ bool final(int s) const { return (s + 1) * per >= units; }  // the last range
 };
 
-// Tile T of the launch's order: item T, or the item whose tiles T is one of
-// (item i's begin at row0_i * g / tc + i: room for a partly filled tile each).
+// x / d for inv = ceil(2^32 / d): exact while x (d - 1) < 2^32
+__device__ __forceinline__ int bkv_div(int x, uint32_t inv) { return inv ? (int)__umulhi((uint32_t)x, inv) : x; }
+
+// Tile T of the launch's order: item T, or (CHUNKS) the item whose tiles T is one
+// of: item i's begin at row0_i * g / tc + i (room for a partly filled tile each).
 // Every thread returns the same; false: no such tile. sh: one int of LDS.
+template <bool CHUNKS>
 __device__ __forceinline__ bool bkv_tile(const BkvAttnArgs& a, int tile, int tc, int* sh, BkvTile& t) {
-    const int n = a.v.meta[BKV_STEP_N];
-    int i = tile, k = 0;
-    if (a.chunks) {
+    const int bs_log = 31 - __clz(a.v.bs);
+    if constexpr (CHUNKS) {
+        const int n = a.v.meta[BKV_STEP_N];
         if (threadIdx.x == 0) *sh = -1;
         __syncthreads();
         for (int x = threadIdx.x; x < n; x += blockDim.x) {
@@ -77,23 +89,23 @@ __device__ __forceinline__ bool bkv_tile(const BkvAttnArgs& a, int tile, int tc,
             if (tile >= lo && tile < hi) *sh = x;
         }
         __syncthreads();
-        i = *sh;
+        const int i = *sh;
         if (i < 0) return false;
         t.it = a.v.step[i];
-        k = tile - (int)((long long)t.it.row0 * a.g / tc + i);
+        t.c0 = (tile - (int)((long long)t.it.row0 * a.g / tc + i)) * tc;
+        t.n = min(tc, t.it.count * a.g - t.c0);
+        if (t.n <= 0) return false;
+        t.keys = t.it.start + (t.c0 + t.n - 1) / a.g + 1;
     } else {
-        if (i >= n) return false;
-        t.it = a.v.step[i];
+        t.it = a.v.step[tile];
+        t.c0 = 0;
+        t.n = t.it.count * a.g;
+        if (t.n <= 0) return false;
+        t.keys = t.it.start + t.it.count;
     }
-    const int cols = t.it.count * a.g;
-    t.c0 = k * tc;
-    t.n = min(tc, cols - t.c0);
-    if (t.n <= 0) return false;
-    t.keys = t.it.start + (t.c0 + t.n - 1) / a.g + 1;
-    t.full = min((t.it.start + t.it.count) / a.v.bs * a.v.bs, (t.keys + 15) & ~15);
+    t.full = min((t.it.start + t.it.count) >> bs_log << bs_log, (t.keys + 15) & ~15);
     t.units = (t.full + kUnit - 1) / kUnit;
-    t.per = max(8, ((t.units + a.splits - 1) / a.splits + 3) & ~3);
-    t.ranges = max(1, (t.units + t.per - 1) / t.per);
+    t.per = max(a.per ? a.per : 8, (bkv_div(t.units + a.splits - 1, a.splits_inv) + 3) & ~3);
     return true;
 }
 
@@ -128,6 +140,13 @@ __device__ __forceinline__ void bkv_split2(float x, float y, half2v& hi, half2v&
     lo = __builtin_convertvector(r, half2v);
 }
 
+// The largest of three, a NaN passed over (fmaxf would first quiet each operand).
+__device__ __forceinline__ float bkv_max3(float a, float b, float c) {
+    float y;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(y) : "v"(a), "v"(b), "v"(c));
+    return y;
+}
+
 // sum / max over the four lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48)
 __device__ __forceinline__ float bkv_max4(float v) {
     v = fmaxf(v, __int_as_float(vk_bfly_partner<16>(__float_as_int(v))));
@@ -138,55 +157,55 @@ __device__ __forceinline__ float bkv_sum4(float v) {
     return v + __int_as_float(vk_bfly_partner<32>(__float_as_int(v)));
 }
 
-template <int HD, int CODEC, int C>
-__global__ __launch_bounds__(256, 2) void vk_bkv_attn(BkvAttnArgs a, const uint8_t* __restrict__ pool,
-                                                      const float2* __restrict__ scales) {
-    constexpr int U = HD / 64, DT = HD / 16, OS = HD + 4;
-    constexpr bool QL = C > 1;  // q's parts in LDS (shared by the waves), else in registers
-    __shared__ uint4 sq[QL ? C * U * 4 * 64 : 1];
-    __shared__ float sqf[C * 16];  // q's factor of each column
-    __shared__ float so[4][16][OS];
-    __shared__ float2 sml[4][16];
-    __shared__ int sh;
-    const int split = blockIdx.x % a.splits, head = blockIdx.y;
-    const int tile = a.tile0 + (int)(blockIdx.x / a.splits);
-    BkvTile t;
-    if (!bkv_tile(a, tile, 16 * C, &sh, t) || split >= t.ranges) return;
-    const BkvView& v = a.v;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, grp = lane >> 4, bs_log = 31 - __clz(v.bs);
+// One wave's query columns in blocks of 16 and what it has summed for them.
+template <int HD, int C, bool CHUNKS>
+struct BkvWave {
+    static constexpr int U = HD / 64, DT = HD / 16;
+    int col, grp;   // lane's column of a block, and its group of 16 lanes
+    float qf[C];    // a score is qf times the product of q's parts
+    int last[C];    // last key that the lane's column sees
+    float M[C], L[C];
+    vk_f32x4 O[C][DT];
 
-    // this wave's units: u0, u0 + 4, .. below u1
-    const int u0 = split * t.per + wave, u1 = min(t.units, (split + 1) * t.per);
-    const int* table = v.table + (size_t)t.it.seq * v.max_blocks;
-    // lane l holds the page of tile l & 1 of the wave's unit k0 + l / 2
-    auto pages_from = [&](int k0) {
-        const int u = min(u0 + 4 * (k0 + (lane >> 1)), t.units - 1);
-        const int key = min(u * kUnit + (lane & 1) * 16, t.full - 16);
-        return table[key >> bs_log];
-    };
-    int pages = 0;
-    if (u0 < u1) pages = pages_from(0);
-
-    // q's parts: lane's 16 values d = 64 u + 16 grp .. of column `col`, two k steps of 8
-    half8v qh[QL ? 1 : 2 * U], ql[QL ? 1 : 2 * U];
-    auto load_q = [&](int ct, half8v* h8, half8v* l8) {
-        const int c = ct * 16 + col;
-        const bool live = c < t.n;
-        const int cc = t.c0 + (live ? c : 0), j = cc / a.g;
-        const float* p = a.q + ((size_t)(t.it.row0 + j) * a.hq + head * a.g + (cc - j * a.g)) * HD + grp * 16;
-        float4 x[4 * U];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int ct = 0; ct < C; ++ct) {
+            M[ct] = -INFINITY;
+            L[ct] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) O[ct][d] = vk_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+    // the row of the item that holds column c of the tile (c < 16 C of the kernel's; chunks: any)
+    __device__ __forceinline__ int item_row(const BkvAttnArgs& a, const BkvTile& t, int c) const {
+        return CHUNKS ? (t.c0 + c) / a.g : bkv_div(c, a.g_inv);
+    }
+    // place in q and out of column c of the tile (of column 0 for one beyond its columns)
+    __device__ __forceinline__ size_t row(const BkvAttnArgs& a, const BkvTile& t, int head, int c) const {
+        c = c < t.n ? c : 0;
+        const int cc = t.c0 + c, j = item_row(a, t, c);
+        return ((size_t)(t.it.row0 + j) * a.hq + head * a.g + (cc - j * a.g)) * HD;
+    }
+    // q of the 16 columns from c0 on: the lane's 16 values d = 64 u + 16 grp .. of
+    // its column (fetch_q), and their parts, two k steps of 8 (split_q)
+    __device__ __forceinline__ void fetch_q(const BkvAttnArgs& a, const BkvTile& t, int head, int c0,
+                                            float4 (&x)[4 * U]) const {
+        const float* p = a.q + row(a, t, head, c0 + col) + grp * 16;
+#pragma unroll
+        for (int i = 0; i < 4 * U; ++i) x[i] = *(const float4*)(p + (i >> 2) * 64 + (i & 3) * 4);
+    }
+    __device__ __forceinline__ void split_q(const BkvAttnArgs& a, const BkvTile& t, int ct, int c0,
+                                            const float4 (&x)[4 * U], half8v (&h8)[2 * U], half8v (&l8)[2 * U]) {
+        const bool live = c0 + col < t.n;
         float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4 * U; ++i) {
-            x[i] = *(const float4*)(p + (i >> 2) * 64 + (i & 3) * 4);
-            if (!live) x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            top = fmaxf(top, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
-        }
-        top = bkv_max4(top);
+        for (int i = 0; i < 4 * U; ++i)
+            top = bkv_max3(top, bkv_max3(fabsf(x[i].x), fabsf(x[i].y), fabsf(x[i].z)), fabsf(x[i].w));
+        top = bkv_max4(live ? top : 0.0f);
         // the largest value goes to 2^14 .. 2^15; rows below 2^-106 keep fewer bits
         const int e = min(141 - (int)(__float_as_uint(top) >> 23), 120);
-        const float up = __uint_as_float((uint32_t)(127 + e) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+        const float up = live ? __uint_as_float((uint32_t)(127 + e) << 23) : 0.0f;
 #pragma unroll
         for (int i = 0; i < 2 * U; ++i) {
             half2v h[4], l[4];
@@ -198,190 +217,79 @@ __global__ __launch_bounds__(256, 2) void vk_bkv_attn(BkvAttnArgs a, const uint8
             h8[i] = half8v{h[0].x, h[0].y, h[1].x, h[1].y, h[2].x, h[2].y, h[3].x, h[3].y};
             l8[i] = half8v{l[0].x, l[0].y, l[1].x, l[1].y, l[2].x, l[2].y, l[3].x, l[3].y};
         }
-        return a.scale_log2 * down;
-    };
-    float qf[C];
-    if constexpr (QL) {
-        for (int ct = wave; ct < C; ct += 4) {
-            half8v h8[2 * U], l8[2 * U];
-            const float f = load_q(ct, h8, l8);
-            if (grp == 0) sqf[ct * 16 + col] = f;
-#pragma unroll
-            for (int i = 0; i < 2 * U; ++i) {
-                sq[((ct * 2 * U + i) * 2 + 0) * 64 + lane] = __builtin_bit_cast(uint4, h8[i]);
-                sq[((ct * 2 * U + i) * 2 + 1) * 64 + lane] = __builtin_bit_cast(uint4, l8[i]);
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int ct = 0; ct < C; ++ct) qf[ct] = sqf[ct * 16 + col];
-    } else {
-        qf[0] = load_q(0, qh, ql);
-    }
-    // last key that each of this lane's columns sees
-    int last[C];
-#pragma unroll
-    for (int ct = 0; ct < C; ++ct) last[ct] = t.it.start + (t.c0 + ct * 16 + col) / a.g;
-    const int first_last = t.it.start + t.c0 / a.g;  // the least of them
-
-    float M[C], L[C];
-    vk_f32x4 O[C][DT];
-#pragma unroll
-    for (int ct = 0; ct < C; ++ct) {
-        M[ct] = -INFINITY;
-        L[ct] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) O[ct][d] = vk_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        qf[ct] = a.scale_log2 * down;
+        last[ct] = t.it.start + item_row(a, t, c0 + col);
     }
     // the running maximum of a column becomes m; what was summed so far shrinks
-    auto raise = [&](int ct, float m) {
+    __device__ __forceinline__ void raise(int ct, float m) {
         if (__any(m > M[ct])) {
-            const float to = fmaxf(M[ct], m), c = M[ct] == -INFINITY ? 0.0f : exp2f(M[ct] - to);
+            const float to = fmaxf(M[ct], m), c = M[ct] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M[ct] - to);
             M[ct] = to;
             L[ct] *= c;
 #pragma unroll
             for (int d = 0; d < DT; ++d) O[ct][d] *= c;
         }
-    };
-
-    const size_t layer_page = (size_t)a.layer * v.n_page;
-    uint4 kr[2][U], vr[2][U];
-    float2 sc[2];
-    const uint8_t *kp[2], *vp[2];
-    auto at = [&](int u, int k) {  // addresses of unit u, the k-th of this wave
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const int page = __builtin_amdgcn_readlane(pages, 2 * (k & 31) + x);
-            const int key = min(u * kUnit + x * 16, t.full - 16);
-            const size_t chunk = (layer_page + page) * v.n_head + head;
-            kp[x] = pool + chunk * 2 * v.bs * HD + (size_t)((key & (v.bs - 1)) >> 4) * 16 * HD + lane * 16;
-            vp[x] = kp[x] + (size_t)v.bs * HD;
-            sc[x] = scales[chunk];
-        }
-    };
-    auto load = [&](uint4 (&r)[2][U], const uint8_t* const (&p)[2]) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int u = 0; u < U; ++u) r[x][u] = *(const uint4*)(p[x] + u * 1024);
-    };
-    if (u0 < u1) {
-        at(u0, 0);
-        load(kr, kp);
-        load(vr, vp);
     }
-    for (int u = u0, k = 0; u < u1; u += 4, ++k) {
-        // S^T of both tiles: raw scores under qf * K's scale
-        vk_f32x4 S[C][2];
-#pragma unroll
-        for (int ct = 0; ct < C; ++ct) S[ct][0] = S[ct][1] = vk_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < 2 * U; ++i) {
-            half8v ka[2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-                ka[x] = bkv_widen8<CODEC>(u4c(kr[x][i >> 1], 2 * (i & 1)), u4c(kr[x][i >> 1], 2 * (i & 1) + 1));
-#pragma unroll
-            for (int ct = 0; ct < C; ++ct) {
-                half8v h8, l8;
-                if constexpr (QL) {
-                    h8 = __builtin_bit_cast(half8v, sq[((ct * 2 * U + i) * 2 + 0) * 64 + lane]);
-                    l8 = __builtin_bit_cast(half8v, sq[((ct * 2 * U + i) * 2 + 1) * 64 + lane]);
-                } else {
-                    h8 = qh[i];
-                    l8 = ql[i];
-                }
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    S[ct][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[x], l8, S[ct][x], 0, 0, 0);
-                    S[ct][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[x], h8, S[ct][x], 0, 0, 0);
-                }
-            }
-        }
-        float ks[2], vf[2], ve[2], back[2];
+    // raw scores of a unit (32 keys from key0 on, none from `full` on) -> the two
+    // parts of 2^14 times its weights, V's scales in them. hide: some key is
+    // hidden from some column.
+    __device__ __forceinline__ void weigh(int ct, const vk_f32x4 (&S)[2], const float2 (&sc)[2], int key0, int full,
+                                          bool hide, half8v& ph, half8v& pl) {
+        float s[8], vf[2], back[2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            ks[x] = sc[x].x;
             const uint32_t b = __float_as_uint(sc[x].y);
             const int e = (int)((b >> 23) & 255);
             const bool plain = e != 0 && e != 255;  // zero: f 0, e 0; not finite: f NaN, e 0
             vf[x] = plain ? __uint_as_float((b & 0x007fffffu) | 0x46800000u) : sc[x].y;  // f 2^14
-            ve[x] = plain ? (float)(e - 127) : 0.0f;
             back[x] = plain ? __uint_as_float((uint32_t)min(254 - e, 253) << 23) : 1.0f;  // 2^-e
+            const float ve = plain ? (float)(e - 127) : 0.0f, f = sc[x].x * qf[ct];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[4 * x + r] = fmaf(S[x][r], f, ve);
         }
-        const bool more = u + 4 < u1;
-        if (more) {
-            if (((k + 1) & 31) == 0) pages = pages_from(k + 1);
-            at(u + 4, k + 1);
-            load(kr, kp);
+        if (hide) {
+            const int lim = min(last[ct] + 1, full);
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (key0 + (r >> 2) * 16 + grp * 4 + (r & 3) >= lim) s[r] = -INFINITY;
         }
-        const bool hide = u * kUnit + kUnit > min(first_last + 1, t.full);
-        half8v ph[C], pl[C];
+        const float m = bkv_max3(bkv_max3(s[0], s[1], s[2]), bkv_max3(s[3], s[4], s[5]), fmaxf(s[6], s[7]));
+        raise(ct, bkv_max4(m));
+        const float base = M[ct] == -INFINITY ? 0.0f : M[ct];
+        float w[8];
 #pragma unroll
-        for (int ct = 0; ct < C; ++ct) {
-            float s[8];
-            float m = -INFINITY;
+        for (int x = 0; x < 2; ++x) {
+            float sum = 0.0f;
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const float f = ks[x] * qf[ct];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) s[4 * x + r] = fmaf(S[ct][x][r], f, ve[x]);
+            for (int r = 0; r < 4; ++r) {
+                const float e = __builtin_amdgcn_exp2f(s[4 * x + r] - base);
+                sum += e;
+                w[4 * x + r] = e * vf[x];
             }
-            if (hide) {
-                const int lim = min(last[ct] + 1, t.full);
-#pragma unroll
-                for (int r = 0; r < 8; ++r)
-                    if (u * kUnit + (r >> 2) * 16 + grp * 4 + (r & 3) >= lim) s[r] = -INFINITY;
-            }
-#pragma unroll
-            for (int r = 0; r < 8; ++r) m = fmaxf(m, s[r]);
-            raise(ct, bkv_max4(m));
-            const float base = M[ct] == -INFINITY ? 0.0f : M[ct];
-            float w[8];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                float sum = 0.0f;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float e = __builtin_amdgcn_exp2f(s[4 * x + r] - base);
-                    sum += e;
-                    w[4 * x + r] = e * vf[x];
-                }
-                L[ct] = fmaf(sum, back[x], L[ct]);
-            }
-            if (hide) {  // a hidden key has no part in a block whose scale is NaN
-#pragma unroll
-                for (int r = 0; r < 8; ++r)
-                    if (s[r] == -INFINITY) w[r] = 0.0f;
-            }
-            half2v h[4], l[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) bkv_split2(w[2 * r], w[2 * r + 1], h[r], l[r]);
-            ph[ct] = half8v{h[0].x, h[0].y, h[1].x, h[1].y, h[2].x, h[2].y, h[3].x, h[3].y};
-            pl[ct] = half8v{l[0].x, l[0].y, l[1].x, l[1].y, l[2].x, l[2].y, l[3].x, l[3].y};
+            L[ct] = fmaf(sum, back[x], L[ct]);
         }
+        if (hide) {  // a hidden key has no part in a block whose scale is NaN
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-            const half8v va = bkv_widen8<CODEC>(u4c(vr[0][d >> 2], d & 3), u4c(vr[1][d >> 2], d & 3));
-#pragma unroll
-            for (int ct = 0; ct < C; ++ct) {
-                O[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[ct], O[ct][d], 0, 0, 0);
-                O[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[ct], O[ct][d], 0, 0, 0);
-            }
+            for (int r = 0; r < 8; ++r)
+                if (s[r] == -INFINITY) w[r] = 0.0f;
         }
-        if (more) load(vr, vp);
+        half2v h[4], l[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) bkv_split2(w[2 * r], w[2 * r + 1], h[r], l[r]);
+        ph = half8v{h[0].x, h[0].y, h[1].x, h[1].y, h[2].x, h[2].y, h[3].x, h[3].y};
+        pl = half8v{l[0].x, l[0].y, l[1].x, l[1].y, l[2].x, l[2].y, l[3].x, l[3].y};
     }
-
-    // the open block's rows: tile `wave` of them, in the last key range
-    const int key0 = t.full + wave * 16;
-    if (split == t.ranges - 1 && key0 < t.keys) {
+    // 16 f32 rows of the open block, from key0 on; columns c0 ..
+    __device__ __forceinline__ void open_rows(const BkvAttnArgs& a, const BkvTile& t, int head, int key0, int c0) {
+        const BkvView& v = a.v;
         const size_t side = (size_t)v.n_head * 2 * v.bs * HD;
         const float* ring = v.ring + ((size_t)a.layer * v.n_seq + t.it.seq) * 2 * side + (size_t)head * 2 * v.bs * HD;
         const int ring_mask = 2 * v.bs - 1;
-        const float* kp1 = ring + (size_t)((key0 + col) & ring_mask) * HD + grp * 4;
+        const float* kp = ring + (size_t)((key0 + col) & ring_mask) * HD + grp * 4;
         const float* vring = ring + side;
-        // V: four rows (keys 4 grp + r), column 16 d + col; rows that no column sees are not used
+        // V: four rows (keys 4 grp + r), columns 16 d + col; rows that no column sees are not used
         float vv[DT][4];
+        float top = 0.0f;
         bool odd = false;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -392,16 +300,12 @@ __global__ __launch_bounds__(256, 2) void vk_bkv_attn(BkvAttnArgs a, const uint8
                 const float y = p[16 * d];
                 vv[d][r] = key < t.keys ? y : 0.0f;
                 odd = odd || !(fabsf(vv[d][r]) < INFINITY);
+                top = fmaxf(top, fabsf(vv[d][r]));
             }
         }
         const bool any_odd = __any(odd);
         // a power of two in the place of a block's scale, so that the maximum
         // weighs these rows like the blocks: the largest |v| is 2^9 .. 2^10 of it
-        float top = 0.0f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) top = fmaxf(top, fabsf(vv[d][r]));
         top = vk_group_max<64>(any_odd ? 0.0f : top);
         const int te = top < 0x1p-100f ? 0 : (int)(__float_as_uint(top) >> 23) - 136;
         const float tdown = __uint_as_float((uint32_t)(127 - te) << 23);
@@ -411,13 +315,11 @@ __global__ __launch_bounds__(256, 2) void vk_bkv_attn(BkvAttnArgs a, const uint8
             for (int r = 0; r < 4; ++r) vv[d][r] *= tdown;
 #pragma unroll
         for (int ct = 0; ct < C; ++ct) {
-            const int c = ct * 16 + col;
-            const int cc = t.c0 + (c < t.n ? c : 0), j = cc / a.g;
-            const float* p = a.q + ((size_t)(t.it.row0 + j) * a.hq + head * a.g + (cc - j * a.g)) * HD + grp * 4;
+            const float* p = a.q + row(a, t, head, c0 + ct * 16 + col) + grp * 4;
             vk_f32x4 s4 = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < HD / 16; ++i) {
-                const float4 x = *(const float4*)(kp1 + 16 * i), y = *(const float4*)(p + 16 * i);
+#pragma unroll 4
+            for (int i = 0; i < DT; ++i) {
+                const float4 x = *(const float4*)(kp + 16 * i), y = *(const float4*)(p + 16 * i);
                 s4 = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x, y.x, s4, 0, 0, 0);
                 s4 = __builtin_amdgcn_mfma_f32_16x16x4f32(x.y, y.y, s4, 0, 0, 0);
                 s4 = __builtin_amdgcn_mfma_f32_16x16x4f32(x.z, y.z, s4, 0, 0, 0);
@@ -444,107 +346,451 @@ __global__ __launch_bounds__(256, 2) void vk_bkv_attn(BkvAttnArgs a, const uint8
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         O[ct][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[d][r], e[r], O[ct][d], 0, 0, 0);
-            } else {
-                // a value that is not finite: only the columns that see its key take it
-                for (int x = 0; x < 16 && key0 + x < t.keys; ++x) {
-                    float w = 0.0f;
+                continue;
+            }
+            // a value that is not finite: only the columns that see its key take it
+            for (int x = 0; x < 16 && key0 + x < t.keys; ++x) {
+                float w = 0.0f;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if ((x & 3) == r) w = __shfl(e[r], (x >> 2) * 16 + col, VK_WAVE);
-                    const float* p1 = vring + (size_t)((key0 + x) & ring_mask) * HD + grp * 4;
-                    if (key0 + x <= last[ct]) {
+                for (int r = 0; r < 4; ++r)
+                    if ((x & 3) == r) w = __shfl(e[r], (x >> 2) * 16 + col, VK_WAVE);
+                const float* p1 = vring + (size_t)((key0 + x) & ring_mask) * HD + grp * 4;
+                if (key0 + x <= last[ct]) {
 #pragma unroll
-                        for (int d = 0; d < DT; ++d) {
-                            const float4 y = *(const float4*)(p1 + 16 * d);
-                            O[ct][d][0] = fmaf(w, y.x, O[ct][d][0]);
-                            O[ct][d][1] = fmaf(w, y.y, O[ct][d][1]);
-                            O[ct][d][2] = fmaf(w, y.z, O[ct][d][2]);
-                            O[ct][d][3] = fmaf(w, y.w, O[ct][d][3]);
-                        }
+                    for (int d = 0; d < DT; ++d) {
+                        const float4 y = *(const float4*)(p1 + 16 * d);
+                        O[ct][d][0] = fmaf(w, y.x, O[ct][d][0]);
+                        O[ct][d][1] = fmaf(w, y.y, O[ct][d][1]);
+                        O[ct][d][2] = fmaf(w, y.z, O[ct][d][2]);
+                        O[ct][d][3] = fmaf(w, y.w, O[ct][d][3]);
                     }
                 }
             }
         }
     }
+};
 
-    // the four waves' results of each 16 columns, merged by all threads
-    const bool direct = t.ranges == 1;
-    const size_t slot = ((size_t)(tile - a.tile0) * v.n_head + head) * a.splits + split;
+// Where the tiles of one (layer, head) are: page p at base + p * stride, its
+// scales at sc[p * n_head].
+struct BkvPlace {
+    const uint8_t* base;
+    const float2* sc;
+    uint32_t stride, n_head;
+    __device__ __forceinline__ BkvPlace(const BkvView& v, int layer, int head, const uint8_t* pool,
+                                        const float2* scales) {
+        const uint32_t chunk = 2u * (uint32_t)(v.bs * v.hd);
+        const size_t first = (size_t)layer * v.n_page * v.n_head + head;
+        base = pool + first * chunk;
+        sc = scales + first;
+        n_head = (uint32_t)v.n_head;
+        stride = n_head * chunk;
+    }
+    // tile of a page that holds key
+    __device__ __forceinline__ const uint8_t* tile(int page, int key, int bs, int hd) const {
+        return base + (uint64_t)(uint32_t)page * stride + (uint32_t)(((key & (bs - 1)) >> 4) * 16 * hd);
+    }
+    __device__ __forceinline__ float2 scale(int page) const { return sc[(uint64_t)(uint32_t)page * n_head]; }
+};
+
+constexpr int kWaves = 4;  // of the kernel below
+
+template <int HD, int CODEC, int C>
+__global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(BkvAttnArgs a, const uint8_t* __restrict__ pool,
+                                                                   const float2* __restrict__ scales) {
+    using W = BkvWave<HD, C, false>;
+    constexpr int U = W::U, DT = W::DT, OS = HD + 4;
+    // q's parts while keys are read (16 columns: in each wave's registers instead),
+    // the waves' outputs after
+    __shared__ union {
+        uint4 q[C > 1 ? C * U * 4 * 64 : 1];
+        float o[kWaves][16][OS];
+    } sh;
+    __shared__ float sqf[C * 16];  // q's factor of each column
+    __shared__ float2 sml[kWaves][16];
+    // ranges are the grid's slowest index: those that short items do not have come last
+    const int tile = a.tile0 + (int)blockIdx.x, head = blockIdx.y, split = blockIdx.z;
+    BkvTile t;
+    if (!bkv_tile<false>(a, tile, 16 * C, nullptr, t) || t.beyond(split)) return;
+    const BkvView& v = a.v;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int bs_log = 31 - __clz(v.bs);
+    W w;
+    w.col = lane & 15;
+    w.grp = lane >> 4;
+
+    // this wave's units: u0, u0 + kWaves, .. below u1
+    const int u0 = split * t.per + wave, u1 = min(t.units, (split + 1) * t.per);
+    const int* table = v.table + (size_t)t.it.seq * v.max_blocks;
+    // lane l holds the page of tile l & 1 of the wave's unit k0 + l / 2
+    auto pages_from = [&](int k0) {
+        const int u = min(u0 + kWaves * (k0 + (lane >> 1)), t.units - 1);
+        const int key = min(u * kUnit + (lane & 1) * 16, t.full - 16);
+        return table[key >> bs_log];
+    };
+    int pages = 0;
+    if (u0 < u1) pages = pages_from(0);
+    const BkvPlace place(v, a.layer, head, pool, scales);
+
+    uint4 kr[2][U], vr[2][U];
+    float2 sc[2];
+    const uint8_t* at[2];
+    // the k-th unit of this wave: its tiles' places, and the loads of K (V: load_v)
+    auto load_k = [&](int u, int k) {
+        if (k > 0 && (k & 31) == 0) pages = pages_from(k);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int page = __builtin_amdgcn_readlane(pages, 2 * (k & 31) + x);
+            at[x] = place.tile(page, min(u * kUnit + x * 16, t.full - 16), v.bs, HD);
+            sc[x] = place.scale(page);
+#pragma unroll
+            for (int i = 0; i < U; ++i) kr[x][i] = ((const uint4*)(at[x] + i * 1024))[lane];
+        }
+    };
+    auto load_v = [&]() {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int i = 0; i < U; ++i) vr[x][i] = ((const uint4*)(at[x] + v.bs * HD + i * 1024))[lane];
+    };
+    half8v qh[2 * U], ql[2 * U];
+    float4 x[4 * U];
+    if (C == 1 || wave < C) w.fetch_q(a, t, head, C == 1 ? 0 : wave * 16, x);
+    w.clear();
+#pragma unroll
+    for (int ct = 0; ct < C; ++ct) w.last[ct] = t.it.start + w.item_row(a, t, ct * 16 + w.col);
+    // The open block's rows, in the last key range: a tile a wave, from the last
+    // wave down (the range's last units are few more often than not), and before
+    // the wave's units: these rows wait for no page.
+    const int open = t.full + (kWaves - 1 - wave) * 16;
+    if (t.final(split) && open < t.keys) w.open_rows(a, t, head, open, 0);
+    if (u0 < u1) {
+        load_k(u0, 0);
+        load_v();
+    }
+    if constexpr (C == 1) {
+        w.split_q(a, t, 0, 0, x, qh, ql);
+    } else {
+        if (wave < C) {
+            w.split_q(a, t, 0, wave * 16, x, qh, ql);
+            if (w.grp == 0) sqf[wave * 16 + w.col] = w.qf[0];
+#pragma unroll
+            for (int i = 0; i < 2 * U; ++i) {
+                sh.q[((wave * 2 * U + i) * 2 + 0) * 64 + lane] = __builtin_bit_cast(uint4, qh[i]);
+                sh.q[((wave * 2 * U + i) * 2 + 1) * 64 + lane] = __builtin_bit_cast(uint4, ql[i]);
+            }
+        }
+        VK_LDS_BARRIER();
+#pragma unroll
+        for (int ct = 0; ct < C; ++ct) {
+            w.qf[ct] = sqf[ct * 16 + w.col];
+            w.last[ct] = t.it.start + w.item_row(a, t, ct * 16 + w.col);
+        }
+    }
+
+    for (int u = u0, k = 0; u < u1; u += kWaves, ++k) {
+        // S^T of both tiles: raw scores under qf * K's scale
+        vk_f32x4 S[C][2];
+#pragma unroll
+        for (int ct = 0; ct < C; ++ct) S[ct][0] = S[ct][1] = vk_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < 2 * U; ++i) {
+            half8v ka[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+                ka[x] = bkv_widen8<CODEC>(u4c(kr[x][i >> 1], 2 * (i & 1)), u4c(kr[x][i >> 1], 2 * (i & 1) + 1));
+#pragma unroll
+            for (int ct = 0; ct < C; ++ct) {
+                half8v h8 = qh[i], l8 = ql[i];
+                if constexpr (C > 1) {
+                    h8 = __builtin_bit_cast(half8v, sh.q[((ct * 2 * U + i) * 2 + 0) * 64 + lane]);
+                    l8 = __builtin_bit_cast(half8v, sh.q[((ct * 2 * U + i) * 2 + 1) * 64 + lane]);
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    S[ct][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[x], l8, S[ct][x], 0, 0, 0);
+                    S[ct][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[x], h8, S[ct][x], 0, 0, 0);
+                }
+            }
+        }
+        const float2 now[2] = {sc[0], sc[1]};
+        const bool more = u + kWaves < u1;
+        if (more) load_k(u + kWaves, k + 1);
+        const bool hide = u * kUnit + kUnit > min(t.it.start + 1, t.full);
+        half8v ph[C], pl[C];
+#pragma unroll
+        for (int ct = 0; ct < C; ++ct) w.weigh(ct, S[ct], now, u * kUnit, t.full, hide, ph[ct], pl[ct]);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            const half8v va = bkv_widen8<CODEC>(u4c(vr[0][d >> 2], d & 3), u4c(vr[1][d >> 2], d & 3));
+#pragma unroll
+            for (int ct = 0; ct < C; ++ct) {
+                w.O[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[ct], w.O[ct][d], 0, 0, 0);
+                w.O[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[ct], w.O[ct][d], 0, 0, 0);
+            }
+        }
+        if (more) load_v();
+    }
+
+    // the waves' results of each 16 columns, merged by all threads
+    const bool direct = t.one();
+    const size_t slot = ((size_t)blockIdx.x * v.n_head + head) * a.splits + split;
 #pragma unroll
     for (int ct = 0; ct < C; ++ct) {
         if (ct * 16 >= t.n) break;
-        const float l = bkv_sum4(L[ct]);
-        if (ct > 0) __syncthreads();
-        if (grp == 0) sml[wave][col] = make_float2(M[ct], l);
+        const float l = bkv_sum4(w.L[ct]);
+        __syncthreads();  // q's parts, or the columns before, are done with
+        if (w.grp == 0) sml[wave][w.col] = make_float2(w.M[ct], l);
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-            *(vk_f32x4*)&so[wave][col][16 * d + 4 * grp] = O[ct][d];
+        for (int d = 0; d < DT; ++d) *(vk_f32x4*)&sh.o[wave][w.col][16 * d + 4 * w.grp] = w.O[ct][d];
         __syncthreads();
-        constexpr int PER = HD / 16;  // values a thread: 16 threads a column
-        const int c = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 4;
+        constexpr int PT = 4 * kWaves, PD = HD / PT;  // threads a column, values a thread
+        const int c = threadIdx.x / PT, d0 = (threadIdx.x % PT) * PD;
         if (ct * 16 + c < t.n) {
-            float m = -INFINITY, sum = 0.0f, w[4];
+            float m = -INFINITY, sum = 0.0f, y[PD];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) m = fmaxf(m, sml[x][c].x);
+            for (int x = 0; x < kWaves; ++x) m = fmaxf(m, sml[x][c].x);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                w[x] = sml[x][c].x == -INFINITY && sml[x][c].y == 0.0f ? 0.0f
-                       : m == -INFINITY ? 1.0f : exp2f(sml[x][c].x - m);
-                sum = fmaf(sml[x][c].y, w[x], sum);
+            for (int i = 0; i < PD; ++i) y[i] = 0.0f;
+#pragma unroll
+            for (int x = 0; x < kWaves; ++x) {
+                const float2 ml = sml[x][c];
+                const float f = ml.x == -INFINITY && ml.y == 0.0f ? 0.0f
+                                : m == -INFINITY                  ? 1.0f
+                                                                  : __builtin_amdgcn_exp2f(ml.x - m);
+                sum = fmaf(ml.y, f, sum);
+                if (f != 0.0f)
+#pragma unroll
+                    for (int i = 0; i < PD; ++i) y[i] = fmaf(sh.o[x][c][d0 + i], f, y[i]);
             }
-            const int cc = t.c0 + ct * 16 + c, j = cc / a.g;
-            float* dst = direct ? a.out + ((size_t)(t.it.row0 + j) * a.hq + head * a.g + (cc - j * a.g)) * HD
+            float* dst = direct ? a.out + w.row(a, t, head, ct * 16 + c)
                                 : a.part + a.part_o + (slot * a.cols + ct * 16 + c) * HD;
             const float f = direct ? 0x1p-14f / sum : 0x1p-14f;
             if (!direct && d0 == 0) ((float2*)a.part)[slot * a.cols + ct * 16 + c] = make_float2(m, sum);
 #pragma unroll
-            for (int b = 0; b < PER / 4; ++b) {
-                const int d = d0 + 64 * b;
-                vk_f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    if (w[x] != 0.0f) y += *(const vk_f32x4*)&so[x][c][d] * w[x];
-                *(vk_f32x4*)(dst + d) = y * f;
-            }
+            for (int i = 0; i < PD; ++i) dst[d0 + i] = y[i] * f;
         }
     }
 }
 
-// The key ranges of a column tile, merged in their order: 16 threads a column
-// (HD = 64) or 32 (128).
-template <int HD>
+constexpr int kChunkCols = 128;  // columns of a workgroup of the kernel below
+
+template <int HD, int CODEC>
+__global__ __launch_bounds__(256, 2) void vk_bkv_attn_chunk(BkvAttnArgs a, const uint8_t* __restrict__ pool,
+                                                            const float2* __restrict__ scales) {
+    constexpr int C = 2;
+    using W = BkvWave<HD, C, true>;
+    constexpr int U = W::U, DT = W::DT;
+    __shared__ uint4 kv[2][8 * U * 64];  // a unit's fragments: K [tile][k step], then V [d tile]
+    __shared__ int sh;
+    // later rows see more keys: they start first
+    const int tile = a.tiles - 1 - (a.tile0 + (int)blockIdx.x), head = blockIdx.y, split = blockIdx.z;
+    BkvTile t;
+    if (!bkv_tile<true>(a, tile, kChunkCols, &sh, t) || t.beyond(split)) return;
+    const BkvView& v = a.v;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int bs_log = 31 - __clz(v.bs), c0 = wave * 32;
+    W w;
+    w.col = lane & 15;
+    w.grp = lane >> 4;
+    const int u0 = split * t.per, u1 = min(t.units, (split + 1) * t.per);
+    const int* table = v.table + (size_t)t.it.seq * v.max_blocks;
+    // lane l holds the page of tile l of the units k0 .. k0 + 31 of the range
+    auto pages_from = [&](int k0) {
+        const int key = min((u0 + k0) * kUnit + lane * 16, t.full - 16);
+        return table[key >> bs_log];
+    };
+    int pages = u0 < u1 ? pages_from(0) : 0;
+    const BkvPlace place(v, a.layer, head, pool, scales);
+    // wave's 1 KB pieces of a unit: U = 2: K's and V's piece (tile wave / 2, half
+    // wave % 2); U = 1: waves 0, 1 K's tiles, 2, 3 V's
+    uint4 raw[U];
+    float2 sc[2], sc_next[2];
+    auto load = [&](int k) {
+        if (k > 0 && (k & 31) == 0) pages = pages_from(k);
+        const int u = u0 + k, xw = U == 2 ? wave >> 1 : wave & 1;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int page = __builtin_amdgcn_readlane(pages, 2 * (k & 31) + x);
+            sc_next[x] = place.scale(page);
+            if (x == xw) {
+                const uint8_t* p = place.tile(page, min(u * kUnit + x * 16, t.full - 16), v.bs, HD);
+                if constexpr (U == 2) {
+                    p += (wave & 1) * 1024;
+                    raw[0] = ((const uint4*)p)[lane];
+                    raw[1] = ((const uint4*)(p + v.bs * HD))[lane];
+                } else {
+                    raw[0] = ((const uint4*)(p + (wave >> 1) * v.bs * HD))[lane];
+                }
+            }
+        }
+    };
+    auto widen_k = [&](uint4* b, const uint4& r, int x, int i) {
+        b[(x * 2 * U + 2 * i) * 64 + lane] = __builtin_bit_cast(uint4, bkv_widen8<CODEC>(r.x, r.y));
+        b[(x * 2 * U + 2 * i + 1) * 64 + lane] = __builtin_bit_cast(uint4, bkv_widen8<CODEC>(r.z, r.w));
+    };
+    auto widen_v = [&](uint4* b, const uint4& r, int x, int i) {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            half2v p, q;
+            bkv_widen<CODEC>(u4c(r, d), p, q);
+            ((uint2*)&b[(4 * U + 4 * i + d) * 64 + lane])[x] =
+                make_uint2(__builtin_bit_cast(uint32_t, p), __builtin_bit_cast(uint32_t, q));
+        }
+    };
+    auto widen = [&](int buf) {
+        if constexpr (U == 2) {
+            widen_k(kv[buf], raw[0], wave >> 1, wave & 1);
+            widen_v(kv[buf], raw[1], wave >> 1, wave & 1);
+        } else if (wave < 2) {
+            widen_k(kv[buf], raw[0], wave, 0);
+        } else {
+            widen_v(kv[buf], raw[0], wave - 2, 0);
+        }
+    };
+    if (u0 < u1) load(0);
+    half8v qh[C][2 * U], ql[C][2 * U];
+#pragma unroll
+    for (int ct = 0; ct < C; ++ct) {
+        float4 x[4 * U];
+        w.fetch_q(a, t, head, c0 + ct * 16, x);
+        w.split_q(a, t, ct, c0 + ct * 16, x, qh[ct], ql[ct]);
+    }
+    w.clear();
+    // keys that the wave's columns see: all of them below `all`, none from `none` on
+    const bool live = c0 < t.n;
+    const int all = min(t.it.start + (t.c0 + c0) / a.g + 1, t.full);
+    const int none = live ? t.it.start + (t.c0 + min(c0 + 31, t.n - 1)) / a.g + 1 : 0;
+    if (u0 < u1) {
+        widen(0);
+        sc[0] = sc_next[0];
+        sc[1] = sc_next[1];
+        if (u0 + 1 < u1) load(1);
+    }
+    VK_LDS_BARRIER();
+    for (int u = u0, k = 0; u < u1; ++u, ++k) {
+        const uint4* b = kv[k & 1];
+        if (u * kUnit < none) {
+            vk_f32x4 S[C][2];
+#pragma unroll
+            for (int ct = 0; ct < C; ++ct) S[ct][0] = S[ct][1] = vk_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 2 * U; ++i) {
+                half8v ka[2];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) ka[x] = __builtin_bit_cast(half8v, b[(x * 2 * U + i) * 64 + lane]);
+#pragma unroll
+                for (int ct = 0; ct < C; ++ct)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        S[ct][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[x], ql[ct][i], S[ct][x], 0, 0, 0);
+                        S[ct][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[x], qh[ct][i], S[ct][x], 0, 0, 0);
+                    }
+            }
+            const bool hide = u * kUnit + kUnit > all;
+            half8v ph[C], pl[C];
+#pragma unroll
+            for (int ct = 0; ct < C; ++ct) w.weigh(ct, S[ct], sc, u * kUnit, t.full, hide, ph[ct], pl[ct]);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const half8v va = __builtin_bit_cast(half8v, b[(4 * U + d) * 64 + lane]);
+#pragma unroll
+                for (int ct = 0; ct < C; ++ct) {
+                    w.O[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[ct], w.O[ct][d], 0, 0, 0);
+                    w.O[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[ct], w.O[ct][d], 0, 0, 0);
+                }
+            }
+        }
+        if (u + 1 < u1) {
+            widen((k + 1) & 1);
+            sc[0] = sc_next[0];
+            sc[1] = sc_next[1];
+            if (u + 2 < u1) load(k + 2);
+        }
+        VK_LDS_BARRIER();
+    }
+    if (!live) return;
+    if (t.final(split))
+        for (int key0 = t.full; key0 < t.keys; key0 += 16) w.open_rows(a, t, head, key0, c0);
+
+    const bool direct = t.one();
+    const size_t slot = ((size_t)blockIdx.x * v.n_head + head) * a.splits + split;
+#pragma unroll
+    for (int ct = 0; ct < C; ++ct) {
+        const int c = c0 + ct * 16 + w.col;
+        const float l = bkv_sum4(w.L[ct]);
+        if (c >= t.n) continue;
+        float* dst = direct ? a.out + w.row(a, t, head, c) : a.part + a.part_o + (slot * a.cols + c) * HD;
+        const float f = direct ? 0x1p-14f / l : 0x1p-14f;
+        if (!direct && w.grp == 0) ((float2*)a.part)[slot * a.cols + c] = make_float2(w.M[ct], l);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) *(vk_f32x4*)(dst + 16 * d + 4 * w.grp) = w.O[ct][d] * f;
+    }
+}
+
+// The key ranges of a column tile, merged in their order: HD / 4 threads a
+// column, eight ranges' loads in flight.
+template <int HD, bool CHUNKS>
 __global__ __launch_bounds__(256) void vk_bkv_attn_merge(BkvAttnArgs a, int tc) {
     __shared__ int sh;
-    const int head = blockIdx.y, tile = a.tile0 + (int)blockIdx.x;
+    constexpr int PT = HD / 4, B = 8;
+    const int head = blockIdx.y;
+    const int tile = CHUNKS ? a.tiles - 1 - (a.tile0 + (int)blockIdx.x) : a.tile0 + (int)blockIdx.x;
     BkvTile t;
-    if (!bkv_tile(a, tile, tc, &sh, t) || t.ranges == 1) return;
-    constexpr int PT = HD / 4;
+    if (!bkv_tile<CHUNKS>(a, tile, tc, &sh, t) || t.one()) return;
+    const int ranges = (t.units + t.per - 1) / t.per;
+    const int c = blockIdx.z * (256 / PT) + threadIdx.x / PT, d = (threadIdx.x % PT) * 4;
+    if (c >= t.n) return;
     const size_t slot = ((size_t)blockIdx.x * a.v.n_head + head) * a.splits;
-    for (int c = threadIdx.x / PT; c < t.n; c += 256 / PT) {
-        const int d = (threadIdx.x % PT) * 4;
-        float m = -INFINITY;
-        for (int s = 0; s < t.ranges; ++s) m = fmaxf(m, ((const float2*)a.part)[(slot + s) * a.cols + c].x);
-        float sum = 0.0f;
-        vk_f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s = 0; s < t.ranges; ++s) {
-            const float2 ml = ((const float2*)a.part)[(slot + s) * a.cols + c];
-            if (ml.x == -INFINITY && ml.y == 0.0f) continue;
-            const float w = m == -INFINITY ? 1.0f : exp2f(ml.x - m);
-            sum = fmaf(ml.y, w, sum);
-            y += *(const vk_f32x4*)(a.part + a.part_o + ((slot + s) * a.cols + c) * HD + d) * w;
+    const float2* pm = (const float2*)a.part + slot * a.cols + c;
+    const float* po = a.part + a.part_o + (slot * a.cols + c) * HD + d;
+    float m = -INFINITY, sum = 0.0f;
+    vk_f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < ranges; s += B) {
+        float2 ml[B];
+        vk_f32x4 o[B];
+#pragma unroll
+        for (int x = 0; x < B; ++x) {
+            const size_t at = (size_t)min(s + x, ranges - 1) * a.cols;
+            ml[x] = pm[at];
+            o[x] = *(const vk_f32x4*)(po + at * HD);
         }
-        const int cc = t.c0 + c, j = cc / a.g;
-        *(vk_f32x4*)(a.out + ((size_t)(t.it.row0 + j) * a.hq + head * a.g + (cc - j * a.g)) * HD + d) = y * (1.0f / sum);
+        float to = m;
+#pragma unroll
+        for (int x = 0; x < B; ++x) to = fmaxf(to, ml[x].x);
+        const float c0 = m == -INFINITY ? 0.0f : exp2f(m - to);
+        sum *= c0;
+        y *= c0;
+        m = to;
+#pragma unroll
+        for (int x = 0; x < B; ++x) {
+            if (s + x >= ranges || (ml[x].x == -INFINITY && ml[x].y == 0.0f)) continue;
+            const float w = m == -INFINITY ? 1.0f : exp2f(ml[x].x - m);
+            sum = fmaf(ml[x].y, w, sum);
+            y += o[x] * w;
+        }
     }
+    const int cc = t.c0 + c, j = CHUNKS ? cc / a.g : bkv_div(cc, a.g_inv);
+    *(vk_f32x4*)(a.out + ((size_t)(t.it.row0 + j) * a.hq + head * a.g + (cc - j * a.g)) * HD + d) = y * (1.0f / sum);
 }
 
 template <int HD, int CODEC>
-static void go_attn(hipStream_t s, const BkvAttnArgs& a, int c, dim3 grid) {
+static void go_attn(hipStream_t s, const BkvAttnArgs& a, int tc, dim3 grid) {
     const uint8_t* pool = a.v.pool;
     const float2* sc = (const float2*)a.v.scales;
-    if (c == 1) hipLaunchKernelGGL((vk_bkv_attn<HD, CODEC, 1>), grid, dim3(256), 0, s, a, pool, sc);
-    else if (c == 2) hipLaunchKernelGGL((vk_bkv_attn<HD, CODEC, 2>), grid, dim3(256), 0, s, a, pool, sc);
-    else hipLaunchKernelGGL((vk_bkv_attn<HD, CODEC, 4>), grid, dim3(256), 0, s, a, pool, sc);
+    if (tc == 16) hipLaunchKernelGGL((vk_bkv_attn<HD, CODEC, 1>), grid, dim3(64 * kWaves), 0, s, a, pool, sc);
+    else if (tc == 32) hipLaunchKernelGGL((vk_bkv_attn<HD, CODEC, 2>), grid, dim3(64 * kWaves), 0, s, a, pool, sc);
+    else hipLaunchKernelGGL((vk_bkv_attn_chunk<HD, CODEC>), grid, dim3(256), 0, s, a, pool, sc);
+}
+
+template <int HD>
+static void go_hd(hipStream_t s, const BkvAttnArgs& a, int tc, unsigned tiles) {
+    const dim3 grid(tiles, (unsigned)a.v.n_head, (unsigned)a.splits);
+    if (a.v.codec == BKV_INT8) go_attn<HD, BKV_INT8>(s, a, tc, grid);
+    else go_attn<HD, BKV_E4M3>(s, a, tc, grid);
+    constexpr unsigned CW = 256 / (HD / 4);  // columns a merging workgroup
+    const dim3 cols(tiles, (unsigned)a.v.n_head, ((unsigned)a.cols + CW - 1) / CW);
+    if (a.splits > 1 && a.chunks) hipLaunchKernelGGL((vk_bkv_attn_merge<HD, true>), cols, dim3(256), 0, s, a, tc);
+    else if (a.splits > 1) hipLaunchKernelGGL((vk_bkv_attn_merge<HD, false>), cols, dim3(256), 0, s, a, tc);
 }
 
 hipError_t launch_bkv_attn(hipStream_t s, const BkvView& v, int layer, int n, int n_rows, int max_count, int max_len,
@@ -560,37 +806,37 @@ hipError_t launch_bkv_attn(hipStream_t s, const BkvView& v, int layer, int n, in
     a.hq = hq;
     a.g = hq / v.n_head;
     const long long cols = (long long)max_count * a.g;
-    const int c = cols <= 16 ? 1 : cols <= 32 ? 2 : 4, tc = 16 * c;
-    a.chunks = cols > tc;
+    const int tc = cols <= 16 ? 16 : cols <= 32 ? 32 : kChunkCols;
+    a.chunks = cols > 32;
     a.cols = a.chunks ? tc : (int)cols;
     const long long tiles = a.chunks ? (long long)n_rows * a.g / tc + n : n;
-    // Key ranges of 256 keys and more, at most 64 a tile and what the workspace
-    // has room for. For tiles of whole items the number does not depend on the
-    // batch, so an item's rows come out the same in any batch.
-    const int room = kBkvMaxParts * 16;
-    const int units = (max_len + kUnit - 1) / kUnit;
-    long long most = std::min<long long>(64, std::max<long long>(1, room / ((long long)v.n_head * a.cols)));
-    if (a.chunks) most = std::min<long long>(most, std::max<long long>(1, 512 / (tiles * v.n_head)));
-    a.splits = (int)std::min<long long>(most, std::max(1, (units + 7) / 8));
+    a.tiles = (int)tiles;
+    const int room = kBkvParts;
+    const int units = std::max(1, (max_len + kUnit - 1) / kUnit);
+    const long long most = std::min<long long>(64, std::max<long long>(1, room / ((long long)v.n_head * a.cols)));
+    if (a.chunks) {
+        // Ranges of 8 to 64 units: enough for two workgroups a CU, and no tile
+        // much longer than the others.
+        const long long per = tiles * v.n_head * units / 1280;
+        a.per = (int)std::max<long long>(std::min<long long>(std::max<long long>(per, 8), 64), (units + most - 1) / most);
+        a.splits = (units + a.per - 1) / a.per;
+    } else {
+        // Key ranges of 256 keys and more, at most 64 a tile and what the workspace
+        // has room for: that does not depend on the batch, so an item's rows come
+        // out the same in any batch.
+        a.splits = (int)std::min<long long>(most, (units + 7) / 8);
+    }
     a.part_o = (size_t)room * 2;
+    auto inv = [](int d) { return d == 1 ? 0u : (uint32_t)(((1ull << 32) + (uint32_t)d - 1) / (uint32_t)d); };
+    a.g_inv = inv(a.g);
+    a.splits_inv = inv(a.splits);
     // tiles a launch: what the workspace holds, and fewer than 2^24 workgroups
     const long long step = a.splits == 1 ? 1 << 20
                                          : std::max<long long>(1, room / ((long long)v.n_head * a.cols * a.splits));
     for (long long t0 = 0; t0 < tiles; t0 += step) {
-        const long long now = std::min(step, tiles - t0);
         a.tile0 = (int)t0;
-        const dim3 grid((unsigned)(now * a.splits), (unsigned)v.n_head);
-        if (v.hd == 64) {
-            if (v.codec == BKV_INT8) go_attn<64, BKV_INT8>(s, a, c, grid);
-            else go_attn<64, BKV_E4M3>(s, a, c, grid);
-            if (a.splits > 1)
-                hipLaunchKernelGGL(vk_bkv_attn_merge<64>, dim3((unsigned)now, (unsigned)v.n_head), dim3(256), 0, s, a, tc);
-        } else {
-            if (v.codec == BKV_INT8) go_attn<128, BKV_INT8>(s, a, c, grid);
-            else go_attn<128, BKV_E4M3>(s, a, c, grid);
-            if (a.splits > 1)
-                hipLaunchKernelGGL(vk_bkv_attn_merge<128>, dim3((unsigned)now, (unsigned)v.n_head), dim3(256), 0, s, a, tc);
-        }
+        if (v.hd == 64) go_hd<64>(s, a, tc, (unsigned)std::min(step, tiles - t0));
+        else go_hd<128>(s, a, tc, (unsigned)std::min(step, tiles - t0));
     }
     return hipGetLastError();
 }

@@ -14,7 +14,7 @@ struct vokra_hip_bkv {
     vokra_hip_ctx* ctx = nullptr;
     BkvView v = {};
     size_t max_rows = 0;
-    float* part = nullptr;  // partial results of split attention
+    float* part = nullptr;  // the context's partial results of split attention
     // host-array calls: item ids (4 x kBkvMaxItems ints) and, for write, attn
     // and read, rows in and out (grown by those calls only)
     int* items = nullptr;
@@ -101,7 +101,7 @@ void release(vokra_hip_bkv* kv) {
     BkvView& v = kv->v;
     for (void* p : {(void*)v.pool, (void*)v.scales, (void*)v.ring, (void*)v.table, (void*)v.len, (void*)v.floor_,
                     (void*)v.claim, (void*)v.refs, (void*)v.used, (void*)v.fresh, (void*)v.moves, (void*)v.remap,
-                    (void*)v.meta, (void*)v.step, (void*)v.plan, (void*)v.work, (void*)kv->part, (void*)kv->items,
+                    (void*)v.meta, (void*)v.step, (void*)v.plan, (void*)v.work, (void*)kv->items,
                     (void*)kv->rows})
         if (p) (void)hipFree(p);
     delete kv;
@@ -175,10 +175,13 @@ int vokra_hip_bkv_create(vokra_hip_ctx_t* c, size_t n_layer, size_t n_head, size
         return ctx_fail(BAD, "bkv_create: a size is too large (n_layer <= 4096, n_head <= 1024, n_seq <= 65535, "
                              "max_time <= 2^24, n_page <= 2^26, max_rows <= 2^20)");
     BK_TRY(hipSetDevice(vk::ctx_device(c)), "hipSetDevice");
+    void* part = nullptr;
+    BK_ST(vk::ctx_bkv_part(c, (size_t)kBkvParts * (128 + 2) * sizeof(float), &part));
     auto* kv = new (std::nothrow) vokra_hip_bkv();
     if (!kv) return ctx_fail(VOKRA_HIP_ERROR_OTHER, "bkv_create: out of host memory");
     kv->ctx = c;
     kv->max_rows = max_rows;
+    kv->part = (float*)part;
     BkvView& v = kv->v;
     v.n_layer = (int)n_layer;
     v.n_head = (int)n_head;
@@ -208,7 +211,6 @@ int vokra_hip_bkv_create(vokra_hip_ctx_t* c, size_t n_layer, size_t n_head, size
     reserve(&e, &v.step, kBkvMaxItems);
     reserve(&e, &v.plan, kBkvMaxItems);
     reserve(&e, &v.work, (size_t)v.max_work);
-    reserve(&e, &kv->part, (size_t)kBkvMaxParts * 16 * (d_head + 2));
     reserve(&e, &kv->items, 4 * (size_t)kBkvMaxItems);
     if (e == hipSuccess) e = vk::launch_bkv_reset(vk::ctx_stream(c), v, true);
     if (e == hipSuccess) e = hipStreamSynchronize(vk::ctx_stream(c));

@@ -153,6 +153,7 @@ struct vokra_hip_ctx {
     // maxima; im2col columns
     DevBuf fe_win, fe_tw, fe_fb, fe_part, cv_col;
     int fe_mels = 0;
+    DevBuf bk_part;  // partial results of the block caches' attention
     DevBuf ru_part;  // per-slice (max, index) partials of the logits rules
     DevBuf lg_part;  // per-workgroup (max, index) partials of the fused logits argmax
     // RoPE frequency table of the last (rope_base, head_dim) the _dev entry saw
@@ -599,6 +600,11 @@ int check_paged_attn(const vokra_hip_kv* kv, size_t layer, size_t n, size_t hq) 
 namespace vk {
 hipStream_t ctx_stream(const vokra_hip_ctx* c) { return c->stream; }
 int ctx_device(const vokra_hip_ctx* c) { return c->device; }
+int ctx_bkv_part(vokra_hip_ctx* c, size_t bytes, void** p) {
+    VK_TRY(c->bk_part.ensure(bytes), "hipMalloc(partial attention)");
+    *p = c->bk_part.p;
+    return VOKRA_HIP_OK;
+}
 int ctx_rules_part(vokra_hip_ctx* c, size_t bytes, void** p) {
     VK_TRY(c->ru_part.ensure(bytes), "hipMalloc(logits rules)");
     *p = c->ru_part.p;
@@ -1799,7 +1805,7 @@ void vokra_hip_destroy(vokra_hip_ctx_t* c) {
     (void)hipStreamSynchronize(c->stream);
     for (DevBuf* b : {&c->in0, &c->in1, &c->in2, &c->out0, &c->act.frag, &c->act.scale, &c->act.gsum, &c->at_qh,
                       &c->at_ql, &c->at_kh, &c->at_kl, &c->at_vh, &c->at_vl, &c->at_po, &c->at_pml, &c->fe_win, &c->fe_tw, &c->fe_fb,
-                      &c->fe_part, &c->cv_col, &c->lg_part, &c->ru_part,
+                      &c->fe_part, &c->cv_col, &c->lg_part, &c->ru_part, &c->bk_part,
                       &c->rope_theta, &c->rope_pos})
         b->release();
     (void)hipStreamDestroy(c->stream);
