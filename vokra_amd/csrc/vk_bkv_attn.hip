@@ -136,15 +136,12 @@ __device__ __forceinline__ uint32_t u4c(const uint4& v, int i) { return i == 0 ?
 __device__ __forceinline__ void bkv_split2(float x, float y, half2v& hi, half2v& lo) {
     const float2v v = {x, y};
     hi = __builtin_convertvector(v, half2v);
-    const float2v r = {fmaf((float)hi.x, -1.0f, x), fmaf((float)hi.y, -1.0f, y)};
+    // x - hi, exact; the factor is kept from the compiler, which would widen hi
+    // first where one mixed-precision instruction does both
+    float minus = -1.0f;
+    asm("" : "+s"(minus));
+    const float2v r = {fmaf((float)hi.x, minus, x), fmaf((float)hi.y, minus, y)};
     lo = __builtin_convertvector(r, half2v);
-}
-
-// The largest of three, a NaN passed over (fmaxf would first quiet each operand).
-__device__ __forceinline__ float bkv_max3(float a, float b, float c) {
-    float y;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(y) : "v"(a), "v"(b), "v"(c));
-    return y;
 }
 
 // sum / max over the four lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48)
@@ -200,7 +197,7 @@ struct BkvWave {
         float top = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4 * U; ++i)
-            top = bkv_max3(top, bkv_max3(fabsf(x[i].x), fabsf(x[i].y), fabsf(x[i].z)), fabsf(x[i].w));
+            top = fmaxf(top, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
         top = bkv_max4(live ? top : 0.0f);
         // the largest value goes to 2^14 .. 2^15; rows below 2^-106 keep fewer bits
         const int e = min(141 - (int)(__float_as_uint(top) >> 23), 120);
@@ -235,43 +232,46 @@ struct BkvWave {
     // hidden from some column.
     __device__ __forceinline__ void weigh(int ct, const vk_f32x4 (&S)[2], const float2 (&sc)[2], int key0, int full,
                                           bool hide, half8v& ph, half8v& pl) {
-        float s[8], vf[2], back[2];
+        float f[2], ve[2], vf[2], back[2], e[8];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const uint32_t b = __float_as_uint(sc[x].y);
-            const int e = (int)((b >> 23) & 255);
-            const bool plain = e != 0 && e != 255;  // zero: f 0, e 0; not finite: f NaN, e 0
+            const int ex = (int)((b >> 23) & 255);
+            const bool plain = ex != 0 && ex != 255;  // zero: f 0, e 0; not finite: f NaN, e 0
             vf[x] = plain ? __uint_as_float((b & 0x007fffffu) | 0x46800000u) : sc[x].y;  // f 2^14
-            back[x] = plain ? __uint_as_float((uint32_t)min(254 - e, 253) << 23) : 1.0f;  // 2^-e
-            const float ve = plain ? (float)(e - 127) : 0.0f, f = sc[x].x * qf[ct];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s[4 * x + r] = fmaf(S[x][r], f, ve);
+            back[x] = plain ? __uint_as_float((uint32_t)min(254 - ex, 253) << 23) : 1.0f;  // 2^-e
+            ve[x] = plain ? (float)(ex - 127) : 0.0f;
+            f[x] = sc[x].x * qf[ct];
         }
-        if (hide) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) e[r] = fmaf(S[r >> 2][r & 3], f[r >> 2], ve[r >> 2]);
+        auto top = [&]() {
+            const float m = fmaxf(fmaxf(fmaxf(e[0], e[1]), e[2]), fmaxf(fmaxf(e[3], e[4]), e[5]));
+            return bkv_max4(fmaxf(m, fmaxf(e[6], e[7])));
+        };
+        if (!hide) {
+            raise(ct, top());
+        } else {
             const int lim = min(last[ct] + 1, full);
 #pragma unroll
             for (int r = 0; r < 8; ++r)
-                if (key0 + (r >> 2) * 16 + grp * 4 + (r & 3) >= lim) s[r] = -INFINITY;
+                if (key0 + (r >> 2) * 16 + grp * 4 + (r & 3) >= lim) e[r] = -INFINITY;
+            raise(ct, top());
         }
-        const float m = bkv_max3(bkv_max3(s[0], s[1], s[2]), bkv_max3(s[3], s[4], s[5]), fmaxf(s[6], s[7]));
-        raise(ct, bkv_max4(m));
         const float base = M[ct] == -INFINITY ? 0.0f : M[ct];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) e[r] = __builtin_amdgcn_exp2f(e[r] - base);
         float w[8];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            float sum = 0.0f;
+            L[ct] = fmaf((e[4 * x] + e[4 * x + 1]) + (e[4 * x + 2] + e[4 * x + 3]), back[x], L[ct]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float e = __builtin_amdgcn_exp2f(s[4 * x + r] - base);
-                sum += e;
-                w[4 * x + r] = e * vf[x];
-            }
-            L[ct] = fmaf(sum, back[x], L[ct]);
+            for (int r = 0; r < 4; ++r) w[4 * x + r] = e[4 * x + r] * vf[x];
         }
         if (hide) {  // a hidden key has no part in a block whose scale is NaN
 #pragma unroll
             for (int r = 0; r < 8; ++r)
-                if (s[r] == -INFINITY) w[r] = 0.0f;
+                if (e[r] == 0.0f) w[r] = 0.0f;
         }
         half2v h[4], l[4];
 #pragma unroll
@@ -349,6 +349,7 @@ struct BkvWave {
                 continue;
             }
             // a value that is not finite: only the columns that see its key take it
+#pragma unroll 1
             for (int x = 0; x < 16 && key0 + x < t.keys; ++x) {
                 float w = 0.0f;
 #pragma unroll
