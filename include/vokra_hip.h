@@ -427,9 +427,10 @@ typedef struct vokra_hip_bkv vokra_hip_bkv_t;
  * d_head 64 or 128 and block_size 16, 32 or 64 (else UNSUPPORTED_OP). Device
  * memory: n_layer * n_head * (n_page * (2 * block_size * d_head + 8) + n_seq *
  * 16 * block_size * d_head) bytes and some tables; the first cache of a
- * context also takes 136 MB for split attention, which all its caches share. Nothing is allocated by the _dev calls, so all of them can be
- * captured into a graph. A cache belongs to its context's stream: calls on one
- * cache run in the order in which they are made. */
+ * context also takes 136 MB for split attention, which all its caches share.
+ * Nothing is allocated by the _dev calls, so all of them can be captured into a
+ * graph. A cache belongs to its context's stream: calls on one cache run in the
+ * order in which they are made. */
 int vokra_hip_bkv_create(vokra_hip_ctx_t *ctx, size_t n_layer, size_t n_head, size_t d_head, size_t n_seq,
                          size_t max_time, size_t block_size, size_t n_page, size_t max_rows, int codec,
                          vokra_hip_bkv_t **out);
@@ -615,8 +616,8 @@ typedef struct vokra_hip_logits_rules {
 /* logits and out [rows][vocab], rows `stride` floats apart in both; out may be
  * logits (in place), or NULL: only next is wanted; next may be NULL. rows <=
  * 65535, vocab <= 2^24. Device pointers (the struct itself in host memory),
- * asynchronous; the first call with a next on a context allocates 1 MB, so one
- * is made before a capture. */
+ * asynchronous; the first call with a next on a context allocates its 768 KB, so
+ * one is made before a capture. */
 int vokra_hip_logits_rules_dev(vokra_hip_ctx_t *ctx, size_t rows, size_t vocab, size_t stride, const float *d_logits,
                                const vokra_hip_logits_rules_t *rules, float *d_out, int32_t *d_next);
 /* Host arrays (rows side by side), synchronous; offsets out of order or range

@@ -20,7 +20,7 @@ enum {
     BKV_DONE,        // its items done
     BKV_STEP_N,      // items of the current step
     BKV_STEP_ROWS,   // rows of the current step
-    BKV_WORK_N,      // (item, block) entries of the current step's write
+    BKV_WORK_N,      // blocks of the current step's write
     BKV_MOVE_N,      // page moves of the last copy / compact
     BKV_PLAN_N,      // items of the last fork / free / copy
     BKV_META_INTS = 16
@@ -31,6 +31,12 @@ enum {
 // destination, source length, source floor.
 struct BkvItem {
     int seq, start, count, row0;
+};
+
+// One block that an item's rows reach: what its write needs.
+struct alignas(16) BkvWork {
+    int seq, start, end, row0;  // the item: rows start .. end - 1, packed from row0 on
+    int block, page, pad[2];    // page: of a block that the step fills, else -1
 };
 
 struct BkvView {
@@ -53,7 +59,7 @@ struct BkvView {
     int* meta;
     BkvItem* step;   // [kBkvMaxItems] the current step, no rows in entries beyond it
     BkvItem* plan;   // [kBkvMaxItems] items of the current fork / free / copy
-    int2* work;      // [max_work] (item, block) of the current step's write
+    BkvWork* work;   // [max_work] the blocks of the current step's write
     int n_layer, n_head, hd, n_seq, bs, n_page, max_blocks, max_time, codec, max_work;
 };
 
@@ -74,7 +80,7 @@ namespace vk {
 hipError_t launch_bkv_reset(hipStream_t s, const BkvView& v, bool clear_data);
 hipError_t launch_bkv_step(hipStream_t s, const BkvView& v, int n, int n_rows, int max_count, const int* seqs,
                            const int* starts, const int* counts);
-// work_bound: at least the step's (item, block) entries
+// work_bound: at least the step's blocks
 hipError_t launch_bkv_write(hipStream_t s, const BkvView& v, int layer, int work_bound, const float* k, const float* vv);
 hipError_t launch_bkv_read(hipStream_t s, const BkvView& v, int layer, int n, const int* seqs, const int* times,
                            float* k, float* vv);

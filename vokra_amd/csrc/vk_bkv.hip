@@ -31,12 +31,13 @@
 
 namespace vk {
 
-constexpr int BKV_TPB = 1024;
+constexpr int BKV_TPB = 1024;  // threads of the planning kernels at most
 
 // ---- workgroup prefix sums ----------------------------------------------------
 
-// Exclusive prefix sum over the 1024 threads; *total = the sum. red: 17 ints.
+// Exclusive prefix sum over the workgroup; *total = the sum. red: 17 ints.
 __device__ __forceinline__ int bkv_scan(int v, int* red, int* total) {
+    const int waves = (int)blockDim.x >> 6;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int x = v;
 #pragma unroll
@@ -49,15 +50,15 @@ __device__ __forceinline__ int bkv_scan(int v, int* red, int* total) {
     __syncthreads();
     if (threadIdx.x == 0) {
         int s = 0;
-        for (int w = 0; w < BKV_TPB / 64; ++w) {
+        for (int w = 0; w < waves; ++w) {
             const int t = red[w];
             red[w] = s;
             s += t;
         }
-        red[BKV_TPB / 64] = s;
+        red[waves] = s;
     }
     __syncthreads();
-    *total = red[BKV_TPB / 64];
+    *total = red[waves];
     return red[wave] + x - v;
 }
 
@@ -73,8 +74,8 @@ __device__ __forceinline__ int bkv_find(const int* off, int n, int k) {
 }
 
 // Takes the `want` lowest free pages (want <= free pages) into v.fresh,
-// ascending, and marks them used. Words from *hint on are searched, 1024 a
-// round; the caller has checked that enough are free.
+// ascending, and marks them used. Words from the hint on are searched, one a
+// thread and round; the caller has checked that enough are free.
 __device__ void bkv_take(const BkvView& v, int want, int* red) {
     const int words = (v.n_page + 31) / 32;
     int base = v.meta[BKV_HINT], got = 0, last = base;
@@ -94,7 +95,7 @@ __device__ void bkv_take(const BkvView& v, int want, int* red) {
         if (taken) v.used[w] |= taken;
         got += total;
         last = base;
-        base += BKV_TPB;
+        base += (int)blockDim.x;
     }
     __syncthreads();
     // every word before the last round's first is full now
@@ -150,7 +151,8 @@ __global__ __launch_bounds__(BKV_TPB) void vk_bkv_step(BkvView v, int n, int n_r
                                                        const int* __restrict__ counts) {
     __shared__ int red[BKV_TPB / 64 + 1];
     __shared__ int off[BKV_TPB];   // prefix of pages taken, then of write entries
-    __shared__ int s_start[BKV_TPB], s_seq[BKV_TPB];
+    __shared__ int s_start[BKV_TPB];
+    __shared__ BkvItem s_item[BKV_TPB];
     __shared__ int s_bad, s_rows;
     const int i = threadIdx.x;
     if (i == 0) {
@@ -179,13 +181,15 @@ __global__ __launch_bounds__(BKV_TPB) void vk_bkv_step(BkvView v, int n, int n_r
     if (i < bad && ok && need > 0 && at + need > free_pages) atomicMin(&s_bad, i);
     __syncthreads();
     const int done = s_bad;
-    if (i >= done) need = 0;
-    at = bkv_scan(need, red, &total);
+    if (done < bad) {  // some item found too few pages: those before it only
+        if (i >= done) need = 0;
+        at = bkv_scan(need, red, &total);
+    }
     off[i] = at;
     s_start[i] = b0;
-    s_seq[i] = seq;
+    s_item[i] = BkvItem{seq, start, cnt, row0};
     __syncthreads();
-    bkv_take(v, total, red);
+    if (total) bkv_take(v, total, red);
     // pages that a taken-back sequence held from its new start on
     if (i < done) {
         for (int b = b0; b < len / v.bs; ++b) {
@@ -194,10 +198,10 @@ __global__ __launch_bounds__(BKV_TPB) void vk_bkv_step(BkvView v, int n, int n_r
         }
     }
     __syncthreads();
-    for (int k = i; k < total; k += BKV_TPB) {
+    for (int k = i; k < total; k += (int)blockDim.x) {
         const int it = bkv_find(off, done, k);
         const int page = v.fresh[k];
-        v.table[(size_t)s_seq[it] * v.max_blocks + s_start[it] + (k - off[it])] = page;
+        v.table[(size_t)s_item[it].seq * v.max_blocks + s_start[it] + (k - off[it])] = page;
         v.refs[page] = 1;
     }
     __syncthreads();
@@ -205,15 +209,9 @@ __global__ __launch_bounds__(BKV_TPB) void vk_bkv_step(BkvView v, int n, int n_r
         const int end = start + cnt, nb = (end + v.bs - 1) / v.bs;
         v.len[seq] = end;
         v.floor_[seq] = max(fl, (nb - 2) * v.bs);
-        BkvItem it;
-        it.seq = seq;
-        it.start = start;
-        it.count = cnt;
-        it.row0 = row0;
-        v.step[i] = it;
-    } else {
-        v.step[i] = BkvItem{0, 0, 0, 0};  // no rows
     }
+    for (int k = i; k < kBkvMaxItems; k += (int)blockDim.x)
+        v.step[k] = k < done ? s_item[k] : BkvItem{0, 0, 0, 0};  // no rows beyond the items done
     // the write's entries: every block that an item's rows reach
     const int nblk = i < done && cnt > 0 ? (start + cnt - 1) / v.bs - b0 + 1 : 0;
     int n_work;
@@ -222,9 +220,17 @@ __global__ __launch_bounds__(BKV_TPB) void vk_bkv_step(BkvView v, int n, int n_r
     if (i < done) atomicMax(&s_rows, row0 + cnt);  // rows of the items done
     __syncthreads();
     n_work = min(n_work, v.max_work);
-    for (int k = i; k < n_work; k += BKV_TPB) {
+    for (int k = i; k < n_work; k += (int)blockDim.x) {
         const int it = bkv_find(off, done, k);
-        v.work[k] = make_int2(it, s_start[it] + (k - off[it]));
+        const BkvItem m = s_item[it];
+        BkvWork e;
+        e.seq = m.seq;
+        e.start = m.start;
+        e.end = m.start + m.count;
+        e.row0 = m.row0;
+        e.block = s_start[it] + (k - off[it]);
+        e.page = (e.block + 1) * v.bs <= e.end ? v.table[(size_t)m.seq * v.max_blocks + e.block] : -1;
+        v.work[k] = e;
     }
     if (i == 0) {
         atomicSub(&v.meta[BKV_FREE], total);
@@ -272,105 +278,167 @@ __device__ __forceinline__ float* bkv_ring(const BkvView& v, int layer, int seq,
     return v.ring + ((((size_t)layer * v.n_seq + seq) * 2 + side) * v.n_head + head) * (size_t)(2 * v.bs) * v.hd;
 }
 
-// One (item, block) entry, head and side: rounds the block if the step fills
-// it, and (the entry of the item's first block only) puts the rows of the
-// item's last two blocks into the ring. Only that workgroup reads ring rows
-// (those of the first block that earlier steps brought), before it writes any,
-// so no two workgroups meet there.
-template <int CODEC>
-__global__ __launch_bounds__(256) void vk_bkv_write(BkvView v, int layer, const float* __restrict__ k,
+// One wave for each block that the step reaches, head and side. If the step
+// fills the block, the wave holds it in registers (NT pieces of 16 tokens by 64
+// values, 16 values a lane, in the order that the pool stores them: a lane's 16
+// bytes of a piece are its own), finds its largest magnitude and stores it
+// rounded: one read, one write, no LDS. The wave of the item's first block also
+// puts the rows of the item's last two blocks into the ring; it alone reads ring
+// rows (those that earlier steps brought), before it writes any, so no two waves
+// meet there. Bound by memory: 5 bytes a value.
+template <int CODEC, int NT>
+__global__ __launch_bounds__(256) void vk_bkv_write(BkvView v, int layer, unsigned wg0, const float* __restrict__ k,
                                                     const float* __restrict__ vv) {
-    extern __shared__ float tile[];  // [bs][hd]
-    __shared__ float red[4];
-    if ((int)blockIdx.x >= v.meta[BKV_WORK_N]) return;
-    const int2 e = v.work[blockIdx.x];
-    const BkvItem it = v.step[e.x];
-    const int head = blockIdx.y, side = blockIdx.z, hd = v.hd, bs = v.bs, block = e.y;
-    const float* in = (side ? vv : k) + (size_t)it.row0 * v.n_head * hd + (size_t)head * hd;
-    float* ring = bkv_ring(v, layer, it.seq, side, head);
-    const int end = it.start + it.count;
-    const bool full = (block + 1) * bs <= end;
-    if (full) {
+    const int n_work = v.meta[BKV_WORK_N], hs = 2 * v.n_head;
+    const long long unit = ((long long)wg0 + blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int entry = __builtin_amdgcn_readfirstlane((int)(unit / hs));
+    if (entry >= n_work) return;
+    const int sub = __builtin_amdgcn_readfirstlane((int)(unit - (long long)entry * hs));
+    const BkvWork e = v.work[entry];
+    const int side = sub & 1, head = sub >> 1, lane = threadIdx.x & 63, hd = v.hd, bs = v.bs;
+    const size_t rs = (size_t)v.n_head * hd;  // floats from row to row
+    const float* in = (side ? vv : k) + (size_t)e.row0 * rs + (size_t)head * hd;
+    float* ring = bkv_ring(v, layer, e.seq, side, head);
+    const int mask = 2 * bs - 1;
+    if (e.page >= 0) {
+        const int pieces = hd >> 6;  // of a tile
+        float x[NT][16];
+#pragma unroll
+        for (int p = 0; p < NT; ++p) {
+            const int t0 = e.block * bs + p / pieces * 16, d0 = p % pieces * 64;
+            if (side == 0) {  // token lane % 16, values 16 (lane / 16) ..
+                const int t = t0 + (lane & 15), d = d0 + (lane >> 4) * 16;
+                const float* r = t >= e.start ? in + (size_t)(t - e.start) * rs + d : ring + (size_t)(t & mask) * hd + d;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float4 y = *(const float4*)(r + 4 * j);
+                    x[p][4 * j] = y.x, x[p][4 * j + 1] = y.y, x[p][4 * j + 2] = y.z, x[p][4 * j + 3] = y.w;
+                }
+            } else {  // tokens 4 (lane / 16) .., values lane % 16 + 0, 16, 32, 48
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int t = t0 + (lane >> 4) * 4 + j, d = d0 + (lane & 15);
+                    const float* r =
+                        t >= e.start ? in + (size_t)(t - e.start) * rs + d : ring + (size_t)(t & mask) * hd + d;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[p][4 * i + j] = r[16 * i];
+                }
+            }
+        }
         float amax = 0.0f;
         bool odd = false;  // a value that is not finite
-        for (int x = threadIdx.x * 4; x < bs * hd; x += 1024) {
-            const int t = block * bs + x / hd, d = x % hd;
-            const float4 r = t >= it.start ? *(const float4*)(in + (size_t)(t - it.start) * v.n_head * hd + d)
-                                           : *(const float4*)(ring + (size_t)(t % (2 * bs)) * hd + d);
-            *(float4*)(tile + x) = r;
-            const float m = fmaxf(fmaxf(fabsf(r.x), fabsf(r.y)), fmaxf(fabsf(r.z), fabsf(r.w)));
-            amax = fmaxf(amax, m);
-            odd = odd || !(fabsf(r.x) < INFINITY) || !(fabsf(r.y) < INFINITY) || !(fabsf(r.z) < INFINITY) ||
-                  !(fabsf(r.w) < INFINITY);
-        }
-        if (odd) amax = INFINITY;
-        amax = vk_group_max<64>(amax);
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = amax;
-        __syncthreads();
-        amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+        for (int p = 0; p < NT; ++p)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float m = fabsf(x[p][i]);
+                amax = fmaxf(amax, m);
+                odd = odd || !(m < INFINITY);
+            }
+        amax = vk_group_max<64>(odd ? INFINITY : amax);
         const float top = CODEC == BKV_INT8 ? 127.0f : 448.0f;
         const bool holds = amax >= 0x1p-100f && amax < INFINITY;
         const float inv = holds ? top / amax : 0.0f;
         const float scale = holds ? amax / top : (amax < INFINITY ? 0.0f : __builtin_nanf(""));
-        const int page = v.table[(size_t)it.seq * v.max_blocks + block];
-        const size_t chunk = bkv_chunk(v, layer, page, head);
-        uint8_t* out = v.pool + chunk * 2 * bs * hd + (size_t)side * bs * hd;
-        if (threadIdx.x == 0) v.scales[chunk * 2 + side] = scale;
-        for (int x = threadIdx.x * 4; x < bs * hd; x += 1024) {  // x = byte offset: four consecutive bytes
-            const int ti = x / (16 * hd), r = x % (16 * hd), lane = (r >> 4) & 63, c = r >> 10, b = r & 15;
-            float y[4];
-            if (side == 0) {
-                const int t = ti * 16 + (lane & 15), d = c * 64 + (lane >> 4) * 16 + b;
-                for (int j = 0; j < 4; ++j) y[j] = tile[t * hd + d + j];
-            } else {
-                const int t = ti * 16 + (lane >> 4) * 4, d = c * 64 + (b >> 2) * 16 + (lane & 15);
-                for (int j = 0; j < 4; ++j) y[j] = tile[(t + j) * hd + d];
+        const size_t chunk = bkv_chunk(v, layer, e.page, head);
+        uint4* out = (uint4*)(v.pool + (chunk * 2 + side) * bs * hd);
+        if (lane == 0) v.scales[chunk * 2 + side] = scale;
+#pragma unroll
+        for (int p = 0; p < NT; ++p) {
+            uint32_t y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float z[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) z[i] = holds ? x[p][4 * j + i] * inv : 0.0f;
+                y[j] = bkv_encode4<CODEC>(z[0], z[1], z[2], z[3]);
             }
-            for (int j = 0; j < 4; ++j) y[j] = holds ? y[j] * inv : 0.0f;
-            *(uint32_t*)(out + x) = bkv_encode4<CODEC>(y[0], y[1], y[2], y[3]);
+            out[p * 64 + lane] = make_uint4(y[0], y[1], y[2], y[3]);
         }
     }
-    if (block != it.start / bs) return;
-    __syncthreads();
-    const int nb = (end + bs - 1) / bs, first = max(it.start, (nb - 2) * bs);
-    for (int x = threadIdx.x * 4; x < (end - first) * hd; x += 1024) {
-        const int t = first + x / hd, d = x % hd;
-        *(float4*)(ring + (size_t)(t % (2 * bs)) * hd + d) =
-            *(const float4*)(in + (size_t)(t - it.start) * v.n_head * hd + d);
+    if (e.block != e.start / bs) return;
+    const int nb = (e.end + bs - 1) / bs, first = max(e.start, (nb - 2) * bs), q4 = hd >> 2;
+    for (int g = lane; g < (e.end - first) * q4; g += 64) {
+        const int t = first + g / q4, d = g % q4 * 4;
+        *(float4*)(ring + (size_t)(t & mask) * hd + d) = *(const float4*)(in + (size_t)(t - e.start) * rs + d);
     }
 }
 
 // ---- read --------------------------------------------------------------------
 
-// Row r: the values held for (seqs[r], times[r]), zeros where nothing is held.
+// Row r: the values held for (seqs[r], times[r]), zeros where nothing is held. A
+// workgroup takes up to 16 rows: where each is comes once into LDS, then a
+// thread widens a row's 16-byte piece of K, or the row's byte of each of the 16
+// of a piece of V (whose other bytes are the rows beside it: in cache).
+constexpr int kReadRows = 16;
 template <int CODEC>
-__global__ __launch_bounds__(256) void vk_bkv_read(BkvView v, int layer, int n, const int* __restrict__ seqs,
+__device__ __forceinline__ float bkv_decode4(uint32_t w, int j) {  // byte j of a word, j a constant
+    if constexpr (CODEC == BKV_INT8) return (float)((w >> (8 * j)) & 255u) - 128.0f;
+    else return bkv_e4m3_f32(w >> (8 * j));
+}
+template <int CODEC>
+__global__ __launch_bounds__(256) void vk_bkv_read(BkvView v, int layer, int n, int per, const int* __restrict__ seqs,
                                                    const int* __restrict__ times, float* __restrict__ k,
                                                    float* __restrict__ vv) {
-    const int w4 = v.n_head * v.hd / 4;
-    const size_t total = (size_t)n * w4;
-    const int side = blockIdx.y;
-    float* out = side ? vv : k;
-    for (size_t g = (size_t)blockIdx.x * 256 + threadIdx.x; g < total; g += (size_t)gridDim.x * 256) {
-        const int r = (int)(g / w4), c = (int)(g % w4) * 4, head = c / v.hd, d = c % v.hd;
-        const int seq = seqs[r], t = times[r];
-        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if ((unsigned)seq < (unsigned)v.n_seq && t >= 0 && t < v.len[seq]) {
-            const int block = t / v.bs;
-            if (block < v.len[seq] / v.bs) {
-                const size_t chunk = bkv_chunk(v, layer, v.table[(size_t)seq * v.max_blocks + block], head);
-                const uint8_t* p = v.pool + chunk * 2 * v.bs * v.hd + (size_t)side * v.bs * v.hd +
-                                   (size_t)(t % v.bs / 16) * 16 * v.hd;
-                const float s = v.scales[chunk * 2 + side];
-                float q[4];
-                for (int j = 0; j < 4; ++j)
-                    q[j] = bkv_decode<CODEC>(p[side ? bkv_v_off(t & 15, d + j) : bkv_k_off(t & 15, d + j)]) * s;
-                y = make_float4(q[0], q[1], q[2], q[3]);
-            } else {
-                y = *(const float4*)(bkv_ring(v, layer, seq, side, head) + (size_t)(t % (2 * v.bs)) * v.hd + d);
-            }
+    __shared__ int s_page[kReadRows], s_t[kReadRows], s_seq[kReadRows];  // page -1: the ring, -2: nothing
+    const int r0 = blockIdx.x * per, rows = min(per, n - r0), hd = v.hd, bs = v.bs, w = v.n_head * hd;
+    if ((int)threadIdx.x < rows) {
+        const int seq = seqs[r0 + threadIdx.x], t = times[r0 + threadIdx.x];
+        int page = -2;
+        if ((unsigned)seq < (unsigned)v.n_seq && t >= 0) {
+            const int len = v.len[seq], block = t / bs;
+            if (t < len) page = block < len / bs ? v.table[(size_t)seq * v.max_blocks + block] : -1;
         }
-        *(float4*)(out + g * 4) = y;
+        s_page[threadIdx.x] = page;
+        s_t[threadIdx.x] = t;
+        s_seq[threadIdx.x] = seq;
+    }
+    __syncthreads();
+    const int kp = w >> 4, vp = w >> 2;  // pieces of a row: K 16 values, V 4
+    for (int g = threadIdx.x; g < rows * kp; g += 256) {
+        const int r = g / kp, c = (g - r * kp) * 16, head = c / hd, d = c % hd, page = s_page[r], t = s_t[r];
+        float4 y[4] = {};
+        if (page >= 0) {
+            const size_t chunk = bkv_chunk(v, layer, page, head);
+            const uint4 b = *(const uint4*)(v.pool + chunk * 2 * bs * hd + (size_t)((t & (bs - 1)) >> 4) * 16 * hd +
+                                            bkv_k_off(t & 15, d));
+            const float s = v.scales[chunk * 2];
+            const uint32_t q[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                y[j] = make_float4(bkv_decode4<CODEC>(q[j], 0) * s, bkv_decode4<CODEC>(q[j], 1) * s,
+                                   bkv_decode4<CODEC>(q[j], 2) * s, bkv_decode4<CODEC>(q[j], 3) * s);
+        } else if (page == -1) {
+            const float* p = bkv_ring(v, layer, s_seq[r], 0, head) + (size_t)(t & (2 * bs - 1)) * hd + d;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = *(const float4*)(p + 4 * j);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *(float4*)(k + (size_t)(r0 + r) * w + c + 4 * j) = y[j];
+    }
+    for (int g = threadIdx.x; g < rows * vp; g += 256) {
+        // values d, d + 16, d + 32, d + 48 of a 64-wide piece
+        const int r = g / vp, i = g - r * vp, c = (i >> 4) * 64, head = c / hd, d = c % hd + (i & 15);
+        const int page = s_page[r], t = s_t[r];
+        float y[4] = {};
+        if (page >= 0) {
+            const size_t chunk = bkv_chunk(v, layer, page, head);
+            const uint4 b = *(const uint4*)(v.pool + (chunk * 2 + 1) * bs * hd +
+                                            (size_t)((t & (bs - 1)) >> 4) * 16 * hd + (bkv_v_off(t & 15, d) & ~15));
+            const float s = v.scales[chunk * 2 + 1];
+            const int sh = (t & 3) * 8;
+            y[0] = bkv_decode4<CODEC>(b.x >> sh, 0) * s;
+            y[1] = bkv_decode4<CODEC>(b.y >> sh, 0) * s;
+            y[2] = bkv_decode4<CODEC>(b.z >> sh, 0) * s;
+            y[3] = bkv_decode4<CODEC>(b.w >> sh, 0) * s;
+        } else if (page == -1) {
+            const float* p = bkv_ring(v, layer, s_seq[r], 1, head) + (size_t)(t & (2 * bs - 1)) * hd + d;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = p[16 * j];
+        }
+        float* o = vv + (size_t)(r0 + r) * w + c + (i & 15);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[16 * j] = y[j];
     }
 }
 
@@ -419,26 +487,35 @@ __global__ __launch_bounds__(BKV_TPB) void vk_bkv_fork_plan(BkvView v, int n, co
     }
 }
 
-// blockIdx.x: item; blockIdx.y < n_layer: that layer's ring rows; else the table row.
-__global__ __launch_bounds__(256) void vk_bkv_fork_rows(BkvView v) {
-    if ((int)blockIdx.x >= v.meta[BKV_PLAN_N]) return;
-    const BkvItem it = v.plan[blockIdx.x];
-    const int layer = blockIdx.y;
-    if (layer == v.n_layer) {
-        for (int b = threadIdx.x; b < it.count / v.bs; b += 256) {
-            const int page = v.table[(size_t)it.seq * v.max_blocks + b];
-            v.table[(size_t)it.start * v.max_blocks + b] = page;
-            atomicAdd(&v.refs[page], 1);
-        }
+// Rows row0 .. count - 1 of the items' sources into the rings of their
+// destinations: one wave for each item, layer, head and side.
+__device__ __forceinline__ void bkv_move_rows(const BkvView& dv, const BkvView& sv, long long unit) {
+    const int hs = 2 * dv.n_head, per = dv.n_layer * hs, lane = threadIdx.x & 63;
+    const int i = (int)(unit / per), rest = (int)(unit - (long long)i * per), layer = rest / hs, h = rest - layer * hs;
+    if (i >= dv.meta[BKV_PLAN_N]) return;
+    const BkvItem it = dv.plan[i];
+    const float* src = bkv_ring(sv, layer, it.seq, 0, 0) + (size_t)h * 2 * sv.bs * sv.hd;
+    float* dst = bkv_ring(dv, layer, it.start, 0, 0) + (size_t)h * 2 * dv.bs * dv.hd;
+    const int mask = 2 * dv.bs - 1, q4 = dv.hd >> 2;
+    for (int g = lane; g < (it.count - it.row0) * q4; g += 64) {
+        const size_t o = (size_t)((it.row0 + g / q4) & mask) * dv.hd + g % q4 * 4;
+        *(float4*)(dst + o) = *(const float4*)(src + o);
+    }
+}
+
+// Workgroups below `rows`: ring rows; the others: an item's table row each.
+__global__ __launch_bounds__(256) void vk_bkv_fork_rows(BkvView v, int rows) {
+    if ((int)blockIdx.x < rows) {
+        bkv_move_rows(v, v, (long long)blockIdx.x * 4 + (threadIdx.x >> 6));
         return;
     }
-    const int per = (it.count - it.row0) * v.hd, hs = 2 * v.n_head;
-    const float* src = bkv_ring(v, layer, it.seq, 0, 0);
-    float* dst = bkv_ring(v, layer, it.start, 0, 0);
-    for (int x = threadIdx.x * 4; x < per * hs; x += 1024) {
-        const int h = x / per, t = it.row0 + x % per / v.hd, d = x % v.hd;
-        const size_t o = ((size_t)h * 2 * v.bs + t % (2 * v.bs)) * v.hd + d;
-        *(float4*)(dst + o) = *(const float4*)(src + o);
+    const int i = (int)blockIdx.x - rows;
+    if (i >= v.meta[BKV_PLAN_N]) return;
+    const BkvItem it = v.plan[i];
+    for (int b = threadIdx.x; b < it.count / v.bs; b += 256) {
+        const int page = v.table[(size_t)it.seq * v.max_blocks + b];
+        v.table[(size_t)it.start * v.max_blocks + b] = page;
+        atomicAdd(&v.refs[page], 1);
     }
 }
 
@@ -463,7 +540,7 @@ __global__ __launch_bounds__(BKV_TPB) void vk_bkv_free_plan(BkvView v, int n, co
             v.floor_[seq] = 0;
         }
     }
-    v.step[i] = BkvItem{0, 0, 0, 0};
+    for (int k = i; k < kBkvMaxItems; k += (int)blockDim.x) v.step[k] = BkvItem{0, 0, 0, 0};
     if (i == 0) {
         v.meta[BKV_STATUS] = done == n ? VOKRA_HIP_OK : VOKRA_HIP_ERROR_INVALID_ARGUMENT;
         v.meta[BKV_DONE] = done;
@@ -510,7 +587,7 @@ __global__ __launch_bounds__(BKV_TPB) void vk_bkv_copy_plan(BkvView dv, BkvView 
     s_dst[i] = dst;
     __syncthreads();
     bkv_take(dv, total, red);
-    for (int k = i; k < total; k += BKV_TPB) {
+    for (int k = i; k < total; k += (int)blockDim.x) {
         const int it = bkv_find(off, done, k), b = k - off[it], page = dv.fresh[k];
         dv.table[(size_t)s_dst[it] * dv.max_blocks + b] = page;
         dv.refs[page] = 1;
@@ -555,16 +632,7 @@ __global__ __launch_bounds__(256) void vk_bkv_move_pages(BkvView dv, BkvView sv)
 
 // The ring rows of copied sequences (all that a step may still go back to).
 __global__ __launch_bounds__(256) void vk_bkv_copy_rows(BkvView dv, BkvView sv) {
-    if ((int)blockIdx.x >= dv.meta[BKV_PLAN_N]) return;
-    const BkvItem it = dv.plan[blockIdx.x];
-    const int layer = blockIdx.y, per = (it.count - it.row0) * dv.hd, hs = 2 * dv.n_head;
-    const float* src = bkv_ring(sv, layer, it.seq, 0, 0);
-    float* dst = bkv_ring(dv, layer, it.start, 0, 0);
-    for (int x = threadIdx.x * 4; x < per * hs; x += 1024) {
-        const int h = x / per, t = it.row0 + x % per / dv.hd, d = x % dv.hd;
-        const size_t o = ((size_t)h * 2 * dv.bs + t % (2 * dv.bs)) * dv.hd + d;
-        *(float4*)(dst + o) = *(const float4*)(src + o);
-    }
+    bkv_move_rows(dv, sv, (long long)blockIdx.x * 4 + (threadIdx.x >> 6));
 }
 
 // u pages are in use: the k-th one at or above u moves to the k-th free one
@@ -642,44 +710,79 @@ hipError_t launch_bkv_reset(hipStream_t s, const BkvView& v, bool clear_data) {
     return hipGetLastError();
 }
 
+// Threads of a planning kernel for n items: four waves keep its barriers short.
+static unsigned plan_threads(int n) { return n <= 256 ? 256 : BKV_TPB; }
+
 hipError_t launch_bkv_step(hipStream_t s, const BkvView& v, int n, int n_rows, int max_count, const int* seqs,
                            const int* starts, const int* counts) {
-    hipLaunchKernelGGL(vk_bkv_step, dim3(1), dim3(BKV_TPB), 0, s, v, n, n_rows, max_count, seqs, starts, counts);
+    hipLaunchKernelGGL(vk_bkv_step, dim3(1), dim3(plan_threads(n)), 0, s, v, n, n_rows, max_count, seqs, starts,
+                       counts);
     return hipGetLastError();
+}
+
+// Workgroups of one launch: a grid holds fewer than 2^32 threads.
+constexpr long long kMaxWgs = 1 << 23;
+
+template <int CODEC, int NT>
+static void go_write(hipStream_t s, const BkvView& v, int layer, long long wgs, const float* k, const float* vv) {
+    for (long long w = 0; w < wgs; w += kMaxWgs)
+        hipLaunchKernelGGL((vk_bkv_write<CODEC, NT>), dim3((unsigned)std::min(kMaxWgs, wgs - w)), dim3(256), 0, s, v,
+                           layer, (unsigned)w, k, vv);
+}
+template <int CODEC>
+static void go_write(hipStream_t s, const BkvView& v, int layer, long long wgs, const float* k, const float* vv) {
+    switch (v.bs / 16 * (v.hd / 64)) {
+    case 1: go_write<CODEC, 1>(s, v, layer, wgs, k, vv); break;
+    case 2: go_write<CODEC, 2>(s, v, layer, wgs, k, vv); break;
+    case 4: go_write<CODEC, 4>(s, v, layer, wgs, k, vv); break;
+    default: go_write<CODEC, 8>(s, v, layer, wgs, k, vv); break;
+    }
 }
 
 hipError_t launch_bkv_write(hipStream_t s, const BkvView& v, int layer, int work_bound, const float* k,
                             const float* vv) {
     if (work_bound == 0) return hipSuccess;
-    const dim3 grid((unsigned)work_bound, (unsigned)v.n_head, 2);
-    const size_t lds = (size_t)v.bs * v.hd * sizeof(float);
-    if (v.codec == BKV_INT8)
-        hipLaunchKernelGGL(vk_bkv_write<BKV_INT8>, grid, dim3(256), lds, s, v, layer, k, vv);
-    else
-        hipLaunchKernelGGL(vk_bkv_write<BKV_E4M3>, grid, dim3(256), lds, s, v, layer, k, vv);
+    const long long wgs = ((long long)work_bound * 2 * v.n_head + 3) / 4;
+    if (v.codec == BKV_INT8) go_write<BKV_INT8>(s, v, layer, wgs, k, vv);
+    else go_write<BKV_E4M3>(s, v, layer, wgs, k, vv);
     return hipGetLastError();
 }
 
 hipError_t launch_bkv_read(hipStream_t s, const BkvView& v, int layer, int n, const int* seqs, const int* times,
                            float* k, float* vv) {
-    if (n == 0) return hipSuccess;
-    const size_t wgs = ((size_t)n * v.n_head * v.hd / 4 + 255) / 256;
-    const dim3 grid((unsigned)std::min<size_t>(wgs, 8192), 2);
-    if (v.codec == BKV_INT8)
-        hipLaunchKernelGGL(vk_bkv_read<BKV_INT8>, grid, dim3(256), 0, s, v, layer, n, seqs, times, k, vv);
-    else
-        hipLaunchKernelGGL(vk_bkv_read<BKV_E4M3>, grid, dim3(256), 0, s, v, layer, n, seqs, times, k, vv);
+    // rows a workgroup: 16 once that leaves four workgroups a CU
+    const int per = std::min(std::max(n / 1024, 1), kReadRows);
+    const size_t w = (size_t)v.n_head * v.hd;
+    for (long long r = 0; r < n; r += kMaxWgs * per) {
+        const int now = (int)std::min<long long>(kMaxWgs * per, n - r);
+        const dim3 grid((unsigned)((now + per - 1) / per));
+        if (v.codec == BKV_INT8)
+            hipLaunchKernelGGL(vk_bkv_read<BKV_INT8>, grid, dim3(256), 0, s, v, layer, now, per, seqs + r, times + r,
+                               k + r * w, vv + r * w);
+        else
+            hipLaunchKernelGGL(vk_bkv_read<BKV_E4M3>, grid, dim3(256), 0, s, v, layer, now, per, seqs + r, times + r,
+                               k + r * w, vv + r * w);
+    }
     return hipGetLastError();
 }
 
+// Workgroups of the ring rows of n items, four waves each. The rings of a cache
+// that fits the card are fewer than a launch has threads for.
+static unsigned row_grid(const BkvView& v, int n) {
+    return (unsigned)(((long long)n * v.n_layer * 2 * v.n_head + 3) / 4);
+}
+
 hipError_t launch_bkv_fork(hipStream_t s, const BkvView& v, int n, const int* src, const int* dst) {
-    hipLaunchKernelGGL(vk_bkv_fork_plan, dim3(1), dim3(BKV_TPB), 0, s, v, n, src, dst);
-    if (n) hipLaunchKernelGGL(vk_bkv_fork_rows, dim3((unsigned)n, (unsigned)v.n_layer + 1), dim3(256), 0, s, v);
+    hipLaunchKernelGGL(vk_bkv_fork_plan, dim3(1), dim3(plan_threads(n)), 0, s, v, n, src, dst);
+    if (n) {
+        const unsigned rows = row_grid(v, n);
+        hipLaunchKernelGGL(vk_bkv_fork_rows, dim3(rows + (unsigned)n), dim3(256), 0, s, v, (int)rows);
+    }
     return hipGetLastError();
 }
 
 hipError_t launch_bkv_free(hipStream_t s, const BkvView& v, int n, const int* seqs) {
-    hipLaunchKernelGGL(vk_bkv_free_plan, dim3(1), dim3(BKV_TPB), 0, s, v, n, seqs);
+    hipLaunchKernelGGL(vk_bkv_free_plan, dim3(1), dim3(plan_threads(n)), 0, s, v, n, seqs);
     if (n) {
         const unsigned y = (unsigned)std::min((v.max_blocks + 255) / 256, 64);
         hipLaunchKernelGGL(vk_bkv_free_pages, dim3((unsigned)n, y), dim3(256), 0, s, v);
@@ -695,7 +798,7 @@ hipError_t launch_bkv_copy(hipStream_t s, const BkvView& dv, const BkvView& sv, 
     hipLaunchKernelGGL(vk_bkv_copy_plan, dim3(1), dim3(BKV_TPB), 0, s, dv, sv, (int)(dv.meta == sv.meta), n, src, dst);
     if (n) {
         hipLaunchKernelGGL(vk_bkv_move_pages, dim3(kMoveGrid), dim3(256), 0, s, dv, sv);
-        hipLaunchKernelGGL(vk_bkv_copy_rows, dim3((unsigned)n, (unsigned)dv.n_layer), dim3(256), 0, s, dv, sv);
+        hipLaunchKernelGGL(vk_bkv_copy_rows, dim3(row_grid(dv, n)), dim3(256), 0, s, dv, sv);
     }
     return hipGetLastError();
 }

@@ -112,7 +112,7 @@ void reserve(hipError_t* e, T** p, size_t n) {
     if (*e == hipSuccess) *e = hipMalloc((void**)p, (n * sizeof(T) + 31) / 16 * 16);
 }
 
-// The (item, block) entries that a step of n items and n_rows rows can have.
+// The blocks that a step of n items and n_rows rows can reach.
 size_t work_bound(const vokra_hip_bkv* kv, size_t n, size_t n_rows) {
     const size_t bs = (size_t)kv->v.bs;
     return std::min(n_rows, n + (n_rows + n * (bs - 2)) / bs);

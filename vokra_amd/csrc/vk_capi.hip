@@ -19,6 +19,7 @@
 
 #include "../../include/vokra_hip.h"
 #include "vk_launch.h"
+#include "vk_step.h"
 
 namespace {
 
@@ -154,7 +155,7 @@ struct vokra_hip_ctx {
     DevBuf fe_win, fe_tw, fe_fb, fe_part, cv_col;
     int fe_mels = 0;
     DevBuf bk_part;  // partial results of the block caches' attention
-    DevBuf ru_part;  // per-slice (max, index) partials of the logits rules
+    DevBuf ru_part;  // rows' maxima and counters of the logits rules, zero between calls
     DevBuf lg_part;  // per-workgroup (max, index) partials of the fused logits argmax
     // RoPE frequency table of the last (rope_base, head_dim) the _dev entry saw
     DevBuf rope_theta, rope_pos;
@@ -606,7 +607,14 @@ int ctx_bkv_part(vokra_hip_ctx* c, size_t bytes, void** p) {
     return VOKRA_HIP_OK;
 }
 int ctx_rules_part(vokra_hip_ctx* c, size_t bytes, void** p) {
-    VK_TRY(c->ru_part.ensure(bytes), "hipMalloc(logits rules)");
+    if (!c->ru_part.p) {
+        VK_TRY(c->ru_part.ensure(bytes), "hipMalloc(logits rules)");
+        hipError_t e = launch_rules_clear(c->stream, c->ru_part.p);
+        if (e != hipSuccess) {
+            c->ru_part.release();
+            return hip_fail(e, "launch(vk_rules_clear)");
+        }
+    }
     *p = c->ru_part.p;
     return VOKRA_HIP_OK;
 }

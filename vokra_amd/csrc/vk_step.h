@@ -18,8 +18,9 @@ struct RopeArgs {
     int units, head_lanes;  // set by the launcher
 };
 
-// Partial (value, index) pairs of the greedy choice that one launch may leave.
-constexpr int kRulesParts = 1 << 17;
+// A context's workspace of the greedy choice: rows' maxima, then their counters.
+constexpr int kRulesRows = 65536;
+constexpr size_t kRulesPartBytes = (size_t)kRulesRows * 12;
 
 struct RulesArgs {
     const float* logits;
@@ -30,14 +31,14 @@ struct RulesArgs {
     const float *repetition, *presence, *frequency, *bias;
     const uint32_t* mask;
     size_t mask_stride;
-    float2* part;
+    unsigned long long* best;  // zero between calls
+    unsigned* done;            // zero between calls
     int rows, vocab, n_hist, n_bias;
 };
 
 namespace vk {
 // units and head_lanes are filled in here
 hipError_t launch_rope_turn(hipStream_t s, RopeArgs a, bool pairs);
-// workgroups a row (partials a row)
-int rules_slices(int vocab);
+hipError_t launch_rules_clear(hipStream_t s, void* part);
 hipError_t launch_rules(hipStream_t s, const RulesArgs& a);
 }  // namespace vk

@@ -288,24 +288,21 @@ int vokra_hip_logits_rules_dev(vokra_hip_ctx_t* c, size_t rows, size_t vocab, si
     a.mask_stride = rules->mask_stride;
     if (d_next) {
         void* p = nullptr;
-        ST_ST(vk::ctx_rules_part(c, kRulesParts * sizeof(float2), &p));
-        a.part = (float2*)p;
+        ST_ST(vk::ctx_rules_part(c, kRulesPartBytes, &p));
+        a.best = (unsigned long long*)p;
+        a.done = (unsigned*)(a.best + kRulesRows);
     }
-    // rows whose partial choices fit the workspace, at a time
-    const size_t step = d_next ? (size_t)kRulesParts / (size_t)vk::rules_slices(a.vocab) : rows;
-    for (size_t r = 0; r < rows; r += step) {
-        a.rows = (int)std::min(step, rows - r);
-        a.logits = d_logits + r * stride;
-        a.out = d_out ? d_out + r * stride : nullptr;
-        a.next = d_next ? d_next + r : nullptr;
-        a.hist_off = rules->n_hist ? rules->hist_offsets + r : nullptr;
-        a.bias_off = rules->n_bias ? rules->bias_offsets + r : nullptr;
-        a.repetition = rules->repetition ? rules->repetition + r : nullptr;
-        a.presence = rules->presence ? rules->presence + r : nullptr;
-        a.frequency = rules->frequency ? rules->frequency + r : nullptr;
-        a.mask = rules->mask ? rules->mask + r * rules->mask_stride : nullptr;
-        ST_TRY(vk::launch_rules(vk::ctx_stream(c), a), "launch(vk_rules)");
-    }
+    a.rows = (int)rows;
+    a.logits = d_logits;
+    a.out = d_out;
+    a.next = d_next;
+    a.hist_off = rules->n_hist ? rules->hist_offsets : nullptr;
+    a.bias_off = rules->n_bias ? rules->bias_offsets : nullptr;
+    a.repetition = rules->repetition;
+    a.presence = rules->presence;
+    a.frequency = rules->frequency;
+    a.mask = rules->mask;
+    ST_TRY(vk::launch_rules(vk::ctx_stream(c), a), "launch(vk_rules)");
     return VOKRA_HIP_OK;
 }
 
