@@ -68,12 +68,13 @@ constexpr int BKV_INT8 = 0, BKV_E4M3 = 1;
 // Byte of element (token t of the tile, d) in a 16-token K or V tile: the
 // order in which the attention's matrix instructions take them, 16 bytes a
 // lane. K: lane (d % 64 / 16) * 16 + t holds d % 16 = 0 .. 15 of chunk d / 64.
-// V: lane (t / 4) * 16 + d % 16 holds tokens t % 4 of four 16-wide d tiles.
+// V: lane (t / 4) * 16 + d % 64 / 4 holds d % 4 = 0 .. 3 (a word each: row
+// d % 64 / 4 of four products) for tokens t % 4 (a byte each).
 __host__ __device__ inline int bkv_k_off(int t, int d) {
     return ((d >> 6) * 64 + ((d >> 4) & 3) * 16 + t) * 16 + (d & 15);
 }
 __host__ __device__ inline int bkv_v_off(int t, int d) {
-    return ((d >> 6) * 64 + (t >> 2) * 16 + (d & 15)) * 16 + ((d >> 4) & 3) * 4 + (t & 3);
+    return ((d >> 6) * 64 + (t >> 2) * 16 + ((d >> 2) & 15)) * 16 + (d & 3) * 4 + (t & 3);
 }
 
 namespace vk {

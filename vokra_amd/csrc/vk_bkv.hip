@@ -314,14 +314,13 @@ __global__ __launch_bounds__(256) void vk_bkv_write(BkvView v, int layer, unsign
                     const float4 y = *(const float4*)(r + 4 * j);
                     x[p][4 * j] = y.x, x[p][4 * j + 1] = y.y, x[p][4 * j + 2] = y.z, x[p][4 * j + 3] = y.w;
                 }
-            } else {  // tokens 4 (lane / 16) .., values lane % 16 + 0, 16, 32, 48
+            } else {  // tokens 4 (lane / 16) .., values 4 (lane % 16) ..
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int t = t0 + (lane >> 4) * 4 + j, d = d0 + (lane & 15);
-                    const float* r =
-                        t >= e.start ? in + (size_t)(t - e.start) * rs + d : ring + (size_t)(t & mask) * hd + d;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[p][4 * i + j] = r[16 * i];
+                    const int t = t0 + (lane >> 4) * 4 + j, d = d0 + (lane & 15) * 4;
+                    const float4 y = *(const float4*)(t >= e.start ? in + (size_t)(t - e.start) * rs + d
+                                                                   : ring + (size_t)(t & mask) * hd + d);
+                    x[p][j] = y.x, x[p][4 + j] = y.y, x[p][8 + j] = y.z, x[p][12 + j] = y.w;
                 }
             }
         }
@@ -368,13 +367,14 @@ __global__ __launch_bounds__(256) void vk_bkv_write(BkvView v, int layer, unsign
 
 // Row r: the values held for (seqs[r], times[r]), zeros where nothing is held. A
 // workgroup takes up to 16 rows: where each is comes once into LDS, then a
-// thread widens a row's 16-byte piece of K, or the row's byte of each of the 16
-// of a piece of V (whose other bytes are the rows beside it: in cache).
+// thread widens four values of each of its rows at a time (V: the row's byte of
+// each word of a 16-byte piece, whose other bytes are the rows beside it), all
+// rows' loads in flight. Bound by memory: 5 bytes a value.
 constexpr int kReadRows = 16;
 template <int CODEC>
-__device__ __forceinline__ float bkv_decode4(uint32_t w, int j) {  // byte j of a word, j a constant
-    if constexpr (CODEC == BKV_INT8) return (float)((w >> (8 * j)) & 255u) - 128.0f;
-    else return bkv_e4m3_f32(w >> (8 * j));
+__device__ __forceinline__ float bkv_decode1(uint32_t w) {  // the low byte of a word
+    if constexpr (CODEC == BKV_INT8) return (float)(w & 255u) - 128.0f;
+    else return bkv_e4m3_f32(w);
 }
 template <int CODEC>
 __global__ __launch_bounds__(256) void vk_bkv_read(BkvView v, int layer, int n, int per, const int* __restrict__ seqs,
@@ -394,51 +394,34 @@ __global__ __launch_bounds__(256) void vk_bkv_read(BkvView v, int layer, int n, 
         s_seq[threadIdx.x] = seq;
     }
     __syncthreads();
-    const int kp = w >> 4, vp = w >> 2;  // pieces of a row: K 16 values, V 4
-    for (int g = threadIdx.x; g < rows * kp; g += 256) {
-        const int r = g / kp, c = (g - r * kp) * 16, head = c / hd, d = c % hd, page = s_page[r], t = s_t[r];
-        float4 y[4] = {};
-        if (page >= 0) {
-            const size_t chunk = bkv_chunk(v, layer, page, head);
-            const uint4 b = *(const uint4*)(v.pool + chunk * 2 * bs * hd + (size_t)((t & (bs - 1)) >> 4) * 16 * hd +
-                                            bkv_k_off(t & 15, d));
-            const float s = v.scales[chunk * 2];
-            const uint32_t q[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                y[j] = make_float4(bkv_decode4<CODEC>(q[j], 0) * s, bkv_decode4<CODEC>(q[j], 1) * s,
-                                   bkv_decode4<CODEC>(q[j], 2) * s, bkv_decode4<CODEC>(q[j], 3) * s);
-        } else if (page == -1) {
-            const float* p = bkv_ring(v, layer, s_seq[r], 0, head) + (size_t)(t & (2 * bs - 1)) * hd + d;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = *(const float4*)(p + 4 * j);
+    const int w4 = w >> 2, hd_log = 31 - __clz(hd), at_once = w4 < 256 ? 256 / w4 : 1;
+    const int first = at_once > 1 ? (int)threadIdx.x / w4 : 0, c0 = at_once > 1 ? (int)threadIdx.x % w4 : (int)threadIdx.x;
+    if (first >= at_once) return;
+    for (int c = c0; c < w4; c += 256) {
+        const int head = c * 4 >> hd_log, d = c * 4 & (hd - 1);
+#pragma unroll 4
+        for (int r = first; r < rows; r += at_once) {
+            const int page = s_page[r], t = s_t[r];
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f), z = y;
+            if (page >= 0) {
+                const size_t chunk = bkv_chunk(v, layer, page, head);
+                const uint8_t* p = v.pool + chunk * 2 * bs * hd + ((t & (bs - 1)) >> 4) * 16 * hd;
+                const uint32_t b = *(const uint32_t*)(p + bkv_k_off(t & 15, d));
+                const uint4 q = *(const uint4*)(p + bs * hd + (bkv_v_off(t & 15, d) & ~15));
+                const float2 s = *(const float2*)(v.scales + chunk * 2);
+                const int sh = (t & 3) * 8;
+                y = make_float4(bkv_decode1<CODEC>(b) * s.x, bkv_decode1<CODEC>(b >> 8) * s.x,
+                                bkv_decode1<CODEC>(b >> 16) * s.x, bkv_decode1<CODEC>(b >> 24) * s.x);
+                z = make_float4(bkv_decode1<CODEC>(q.x >> sh) * s.y, bkv_decode1<CODEC>(q.y >> sh) * s.y,
+                                bkv_decode1<CODEC>(q.z >> sh) * s.y, bkv_decode1<CODEC>(q.w >> sh) * s.y);
+            } else if (page == -1) {
+                const float* p = bkv_ring(v, layer, s_seq[r], 0, head) + (size_t)(t & (2 * bs - 1)) * hd + d;
+                y = *(const float4*)p;
+                z = *(const float4*)(p + (size_t)v.n_head * 2 * bs * hd);
+            }
+            *(float4*)(k + (size_t)(r0 + r) * w + c * 4) = y;
+            *(float4*)(vv + (size_t)(r0 + r) * w + c * 4) = z;
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) *(float4*)(k + (size_t)(r0 + r) * w + c + 4 * j) = y[j];
-    }
-    for (int g = threadIdx.x; g < rows * vp; g += 256) {
-        // values d, d + 16, d + 32, d + 48 of a 64-wide piece
-        const int r = g / vp, i = g - r * vp, c = (i >> 4) * 64, head = c / hd, d = c % hd + (i & 15);
-        const int page = s_page[r], t = s_t[r];
-        float y[4] = {};
-        if (page >= 0) {
-            const size_t chunk = bkv_chunk(v, layer, page, head);
-            const uint4 b = *(const uint4*)(v.pool + (chunk * 2 + 1) * bs * hd +
-                                            (size_t)((t & (bs - 1)) >> 4) * 16 * hd + (bkv_v_off(t & 15, d) & ~15));
-            const float s = v.scales[chunk * 2 + 1];
-            const int sh = (t & 3) * 8;
-            y[0] = bkv_decode4<CODEC>(b.x >> sh, 0) * s;
-            y[1] = bkv_decode4<CODEC>(b.y >> sh, 0) * s;
-            y[2] = bkv_decode4<CODEC>(b.z >> sh, 0) * s;
-            y[3] = bkv_decode4<CODEC>(b.w >> sh, 0) * s;
-        } else if (page == -1) {
-            const float* p = bkv_ring(v, layer, s_seq[r], 1, head) + (size_t)(t & (2 * bs - 1)) * hd + d;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = p[16 * j];
-        }
-        float* o = vv + (size_t)(r0 + r) * w + c + (i & 15);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[16 * j] = y[j];
     }
 }
 

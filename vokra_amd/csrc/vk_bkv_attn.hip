@@ -162,8 +162,12 @@ struct BkvWave {
     float qf[C];    // a score is qf times the product of q's parts
     int last[C];    // last key that the lane's column sees
     float M[C], L[C];
-    vk_f32x4 O[C][DT];
+    vk_f32x4 O[C][DT];  // [4 c + i][r]: value 64 c + 16 grp + 4 r + i of the lane's column
 
+    // values 64 c + 16 grp + 4 r .. of the lane's column
+    __device__ __forceinline__ vk_f32x4 out4(int ct, int c, int r) const {
+        return vk_f32x4{O[ct][4 * c][r], O[ct][4 * c + 1][r], O[ct][4 * c + 2][r], O[ct][4 * c + 3][r]};
+    }
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int ct = 0; ct < C; ++ct) {
@@ -287,18 +291,23 @@ struct BkvWave {
         const int ring_mask = 2 * v.bs - 1;
         const float* kp = ring + (size_t)((key0 + col) & ring_mask) * HD + grp * 4;
         const float* vring = ring + side;
-        // V: four rows (keys 4 grp + r), columns 16 d + col; rows that no column sees are not used
+        // V: four rows (keys 4 grp + r), values 64 c + 4 col + i as row col of product
+        // 4 c + i; rows that no column sees are not used
         float vv[DT][4];
         float top = 0.0f;
         bool odd = false;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int key = key0 + grp * 4 + r;
-            const float* p = vring + (size_t)(key & ring_mask) * HD + col;
+            const float* p = vring + (size_t)(key & ring_mask) * HD + 4 * col;
+#pragma unroll
+            for (int c = 0; c < U; ++c) {
+                const float4 y = *(const float4*)(p + 64 * c);
+                vv[4 * c][r] = y.x, vv[4 * c + 1][r] = y.y, vv[4 * c + 2][r] = y.z, vv[4 * c + 3][r] = y.w;
+            }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const float y = p[16 * d];
-                vv[d][r] = key < t.keys ? y : 0.0f;
+                if (key >= t.keys) vv[d][r] = 0.0f;
                 odd = odd || !(fabsf(vv[d][r]) < INFINITY);
                 top = fmaxf(top, fabsf(vv[d][r]));
             }
@@ -355,16 +364,18 @@ struct BkvWave {
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     if ((x & 3) == r) w = __shfl(e[r], (x >> 2) * 16 + col, VK_WAVE);
-                const float* p1 = vring + (size_t)((key0 + x) & ring_mask) * HD + grp * 4;
+                const float* p1 = vring + (size_t)((key0 + x) & ring_mask) * HD + grp * 16;
                 if (key0 + x <= last[ct]) {
 #pragma unroll
-                    for (int d = 0; d < DT; ++d) {
-                        const float4 y = *(const float4*)(p1 + 16 * d);
-                        O[ct][d][0] = fmaf(w, y.x, O[ct][d][0]);
-                        O[ct][d][1] = fmaf(w, y.y, O[ct][d][1]);
-                        O[ct][d][2] = fmaf(w, y.z, O[ct][d][2]);
-                        O[ct][d][3] = fmaf(w, y.w, O[ct][d][3]);
-                    }
+                    for (int c = 0; c < U; ++c)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float4 y = *(const float4*)(p1 + 64 * c + 4 * r);
+                            O[ct][4 * c][r] = fmaf(w, y.x, O[ct][4 * c][r]);
+                            O[ct][4 * c + 1][r] = fmaf(w, y.y, O[ct][4 * c + 1][r]);
+                            O[ct][4 * c + 2][r] = fmaf(w, y.z, O[ct][4 * c + 2][r]);
+                            O[ct][4 * c + 3][r] = fmaf(w, y.w, O[ct][4 * c + 3][r]);
+                        }
                 }
             }
         }
@@ -542,7 +553,8 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(BkvAt
         __syncthreads();  // q's parts, or the columns before, are done with
         if (w.grp == 0) sml[wave][w.col] = make_float2(w.M[ct], l);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) *(vk_f32x4*)&sh.o[wave][w.col][16 * d + 4 * w.grp] = w.O[ct][d];
+        for (int d = 0; d < DT; ++d)
+            *(vk_f32x4*)&sh.o[wave][w.col][(d >> 2) * 64 + 16 * w.grp + (d & 3) * 4] = w.out4(ct, d >> 2, d & 3);
         __syncthreads();
         constexpr int PT = 4 * kWaves, PD = HD / PT;  // threads a column, values a thread
         const int c = threadIdx.x / PT, d0 = (threadIdx.x % PT) * PD;
@@ -724,7 +736,8 @@ __global__ __launch_bounds__(256, 2) void vk_bkv_attn_chunk(BkvAttnArgs a, const
         const float f = direct ? 0x1p-14f / l : 0x1p-14f;
         if (!direct && w.grp == 0) ((float2*)a.part)[slot * a.cols + c] = make_float2(w.M[ct], l);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) *(vk_f32x4*)(dst + 16 * d + 4 * w.grp) = w.O[ct][d] * f;
+        for (int d = 0; d < DT; ++d)
+            *(vk_f32x4*)(dst + (d >> 2) * 64 + 16 * w.grp + (d & 3) * 4) = w.out4(ct, d >> 2, d & 3) * f;
     }
 }
 

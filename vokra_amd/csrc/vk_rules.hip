@@ -55,24 +55,33 @@ __global__ __launch_bounds__(256) void vk_rules(RulesArgs a) {
     const bool hist = a.hist_off, biased = a.bias_off;
     const int h0 = hist ? max(a.hist_off[row], 0) : 0, h1 = hist ? min(a.hist_off[row + 1], a.n_hist) : 0;
     const int b0 = biased ? max(a.bias_off[row], 0) : 0, b1 = biased ? min(a.bias_off[row + 1], a.n_bias) : 0;
+    const float rep = a.repetition ? a.repetition[row] : 1.0f, pres = a.presence ? a.presence[row] : 0.0f,
+                freq = a.frequency ? a.frequency[row] : 0.0f;
     const bool listed = h1 > h0 || b1 > b0;
     if (listed) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) count4[t + 256 * j] = slot4[t + 256 * j] = make_int4(0, 0, 0, 0);
         __syncthreads();
         const int lo = max(c0, 0), hi = min(c0 + RU_SLICE, a.vocab);
-        for (int i = h0 + t; i < h1; i += 256) {
-            const int v = a.hist[i];
-            if (v >= lo && v < hi) atomicAdd(&count[v - c0], 1);
+        // eight (two) loads in flight
+        for (int i = h0 + t; i < h1; i += 8 * 256) {
+            int v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = i + 256 * j < h1 ? a.hist[i + 256 * j] : -1;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (v[j] >= lo && v[j] < hi) atomicAdd(&count[v[j] - c0], 1);
         }
-        for (int i = b0 + t; i < b1; i += 256) {
-            const int v = a.bias_ids[i];
-            if (v >= lo && v < hi) atomicMax(&slot[v - c0], i - b0 + 1);
+        for (int i = b0 + t; i < b1; i += 2 * 256) {
+            int v[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) v[j] = i + 256 * j < b1 ? a.bias_ids[i + 256 * j] : -1;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (v[j] >= lo && v[j] < hi) atomicMax(&slot[v[j] - c0], i + 256 * j - b0 + 1);
         }
         __syncthreads();
     }
-    const float rep = a.repetition ? a.repetition[row] : 1.0f, pres = a.presence ? a.presence[row] : 0.0f,
-                freq = a.frequency ? a.frequency[row] : 0.0f;
     const uint32_t* mask = a.mask ? a.mask + (size_t)row * a.mask_stride : nullptr;
     float* out = a.out ? a.out + (size_t)row * a.stride : nullptr;
     const bool vec = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(x)) & 15) == 0;
@@ -144,10 +153,11 @@ __global__ __launch_bounds__(256) void vk_rules(RulesArgs a) {
     const uint32_t b = __float_as_uint(bv), ord = b & 0x80000000u ? ~b : b | 0x80000000u;
     unsigned long long key = bv > -INFINITY ? ((unsigned long long)ord << 32) | (0xffffffffu - (uint32_t)bi) : 0ull;
     if (gridDim.x > 1) {
-        // the maximum has reached memory when its old value is here; then this
+        // the maximum has been taken when its old value is here; only then this
         // workgroup is counted
-        const unsigned long long old = atomicMax(&a.best[row], key);
-        if (atomicAdd(&a.done[row], old == ~0ull ? 2u : 1u) != gridDim.x - 1) return;
+        unsigned long long old = atomicMax(&a.best[row], key);
+        asm volatile("" : "+v"(old)::"memory");
+        if (atomicAdd(&a.done[row], 1u) != gridDim.x - 1) return;
         key = atomicExch(&a.best[row], 0ull);
         atomicExch(&a.done[row], 0u);
     }
