@@ -50,7 +50,6 @@ struct BkvView {
     int* table;      // [n_seq][max_blocks] page of each full block, -1 = none
     int* len;        // [n_seq] rows held
     int* floor_;     // [n_seq] the lowest row a step may start at
-    int* claim;      // [n_seq] scratch of the planning kernels
     int* refs;       // [n_page] sequences that hold the page
     uint32_t* used;  // bitmap of refs != 0
     int* fresh;      // [n_page] pages taken by the current call
@@ -67,11 +66,12 @@ constexpr int BKV_INT8 = 0, BKV_E4M3 = 1;
 
 // Byte of element (token t of the tile, d) in a 16-token K or V tile: the
 // order in which the attention's matrix instructions take them, 16 bytes a
-// lane. K: lane (d % 64 / 16) * 16 + t holds d % 16 = 0 .. 15 of chunk d / 64.
-// V: lane (t / 4) * 16 + d % 64 / 4 holds d % 4 = 0 .. 3 (a word each: row
-// d % 64 / 4 of four products) for tokens t % 4 (a byte each).
+// lane, and in which 16-byte reads of rows leave them.
+// K: lane (d % 16 / 4) * 16 + t holds word d % 64 / 16, byte d % 4.
+// V: lane (t / 4) * 16 + d % 64 / 4 holds word d % 4 (row d % 64 / 4 of four
+// products), byte t % 4.
 __host__ __device__ inline int bkv_k_off(int t, int d) {
-    return ((d >> 6) * 64 + ((d >> 4) & 3) * 16 + t) * 16 + (d & 15);
+    return ((d >> 6) * 64 + ((d >> 2) & 3) * 16 + t) * 16 + ((d >> 4) & 3) * 4 + (d & 3);
 }
 __host__ __device__ inline int bkv_v_off(int t, int d) {
     return ((d >> 6) * 64 + (t >> 2) * 16 + ((d >> 2) & 15)) * 16 + (d & 3) * 4 + (t & 3);

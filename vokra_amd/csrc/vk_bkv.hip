@@ -19,8 +19,8 @@
 // copies one row of the page table and the open block's rows.
 //
 // Planning is one workgroup (items are at most 1024, one thread each): checks,
-// prefix sums over the pages that the items take, pages from a bitmap (lowest
-// first, so the result does not depend on the order of earlier frees). The
+// prefix sums over what they take, pages from a bitmap (lowest first, so the
+// result does not depend on the order of earlier frees). The
 // first item that fails ends the call; the ones before it stay done.
 #include <algorithm>
 #include <climits>
@@ -35,31 +35,37 @@ constexpr int BKV_TPB = 1024;  // threads of the planning kernels at most
 
 // ---- workgroup prefix sums ----------------------------------------------------
 
-// Exclusive prefix sum over the workgroup; *total = the sum. red: 17 ints.
-__device__ __forceinline__ int bkv_scan(int v, int* red, int* total) {
-    const int waves = (int)blockDim.x >> 6;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int x = v;
+// Exclusive prefix sums of N numbers a thread over the workgroup, in place;
+// totals in sum. red: 17 N ints.
+template <int N>
+__device__ __forceinline__ void bkv_scan(int (&v)[N], int (&sum)[N], int* red) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = (int)blockDim.x >> 6;
+    int x[N];
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o, VK_WAVE);
-        if (lane >= o) x += y;
-    }
-    __syncthreads();
-    if (lane == 63) red[wave] = x;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        int s = 0;
-        for (int w = 0; w < waves; ++w) {
-            const int t = red[w];
-            red[w] = s;
-            s += t;
+    for (int j = 0; j < N; ++j) {
+        x[j] = v[j];
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(x[j], o, VK_WAVE);
+            if (lane >= o) x[j] += y;
         }
-        red[waves] = s;
     }
     __syncthreads();
-    *total = red[waves];
-    return red[wave] + x - v;
+    if (lane == 63)
+#pragma unroll
+        for (int j = 0; j < N; ++j) red[wave * N + j] = x[j];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        int before = 0, all = 0;
+        for (int w = 0; w < waves; ++w) {
+            const int t = red[w * N + j];
+            if (w < wave) before += t;
+            all += t;
+        }
+        v[j] = before + x[j] - v[j];
+        sum[j] = all;
+    }
 }
 
 // The last index i in [0, n) with off[i] <= k (off ascending, off[0] = 0).
@@ -83,8 +89,9 @@ __device__ void bkv_take(const BkvView& v, int want, int* red) {
         const int w = base + (int)threadIdx.x;
         uint32_t avail = w < words ? ~v.used[w] : 0u;
         if (w == words - 1 && (v.n_page & 31)) avail &= (1u << (v.n_page & 31)) - 1u;
-        int total;
-        int at = got + bkv_scan(__popc(avail), red, &total);
+        int n[1] = {(int)__popc(avail)}, total[1];
+        bkv_scan(n, total, red);
+        int at = got + n[0];
         uint32_t taken = 0;
         while (avail && at < want) {
             const int b = __ffs(avail) - 1;
@@ -93,7 +100,7 @@ __device__ void bkv_take(const BkvView& v, int want, int* red) {
             avail &= avail - 1;
         }
         if (taken) v.used[w] |= taken;
-        got += total;
+        got += total[0];
         last = base;
         base += (int)blockDim.x;
     }
@@ -121,7 +128,6 @@ __global__ void vk_bkv_reset(BkvView v) {
     for (size_t i = i0; i < (size_t)v.n_seq; i += step) {
         v.len[i] = 0;
         v.floor_[i] = 0;
-        v.claim[i] = INT_MAX;
     }
     for (size_t i = i0; i < (size_t)v.n_page; i += step) v.refs[i] = 0;
     for (size_t i = i0; i < (size_t)(v.n_page + 31) / 32; i += step) v.used[i] = 0;
@@ -136,110 +142,103 @@ __global__ void vk_bkv_fill(uint4* p, size_t n) {
 
 // ---- step --------------------------------------------------------------------
 
-// Every item names its sequence once: claim[seq] = the lowest item that names
-// it. The first barrier orders the clearing before the claims.
-__device__ __forceinline__ bool bkv_claim(const BkvView& v, int i, bool in_range, int seq) {
-    if (in_range) v.claim[seq] = INT_MAX;
-    __syncthreads();
-    if (in_range) atomicMin(&v.claim[seq], i);
-    __syncthreads();
-    return in_range && __hip_atomic_load(&v.claim[seq], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == i;
+// Whether an item before i names id, and whether any of the n items does
+// (ids in LDS, 16-byte aligned, those beyond n negative).
+__device__ __forceinline__ void bkv_named(const int* ids, int n, int i, int id, bool* before, bool* any) {
+    *before = *any = false;
+    for (int j = 0; j < n; j += 4) {
+        const int4 x = *(const int4*)(ids + j);
+        const bool m[4] = {x.x == id, x.y == id, x.z == id, x.w == id};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            *any = *any || m[c];
+            *before = *before || (m[c] && j + c < i);
+        }
+    }
 }
 
+// One thread an item; about five trips to memory, whatever the items are.
 __global__ __launch_bounds__(BKV_TPB) void vk_bkv_step(BkvView v, int n, int n_rows, int max_count,
                                                        const int* __restrict__ seqs, const int* __restrict__ starts,
                                                        const int* __restrict__ counts) {
-    __shared__ int red[BKV_TPB / 64 + 1];
-    __shared__ int off[BKV_TPB];   // prefix of pages taken, then of write entries
-    __shared__ int s_start[BKV_TPB];
+    __shared__ int red[3 * (BKV_TPB / 64)];
+    __shared__ __align__(16) int s_seq[BKV_TPB];
+    __shared__ int s_page[BKV_TPB + 1], s_work[BKV_TPB + 1];  // prefixes: pages taken, blocks reached
     __shared__ BkvItem s_item[BKV_TPB];
-    __shared__ int s_bad, s_rows;
-    const int i = threadIdx.x;
-    if (i == 0) {
-        s_bad = n;
-        s_rows = 0;
-    }
+    __shared__ int s_bad, s_done;
+    const int i = threadIdx.x, bs_log = 31 - __clz(v.bs);
     const int seq = i < n ? seqs[i] : -1, start = i < n ? starts[i] : 0, count = i < n ? counts[i] : 0;
-    const bool in_range = i < n && (unsigned)seq < (unsigned)v.n_seq;
-    const bool mine = bkv_claim(v, i, in_range, seq);
+    const int free_pages = v.meta[BKV_FREE];
+    const bool in_range = (unsigned)seq < (unsigned)v.n_seq;
     const int len = in_range ? v.len[seq] : 0, fl = in_range ? v.floor_[seq] : 0;
-    bool ok = mine && count >= 0 && count <= max_count && start >= fl && start <= len &&
+    s_seq[i] = seq;
+    if (i == 0) s_bad = s_done = n;
+    __syncthreads();
+    bool named, any;
+    bkv_named(s_seq, n, i, seq, &named, &any);
+    bool ok = in_range && !named && count >= 0 && count <= max_count && start >= fl && start <= len &&
               count <= v.max_time - start;
-    const int cnt = ok ? count : 0;
-    int rows;
-    const int row0 = bkv_scan(cnt, red, &rows);
-    if (row0 + cnt > n_rows) ok = false;
+    // rows; pages: of the blocks that the step's rows fill; blocks that they reach
+    const int cnt = ok ? count : 0, b0 = start >> bs_log, b1 = ok ? (start + cnt) >> bs_log : b0;
+    const int need = b1 - b0;
+    int at[3] = {cnt, need, cnt > 0 ? ((start + cnt - 1) >> bs_log) - b0 + 1 : 0}, sum[3];
+    bkv_scan(at, sum, red);
+    // up to the first item that fails, the prefixes hold no item that does
+    if (at[0] + cnt > n_rows) ok = false;
     if (i < n && !ok) atomicMin(&s_bad, i);
     __syncthreads();
     const int bad = s_bad;
-    // pages: the blocks that are full after the step and reach into its rows
-    const int b0 = start / v.bs, b1 = ok ? (start + cnt) / v.bs : b0;
-    int need = ok && i < bad ? b1 - b0 : 0, total;
-    const int free_pages = v.meta[BKV_FREE];
-    int at = bkv_scan(need, red, &total);
-    __syncthreads();
-    if (i < bad && ok && need > 0 && at + need > free_pages) atomicMin(&s_bad, i);
-    __syncthreads();
-    const int done = s_bad;
-    if (done < bad) {  // some item found too few pages: those before it only
-        if (i >= done) need = 0;
-        at = bkv_scan(need, red, &total);
+    if (i < bad && need > 0 && at[1] + need > free_pages) atomicMin(&s_done, i);
+    s_item[i] = BkvItem{seq, start, cnt, at[0]};
+    s_page[i] = at[1];
+    s_work[i] = at[2];
+    if (i + 1 == (int)blockDim.x) {
+        s_page[i + 1] = sum[1];
+        s_work[i + 1] = sum[2];
     }
-    off[i] = at;
-    s_start[i] = b0;
-    s_item[i] = BkvItem{seq, start, cnt, row0};
     __syncthreads();
+    const int done = min(s_done, bad), total = s_page[done], n_work = min(s_work[done], v.max_work);
     if (total) bkv_take(v, total, red);
-    // pages that a taken-back sequence held from its new start on
     if (i < done) {
-        for (int b = b0; b < len / v.bs; ++b) {
-            bkv_drop(v, v.table[(size_t)seq * v.max_blocks + b]);
-            v.table[(size_t)seq * v.max_blocks + b] = -1;
+        // pages that a taken-back sequence held from its new start on
+        for (int b = b0; b < len >> bs_log; ++b) {
+            int* e = v.table + (size_t)seq * v.max_blocks + b;
+            bkv_drop(v, *e);
+            if (b >= b1) *e = -1;
         }
-    }
-    __syncthreads();
-    for (int k = i; k < total; k += (int)blockDim.x) {
-        const int it = bkv_find(off, done, k);
-        const int page = v.fresh[k];
-        v.table[(size_t)s_item[it].seq * v.max_blocks + s_start[it] + (k - off[it])] = page;
-        v.refs[page] = 1;
-    }
-    __syncthreads();
-    if (i < done) {
-        const int end = start + cnt, nb = (end + v.bs - 1) / v.bs;
+        const int end = start + cnt, nb = (end + v.bs - 1) >> bs_log;
         v.len[seq] = end;
         v.floor_[seq] = max(fl, (nb - 2) * v.bs);
     }
-    for (int k = i; k < kBkvMaxItems; k += (int)blockDim.x)
-        v.step[k] = k < done ? s_item[k] : BkvItem{0, 0, 0, 0};  // no rows beyond the items done
-    // the write's entries: every block that an item's rows reach
-    const int nblk = i < done && cnt > 0 ? (start + cnt - 1) / v.bs - b0 + 1 : 0;
-    int n_work;
-    const int w0 = bkv_scan(nblk, red, &n_work);
-    off[i] = w0;
-    if (i < done) atomicMax(&s_rows, row0 + cnt);  // rows of the items done
-    __syncthreads();
-    n_work = min(n_work, v.max_work);
+    __syncthreads();  // an entry's old page is read before its new one is there
+    for (int k = i; k < total; k += (int)blockDim.x) {
+        const int it = bkv_find(s_page, done, k), page = v.fresh[k];
+        v.table[(size_t)s_item[it].seq * v.max_blocks + (s_item[it].start >> bs_log) + (k - s_page[it])] = page;
+        v.refs[page] = 1;
+    }
     for (int k = i; k < n_work; k += (int)blockDim.x) {
-        const int it = bkv_find(off, done, k);
+        const int it = bkv_find(s_work, done, k), b = k - s_work[it];
         const BkvItem m = s_item[it];
         BkvWork e;
         e.seq = m.seq;
         e.start = m.start;
         e.end = m.start + m.count;
         e.row0 = m.row0;
-        e.block = s_start[it] + (k - off[it]);
-        e.page = (e.block + 1) * v.bs <= e.end ? v.table[(size_t)m.seq * v.max_blocks + e.block] : -1;
+        e.block = (m.start >> bs_log) + b;
+        e.page = (e.block + 1) * v.bs <= e.end ? v.fresh[s_page[it] + b] : -1;
+        e.pad[0] = e.pad[1] = 0;
         v.work[k] = e;
     }
+    for (int k = i; k < kBkvMaxItems; k += (int)blockDim.x)
+        v.step[k] = k < done ? s_item[k] : BkvItem{0, 0, 0, 0};  // no rows beyond the items done
     if (i == 0) {
         atomicSub(&v.meta[BKV_FREE], total);
-        v.meta[BKV_STATUS] = done == n ? VOKRA_HIP_OK
+        v.meta[BKV_STATUS] = done == n    ? VOKRA_HIP_OK
                              : done < bad ? VOKRA_HIP_ERROR_KV_CACHE_EXHAUSTED
                                           : VOKRA_HIP_ERROR_INVALID_ARGUMENT;
         v.meta[BKV_DONE] = done;
         v.meta[BKV_STEP_N] = done;
-        v.meta[BKV_STEP_ROWS] = s_rows;
+        v.meta[BKV_STEP_ROWS] = done ? s_item[done - 1].row0 + s_item[done - 1].count : 0;
         v.meta[BKV_WORK_N] = n_work;
     }
 }
@@ -306,12 +305,12 @@ __global__ __launch_bounds__(256) void vk_bkv_write(BkvView v, int layer, unsign
 #pragma unroll
         for (int p = 0; p < NT; ++p) {
             const int t0 = e.block * bs + p / pieces * 16, d0 = p % pieces * 64;
-            if (side == 0) {  // token lane % 16, values 16 (lane / 16) ..
-                const int t = t0 + (lane & 15), d = d0 + (lane >> 4) * 16;
+            if (side == 0) {  // token lane % 16, values 4 (lane / 16) .. + 0, 16, 32, 48
+                const int t = t0 + (lane & 15), d = d0 + (lane >> 4) * 4;
                 const float* r = t >= e.start ? in + (size_t)(t - e.start) * rs + d : ring + (size_t)(t & mask) * hd + d;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float4 y = *(const float4*)(r + 4 * j);
+                    const float4 y = *(const float4*)(r + 16 * j);
                     x[p][4 * j] = y.x, x[p][4 * j + 1] = y.y, x[p][4 * j + 2] = y.z, x[p][4 * j + 3] = y.w;
                 }
             } else {  // tokens 4 (lane / 16) .., values 4 (lane % 16) ..
@@ -428,27 +427,28 @@ __global__ __launch_bounds__(256) void vk_bkv_read(BkvView v, int layer, int n, 
 // ---- fork, free, copy, compact -------------------------------------------------
 
 // The checks that a fork and a copy share: source and destination in range,
-// the destination empty, named once and no source of the call's.
-// A source that is some item's destination is refused (`same`: both ids are of
-// one cache).
+// the destination empty, named once and no source of the call's (`same`: both
+// ids are of one cache).
 __device__ __forceinline__ bool bkv_pair_ok(const BkvView& dv, const BkvView& sv, bool same, int i, int n, int src,
-                                            int dst) {
-    const bool rs = i < n && (unsigned)src < (unsigned)sv.n_seq, rd = i < n && (unsigned)dst < (unsigned)dv.n_seq;
-    if (same && rs) dv.claim[src] = INT_MAX;
-    const bool mine = bkv_claim(dv, i, rd, dst);
-    bool ok = rs && mine && dv.len[dst] == 0;
-    if (same && ok)
-        ok = __hip_atomic_load(&dv.claim[src], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == INT_MAX;
-    return ok;
+                                            int dst, int* s_dst) {
+    const bool rs = (unsigned)src < (unsigned)sv.n_seq, rd = (unsigned)dst < (unsigned)dv.n_seq;
+    const int dst_len = rd ? dv.len[dst] : 1;
+    s_dst[i] = dst;
+    __syncthreads();
+    bool named, any, before;
+    bkv_named(s_dst, n, i, dst, &named, &any);
+    bkv_named(s_dst, n, i, src, &before, &any);
+    return rs && rd && dst_len == 0 && !named && !(same && any);
 }
 
 __global__ __launch_bounds__(BKV_TPB) void vk_bkv_fork_plan(BkvView v, int n, const int* __restrict__ srcs,
                                                             const int* __restrict__ dsts) {
+    __shared__ __align__(16) int s_dst[BKV_TPB];
     __shared__ int s_bad;
     const int i = threadIdx.x;
     if (i == 0) s_bad = n;
     const int src = i < n ? srcs[i] : -1, dst = i < n ? dsts[i] : -1;
-    const bool ok = bkv_pair_ok(v, v, true, i, n, src, dst);
+    const bool ok = bkv_pair_ok(v, v, true, i, n, src, dst, s_dst);
     if (i < n && !ok) atomicMin(&s_bad, i);
     __syncthreads();
     const int done = s_bad;
@@ -503,13 +503,17 @@ __global__ __launch_bounds__(256) void vk_bkv_fork_rows(BkvView v, int rows) {
 }
 
 __global__ __launch_bounds__(BKV_TPB) void vk_bkv_free_plan(BkvView v, int n, const int* __restrict__ seqs) {
+    __shared__ __align__(16) int s_seq[BKV_TPB];
     __shared__ int s_bad;
     const int i = threadIdx.x;
     if (i == 0) s_bad = n;
     const int seq = i < n ? seqs[i] : -1;
-    const bool in_range = i < n && (unsigned)seq < (unsigned)v.n_seq;
-    const bool mine = bkv_claim(v, i, in_range, seq);
-    if (i < n && !in_range) atomicMin(&s_bad, i);
+    s_seq[i] = seq;
+    __syncthreads();
+    if (i < n && (unsigned)seq >= (unsigned)v.n_seq) atomicMin(&s_bad, i);
+    bool named, any;
+    bkv_named(s_seq, n, i, seq, &named, &any);
+    const bool mine = !named;
     __syncthreads();
     const int done = s_bad;
     if (i < done) {
@@ -545,31 +549,30 @@ __global__ __launch_bounds__(256) void vk_bkv_free_pages(BkvView v) {
 __global__ __launch_bounds__(BKV_TPB) void vk_bkv_copy_plan(BkvView dv, BkvView sv, int same, int n,
                                                             const int* __restrict__ srcs,
                                                             const int* __restrict__ dsts) {
-    __shared__ int red[BKV_TPB / 64 + 1];
-    __shared__ int off[BKV_TPB], s_src[BKV_TPB], s_dst[BKV_TPB];
-    __shared__ int s_bad;
+    __shared__ int red[BKV_TPB / 64];
+    __shared__ int off[BKV_TPB + 1], s_src[BKV_TPB];
+    __shared__ __align__(16) int s_dst[BKV_TPB];
+    __shared__ int s_bad, s_done;
     const int i = threadIdx.x;
-    if (i == 0) s_bad = n;
+    if (i == 0) s_bad = s_done = n;
     const int src = i < n ? srcs[i] : -1, dst = i < n ? dsts[i] : -1;
-    bool ok = bkv_pair_ok(dv, sv, same != 0, i, n, src, dst);
+    const int free_pages = dv.meta[BKV_FREE];
+    bool ok = bkv_pair_ok(dv, sv, same != 0, i, n, src, dst, s_dst);
     const int len = ok ? sv.len[src] : 0;
     if (len > dv.max_time) ok = false;
+    const int need = ok ? len / dv.bs : 0;
+    int at[1] = {need}, sum[1];
+    bkv_scan(at, sum, red);
     if (i < n && !ok) atomicMin(&s_bad, i);
+    off[i] = at[0];
+    s_src[i] = src;
+    if (i + 1 == (int)blockDim.x) off[i + 1] = sum[0];
     __syncthreads();
     const int bad = s_bad;
-    int need = i < bad ? len / dv.bs : 0, total;
-    const int free_pages = dv.meta[BKV_FREE];
-    int at = bkv_scan(need, red, &total);
-    if (i < bad && need > 0 && at + need > free_pages) atomicMin(&s_bad, i);
+    if (i < bad && need > 0 && at[0] + need > free_pages) atomicMin(&s_done, i);
     __syncthreads();
-    const int done = s_bad;
-    if (i >= done) need = 0;
-    at = bkv_scan(need, red, &total);
-    off[i] = at;
-    s_src[i] = src;
-    s_dst[i] = dst;
-    __syncthreads();
-    bkv_take(dv, total, red);
+    const int done = min(s_done, bad), total = off[done];
+    if (total) bkv_take(dv, total, red);
     for (int k = i; k < total; k += (int)blockDim.x) {
         const int it = bkv_find(off, done, k), b = k - off[it], page = dv.fresh[k];
         dv.table[(size_t)s_dst[it] * dv.max_blocks + b] = page;
@@ -621,7 +624,7 @@ __global__ __launch_bounds__(256) void vk_bkv_copy_rows(BkvView dv, BkvView sv) 
 // u pages are in use: the k-th one at or above u moves to the k-th free one
 // below u. v.fresh takes the free ones, v.moves the pairs.
 __global__ __launch_bounds__(BKV_TPB) void vk_bkv_compact_plan(BkvView v) {
-    __shared__ int red[BKV_TPB / 64 + 1];
+    __shared__ int red[2 * (BKV_TPB / 64)];
     const int u = v.n_page - v.meta[BKV_FREE], words = (v.n_page + 31) / 32;
     int holes = 0, movers = 0;
     for (int base = 0; base < words; base += BKV_TPB) {
@@ -631,13 +634,13 @@ __global__ __launch_bounds__(BKV_TPB) void vk_bkv_compact_plan(BkvView v) {
         const int below = min(max(u - w * 32, 0), 32);
         const uint32_t low = w < words ? (below == 32 ? ~0u : (1u << below) - 1u) : 0u;
         uint32_t h = ~bits & low, m = bits & ~low;
-        int nh, nm;
-        int ah = holes + bkv_scan(__popc(h), red, &nh);
-        int am = movers + bkv_scan(__popc(m), red, &nm);
+        int at[2] = {(int)__popc(h), (int)__popc(m)}, all[2];
+        bkv_scan(at, all, red);
+        int ah = holes + at[0], am = movers + at[1];
         for (; h; h &= h - 1) v.fresh[ah++] = w * 32 + __ffs(h) - 1;
         for (; m; m &= m - 1) v.moves[am++].x = w * 32 + __ffs(m) - 1;
-        holes += nh;
-        movers += nm;
+        holes += all[0];
+        movers += all[1];
     }
     __syncthreads();
     for (int k = threadIdx.x; k < movers; k += BKV_TPB) {
@@ -778,7 +781,7 @@ constexpr unsigned kMoveGrid = 2048;
 
 hipError_t launch_bkv_copy(hipStream_t s, const BkvView& dv, const BkvView& sv, int n, const int* src,
                            const int* dst) {
-    hipLaunchKernelGGL(vk_bkv_copy_plan, dim3(1), dim3(BKV_TPB), 0, s, dv, sv, (int)(dv.meta == sv.meta), n, src, dst);
+    hipLaunchKernelGGL(vk_bkv_copy_plan, dim3(1), dim3(plan_threads(n)), 0, s, dv, sv, (int)(dv.meta == sv.meta), n, src, dst);
     if (n) {
         hipLaunchKernelGGL(vk_bkv_move_pages, dim3(kMoveGrid), dim3(256), 0, s, dv, sv);
         hipLaunchKernelGGL(vk_bkv_copy_rows, dim3(row_grid(dv, n)), dim3(256), 0, s, dv, sv);

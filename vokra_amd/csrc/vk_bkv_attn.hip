@@ -187,13 +187,13 @@ struct BkvWave {
         const int cc = t.c0 + c, j = item_row(a, t, c);
         return ((size_t)(t.it.row0 + j) * a.hq + head * a.g + (cc - j * a.g)) * HD;
     }
-    // q of the 16 columns from c0 on: the lane's 16 values d = 64 u + 16 grp .. of
-    // its column (fetch_q), and their parts, two k steps of 8 (split_q)
+    // q of the 16 columns from c0 on: of the lane's column the values 16 i + 4 grp ..
+    // (fetch_q), and their parts, k steps of 8 (split_q)
     __device__ __forceinline__ void fetch_q(const BkvAttnArgs& a, const BkvTile& t, int head, int c0,
                                             float4 (&x)[4 * U]) const {
-        const float* p = a.q + row(a, t, head, c0 + col) + grp * 16;
+        const float* p = a.q + row(a, t, head, c0 + col) + grp * 4;
 #pragma unroll
-        for (int i = 0; i < 4 * U; ++i) x[i] = *(const float4*)(p + (i >> 2) * 64 + (i & 3) * 4);
+        for (int i = 0; i < 4 * U; ++i) x[i] = *(const float4*)(p + 16 * i);
     }
     __device__ __forceinline__ void split_q(const BkvAttnArgs& a, const BkvTile& t, int ct, int c0,
                                             const float4 (&x)[4 * U], half8v (&h8)[2 * U], half8v (&l8)[2 * U]) {

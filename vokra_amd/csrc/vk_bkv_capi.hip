@@ -100,7 +100,7 @@ int status_of(vokra_hip_bkv* kv, const char* what, size_t* n_done) {
 void release(vokra_hip_bkv* kv) {
     BkvView& v = kv->v;
     for (void* p : {(void*)v.pool, (void*)v.scales, (void*)v.ring, (void*)v.table, (void*)v.len, (void*)v.floor_,
-                    (void*)v.claim, (void*)v.refs, (void*)v.used, (void*)v.fresh, (void*)v.moves, (void*)v.remap,
+                    (void*)v.refs, (void*)v.used, (void*)v.fresh, (void*)v.moves, (void*)v.remap,
                     (void*)v.meta, (void*)v.step, (void*)v.plan, (void*)v.work, (void*)kv->items,
                     (void*)kv->rows})
         if (p) (void)hipFree(p);
@@ -201,7 +201,6 @@ int vokra_hip_bkv_create(vokra_hip_ctx_t* c, size_t n_layer, size_t n_head, size
     reserve(&e, &v.table, n_seq * (size_t)v.max_blocks);
     reserve(&e, &v.len, n_seq);
     reserve(&e, &v.floor_, n_seq);
-    reserve(&e, &v.claim, n_seq);
     reserve(&e, &v.refs, n_page);
     reserve(&e, &v.used, (n_page + 31) / 32);
     reserve(&e, &v.fresh, n_page);
