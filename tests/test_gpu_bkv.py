@@ -300,8 +300,8 @@ def test_attention_where_values_are_not_finite(ctx):
     assert np.array_equal(np.isnan(got).all(-1), bad) and np.array_equal(np.isnan(got).any(-1), bad)
 
 
-def test_an_item_is_the_same_in_any_batch(ctx):
-    """Decode rows of a sequence alone, in a batch, and in another order."""
+def test_the_order_of_a_batch_does_not_matter(ctx):
+    """Decode rows of four sequences in two orders: the same bits."""
     print("[case] bkv attn batch", flush=True)
     p = Pair(ctx, 1, 2, 128, 4, 700, 16, 100, 1500)
     lens = np.array([700, 33, 260, 1])

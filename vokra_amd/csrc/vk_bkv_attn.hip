@@ -51,7 +51,7 @@ struct BkvAttnArgs {
     int tiles;          // column tiles of the call
     int chunks;         // 0: one column tile an item; 1: as many as its columns need
     int splits;         // key ranges a column tile may have (grid)
-    int per;            // least units of a key range (chunks), 0: 8
+    int per;            // least units of a key range
     int cols;           // columns a slot has room for
 };
 
@@ -105,7 +105,7 @@ __device__ __forceinline__ bool bkv_tile(const BkvAttnArgs& a, int tile, int tc,
     }
     t.full = min((t.it.start + t.it.count) >> bs_log << bs_log, (t.keys + 15) & ~15);
     t.units = (t.full + kUnit - 1) / kUnit;
-    t.per = max(a.per ? a.per : 8, (bkv_div(t.units + a.splits - 1, a.splits_inv) + 3) & ~3);
+    t.per = max(a.per, (bkv_div(t.units + a.splits - 1, a.splits_inv) + 3) & ~3);
     return true;
 }
 
@@ -828,18 +828,13 @@ hipError_t launch_bkv_attn(hipStream_t s, const BkvView& v, int layer, int n, in
     const int room = kBkvParts;
     const int units = std::max(1, (max_len + kUnit - 1) / kUnit);
     const long long most = std::min<long long>(64, std::max<long long>(1, room / ((long long)v.n_head * a.cols)));
-    if (a.chunks) {
-        // Ranges of 8 to 64 units: enough for two workgroups a CU, and no tile
-        // much longer than the others.
-        const long long per = tiles * v.n_head * units / 1280;
-        a.per = (int)std::max<long long>(std::min<long long>(std::max<long long>(per, 8), 64), (units + most - 1) / most);
-        a.splits = (units + a.per - 1) / a.per;
-    } else {
-        // Key ranges of 256 keys and more, at most 64 a tile and what the workspace
-        // has room for: that does not depend on the batch, so an item's rows come
-        // out the same in any batch.
-        a.splits = (int)std::min<long long>(most, (units + 7) / 8);
-    }
+    // Units a key range: the call's units at the longest rows' length over 512
+    // (1280 for chunks), so that there are ranges for every CU and few to merge.
+    const long long all = tiles * v.n_head * units;
+    const long long per = a.chunks ? std::min<long long>(std::max<long long>(all / 1280, 8), 64)
+                                   : std::max<long long>(all / 512, 8);
+    a.per = (int)((std::max(per, (units + most - 1) / most) + 3) / 4 * 4);
+    a.splits = (units + a.per - 1) / a.per;
     a.part_o = (size_t)room * 2;
     auto inv = [](int d) { return d == 1 ? 0u : (uint32_t)(((1ull << 32) + (uint32_t)d - 1) / (uint32_t)d); };
     a.g_inv = inv(a.g);
