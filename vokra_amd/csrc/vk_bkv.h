@@ -10,6 +10,8 @@
 
 constexpr int kBkvMaxItems = 1024;   // items of one call: one thread of the planning workgroup each
 constexpr int kBkvParts = 1 << 18;  // query rows of which a split attention can hold a partial result
+// a context's partial results ((max, sum) and up to 128 values a row) and counters
+constexpr size_t kBkvPartBytes = (size_t)kBkvParts * (128 + 2 + 1) * 4;
 
 // What planning kernels leave for the kernels of the same call or step.
 // meta (int32): see the BKV_ indices.
@@ -78,6 +80,7 @@ __host__ __device__ inline int bkv_v_off(int t, int d) {
 }
 
 namespace vk {
+hipError_t launch_bkv_part_clear(hipStream_t s, void* part);
 hipError_t launch_bkv_reset(hipStream_t s, const BkvView& v, bool clear_data);
 hipError_t launch_bkv_step(hipStream_t s, const BkvView& v, int n, int n_rows, int max_count, const int* seqs,
                            const int* starts, const int* counts);
@@ -93,8 +96,8 @@ hipError_t launch_bkv_compact(hipStream_t s, const BkvView& v);
 // out (2 ints): length of seq, page of block
 hipError_t launch_bkv_peek(hipStream_t s, const BkvView& v, int seq, int block, int* out);
 // Rows of the current step (n items, n_rows rows, at most max_count each, no
-// more than max_len rows held by any) against the cache; part: kBkvParts *
-// (hd + 2) floats.
+// more than max_len rows held by any) against the cache; part:
+// kBkvPartBytes, its counters zero.
 hipError_t launch_bkv_attn(hipStream_t s, const BkvView& v, int layer, int n, int n_rows, int max_count, int max_len,
                            int hq, const float* q, float scale, float* out, float* part);
 }  // namespace vk

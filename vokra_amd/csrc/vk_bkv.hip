@@ -682,6 +682,11 @@ __global__ void vk_bkv_peek(BkvView v, int seq, int block, int* out) {
 
 // ---- launchers -----------------------------------------------------------------
 
+hipError_t launch_bkv_part_clear(hipStream_t s, void* part) {
+    hipLaunchKernelGGL(vk_bkv_fill, dim3(2048), dim3(256), 0, s, (uint4*)part, kBkvPartBytes / 16);
+    return hipGetLastError();
+}
+
 hipError_t launch_bkv_reset(hipStream_t s, const BkvView& v, bool clear_data) {
     hipLaunchKernelGGL(vk_bkv_reset, dim3(256), dim3(256), 0, s, v);
     if (clear_data) {

@@ -9,7 +9,8 @@
 // Columns: the count_i * G query rows of an item that read one kv head.
 // vk_bkv_attn takes up to 32 of them over a range of keys; its four waves take
 // the range's units of 32 keys in turn, each with an online softmax of its own,
-// and merge through LDS at the end: no barrier in the key loop.
+// and merge through LDS at the end: no barrier in the key loop. A tile of 16
+// columns whose keys are split over workgroups is joined by the last of them.
 // vk_bkv_attn_chunk takes 128, 32 a wave, all waves over the same units, which
 // they widen to fp16 in LDS together (double buffered, one barrier a unit).
 // The 8-bit values are exact in fp16, so a product is two fp16 matrix
@@ -44,6 +45,7 @@ struct BkvAttnArgs {
     float* out;
     float* part;        // [slot][cols][2] (max, sum), then [slot][cols][hd] partial outputs
     size_t part_o;      // floats before the partial outputs
+    unsigned* joined;   // [tile][head] ranges that have written theirs, zero between calls
     float scale_log2;   // scale * log2(e)
     int layer, hq, g;   // g = hq / n_head
     uint32_t g_inv, splits_inv;  // ceil(2^32 / g), ceil(2^32 / splits): see bkv_div
@@ -152,6 +154,59 @@ __device__ __forceinline__ float bkv_max4(float v) {
 __device__ __forceinline__ float bkv_sum4(float v) {
     v += __int_as_float(vk_bfly_partner<16>(__float_as_int(v)));
     return v + __int_as_float(vk_bfly_partner<32>(__float_as_int(v)));
+}
+
+// A value that a workgroup on another XCD reads in this launch: past the caches
+// that are the XCD's own.
+__device__ __forceinline__ void bkv_put2(float* p, float a, float b) {
+    const unsigned long long v = ((unsigned long long)__float_as_uint(b) << 32) | __float_as_uint(a);
+    __hip_atomic_store((unsigned long long*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 bkv_get2(const float* p) {
+    const unsigned long long v =
+        __hip_atomic_load((const unsigned long long*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+
+// Values d .. d + 3 of a column from the partial results of its key ranges,
+// joined in the ranges' order, eight ranges' loads in flight. pm, po: the first
+// range's (max, sum) and outputs, cols columns a range. SAME: written by this launch.
+template <int HD, bool SAME>
+__device__ __forceinline__ vk_f32x4 bkv_join(const float* pm, const float* po, int ranges, int cols) {
+    constexpr int B = 8;
+    float m = -INFINITY, sum = 0.0f;
+    vk_f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < ranges; s += B) {
+        float2 ml[B];
+        vk_f32x4 o[B];
+#pragma unroll
+        for (int x = 0; x < B; ++x) {
+            const size_t at = (size_t)min(s + x, ranges - 1) * cols;
+            if constexpr (SAME) {
+                ml[x] = bkv_get2(pm + at * 2);
+                const float2 a = bkv_get2(po + at * HD), b = bkv_get2(po + at * HD + 2);
+                o[x] = vk_f32x4{a.x, a.y, b.x, b.y};
+            } else {
+                ml[x] = *(const float2*)(pm + at * 2);
+                o[x] = *(const vk_f32x4*)(po + at * HD);
+            }
+        }
+        float to = m;
+#pragma unroll
+        for (int x = 0; x < B; ++x) to = fmaxf(to, ml[x].x);
+        const float c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
+        sum *= c;
+        y *= c;
+        m = to;
+#pragma unroll
+        for (int x = 0; x < B; ++x) {
+            if (s + x >= ranges || (ml[x].x == -INFINITY && ml[x].y == 0.0f)) continue;
+            const float w = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml[x].x - m);
+            sum = fmaf(ml[x].y, w, sum);
+            y += o[x] * w;
+        }
+    }
+    return y * (1.0f / sum);
 }
 
 // One wave's query columns in blocks of 16 and what it has summed for them.
@@ -419,6 +474,7 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(BkvAt
     } sh;
     __shared__ float sqf[C * 16];  // q's factor of each column
     __shared__ float2 sml[kWaves][16];
+    __shared__ bool s_last;
     // ranges are the grid's slowest index: those that short items do not have come last
     const int tile = a.tile0 + (int)blockIdx.x, head = blockIdx.y, split = blockIdx.z;
     BkvTile t;
@@ -575,13 +631,44 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(BkvAt
 #pragma unroll
                     for (int i = 0; i < PD; ++i) y[i] = fmaf(sh.o[x][c][d0 + i], f, y[i]);
             }
-            float* dst = direct ? a.out + w.row(a, t, head, ct * 16 + c)
-                                : a.part + a.part_o + (slot * a.cols + ct * 16 + c) * HD;
-            const float f = direct ? 0x1p-14f / sum : 0x1p-14f;
-            if (!direct && d0 == 0) ((float2*)a.part)[slot * a.cols + ct * 16 + c] = make_float2(m, sum);
+            if (direct) {
+                float* dst = a.out + w.row(a, t, head, ct * 16 + c) + d0;
+                const float f = 0x1p-14f / sum;
 #pragma unroll
-            for (int i = 0; i < PD; ++i) dst[d0 + i] = y[i] * f;
+                for (int i = 0; i < PD; ++i) dst[i] = y[i] * f;
+            } else {
+                const size_t at = slot * a.cols + ct * 16 + c;
+                float *pm = a.part + at * 2, *po = a.part + a.part_o + at * HD + d0;
+                if constexpr (C == 1) {
+                    if (d0 == 0) bkv_put2(pm, m, sum);
+#pragma unroll
+                    for (int i = 0; i < PD; i += 2) bkv_put2(po + i, y[i] * 0x1p-14f, y[i + 1] * 0x1p-14f);
+                } else {
+                    if (d0 == 0) *(float2*)pm = make_float2(m, sum);
+#pragma unroll
+                    for (int i = 0; i < PD; ++i) po[i] = y[i] * 0x1p-14f;
+                }
+            }
         }
+    }
+    if (direct || C > 1) return;
+    // The tile's last workgroup to get here joins the ranges: each counts itself
+    // once its results have reached memory. All write before any waits, so the
+    // order in which they run does not matter, and nothing spins.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    const int ranges = (t.units + t.per - 1) / t.per;
+    unsigned* count = a.joined + (size_t)blockIdx.x * v.n_head + head;
+    if (threadIdx.x == 0) s_last = atomicAdd(count, 1u) == (unsigned)ranges - 1;
+    __syncthreads();
+    if (!s_last) return;
+    if (threadIdx.x == 0) atomicExch(count, 0u);
+    constexpr int PT = HD / 4;
+    const size_t first = (slot - split) * a.cols;
+    for (int c = threadIdx.x / PT; c < t.n; c += 64 * kWaves / PT) {
+        const int d = (threadIdx.x % PT) * 4;
+        *(vk_f32x4*)(a.out + w.row(a, t, head, c) + d) =
+            bkv_join<HD, true>(a.part + (first + c) * 2, a.part + a.part_o + (first + c) * HD + d, ranges, a.cols);
     }
 }
 
@@ -741,50 +828,22 @@ __global__ __launch_bounds__(256, 2) void vk_bkv_attn_chunk(BkvAttnArgs a, const
     }
 }
 
-// The key ranges of a column tile, merged in their order: HD / 4 threads a
-// column, eight ranges' loads in flight.
+// The key ranges of tiles of more than 16 columns (their own last workgroup would
+// take longer over them than a launch does): HD / 4 threads a column.
 template <int HD, bool CHUNKS>
-__global__ __launch_bounds__(256) void vk_bkv_attn_merge(BkvAttnArgs a, int tc) {
+__global__ __launch_bounds__(256) void vk_bkv_attn_merge(BkvAttnArgs a) {
     __shared__ int sh;
-    constexpr int PT = HD / 4, B = 8;
+    constexpr int PT = HD / 4;
     const int head = blockIdx.y;
     const int tile = CHUNKS ? a.tiles - 1 - (a.tile0 + (int)blockIdx.x) : a.tile0 + (int)blockIdx.x;
     BkvTile t;
-    if (!bkv_tile<CHUNKS>(a, tile, tc, &sh, t) || t.one()) return;
-    const int ranges = (t.units + t.per - 1) / t.per;
+    if (!bkv_tile<CHUNKS>(a, tile, kChunkCols, &sh, t) || t.one()) return;
     const int c = blockIdx.z * (256 / PT) + threadIdx.x / PT, d = (threadIdx.x % PT) * 4;
     if (c >= t.n) return;
-    const size_t slot = ((size_t)blockIdx.x * a.v.n_head + head) * a.splits;
-    const float2* pm = (const float2*)a.part + slot * a.cols + c;
-    const float* po = a.part + a.part_o + (slot * a.cols + c) * HD + d;
-    float m = -INFINITY, sum = 0.0f;
-    vk_f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < ranges; s += B) {
-        float2 ml[B];
-        vk_f32x4 o[B];
-#pragma unroll
-        for (int x = 0; x < B; ++x) {
-            const size_t at = (size_t)min(s + x, ranges - 1) * a.cols;
-            ml[x] = pm[at];
-            o[x] = *(const vk_f32x4*)(po + at * HD);
-        }
-        float to = m;
-#pragma unroll
-        for (int x = 0; x < B; ++x) to = fmaxf(to, ml[x].x);
-        const float c0 = m == -INFINITY ? 0.0f : exp2f(m - to);
-        sum *= c0;
-        y *= c0;
-        m = to;
-#pragma unroll
-        for (int x = 0; x < B; ++x) {
-            if (s + x >= ranges || (ml[x].x == -INFINITY && ml[x].y == 0.0f)) continue;
-            const float w = m == -INFINITY ? 1.0f : exp2f(ml[x].x - m);
-            sum = fmaf(ml[x].y, w, sum);
-            y += o[x] * w;
-        }
-    }
+    const size_t first = ((size_t)blockIdx.x * a.v.n_head + head) * a.splits * a.cols + c;
     const int cc = t.c0 + c, j = CHUNKS ? cc / a.g : bkv_div(cc, a.g_inv);
-    *(vk_f32x4*)(a.out + ((size_t)(t.it.row0 + j) * a.hq + head * a.g + (cc - j * a.g)) * HD + d) = y * (1.0f / sum);
+    *(vk_f32x4*)(a.out + ((size_t)(t.it.row0 + j) * a.hq + head * a.g + (cc - j * a.g)) * HD + d) =
+        bkv_join<HD, false>(a.part + first * 2, a.part + a.part_o + first * HD + d, (t.units + t.per - 1) / t.per, a.cols);
 }
 
 template <int HD, int CODEC>
@@ -802,9 +861,10 @@ static void go_hd(hipStream_t s, const BkvAttnArgs& a, int tc, unsigned tiles) {
     if (a.v.codec == BKV_INT8) go_attn<HD, BKV_INT8>(s, a, tc, grid);
     else go_attn<HD, BKV_E4M3>(s, a, tc, grid);
     constexpr unsigned CW = 256 / (HD / 4);  // columns a merging workgroup
+    if (a.splits == 1 || tc == 16) return;
     const dim3 cols(tiles, (unsigned)a.v.n_head, ((unsigned)a.cols + CW - 1) / CW);
-    if (a.splits > 1 && a.chunks) hipLaunchKernelGGL((vk_bkv_attn_merge<HD, true>), cols, dim3(256), 0, s, a, tc);
-    else if (a.splits > 1) hipLaunchKernelGGL((vk_bkv_attn_merge<HD, false>), cols, dim3(256), 0, s, a, tc);
+    if (a.chunks) hipLaunchKernelGGL((vk_bkv_attn_merge<HD, true>), cols, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((vk_bkv_attn_merge<HD, false>), cols, dim3(256), 0, s, a);
 }
 
 hipError_t launch_bkv_attn(hipStream_t s, const BkvView& v, int layer, int n, int n_rows, int max_count, int max_len,
@@ -836,6 +896,7 @@ hipError_t launch_bkv_attn(hipStream_t s, const BkvView& v, int layer, int n, in
     a.per = (int)((std::max(per, (units + most - 1) / most) + 3) / 4 * 4);
     a.splits = (units + a.per - 1) / a.per;
     a.part_o = (size_t)room * 2;
+    a.joined = (unsigned*)(part + (size_t)room * (128 + 2));
     auto inv = [](int d) { return d == 1 ? 0u : (uint32_t)(((1ull << 32) + (uint32_t)d - 1) / (uint32_t)d); };
     a.g_inv = inv(a.g);
     a.splits_inv = inv(a.splits);

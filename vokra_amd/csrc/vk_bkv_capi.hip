@@ -176,7 +176,7 @@ int vokra_hip_bkv_create(vokra_hip_ctx_t* c, size_t n_layer, size_t n_head, size
                              "max_time <= 2^24, n_page <= 2^26, max_rows <= 2^20)");
     BK_TRY(hipSetDevice(vk::ctx_device(c)), "hipSetDevice");
     void* part = nullptr;
-    BK_ST(vk::ctx_bkv_part(c, (size_t)kBkvParts * (128 + 2) * sizeof(float), &part));
+    BK_ST(vk::ctx_bkv_part(c, &part));
     auto* kv = new (std::nothrow) vokra_hip_bkv();
     if (!kv) return ctx_fail(VOKRA_HIP_ERROR_OTHER, "bkv_create: out of host memory");
     kv->ctx = c;

@@ -18,6 +18,7 @@
 #include <vector>
 
 #include "../../include/vokra_hip.h"
+#include "vk_bkv.h"
 #include "vk_launch.h"
 #include "vk_step.h"
 
@@ -601,22 +602,25 @@ int check_paged_attn(const vokra_hip_kv* kv, size_t layer, size_t n, size_t hq) 
 namespace vk {
 hipStream_t ctx_stream(const vokra_hip_ctx* c) { return c->stream; }
 int ctx_device(const vokra_hip_ctx* c) { return c->device; }
-int ctx_bkv_part(vokra_hip_ctx* c, size_t bytes, void** p) {
-    VK_TRY(c->bk_part.ensure(bytes), "hipMalloc(partial attention)");
-    *p = c->bk_part.p;
-    return VOKRA_HIP_OK;
-}
-int ctx_rules_part(vokra_hip_ctx* c, size_t bytes, void** p) {
-    if (!c->ru_part.p) {
-        VK_TRY(c->ru_part.ensure(bytes), "hipMalloc(logits rules)");
-        hipError_t e = launch_rules_clear(c->stream, c->ru_part.p);
+// A workspace of the context that is zero when a call finds it: allocated and
+// cleared at its first use, never replaced.
+static int clean_part(vokra_hip_ctx* c, DevBuf& b, size_t bytes, hipError_t (*clear)(hipStream_t, void*), void** p) {
+    if (!b.p) {
+        VK_TRY(b.ensure(bytes), "hipMalloc(workspace)");
+        hipError_t e = clear(c->stream, b.p);
         if (e != hipSuccess) {
-            c->ru_part.release();
-            return hip_fail(e, "launch(vk_rules_clear)");
+            b.release();
+            return hip_fail(e, "launch(workspace)");
         }
     }
-    *p = c->ru_part.p;
+    *p = b.p;
     return VOKRA_HIP_OK;
+}
+int ctx_bkv_part(vokra_hip_ctx* c, void** p) {
+    return clean_part(c, c->bk_part, kBkvPartBytes, launch_bkv_part_clear, p);
+}
+int ctx_rules_part(vokra_hip_ctx* c, void** p) {
+    return clean_part(c, c->ru_part, kRulesPartBytes, launch_rules_clear, p);
 }
 
 // Drains the context stream and turns a raised fp16-range flag of the

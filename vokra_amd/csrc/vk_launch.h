@@ -333,9 +333,9 @@ namespace vk {
 hipStream_t ctx_stream(const vokra_hip_ctx* c);
 int ctx_device(const vokra_hip_ctx* c);
 // The context's workspace of the logits rules: allocated at the first call, never replaced.
-int ctx_rules_part(vokra_hip_ctx* c, size_t bytes, void** p);
+int ctx_rules_part(vokra_hip_ctx* c, void** p);
 // The same for the partial results of the block caches' attention (first cache).
-int ctx_bkv_part(vokra_hip_ctx* c, size_t bytes, void** p);
+int ctx_bkv_part(vokra_hip_ctx* c, void** p);
 int range_check(vokra_hip_ctx* c);  // INVALID_ARGUMENT when an fp16-range flag is raised
 int ctx_fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 // Fused forms of entry-point sequences for the sessions (vk_capi.hip); each

@@ -288,7 +288,7 @@ int vokra_hip_logits_rules_dev(vokra_hip_ctx_t* c, size_t rows, size_t vocab, si
     a.mask_stride = rules->mask_stride;
     if (d_next) {
         void* p = nullptr;
-        ST_ST(vk::ctx_rules_part(c, kRulesPartBytes, &p));
+        ST_ST(vk::ctx_rules_part(c, &p));
         a.best = (unsigned long long*)p;
         a.done = (unsigned*)(a.best + kRulesRows);
     }
