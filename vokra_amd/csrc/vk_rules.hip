@@ -7,11 +7,16 @@
 //   v not allowed by the mask: x = -inf;
 // then the first largest x above -inf (a NaN never is), -1 if there is none.
 //
-// A workgroup takes 4096 columns of a row, from a 16-byte boundary on: it loads
-// them, gathers the counts of the history's tokens in them (integer adds, so
-// their order does not matter) and the last bias entry of each (integer max) in
-// LDS meanwhile, and writes each column once. Bound by those 8 bytes a column;
-// a long history is read by every workgroup of its row (from cache).
+// A workgroup takes 4096 or 8192 columns of a row, from a 16-byte boundary on,
+// into registers. One table in LDS, a number a column, first counts the history's
+// tokens in them (integer adds, so their order does not matter) and then holds
+// the last bias entry of each (integer max); each list is read by every workgroup
+// of its row, from cache, and skipped where a row has none. Each column is
+// written once. Bound by those 8 bytes a column: 192 rows of 128259 columns with up
+// to 2048 tokens and 300 biases a row take 54 us (3.7 TB/s), 48 of them with the
+// lists left out; 32 rows of 32000 columns take 8.8 us, which is dependent rounds
+// of memory. Two tables at once, filled between the same barriers, took 69 us: 33 KB
+// of LDS leave half the waves.
 // The choice: each workgroup's best goes into the row's 64-bit maximum (value,
 // then the lower index: the order of the workgroups does not matter), and the
 // last of the row's workgroups writes it out and clears it for the next call.
@@ -20,7 +25,7 @@
 
 namespace vk {
 
-constexpr int RU_SLICE = 4096;
+constexpr int RU_T = 512;  // threads
 
 // (value desc, index asc): the first strict maximum
 __device__ __forceinline__ void ru_merge(float& v, int& i, float w, int j) {
@@ -30,26 +35,28 @@ __device__ __forceinline__ void ru_merge(float& v, int& i, float w, int j) {
     }
 }
 
-__global__ __launch_bounds__(256) void vk_rules(RulesArgs a) {
-    __shared__ int4 count4[RU_SLICE / 4], slot4[RU_SLICE / 4];
-    __shared__ float rv[4];
-    __shared__ int ri[4];
-    int *count = (int*)count4, *slot = (int*)slot4;
+// RU_VEC: 16-byte pieces a thread
+template <int RU_VEC>
+__global__ __launch_bounds__(RU_T) void vk_rules(RulesArgs a) {
+    constexpr int RU_SLICE = 4 * RU_T * RU_VEC;
+    __shared__ int4 table4[RU_SLICE / 4];
+    __shared__ float rv[RU_T / 64];
+    __shared__ int ri[RU_T / 64];
+    int* table = (int*)table4;
     const int row = blockIdx.y, t = threadIdx.x;
     const float* x = a.logits + (size_t)row * a.stride;
     // column c0 + 4 k lies on a 16-byte boundary of the row
     const int c0 = (int)blockIdx.x * RU_SLICE - (int)((reinterpret_cast<uintptr_t>(x) >> 2) & 3);
-    float4 y[4];
+    float y[4 * RU_VEC];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int c = c0 + 4 * (t + 256 * j);
+    for (int j = 0; j < RU_VEC; ++j) {
+        const int c = c0 + 4 * (t + RU_T * j);
         if (c >= 0 && c + 3 < a.vocab) {
-            y[j] = *(const float4*)(x + c);
+            const float4 x4 = *(const float4*)(x + c);
+            y[4 * j] = x4.x, y[4 * j + 1] = x4.y, y[4 * j + 2] = x4.z, y[4 * j + 3] = x4.w;
         } else {
-            float z[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) z[i] = c + i >= 0 && c + i < a.vocab ? x[c + i] : 0.0f;
-            y[j] = make_float4(z[0], z[1], z[2], z[3]);
+            for (int i = 0; i < 4; ++i) y[4 * j + i] = c + i >= 0 && c + i < a.vocab ? x[c + i] : 0.0f;
         }
     }
     const bool hist = a.hist_off, biased = a.bias_off;
@@ -57,30 +64,57 @@ __global__ __launch_bounds__(256) void vk_rules(RulesArgs a) {
     const int b0 = biased ? max(a.bias_off[row], 0) : 0, b1 = biased ? min(a.bias_off[row + 1], a.n_bias) : 0;
     const float rep = a.repetition ? a.repetition[row] : 1.0f, pres = a.presence ? a.presence[row] : 0.0f,
                 freq = a.frequency ? a.frequency[row] : 0.0f;
-    const bool listed = h1 > h0 || b1 > b0;
-    if (listed) {
+    const int lo = max(c0, 0), hi = min(c0 + RU_SLICE, a.vocab);
+    int4* mine = table4 + t;  // + RU_T j: this thread's columns
+    if (h1 > h0 || b1 > b0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) count4[t + 256 * j] = slot4[t + 256 * j] = make_int4(0, 0, 0, 0);
+        for (int j = 0; j < RU_VEC; ++j) mine[RU_T * j] = make_int4(0, 0, 0, 0);
         __syncthreads();
-        const int lo = max(c0, 0), hi = min(c0 + RU_SLICE, a.vocab);
-        // eight (two) loads in flight
-        for (int i = h0 + t; i < h1; i += 8 * 256) {
-            int v[8];
+    }
+    if (h1 > h0) {
+        for (int i = h0 + t; i < h1; i += 8 * RU_T) {
+            int v[8];  // loads in flight
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = i + 256 * j < h1 ? a.hist[i + 256 * j] : -1;
+            for (int j = 0; j < 8; ++j) v[j] = i + RU_T * j < h1 ? a.hist[i + RU_T * j] : -1;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (v[j] >= lo && v[j] < hi) atomicAdd(&count[v[j] - c0], 1);
-        }
-        for (int i = b0 + t; i < b1; i += 2 * 256) {
-            int v[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) v[j] = i + 256 * j < b1 ? a.bias_ids[i + 256 * j] : -1;
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (v[j] >= lo && v[j] < hi) atomicMax(&slot[v[j] - c0], i + 256 * j - b0 + 1);
+                if (v[j] >= lo && v[j] < hi) atomicAdd(&table[v[j] - c0], 1);
         }
         __syncthreads();
+#pragma unroll
+        for (int j = 0; j < RU_VEC; ++j) {
+            const int4 k4 = mine[RU_T * j];
+            if (!(k4.x | k4.y | k4.z | k4.w)) continue;
+            float* z = &y[4 * j];
+            const int k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (k[i]) {
+                    z[i] = z[i] > 0.0f ? z[i] / rep : z[i] * rep;
+                    z[i] = z[i] - (pres + freq * (float)k[i]);
+                }
+            mine[RU_T * j] = make_int4(0, 0, 0, 0);
+        }
+    }
+    if (b1 > b0) {
+        if (h1 > h0) __syncthreads();
+        for (int i = b0 + t; i < b1; i += 2 * RU_T) {
+            int v[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) v[j] = i + RU_T * j < b1 ? a.bias_ids[i + RU_T * j] : -1;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (v[j] >= lo && v[j] < hi) atomicMax(&table[v[j] - c0], i + RU_T * j - b0 + 1);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < RU_VEC; ++j) {
+            const int4 s4 = mine[RU_T * j];
+            const int s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (s[i]) y[4 * j + i] = y[4 * j + i] + a.bias[b0 + s[i] - 1];
+        }
     }
     const uint32_t* mask = a.mask ? a.mask + (size_t)row * a.mask_stride : nullptr;
     float* out = a.out ? a.out + (size_t)row * a.stride : nullptr;
@@ -88,21 +122,9 @@ __global__ __launch_bounds__(256) void vk_rules(RulesArgs a) {
     float bv = -INFINITY;
     int bi = INT_MAX;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int g = t + 256 * j, c = c0 + 4 * g;
-        float z[4] = {y[j].x, y[j].y, y[j].z, y[j].w};
-        if (listed) {
-            const int4 k4 = count4[g], s4 = slot4[g];
-            const int k[4] = {k4.x, k4.y, k4.z, k4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (k[i]) {
-                    z[i] = z[i] > 0.0f ? z[i] / rep : z[i] * rep;
-                    z[i] = z[i] - (pres + freq * (float)k[i]);
-                }
-                if (s[i]) z[i] = z[i] + a.bias[b0 + s[i] - 1];
-            }
-        }
+    for (int j = 0; j < RU_VEC; ++j) {
+        const int c = c0 + 4 * (t + RU_T * j);
+        float* z = &y[4 * j];
         if (mask) {
             // the four bits lie in one word or two
             const int w0 = max(c, 0) >> 5, w1 = min(max(c + 3, 0), a.vocab - 1) >> 5;
@@ -147,7 +169,7 @@ __global__ __launch_bounds__(256) void vk_rules(RulesArgs a) {
     }
     __syncthreads();
     if (t != 0) return;
-    for (int w = 1; w < 4; ++w) ru_merge(bv, bi, rv[w], ri[w]);
+    for (int w = 1; w < RU_T / 64; ++w) ru_merge(bv, bi, rv[w], ri[w]);
     // the value's bits in the order of the values, above the lower index first; 0: nothing
     if (bv == 0.0f) bv = 0.0f;  // one zero
     const uint32_t b = __float_as_uint(bv), ord = b & 0x80000000u ? ~b : b | 0x80000000u;
@@ -174,10 +196,23 @@ hipError_t launch_rules_clear(hipStream_t s, void* part) {
     return hipGetLastError();
 }
 
-hipError_t launch_rules(hipStream_t s, const RulesArgs& a) {
+template <int RU_VEC>
+static void rules_grid(hipStream_t s, const RulesArgs& a) {
+    constexpr int slice = 4 * RU_T * RU_VEC;
     // a row may begin up to three columns before a boundary
-    hipLaunchKernelGGL(vk_rules, dim3((unsigned)((a.vocab + 3 + RU_SLICE - 1) / RU_SLICE), (unsigned)a.rows), dim3(256),
-                       0, s, a);
+    hipLaunchKernelGGL(vk_rules<RU_VEC>, dim3((unsigned)((a.vocab + 3 + slice - 1) / slice), (unsigned)a.rows),
+                       dim3(RU_T), 0, s, a);
+}
+
+hipError_t launch_rules(hipStream_t s, const RulesArgs& a) {
+    // up to two workgroups of 4096 columns a CU, half the columns a thread end
+    // earlier (32 rows of 32000 columns: 8.8 us against 9.8); above that, whole
+    // slices halve the reads of the rows' lists (64 rows of 51866 columns: 11.2 us
+    // against 12.5, 192 of 128259: 54 against 65)
+    if ((size_t)a.rows * a.vocab <= (size_t)512 * 4096)
+        rules_grid<2>(s, a);
+    else
+        rules_grid<4>(s, a);
     return hipGetLastError();
 }
 
