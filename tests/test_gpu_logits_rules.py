@@ -51,7 +51,7 @@ def same(got, want):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 31), (2, 32), (2, 33), (5, 1000), (1, 4096), (2, 4097), (7, 51866),
-                                        (33, 8191), (2, 130001)])
+                                        (33, 8191), (2, 130001), (41, 51866)])
 def test_every_rule_at_once_and_alone(ctx, rows, vocab):
     print("[case] rules", rows, vocab, flush=True)
     g = np.random.default_rng(vocab)
