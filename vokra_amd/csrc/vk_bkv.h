@@ -10,8 +10,10 @@
 
 constexpr int kBkvMaxItems = 1024;   // items of one call: one thread of the planning workgroup each
 constexpr int kBkvParts = 1 << 18;  // query rows of which a split attention can hold a partial result
-// a context's partial results ((max, sum) and up to 128 values a row) and counters
-constexpr size_t kBkvPartBytes = (size_t)kBkvParts * (128 + 2 + 1) * 4;
+constexpr int kBkvShares = 512;  // workgroups that share a chunked attention: two a CU
+// a context's partial results ((max, sum) and up to 128 values a row), counters,
+// and the tiles that go on in a later share
+constexpr size_t kBkvPartBytes = (size_t)kBkvParts * (128 + 2 + 1) * 4 + kBkvShares * 16;
 
 // What planning kernels leave for the kernels of the same call or step.
 // meta (int32): see the BKV_ indices.

@@ -39,6 +39,11 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef float float2v __attribute__((ext_vector_type(2)));
 
+// A tile of vk_bkv_attn_chunk whose keys several shares of the work have.
+struct alignas(16) BkvOpen {
+    int item, tile, head, pieces;  // pieces 0: none
+};
+
 struct BkvAttnArgs {
     BkvView v;
     const float* q;
@@ -49,10 +54,10 @@ struct BkvAttnArgs {
     float scale_log2;   // scale * log2(e)
     int layer, hq, g;   // g = hq / n_head
     uint32_t g_inv, splits_inv;  // ceil(2^32 / g), ceil(2^32 / splits): see bkv_div
-    int tile0;          // first column tile of this launch
-    int tiles;          // column tiles of the call
-    int chunks;         // 0: one column tile an item; 1: as many as its columns need
-    int splits;         // key ranges a column tile may have (grid)
+    BkvOpen* open;      // of each share: the tile whose first piece is its last
+    int tile0;          // first item of this launch
+    int tiles;          // chunks: places of tiles, see bkv_share
+    int splits;         // key ranges an item may have (grid)
     int per;            // least units of a key range
     int cols;           // columns a slot has room for
 };
@@ -65,7 +70,7 @@ struct BkvTile {
     int c0, n;      // first column, columns
     int keys;       // keys that its last row sees
     int full;       // keys in full blocks, no more than keys rounded up to a tile
-    int units, per; // units of the 8-bit part, units a key range
+    int units, per; // units of the 8-bit part, units a key range (vk_bkv_attn)
     __device__ __forceinline__ bool one() const { return per >= units; }               // one key range
     __device__ __forceinline__ bool beyond(int s) const { return s && s * per >= units; }  // no range s
     __device__ __forceinline__ bool final(int s) const { return (s + 1) * per >= units; }  // the last range
@@ -74,40 +79,33 @@ struct BkvTile {
 // x / d for inv = ceil(2^32 / d): exact while x (d - 1) < 2^32
 __device__ __forceinline__ int bkv_div(int x, uint32_t inv) { return inv ? (int)__umulhi((uint32_t)x, inv) : x; }
 
-// Tile T of the launch's order: item T, or (CHUNKS) the item whose tiles T is one
-// of: item i's begin at row0_i * g / tc + i (room for a partly filled tile each).
-// Every thread returns the same; false: no such tile. sh: one int of LDS.
-template <bool CHUNKS>
-__device__ __forceinline__ bool bkv_tile(const BkvAttnArgs& a, int tile, int tc, int* sh, BkvTile& t) {
-    const int bs_log = 31 - __clz(a.v.bs);
-    if constexpr (CHUNKS) {
-        const int n = a.v.meta[BKV_STEP_N];
-        if (threadIdx.x == 0) *sh = -1;
-        __syncthreads();
-        for (int x = threadIdx.x; x < n; x += blockDim.x) {
-            const BkvItem it = a.v.step[x];
-            const long long lo = (long long)it.row0 * a.g / tc + x;
-            const long long hi = (long long)(it.row0 + it.count) * a.g / tc + x + 1;
-            if (tile >= lo && tile < hi) *sh = x;
-        }
-        __syncthreads();
-        const int i = *sh;
-        if (i < 0) return false;
-        t.it = a.v.step[i];
-        t.c0 = (tile - (int)((long long)t.it.row0 * a.g / tc + i)) * tc;
-        t.n = min(tc, t.it.count * a.g - t.c0);
-        if (t.n <= 0) return false;
-        t.keys = t.it.start + (t.c0 + t.n - 1) / a.g + 1;
-    } else {
-        t.it = a.v.step[tile];
-        t.c0 = 0;
-        t.n = t.it.count * a.g;
-        if (t.n <= 0) return false;
-        t.keys = t.it.start + t.it.count;
-    }
+__device__ __forceinline__ void bkv_keys(const BkvView& v, BkvTile& t) {
+    const int bs_log = 31 - __clz(v.bs);
     t.full = min((t.it.start + t.it.count) >> bs_log << bs_log, (t.keys + 15) & ~15);
     t.units = (t.full + kUnit - 1) / kUnit;
+}
+// All columns of an item (vk_bkv_attn); false: none.
+__device__ __forceinline__ bool bkv_tile(const BkvAttnArgs& a, int item, BkvTile& t) {
+    t.it = a.v.step[item];
+    t.c0 = 0;
+    t.n = t.it.count * a.g;
+    if (t.n <= 0) return false;
+    t.keys = t.it.start + t.it.count;
+    bkv_keys(a.v, t);
     t.per = max(a.per, (bkv_div(t.units + a.splits - 1, a.splits_inv) + 3) & ~3);
+    return true;
+}
+
+constexpr int kChunkCols = 128;  // columns of a tile of vk_bkv_attn_chunk
+
+// Columns kChunkCols * tile .. of an item; false: it has none there.
+__device__ __forceinline__ bool bkv_chunk(const BkvAttnArgs& a, const BkvItem& it, int tile, BkvTile& t) {
+    t.it = it;
+    t.c0 = tile * kChunkCols;
+    t.n = min(kChunkCols, it.count * a.g - t.c0);
+    if (t.n <= 0) return false;
+    t.keys = it.start + (t.c0 + t.n - 1) / a.g + 1;
+    bkv_keys(a.v, t);
     return true;
 }
 
@@ -170,9 +168,11 @@ __device__ __forceinline__ float2 bkv_get2(const float* p) {
 
 // Values d .. d + 3 of a column from the partial results of its key ranges,
 // joined in the ranges' order, eight ranges' loads in flight. pm, po: the first
-// range's (max, sum) and outputs, cols columns a range. SAME: written by this launch.
+// range's (max, sum) and outputs, cols columns a slot; range s > 0 is s * step - back
+// slots behind. SAME: written by this launch.
 template <int HD, bool SAME>
-__device__ __forceinline__ vk_f32x4 bkv_join(const float* pm, const float* po, int ranges, int cols) {
+__device__ __forceinline__ vk_f32x4 bkv_join(const float* pm, const float* po, int ranges, int cols, int step,
+                                              int back) {
     constexpr int B = 8;
     float m = -INFINITY, sum = 0.0f;
     vk_f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -181,7 +181,8 @@ __device__ __forceinline__ vk_f32x4 bkv_join(const float* pm, const float* po, i
         vk_f32x4 o[B];
 #pragma unroll
         for (int x = 0; x < B; ++x) {
-            const size_t at = (size_t)min(s + x, ranges - 1) * cols;
+            const int r = min(s + x, ranges - 1);
+            const size_t at = r ? (size_t)(r * step - back) * cols : 0;
             if constexpr (SAME) {
                 ml[x] = bkv_get2(pm + at * 2);
                 const float2 a = bkv_get2(po + at * HD), b = bkv_get2(po + at * HD + 2);
@@ -478,7 +479,7 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(BkvAt
     // ranges are the grid's slowest index: those that short items do not have come last
     const int tile = a.tile0 + (int)blockIdx.x, head = blockIdx.y, split = blockIdx.z;
     BkvTile t;
-    if (!bkv_tile<false>(a, tile, 16 * C, nullptr, t) || t.beyond(split)) return;
+    if (!bkv_tile(a, tile, t) || t.beyond(split)) return;
     const BkvView& v = a.v;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int bs_log = 31 - __clz(v.bs);
@@ -668,11 +669,105 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(BkvAt
     for (int c = threadIdx.x / PT; c < t.n; c += 64 * kWaves / PT) {
         const int d = (threadIdx.x % PT) * 4;
         *(vk_f32x4*)(a.out + w.row(a, t, head, c) + d) =
-            bkv_join<HD, true>(a.part + (first + c) * 2, a.part + a.part_o + (first + c) * HD + d, ranges, a.cols);
+            bkv_join<HD, true>(a.part + (first + c) * 2, a.part + a.part_o + (first + c) * HD + d, ranges, a.cols,
+                               1, 0);
     }
 }
 
-constexpr int kChunkCols = 128;  // columns of a workgroup of the kernel below
+// ---- chunks ----------------------------------------------------------------------
+// The call's work is one line of (head, item, tile, unit), kTileCost units more a
+// tile for its start and its open block's rows. Every workgroup takes an even share
+// of the line, so all end together whatever the lengths are; a share holds whole
+// tiles and at most two pieces, one at each end, whose results are joined by the
+// kernel below. (One workgroup for each key range of each tile left 40 % of the
+// waves' places empty at six chunks of 450 .. 1030 rows over up to 4500 keys, and
+// finer ranges cost more to join than they gave: 264 us; shares: FIGURE.)
+
+constexpr int kLeast = 8, kTileCost = 5;
+
+struct BkvShare {
+    long long begin, end;       // on the line
+    int size, index;            // of every share; of this one
+    int item, tile, head, at;   // where it begins
+};
+
+// The share of workgroup w, the same on all threads; false: sh.index has none. The places of tiles: item i's
+// begin at row0_i * g / kChunkCols + i (room for a partly filled tile each). lds:
+// kBkvMaxItems ints and 16 more.
+__device__ __forceinline__ bool bkv_share(const BkvAttnArgs& a, int w, int* lds, BkvShare& sh) {
+    const int n = a.v.meta[BKV_STEP_N], t = threadIdx.x;
+    int* first = lds;
+    long long* sums = (long long*)(lds + kBkvMaxItems);
+    for (int x = t; x < n; x += 256) first[x] = (int)((long long)a.v.step[x].row0 * a.g / kChunkCols) + x;
+    __syncthreads();
+    // this thread's places, and the first one's item
+    const int m = (a.tiles + 255) / 256, p0 = t * m, p1 = min(p0 + m, a.tiles);
+    int lo = 0, hi = n;  // the last item that begins at or before p0
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first[mid] <= p0) lo = mid;
+        else hi = mid;
+    }
+    // calls f(item, tile, cost) for each tile until it returns true
+    auto walk = [&](auto f) {
+        if (n == 0) return;
+        int i = lo;
+        BkvItem it = a.v.step[i];
+        for (int p = p0; p < p1; ++p) {
+            while (i + 1 < n && first[i + 1] <= p) it = a.v.step[++i];
+            BkvTile x;
+            if (bkv_chunk(a, it, p - first[i], x) && f(i, p - first[i], x.units + kTileCost)) return;
+        }
+    };
+    long long mine = 0;
+    walk([&](int, int, int cost) {
+        mine += cost;
+        return false;
+    });
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const long long x = __shfl_up(upto, o, 64);
+        if ((t & 63) >= o) upto += x;
+    }
+    if ((t & 63) == 63) sums[t >> 6] = upto;
+    __syncthreads();
+    long long one = 0;  // a head's
+    for (int x = 0; x < 4; ++x) {
+        if (x < t >> 6) upto += sums[x];
+        one += sums[x];
+    }
+    const long long all = one * a.v.n_head;
+    sh.size = (int)max((all + kBkvShares - 1) / kBkvShares, (long long)kLeast);
+    const int shares = (int)((all + sh.size - 1) / sh.size);
+    // neighbours on one XCD (they read the same keys)
+    const int per = (shares + 7) / 8;
+    sh.index = (w >> 3) < per ? (w & 7) * per + (w >> 3) : w;
+    if (sh.index >= shares) return false;
+    sh.begin = (long long)sh.index * sh.size;
+    sh.end = min(sh.begin + sh.size, all);
+    sh.head = (int)(sh.begin / one);
+    const long long off = sh.begin - sh.head * one;
+    int* found = (int*)(sums + 4);
+    if (off >= upto - mine && off < upto) {
+        long long at = upto - mine;
+        walk([&](int i, int tile, int cost) {
+            if (off < at + cost) {
+                found[0] = i;
+                found[1] = tile;
+                found[2] = (int)(off - at);
+                return true;
+            }
+            at += cost;
+            return false;
+        });
+    }
+    __syncthreads();
+    sh.item = __builtin_amdgcn_readfirstlane(found[0]);
+    sh.tile = __builtin_amdgcn_readfirstlane(found[1]);
+    sh.at = __builtin_amdgcn_readfirstlane(found[2]);
+    return true;
+}
 
 template <int HD, int CODEC>
 __global__ __launch_bounds__(256, 2) void vk_bkv_attn_chunk(BkvAttnArgs a, const uint8_t* __restrict__ pool,
@@ -681,169 +776,214 @@ __global__ __launch_bounds__(256, 2) void vk_bkv_attn_chunk(BkvAttnArgs a, const
     using W = BkvWave<HD, C, true>;
     constexpr int U = W::U, DT = W::DT;
     __shared__ uint4 kv[2][8 * U * 64];  // a unit's fragments: K [tile][k step], then V [d tile]
-    __shared__ int sh;
-    // later rows see more keys: they start first
-    const int tile = a.tiles - 1 - (a.tile0 + (int)blockIdx.x), head = blockIdx.y, split = blockIdx.z;
-    BkvTile t;
-    if (!bkv_tile<true>(a, tile, kChunkCols, &sh, t) || t.beyond(split)) return;
+    static_assert(sizeof(kv) >= (kBkvMaxItems + 16) * sizeof(int), "bkv_share");
+    BkvShare sh;
+    if (!bkv_share(a, blockIdx.x, (int*)kv, sh)) {
+        if (threadIdx.x == 0) a.open[sh.index].pieces = 0;
+        return;
+    }
+    __syncthreads();
     const BkvView& v = a.v;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int bs_log = 31 - __clz(v.bs), c0 = wave * 32;
     W w;
     w.col = lane & 15;
     w.grp = lane >> 4;
-    const int u0 = split * t.per, u1 = min(t.units, (split + 1) * t.per);
-    const int* table = v.table + (size_t)t.it.seq * v.max_blocks;
-    // lane l holds the page of tile l of the units k0 .. k0 + 31 of the range
-    auto pages_from = [&](int k0) {
-        const int key = min((u0 + k0) * kUnit + lane * 16, t.full - 16);
-        return table[key >> bs_log];
-    };
-    int pages = u0 < u1 ? pages_from(0) : 0;
-    const BkvPlace place(v, a.layer, head, pool, scales);
-    // wave's 1 KB pieces of a unit: U = 2: K's and V's piece (tile wave / 2, half
-    // wave % 2); U = 1: waves 0, 1 K's tiles, 2, 3 V's
-    uint4 raw[U];
-    float2 sc[2], sc_next[2];
-    auto load = [&](int k) {
-        if (k > 0 && (k & 31) == 0) pages = pages_from(k);
-        const int u = u0 + k, xw = U == 2 ? wave >> 1 : wave & 1;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const int page = __builtin_amdgcn_readlane(pages, 2 * (k & 31) + x);
-            sc_next[x] = place.scale(page);
-            if (x == xw) {
-                const uint8_t* p = place.tile(page, min(u * kUnit + x * 16, t.full - 16), v.bs, HD);
-                if constexpr (U == 2) {
-                    p += (wave & 1) * 1024;
-                    raw[0] = ((const uint4*)p)[lane];
-                    raw[1] = ((const uint4*)(p + v.bs * HD))[lane];
-                } else {
-                    raw[0] = ((const uint4*)(p + (wave >> 1) * v.bs * HD))[lane];
-                }
+    int item = sh.item, head = sh.head, tile = sh.tile, at = sh.at;
+    int left = (int)(sh.end - sh.begin);
+    BkvOpen open = {0, 0, 0, 0};
+    BkvItem it = v.step[item];
+    for (bool begin = true; left > 0; begin = false) {
+        BkvTile t;
+        if (!bkv_chunk(a, it, tile, t)) {  // the next item, or the next head
+            tile = 0;
+            if (++item == v.meta[BKV_STEP_N]) {
+                item = 0;
+                ++head;
             }
+            it = v.step[item];
+            continue;
         }
-    };
-    auto widen_k = [&](uint4* b, const uint4& r, int x, int i) {
-        b[(x * 2 * U + 2 * i) * 64 + lane] = __builtin_bit_cast(uint4, bkv_widen8<CODEC>(r.x, r.y));
-        b[(x * 2 * U + 2 * i + 1) * 64 + lane] = __builtin_bit_cast(uint4, bkv_widen8<CODEC>(r.z, r.w));
-    };
-    auto widen_v = [&](uint4* b, const uint4& r, int x, int i) {
+        const int cost = t.units + kTileCost, to = min(cost, at + left);
+        const int u0 = min(at, t.units), u1 = min(to, t.units);
+        const bool last = to == cost, whole = last && at == 0;
+        const int* table = v.table + (size_t)t.it.seq * v.max_blocks;
+        // lane l holds the page of tile l of the units k0 .. k0 + 31 of the range
+        auto pages_from = [&](int k0) {
+            const int key = min((u0 + k0) * kUnit + lane * 16, t.full - 16);
+            return table[key >> bs_log];
+        };
+        int pages = u0 < u1 ? pages_from(0) : 0;
+        const BkvPlace place(v, a.layer, head, pool, scales);
+        // wave's 1 KB pieces of a unit: U = 2: K's and V's piece (tile wave / 2, half
+        // wave % 2); U = 1: waves 0, 1 K's tiles, 2, 3 V's
+        uint4 raw[U];
+        float2 sc[2], sc_next[2];
+        auto load = [&](int k) {
+            if (k > 0 && (k & 31) == 0) pages = pages_from(k);
+            const int u = u0 + k, xw = U == 2 ? wave >> 1 : wave & 1;
 #pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            half2v p, q;
-            bkv_widen<CODEC>(u4c(r, d), p, q);
-            ((uint2*)&b[(4 * U + 4 * i + d) * 64 + lane])[x] =
-                make_uint2(__builtin_bit_cast(uint32_t, p), __builtin_bit_cast(uint32_t, q));
-        }
-    };
-    auto widen = [&](int buf) {
-        if constexpr (U == 2) {
-            widen_k(kv[buf], raw[0], wave >> 1, wave & 1);
-            widen_v(kv[buf], raw[1], wave >> 1, wave & 1);
-        } else if (wave < 2) {
-            widen_k(kv[buf], raw[0], wave, 0);
-        } else {
-            widen_v(kv[buf], raw[0], wave - 2, 0);
-        }
-    };
-    if (u0 < u1) load(0);
-    half8v qh[C][2 * U], ql[C][2 * U];
-#pragma unroll
-    for (int ct = 0; ct < C; ++ct) {
-        float4 x[4 * U];
-        w.fetch_q(a, t, head, c0 + ct * 16, x);
-        w.split_q(a, t, ct, c0 + ct * 16, x, qh[ct], ql[ct]);
-    }
-    w.clear();
-    // keys that the wave's columns see: all of them below `all`, none from `none` on
-    const bool live = c0 < t.n;
-    const int all = min(t.it.start + (t.c0 + c0) / a.g + 1, t.full);
-    const int none = live ? t.it.start + (t.c0 + min(c0 + 31, t.n - 1)) / a.g + 1 : 0;
-    if (u0 < u1) {
-        widen(0);
-        sc[0] = sc_next[0];
-        sc[1] = sc_next[1];
-        if (u0 + 1 < u1) load(1);
-    }
-    VK_LDS_BARRIER();
-    for (int u = u0, k = 0; u < u1; ++u, ++k) {
-        const uint4* b = kv[k & 1];
-        if (u * kUnit < none) {
-            vk_f32x4 S[C][2];
-#pragma unroll
-            for (int ct = 0; ct < C; ++ct) S[ct][0] = S[ct][1] = vk_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < 2 * U; ++i) {
-                half8v ka[2];
-#pragma unroll
-                for (int x = 0; x < 2; ++x) ka[x] = __builtin_bit_cast(half8v, b[(x * 2 * U + i) * 64 + lane]);
-#pragma unroll
-                for (int ct = 0; ct < C; ++ct)
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        S[ct][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[x], ql[ct][i], S[ct][x], 0, 0, 0);
-                        S[ct][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[x], qh[ct][i], S[ct][x], 0, 0, 0);
+            for (int x = 0; x < 2; ++x) {
+                const int page = __builtin_amdgcn_readlane(pages, 2 * (k & 31) + x);
+                sc_next[x] = place.scale(page);
+                if (x == xw) {
+                    const uint8_t* p = place.tile(page, min(u * kUnit + x * 16, t.full - 16), v.bs, HD);
+                    if constexpr (U == 2) {
+                        p += (wave & 1) * 1024;
+                        raw[0] = ((const uint4*)p)[lane];
+                        raw[1] = ((const uint4*)(p + v.bs * HD))[lane];
+                    } else {
+                        raw[0] = ((const uint4*)(p + (wave >> 1) * v.bs * HD))[lane];
                     }
-            }
-            const bool hide = u * kUnit + kUnit > all;
-            half8v ph[C], pl[C];
-#pragma unroll
-            for (int ct = 0; ct < C; ++ct) w.weigh(ct, S[ct], sc, u * kUnit, t.full, hide, ph[ct], pl[ct]);
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const half8v va = __builtin_bit_cast(half8v, b[(4 * U + d) * 64 + lane]);
-#pragma unroll
-                for (int ct = 0; ct < C; ++ct) {
-                    w.O[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[ct], w.O[ct][d], 0, 0, 0);
-                    w.O[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[ct], w.O[ct][d], 0, 0, 0);
                 }
             }
+        };
+        auto widen_k = [&](uint4* b, const uint4& r, int x, int i) {
+            b[(x * 2 * U + 2 * i) * 64 + lane] = __builtin_bit_cast(uint4, bkv_widen8<CODEC>(r.x, r.y));
+            b[(x * 2 * U + 2 * i + 1) * 64 + lane] = __builtin_bit_cast(uint4, bkv_widen8<CODEC>(r.z, r.w));
+        };
+        auto widen_v = [&](uint4* b, const uint4& r, int x, int i) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                half2v p, q;
+                bkv_widen<CODEC>(u4c(r, d), p, q);
+                ((uint2*)&b[(4 * U + 4 * i + d) * 64 + lane])[x] =
+                    make_uint2(__builtin_bit_cast(uint32_t, p), __builtin_bit_cast(uint32_t, q));
+            }
+        };
+        auto widen = [&](int buf) {
+            if constexpr (U == 2) {
+                widen_k(kv[buf], raw[0], wave >> 1, wave & 1);
+                widen_v(kv[buf], raw[1], wave >> 1, wave & 1);
+            } else if (wave < 2) {
+                widen_k(kv[buf], raw[0], wave, 0);
+            } else {
+                widen_v(kv[buf], raw[0], wave - 2, 0);
+            }
+        };
+        if (u0 < u1) load(0);
+        half8v qh[C][2 * U], ql[C][2 * U];
+#pragma unroll
+        for (int ct = 0; ct < C; ++ct) {
+            float4 x[4 * U];
+            w.fetch_q(a, t, head, c0 + ct * 16, x);
+            w.split_q(a, t, ct, c0 + ct * 16, x, qh[ct], ql[ct]);
         }
-        if (u + 1 < u1) {
-            widen((k + 1) & 1);
+        w.clear();
+        // keys that the wave's columns see: all of them below `all`, none from `none` on
+        const bool live = c0 < t.n;
+        const int all = min(t.it.start + (t.c0 + c0) / a.g + 1, t.full);
+        const int none = live ? t.it.start + (t.c0 + min(c0 + 31, t.n - 1)) / a.g + 1 : 0;
+        if (u0 < u1) {
+            widen(0);
             sc[0] = sc_next[0];
             sc[1] = sc_next[1];
-            if (u + 2 < u1) load(k + 2);
+            if (u0 + 1 < u1) load(1);
         }
         VK_LDS_BARRIER();
-    }
-    if (!live) return;
-    if (t.final(split))
-        for (int key0 = t.full; key0 < t.keys; key0 += 16) w.open_rows(a, t, head, key0, c0);
-
-    const bool direct = t.one();
-    const size_t slot = ((size_t)blockIdx.x * v.n_head + head) * a.splits + split;
+        for (int u = u0, k = 0; u < u1; ++u, ++k) {
+            const uint4* b = kv[k & 1];
+            if (u * kUnit < none) {
+                vk_f32x4 S[C][2];
 #pragma unroll
-    for (int ct = 0; ct < C; ++ct) {
-        const int c = c0 + ct * 16 + w.col;
-        const float l = bkv_sum4(w.L[ct]);
-        if (c >= t.n) continue;
-        float* dst = direct ? a.out + w.row(a, t, head, c) : a.part + a.part_o + (slot * a.cols + c) * HD;
-        const float f = direct ? 0x1p-14f / l : 0x1p-14f;
-        if (!direct && w.grp == 0) ((float2*)a.part)[slot * a.cols + c] = make_float2(w.M[ct], l);
+                for (int ct = 0; ct < C; ++ct) S[ct][0] = S[ct][1] = vk_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-            *(vk_f32x4*)(dst + (d >> 2) * 64 + 16 * w.grp + (d & 3) * 4) = w.out4(ct, d >> 2, d & 3) * f;
+                for (int i = 0; i < 2 * U; ++i) {
+                    half8v ka[2];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) ka[x] = __builtin_bit_cast(half8v, b[(x * 2 * U + i) * 64 + lane]);
+#pragma unroll
+                    for (int ct = 0; ct < C; ++ct)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            S[ct][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[x], ql[ct][i], S[ct][x], 0, 0, 0);
+                            S[ct][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[x], qh[ct][i], S[ct][x], 0, 0, 0);
+                        }
+                }
+                const bool hide = u * kUnit + kUnit > all;
+                half8v ph[C], pl[C];
+#pragma unroll
+                for (int ct = 0; ct < C; ++ct) w.weigh(ct, S[ct], sc, u * kUnit, t.full, hide, ph[ct], pl[ct]);
+                // from here to the barrier before the other workgroup's waves: it is what
+                // this one's wait for (212 us against 204)
+                __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const half8v va = __builtin_bit_cast(half8v, b[(4 * U + d) * 64 + lane]);
+#pragma unroll
+                    for (int ct = 0; ct < C; ++ct) {
+                        w.O[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[ct], w.O[ct][d], 0, 0, 0);
+                        w.O[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[ct], w.O[ct][d], 0, 0, 0);
+                    }
+                }
+            }
+            if (u + 1 < u1) {
+                widen((k + 1) & 1);
+                sc[0] = sc_next[0];
+                sc[1] = sc_next[1];
+                if (u + 2 < u1) load(k + 2);
+            }
+            VK_LDS_BARRIER();
+            __builtin_amdgcn_s_setprio(0);
+        }
+        if (live) {
+            if (last)
+                for (int key0 = t.full; key0 < t.keys; key0 += 16) w.open_rows(a, t, head, key0, c0);
+            const size_t slot = 2 * sh.index + !begin;
+#pragma unroll
+            for (int ct = 0; ct < C; ++ct) {
+                const int c = c0 + ct * 16 + w.col;
+                const float l = bkv_sum4(w.L[ct]);
+                if (c >= t.n) continue;
+                float* dst = whole ? a.out + w.row(a, t, head, c) : a.part + a.part_o + (slot * kChunkCols + c) * HD;
+                const float f = whole ? 0x1p-14f / l : 0x1p-14f;
+                if (!whole && w.grp == 0) ((float2*)a.part)[slot * kChunkCols + c] = make_float2(w.M[ct], l);
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+                    *(vk_f32x4*)(dst + (d >> 2) * 64 + 16 * w.grp + (d & 3) * 4) = w.out4(ct, d >> 2, d & 3) * f;
+            }
+        }
+        // a tile that begins here and goes on in later shares
+        if (!last && at == 0) open = {item, tile, 2 * head + !begin, 1 + (cost - to + sh.size - 1) / sh.size};
+        left -= to - at;
+        at = 0;
+        ++tile;
     }
+    if (threadIdx.x == 0) a.open[sh.index] = open;
 }
 
-// The key ranges of tiles of more than 16 columns (their own last workgroup would
-// take longer over them than a launch does): HD / 4 threads a column.
-template <int HD, bool CHUNKS>
-__global__ __launch_bounds__(256) void vk_bkv_attn_merge(BkvAttnArgs a) {
-    __shared__ int sh;
+// The pieces of a tile of chunks (share blockIdx.x has the first), HD / 4 threads a column.
+template <int HD>
+__global__ __launch_bounds__(256) void vk_bkv_attn_join(BkvAttnArgs a) {
     constexpr int PT = HD / 4;
-    const int head = blockIdx.y;
-    const int tile = CHUNKS ? a.tiles - 1 - (a.tile0 + (int)blockIdx.x) : a.tile0 + (int)blockIdx.x;
+    const BkvOpen o = a.open[blockIdx.x];
+    if (o.pieces == 0) return;
     BkvTile t;
-    if (!bkv_tile<CHUNKS>(a, tile, kChunkCols, &sh, t) || t.one()) return;
+    bkv_chunk(a, a.v.step[o.item], o.tile, t);
+    const int c = blockIdx.y * (256 / PT) + threadIdx.x / PT, d = (threadIdx.x % PT) * 4;
+    if (c >= t.n) return;
+    const int head = o.head >> 1, second = o.head & 1;
+    const size_t first = (size_t)(2 * blockIdx.x + second) * kChunkCols + c;
+    const int cc = t.c0 + c, j = cc / a.g;
+    *(vk_f32x4*)(a.out + ((size_t)(t.it.row0 + j) * a.hq + head * a.g + (cc - j * a.g)) * HD + d) =
+        bkv_join<HD, false>(a.part + first * 2, a.part + a.part_o + first * HD + d, o.pieces, kChunkCols, 2, second);
+}
+
+// The key ranges of items of 17 to 32 columns (their own last workgroup would take
+// longer over them than a launch does): HD / 4 threads a column.
+template <int HD>
+__global__ __launch_bounds__(256) void vk_bkv_attn_merge(BkvAttnArgs a) {
+    constexpr int PT = HD / 4;
+    const int head = blockIdx.y, tile = a.tile0 + (int)blockIdx.x;
+    BkvTile t;
+    if (!bkv_tile(a, tile, t) || t.one()) return;
     const int c = blockIdx.z * (256 / PT) + threadIdx.x / PT, d = (threadIdx.x % PT) * 4;
     if (c >= t.n) return;
     const size_t first = ((size_t)blockIdx.x * a.v.n_head + head) * a.splits * a.cols + c;
-    const int cc = t.c0 + c, j = CHUNKS ? cc / a.g : bkv_div(cc, a.g_inv);
-    *(vk_f32x4*)(a.out + ((size_t)(t.it.row0 + j) * a.hq + head * a.g + (cc - j * a.g)) * HD + d) =
-        bkv_join<HD, false>(a.part + first * 2, a.part + a.part_o + first * HD + d, (t.units + t.per - 1) / t.per, a.cols);
+    const int j = bkv_div(c, a.g_inv);
+    *(vk_f32x4*)(a.out + ((size_t)(t.it.row0 + j) * a.hq + head * a.g + (c - j * a.g)) * HD + d) =
+        bkv_join<HD, false>(a.part + first * 2, a.part + a.part_o + first * HD + d, (t.units + t.per - 1) / t.per, a.cols,
+                            1, 0);
 }
 
 template <int HD, int CODEC>
@@ -856,15 +996,15 @@ static void go_attn(hipStream_t s, const BkvAttnArgs& a, int tc, dim3 grid) {
 }
 
 template <int HD>
-static void go_hd(hipStream_t s, const BkvAttnArgs& a, int tc, unsigned tiles) {
-    const dim3 grid(tiles, (unsigned)a.v.n_head, (unsigned)a.splits);
+static void go_hd(hipStream_t s, const BkvAttnArgs& a, int tc, dim3 grid) {
     if (a.v.codec == BKV_INT8) go_attn<HD, BKV_INT8>(s, a, tc, grid);
     else go_attn<HD, BKV_E4M3>(s, a, tc, grid);
-    constexpr unsigned CW = 256 / (HD / 4);  // columns a merging workgroup
-    if (a.splits == 1 || tc == 16) return;
-    const dim3 cols(tiles, (unsigned)a.v.n_head, ((unsigned)a.cols + CW - 1) / CW);
-    if (a.chunks) hipLaunchKernelGGL((vk_bkv_attn_merge<HD, true>), cols, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((vk_bkv_attn_merge<HD, false>), cols, dim3(256), 0, s, a);
+    constexpr unsigned CW = 256 / (HD / 4);  // columns a joining workgroup
+    const unsigned cols = ((unsigned)a.cols + CW - 1) / CW;
+    if (tc == kChunkCols)
+        hipLaunchKernelGGL(vk_bkv_attn_join<HD>, dim3(kBkvShares, cols), dim3(256), 0, s, a);
+    else if (a.splits > 1 && tc != 16)
+        hipLaunchKernelGGL(vk_bkv_attn_merge<HD>, dim3(grid.x, grid.y, cols), dim3(256), 0, s, a);
 }
 
 hipError_t launch_bkv_attn(hipStream_t s, const BkvView& v, int layer, int n, int n_rows, int max_count, int max_len,
@@ -881,32 +1021,35 @@ hipError_t launch_bkv_attn(hipStream_t s, const BkvView& v, int layer, int n, in
     a.g = hq / v.n_head;
     const long long cols = (long long)max_count * a.g;
     const int tc = cols <= 16 ? 16 : cols <= 32 ? 32 : kChunkCols;
-    a.chunks = cols > 32;
-    a.cols = a.chunks ? tc : (int)cols;
-    const long long tiles = a.chunks ? (long long)n_rows * a.g / tc + n : n;
-    a.tiles = (int)tiles;
     const int room = kBkvParts;
-    const int units = std::max(1, (max_len + kUnit - 1) / kUnit);
-    const long long most = std::min<long long>(64, std::max<long long>(1, room / ((long long)v.n_head * a.cols)));
-    // Units a key range: the call's units at the longest rows' length over 512
-    // (1280 for chunks), so that there are ranges for every CU and few to merge.
-    const long long all = tiles * v.n_head * units;
-    const long long per = a.chunks ? std::min<long long>(std::max<long long>(all / 1280, 8), 64)
-                                   : std::max<long long>(all / 512, 8);
-    a.per = (int)((std::max(per, (units + most - 1) / most) + 3) / 4 * 4);
-    a.splits = (units + a.per - 1) / a.per;
     a.part_o = (size_t)room * 2;
     a.joined = (unsigned*)(part + (size_t)room * (128 + 2));
+    a.open = (BkvOpen*)(a.joined + room);
     auto inv = [](int d) { return d == 1 ? 0u : (uint32_t)(((1ull << 32) + (uint32_t)d - 1) / (uint32_t)d); };
     a.g_inv = inv(a.g);
+    auto go = [&](dim3 grid) { v.hd == 64 ? go_hd<64>(s, a, tc, grid) : go_hd<128>(s, a, tc, grid); };
+    if (tc == kChunkCols) {
+        static_assert(2 * kBkvShares * kChunkCols <= kBkvParts && sizeof(BkvOpen) == 16, "");
+        a.tiles = (int)((long long)n_rows * a.g / kChunkCols + n);
+        a.cols = kChunkCols;
+        go(dim3(kBkvShares));
+        return hipGetLastError();
+    }
+    a.cols = (int)cols;
+    const int units = std::max(1, (max_len + kUnit - 1) / kUnit);
+    const long long most = std::min<long long>(64, std::max<long long>(1, room / ((long long)v.n_head * a.cols)));
+    // Units a key range: the call's units at the longest rows' length over 512, so
+    // that there are ranges for every CU and few to merge.
+    const long long per = std::max<long long>((long long)n * v.n_head * units / 512, 8);
+    a.per = (int)((std::max(per, (units + most - 1) / most) + 3) / 4 * 4);
+    a.splits = (units + a.per - 1) / a.per;
     a.splits_inv = inv(a.splits);
-    // tiles a launch: what the workspace holds, and fewer than 2^24 workgroups
-    const long long step = a.splits == 1 ? 1 << 20
-                                         : std::max<long long>(1, room / ((long long)v.n_head * a.cols * a.splits));
-    for (long long t0 = 0; t0 < tiles; t0 += step) {
+    // items a launch: what the workspace holds
+    const long long step =
+        a.splits == 1 ? n : std::max<long long>(1, room / ((long long)v.n_head * a.cols * a.splits));
+    for (long long t0 = 0; t0 < n; t0 += step) {
         a.tile0 = (int)t0;
-        if (v.hd == 64) go_hd<64>(s, a, tc, (unsigned)std::min(step, tiles - t0));
-        else go_hd<128>(s, a, tc, (unsigned)std::min(step, tiles - t0));
+        go(dim3((unsigned)std::min(step, n - t0), (unsigned)v.n_head, (unsigned)a.splits));
     }
     return hipGetLastError();
 }
