@@ -144,15 +144,43 @@ __device__ __forceinline__ void bkv_split2(float x, float y, half2v& hi, half2v&
     lo = __builtin_convertvector(r, half2v);
 }
 
-// sum / max over the four lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48)
+// sum / max over the four lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48): a swap
+// of rows of a value with itself leaves the two that meet in the lane
+template <class F>
+__device__ __forceinline__ float bkv_fold4(float v, F f) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 __device__ __forceinline__ float bkv_max4(float v) {
-    v = fmaxf(v, __int_as_float(vk_bfly_partner<16>(__float_as_int(v))));
-    return fmaxf(v, __int_as_float(vk_bfly_partner<32>(__float_as_int(v))));
+    return bkv_fold4(v, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float bkv_sum4(float v) {
-    v += __int_as_float(vk_bfly_partner<16>(__float_as_int(v)));
-    return v + __int_as_float(vk_bfly_partner<32>(__float_as_int(v)));
+    return bkv_fold4(v, [](float a, float b) { return a + b; });
 }
+
+// A tile's scales as the weights need them: K's, and V's f 2^e (f in [1, 2)) as
+// f 2^14, 2^-e and e. Zero: 0, 1, 0; not finite: NaN, 1, 0.
+struct BkvScale {
+    float k, vf, back, ve;
+    __device__ __forceinline__ void set(float2 sc) {
+        const uint32_t b = __float_as_uint(sc.y);
+        const int ex = (int)((b >> 23) & 255);
+        const bool plain = ex != 0 && ex != 255;
+        const float f14 = __uint_as_float((b & 0x007fffffu) | 0x46800000u);
+        const int e = plain ? ex : 127;
+        k = sc.x;
+        vf = plain ? f14 : sc.y;
+        back = __uint_as_float((uint32_t)min(254 - e, 253) << 23);
+        ve = (float)(e - 127);
+    }
+    // of lane l, in all lanes
+    __device__ __forceinline__ BkvScale at(int l) const {
+        auto get = [l](float x) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), l)); };
+        return BkvScale{get(k), get(vf), get(back), get(ve)};
+    }
+};
 
 // A value that a workgroup on another XCD reads in this launch: past the caches
 // that are the XCD's own.
@@ -290,21 +318,12 @@ struct BkvWave {
     // raw scores of a unit (32 keys from key0 on, none from `full` on) -> the two
     // parts of 2^14 times its weights, V's scales in them. hide: some key is
     // hidden from some column.
-    __device__ __forceinline__ void weigh(int ct, const vk_f32x4 (&S)[2], const float2 (&sc)[2], int key0, int full,
+    __device__ __forceinline__ void weigh(int ct, const vk_f32x4 (&S)[2], const BkvScale (&sc)[2], int key0, int full,
                                           bool hide, half8v& ph, half8v& pl) {
-        float f[2], ve[2], vf[2], back[2], e[8];
+        const float f[2] = {sc[0].k * qf[ct], sc[1].k * qf[ct]};
+        float e[8];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const uint32_t b = __float_as_uint(sc[x].y);
-            const int ex = (int)((b >> 23) & 255);
-            const bool plain = ex != 0 && ex != 255;  // zero: f 0, e 0; not finite: f NaN, e 0
-            vf[x] = plain ? __uint_as_float((b & 0x007fffffu) | 0x46800000u) : sc[x].y;  // f 2^14
-            back[x] = plain ? __uint_as_float((uint32_t)min(254 - ex, 253) << 23) : 1.0f;  // 2^-e
-            ve[x] = plain ? (float)(ex - 127) : 0.0f;
-            f[x] = sc[x].x * qf[ct];
-        }
-#pragma unroll
-        for (int r = 0; r < 8; ++r) e[r] = fmaf(S[r >> 2][r & 3], f[r >> 2], ve[r >> 2]);
+        for (int r = 0; r < 8; ++r) e[r] = fmaf(S[r >> 2][r & 3], f[r >> 2], sc[r >> 2].ve);
         auto top = [&]() {
             const float m = fmaxf(fmaxf(fmaxf(e[0], e[1]), e[2]), fmaxf(fmaxf(e[3], e[4]), e[5]));
             return bkv_max4(fmaxf(m, fmaxf(e[6], e[7])));
@@ -324,9 +343,9 @@ struct BkvWave {
         float w[8];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            L[ct] = fmaf((e[4 * x] + e[4 * x + 1]) + (e[4 * x + 2] + e[4 * x + 3]), back[x], L[ct]);
+            L[ct] = fmaf((e[4 * x] + e[4 * x + 1]) + (e[4 * x + 2] + e[4 * x + 3]), sc[x].back, L[ct]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) w[4 * x + r] = e[4 * x + r] * vf[x];
+            for (int r = 0; r < 4; ++r) w[4 * x + r] = e[4 * x + r] * sc[x].vf;
         }
         if (hide) {  // a hidden key has no part in a block whose scale is NaN
 #pragma unroll
@@ -499,10 +518,14 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(BkvAt
     int pages = 0;
     if (u0 < u1) pages = pages_from(0);
     const BkvPlace place(v, a.layer, head, pool, scales);
+    // zero, but a vector register to the compiler: a scale is loaded and taken apart
+    // in all lanes, where scalar registers made branches of it
+    int zero = 0;
+    asm("" : "+v"(zero));
 
     uint4 kr[2][U], vr[2][U];
-    float2 sc[2];
     const uint8_t* at[2];
+    float2 sc[2];
     // the k-th unit of this wave: its tiles' places, and the loads of K (V: load_v)
     auto load_k = [&](int u, int k) {
         if (k > 0 && (k & 31) == 0) pages = pages_from(k);
@@ -510,7 +533,7 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(BkvAt
         for (int x = 0; x < 2; ++x) {
             const int page = __builtin_amdgcn_readlane(pages, 2 * (k & 31) + x);
             at[x] = place.tile(page, min(u * kUnit + x * 16, t.full - 16), v.bs, HD);
-            sc[x] = place.scale(page);
+            sc[x] = place.scale(page + zero);
 #pragma unroll
             for (int i = 0; i < U; ++i) kr[x][i] = ((const uint4*)(at[x] + i * 1024))[lane];
         }
@@ -534,11 +557,12 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(BkvAt
     if (t.final(split) && open < t.keys) w.open_rows(a, t, head, open, 0);
     if (u0 < u1) {
         load_k(u0, 0);
+        __builtin_amdgcn_sched_barrier(0);  // K first, as in the loop: its wait is for K alone
         load_v();
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (C == 1) w.split_q(a, t, 0, 0, x, qh, ql);
     }
-    if constexpr (C == 1) {
-        w.split_q(a, t, 0, 0, x, qh, ql);
-    } else {
+    if constexpr (C > 1) {
         if (wave < C) {
             w.split_q(a, t, 0, wave * 16, x, qh, ql);
             if (w.grp == 0) sqf[wave * 16 + w.col] = w.qf[0];
@@ -581,7 +605,9 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(BkvAt
                 }
             }
         }
-        const float2 now[2] = {sc[0], sc[1]};
+        BkvScale now[2];
+        now[0].set(sc[0]);
+        now[1].set(sc[1]);
         const bool more = u + kWaves < u1;
         if (more) load_k(u + kWaves, k + 1);
         const bool hide = u * kUnit + kUnit > min(t.it.start + 1, t.full);
@@ -813,19 +839,27 @@ __global__ __launch_bounds__(256, 2) void vk_bkv_attn_chunk(BkvAttnArgs a, const
             const int key = min((u0 + k0) * kUnit + lane * 16, t.full - 16);
             return table[key >> bs_log];
         };
-        int pages = u0 < u1 ? pages_from(0) : 0;
+        int pages = 0;
+        BkvScale scale;  // of the lanes' pages
         const BkvPlace place(v, a.layer, head, pool, scales);
+        if (u0 < u1) {
+            pages = pages_from(0);
+            scale.set(place.scale(pages));
+        }
         // wave's 1 KB pieces of a unit: U = 2: K's and V's piece (tile wave / 2, half
         // wave % 2); U = 1: waves 0, 1 K's tiles, 2, 3 V's
         uint4 raw[U];
-        float2 sc[2], sc_next[2];
+        BkvScale sc[2], sc_next[2];
         auto load = [&](int k) {
-            if (k > 0 && (k & 31) == 0) pages = pages_from(k);
+            if (k > 0 && (k & 31) == 0) {
+                pages = pages_from(k);
+                scale.set(place.scale(pages));
+            }
             const int u = u0 + k, xw = U == 2 ? wave >> 1 : wave & 1;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const int page = __builtin_amdgcn_readlane(pages, 2 * (k & 31) + x);
-                sc_next[x] = place.scale(page);
+                sc_next[x] = scale.at(2 * (k & 31) + x);
                 if (x == xw) {
                     const uint8_t* p = place.tile(page, min(u * kUnit + x * 16, t.full - 16), v.bs, HD);
                     if constexpr (U == 2) {
