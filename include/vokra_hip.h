@@ -459,7 +459,7 @@ int vokra_hip_bkv_step(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t n, cons
  * INVALID_ARGUMENT); max_len, the longest sequence after the step, only sizes
  * the attention's split. In a graph: a captured write or attn covers steps of
  * at most the n, n_rows and max_count that the last step before its capture
- * was given. */
+ * was given, and passes over items beyond. */
 int vokra_hip_bkv_step_dev(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t n, size_t n_rows, size_t max_count,
                            size_t max_len, const int32_t *d_seqs, const int32_t *d_starts, const int32_t *d_counts);
 /* Synchronizes; the outcome of the last step, fork, free, copy (on its
@@ -468,7 +468,8 @@ int vokra_hip_bkv_step_dev(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t n, 
 int vokra_hip_bkv_status(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t *n_done);
 
 /* The step's rows of one layer, k and v [rows][n_head * d_head], into the
- * cache. Every layer is written once a step, before that layer's attn. */
+ * cache. Every layer is written once a step, before that layer's attn, and
+ * before a sequence of the step is forked, copied or stepped again. */
 int vokra_hip_bkv_write(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t layer, const float *k_rows,
                         const float *v_rows);
 /* Device arrays (16-byte aligned), asynchronous. */
@@ -481,7 +482,7 @@ int vokra_hip_bkv_write_dev(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t la
  * d_head], n_head_q any multiple of n_head. f32 in and out: products of a query
  * or a weight with 8-bit values run as two fp16 parts of the f32 operand (22
  * bits), those with f32 rows in f32, sums in f32. Rows that the step does not
- * reach are left as they are. One token a sequence, several (drafts) and long
+ * reach are left as they are; out does not overlap q. One token a sequence, several (drafts) and long
  * chunks of prompts take the same call. */
 int vokra_hip_bkv_attn(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t layer, size_t n_head_q, const float *q,
                        float scale, float *out);
@@ -576,8 +577,8 @@ void vokra_hip_rope_destroy(vokra_hip_rope_t *rope);
 /* Row r of q [n_head_q heads] and k [n_head_k heads] at positions[r] (any
  * int32), one launch; either may have no heads. Rows lie q_stride (and so on)
  * floats apart, so q and k may be parts of one projection's rows. An output is
- * its input (in place, the same stride) or does not overlap it. Device
- * pointers, asynchronous; at most 2^32 values. */
+ * its input (in place, the same stride) or overlaps no input. Device pointers,
+ * asynchronous; at most 2^32 values. */
 int vokra_hip_rope_apply_dev(vokra_hip_ctx_t *ctx, const vokra_hip_rope_t *rope, size_t rows,
                              const int32_t *d_positions, size_t n_head_q, const float *d_q, size_t q_stride,
                              float *d_q_out, size_t q_out_stride, size_t n_head_k, const float *d_k, size_t k_stride,

@@ -382,6 +382,68 @@ def test_copy_to_a_smaller_cache_and_compaction(ctx):
     a.check_rows()
 
 
+def test_a_step_is_written_where_compaction_has_moved_its_pages(ctx):
+    print("[case] bkv compact in a step", flush=True)
+    p = Pair(ctx, 2, 2, 64, 3, 200, 16, 20, 200)
+    p.step([0, 1], [0, 0], [160, 20])
+    p.both("free", [0])
+    p.step([1, 2], [20, 0], [0, 100])
+    p.both("free", [1])
+    p.step([0, 2], [0, 100], [40, 30], write=False)
+    p.ref.compact()
+    p.dev.compact()
+    for layer in range(2):
+        k, v = p.rows(70)
+        p.dev.write(layer, k, v)
+        p.ref.write(layer, k, v)
+        p.check_attn(layer, 70, 2)
+    p.check_state()
+    p.check_rows()
+
+
+@pytest.mark.parametrize("count,kvh", [(1, 2), (2, 1), (9, 1)])
+def test_captured_calls_pass_over_a_larger_step(ctx, count, kvh):
+    """write and attn of a graph meet steps of more items, rows, or rows an item
+    than the step before the capture: they do what fits and nothing else."""
+    print("[case] bkv graph small", count, kvh, flush=True)
+    heads, hd, n = 8, 64, 3
+    p = Pair(ctx, 1, kvh, hd, 6, 300, 16, 100, 450)
+    p.step(np.arange(6), np.zeros(6, int), [100, 37, 64, 5, 150, 80])
+    lens = np.array(p.ref.len)
+    rows, w, wq = n * count, kvh * hd, heads * hd
+    p.step(np.arange(n), lens[:n], [count] * n)
+    up = lambda a: hip.DeviceBuffer.from_array(ctx, a)  # noqa: E731
+    xs = [p.g.standard_normal((rows, x)).astype(np.float32) for x in (w, w, wq)]
+    k, v, q = (up(x) for x in xs)
+    mark = np.full((rows + 4) * wq, 7.5, np.float32)
+    o = up(mark)
+
+    def body():
+        p.dev.write_dev(0, k, v)
+        p.dev.attn_dev(0, heads, q, 0.125, o)
+
+    body()
+    p.ref.write(0, xs[0], xs[1])
+    graph = ctx.capture(body)
+    for counts in ([count] * 6, [count, count + 1, count - 1], [5 * count, 1, 1], [count] * n):
+        m = len(counts)
+        p.step(np.arange(m), p.ref.len[:m], counts, write=False)
+        o.upload(mark)
+        graph.launch()
+        ctx.synchronize()
+        got = o.download(np.float32, mark.size)
+        assert np.all(got[rows * wq:] == 7.5)
+        if counts == [count] * n:
+            p.ref.write(0, xs[0], xs[1])
+            want, tol = p.ref.attn(0, xs[2], heads, np.float32(0.125))
+            assert np.all(np.abs(got[:rows * wq].reshape(rows, wq) - want) <= tol)
+        kk, vv = p.rows(sum(counts))
+        p.dev.write(0, kk, vv)
+        p.ref.write(0, kk, vv)
+        p.check_attn(0, sum(counts), heads)
+    p.check_rows()
+
+
 def test_more_pages_than_32_bits_of_bytes(ctx):
     """A pool of over 4 GiB: the last pages hold what the first ones do."""
     print("[case] bkv large pool", flush=True)

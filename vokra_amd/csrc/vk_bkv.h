@@ -86,8 +86,9 @@ hipError_t launch_bkv_part_clear(hipStream_t s, void* part);
 hipError_t launch_bkv_reset(hipStream_t s, const BkvView& v, bool clear_data);
 hipError_t launch_bkv_step(hipStream_t s, const BkvView& v, int n, int n_rows, int max_count, const int* seqs,
                            const int* starts, const int* counts);
-// work_bound: at least the step's blocks
-hipError_t launch_bkv_write(hipStream_t s, const BkvView& v, int layer, int work_bound, const float* k, const float* vv);
+// n_rows, work_bound: at least the step's rows, blocks
+hipError_t launch_bkv_write(hipStream_t s, const BkvView& v, int layer, int n_rows, int work_bound, const float* k,
+                            const float* vv);
 hipError_t launch_bkv_read(hipStream_t s, const BkvView& v, int layer, int n, const int* seqs, const int* times,
                            float* k, float* vv);
 hipError_t launch_bkv_fork(hipStream_t s, const BkvView& v, int n, const int* src, const int* dst);

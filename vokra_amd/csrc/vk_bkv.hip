@@ -286,14 +286,15 @@ __device__ __forceinline__ float* bkv_ring(const BkvView& v, int layer, int seq,
 // rows (those that earlier steps brought), before it writes any, so no two waves
 // meet there. Bound by memory: 5 bytes a value.
 template <int CODEC, int NT>
-__global__ __launch_bounds__(256) void vk_bkv_write(BkvView v, int layer, unsigned wg0, const float* __restrict__ k,
-                                                    const float* __restrict__ vv) {
+__global__ __launch_bounds__(256) void vk_bkv_write(BkvView v, int layer, int n_rows, unsigned wg0,
+                                                    const float* __restrict__ k, const float* __restrict__ vv) {
     const int n_work = v.meta[BKV_WORK_N], hs = 2 * v.n_head;
     const long long unit = ((long long)wg0 + blockIdx.x) * 4 + (threadIdx.x >> 6);
     const int entry = __builtin_amdgcn_readfirstlane((int)(unit / hs));
     if (entry >= n_work) return;
     const int sub = __builtin_amdgcn_readfirstlane((int)(unit - (long long)entry * hs));
     const BkvWork e = v.work[entry];
+    if (e.row0 + (e.end - e.start) > n_rows) return;  // a later step, met by a captured write
     const int side = sub & 1, head = sub >> 1, lane = threadIdx.x & 63, hd = v.hd, bs = v.bs;
     const size_t rs = (size_t)v.n_head * hd;  // floats from row to row
     const float* in = (side ? vv : k) + (size_t)e.row0 * rs + (size_t)head * hd;
@@ -662,7 +663,8 @@ __global__ __launch_bounds__(BKV_TPB) void vk_bkv_compact_plan(BkvView v) {
     }
 }
 
-// Table entries of moved pages, one sequence a workgroup.
+// Table entries of moved pages, one sequence a workgroup, and the pages that the
+// current step's rows are still to be written to.
 __global__ __launch_bounds__(256) void vk_bkv_compact_table(BkvView v) {
     if (v.meta[BKV_MOVE_N] == 0) return;
     const int u = v.n_page - v.meta[BKV_FREE];
@@ -673,6 +675,8 @@ __global__ __launch_bounds__(256) void vk_bkv_compact_table(BkvView v) {
             if (*e >= u) *e = v.remap[*e];
         }
     }
+    for (int k = blockIdx.x * 256 + threadIdx.x; k < v.meta[BKV_WORK_N]; k += gridDim.x * 256)
+        if (v.work[k].page >= u) v.work[k].page = v.remap[v.work[k].page];
 }
 
 __global__ void vk_bkv_peek(BkvView v, int seq, int block, int* out) {
@@ -715,27 +719,29 @@ hipError_t launch_bkv_step(hipStream_t s, const BkvView& v, int n, int n_rows, i
 constexpr long long kMaxWgs = 1 << 23;
 
 template <int CODEC, int NT>
-static void go_write(hipStream_t s, const BkvView& v, int layer, long long wgs, const float* k, const float* vv) {
+static void go_write(hipStream_t s, const BkvView& v, int layer, int n_rows, long long wgs, const float* k,
+                     const float* vv) {
     for (long long w = 0; w < wgs; w += kMaxWgs)
         hipLaunchKernelGGL((vk_bkv_write<CODEC, NT>), dim3((unsigned)std::min(kMaxWgs, wgs - w)), dim3(256), 0, s, v,
-                           layer, (unsigned)w, k, vv);
+                           layer, n_rows, (unsigned)w, k, vv);
 }
 template <int CODEC>
-static void go_write(hipStream_t s, const BkvView& v, int layer, long long wgs, const float* k, const float* vv) {
+static void go_write(hipStream_t s, const BkvView& v, int layer, int n_rows, long long wgs, const float* k,
+                     const float* vv) {
     switch (v.bs / 16 * (v.hd / 64)) {
-    case 1: go_write<CODEC, 1>(s, v, layer, wgs, k, vv); break;
-    case 2: go_write<CODEC, 2>(s, v, layer, wgs, k, vv); break;
-    case 4: go_write<CODEC, 4>(s, v, layer, wgs, k, vv); break;
-    default: go_write<CODEC, 8>(s, v, layer, wgs, k, vv); break;
+    case 1: go_write<CODEC, 1>(s, v, layer, n_rows, wgs, k, vv); break;
+    case 2: go_write<CODEC, 2>(s, v, layer, n_rows, wgs, k, vv); break;
+    case 4: go_write<CODEC, 4>(s, v, layer, n_rows, wgs, k, vv); break;
+    default: go_write<CODEC, 8>(s, v, layer, n_rows, wgs, k, vv); break;
     }
 }
 
-hipError_t launch_bkv_write(hipStream_t s, const BkvView& v, int layer, int work_bound, const float* k,
+hipError_t launch_bkv_write(hipStream_t s, const BkvView& v, int layer, int n_rows, int work_bound, const float* k,
                             const float* vv) {
     if (work_bound == 0) return hipSuccess;
     const long long wgs = ((long long)work_bound * 2 * v.n_head + 3) / 4;
-    if (v.codec == BKV_INT8) go_write<BKV_INT8>(s, v, layer, wgs, k, vv);
-    else go_write<BKV_E4M3>(s, v, layer, wgs, k, vv);
+    if (v.codec == BKV_INT8) go_write<BKV_INT8>(s, v, layer, n_rows, wgs, k, vv);
+    else go_write<BKV_E4M3>(s, v, layer, n_rows, wgs, k, vv);
     return hipGetLastError();
 }
 

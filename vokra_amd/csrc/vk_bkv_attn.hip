@@ -53,6 +53,7 @@ struct BkvAttnArgs {
     unsigned* joined;   // [tile][head] ranges that have written theirs, zero between calls
     float scale_log2;   // scale * log2(e)
     int layer, hq, g;   // g = hq / n_head
+    int n, rows, count; // most items, rows, and rows an item: items beyond are passed over
     uint32_t g_inv, splits_inv;  // ceil(2^32 / g), ceil(2^32 / splits): see bkv_div
     BkvOpen* open;      // of each share: the tile whose first piece is its last
     int tile0;          // first item of this launch
@@ -79,6 +80,11 @@ struct BkvTile {
 // x / d for inv = ceil(2^32 / d): exact while x (d - 1) < 2^32
 __device__ __forceinline__ int bkv_div(int x, uint32_t inv) { return inv ? (int)__umulhi((uint32_t)x, inv) : x; }
 
+// Whether the call's buffers and launches have room for an item (a captured call
+// may meet a later step).
+__device__ __forceinline__ bool bkv_fits(const BkvAttnArgs& a, const BkvItem& it) {
+    return it.count <= a.count && it.row0 + it.count <= a.rows;
+}
 __device__ __forceinline__ void bkv_keys(const BkvView& v, BkvTile& t) {
     const int bs_log = 31 - __clz(v.bs);
     t.full = min((t.it.start + t.it.count) >> bs_log << bs_log, (t.keys + 15) & ~15);
@@ -89,7 +95,7 @@ __device__ __forceinline__ bool bkv_tile(const BkvAttnArgs& a, int item, BkvTile
     t.it = a.v.step[item];
     t.c0 = 0;
     t.n = t.it.count * a.g;
-    if (t.n <= 0) return false;
+    if (t.n <= 0 || !bkv_fits(a, t.it)) return false;
     t.keys = t.it.start + t.it.count;
     bkv_keys(a.v, t);
     t.per = max(a.per, (bkv_div(t.units + a.splits - 1, a.splits_inv) + 3) & ~3);
@@ -103,7 +109,7 @@ __device__ __forceinline__ bool bkv_chunk(const BkvAttnArgs& a, const BkvItem& i
     t.it = it;
     t.c0 = tile * kChunkCols;
     t.n = min(kChunkCols, it.count * a.g - t.c0);
-    if (t.n <= 0) return false;
+    if (t.n <= 0 || !bkv_fits(a, it)) return false;
     t.keys = it.start + (t.c0 + t.n - 1) / a.g + 1;
     bkv_keys(a.v, t);
     return true;
@@ -702,13 +708,18 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(BkvAt
 
 // ---- chunks ----------------------------------------------------------------------
 // The call's work is one line of (head, item, tile, unit), kTileCost units more a
-// tile for its start and its open block's rows. Every workgroup takes an even share
-// of the line, so all end together whatever the lengths are; a share holds whole
-// tiles and at most two pieces, one at each end, whose results are joined by the
-// kernel below. (One workgroup for each key range of each tile left 40 % of the
-// waves' places empty at six chunks of 450 .. 1030 rows over up to 4500 keys, and
-// finer ranges cost more to join than they gave: 264 us; shares: FIGURE.)
+// tile for its start and end. Every workgroup takes an even share of the line, so
+// all end together whatever the lengths are; a share holds whole tiles and at most
+// two pieces, one at each end, whose results the kernel below joins. One workgroup
+// for each key range of each tile left 40 % of the waves' places empty at six chunks
+// of 450 .. 1030 rows over up to 4500 keys, 16 heads over 2 of 128, and finer ranges
+// cost more to join than they gave: 264 us against 204 with shares.
+// That call takes 188 us now: 0.43 PFLOP/s of the operator, 0.86 of fp16 products.
+// Of a unit's time about a quarter each is the products and the weights, the
+// rest starts, joins (20 us: 96 MB) and waits for the four waves' common units.
 
+// The least share, in units (16 was slower by a tenth where drafts of 8 .. 16 rows
+// make small calls), and a tile's start and end (2: 212 us, 12: 223, 5: 204).
 constexpr int kLeast = 8, kTileCost = 5;
 
 struct BkvShare {
@@ -717,11 +728,11 @@ struct BkvShare {
     int item, tile, head, at;   // where it begins
 };
 
-// The share of workgroup w, the same on all threads; false: sh.index has none. The places of tiles: item i's
-// begin at row0_i * g / kChunkCols + i (room for a partly filled tile each). lds:
-// kBkvMaxItems ints and 16 more.
+// The share of workgroup w, the same on all threads; false: sh.index has none. The
+// places of tiles: item i's begin at row0_i * g / kChunkCols + i (room for a partly
+// filled tile each). lds: kBkvMaxItems ints and 16 more. About 3 us.
 __device__ __forceinline__ bool bkv_share(const BkvAttnArgs& a, int w, int* lds, BkvShare& sh) {
-    const int n = a.v.meta[BKV_STEP_N], t = threadIdx.x;
+    const int n = min(a.v.meta[BKV_STEP_N], a.n), t = threadIdx.x;
     int* first = lds;
     long long* sums = (long long*)(lds + kBkvMaxItems);
     for (int x = t; x < n; x += 256) first[x] = (int)((long long)a.v.step[x].row0 * a.g / kChunkCols) + x;
@@ -823,7 +834,7 @@ __global__ __launch_bounds__(256, 2) void vk_bkv_attn_chunk(BkvAttnArgs a, const
         BkvTile t;
         if (!bkv_chunk(a, it, tile, t)) {  // the next item, or the next head
             tile = 0;
-            if (++item == v.meta[BKV_STEP_N]) {
+            if (++item == min(v.meta[BKV_STEP_N], a.n)) {
                 item = 0;
                 ++head;
             }
@@ -1053,6 +1064,9 @@ hipError_t launch_bkv_attn(hipStream_t s, const BkvView& v, int layer, int n, in
     a.layer = layer;
     a.hq = hq;
     a.g = hq / v.n_head;
+    a.n = n;
+    a.rows = n_rows;
+    a.count = max_count;
     const long long cols = (long long)max_count * a.g;
     const int tc = cols <= 16 ? 16 : cols <= 32 ? 32 : kChunkCols;
     const int room = kBkvParts;

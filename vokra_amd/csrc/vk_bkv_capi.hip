@@ -278,7 +278,7 @@ int vokra_hip_bkv_write_dev(vokra_hip_ctx_t* c, vokra_hip_bkv_t* kv, size_t laye
     if (kv->step_rows == 0) return VOKRA_HIP_OK;
     if (!d_k || !d_v) return ctx_fail(BAD, "bkv_write: NULL buffer");
     if (!aligned16(d_k) || !aligned16(d_v)) return ctx_fail(BAD, "bkv_write: k and v must be 16-byte aligned");
-    BK_TRY(vk::launch_bkv_write(vk::ctx_stream(c), kv->v, (int)layer,
+    BK_TRY(vk::launch_bkv_write(vk::ctx_stream(c), kv->v, (int)layer, (int)kv->step_rows,
                                 (int)work_bound(kv, kv->step_n, kv->step_rows), d_k, d_v),
            "launch(vk_bkv_write)");
     return VOKRA_HIP_OK;
