@@ -230,6 +230,8 @@ ATTN = [  # codec, bs, hd, heads, kv heads, lens, counts
     (1, 16, 128, 24, 1, [90], [40]),
     (0, 16, 64, 40, 20, [1100], [1]),
     (0, 16, 128, 32, 1, [50, 900], [1, 1]),
+    (0, 16, 128, 4, 1, [9000, 20], [1, 1]),
+    (1, 32, 64, 32, 1, [6001], [1]),
     (0, 16, 64, 20, 20, [1000, 300, 31, 640], [900, 0, 31, 600]),
     (1, 32, 128, 16, 1, [5, 2300, 77], [5, 400, 77]),
     (0, 32, 64, 3, 1, [64, 3, 500, 90] * 20, [50, 3, 1, 0] * 20),

@@ -284,7 +284,9 @@ __device__ __forceinline__ float* bkv_ring(const BkvView& v, int layer, int seq,
 // rounded: one read, one write, no LDS. The wave of the item's first block also
 // puts the rows of the item's last two blocks into the ring; it alone reads ring
 // rows (those that earlier steps brought), before it writes any, so no two waves
-// meet there. Bound by memory: 5 bytes a value.
+// meet there. Bound by memory, 5 bytes a value: 17.7 thousand rows of 8 heads of 128
+// (K and V, blocks of 32) take 52 us, 3.5 TB/s; 64 rows take 4.4 us, which is the
+// launch and three dependent rounds of memory.
 template <int CODEC, int NT>
 __global__ __launch_bounds__(256) void vk_bkv_write(BkvView v, int layer, int n_rows, unsigned wg0,
                                                     const float* __restrict__ k, const float* __restrict__ vv) {
@@ -369,7 +371,8 @@ __global__ __launch_bounds__(256) void vk_bkv_write(BkvView v, int layer, int n_
 // workgroup takes up to 16 rows: where each is comes once into LDS, then a
 // thread widens four values of each of its rows at a time (V: the row's byte of
 // each word of a 16-byte piece, whose other bytes are the rows beside it), all
-// rows' loads in flight. Bound by memory: 5 bytes a value.
+// rows' loads in flight. Bound by memory, 5 bytes a value: 17.7 thousand rows of 8
+// heads of 128 take 50 us, 3.6 TB/s.
 constexpr int kReadRows = 16;
 template <int CODEC>
 __device__ __forceinline__ float bkv_decode1(uint32_t w) {  // the low byte of a word
@@ -602,6 +605,7 @@ __global__ __launch_bounds__(BKV_TPB) void vk_bkv_copy_plan(BkvView dv, BkvView 
 }
 
 // The moves' bytes and scales, every layer: runs of n_head * 2 * bs * hd bytes.
+// Bound by memory: 210 MB of pages moved in 92 us, 4.6 TB/s read and written.
 __global__ __launch_bounds__(256) void vk_bkv_move_pages(BkvView dv, BkvView sv) {
     const int n = dv.meta[BKV_MOVE_N];
     const size_t run = (size_t)dv.n_head * 2 * dv.bs * dv.hd;
@@ -747,7 +751,9 @@ hipError_t launch_bkv_write(hipStream_t s, const BkvView& v, int layer, int n_ro
 
 hipError_t launch_bkv_read(hipStream_t s, const BkvView& v, int layer, int n, const int* seqs, const int* times,
                            float* k, float* vv) {
-    // rows a workgroup: 16 once that leaves four workgroups a CU
+    // rows a workgroup: up to 16, once that leaves four workgroups a CU (64 rows of 20
+    // heads of 64, written and read in 8 layers: 70 us, 175 with 16; 26 thousand rows
+    // of 4 heads of 128, moved and read in 8 layers: 322 us, 362 with one)
     const int per = std::min(std::max(n / 1024, 1), kReadRows);
     const size_t w = (size_t)v.n_head * v.hd;
     for (long long r = 0; r < n; r += kMaxWgs * per) {

@@ -10,9 +10,18 @@
 // vk_bkv_attn takes up to 32 of them over a range of keys; its four waves take
 // the range's units of 32 keys in turn, each with an online softmax of its own,
 // and merge through LDS at the end: no barrier in the key loop. A tile of 16
-// columns whose keys are split over workgroups is joined by the last of them.
+// columns whose keys are split over workgroups is joined by the last of them
+// (111 us for six layers of 32 streams, 118 with a launch of its own for it).
 // vk_bkv_attn_chunk takes 128, 32 a wave, all waves over the same units, which
 // they widen to fp16 in LDS together (double buffered, one barrier a unit).
+//
+// vk_bkv_attn is bound by the pages' bytes where there are many (six sequences of
+// 9 .. 65 thousand keys, e4m3, 32 heads over 8 of 128, up to 4 rows: 457 MB in 97
+// us, 4.7 TB/s, a large copy's rate here is 4.9), by dependent rounds of memory
+// (item, page, keys, results, join: 8 us) where there are few: 32 streams of 512 ..
+// 4096 keys, 16 heads over 2 of 128, take 17.6 us for 38 MB. Four waves a workgroup,
+// three workgroups a CU: eight waves took 28 us for those, and two units' loads in
+// flight a wave spilled or left two workgroups.
 // The 8-bit values are exact in fp16, so a product is two fp16 matrix
 // instructions, one for each part of the f32 operand (22 bits): q in two parts
 // under a power of two that puts its row's largest value at 2^14, weights in two
@@ -26,9 +35,10 @@
 // maximum is that of s + e, so the largest weight has the largest product, and a
 // block of small values keeps its bits beside one of large values; the sum of
 // weights takes 2^-e back out. Two fp16 parts of 2^14 w hold a weight to 2^-22,
-// or to 2^-39 of the largest where it is smaller than 2^-17 of that. The open block's rows are f32 on both sides and
-// use the f32 matrix instruction.
+// or to 2^-39 of the largest where it is smaller than 2^-17 of that. The open
+// block's rows are f32 on both sides and use the f32 matrix instruction.
 #include <algorithm>
+#include <cmath>
 
 #include "vk_bkv.h"
 #include "vk_common.h"
@@ -525,7 +535,7 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(BkvAt
     if (u0 < u1) pages = pages_from(0);
     const BkvPlace place(v, a.layer, head, pool, scales);
     // zero, but a vector register to the compiler: a scale is loaded and taken apart
-    // in all lanes, where scalar registers made branches of it
+    // in all lanes, where scalar registers made branches of it (18.4 us against 17.6)
     int zero = 0;
     asm("" : "+v"(zero));
 
@@ -1085,10 +1095,17 @@ hipError_t launch_bkv_attn(hipStream_t s, const BkvView& v, int layer, int n, in
     }
     a.cols = (int)cols;
     const int units = std::max(1, (max_len + kUnit - 1) / kUnit);
-    const long long most = std::min<long long>(64, std::max<long long>(1, room / ((long long)v.n_head * a.cols)));
     // Units a key range: the call's units at the longest rows' length over 512, so
-    // that there are ranges for every CU and few to merge.
+    // that there are ranges for every CU (six sequences of 9 .. 65 thousand keys take
+    // 99 us, over 256 142; over 1024, 32 streams of up to 4096 take 22.5 us against
+    // 17.6), and 8 at least (16: one sequence of 2000 keys takes 10.8 us against 8.8).
     const long long per = std::max<long long>((long long)n * v.n_head * units / 512, 8);
+    // Ranges: a wave's units fall with their number, the join's rounds rise with it;
+    // together least near the root of twice the units (one sequence of 32768 keys, 8
+    // kv heads: 45 ranges 23.5 us, 64 28.6, 16 29.7; of 12000 keys, one kv head: 27
+    // 12.9, 64 14.6).
+    const long long most = std::min<long long>(std::max(8, (int)std::sqrt(2.0 * units)),
+                                               std::max<long long>(1, room / ((long long)v.n_head * a.cols)));
     a.per = (int)((std::max(per, (units + most - 1) / most) + 3) / 4 * 4);
     a.splits = (units + a.per - 1) / a.per;
     a.splits_inv = inv(a.splits);
