@@ -728,9 +728,10 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(BkvAt
 // Of a unit's time about a quarter each is the products and the weights, the
 // rest starts, joins (20 us: 96 MB) and waits for the four waves' common units.
 
-// The least share, in units (16 was slower by a tenth where drafts of 8 .. 16 rows
-// make small calls), and a tile's start and end (2: 212 us, 12: 223, 5: 204).
-constexpr int kLeast = 8, kTileCost = 5;
+// The least share, in units (five sequences of up to 1000 keys and 61 rows: 30 us, 33
+// with 8, 41 with 12), and a tile's start and end (2: 212 us for the call above, 5:
+// 204, 12: 223).
+constexpr int kLeast = 4, kTileCost = 5;
 
 struct BkvShare {
     long long begin, end;       // on the line
@@ -852,8 +853,15 @@ __global__ __launch_bounds__(256, 2) void vk_bkv_attn_chunk(BkvAttnArgs a, const
             continue;
         }
         const int cost = t.units + kTileCost, to = min(cost, at + left);
-        const int u0 = min(at, t.units), u1 = min(to, t.units);
-        const bool last = to == cost, whole = last && at == 0;
+        // the share with a tile's last unit ends it, also where the line does not
+        if (at > 0 && at >= t.units) {
+            left -= to - at;
+            at = 0;
+            ++tile;
+            continue;
+        }
+        const int u0 = at, u1 = min(to, t.units);
+        const bool last = to >= t.units, whole = last && at == 0;
         const int* table = v.table + (size_t)t.it.seq * v.max_blocks;
         // lane l holds the page of tile l of the units k0 .. k0 + 31 of the range
         auto pages_from = [&](int k0) {
@@ -999,7 +1007,7 @@ __global__ __launch_bounds__(256, 2) void vk_bkv_attn_chunk(BkvAttnArgs a, const
             }
         }
         // a tile that begins here and goes on in later shares
-        if (!last && at == 0) open = {item, tile, 2 * head + !begin, 1 + (cost - to + sh.size - 1) / sh.size};
+        if (!last && at == 0) open = {item, tile, 2 * head + !begin, 1 + (t.units - to + sh.size - 1) / sh.size};
         left -= to - at;
         at = 0;
         ++tile;
