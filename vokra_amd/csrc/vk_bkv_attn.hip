@@ -211,13 +211,12 @@ __device__ __forceinline__ float2 bkv_get2(const float* p) {
 }
 
 // Values d .. d + 3 of a column from the partial results of its key ranges,
-// joined in the ranges' order, eight ranges' loads in flight. pm, po: the first
-// range's (max, sum) and outputs, cols columns a slot; range s > 0 is s * step - back
-// slots behind. SAME: written by this launch.
-template <int HD, bool SAME>
+// joined in the ranges' order, B ranges' loads in flight. pm, po: the first range's
+// (max, sum) and outputs, cols columns a slot; range s > 0 is s * step - back slots
+// behind. SAME: written by this launch.
+template <int HD, bool SAME, int B>
 __device__ __forceinline__ vk_f32x4 bkv_join(const float* pm, const float* po, int ranges, int cols, int step,
                                               int back) {
-    constexpr int B = 8;
     float m = -INFINITY, sum = 0.0f;
     vk_f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s = 0; s < ranges; s += B) {
@@ -711,7 +710,7 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(BkvAt
     for (int c = threadIdx.x / PT; c < t.n; c += 64 * kWaves / PT) {
         const int d = (threadIdx.x % PT) * 4;
         *(vk_f32x4*)(a.out + w.row(a, t, head, c) + d) =
-            bkv_join<HD, true>(a.part + (first + c) * 2, a.part + a.part_o + (first + c) * HD + d, ranges, a.cols,
+            bkv_join<HD, true, 8>(a.part + (first + c) * 2, a.part + a.part_o + (first + c) * HD + d, ranges, a.cols,
                                1, 0);
     }
 }
@@ -724,9 +723,9 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(BkvAt
 // for each key range of each tile left 40 % of the waves' places empty at six chunks
 // of 450 .. 1030 rows over up to 4500 keys, 16 heads over 2 of 128, and finer ranges
 // cost more to join than they gave: 264 us against 204 with shares.
-// That call takes 188 us now: 0.43 PFLOP/s of the operator, 0.86 of fp16 products.
+// That call takes 183 us now: 0.44 PFLOP/s of the operator, 0.88 of fp16 products.
 // Of a unit's time about a quarter each is the products and the weights, the
-// rest starts, joins (20 us: 96 MB) and waits for the four waves' common units.
+// rest starts, joins (15 us: 96 MB) and waits for the four waves' common units.
 
 // The least share, in units (five sequences of up to 1000 keys and 61 rows: 30 us, 33
 // with 8, 41 with 12), and a tile's start and end (2: 212 us for the call above, 5:
@@ -1015,7 +1014,8 @@ __global__ __launch_bounds__(256, 2) void vk_bkv_attn_chunk(BkvAttnArgs a, const
     if (threadIdx.x == 0) a.open[sh.index] = open;
 }
 
-// The pieces of a tile of chunks (share blockIdx.x has the first), HD / 4 threads a column.
+// The pieces of a tile of chunks (share blockIdx.x has the first), HD / 4 threads a
+// column. Mostly two or three: eight loads in flight made the call above 5 us longer.
 template <int HD>
 __global__ __launch_bounds__(256) void vk_bkv_attn_join(BkvAttnArgs a) {
     constexpr int PT = HD / 4;
@@ -1029,7 +1029,7 @@ __global__ __launch_bounds__(256) void vk_bkv_attn_join(BkvAttnArgs a) {
     const size_t first = (size_t)(2 * blockIdx.x + second) * kChunkCols + c;
     const int cc = t.c0 + c, j = cc / a.g;
     *(vk_f32x4*)(a.out + ((size_t)(t.it.row0 + j) * a.hq + head * a.g + (cc - j * a.g)) * HD + d) =
-        bkv_join<HD, false>(a.part + first * 2, a.part + a.part_o + first * HD + d, o.pieces, kChunkCols, 2, second);
+        bkv_join<HD, false, 2>(a.part + first * 2, a.part + a.part_o + first * HD + d, o.pieces, kChunkCols, 2, second);
 }
 
 // The key ranges of items of 17 to 32 columns (their own last workgroup would take
@@ -1045,7 +1045,7 @@ __global__ __launch_bounds__(256) void vk_bkv_attn_merge(BkvAttnArgs a) {
     const size_t first = ((size_t)blockIdx.x * a.v.n_head + head) * a.splits * a.cols + c;
     const int j = bkv_div(c, a.g_inv);
     *(vk_f32x4*)(a.out + ((size_t)(t.it.row0 + j) * a.hq + head * a.g + (c - j * a.g)) * HD + d) =
-        bkv_join<HD, false>(a.part + first * 2, a.part + a.part_o + first * HD + d, (t.units + t.per - 1) / t.per, a.cols,
+        bkv_join<HD, false, 8>(a.part + first * 2, a.part + a.part_o + first * HD + d, (t.units + t.per - 1) / t.per, a.cols,
                             1, 0);
 }
 
