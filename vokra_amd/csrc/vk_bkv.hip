@@ -285,7 +285,7 @@ __device__ __forceinline__ float* bkv_ring(const BkvView& v, int layer, int seq,
 // puts the rows of the item's last two blocks into the ring; it alone reads ring
 // rows (those that earlier steps brought), before it writes any, so no two waves
 // meet there. Bound by memory, 5 bytes a value: 17.7 thousand rows of 8 heads of 128
-// (K and V, blocks of 32) take 52 us, 3.5 TB/s; 64 rows take 4.4 us, which is the
+// (K and V, blocks of 32) take 48 us, 3.8 TB/s; 64 rows take 4.4 us, which is the
 // launch and three dependent rounds of memory.
 template <int CODEC, int NT>
 __global__ __launch_bounds__(256) void vk_bkv_write(BkvView v, int layer, int n_rows, unsigned wg0,
@@ -371,9 +371,14 @@ __global__ __launch_bounds__(256) void vk_bkv_write(BkvView v, int layer, int n_
 // workgroup takes up to 16 rows: where each is comes once into LDS, then a
 // thread widens four values of each of its rows at a time (V: the row's byte of
 // each word of a 16-byte piece, whose other bytes are the rows beside it), all
-// rows' loads in flight. Bound by memory, 5 bytes a value: 17.7 thousand rows of 8
-// heads of 128 take 50 us, 3.6 TB/s.
+// rows' loads in flight. The rows go past the caches: they are what a cache cannot
+// hold, the pages may be (four layers of 17.7 thousand rows of 8 heads of 128, written
+// and read: 399 us against 440). Bound by memory, 5 bytes a value: those rows take 47
+// us, 3.9 TB/s.
 constexpr int kReadRows = 16;
+__device__ __forceinline__ void bkv_stream(float* p, const float4& x) {
+    __builtin_nontemporal_store(vk_f32x4{x.x, x.y, x.z, x.w}, (vk_f32x4*)p);
+}
 template <int CODEC>
 __device__ __forceinline__ float bkv_decode1(uint32_t w) {  // the low byte of a word
     if constexpr (CODEC == BKV_INT8) return (float)(w & 255u) - 128.0f;
@@ -422,8 +427,8 @@ __global__ __launch_bounds__(256) void vk_bkv_read(BkvView v, int layer, int n, 
                 y = *(const float4*)p;
                 z = *(const float4*)(p + (size_t)v.n_head * 2 * bs * hd);
             }
-            *(float4*)(k + (size_t)(r0 + r) * w + c * 4) = y;
-            *(float4*)(vv + (size_t)(r0 + r) * w + c * 4) = z;
+            bkv_stream(k + (size_t)(r0 + r) * w + c * 4, y);
+            bkv_stream(vv + (size_t)(r0 + r) * w + c * 4, z);
         }
     }
 }
@@ -605,7 +610,8 @@ __global__ __launch_bounds__(BKV_TPB) void vk_bkv_copy_plan(BkvView dv, BkvView 
 }
 
 // The moves' bytes and scales, every layer: runs of n_head * 2 * bs * hd bytes.
-// Bound by memory: 210 MB of pages moved in 92 us, 4.6 TB/s read and written.
+// Bound by memory: 210 MB of pages move in 74 us, 5.7 TB/s read and written, some of
+// it in the cache behind the L2s; with stores past the caches 30 us longer.
 __global__ __launch_bounds__(256) void vk_bkv_move_pages(BkvView dv, BkvView sv) {
     const int n = dv.meta[BKV_MOVE_N];
     const size_t run = (size_t)dv.n_head * 2 * dv.bs * dv.hd;

@@ -12,11 +12,11 @@
 // tokens in them (integer adds, so their order does not matter) and then holds
 // the last bias entry of each (integer max); each list is read by every workgroup
 // of its row, from cache, and skipped where a row has none. Each column is
-// written once. Bound by those 8 bytes a column: 192 rows of 128259 columns with up
-// to 2048 tokens and 300 biases a row take 54 us (3.7 TB/s), 48 of them with the
-// lists left out; 32 rows of 32000 columns take 8.8 us, which is dependent rounds
-// of memory. Two tables at once, filled between the same barriers, took 69 us: 33 KB
-// of LDS leave half the waves.
+// read and written once, past the caches. Bound by those 8 bytes: 192 rows of 128259
+// columns with up to 2048 tokens and 300 biases a row take 50 us (4.0 TB/s; 54 through
+// the caches, 256 rows of 100000 with a mask 46 against 56); 32 rows of 32000 columns
+// take 8.5 us, which is dependent rounds of memory. Two tables at once, filled between
+// the same barriers, took 15 us longer: 33 KB of LDS leave half the waves.
 // The choice: each workgroup's best goes into the row's 64-bit maximum (value,
 // then the lower index: the order of the workgroups does not matter), and the
 // last of the row's workgroups writes it out and clears it for the next call.
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(RU_T) void vk_rules(RulesArgs a) {
     for (int j = 0; j < RU_VEC; ++j) {
         const int c = c0 + 4 * (t + RU_T * j);
         if (c >= 0 && c + 3 < a.vocab) {
-            const float4 x4 = *(const float4*)(x + c);
+            const vk_f32x4 x4 = __builtin_nontemporal_load((const vk_f32x4*)(x + c));
             y[4 * j] = x4.x, y[4 * j + 1] = x4.y, y[4 * j + 2] = x4.z, y[4 * j + 3] = x4.w;
         } else {
 #pragma unroll
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(RU_T) void vk_rules(RulesArgs a) {
         }
         if (c >= 0 && c + 3 < a.vocab) {
             if (out && vec) {
-                *(float4*)(out + c) = make_float4(z[0], z[1], z[2], z[3]);
+                __builtin_nontemporal_store(vk_f32x4{z[0], z[1], z[2], z[3]}, (vk_f32x4*)(out + c));
             } else if (out) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) out[c + i] = z[i];
