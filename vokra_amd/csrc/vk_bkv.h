@@ -23,7 +23,6 @@ enum {
     BKV_STATUS,      // status of the last step / fork / free / copy (VOKRA_HIP_OK, _INVALID_ARGUMENT, _EXHAUSTED)
     BKV_DONE,        // its items done
     BKV_STEP_N,      // items of the current step
-    BKV_STEP_ROWS,   // rows of the current step
     BKV_WORK_N,      // blocks of the current step's write
     BKV_MOVE_N,      // page moves of the last copy / compact
     BKV_PLAN_N,      // items of the last fork / free / copy

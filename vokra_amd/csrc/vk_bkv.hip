@@ -238,7 +238,6 @@ __global__ __launch_bounds__(BKV_TPB) void vk_bkv_step(BkvView v, int n, int n_r
                                           : VOKRA_HIP_ERROR_INVALID_ARGUMENT;
         v.meta[BKV_DONE] = done;
         v.meta[BKV_STEP_N] = done;
-        v.meta[BKV_STEP_ROWS] = done ? s_item[done - 1].row0 + s_item[done - 1].count : 0;
         v.meta[BKV_WORK_N] = n_work;
     }
 }
@@ -258,16 +257,12 @@ __device__ __forceinline__ float bkv_e4m3_f32(uint32_t byte) {
 template <int CODEC>
 __device__ __forceinline__ uint32_t bkv_encode4(float a, float b, float c, float d) {
     if constexpr (CODEC == BKV_INT8) {
-        const int ia = (int)rintf(a) + 128, ib = (int)rintf(b) + 128, ic = (int)rintf(c) + 128, id = (int)rintf(d) + 128;
+        const int ia = (int)rintf(a) + 128, ib = (int)rintf(b) + 128;
+        const int ic = (int)rintf(c) + 128, id = (int)rintf(d) + 128;
         return (uint32_t)ia | ((uint32_t)ib << 8) | ((uint32_t)ic << 16) | ((uint32_t)id << 24);
     } else {
         return bkv_e4m3_pk(a, b) | (bkv_e4m3_pk(c, d) << 16);
     }
-}
-template <int CODEC>
-__device__ __forceinline__ float bkv_decode(uint32_t byte) {
-    if constexpr (CODEC == BKV_INT8) return (float)((int)byte - 128);
-    else return bkv_e4m3_f32(byte);
 }
 
 __device__ __forceinline__ size_t bkv_chunk(const BkvView& v, int layer, int page, int head) {
@@ -310,7 +305,8 @@ __global__ __launch_bounds__(256) void vk_bkv_write(BkvView v, int layer, int n_
             const int t0 = e.block * bs + p / pieces * 16, d0 = p % pieces * 64;
             if (side == 0) {  // token lane % 16, values 4 (lane / 16) .. + 0, 16, 32, 48
                 const int t = t0 + (lane & 15), d = d0 + (lane >> 4) * 4;
-                const float* r = t >= e.start ? in + (size_t)(t - e.start) * rs + d : ring + (size_t)(t & mask) * hd + d;
+                const float* r = t >= e.start ? in + (size_t)(t - e.start) * rs + d
+                                              : ring + (size_t)(t & mask) * hd + d;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float4 y = *(const float4*)(r + 16 * j);
@@ -403,7 +399,7 @@ __global__ __launch_bounds__(256) void vk_bkv_read(BkvView v, int layer, int n, 
     }
     __syncthreads();
     const int w4 = w >> 2, hd_log = 31 - __clz(hd), at_once = w4 < 256 ? 256 / w4 : 1;
-    const int first = at_once > 1 ? (int)threadIdx.x / w4 : 0, c0 = at_once > 1 ? (int)threadIdx.x % w4 : (int)threadIdx.x;
+    const int t0 = (int)threadIdx.x, first = at_once > 1 ? t0 / w4 : 0, c0 = at_once > 1 ? t0 % w4 : t0;
     if (first >= at_once) return;
     for (int c = c0; c < w4; c += 256) {
         const int head = c * 4 >> hd_log, d = c * 4 & (hd - 1);
@@ -541,7 +537,7 @@ __global__ __launch_bounds__(BKV_TPB) void vk_bkv_free_plan(BkvView v, int n, co
         v.meta[BKV_STATUS] = done == n ? VOKRA_HIP_OK : VOKRA_HIP_ERROR_INVALID_ARGUMENT;
         v.meta[BKV_DONE] = done;
         v.meta[BKV_PLAN_N] = done;
-        v.meta[BKV_STEP_N] = v.meta[BKV_STEP_ROWS] = v.meta[BKV_WORK_N] = 0;  // a step ends with a free
+        v.meta[BKV_STEP_N] = v.meta[BKV_WORK_N] = 0;  // a step ends with a free
     }
 }
 
@@ -805,7 +801,8 @@ constexpr unsigned kMoveGrid = 2048;
 hipError_t launch_bkv_copy(hipStream_t s, const BkvView& dv, const BkvView& sv, int n, const int* src,
                            const int* dst) {
     // all threads, as the pages of few items are many: 1600 pages 15 -> 11 us
-    hipLaunchKernelGGL(vk_bkv_copy_plan, dim3(1), dim3(BKV_TPB), 0, s, dv, sv, (int)(dv.meta == sv.meta), n, src, dst);
+    hipLaunchKernelGGL(vk_bkv_copy_plan, dim3(1), dim3(BKV_TPB), 0, s, dv, sv, (int)(dv.meta == sv.meta), n, src,
+                       dst);
     if (n) {
         hipLaunchKernelGGL(vk_bkv_move_pages, dim3(kMoveGrid), dim3(256), 0, s, dv, sv);
         hipLaunchKernelGGL(vk_bkv_copy_rows, dim3(row_grid(dv, n)), dim3(256), 0, s, dv, sv);

@@ -146,7 +146,9 @@ __device__ __forceinline__ half8v bkv_widen8(uint32_t w0, uint32_t w1) {
     return half8v{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
-__device__ __forceinline__ uint32_t u4c(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ uint32_t u4c(const uint4& v, int i) {
+    return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
 
 // hi = fp16(x), lo = fp16(x - hi) of two values
 __device__ __forceinline__ void bkv_split2(float x, float y, half2v& hi, half2v& lo) {
@@ -497,8 +499,8 @@ struct BkvPlace {
 constexpr int kWaves = 4;  // of the kernel below
 
 template <int HD, int CODEC, int C>
-__global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(BkvAttnArgs a, const uint8_t* __restrict__ pool,
-                                                                   const float2* __restrict__ scales) {
+__global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(
+    BkvAttnArgs a, const uint8_t* __restrict__ pool, const float2* __restrict__ scales) {
     using W = BkvWave<HD, C, false>;
     constexpr int U = W::U, DT = W::DT, OS = HD + 4;
     // q's parts while keys are read (16 columns: in each wave's registers instead),
@@ -1045,8 +1047,8 @@ __global__ __launch_bounds__(256) void vk_bkv_attn_merge(BkvAttnArgs a) {
     const size_t first = ((size_t)blockIdx.x * a.v.n_head + head) * a.splits * a.cols + c;
     const int j = bkv_div(c, a.g_inv);
     *(vk_f32x4*)(a.out + ((size_t)(t.it.row0 + j) * a.hq + head * a.g + (c - j * a.g)) * HD + d) =
-        bkv_join<HD, false, 8>(a.part + first * 2, a.part + a.part_o + first * HD + d, (t.units + t.per - 1) / t.per, a.cols,
-                            1, 0);
+        bkv_join<HD, false, 8>(a.part + first * 2, a.part + a.part_o + first * HD + d, (t.units + t.per - 1) / t.per,
+                               a.cols, 1, 0);
 }
 
 template <int HD, int CODEC>

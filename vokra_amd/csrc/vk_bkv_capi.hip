@@ -62,7 +62,8 @@ int check_layer(const vokra_hip_bkv* kv, size_t layer) {
 // Host ids into the cache's staging: array k of the call.
 int stage_ids(vokra_hip_bkv* kv, int k, const int32_t* ids, size_t n, const int** d) {
     int* p = kv->items + (size_t)k * kBkvMaxItems;
-    BK_TRY(hipMemcpyAsync(p, ids, n * sizeof(int32_t), hipMemcpyHostToDevice, vk::ctx_stream(kv->ctx)), "hipMemcpyAsync");
+    BK_TRY(hipMemcpyAsync(p, ids, n * sizeof(int32_t), hipMemcpyHostToDevice, vk::ctx_stream(kv->ctx)),
+           "hipMemcpyAsync");
     *d = p;
     return VOKRA_HIP_OK;
 }
@@ -239,7 +240,8 @@ int vokra_hip_bkv_step_dev(vokra_hip_ctx_t* c, vokra_hip_bkv_t* kv, size_t n, si
                            size_t max_len, const int32_t* d_seqs, const int32_t* d_starts, const int32_t* d_counts) {
     BK_ST(check(c, kv, "bkv_step"));
     BK_ST(check_items(n, "bkv_step"));
-    if (n_rows > kv->max_rows) return ctx_fail(BAD, "bkv_step: %zu rows, the cache takes %zu a step", n_rows, kv->max_rows);
+    if (n_rows > kv->max_rows)
+        return ctx_fail(BAD, "bkv_step: %zu rows, the cache takes %zu a step", n_rows, kv->max_rows);
     if (n && (!d_seqs || !d_starts || !d_counts)) return ctx_fail(BAD, "bkv_step: NULL buffer");
     return step_launch(kv, n, n_rows, std::min(max_count, n_rows), max_len, d_seqs, d_starts, d_counts);
 }
@@ -256,7 +258,8 @@ int vokra_hip_bkv_step(vokra_hip_ctx_t* c, vokra_hip_bkv_t* kv, size_t n, const 
         max_count = std::max(max_count, count);
         max_len = std::max(max_len, (size_t)std::max(starts[i], 0) + count);
     }
-    if (n_rows > kv->max_rows) return ctx_fail(BAD, "bkv_step: %zu rows, the cache takes %zu a step", n_rows, kv->max_rows);
+    if (n_rows > kv->max_rows)
+        return ctx_fail(BAD, "bkv_step: %zu rows, the cache takes %zu a step", n_rows, kv->max_rows);
     const int *ds = nullptr, *da = nullptr, *dc = nullptr;
     if (n) {
         BK_ST(stage_ids(kv, 0, seqs, n, &ds));
