@@ -725,7 +725,7 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(
 // for each key range of each tile left 40 % of the waves' places empty at six chunks
 // of 450 .. 1030 rows over up to 4500 keys, 16 heads over 2 of 128, and finer ranges
 // cost more to join than they gave: 264 us against 204 with shares.
-// That call takes 183 us now: 0.44 PFLOP/s of the operator, 0.88 of fp16 products.
+// That call takes 182 us now: 0.40 PFLOP/s of the operator, 0.80 of fp16 products.
 // Of a unit's time about a quarter each is the products and the weights, the
 // rest starts, joins (15 us: 96 MB) and waits for the four waves' common units.
 
