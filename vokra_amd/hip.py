@@ -800,8 +800,7 @@ class BlockKvCache:
         return out
 
     def attn_dev(self, layer, n_head_q, d_q, scale, d_out):
-        _check(lib().vokra_hip_bkv_attn_dev(self._ctx._h, self._h, layer, n_head_q, d_q.ptr, C.c_float(scale),
-                                            d_out.ptr))
+        _check(lib().vokra_hip_bkv_attn_dev(self._ctx._h, self._h, layer, n_head_q, d_q.ptr, float(scale), d_out.ptr))
 
     def read(self, layer, seqs, times):
         """(k, v) rows [n, n_head * d_head] as the cache holds them, zeros where none is."""
@@ -891,19 +890,19 @@ class RopePlan:
                   k_stride=None, q_out_stride=None, k_out_stride=None):
         """Rows of q and k at positions[r]; an output may be its input. Strides in
         floats; where not given, the heads' width, and in place the input's."""
-        def st(x, n):
-            return n * self.head_dim if x is None else x
-        if d_q_out is d_q and q_out_stride is None:
-            q_out_stride = q_stride
-        if d_k_out is d_k and k_out_stride is None:
-            k_out_stride = k_stride
-
-        def p(x):
-            return None if x is None else x.ptr
+        wq, wk = n_head_q * self.head_dim, n_head_k * self.head_dim
+        if q_stride is None:
+            q_stride = wq
+        if q_out_stride is None:
+            q_out_stride = q_stride if d_q_out is d_q else wq
+        if k_stride is None:
+            k_stride = wk
+        if k_out_stride is None:
+            k_out_stride = k_stride if d_k_out is d_k else wk
         _check(lib().vokra_hip_rope_apply_dev(
-            self._ctx._h, self._h, rows, d_positions.ptr, n_head_q, p(d_q), st(q_stride, n_head_q), p(d_q_out),
-            st(q_out_stride, n_head_q), n_head_k, p(d_k), st(k_stride, n_head_k), p(d_k_out),
-            st(k_out_stride, n_head_k)))
+            self._ctx._h, self._h, rows, d_positions.ptr, n_head_q, None if d_q is None else d_q.ptr, q_stride,
+            None if d_q_out is None else d_q_out.ptr, q_out_stride, n_head_k, None if d_k is None else d_k.ptr, k_stride,
+            None if d_k_out is None else d_k_out.ptr, k_out_stride))
 
     def apply(self, positions, q=None, k=None):
         """Host rows [n, heads * head_dim]; returns (q, k), None where none is given."""
