@@ -427,7 +427,7 @@ typedef struct vokra_hip_bkv vokra_hip_bkv_t;
  * d_head 64 or 128 and block_size 16, 32 or 64 (else UNSUPPORTED_OP). Device
  * memory: n_layer * n_head * (n_page * (2 * block_size * d_head + 8) + n_seq *
  * 16 * block_size * d_head) bytes and some tables; the first cache of a
- * context also takes 137 MB for split attention, which all its caches share.
+ * context also takes 68 MB for split attention, which all its caches share.
  * Nothing is allocated by the _dev calls, so all of them can be captured into a
  * graph. A cache belongs to its context's stream: calls on one cache run in the
  * order in which they are made. */

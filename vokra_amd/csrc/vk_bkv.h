@@ -9,11 +9,11 @@
 #include <stdint.h>
 
 constexpr int kBkvMaxItems = 1024;   // items of one call: one thread of the planning workgroup each
-constexpr int kBkvParts = 1 << 18;  // query rows of which a split attention can hold a partial result
+constexpr int kBkvParts = 1 << 17;  // query rows of which a split attention can hold a partial result
 constexpr int kBkvShares = 512;  // workgroups that share a chunked attention: two a CU
 // a context's partial results ((max, sum) and up to 128 values a row), counters,
 // and the tiles that go on in a later share
-constexpr size_t kBkvPartBytes = (size_t)kBkvParts * (128 + 2 + 1) * 4 + kBkvShares * 16;
+constexpr size_t kBkvPartBytes = (size_t)kBkvParts * (128 + 2) * 4 + kBkvShares * (4 + 16);
 
 // What planning kernels leave for the kernels of the same call or step.
 // meta (int32): see the BKV_ indices.

@@ -66,7 +66,6 @@ struct BkvAttnArgs {
     int n, rows, count; // most items, rows, and rows an item: items beyond are passed over
     uint32_t g_inv, splits_inv;  // ceil(2^32 / g), ceil(2^32 / splits): see bkv_div
     BkvOpen* open;      // of each share: the tile whose first piece is its last
-    int tile0;          // first item of this launch
     int tiles;          // chunks: places of tiles, see bkv_share
     int splits;         // key ranges an item may have (grid)
     int per;            // least units of a key range
@@ -513,7 +512,7 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(
     __shared__ float2 sml[kWaves][16];
     __shared__ bool s_last;
     // ranges are the grid's slowest index: those that short items do not have come last
-    const int tile = a.tile0 + (int)blockIdx.x, head = blockIdx.y, split = blockIdx.z;
+    const int tile = blockIdx.x, head = blockIdx.y, split = blockIdx.z;
     BkvTile t;
     if (!bkv_tile(a, tile, t) || t.beyond(split)) return;
     const BkvView& v = a.v;
@@ -1039,7 +1038,7 @@ __global__ __launch_bounds__(256) void vk_bkv_attn_join(BkvAttnArgs a) {
 template <int HD>
 __global__ __launch_bounds__(256) void vk_bkv_attn_merge(BkvAttnArgs a) {
     constexpr int PT = HD / 4;
-    const int head = blockIdx.y, tile = a.tile0 + (int)blockIdx.x;
+    const int head = blockIdx.y, tile = blockIdx.x;
     BkvTile t;
     if (!bkv_tile(a, tile, t) || t.one()) return;
     const int c = blockIdx.z * (256 / PT) + threadIdx.x / PT, d = (threadIdx.x % PT) * 4;
@@ -1089,10 +1088,9 @@ hipError_t launch_bkv_attn(hipStream_t s, const BkvView& v, int layer, int n, in
     a.count = max_count;
     const long long cols = (long long)max_count * a.g;
     const int tc = cols <= 16 ? 16 : cols <= 32 ? 32 : kChunkCols;
-    const int room = kBkvParts;
-    a.part_o = (size_t)room * 2;
-    a.joined = (unsigned*)(part + (size_t)room * (128 + 2));
-    a.open = (BkvOpen*)(a.joined + room);
+    a.part_o = (size_t)kBkvParts * 2;
+    a.joined = (unsigned*)(part + (size_t)kBkvParts * (128 + 2));
+    a.open = (BkvOpen*)(a.joined + kBkvShares);
     auto inv = [](int d) { return d == 1 ? 0u : (uint32_t)(((1ull << 32) + (uint32_t)d - 1) / (uint32_t)d); };
     a.g_inv = inv(a.g);
     auto go = [&](dim3 grid) { v.hd == 64 ? go_hd<64>(s, a, tc, grid) : go_hd<128>(s, a, tc, grid); };
@@ -1114,18 +1112,14 @@ hipError_t launch_bkv_attn(hipStream_t s, const BkvView& v, int layer, int n, in
     // together least near the root of twice the units (one sequence of 32768 keys, 8
     // kv heads: 45 ranges 23.5 us, 64 28.6, 16 29.7; of 12000 keys, one kv head: 27
     // 12.9, 64 14.6).
-    const long long most = std::min<long long>(std::max(8, (int)std::sqrt(2.0 * units)),
-                                               std::max<long long>(1, room / ((long long)v.n_head * a.cols)));
+    const long long most = std::max(8, (int)std::sqrt(2.0 * units));
     a.per = (int)((std::max(per, (units + most - 1) / most) + 3) / 4 * 4);
     a.splits = (units + a.per - 1) / a.per;
     a.splits_inv = inv(a.splits);
-    // items a launch: what the workspace holds
-    const long long step =
-        a.splits == 1 ? n : std::max<long long>(1, room / ((long long)v.n_head * a.cols * a.splits));
-    for (long long t0 = 0; t0 < n; t0 += step) {
-        a.tile0 = (int)t0;
-        go(dim3((unsigned)std::min(step, n - t0), (unsigned)v.n_head, (unsigned)a.splits));
-    }
+    // More than one range only where n * n_head < 512 (per >= units above), and then
+    // fewer than 1100 ranges of up to 32 columns in all: the workspace holds them.
+    static_assert(1100 * 32 <= kBkvParts && kBkvShares == 512, "");
+    go(dim3((unsigned)n, (unsigned)v.n_head, (unsigned)a.splits));
     return hipGetLastError();
 }
 
