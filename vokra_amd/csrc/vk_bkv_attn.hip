@@ -19,7 +19,7 @@
 // 9 .. 65 thousand keys, e4m3, 32 heads over 8 of 128, up to 4 rows: 457 MB in 97
 // us, 4.7 TB/s, a large copy's rate here is 4.9), by dependent rounds of memory
 // (item, page, keys, results, join: 8 us) where there are few: 32 streams of 512 ..
-// 4096 keys, 16 heads over 2 of 128, take 17.6 us for 38 MB. Four waves a workgroup,
+// 4096 keys, 16 heads over 2 of 128, take 17.1 us for 38 MB. Four waves a workgroup,
 // three workgroups a CU: eight waves took 28 us for those, and two units' loads in
 // flight a wave spilled or left two workgroups.
 // The 8-bit values are exact in fp16, so a product is two fp16 matrix
@@ -199,8 +199,10 @@ struct BkvScale {
     }
 };
 
-// A value that a workgroup on another XCD reads in this launch: past the caches
-// that are the XCD's own.
+// Values that a workgroup on another XCD reads in this launch: past the caches
+// that are the XCD's own. Four at a time by the buffer instructions, whose policy
+// bit 4 (sc1) is what an access of the device's scope carries; with pairs 32 streams
+// took 17.6 us, 17.1 so.
 __device__ __forceinline__ void bkv_put2(float* p, float a, float b) {
     const unsigned long long v = ((unsigned long long)__float_as_uint(b) << 32) | __float_as_uint(a);
     __hip_atomic_store((unsigned long long*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -211,13 +213,23 @@ __device__ __forceinline__ float2 bkv_get2(const float* p) {
     return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
+__device__ __forceinline__ void bkv_put4(float* out, size_t at, vk_f32x4 x) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)out, 0, kBkvParts * 128 * 4, 0x20000);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, x), r, (int)(at * 4), 0, 16);
+}
+__device__ __forceinline__ vk_f32x4 bkv_get4(const float* out, size_t at) {
+    const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)out, 0, kBkvParts * 128 * 4, 0x20000);
+    return __builtin_bit_cast(vk_f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(at * 4), 0, 16));
+}
+
 // Values d .. d + 3 of a column from the partial results of its key ranges,
-// joined in the ranges' order, B ranges' loads in flight. pm, po: the first range's
-// (max, sum) and outputs, cols columns a slot; range s > 0 is s * step - back slots
-// behind. SAME: written by this launch.
+// joined in the ranges' order, B ranges' loads in flight. pm: the first range's
+// (max, sum), part_o + o: its outputs, cols columns a slot; range s > 0 is s * step -
+// back slots behind. SAME: written by this launch.
 template <int HD, bool SAME, int B>
-__device__ __forceinline__ vk_f32x4 bkv_join(const float* pm, const float* po, int ranges, int cols, int step,
-                                              int back) {
+__device__ __forceinline__ vk_f32x4 bkv_join(const float* pm, const float* part_o, size_t o0, int ranges,
+                                              int cols, int step, int back) {
     float m = -INFINITY, sum = 0.0f;
     vk_f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s = 0; s < ranges; s += B) {
@@ -229,11 +241,10 @@ __device__ __forceinline__ vk_f32x4 bkv_join(const float* pm, const float* po, i
             const size_t at = r ? (size_t)(r * step - back) * cols : 0;
             if constexpr (SAME) {
                 ml[x] = bkv_get2(pm + at * 2);
-                const float2 a = bkv_get2(po + at * HD), b = bkv_get2(po + at * HD + 2);
-                o[x] = vk_f32x4{a.x, a.y, b.x, b.y};
+                o[x] = bkv_get4(part_o, o0 + at * HD);
             } else {
                 ml[x] = *(const float2*)(pm + at * 2);
-                o[x] = *(const vk_f32x4*)(po + at * HD);
+                o[x] = *(const vk_f32x4*)(part_o + o0 + at * HD);
             }
         }
         float to = m;
@@ -681,15 +692,17 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(
                 for (int i = 0; i < PD; ++i) dst[i] = y[i] * f;
             } else {
                 const size_t at = slot * a.cols + ct * 16 + c;
-                float *pm = a.part + at * 2, *po = a.part + a.part_o + at * HD + d0;
+                float* pm = a.part + at * 2;
                 if constexpr (C == 1) {
                     if (d0 == 0) bkv_put2(pm, m, sum);
 #pragma unroll
-                    for (int i = 0; i < PD; i += 2) bkv_put2(po + i, y[i] * 0x1p-14f, y[i + 1] * 0x1p-14f);
+                    for (int i = 0; i < PD; i += 4)
+                        bkv_put4(a.part + a.part_o, at * HD + d0 + i,
+                                 vk_f32x4{y[i], y[i + 1], y[i + 2], y[i + 3]} * 0x1p-14f);
                 } else {
                     if (d0 == 0) *(float2*)pm = make_float2(m, sum);
 #pragma unroll
-                    for (int i = 0; i < PD; ++i) po[i] = y[i] * 0x1p-14f;
+                    for (int i = 0; i < PD; ++i) a.part[a.part_o + at * HD + d0 + i] = y[i] * 0x1p-14f;
                 }
             }
         }
@@ -711,8 +724,8 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(
     for (int c = threadIdx.x / PT; c < t.n; c += 64 * kWaves / PT) {
         const int d = (threadIdx.x % PT) * 4;
         *(vk_f32x4*)(a.out + w.row(a, t, head, c) + d) =
-            bkv_join<HD, true, 8>(a.part + (first + c) * 2, a.part + a.part_o + (first + c) * HD + d, ranges, a.cols,
-                               1, 0);
+            bkv_join<HD, true, 8>(a.part + (first + c) * 2, a.part + a.part_o, (first + c) * HD + d, ranges, a.cols, 1,
+                                  0);
     }
 }
 
@@ -1030,7 +1043,7 @@ __global__ __launch_bounds__(256) void vk_bkv_attn_join(BkvAttnArgs a) {
     const size_t first = (size_t)(2 * blockIdx.x + second) * kChunkCols + c;
     const int cc = t.c0 + c, j = cc / a.g;
     *(vk_f32x4*)(a.out + ((size_t)(t.it.row0 + j) * a.hq + head * a.g + (cc - j * a.g)) * HD + d) =
-        bkv_join<HD, false, 2>(a.part + first * 2, a.part + a.part_o + first * HD + d, o.pieces, kChunkCols, 2, second);
+        bkv_join<HD, false, 2>(a.part + first * 2, a.part + a.part_o, first * HD + d, o.pieces, kChunkCols, 2, second);
 }
 
 // The key ranges of items of 17 to 32 columns (their own last workgroup would take
@@ -1046,7 +1059,7 @@ __global__ __launch_bounds__(256) void vk_bkv_attn_merge(BkvAttnArgs a) {
     const size_t first = ((size_t)blockIdx.x * a.v.n_head + head) * a.splits * a.cols + c;
     const int j = bkv_div(c, a.g_inv);
     *(vk_f32x4*)(a.out + ((size_t)(t.it.row0 + j) * a.hq + head * a.g + (c - j * a.g)) * HD + d) =
-        bkv_join<HD, false, 8>(a.part + first * 2, a.part + a.part_o + first * HD + d, (t.units + t.per - 1) / t.per,
+        bkv_join<HD, false, 8>(a.part + first * 2, a.part + a.part_o, first * HD + d, (t.units + t.per - 1) / t.per,
                                a.cols, 1, 0);
 }
 
