@@ -17,6 +17,12 @@ def ctx():
     c.close()
 
 
+class _Ids:
+    def __init__(self, ctx, a):
+        self.b = hip.DeviceBuffer.from_array(ctx, np.ascontiguousarray(a, np.int32))
+        self.ptr = self.b.ptr
+
+
 class Pair:
     """The device cache and its restatement, driven together."""
 
@@ -251,6 +257,35 @@ def test_attention(ctx, codec, bs, hd, heads, kvh, lens, counts):
     assert np.all(np.isfinite(got))
 
 
+@pytest.mark.parametrize("codec,bs,hd,heads,kvh,lens,counts", ATTN + [
+    (0, 16, 128, 16, 2, [1500, 700], [1400, 300]), (1, 64, 64, 5, 5, [1, 2, 640], [1, 2, 600])])
+def test_attention_of_steps_that_may_be_larger(ctx, codec, bs, hd, heads, kvh, lens, counts):
+    """The same under bounds far above the step's rows, which lay its work out by
+    shares of all workgroups; rows behind the step's stay as they are."""
+    print("[case] bkv attn shares", codec, bs, hd, heads, kvh, lens, counts, flush=True)
+    n, room = len(lens), 1 << 20
+    p = Pair(ctx, 1, kvh, hd, n, max(max(lens), 64), bs, sum(lens) // bs + n, room, codec, seed=sum(lens))
+    lens, counts = np.array(lens), np.array(counts)
+    p.step(np.arange(n), np.zeros(n, int), lens - counts)
+    assert p.ref.step(list(range(n)), list(lens - counts), list(counts)) == (bm.OK, n)
+    p.dev.step_dev(n, room, room, 1 << 24, *(_Ids(ctx, a) for a in (np.arange(n), lens - counts, counts)))
+    assert p.dev.status() == n
+    rows = int(counts.sum())
+    k, v = p.rows(rows)
+    q = p.g.standard_normal((rows, heads * hd)).astype(np.float32) * 2
+    up = lambda a: hip.DeviceBuffer.from_array(ctx, a)  # noqa: E731
+    out = up(np.full((rows + 1) * heads * hd, 7.5, np.float32))
+    p.dev.write_dev(0, up(k), up(v))
+    p.ref.write(0, k, v)
+    p.dev.attn_dev(0, heads, up(q), hd ** -0.5, out)
+    ctx.synchronize()
+    got = out.download(np.float32, (rows + 1) * heads * hd).reshape(rows + 1, heads * hd)
+    want, tol = p.ref.attn(0, q, heads, np.float32(hd ** -0.5))
+    err = np.abs(got[:rows].astype(np.float64) - want) / tol
+    assert np.nanmax(err) <= 1 and not np.isnan(err).any()
+    assert np.all(got[rows] == 7.5)
+
+
 def test_attention_of_large_small_and_zero_values(ctx):
     """Scales far apart between blocks and heads, zero blocks, query rows of every
     size: no overflow, and small blocks keep their bits beside large ones."""
@@ -477,12 +512,6 @@ def test_more_pages_than_32_bits_of_bytes(ctx):
     assert kv.page_of(1, 2) < 6
     again = kv.read(0, np.full(200, 1), np.arange(200))
     assert np.array_equal(again[0], rows[0]) and np.array_equal(again[1], rows[1])
-
-
-class _Ids:
-    def __init__(self, ctx, a):
-        self.b = hip.DeviceBuffer.from_array(ctx, np.ascontiguousarray(a, np.int32))
-        self.ptr = self.b.ptr
 
 
 def test_a_captured_step_replays_with_what_the_arrays_hold(ctx):

@@ -7,7 +7,7 @@
 // scale, f32 rows in the open block.
 //
 // Columns: the count_i * G query rows of an item that read one kv head.
-// vk_bkv_attn takes up to 32 of them over a range of keys; its four waves take
+// vk_bkv_attn takes 16 or 32 of them over a range of keys; its four waves take
 // the range's units of 32 keys in turn, each with an online softmax of its own,
 // and merge through LDS at the end: no barrier in the key loop. A tile of 16
 // columns whose keys are split over workgroups is joined by the last of them
@@ -64,9 +64,10 @@ struct BkvAttnArgs {
     float scale_log2;   // scale * log2(e)
     int layer, hq, g;   // g = hq / n_head
     int n, rows, count; // most items, rows, and rows an item: items beyond are passed over
-    uint32_t g_inv, splits_inv;  // ceil(2^32 / g), ceil(2^32 / splits): see bkv_div
+    uint32_t g_inv, splits_inv, parts_inv;  // ceil(2^32 / g) and so on: see bkv_div
     BkvOpen* open;      // of each share: the tile whose first piece is its last
     int tiles;          // chunks: places of tiles, see bkv_share
+    int parts;          // tiles that an item may have
     int splits;         // key ranges an item may have (grid)
     int per;            // least units of a key range
     int cols;           // columns a slot has room for
@@ -99,13 +100,15 @@ __device__ __forceinline__ void bkv_keys(const BkvView& v, BkvTile& t) {
     t.full = min((t.it.start + t.it.count) >> bs_log << bs_log, (t.keys + 15) & ~15);
     t.units = (t.full + kUnit - 1) / kUnit;
 }
-// All columns of an item (vk_bkv_attn); false: none.
-__device__ __forceinline__ bool bkv_tile(const BkvAttnArgs& a, int item, BkvTile& t) {
+// A tile of vk_bkv_attn: the columns of an item, a.cols of them where it has more; false:
+// none.
+__device__ __forceinline__ bool bkv_tile(const BkvAttnArgs& a, int tile, BkvTile& t) {
+    const int item = bkv_div(tile, a.parts_inv);
     t.it = a.v.step[item];
-    t.c0 = 0;
-    t.n = t.it.count * a.g;
+    t.c0 = (tile - item * a.parts) * a.cols;
+    t.n = min(t.it.count * a.g - t.c0, a.cols);
     if (t.n <= 0 || !bkv_fits(a, t.it)) return false;
-    t.keys = t.it.start + t.it.count;
+    t.keys = t.it.start + bkv_div(t.c0 + t.n - 1, a.g_inv) + 1;
     bkv_keys(a.v, t);
     t.per = max(a.per, (bkv_div(t.units + a.splits - 1, a.splits_inv) + 3) & ~3);
     return true;
@@ -290,7 +293,7 @@ struct BkvWave {
     }
     // the row of the item that holds column c of the tile (c < 16 C of the kernel's; chunks: any)
     __device__ __forceinline__ int item_row(const BkvAttnArgs& a, const BkvTile& t, int c) const {
-        return CHUNKS ? (t.c0 + c) / a.g : bkv_div(c, a.g_inv);
+        return CHUNKS ? (t.c0 + c) / a.g : bkv_div(t.c0 + c, a.g_inv);
     }
     // place in q and out of column c of the tile (of column 0 for one beyond its columns)
     __device__ __forceinline__ size_t row(const BkvAttnArgs& a, const BkvTile& t, int head, int c) const {
@@ -1046,7 +1049,7 @@ __global__ __launch_bounds__(256) void vk_bkv_attn_join(BkvAttnArgs a) {
         bkv_join<HD, false, 2>(a.part + first * 2, a.part + a.part_o, first * HD + d, o.pieces, kChunkCols, 2, second);
 }
 
-// The key ranges of items of 17 to 32 columns (their own last workgroup would take
+// The key ranges of tiles of 17 to 32 columns (their own last workgroup would take
 // longer over them than a launch does): HD / 4 threads a column.
 template <int HD>
 __global__ __launch_bounds__(256) void vk_bkv_attn_merge(BkvAttnArgs a) {
@@ -1057,8 +1060,8 @@ __global__ __launch_bounds__(256) void vk_bkv_attn_merge(BkvAttnArgs a) {
     const int c = blockIdx.z * (256 / PT) + threadIdx.x / PT, d = (threadIdx.x % PT) * 4;
     if (c >= t.n) return;
     const size_t first = ((size_t)blockIdx.x * a.v.n_head + head) * a.splits * a.cols + c;
-    const int j = bkv_div(c, a.g_inv);
-    *(vk_f32x4*)(a.out + ((size_t)(t.it.row0 + j) * a.hq + head * a.g + (c - j * a.g)) * HD + d) =
+    const int cc = t.c0 + c, j = bkv_div(cc, a.g_inv);
+    *(vk_f32x4*)(a.out + ((size_t)(t.it.row0 + j) * a.hq + head * a.g + (cc - j * a.g)) * HD + d) =
         bkv_join<HD, false, 8>(a.part + first * 2, a.part + a.part_o, first * HD + d, (t.units + t.per - 1) / t.per,
                                a.cols, 1, 0);
 }
@@ -1100,7 +1103,15 @@ hipError_t launch_bkv_attn(hipStream_t s, const BkvView& v, int layer, int n, in
     a.rows = n_rows;
     a.count = max_count;
     const long long cols = (long long)max_count * a.g;
-    const int tc = cols <= 16 ? 16 : cols <= 32 ? 32 : kChunkCols;
+    const int units = std::max(1, (max_len + kUnit - 1) / kUnit);
+    // Tiles of 32 columns an item, or shares of tiles of 128 where those are mostly full
+    // and there is work enough for all shares, in units by such tiles: 16 heads over 2
+    // of 128, one prompt of 1000 rows (16 thousand) takes 30 us so and 39 by shares, one
+    // of 2000 (63 thousand) 71 and 64; 8 sequences of up to 4096 keys and 16 rows, 32
+    // heads over 8, 31 and 45.
+    const long long parts = (cols + 31) / 32;
+    const bool few = cols <= 96 || (parts * n * v.n_head * units <= 48 << 10 && cols * a.g < 1ll << 32);
+    const int tc = cols <= 16 ? 16 : few ? 32 : kChunkCols;
     a.part_o = (size_t)kBkvParts * 2;
     a.joined = (unsigned*)(part + (size_t)kBkvParts * (128 + 2));
     a.open = (BkvOpen*)(a.joined + kBkvShares);
@@ -1114,13 +1125,15 @@ hipError_t launch_bkv_attn(hipStream_t s, const BkvView& v, int layer, int n, in
         go(dim3(kBkvShares));
         return hipGetLastError();
     }
-    a.cols = (int)cols;
-    const int units = std::max(1, (max_len + kUnit - 1) / kUnit);
+    a.cols = (int)std::min<long long>(cols, 32);
+    a.parts = (int)parts;
+    a.parts_inv = inv(a.parts);
+    const int tiles = a.parts * n;
     // Units a key range: the call's units at the longest rows' length over 512, so
     // that there are ranges for every CU (six sequences of 9 .. 65 thousand keys take
     // 99 us, over 256 142; over 1024, 32 streams of up to 4096 take 22.5 us against
     // 17.6), and 8 at least (16: one sequence of 2000 keys takes 10.8 us against 8.8).
-    const long long per = std::max<long long>((long long)n * v.n_head * units / 512, 8);
+    const long long per = std::max<long long>((long long)tiles * v.n_head * units / 512, 8);
     // Ranges: a wave's units fall with their number, the join's rounds rise with it;
     // together least near the root of twice the units (one sequence of 32768 keys, 8
     // kv heads: 45 ranges 23.5 us, 64 28.6, 16 29.7; of 12000 keys, one kv head: 27
@@ -1129,10 +1142,10 @@ hipError_t launch_bkv_attn(hipStream_t s, const BkvView& v, int layer, int n, in
     a.per = (int)((std::max(per, (units + most - 1) / most) + 3) / 4 * 4);
     a.splits = (units + a.per - 1) / a.per;
     a.splits_inv = inv(a.splits);
-    // More than one range only where n * n_head < 512 (per >= units above), and then
+    // More than one range only where tiles * n_head < 512 (per >= units above), and then
     // fewer than 1100 ranges of up to 32 columns in all: the workspace holds them.
     static_assert(1100 * 32 <= kBkvParts && kBkvShares == 512, "");
-    go(dim3((unsigned)n, (unsigned)v.n_head, (unsigned)a.splits));
+    go(dim3((unsigned)tiles, (unsigned)v.n_head, (unsigned)a.splits));
     return hipGetLastError();
 }
 
