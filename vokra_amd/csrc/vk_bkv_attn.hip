@@ -1111,7 +1111,10 @@ hipError_t launch_bkv_attn(hipStream_t s, const BkvView& v, int layer, int n, in
     // heads over 8, 31 and 45.
     const long long parts = (cols + 31) / 32;
     const bool few = cols <= 96 || (parts * n * v.n_head * units <= 48 << 10 && cols * a.g < 1ll << 32);
-    const int tc = cols <= 16 ? 16 : few ? 32 : kChunkCols;
+    // Of those, tiles of 16, which join in their own launch, while few keys are read twice
+    // for it: 16 sequences of up to 3000 keys, 4 rows, 16 heads over 2 take 15.3 us so and
+    // 18.5 in tiles of 32, one of 16000 keys, 8 rows, 32 heads over 8, 24.6 and 22.
+    const int tc = cols <= 16 || (few && cols * units <= 6144) ? 16 : few ? 32 : kChunkCols;
     a.part_o = (size_t)kBkvParts * 2;
     a.joined = (unsigned*)(part + (size_t)kBkvParts * (128 + 2));
     a.open = (BkvOpen*)(a.joined + kBkvShares);
@@ -1125,8 +1128,8 @@ hipError_t launch_bkv_attn(hipStream_t s, const BkvView& v, int layer, int n, in
         go(dim3(kBkvShares));
         return hipGetLastError();
     }
-    a.cols = (int)std::min<long long>(cols, 32);
-    a.parts = (int)parts;
+    a.cols = (int)std::min<long long>(cols, tc);
+    a.parts = (int)((cols + tc - 1) / tc);
     a.parts_inv = inv(a.parts);
     const int tiles = a.parts * n;
     // Units a key range: the call's units at the longest rows' length over 512, so
