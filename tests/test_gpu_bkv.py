@@ -238,6 +238,9 @@ ATTN = [  # codec, bs, hd, heads, kv heads, lens, counts
     (0, 16, 128, 32, 1, [50, 900], [1, 1]),
     (0, 16, 128, 4, 1, [9000, 20], [1, 1]),
     (1, 32, 64, 32, 1, [6001], [1]),
+    (0, 16, 64, 8, 2, [6500, 300], [16, 9]),
+    (1, 64, 128, 32, 1, [7000, 90], [1, 1]),
+    (0, 32, 128, 16, 2, [5000], [11]),
     (0, 16, 64, 20, 20, [1000, 300, 31, 640], [900, 0, 31, 600]),
     (1, 32, 128, 16, 1, [5, 2300, 77], [5, 400, 77]),
     (0, 32, 64, 3, 1, [64, 3, 500, 90] * 20, [50, 3, 1, 0] * 20),
