@@ -152,6 +152,28 @@ def test_strided_rows_in_place_and_out(ctx, layout, hd, rot, n, shift):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("layout", [HALF, PAIRS])
+def test_more_rows_than_the_caches_hold(ctx, layout):
+    """One call over 34 million values and the same rows in three: equal bits."""
+    print("[case] rope large", layout, flush=True)
+    n, h, hd = 4101, 64, 128
+    g = np.random.default_rng(9)
+    x = g.random((n, h * hd), np.float32) - np.float32(0.5)
+    pos = g.integers(0, 200000, n).astype(np.int32)
+    up = lambda a: hip.DeviceBuffer.from_array(ctx, a)  # noqa: E731
+    d, dp, whole, parts = up(x), up(pos), up(np.zeros_like(x)), up(np.zeros_like(x))
+    plan = ctx.rope_plan(hd, 64, layout)
+    plan.apply_dev(n, dp, h, d, whole)
+    for a, b in ((0, 1400), (1400, 2800), (2800, n)):
+        plan.apply_dev(b - a, _At(dp, a), h, _At(d, a * h * hd), _At(parts, a * h * hd))
+    ctx.synchronize()
+    got = whole.download(np.float32, x.size)
+    assert np.array_equal(got, parts.download(np.float32, x.size))
+    some = [0, 2047, n - 1]
+    check(got.reshape(n, -1)[some], x[some].reshape(3, h, hd), pos[some], thetas(64, 10000.0), layout)
+
+
+@pytest.mark.gpu
 def test_a_captured_turn_takes_the_positions_of_its_replay(ctx):
     print("[case] rope graph", flush=True)
     up = lambda a: hip.DeviceBuffer.from_array(ctx, a)  # noqa: E731

@@ -11,9 +11,9 @@
 //
 // Bound by memory: 8 bytes an element moved, about 40 VALU operations a pair
 // for its sine and cosine, which the heads that a thread turns share. 8191 rows of
-// 32 + 8 heads of 128, half of each turned, to another buffer: 336 MB in 62 us, 5.4
-// TB/s (they fit the cache behind the L2s); 32 rows of 16 + 2 heads take 4.9 us, the
-// launch and three dependent rounds of memory.
+// 32 + 8 heads of 128, half of each turned, to another buffer: 336 MB in 59 us, 5.7
+// TB/s (part of them in the cache behind the L2s); 32 rows of 16 + 2 heads take 4.7
+// us, the launch and three dependent rounds of memory.
 #include <algorithm>
 
 #include "vk_common.h"
@@ -41,12 +41,18 @@ __device__ __forceinline__ float2 rope_cos_sin(int pos, uint64_t turn, float mag
     return make_float2((quad == 1 || quad == 2 ? -cq : cq) * mag, (quad >= 2 ? -sq : sq) * mag);
 }
 
+template <bool PAST>
+__device__ __forceinline__ void rope_put(float* p, vk_f32x4 x) {
+    if constexpr (PAST) __builtin_nontemporal_store(x, (vk_f32x4*)p);
+    else *(vk_f32x4*)p = x;
+}
+
 // A thread turns V pairs (or copies as many floats beyond rot, where the
 // output is another buffer) of the heads hl, hl + HL, ...; units of a head run
 // fastest over the threads, then the HL head lanes, then rows.
 // V = 4 (half layout) or 2 (pairs side by side): 16-byte accesses; V = 1: any
-// size and alignment.
-template <int V, bool PAIRS>
+// size and alignment. PAST: stores go past the caches.
+template <int V, bool PAIRS, bool PAST>
 __global__ __launch_bounds__(256) void vk_rope_turn(RopeArgs a) {
     const int units = a.units;
     const size_t g = (size_t)blockIdx.x * 256 + threadIdx.x;
@@ -103,10 +109,10 @@ __global__ __launch_bounds__(256) void vk_rope_turn(RopeArgs a) {
             }
         }
         if constexpr (V == 4) {
-            *(float4*)(y + i0) = make_float4(p[0], p[1], p[2], p[3]);
-            *(float4*)(y + i1) = make_float4(r[0], r[1], r[2], r[3]);
+            rope_put<PAST>(y + i0, vk_f32x4{p[0], p[1], p[2], p[3]});
+            rope_put<PAST>(y + i1, vk_f32x4{r[0], r[1], r[2], r[3]});
         } else if constexpr (V == 2) {
-            *(float4*)(y + i0) = make_float4(p[0], p[1], r[0], r[1]);
+            rope_put<PAST>(y + i0, vk_f32x4{p[0], p[1], r[0], r[1]});
         } else {
             y[i0] = p[0];
             if (i1 < a.hd) y[i1] = r[0];
@@ -130,15 +136,15 @@ hipError_t launch_rope_turn(hipStream_t s, RopeArgs a, bool pairs) {
     const int heads = a.heads_q + a.heads_k;
     const size_t all = (size_t)a.rows * a.units * heads;
     a.head_lanes = all / 256 < 2048 ? heads : (heads + 3) / 4;
+    // outputs that the caches cannot hold beside the inputs go past them (63 us -> 59 for
+    // the call above; 1500 rows, which they hold, take 10.9 us with them and 11.2 past)
+    const bool past = v > 1 && (size_t)a.rows * heads * a.hd > (size_t)32 << 20;
     const size_t threads = (size_t)a.rows * a.units * a.head_lanes;
     const dim3 grid((unsigned)((threads + 255) / 256));
-    if (pairs) {
-        if (v == 2) hipLaunchKernelGGL((vk_rope_turn<2, true>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((vk_rope_turn<1, true>), grid, dim3(256), 0, s, a);
-    } else {
-        if (v == 4) hipLaunchKernelGGL((vk_rope_turn<4, false>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((vk_rope_turn<1, false>), grid, dim3(256), 0, s, a);
-    }
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a); };
+    if (v == 2) past ? go(vk_rope_turn<2, true, true>) : go(vk_rope_turn<2, true, false>);
+    else if (v == 4) past ? go(vk_rope_turn<4, false, true>) : go(vk_rope_turn<4, false, false>);
+    else pairs ? go(vk_rope_turn<1, true, false>) : go(vk_rope_turn<1, false, false>);
     return hipGetLastError();
 }
 
