@@ -261,13 +261,16 @@ def test_attention(ctx, codec, bs, hd, heads, kvh, lens, counts):
 
 
 @pytest.mark.parametrize("codec,bs,hd,heads,kvh,lens,counts", ATTN + [
-    (0, 16, 128, 16, 2, [1500, 700], [1400, 300]), (1, 64, 64, 5, 5, [1, 2, 640], [1, 2, 600])])
-def test_attention_of_steps_that_may_be_larger(ctx, codec, bs, hd, heads, kvh, lens, counts):
+    (0, 16, 128, 16, 2, [1500, 700], [1400, 300]), (1, 64, 64, 5, 5, [1, 2, 640], [1, 2, 600]),
+    (0, 16, 128, 24, 1, [900, 300, 40, 65], [200, 1, 1, 2])])
+@pytest.mark.parametrize("far", [False, True])
+def test_attention_of_steps_that_may_be_larger(ctx, codec, bs, hd, heads, kvh, lens, counts, far):
     """The same under bounds far above the step's rows, which lay its work out by
-    shares of all workgroups; rows behind the step's stay as they are."""
-    print("[case] bkv attn shares", codec, bs, hd, heads, kvh, lens, counts, flush=True)
+    shares of all workgroups (and, far, items of few rows in a launch of their own);
+    rows behind the step's stay as they are."""
+    print("[case] bkv attn shares", codec, bs, hd, heads, kvh, lens, counts, far, flush=True)
     n, room = len(lens), 1 << 20
-    p = Pair(ctx, 1, kvh, hd, n, max(max(lens), 64), bs, sum(lens) // bs + n, room, codec, seed=sum(lens))
+    p = Pair(ctx, 1, kvh, hd, n, 1 << 20 if far else max(max(lens), 64), bs, sum(lens) // bs + n, room, codec, seed=sum(lens))
     lens, counts = np.array(lens), np.array(counts)
     p.step(np.arange(n), np.zeros(n, int), lens - counts)
     assert p.ref.step(list(range(n)), list(lens - counts), list(counts)) == (bm.OK, n)

@@ -64,6 +64,7 @@ struct BkvAttnArgs {
     float scale_log2;   // scale * log2(e)
     int layer, hq, g;   // g = hq / n_head
     int n, rows, count; // most items, rows, and rows an item: items beyond are passed over
+    int done;           // chunks: items of so few rows are an earlier launch's
     uint32_t g_inv, splits_inv, parts_inv;  // ceil(2^32 / g) and so on: see bkv_div
     BkvOpen* open;      // of each share: the tile whose first piece is its last
     int tiles;          // chunks: places of tiles, see bkv_share
@@ -121,7 +122,7 @@ __device__ __forceinline__ bool bkv_chunk(const BkvAttnArgs& a, const BkvItem& i
     t.it = it;
     t.c0 = tile * kChunkCols;
     t.n = min(kChunkCols, it.count * a.g - t.c0);
-    if (t.n <= 0 || !bkv_fits(a, it)) return false;
+    if (t.n <= 0 || it.count <= a.done || !bkv_fits(a, it)) return false;
     t.keys = it.start + (t.c0 + t.n - 1) / a.g + 1;
     bkv_keys(a.v, t);
     return true;
@@ -1120,35 +1121,50 @@ hipError_t launch_bkv_attn(hipStream_t s, const BkvView& v, int layer, int n, in
     a.open = (BkvOpen*)(a.joined + kBkvShares);
     auto inv = [](int d) { return d == 1 ? 0u : (uint32_t)(((1ull << 32) + (uint32_t)d - 1) / (uint32_t)d); };
     a.g_inv = inv(a.g);
-    auto go = [&](dim3 grid) { v.hd == 64 ? go_hd<64>(s, a, tc, grid) : go_hd<128>(s, a, tc, grid); };
-    if (tc == kChunkCols) {
-        static_assert(2 * kBkvShares * kChunkCols <= kBkvParts && sizeof(BkvOpen) == 16, "");
-        a.tiles = (int)((long long)n_rows * a.g / kChunkCols + n);
-        a.cols = kChunkCols;
-        go(dim3(kBkvShares));
+    // items of up to `count` rows in tiles of tc columns, 16 or 32
+    auto ranges = [&](int count, int tc) {
+        BkvAttnArgs b = a;
+        b.count = count;
+        const int cols = count * b.g;
+        b.cols = std::min(cols, tc);
+        b.parts = (cols + tc - 1) / tc;
+        b.parts_inv = inv(b.parts);
+        const int tiles = b.parts * n;
+        // Units a key range: the call's units at the longest rows' length over 512, so
+        // that there are ranges for every CU (six sequences of 9 .. 65 thousand keys take
+        // 99 us, over 256 142; over 1024, 32 streams of up to 4096 take 22.5 us against
+        // 17.6), and 8 at least (16: one sequence of 2000 keys takes 10.8 us against 8.8).
+        const long long per = std::max<long long>((long long)tiles * v.n_head * units / 512, 8);
+        // Ranges: a wave's units fall with their number, the join's rounds rise with it;
+        // together least near the root of twice the units (one sequence of 32768 keys, 8
+        // kv heads: 45 ranges 23.5 us, 64 28.6, 16 29.7; of 12000 keys, one kv head: 27
+        // 12.9, 64 14.6).
+        const long long most = std::max(8, (int)std::sqrt(2.0 * units));
+        b.per = (int)((std::max(per, (units + most - 1) / most) + 3) / 4 * 4);
+        b.splits = (units + b.per - 1) / b.per;
+        b.splits_inv = inv(b.splits);
+        // More than one range only where tiles * n_head < 512 (per >= units above), and
+        // then fewer than 1100 ranges of up to 32 columns in all: the workspace holds them.
+        static_assert(1100 * 32 <= kBkvParts && kBkvShares == 512, "");
+        const dim3 grid((unsigned)tiles, (unsigned)v.n_head, (unsigned)b.splits);
+        v.hd == 64 ? go_hd<64>(s, b, tc, grid) : go_hd<128>(s, b, tc, grid);
+    };
+    if (tc != kChunkCols) {
+        ranges(max_count, tc);
         return hipGetLastError();
     }
-    a.cols = (int)std::min<long long>(cols, tc);
-    a.parts = (int)((cols + tc - 1) / tc);
-    a.parts_inv = inv(a.parts);
-    const int tiles = a.parts * n;
-    // Units a key range: the call's units at the longest rows' length over 512, so
-    // that there are ranges for every CU (six sequences of 9 .. 65 thousand keys take
-    // 99 us, over 256 142; over 1024, 32 streams of up to 4096 take 22.5 us against
-    // 17.6), and 8 at least (16: one sequence of 2000 keys takes 10.8 us against 8.8).
-    const long long per = std::max<long long>((long long)tiles * v.n_head * units / 512, 8);
-    // Ranges: a wave's units fall with their number, the join's rounds rise with it;
-    // together least near the root of twice the units (one sequence of 32768 keys, 8
-    // kv heads: 45 ranges 23.5 us, 64 28.6, 16 29.7; of 12000 keys, one kv head: 27
-    // 12.9, 64 14.6).
-    const long long most = std::max(8, (int)std::sqrt(2.0 * units));
-    a.per = (int)((std::max(per, (units + most - 1) / most) + 3) / 4 * 4);
-    a.splits = (units + a.per - 1) / a.per;
-    a.splits_inv = inv(a.splits);
-    // More than one range only where tiles * n_head < 512 (per >= units above), and then
-    // fewer than 1100 ranges of up to 32 columns in all: the workspace holds them.
-    static_assert(1100 * 32 <= kBkvParts && kBkvShares == 512, "");
-    go(dim3((unsigned)tiles, (unsigned)v.n_head, (unsigned)a.splits));
+    // Far fewer rows than items of the most have: single tokens beside a prompt's chunk,
+    // which would each take a tile of 128 columns and go first where that is much (63
+    // of 200 .. 3000 keys and a chunk of 1000, 32 heads over 8: 116 us against 140; 31 of
+    // up to 4096 and one of 256, 16 heads over 2: 51 against 46, so not there).
+    if ((long long)n_rows * 3 <= (long long)n * max_count && (long long)n * v.n_head * units > 16 << 10 && a.g <= 32) {
+        a.done = (a.g <= 16 ? 16 : 32) / a.g;
+        ranges(a.done, a.g <= 16 ? 16 : 32);
+    }
+    static_assert(2 * kBkvShares * kChunkCols <= kBkvParts && sizeof(BkvOpen) == 16, "");
+    a.tiles = (int)((long long)n_rows * a.g / kChunkCols + n);
+    a.cols = kChunkCols;
+    v.hd == 64 ? go_hd<64>(s, a, tc, dim3(kBkvShares)) : go_hd<128>(s, a, tc, dim3(kBkvShares));
     return hipGetLastError();
 }
 
