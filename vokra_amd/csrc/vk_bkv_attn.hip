@@ -381,7 +381,7 @@ struct BkvWave {
         if (hide) {  // a hidden key has no part in a block whose scale is NaN
 #pragma unroll
             for (int r = 0; r < 8; ++r)
-                if (e[r] == 0.0f) w[r] = 0.0f;
+                if (key0 + (r >> 2) * 16 + grp * 4 + (r & 3) >= min(last[ct] + 1, full)) w[r] = 0.0f;
         }
         half2v h[4], l[4];
 #pragma unroll
@@ -685,9 +685,8 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(
                                 : m == -INFINITY                  ? 1.0f
                                                                   : __builtin_amdgcn_exp2f(ml.x - m);
                 sum = fmaf(ml.y, f, sum);
-                if (f != 0.0f)
 #pragma unroll
-                    for (int i = 0; i < PD; ++i) y[i] = fmaf(sh.o[x][c][d0 + i], f, y[i]);
+                for (int i = 0; i < PD; ++i) y[i] = fmaf(sh.o[x][c][d0 + i], f, y[i]);
             }
             if (direct) {
                 float* dst = a.out + w.row(a, t, head, ct * 16 + c) + d0;
