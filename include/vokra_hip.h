@@ -481,7 +481,8 @@ int vokra_hip_bkv_write_dev(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t la
  * query head h with kv head h / (n_head_q / n_head); q, out [rows][n_head_q *
  * d_head], n_head_q any multiple of n_head. f32 in and out: products of a query
  * or a weight with 8-bit values run as two fp16 parts of the f32 operand (22
- * bits), those with f32 rows in f32, sums in f32. Rows that the step does not
+ * bits), those with f32 rows in f32, sums in f32; a key whose weight is below 2^-112
+ * of its row's largest may count as less. Rows that the step does not
  * reach are left as they are; out does not overlap q. One token a sequence,
  * several (drafts) and long chunks of prompts take the same call; how a row's
  * keys are split depends on the whole step, and its last bits may with it. */

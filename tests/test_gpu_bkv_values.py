@@ -1,6 +1,6 @@
 """GPU parity of the block-scaled cache's attention at values that few caches hold:
-blocks that are not finite at the causal edge. The restatement and its bound are
-those of bkv_model."""
+zero blocks beside small ones, both ends of f32, blocks that are not finite at the
+causal edge. The restatement and its bound are those of bkv_model."""
 import numpy as np
 import pytest
 
@@ -93,3 +93,37 @@ def test_nan_blocks_of_either_side_stay_hidden_from_earlier_rows(ctx, count, hea
             assert np.array_equal(np.isnan(got), np.isnan(want)) and np.isnan(want).any()
             err = np.abs(got - want) / tol
             assert not np.any(err > 1), f"{np.nanmax(err)} of the bound"
+
+
+# (magnitudes of the blocks in turn, of the open block's rows)
+SIZES = [([0, 1e-6], 1e-6), ([0, 1e-8, 1e-8], 1e-8), ([1e-10, 0], 0), ([1e-8], 0), ([1e-12, 0, 0], 1e-12),
+         ([0], 1e-12), ([0], 1e-33), ([1e20, 1e-20], 1e-20), ([1e-20], 1e20), ([1e-28, 0, 1e-28], 1e-33),
+         ([3.4e38, 1e-30, 0], 1.0), ([1.0, 0], 3.4e38), ([0], 0)]
+
+
+@pytest.mark.parametrize("count,t,far", [(2, 605, False), (12, 605, True), (24, 2100, False), (40, 605, True)])
+@pytest.mark.parametrize("codec,hd", [(0, 128), (1, 64)])
+def test_attention_of_values_far_apart(ctx, codec, hd, count, t, far):
+    """Blocks of zeros have no part in how far small blocks' weights are rounded, and a
+    key counts in the sum of weights whatever its values are: one and several key
+    ranges, tiles of 16, 32 and 128 columns."""
+    for n, (sizes, rest) in enumerate(SIZES):
+        print("[case] bkv far apart", codec, hd, count, t, far, sizes, rest, flush=True)
+        size = np.repeat(np.resize(sizes, t // 16 + 1), 16)[:t].astype(np.float64)
+        size[t // 16 * 16:] = rest
+        p = filled(ctx, codec, hd, t, count, size, far, seed=n)
+        got, want, tol = attend(ctx, p, t, count, 4, far)
+        assert np.all(np.isfinite(want))
+        err = np.abs(got - want) / tol
+        assert np.all(err <= 1), f"{err.max()} of the bound"
+
+
+def test_attention_under_a_negative_scale(ctx):
+    """A scale below zero turns the order of the scores round; zero weighs all alike."""
+    for scale in (-0.125, 0.0):
+        print("[case] bkv scale", scale, flush=True)
+        p = Pair(ctx, 1, 2, 64, 2, 300, 16, 40, 600)
+        p.step([0, 1], [0, 0], [290, 45])
+        p.check_attn(0, 335, 4, scale)
+        p.step([0, 1], [290, 45], [1, 3])
+        p.check_attn(0, 4, 4, scale)

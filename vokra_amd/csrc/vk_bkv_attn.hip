@@ -16,10 +16,10 @@
 // they widen to fp16 in LDS together (double buffered, one barrier a unit).
 //
 // vk_bkv_attn is bound by the pages' bytes where there are many (six sequences of
-// 9 .. 65 thousand keys, e4m3, 32 heads over 8 of 128, up to 4 rows: 457 MB in 97
+// 9 .. 65 thousand keys, e4m3, 32 heads over 8 of 128, up to 4 rows: 457 MB in 98
 // us, 4.7 TB/s, a large copy's rate here is 4.9), by dependent rounds of memory
 // (item, page, keys, results, join: 8 us) where there are few: 32 streams of 512 ..
-// 4096 keys, 16 heads over 2 of 128, take 17.1 us for 38 MB. Four waves a workgroup,
+// 4096 keys, 16 heads over 2 of 128, take 17.3 us for 38 MB. Four waves a workgroup,
 // three workgroups a CU: eight waves took 28 us for those, and two units' loads in
 // flight a wave spilled or left two workgroups.
 // The 8-bit values are exact in fp16, so a product is two fp16 matrix
@@ -31,12 +31,15 @@
 //   P's accumulator layout (4 consecutive keys a lane) is the operand layout of
 //     O^T [d][columns] = V^T P^T under the key order that V's tiles use, so the
 //     weights go from the softmax to the product without leaving the lane.
-// A block's V scale f 2^e (f in [1, 2)) goes into the weights: the running
-// maximum is that of s + e, so the largest weight has the largest product, and a
-// block of small values keeps its bits beside one of large values; the sum of
-// weights takes 2^-e back out. Two fp16 parts of 2^14 w hold a weight to 2^-22,
-// or to 2^-39 of the largest where it is smaller than 2^-17 of that. The open
-// block's rows are f32 on both sides and use the f32 matrix instruction.
+// Weights w = 2^(s - M) are summed as they are, M the running maximum of s, rounded
+// up. For the product a block's V scale v = f 2^e (f in [1, 2)) goes into them, as w v
+// 2^-E: E is the running maximum of s - M + e, rounded up, so the largest product is near
+// 1 whatever the blocks' values are, a block of small values keeps its bits beside one of
+// large values, and zeros (e is below that of any other block) take nothing from either.
+// Two fp16 parts of 2^14 of that hold it to 2^-22, or to 2^-39 of the largest where it is
+// smaller than 2^-17 of that. M and E are whole numbers, so what was summed is brought
+// under new ones exactly, and seldom. The open block's rows are f32 on both sides and use
+// the f32 matrix instruction.
 #include <algorithm>
 #include <cmath>
 
@@ -58,7 +61,7 @@ struct BkvAttnArgs {
     BkvView v;
     const float* q;
     float* out;
-    float* part;        // [slot][cols][2] (max, sum), then [slot][cols][hd] partial outputs
+    float* part;        // [slot][cols][2] (max, sum), then [slot][cols][hd] outputs of a key range
     size_t part_o;      // floats before the partial outputs
     unsigned* joined;   // [tile][head] ranges that have written theirs, zero between calls
     float scale_log2;   // scale * log2(e)
@@ -180,28 +183,46 @@ __device__ __forceinline__ float bkv_max4(float v) {
 __device__ __forceinline__ float bkv_sum4(float v) {
     return bkv_fold4(v, [](float a, float b) { return a + b; });
 }
+// The maxima of two values: of a in the even lane groups, of b in the odd ones (NaN where
+// one is).
+__device__ __forceinline__ float bkv_max_two(float a, float b) {
+    auto top = [](uint32_t x, uint32_t y) { return __builtin_elementwise_maximum(__uint_as_float(x), __uint_as_float(y)); };
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    const uint32_t v = __float_as_uint(top(r[0], r[1]));
+    r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return top(r[0], r[1]);
+}
+// The larger of two neighbouring groups' values, in both.
+__device__ __forceinline__ float bkv_max2(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 
-// A tile's scales as the weights need them: K's, and V's f 2^e (f in [1, 2)) as
-// f 2^14, 2^-e and e. Zero: 0, 1, 0; not finite: NaN, 1, 0.
+// The least E, below the e of every block that holds more than zeros: 2^(14 - E) fits f32.
+constexpr float kLeastE = -113.0f;
+
+// p v, p = 2^(14 - E): the factor of a weight. A weight is 2^(E - e) at most, so one that
+// would take a factor above 2^126 here is below 2^-112: it counts as less.
+__device__ __forceinline__ float bkv_factor(float v, float p) { return fminf(v * p, 0x1p126f); }
+
+// A tile's scales as the weights need them: K's (NaN where V's is: then its scores are,
+// of the keys that a row sees), V's, and V's exponent (zero: -127).
 struct BkvScale {
-    float k, vf, back, ve;
+    float k, v, ve;
     __device__ __forceinline__ void set(float2 sc) {
-        const uint32_t b = __float_as_uint(sc.y);
-        const int ex = (int)((b >> 23) & 255);
-        const bool plain = ex != 0 && ex != 255;
-        const float f14 = __uint_as_float((b & 0x007fffffu) | 0x46800000u);
-        const int e = plain ? ex : 127;
-        k = sc.x;
-        vf = plain ? f14 : sc.y;
-        back = __uint_as_float((uint32_t)min(254 - e, 253) << 23);
-        ve = (float)(e - 127);
+        k = fmaf(sc.y, 0.0f, sc.x);
+        v = sc.y;
+        ve = (float)((int)(__float_as_uint(sc.y) >> 23) - 127);
     }
     // of lane l, in all lanes
     __device__ __forceinline__ BkvScale at(int l) const {
         auto get = [l](float x) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), l)); };
-        return BkvScale{get(k), get(vf), get(back), get(ve)};
+        return BkvScale{get(k), get(v), get(ve)};
     }
 };
+
+// M of a column that has seen no key: no score is below it.
+constexpr float kNoKey = -0x1.fffffep127f;
 
 // Values that a workgroup on another XCD reads in this launch: past the caches
 // that are the XCD's own. Four at a time by the buffer instructions, whose policy
@@ -229,12 +250,13 @@ __device__ __forceinline__ vk_f32x4 bkv_get4(const float* out, size_t at) {
 
 // Values d .. d + 3 of a column from the partial results of its key ranges,
 // joined in the ranges' order, B ranges' loads in flight. pm: the first range's
-// (max, sum), part_o + o: its outputs, cols columns a slot; range s > 0 is s * step -
-// back slots behind. SAME: written by this launch.
+// (max, sum), part_o + o0: its outputs, cols columns a slot; range s > 0 is s * step -
+// back slots behind. SAME: written by this launch. What is joined is an output at
+// every step, so it stays in f32's range where the values do.
 template <int HD, bool SAME, int B>
 __device__ __forceinline__ vk_f32x4 bkv_join(const float* pm, const float* part_o, size_t o0, int ranges,
                                               int cols, int step, int back) {
-    float m = -INFINITY, sum = 0.0f;
+    float m = kNoKey, sum = 0.0f;
     vk_f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s = 0; s < ranges; s += B) {
         float2 ml[B];
@@ -254,19 +276,20 @@ __device__ __forceinline__ vk_f32x4 bkv_join(const float* pm, const float* part_
         float to = m;
 #pragma unroll
         for (int x = 0; x < B; ++x) to = fmaxf(to, ml[x].x);
-        const float c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
-        sum *= c;
-        y *= c;
+        const float before = sum * __builtin_amdgcn_exp2f(m - to);
         m = to;
+        sum = before;
 #pragma unroll
         for (int x = 0; x < B; ++x) {
-            if (s + x >= ranges || (ml[x].x == -INFINITY && ml[x].y == 0.0f)) continue;
-            const float w = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml[x].x - m);
-            sum = fmaf(ml[x].y, w, sum);
-            y += o[x] * w;
+            ml[x].y = s + x < ranges ? ml[x].y * __builtin_amdgcn_exp2f(ml[x].x - m) : 0.0f;
+            sum += ml[x].y;
         }
+        const float f = 1.0f / sum;
+        y *= before * f;
+#pragma unroll
+        for (int x = 0; x < B; ++x) y += o[x] * (ml[x].y * f);
     }
-    return y * (1.0f / sum);
+    return y;
 }
 
 // One wave's query columns in blocks of 16 and what it has summed for them.
@@ -274,9 +297,9 @@ template <int HD, int C, bool CHUNKS>
 struct BkvWave {
     static constexpr int U = HD / 64, DT = HD / 16;
     int col, grp;   // lane's column of a block, and its group of 16 lanes
-    float qf[C];    // a score is qf times the product of q's parts
+    float qf[C];    // a score is qf (not below zero) times the product of q's parts
     int last[C];    // last key that the lane's column sees
-    float M[C], L[C];
+    float M[C], L[C], E[C], P[C];  // P = 2^(14 - E)
     vk_f32x4 O[C][DT];  // [4 c + i][r]: value 64 c + 16 grp + 4 r + i of the lane's column
 
     // values 64 c + 16 grp + 4 r .. of the lane's column
@@ -286,8 +309,10 @@ struct BkvWave {
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int ct = 0; ct < C; ++ct) {
-            M[ct] = -INFINITY;
+            M[ct] = kNoKey;
             L[ct] = 0.0f;
+            E[ct] = kLeastE;
+            P[ct] = 0x1p127f;
 #pragma unroll
             for (int d = 0; d < DT; ++d) O[ct][d] = vk_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
@@ -321,7 +346,7 @@ struct BkvWave {
         // the largest value goes to 2^14 .. 2^15; rows below 2^-106 keep fewer bits
         const int e = min(141 - (int)(__float_as_uint(top) >> 23), 120);
         const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-        const float up = live ? __uint_as_float((uint32_t)(127 + e) << 23) : 0.0f;
+        const float up = live ? copysignf(__uint_as_float((uint32_t)(127 + e) << 23), a.scale_log2) : 0.0f;
 #pragma unroll
         for (int i = 0; i < 2 * U; ++i) {
             half2v h[4], l[4];
@@ -333,55 +358,69 @@ struct BkvWave {
             h8[i] = half8v{h[0].x, h[0].y, h[1].x, h[1].y, h[2].x, h[2].y, h[3].x, h[3].y};
             l8[i] = half8v{l[0].x, l[0].y, l[1].x, l[1].y, l[2].x, l[2].y, l[3].x, l[3].y};
         }
-        qf[ct] = a.scale_log2 * down;
+        qf[ct] = fabsf(a.scale_log2) * down;
         last[ct] = t.it.start + item_row(a, t, c0 + col);
     }
-    // the running maximum of a column becomes m; what was summed so far shrinks
-    __device__ __forceinline__ void raise(int ct, float m) {
-        if (__any(m > M[ct])) {
-            const float to = fmaxf(M[ct], m), c = M[ct] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M[ct] - to);
+    // M and E of a column take a tile or two in, of which lanes of odd groups have one
+    // and those of even groups the other: its largest score t and its V's exponent v;
+    // what was summed so far shrinks
+    __device__ __forceinline__ void raise(int ct, float t, float v) {
+        if (__any(t - M[ct] > fminf(E[ct] - v, 0.0f))) {
+            const float to = fmaxf(M[ct], ceilf(bkv_max2(t))), up = M[ct] - to, eo = E[ct] + up;
+            const float ee = fmaxf(fmaxf(eo, kLeastE), ceilf(bkv_max2(t - to + v)));
+            const float c = __builtin_amdgcn_exp2f(eo - ee);
+            L[ct] *= __builtin_amdgcn_exp2f(up);
             M[ct] = to;
-            L[ct] *= c;
+            E[ct] = ee;
+            P[ct] = ldexpf(1.0f, 14 - (int)ee);
 #pragma unroll
             for (int d = 0; d < DT; ++d) O[ct][d] *= c;
         }
     }
-    // raw scores of a unit (32 keys from key0 on, none from `full` on) -> the two
-    // parts of 2^14 times its weights, V's scales in them. hide: some key is
-    // hidden from some column.
-    __device__ __forceinline__ void weigh(int ct, const vk_f32x4 (&S)[2], const BkvScale (&sc)[2], int key0, int full,
-                                          bool hide, half8v& ph, half8v& pl) {
-        const float f[2] = {sc[0].k * qf[ct], sc[1].k * qf[ct]};
-        float e[8];
+    // The column's output so far in O, with the weights' sum over its lanes. A sum of
+    // weights' products may leave f32's range where no value does; this does not.
+    __device__ __forceinline__ float finish(int ct) {
+        const float l = bkv_sum4(L[ct]), f = l == 0.0f ? 0.0f : 1.0f / l;
+        const int x = (int)E[ct] - 14;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) e[r] = fmaf(S[r >> 2][r & 3], f[r >> 2], sc[r >> 2].ve);
-        auto top = [&]() {
-            const float m = fmaxf(fmaxf(fmaxf(e[0], e[1]), e[2]), fmaxf(fmaxf(e[3], e[4]), e[5]));
-            return bkv_max4(fmaxf(m, fmaxf(e[6], e[7])));
-        };
-        if (!hide) {
-            raise(ct, top());
-        } else {
-            const int lim = min(last[ct] + 1, full);
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) O[ct][d][r] = ldexpf(O[ct][d][r] * f, x);
+        return l;
+    }
+    // raw scores of a unit (32 keys from key0 on, none from `full` on) -> the two
+    // parts of 2^14 times its weights, V's scales under 2^E in them. hide: some key is
+    // hidden from some column.
+    __device__ __forceinline__ void weigh(int ct, vk_f32x4 (&S)[2], const BkvScale (&sc)[2], int key0, int full,
+                                          bool hide, half8v& ph, half8v& pl) {
+        // no factor is below zero: the largest raw score of a tile is its largest score
+        const float f[2] = {sc[0].k * qf[ct], sc[1].k * qf[ct]};
+        auto hidden = [&](int lim, int r) { return key0 + (r >> 2) * 16 + grp * 4 + (r & 3) >= lim; };
+        auto top = [](float a, float b) { return __builtin_elementwise_maximum(a, b); };
+        int lim = min(last[ct] + 1, full);
+        if (hide)
 #pragma unroll
             for (int r = 0; r < 8; ++r)
-                if (key0 + (r >> 2) * 16 + grp * 4 + (r & 3) >= lim) e[r] = -INFINITY;
-            raise(ct, top());
-        }
-        const float base = M[ct] == -INFINITY ? 0.0f : M[ct];
+                if (hidden(lim, r)) S[r >> 2][r & 3] = -INFINITY;
+        const float t0 = top(top(top(S[0][0], S[0][1]), S[0][2]), S[0][3]);
+        const float t1 = top(top(top(S[1][0], S[1][1]), S[1][2]), S[1][3]);
+        raise(ct, bkv_max_two(t0, t1) * ((grp & 1 ? sc[1].k : sc[0].k) * qf[ct]), grp & 1 ? sc[1].ve : sc[0].ve);
+        float e[8];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) e[r] = __builtin_amdgcn_exp2f(e[r] - base);
+        for (int r = 0; r < 8; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(S[r >> 2][r & 3], f[r >> 2], -M[ct]));
+        if (hide) {  // also where the factor is zero or NaN
+            asm("" : "+v"(lim));  // (else both branches' comparisons are made before either)
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (hidden(lim, r)) e[r] = 0.0f;
+        }
+        L[ct] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
         float w[8];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            L[ct] = fmaf((e[4 * x] + e[4 * x + 1]) + (e[4 * x + 2] + e[4 * x + 3]), sc[x].back, L[ct]);
+            const float g = bkv_factor(sc[x].v, P[ct]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) w[4 * x + r] = e[4 * x + r] * sc[x].vf;
-        }
-        if (hide) {  // a hidden key has no part in a block whose scale is NaN
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-                if (key0 + (r >> 2) * 16 + grp * 4 + (r & 3) >= min(last[ct] + 1, full)) w[r] = 0.0f;
+            for (int r = 0; r < 4; ++r) w[4 * x + r] = e[4 * x + r] * g;
         }
         half2v h[4], l[4];
 #pragma unroll
@@ -419,10 +458,17 @@ struct BkvWave {
             }
         }
         const bool any_odd = __any(odd);
-        // a power of two in the place of a block's scale, so that the maximum
-        // weighs these rows like the blocks: the largest |v| is 2^9 .. 2^10 of it
-        top = vk_group_max<64>(any_odd ? 0.0f : top);
-        const int te = top < 0x1p-100f ? 0 : (int)(__float_as_uint(top) >> 23) - 136;
+        if (any_odd) {  // of the values that are finite, at least 1
+            top = 1.0f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, fabsf(vv[d][r]) < INFINITY ? fabsf(vv[d][r]) : 0.0f);
+        }
+        // a power of two in the place of a block's scale, so that E weighs these
+        // rows like the blocks: the largest |v| is 2^9 .. 2^10 of it (less below 2^-100)
+        top = vk_group_max<64>(top);
+        const int te = max((int)(__float_as_uint(top) >> 23), 27) - 136;
         const float tdown = __uint_as_float((uint32_t)(127 - te) << 23);
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -443,17 +489,17 @@ struct BkvWave {
             float s[4], m = -INFINITY;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                s[r] = key0 + grp * 4 + r <= last[ct] ? fmaf(s4[r], a.scale_log2, (float)te) : -INFINITY;
+                s[r] = key0 + grp * 4 + r <= last[ct] ? s4[r] * a.scale_log2 : -INFINITY;
                 m = fmaxf(m, s[r]);
             }
-            raise(ct, bkv_max4(m));
-            const float base = M[ct] == -INFINITY ? 0.0f : M[ct];
+            raise(ct, bkv_max4(m), (float)te);
+            const float g = bkv_factor(__uint_as_float((uint32_t)(127 + te) << 23), P[ct]);
             float e[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                e[r] = __builtin_amdgcn_exp2f(s[r] - base);
-                L[ct] = fmaf(e[r], tdown, L[ct]);
-                e[r] *= 16384.0f;
+                e[r] = __builtin_amdgcn_exp2f(s[r] - M[ct]);
+                L[ct] += e[r];
+                e[r] *= g;
             }
             if (!any_odd) {
 #pragma unroll
@@ -477,10 +523,10 @@ struct BkvWave {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             const float4 y = *(const float4*)(p1 + 64 * c + 4 * r);
-                            O[ct][4 * c][r] = fmaf(w, y.x, O[ct][4 * c][r]);
-                            O[ct][4 * c + 1][r] = fmaf(w, y.y, O[ct][4 * c + 1][r]);
-                            O[ct][4 * c + 2][r] = fmaf(w, y.z, O[ct][4 * c + 2][r]);
-                            O[ct][4 * c + 3][r] = fmaf(w, y.w, O[ct][4 * c + 3][r]);
+                            O[ct][4 * c][r] = fmaf(w, y.x * tdown, O[ct][4 * c][r]);
+                            O[ct][4 * c + 1][r] = fmaf(w, y.y * tdown, O[ct][4 * c + 1][r]);
+                            O[ct][4 * c + 2][r] = fmaf(w, y.z * tdown, O[ct][4 * c + 2][r]);
+                            O[ct][4 * c + 3][r] = fmaf(w, y.w * tdown, O[ct][4 * c + 3][r]);
                         }
                 }
             }
@@ -512,8 +558,10 @@ struct BkvPlace {
 
 constexpr int kWaves = 4;  // of the kernel below
 
+// 16 columns: three workgroups a CU, five of heads of 64 (64 sequences of up to 448 keys,
+// 20 heads: 16.3 us, 19.4 with four).
 template <int HD, int CODEC, int C>
-__global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(
+__global__ __launch_bounds__(64 * kWaves, C == 2 ? 2 : HD == 64 ? 5 : 3) void vk_bkv_attn(
     BkvAttnArgs a, const uint8_t* __restrict__ pool, const float2* __restrict__ scales) {
     using W = BkvWave<HD, C, false>;
     constexpr int U = W::U, DT = W::DT, OS = HD + 4;
@@ -663,7 +711,7 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(
 #pragma unroll
     for (int ct = 0; ct < C; ++ct) {
         if (ct * 16 >= t.n) break;
-        const float l = bkv_sum4(w.L[ct]);
+        const float l = w.finish(ct);
         __syncthreads();  // q's parts, or the columns before, are done with
         if (w.grp == 0) sml[wave][w.col] = make_float2(w.M[ct], l);
 #pragma unroll
@@ -673,39 +721,37 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(
         constexpr int PT = 4 * kWaves, PD = HD / PT;  // threads a column, values a thread
         const int c = threadIdx.x / PT, d0 = (threadIdx.x % PT) * PD;
         if (ct * 16 + c < t.n) {
-            float m = -INFINITY, sum = 0.0f, y[PD];
+            float m = kNoKey, sum = 0.0f, f[kWaves];
 #pragma unroll
             for (int x = 0; x < kWaves; ++x) m = fmaxf(m, sml[x][c].x);
 #pragma unroll
-            for (int i = 0; i < PD; ++i) y[i] = 0.0f;
-#pragma unroll
             for (int x = 0; x < kWaves; ++x) {
-                const float2 ml = sml[x][c];
-                const float f = ml.x == -INFINITY && ml.y == 0.0f ? 0.0f
-                                : m == -INFINITY                  ? 1.0f
-                                                                  : __builtin_amdgcn_exp2f(ml.x - m);
-                sum = fmaf(ml.y, f, sum);
+                f[x] = sml[x][c].y * __builtin_amdgcn_exp2f(sml[x][c].x - m);
+                sum += f[x];
+            }
+            const float inv = 1.0f / sum;
+            vk_f32x4 y[PD / 4];
 #pragma unroll
-                for (int i = 0; i < PD; ++i) y[i] = fmaf(sh.o[x][c][d0 + i], f, y[i]);
+            for (int i = 0; i < PD / 4; ++i) {
+                y[i] = vk_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int x = 0; x < kWaves; ++x) y[i] += *(const vk_f32x4*)&sh.o[x][c][d0 + 4 * i] * (f[x] * inv);
             }
             if (direct) {
                 float* dst = a.out + w.row(a, t, head, ct * 16 + c) + d0;
-                const float f = 0x1p-14f / sum;
 #pragma unroll
-                for (int i = 0; i < PD; ++i) dst[i] = y[i] * f;
+                for (int i = 0; i < PD / 4; ++i) *(vk_f32x4*)(dst + 4 * i) = y[i];
             } else {
                 const size_t at = slot * a.cols + ct * 16 + c;
-                float* pm = a.part + at * 2;
+                float *pm = a.part + at * 2, *po = a.part + a.part_o;
                 if constexpr (C == 1) {
                     if (d0 == 0) bkv_put2(pm, m, sum);
 #pragma unroll
-                    for (int i = 0; i < PD; i += 4)
-                        bkv_put4(a.part + a.part_o, at * HD + d0 + i,
-                                 vk_f32x4{y[i], y[i + 1], y[i + 2], y[i + 3]} * 0x1p-14f);
+                    for (int i = 0; i < PD / 4; ++i) bkv_put4(po, at * HD + d0 + 4 * i, y[i]);
                 } else {
                     if (d0 == 0) *(float2*)pm = make_float2(m, sum);
 #pragma unroll
-                    for (int i = 0; i < PD; ++i) a.part[a.part_o + at * HD + d0 + i] = y[i] * 0x1p-14f;
+                    for (int i = 0; i < PD / 4; ++i) *(vk_f32x4*)(po + at * HD + d0 + 4 * i) = y[i];
                 }
             }
         }
@@ -740,7 +786,7 @@ __global__ __launch_bounds__(64 * kWaves, C == 1 ? 3 : 2) void vk_bkv_attn(
 // for each key range of each tile left 40 % of the waves' places empty at six chunks
 // of 450 .. 1030 rows over up to 4500 keys, 16 heads over 2 of 128, and finer ranges
 // cost more to join than they gave: 264 us against 204 with shares.
-// That call takes 182 us now: 0.40 PFLOP/s of the operator, 0.80 of fp16 products.
+// That call takes 186 us now: 0.39 PFLOP/s of the operator, 0.79 of fp16 products.
 // Of a unit's time about a quarter each is the products and the weights, the
 // rest starts, joins (15 us: 96 MB) and waits for the four waves' common units.
 
@@ -1012,14 +1058,13 @@ __global__ __launch_bounds__(256, 2) void vk_bkv_attn_chunk(BkvAttnArgs a, const
 #pragma unroll
             for (int ct = 0; ct < C; ++ct) {
                 const int c = c0 + ct * 16 + w.col;
-                const float l = bkv_sum4(w.L[ct]);
+                const float l = w.finish(ct);
                 if (c >= t.n) continue;
                 float* dst = whole ? a.out + w.row(a, t, head, c) : a.part + a.part_o + (slot * kChunkCols + c) * HD;
-                const float f = whole ? 0x1p-14f / l : 0x1p-14f;
                 if (!whole && w.grp == 0) ((float2*)a.part)[slot * kChunkCols + c] = make_float2(w.M[ct], l);
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
-                    *(vk_f32x4*)(dst + (d >> 2) * 64 + 16 * w.grp + (d & 3) * 4) = w.out4(ct, d >> 2, d & 3) * f;
+                    *(vk_f32x4*)(dst + (d >> 2) * 64 + 16 * w.grp + (d & 3) * 4) = w.out4(ct, d >> 2, d & 3);
             }
         }
         // a tile that begins here and goes on in later shares
