@@ -579,8 +579,10 @@ void vokra_hip_rope_destroy(vokra_hip_rope_t *rope);
 /* Row r of q [n_head_q heads] and k [n_head_k heads] at positions[r] (any
  * int32), one launch; either may have no heads. Rows lie q_stride (and so on)
  * floats apart, so q and k may be parts of one projection's rows. An output is
- * its input (in place, the same stride) or overlaps no input. Device pointers,
- * asynchronous; at most 2^32 values. */
+ * its input (in place, the same stride) or overlaps no input; the two overlap
+ * neither each other nor positions (INVALID_ARGUMENT). Rows of one stride may lie
+ * between each other; of two strides, and for positions, whole ranges are compared.
+ * Device pointers, asynchronous; at most 2^32 values. */
 int vokra_hip_rope_apply_dev(vokra_hip_ctx_t *ctx, const vokra_hip_rope_t *rope, size_t rows,
                              const int32_t *d_positions, size_t n_head_q, const float *d_q, size_t q_stride,
                              float *d_q_out, size_t q_out_stride, size_t n_head_k, const float *d_k, size_t k_stride,

@@ -110,6 +110,18 @@ bool meet(const void* a, size_t na, const void* b, size_t nb) {
     return x < y + nb && y < x + na;
 }
 
+// Whether rows of two buffers meet, wa and wb floats of them, sa and sb floats from row to
+// row. Rows of one stride may lie between each other; of two strides the whole ranges count.
+bool rows_meet(size_t rows, const float* a, size_t wa, size_t sa, const float* b, size_t wb, size_t sb) {
+    if (!meet(a, ((rows - 1) * sa + wa) * 4, b, ((rows - 1) * sb + wb) * 4)) return false;
+    if (sa != sb) return true;
+    // row i of a, row i + k of b: -4 wb < d + 4 k s < 4 wa, |k| < rows
+    const int64_t d = (int64_t)(reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a));
+    const int64_t s = (int64_t)sa * 4, lo = -(int64_t)wb * 4 - d + 1, hi = (int64_t)wa * 4 - d - 1;
+    const int64_t k0 = lo >= 0 ? (lo + s - 1) / s : -(-lo / s), k1 = hi >= 0 ? hi / s : -((-hi + s - 1) / s);
+    return std::max(k0, 1 - (int64_t)rows) <= std::min(k1, (int64_t)rows - 1);
+}
+
 int rope_side(const vokra_hip_rope* p, const char* name, size_t rows, size_t heads, const float* x, size_t stride,
               const float* y, size_t out_stride) {
     if (heads == 0) return VOKRA_HIP_OK;
@@ -121,7 +133,7 @@ int rope_side(const vokra_hip_rope* p, const char* name, size_t rows, size_t hea
         return ctx_fail(BAD, "rope_apply: a row stride of %s is too large", name);
     if (x == y) {
         if (stride != out_stride) return ctx_fail(BAD, "rope_apply: %s in place needs one row stride", name);
-    } else if (meet(x, ((rows - 1) * stride + w) * 4, y, ((rows - 1) * out_stride + w) * 4)) {
+    } else if (rows_meet(rows, x, w, stride, y, w, out_stride)) {
         return ctx_fail(BAD, "rope_apply: %s and its output overlap without being the same", name);
     }
     return VOKRA_HIP_OK;
@@ -222,6 +234,15 @@ int vokra_hip_rope_apply_dev(vokra_hip_ctx_t* c, const vokra_hip_rope_t* p, size
     if (!d_positions) return ctx_fail(BAD, "rope_apply: positions is NULL");
     ST_ST(rope_side(p, "q", rows, n_head_q, d_q, q_stride, d_q_out, q_out_stride));
     ST_ST(rope_side(p, "k", rows, n_head_k, d_k, k_stride, d_k_out, k_out_stride));
+    const size_t wq = n_head_q * p->hd, wk = n_head_k * p->hd;
+    if (wq && wk &&
+        (rows_meet(rows, d_q_out, wq, q_out_stride, d_k, wk, k_stride) ||
+         rows_meet(rows, d_k_out, wk, k_out_stride, d_q, wq, q_stride) ||
+         rows_meet(rows, d_q_out, wq, q_out_stride, d_k_out, wk, k_out_stride)))
+        return ctx_fail(BAD, "rope_apply: an output overlaps the other side's input or output");
+    if ((wq && meet(d_q_out, ((rows - 1) * q_out_stride + wq) * 4, d_positions, rows * 4)) ||
+        (wk && meet(d_k_out, ((rows - 1) * k_out_stride + wk) * 4, d_positions, rows * 4)))
+        return ctx_fail(BAD, "rope_apply: an output overlaps positions");
     ST_TRY(hipSetDevice(vk::ctx_device(c)), "hipSetDevice");
     RopeArgs a = {};
     a.q = n_head_q ? d_q : d_k;  // (an absent side is given the other's address and never read)
