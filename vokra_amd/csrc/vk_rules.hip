@@ -72,10 +72,11 @@ __global__ __launch_bounds__(RU_T) void vk_rules(RulesArgs a) {
         __syncthreads();
     }
     if (h1 > h0) {
-        for (int i = h0 + t; i < h1; i += 8 * RU_T) {
+        // (places beyond a list's end may be beyond int)
+        for (unsigned i = (unsigned)h0 + t; i < (unsigned)h1; i += 8 * RU_T) {
             int v[8];  // loads in flight
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = i + RU_T * j < h1 ? a.hist[i + RU_T * j] : -1;
+            for (int j = 0; j < 8; ++j) v[j] = i + RU_T * j < (unsigned)h1 ? a.hist[i + RU_T * j] : -1;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (v[j] >= lo && v[j] < hi) atomicAdd(&table[v[j] - c0], 1);
@@ -98,13 +99,13 @@ __global__ __launch_bounds__(RU_T) void vk_rules(RulesArgs a) {
     }
     if (b1 > b0) {
         if (h1 > h0) __syncthreads();
-        for (int i = b0 + t; i < b1; i += 2 * RU_T) {
+        for (unsigned i = (unsigned)b0 + t; i < (unsigned)b1; i += 2 * RU_T) {
             int v[2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) v[j] = i + RU_T * j < b1 ? a.bias_ids[i + RU_T * j] : -1;
+            for (int j = 0; j < 2; ++j) v[j] = i + RU_T * j < (unsigned)b1 ? a.bias_ids[i + RU_T * j] : -1;
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-                if (v[j] >= lo && v[j] < hi) atomicMax(&table[v[j] - c0], i + RU_T * j - b0 + 1);
+                if (v[j] >= lo && v[j] < hi) atomicMax(&table[v[j] - c0], (int)(i + RU_T * j - b0) + 1);
         }
         __syncthreads();
 #pragma unroll
