@@ -1,5 +1,7 @@
-"""Which overlaps of buffers a rotary plan refuses, and rows that lie between each
+"""Which overlaps of buffers and sizes a rotary plan refuses, and rows that lie between each
 other without overlapping."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -54,3 +56,14 @@ def test_rows_between_rows(ctx):
     assert np.array_equal(got[:, :wq + wk], rows[:, :wq + wk])
     x = np.ascontiguousarray(rows[:, :wq + wk]).reshape(n, hq + hk, hd)
     check(np.ascontiguousarray(got[:, wq + wk:]), x, pos, thetas(hd, 10000.0), hip.RopeLayout.HALF)
+
+
+def test_sizes_beyond_a_call_are_refused_before_any_copy(ctx):
+    """Sizes whose product leaves 64 bits, too: nothing of the (short) arrays is read."""
+    print("[case] rope sizes", flush=True)
+    x, pos = np.zeros(64, np.float32), np.zeros(1, np.int32)
+    f, i = hip._ptr(x, C.c_float), hip._ptr(pos, C.c_int32)
+    for hd in (64, 65536):
+        plan = ctx.rope_plan(hd, 64)
+        for rows, hq, hk in ((2 ** 31 - 1, 65535, 65535), (2 ** 31, 1, 0), (1, 70000, 0), (1 << 27, 1, 1 if hd > 64 else 64)):
+            assert hip.lib().vokra_hip_rope_apply(ctx._h, plan._h, rows, i, hq, f, f, hk, f, f) == 5

@@ -104,6 +104,15 @@ int rope_check(const vokra_hip_rope_config_t& f) {
     return VOKRA_HIP_OK;
 }
 
+// A launch has fewer than 2^32 threads, one for two values at least; sizes in bytes fit.
+int rope_size(const vokra_hip_rope* p, size_t rows, size_t n_head_q, size_t n_head_k) {
+    if (n_head_q > 65535 || n_head_k > 65535) return ctx_fail(BAD, "rope_apply: at most 65535 heads");
+    const size_t w = (n_head_q + n_head_k) * p->hd;
+    if (rows > (size_t)INT32_MAX || w > ((size_t)1 << 30) || rows * w > ((size_t)1 << 32))
+        return ctx_fail(BAD, "rope_apply: more than 2^32 values, or 2^30 a row");
+    return VOKRA_HIP_OK;
+}
+
 // [p, p + bytes) of two buffers meet
 bool meet(const void* a, size_t na, const void* b, size_t nb) {
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
@@ -225,12 +234,8 @@ int vokra_hip_rope_apply_dev(vokra_hip_ctx_t* c, const vokra_hip_rope_t* p, size
                              size_t n_head_q, const float* d_q, size_t q_stride, float* d_q_out, size_t q_out_stride,
                              size_t n_head_k, const float* d_k, size_t k_stride, float* d_k_out, size_t k_out_stride) {
     if (!c || !p || p->ctx != c) return ctx_fail(BAD, "rope_apply: bad context or plan");
-    if (n_head_q > 65535 || n_head_k > 65535) return ctx_fail(BAD, "rope_apply: at most 65535 heads");
     if (rows == 0 || n_head_q + n_head_k == 0) return VOKRA_HIP_OK;
-    // a launch has fewer than 2^32 threads, one for two values at least
-    if (rows > (size_t)INT32_MAX || (n_head_q + n_head_k) * p->hd > ((size_t)1 << 30) ||
-        rows * ((n_head_q + n_head_k) * p->hd) > ((size_t)1 << 32))
-        return ctx_fail(BAD, "rope_apply: more than 2^32 values, or 2^30 a row");
+    ST_ST(rope_size(p, rows, n_head_q, n_head_k));
     if (!d_positions) return ctx_fail(BAD, "rope_apply: positions is NULL");
     ST_ST(rope_side(p, "q", rows, n_head_q, d_q, q_stride, d_q_out, q_out_stride));
     ST_ST(rope_side(p, "k", rows, n_head_k, d_k, k_stride, d_k_out, k_out_stride));
@@ -270,8 +275,7 @@ int vokra_hip_rope_apply(vokra_hip_ctx_t* c, const vokra_hip_rope_t* p, size_t r
                          float* k_out) {
     if (!c || !p || p->ctx != c) return ctx_fail(BAD, "rope_apply: bad context or plan");
     if (rows == 0 || n_head_q + n_head_k == 0) return VOKRA_HIP_OK;
-    if (n_head_q > 65535 || n_head_k > 65535 || rows > (size_t)INT32_MAX)
-        return ctx_fail(BAD, "rope_apply: too many heads or rows");
+    ST_ST(rope_size(p, rows, n_head_q, n_head_k));
     if (!positions || (n_head_q && (!q || !q_out)) || (n_head_k && (!k || !k_out)))
         return ctx_fail(BAD, "rope_apply: NULL buffer");
     ST_TRY(hipSetDevice(vk::ctx_device(c)), "hipSetDevice");
