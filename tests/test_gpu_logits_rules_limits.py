@@ -48,3 +48,17 @@ def test_rows_at_the_end_of_the_longest_lists(ctx):
     got = out.download(F, x.size).reshape(x.shape), nxt.download(np.int32, rows)
     same(got, rules(x, history=list(hist.reshape(rows, n)), repetition=[1.5] * rows,
                     biases=[list(zip(i, v)) for i, v in zip(ids.reshape(rows, n), val.reshape(rows, n))]))
+
+
+def test_mask_strides_beyond_every_mask_are_refused(ctx):
+    """A stride whose bytes leave 64 bits, on the device and on the host."""
+    print("[case] rules mask stride", flush=True)
+    x, nxt, mask = np.zeros((3, 40), F), np.zeros(3, np.int32), np.zeros(2, np.uint32)
+    d, d_next, d_mask = _up(ctx, x), _up(ctx, nxt), _up(ctx, mask)
+    for stride in (1, (1 << 40) + 1, 1 << 61, 2 ** 63):
+        with pytest.raises(hip.InvalidArgument):
+            ctx.logits_rules_dev(3, 40, d, hip.LogitsRules(mask=d_mask, mask_stride=stride), d, d_next)
+        c = hip._LogitsRules()
+        c.mask, c.mask_stride = mask.ctypes.data, stride
+        assert hip.lib().vokra_hip_logits_rules(ctx._h, 3, 40, hip._ptr(x, C.c_float), C.byref(c),
+                                                hip._ptr(x, C.c_float), hip._ptr(nxt, C.c_int32)) == 5

@@ -162,8 +162,9 @@ int rules_check(const vokra_hip_logits_rules_t* r, size_t rows, size_t vocab, si
     if (r->n_hist && (!r->hist || !r->hist_offsets)) return ctx_fail(BAD, "logits_rules: history without its arrays");
     if (r->n_bias && (!r->bias_ids || !r->bias || !r->bias_offsets))
         return ctx_fail(BAD, "logits_rules: biases without their arrays");
-    if (r->mask && r->mask_stride != 0 && r->mask_stride < (vocab + 31) / 32)
-        return ctx_fail(BAD, "logits_rules: mask stride %zu below %zu words", r->mask_stride, (vocab + 31) / 32);
+    if (r->mask && r->mask_stride != 0 && (r->mask_stride < (vocab + 31) / 32 || r->mask_stride > ((size_t)1 << 40)))
+        return ctx_fail(BAD, "logits_rules: mask stride %zu below %zu words or too large", r->mask_stride,
+                        (vocab + 31) / 32);
     if (out && out != logits && meet(logits, ((rows - 1) * stride + vocab) * 4, out, ((rows - 1) * stride + vocab) * 4))
         return ctx_fail(BAD, "logits_rules: logits and out overlap without being the same");
     return VOKRA_HIP_OK;
