@@ -216,7 +216,6 @@ int vokra_hip_bkv_create(vokra_hip_ctx_t* c, size_t n_layer, size_t n_head, size
     if (e == hipSuccess) e = hipStreamSynchronize(vk::ctx_stream(c));
     if (e != hipSuccess) {
         release(kv);
-        (void)hipGetLastError();
         return ctx_fail(VOKRA_HIP_ERROR_BACKEND_UNAVAILABLE, "bkv_create: %s", hipGetErrorString(e));
     }
     *out = kv;

@@ -33,6 +33,8 @@ int fail(int code, const char* fmt, ...) {
     vsnprintf(buf, sizeof buf, fmt, ap);
     va_end(ap);
     g_last_error = buf;
+    // HIP keeps an error until it is asked for: reported here, it is not the next launch's
+    if (code == VOKRA_HIP_ERROR_BACKEND_UNAVAILABLE) (void)hipGetLastError();
     return code;
 }
 
