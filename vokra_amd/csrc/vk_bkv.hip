@@ -771,10 +771,11 @@ hipError_t launch_bkv_read(hipStream_t s, const BkvView& v, int layer, int n, co
     return hipGetLastError();
 }
 
-// Workgroups of the ring rows of n items, four waves each. The rings of a cache
-// that fits the card are fewer than a launch has threads for.
+// Workgroups of the ring rows of n items, four waves each. Items name a destination each,
+// so no more than n_seq are done, and the rings of a cache that fits the card are fewer than
+// a launch has threads for.
 static unsigned row_grid(const BkvView& v, int n) {
-    return (unsigned)(((long long)n * v.n_layer * 2 * v.n_head + 3) / 4);
+    return (unsigned)(((long long)std::min(n, v.n_seq) * v.n_layer * 2 * v.n_head + 3) / 4);
 }
 
 hipError_t launch_bkv_fork(hipStream_t s, const BkvView& v, int n, const int* src, const int* dst) {
