@@ -483,9 +483,10 @@ int vokra_hip_bkv_write_dev(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t la
  * or a weight with 8-bit values run as two fp16 parts of the f32 operand (22
  * bits), those with f32 rows in f32, sums in f32; a key whose weight is below 2^-112
  * of its row's largest may count as less. Rows that the step does not
- * reach are left as they are; out does not overlap q. One token a sequence,
- * several (drafts) and long chunks of prompts take the same call; how a row's
- * keys are split depends on the whole step, and its last bits may with it. */
+ * reach are left as they are; out does not overlap q (the same buffer for both
+ * is INVALID_ARGUMENT). One token a sequence, several (drafts) and long chunks of
+ * prompts take the same call; how a row's keys are split depends on the whole
+ * step, and its last bits may with it. */
 int vokra_hip_bkv_attn(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t layer, size_t n_head_q, const float *q,
                        float scale, float *out);
 /* Device arrays (16-byte aligned), asynchronous. */

@@ -127,3 +127,14 @@ def test_attention_under_a_negative_scale(ctx):
         p.check_attn(0, 335, 4, scale)
         p.step([0, 1], [290, 45], [1, 3])
         p.check_attn(0, 4, 4, scale)
+
+
+def test_one_buffer_for_q_and_the_output_is_refused(ctx):
+    print("[case] bkv attn one buffer", flush=True)
+    kv = ctx.block_kv_cache(1, 2, 64, 3, 100, 16, 10, 64)
+    kv.step([0, 1], [0, 0], [3, 2])
+    q, out = (hip.DeviceBuffer.from_array(ctx, np.zeros(5 * 256, np.float32)) for _ in (0, 1))
+    with pytest.raises(hip.InvalidArgument):
+        kv.attn_dev(0, 4, q, 0.125, q)
+    kv.attn_dev(0, 4, q, 0.125, out)
+    ctx.synchronize()

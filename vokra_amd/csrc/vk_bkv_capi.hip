@@ -310,6 +310,7 @@ int vokra_hip_bkv_attn_dev(vokra_hip_ctx_t* c, vokra_hip_bkv_t* kv, size_t layer
     if (kv->step_rows == 0) return VOKRA_HIP_OK;
     if (!d_q || !d_out) return ctx_fail(BAD, "bkv_attn: NULL buffer");
     if (!aligned16(d_q) || !aligned16(d_out)) return ctx_fail(BAD, "bkv_attn: q and out must be 16-byte aligned");
+    if (d_q == d_out) return ctx_fail(BAD, "bkv_attn: out overlaps q");
     return attn_launch(kv, layer, n_head_q, d_q, scale, d_out);
 }
 
