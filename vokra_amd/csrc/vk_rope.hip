@@ -7,13 +7,15 @@
 // product of position and frequency is off by 2^-24 of the whole angle: a
 // tenth of a radian at position 10^6). The top 32 bits give the quadrant and a
 // rest in [-pi/4, pi/4], whose sine and cosine are Taylor polynomials in f32
-// (degrees 9 and 10: the first terms left out are below 2e-9).
+// (degrees 9 and 10: the first terms left out are below 2e-9). They are multiplied by the
+// magnitude after that, so where it is not 1 they are rounded twice: half a step of
+// f32 more, for one product a pair instead of one a value.
 //
 // Bound by memory: 8 bytes an element moved, about 40 VALU operations a pair
 // for its sine and cosine, which the heads that a thread turns share. 8191 rows of
 // 32 + 8 heads of 128, half of each turned, to another buffer: 336 MB in 59 us, 5.7
-// TB/s (part of them in the cache behind the L2s); 32 rows of 16 + 2 heads take 4.7
-// us, the launch and three dependent rounds of memory.
+// TB/s (part of them in the cache behind the L2s); 32 rows of 16 + 2 heads take 2.9
+// us, which is dependent rounds of memory (the call 4.7, most of it the host's).
 #include <algorithm>
 
 #include "vk_common.h"
@@ -130,12 +132,13 @@ hipError_t launch_rope_turn(hipStream_t s, RopeArgs a, bool pairs) {
     const bool vec = (addr & 15) == 0 && strides % 4 == 0 && a.hd % 4 == 0;
     const int v = !vec ? 1 : pairs ? (a.rot % 4 == 0 ? 2 : 1) : (half % 4 == 0 && (!copies || tail % 8 == 0) ? 4 : 1);
     a.units = half / v + (copies ? (tail + 2 * v - 1) / (2 * v) : 0);
-    // heads a thread: one where that leaves fewer than 2048 workgroups (32 rows of 18
-    // heads: 5.1 us, four 5.4), four where there is work enough (sine and cosine
-    // shared: 500 rows of 40 heads 5.6 us, one 6.3)
+    // heads a thread: one where that leaves fewer than 1024 workgroups, four (sine and cosine
+    // shared) from there on. The kernel's time, half layout of 128, one head a thread and
+    // four: 32 rows of 18 heads 3.0 and 3.9 us, 300 rows of 40 (750 workgroups) 4.1 and
+    // 4.5, 500 (1250) 5.2 and 5.0, 800 6.9 and 5.8, 2000 13.8 and 13.6
     const int heads = a.heads_q + a.heads_k;
     const size_t all = (size_t)a.rows * a.units * heads;
-    a.head_lanes = all / 256 < 2048 ? heads : (heads + 3) / 4;
+    a.head_lanes = all / 256 < 1024 ? heads : (heads + 3) / 4;
     // outputs that the caches cannot hold beside the inputs go past them (63 us -> 59 for
     // the call above; 1500 rows, which they hold, take 10.9 us with them and 11.2 past)
     const bool past = v > 1 && (size_t)a.rows * heads * a.hd > (size_t)32 << 20;
