@@ -476,9 +476,14 @@ int vokra_hip_bkv_write(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t layer,
 int vokra_hip_bkv_write_dev(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t layer, const float *d_k,
                             const float *d_v);
 /* Attention of the step's rows: the row at position p of its sequence attends
- * to rows 0..p as the cache holds them,
- *   out = softmax((q * scale) . K^T) . V,
- * query head h with kv head h / (n_head_q / n_head); q, out [rows][n_head_q *
+ * to rows 0..p as the cache holds them once the step is written,
+ *   out = softmax((q * scale) . K^T) . V.
+ * Where the step fills p's block, that block is held in 8 bits, under a scale in
+ * which the step's rows behind p have a part: a draft's output depends, within the
+ * rounding of 8 bits, on the drafts behind it (also on ones that are then taken
+ * back), and a prompt's rows on where the prompt is cut into steps. Steps of one
+ * row a sequence, and steps that fill no block, have no such rows.
+ * Query head h with kv head h / (n_head_q / n_head); q, out [rows][n_head_q *
  * d_head], n_head_q any multiple of n_head. f32 in and out: products of a query
  * or a weight with 8-bit values run as two fp16 parts of the f32 operand (22
  * bits), those with f32 rows in f32, sums in f32; a key whose weight is below 2^-112
@@ -486,7 +491,7 @@ int vokra_hip_bkv_write_dev(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t la
  * reach are left as they are; out does not overlap q (the same buffer for both
  * is INVALID_ARGUMENT). One token a sequence, several (drafts) and long chunks of
  * prompts take the same call; how a row's keys are split depends on the whole
- * step, and its last bits may with it. */
+ * step, and beside the above its last f32 bits may with it. */
 int vokra_hip_bkv_attn(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t layer, size_t n_head_q, const float *q,
                        float scale, float *out);
 /* Device arrays (16-byte aligned), asynchronous. */
@@ -607,7 +612,9 @@ int vokra_hip_rope_apply(vokra_hip_ctx_t *ctx, const vokra_hip_rope_t *rope, siz
  * are passed over (padding). n_hist and n_bias are the lists' lengths, and no
  * offset reads beyond them. repetition, presence, frequency: one value a row,
  * NULL = 1, 0, 0. mask: word v / 32, bit v % 32 of a row, rows mask_stride
- * words apart (0: one mask for all rows); NULL = every token is allowed. */
+ * words apart (0: one mask for all rows); NULL = every token is allowed. Penalties
+ * that count different histories take a call each, the first without a mask and
+ * next (biases and masks come after every penalty). */
 typedef struct vokra_hip_logits_rules {
     size_t n_hist;
     const int32_t *hist, *hist_offsets;

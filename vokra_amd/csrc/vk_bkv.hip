@@ -36,7 +36,7 @@ constexpr int BKV_TPB = 1024;  // threads of the planning kernels at most
 // ---- workgroup prefix sums ----------------------------------------------------
 
 // Exclusive prefix sums of N numbers a thread over the workgroup, in place;
-// totals in sum. red: 17 N ints.
+// totals in sum. red: N ints a wave.
 template <int N>
 __device__ __forceinline__ void bkv_scan(int (&v)[N], int (&sum)[N], int* red) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = (int)blockDim.x >> 6;

@@ -14,7 +14,7 @@
 // Bound by memory: 8 bytes an element moved, about 40 VALU operations a pair
 // for its sine and cosine, which the heads that a thread turns share. 8191 rows of
 // 32 + 8 heads of 128, half of each turned, to another buffer: 336 MB in 59 us, 5.7
-// TB/s (part of them in the cache behind the L2s); 32 rows of 16 + 2 heads take 2.9
+// TB/s (part of them in the cache behind the L2s); 32 rows of 16 + 2 heads take 3
 // us, which is dependent rounds of memory (the call 4.7, most of it the host's).
 #include <algorithm>
 
