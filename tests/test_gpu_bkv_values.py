@@ -138,3 +138,16 @@ def test_one_buffer_for_q_and_the_output_is_refused(ctx):
         kv.attn_dev(0, 4, q, 0.125, q)
     kv.attn_dev(0, 4, q, 0.125, out)
     ctx.synchronize()
+
+
+@pytest.mark.parametrize("first,count,heads,far", [(250, 22, 2, False), (250, 5, 2, False), (2040, 48, 2, False),
+                                                   (505, 30, 4, False), (250, 60, 4, True), (250, 300, 2, True)])
+@pytest.mark.parametrize("codec,hd", [(0, 64), (1, 128)])
+def test_key_ranges_hidden_from_a_tiles_first_rows(ctx, codec, hd, first, count, heads, far):
+    """The last key range of a tile begins behind its first rows, which have no key in it."""
+    print("[case] bkv hidden range", codec, hd, first, count, heads, far, flush=True)
+    t = first + count
+    p = filled(ctx, codec, hd, t, count, np.ones(t), far, seed=t)
+    got, want, tol = attend(ctx, p, t, count, heads, far)
+    err = np.abs(got - want) / tol
+    assert np.all(err <= 1), f"{np.nanmax(err)} of the bound"

@@ -729,7 +729,7 @@ __global__ __launch_bounds__(64 * kWaves, C == 2 ? 2 : HD == 64 ? 5 : 3) void vk
                 f[x] = sml[x][c].y * __builtin_amdgcn_exp2f(sml[x][c].x - m);
                 sum += f[x];
             }
-            const float inv = 1.0f / sum;
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // 0: the range is hidden from the column
             vk_f32x4 y[PD / 4];
 #pragma unroll
             for (int i = 0; i < PD / 4; ++i) {
