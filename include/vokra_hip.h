@@ -468,7 +468,8 @@ int vokra_hip_bkv_step_dev(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t n, 
 int vokra_hip_bkv_status(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t *n_done);
 
 /* The step's rows of one layer, k and v [rows][n_head * d_head], into the
- * cache. Every layer is written once a step, before that layer's attn, and
+ * cache (the host forms of write and attn take n_rows rows after a step_dev,
+ * however many its counts name). Every layer is written once a step, before that layer's attn, and
  * before a sequence of the step is forked, copied or stepped again. */
 int vokra_hip_bkv_write(vokra_hip_ctx_t *ctx, vokra_hip_bkv_t *kv, size_t layer, const float *k_rows,
                         const float *v_rows);
