@@ -36,10 +36,10 @@
 // 2^-E: E is the running maximum of s - M + e, rounded up, so the largest product is near
 // 1 whatever the blocks' values are, a block of small values keeps its bits beside one of
 // large values, and zeros (e is below that of any other block) take nothing from either.
-// Two fp16 parts of 2^14 of that hold it to 2^-22, or to 2^-39 of the largest where it is
-// smaller than 2^-17 of that. M and E are whole numbers, so what was summed is brought
-// under new ones exactly, and seldom. The open block's rows are f32 on both sides and use
-// the f32 matrix instruction.
+// Two fp16 parts of 2^14 of that hold it to 2^-22, or to 2^-38 of the largest where it is
+// smaller than 2^-16 of that (the largest is above 2^13 and below 2^15). M and E are whole
+// numbers, so what was summed is brought under new ones exactly, and seldom. The open
+// block's rows are f32 on both sides and use the f32 matrix instruction.
 #include <algorithm>
 #include <cmath>
 
