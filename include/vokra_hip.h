@@ -598,6 +598,27 @@ int vokra_hip_rope_apply_dev(vokra_hip_ctx_t *ctx, const vokra_hip_rope_t *rope,
 int vokra_hip_rope_apply(vokra_hip_ctx_t *ctx, const vokra_hip_rope_t *rope, size_t rows, const int32_t *positions,
                          size_t n_head_q, const float *q, float *q_out, size_t n_head_k, const float *k, float *k_out);
 
+/* The same with a norm of every head in front, one pass: x is divided by the root
+ * of its mean square, x / sqrt(sum x^2 / head_dim + eps), multiplied by gamma and then
+ * turned; the values beyond rot_dim are normed too. gamma: head_dim values for all
+ * heads of a side (stride 0), or a row for each head, stride floats apart (at least
+ * head_dim); NULL: ones. No counterpart in the reference (its heads have no norms).
+ * Everything else as in rope_apply; gammas overlap no output. */
+typedef struct vokra_hip_head_norm {
+    const float *q_gamma, *k_gamma;
+    size_t q_gamma_stride, k_gamma_stride;
+    float eps; /* finite, >= 0 */
+} vokra_hip_head_norm_t;
+/* Device pointers (the struct itself in host memory), asynchronous. */
+int vokra_hip_rope_norm_apply_dev(vokra_hip_ctx_t *ctx, const vokra_hip_rope_t *rope, const vokra_hip_head_norm_t *norm,
+                                  size_t rows, const int32_t *d_positions, size_t n_head_q, const float *d_q,
+                                  size_t q_stride, float *d_q_out, size_t q_out_stride, size_t n_head_k,
+                                  const float *d_k, size_t k_stride, float *d_k_out, size_t k_out_stride);
+/* Host arrays (gammas too), synchronous; rows lie side by side. */
+int vokra_hip_rope_norm_apply(vokra_hip_ctx_t *ctx, const vokra_hip_rope_t *rope, const vokra_hip_head_norm_t *norm,
+                              size_t rows, const int32_t *positions, size_t n_head_q, const float *q, float *q_out,
+                              size_t n_head_k, const float *k, float *k_out);
+
 /* The rules that logits pass before a token is chosen, and the greedy choice.
  * No counterpart in the reference (its sampler takes the argmax of the logits
  * as they are, crates/vokra-core/src/decode/sampler.rs:197-206). For token v of

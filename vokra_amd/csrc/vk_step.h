@@ -1,7 +1,8 @@
 // vk_step.h — launchers of the operators around a decode step that are no
-// part of a session: rotary positions by a plan (vk_rope.hip) and the rules
-// that logits pass before the greedy choice (vk_rules.hip). The C-ABI layer
-// (vk_step_capi.hip) checks their arguments.
+// part of a session: rotary positions by a plan, with or without norms of the
+// heads before them (vk_rope.hip), and the rules that logits pass before the
+// greedy choice (vk_rules.hip). The C-ABI layer (vk_step_capi.hip) checks their
+// arguments.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stddef.h>
@@ -16,6 +17,11 @@ struct RopeArgs {
     float mag;
     int rows, heads_q, heads_k, hd, rot;
     int units, head_lanes;  // set by the launcher
+    // norms (launch_rope_norm): weights of q's and k's heads (NULL: ones), floats from
+    // head to head (0: one row for all)
+    const float *q_gamma, *k_gamma;
+    size_t qg_stride, kg_stride;
+    float eps;
 };
 
 // A context's workspace of the greedy choice: rows' maxima, then their counters.
@@ -39,6 +45,7 @@ struct RulesArgs {
 namespace vk {
 // units and head_lanes are filled in here
 hipError_t launch_rope_turn(hipStream_t s, RopeArgs a, bool pairs);
+hipError_t launch_rope_norm(hipStream_t s, RopeArgs a, bool pairs);
 hipError_t launch_rules_clear(hipStream_t s, void* part);
 hipError_t launch_rules(hipStream_t s, const RulesArgs& a);
 }  // namespace vk

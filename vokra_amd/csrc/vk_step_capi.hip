@@ -180,6 +180,116 @@ int to_device(hipStream_t s, Temp& t, const void* h, size_t bytes, const void** 
     return VOKRA_HIP_OK;
 }
 
+int norm_check(const vokra_hip_rope* p, const vokra_hip_head_norm_t& f, size_t n_head_q, size_t n_head_k) {
+    if (!std::isfinite(f.eps) || f.eps < 0.0f) return ctx_fail(BAD, "rope_norm_apply: eps must be finite and >= 0");
+    for (int i = 0; i < 2; ++i) {
+        const size_t st = i ? f.k_gamma_stride : f.q_gamma_stride;
+        if ((i ? n_head_k : n_head_q) && (i ? f.k_gamma : f.q_gamma) && st != 0 &&
+            (st < p->hd || st > ((size_t)1 << 40)))
+            return ctx_fail(BAD, "rope_norm_apply: a gamma stride of %zu is below head_dim %zu or too large", st, p->hd);
+    }
+    return VOKRA_HIP_OK;
+}
+
+// Rows through the plan, with norms of the heads before it where norm is given.
+int rope_run(vokra_hip_ctx* c, const vokra_hip_rope* p, const vokra_hip_head_norm_t* norm, size_t rows,
+             const int32_t* d_positions, size_t n_head_q, const float* d_q, size_t q_stride, float* d_q_out,
+             size_t q_out_stride, size_t n_head_k, const float* d_k, size_t k_stride, float* d_k_out,
+             size_t k_out_stride) {
+    if (!c || !p || p->ctx != c) return ctx_fail(BAD, "rope_apply: bad context or plan");
+    if (rows == 0 || n_head_q + n_head_k == 0) return VOKRA_HIP_OK;
+    ST_ST(rope_size(p, rows, n_head_q, n_head_k));
+    if (norm) ST_ST(norm_check(p, *norm, n_head_q, n_head_k));
+    if (!d_positions) return ctx_fail(BAD, "rope_apply: positions is NULL");
+    ST_ST(rope_side(p, "q", rows, n_head_q, d_q, q_stride, d_q_out, q_out_stride));
+    ST_ST(rope_side(p, "k", rows, n_head_k, d_k, k_stride, d_k_out, k_out_stride));
+    const size_t wq = n_head_q * p->hd, wk = n_head_k * p->hd;
+    if (wq && wk &&
+        (rows_meet(rows, d_q_out, wq, q_out_stride, d_k, wk, k_stride) ||
+         rows_meet(rows, d_k_out, wk, k_out_stride, d_q, wq, q_stride) ||
+         rows_meet(rows, d_q_out, wq, q_out_stride, d_k_out, wk, k_out_stride)))
+        return ctx_fail(BAD, "rope_apply: an output overlaps the other side's input or output");
+    if ((wq && meet(d_q_out, ((rows - 1) * q_out_stride + wq) * 4, d_positions, rows * 4)) ||
+        (wk && meet(d_k_out, ((rows - 1) * k_out_stride + wk) * 4, d_positions, rows * 4)))
+        return ctx_fail(BAD, "rope_apply: an output overlaps positions");
+    const float* gamma[2] = {norm && wq ? norm->q_gamma : nullptr, norm && wk ? norm->k_gamma : nullptr};
+    for (int i = 0; i < 2; ++i) {
+        if (!gamma[i]) continue;
+        const size_t n = ((i ? n_head_k : n_head_q) - 1) * (i ? norm->k_gamma_stride : norm->q_gamma_stride) + p->hd;
+        if ((wq && meet(d_q_out, ((rows - 1) * q_out_stride + wq) * 4, gamma[i], n * 4)) ||
+            (wk && meet(d_k_out, ((rows - 1) * k_out_stride + wk) * 4, gamma[i], n * 4)))
+            return ctx_fail(BAD, "rope_norm_apply: an output overlaps a gamma");
+    }
+    ST_TRY(hipSetDevice(vk::ctx_device(c)), "hipSetDevice");
+    RopeArgs a = {};
+    a.q = n_head_q ? d_q : d_k;  // (an absent side is given the other's address and never read)
+    a.k = d_k;
+    a.q_out = n_head_q ? d_q_out : d_k_out;
+    a.k_out = d_k_out;
+    a.q_stride = n_head_q ? q_stride : k_stride;
+    a.qo_stride = n_head_q ? q_out_stride : k_out_stride;
+    a.k_stride = k_stride;
+    a.ko_stride = k_out_stride;
+    a.positions = d_positions;
+    a.turn = p->turn;
+    a.mag = p->mag;
+    a.rows = (int)rows;
+    a.heads_q = (int)n_head_q;
+    a.heads_k = (int)n_head_k;
+    a.hd = (int)p->hd;
+    a.rot = (int)p->rot;
+    if (norm) {
+        a.q_gamma = gamma[0];
+        a.k_gamma = gamma[1];
+        a.qg_stride = gamma[0] ? norm->q_gamma_stride : 0;
+        a.kg_stride = gamma[1] ? norm->k_gamma_stride : 0;
+        a.eps = norm->eps;
+        ST_TRY(vk::launch_rope_norm(vk::ctx_stream(c), a, p->pairs), "launch(vk_rope_norm)");
+        return VOKRA_HIP_OK;
+    }
+    ST_TRY(vk::launch_rope_turn(vk::ctx_stream(c), a, p->pairs), "launch(vk_rope_turn)");
+    return VOKRA_HIP_OK;
+}
+
+// The same on host arrays, gammas included.
+int rope_run_host(vokra_hip_ctx* c, const vokra_hip_rope* p, const vokra_hip_head_norm_t* norm, size_t rows,
+                  const int32_t* positions, size_t n_head_q, const float* q, float* q_out, size_t n_head_k,
+                  const float* k, float* k_out) {
+    if (!c || !p || p->ctx != c) return ctx_fail(BAD, "rope_apply: bad context or plan");
+    if (rows == 0 || n_head_q + n_head_k == 0) return VOKRA_HIP_OK;
+    ST_ST(rope_size(p, rows, n_head_q, n_head_k));
+    if (norm) ST_ST(norm_check(p, *norm, n_head_q, n_head_k));
+    if (!positions || (n_head_q && (!q || !q_out)) || (n_head_k && (!k || !k_out)))
+        return ctx_fail(BAD, "rope_apply: NULL buffer");
+    ST_TRY(hipSetDevice(vk::ctx_device(c)), "hipSetDevice");
+    hipStream_t s = vk::ctx_stream(c);
+    const size_t wq = n_head_q * p->hd, wk = n_head_k * p->hd;
+    Temp x, pos, gq, gk;
+    ST_TRY(x.make(rows * (wq + wk) * sizeof(float)), "hipMalloc");
+    ST_TRY(pos.make(rows * sizeof(int32_t)), "hipMalloc");
+    float *dq = (float*)x.p, *dk = dq + rows * wq;
+    ST_TRY(hipMemcpyAsync(pos.p, positions, rows * sizeof(int32_t), hipMemcpyHostToDevice, s), "hipMemcpyAsync");
+    if (wq) ST_TRY(hipMemcpyAsync(dq, q, rows * wq * sizeof(float), hipMemcpyHostToDevice, s), "hipMemcpyAsync");
+    if (wk) ST_TRY(hipMemcpyAsync(dk, k, rows * wk * sizeof(float), hipMemcpyHostToDevice, s), "hipMemcpyAsync");
+    vokra_hip_head_norm_t dev = {};
+    if (norm) {
+        dev = *norm;
+        const size_t nq = wq ? (n_head_q - 1) * norm->q_gamma_stride + p->hd : 0;
+        const size_t nk = wk ? (n_head_k - 1) * norm->k_gamma_stride + p->hd : 0;
+        const void* d = nullptr;
+        ST_ST(to_device(s, gq, nq ? norm->q_gamma : nullptr, nq * sizeof(float), &d));
+        dev.q_gamma = (const float*)d;
+        ST_ST(to_device(s, gk, nk ? norm->k_gamma : nullptr, nk * sizeof(float), &d));
+        dev.k_gamma = (const float*)d;
+    }
+    ST_ST(rope_run(c, p, norm ? &dev : nullptr, rows, (const int32_t*)pos.p, n_head_q, dq, wq, dq, wq, n_head_k, dk, wk,
+                   dk, wk));
+    if (wq) ST_TRY(hipMemcpyAsync(q_out, dq, rows * wq * sizeof(float), hipMemcpyDeviceToHost, s), "hipMemcpyAsync");
+    if (wk) ST_TRY(hipMemcpyAsync(k_out, dk, rows * wk * sizeof(float), hipMemcpyDeviceToHost, s), "hipMemcpyAsync");
+    ST_TRY(hipStreamSynchronize(s), "hipStreamSynchronize");
+    return VOKRA_HIP_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -234,67 +344,30 @@ void vokra_hip_rope_destroy(vokra_hip_rope_t* p) {
 int vokra_hip_rope_apply_dev(vokra_hip_ctx_t* c, const vokra_hip_rope_t* p, size_t rows, const int32_t* d_positions,
                              size_t n_head_q, const float* d_q, size_t q_stride, float* d_q_out, size_t q_out_stride,
                              size_t n_head_k, const float* d_k, size_t k_stride, float* d_k_out, size_t k_out_stride) {
-    if (!c || !p || p->ctx != c) return ctx_fail(BAD, "rope_apply: bad context or plan");
-    if (rows == 0 || n_head_q + n_head_k == 0) return VOKRA_HIP_OK;
-    ST_ST(rope_size(p, rows, n_head_q, n_head_k));
-    if (!d_positions) return ctx_fail(BAD, "rope_apply: positions is NULL");
-    ST_ST(rope_side(p, "q", rows, n_head_q, d_q, q_stride, d_q_out, q_out_stride));
-    ST_ST(rope_side(p, "k", rows, n_head_k, d_k, k_stride, d_k_out, k_out_stride));
-    const size_t wq = n_head_q * p->hd, wk = n_head_k * p->hd;
-    if (wq && wk &&
-        (rows_meet(rows, d_q_out, wq, q_out_stride, d_k, wk, k_stride) ||
-         rows_meet(rows, d_k_out, wk, k_out_stride, d_q, wq, q_stride) ||
-         rows_meet(rows, d_q_out, wq, q_out_stride, d_k_out, wk, k_out_stride)))
-        return ctx_fail(BAD, "rope_apply: an output overlaps the other side's input or output");
-    if ((wq && meet(d_q_out, ((rows - 1) * q_out_stride + wq) * 4, d_positions, rows * 4)) ||
-        (wk && meet(d_k_out, ((rows - 1) * k_out_stride + wk) * 4, d_positions, rows * 4)))
-        return ctx_fail(BAD, "rope_apply: an output overlaps positions");
-    ST_TRY(hipSetDevice(vk::ctx_device(c)), "hipSetDevice");
-    RopeArgs a = {};
-    a.q = n_head_q ? d_q : d_k;  // (an absent side is given the other's address and never read)
-    a.k = d_k;
-    a.q_out = n_head_q ? d_q_out : d_k_out;
-    a.k_out = d_k_out;
-    a.q_stride = n_head_q ? q_stride : k_stride;
-    a.qo_stride = n_head_q ? q_out_stride : k_out_stride;
-    a.k_stride = k_stride;
-    a.ko_stride = k_out_stride;
-    a.positions = d_positions;
-    a.turn = p->turn;
-    a.mag = p->mag;
-    a.rows = (int)rows;
-    a.heads_q = (int)n_head_q;
-    a.heads_k = (int)n_head_k;
-    a.hd = (int)p->hd;
-    a.rot = (int)p->rot;
-    ST_TRY(vk::launch_rope_turn(vk::ctx_stream(c), a, p->pairs), "launch(vk_rope_turn)");
-    return VOKRA_HIP_OK;
+    return rope_run(c, p, nullptr, rows, d_positions, n_head_q, d_q, q_stride, d_q_out, q_out_stride, n_head_k, d_k,
+                    k_stride, d_k_out, k_out_stride);
+}
+
+int vokra_hip_rope_norm_apply_dev(vokra_hip_ctx_t* c, const vokra_hip_rope_t* p, const vokra_hip_head_norm_t* norm,
+                                  size_t rows, const int32_t* d_positions, size_t n_head_q, const float* d_q,
+                                  size_t q_stride, float* d_q_out, size_t q_out_stride, size_t n_head_k,
+                                  const float* d_k, size_t k_stride, float* d_k_out, size_t k_out_stride) {
+    if (!norm) return ctx_fail(BAD, "rope_norm_apply: norm is NULL");
+    return rope_run(c, p, norm, rows, d_positions, n_head_q, d_q, q_stride, d_q_out, q_out_stride, n_head_k, d_k,
+                    k_stride, d_k_out, k_out_stride);
 }
 
 int vokra_hip_rope_apply(vokra_hip_ctx_t* c, const vokra_hip_rope_t* p, size_t rows, const int32_t* positions,
                          size_t n_head_q, const float* q, float* q_out, size_t n_head_k, const float* k,
                          float* k_out) {
-    if (!c || !p || p->ctx != c) return ctx_fail(BAD, "rope_apply: bad context or plan");
-    if (rows == 0 || n_head_q + n_head_k == 0) return VOKRA_HIP_OK;
-    ST_ST(rope_size(p, rows, n_head_q, n_head_k));
-    if (!positions || (n_head_q && (!q || !q_out)) || (n_head_k && (!k || !k_out)))
-        return ctx_fail(BAD, "rope_apply: NULL buffer");
-    ST_TRY(hipSetDevice(vk::ctx_device(c)), "hipSetDevice");
-    hipStream_t s = vk::ctx_stream(c);
-    const size_t wq = n_head_q * p->hd, wk = n_head_k * p->hd;
-    Temp x, pos;
-    ST_TRY(x.make(rows * (wq + wk) * sizeof(float)), "hipMalloc");
-    ST_TRY(pos.make(rows * sizeof(int32_t)), "hipMalloc");
-    float *dq = (float*)x.p, *dk = dq + rows * wq;
-    ST_TRY(hipMemcpyAsync(pos.p, positions, rows * sizeof(int32_t), hipMemcpyHostToDevice, s), "hipMemcpyAsync");
-    if (wq) ST_TRY(hipMemcpyAsync(dq, q, rows * wq * sizeof(float), hipMemcpyHostToDevice, s), "hipMemcpyAsync");
-    if (wk) ST_TRY(hipMemcpyAsync(dk, k, rows * wk * sizeof(float), hipMemcpyHostToDevice, s), "hipMemcpyAsync");
-    ST_ST(vokra_hip_rope_apply_dev(c, p, rows, (const int32_t*)pos.p, n_head_q, dq, wq, dq, wq, n_head_k, dk, wk, dk,
-                                   wk));
-    if (wq) ST_TRY(hipMemcpyAsync(q_out, dq, rows * wq * sizeof(float), hipMemcpyDeviceToHost, s), "hipMemcpyAsync");
-    if (wk) ST_TRY(hipMemcpyAsync(k_out, dk, rows * wk * sizeof(float), hipMemcpyDeviceToHost, s), "hipMemcpyAsync");
-    ST_TRY(hipStreamSynchronize(s), "hipStreamSynchronize");
-    return VOKRA_HIP_OK;
+    return rope_run_host(c, p, nullptr, rows, positions, n_head_q, q, q_out, n_head_k, k, k_out);
+}
+
+int vokra_hip_rope_norm_apply(vokra_hip_ctx_t* c, const vokra_hip_rope_t* p, const vokra_hip_head_norm_t* norm,
+                              size_t rows, const int32_t* positions, size_t n_head_q, const float* q, float* q_out,
+                              size_t n_head_k, const float* k, float* k_out) {
+    if (!norm) return ctx_fail(BAD, "rope_norm_apply: norm is NULL");
+    return rope_run_host(c, p, norm, rows, positions, n_head_q, q, q_out, n_head_k, k, k_out);
 }
 
 int vokra_hip_logits_rules_dev(vokra_hip_ctx_t* c, size_t rows, size_t vocab, size_t stride, const float* d_logits,

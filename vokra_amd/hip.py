@@ -156,6 +156,12 @@ class RopeConfig(C.Structure):
                [("divisors", C.POINTER(C.c_double))]
 
 
+class _HeadNorm(C.Structure):
+    """vokra_hip_head_norm_t"""
+    _fields_ = [(n, C.c_void_p) for n in ("q_gamma", "k_gamma")] + \
+               [(n, C.c_size_t) for n in ("q_gamma_stride", "k_gamma_stride")] + [("eps", C.c_float)]
+
+
 class _LogitsRules(C.Structure):
     """vokra_hip_logits_rules_t"""
     _fields_ = [("n_hist", C.c_size_t), ("hist", C.c_void_p), ("hist_offsets", C.c_void_p),
@@ -281,6 +287,8 @@ def _declare(L):
     L.vokra_hip_rope_destroy.restype = None
     L.vokra_hip_rope_apply_dev.argtypes = [P, P, sz, P, sz, P, sz, P, sz, sz, P, sz, P, sz]
     L.vokra_hip_rope_apply.argtypes = [P, P, sz, i32p, sz, f32p, f32p, sz, f32p, f32p]
+    L.vokra_hip_rope_norm_apply_dev.argtypes = [P, P, C.POINTER(_HeadNorm), sz, P, sz, P, sz, P, sz, sz, P, sz, P, sz]
+    L.vokra_hip_rope_norm_apply.argtypes = [P, P, C.POINTER(_HeadNorm), sz, i32p, sz, f32p, f32p, sz, f32p, f32p]
     L.vokra_hip_logits_rules_dev.argtypes = [P, sz, sz, sz, P, C.POINTER(_LogitsRules), P, P]
     L.vokra_hip_logits_rules.argtypes = [P, sz, sz, f32p, C.POINTER(_LogitsRules), f32p, i32p]
     L.vokra_hip_gemm_f32.argtypes = [P, sz, sz, sz, f32p, sz, f32p, sz, f32p, f32p, sz]
@@ -890,34 +898,66 @@ class RopePlan:
                   k_stride=None, q_out_stride=None, k_out_stride=None):
         """Rows of q and k at positions[r]; an output may be its input. Strides in
         floats; where not given, the heads' width, and in place the input's."""
-        wq, wk = n_head_q * self.head_dim, n_head_k * self.head_dim
-        if q_stride is None:
-            q_stride = wq
-        if q_out_stride is None:
-            q_out_stride = q_stride if d_q_out is d_q else wq
-        if k_stride is None:
-            k_stride = wk
-        if k_out_stride is None:
-            k_out_stride = k_stride if d_k_out is d_k else wk
-        _check(lib().vokra_hip_rope_apply_dev(
-            self._ctx._h, self._h, rows, d_positions.ptr, n_head_q, None if d_q is None else d_q.ptr, q_stride,
-            None if d_q_out is None else d_q_out.ptr, q_out_stride, n_head_k, None if d_k is None else d_k.ptr, k_stride,
-            None if d_k_out is None else d_k_out.ptr, k_out_stride))
+        _check(lib().vokra_hip_rope_apply_dev(self._ctx._h, self._h, rows, d_positions.ptr,
+                                              *self._sides(n_head_q, d_q, d_q_out, q_stride, q_out_stride),
+                                              *self._sides(n_head_k, d_k, d_k_out, k_stride, k_out_stride)))
+
+    def _sides(self, heads, d_x, d_out, stride, out_stride):
+        w = heads * self.head_dim
+        if stride is None:
+            stride = w
+        if out_stride is None:
+            out_stride = stride if d_out is d_x else w
+        return heads, None if d_x is None else d_x.ptr, stride, None if d_out is None else d_out.ptr, out_stride
+
+    def norm_apply_dev(self, rows, d_positions, eps, n_head_q, d_q, d_q_gamma, d_q_out, n_head_k=0, d_k=None,
+                       d_k_gamma=None, d_k_out=None, q_gamma_stride=0, k_gamma_stride=0, q_stride=None, k_stride=None,
+                       q_out_stride=None, k_out_stride=None):
+        """apply_dev with every head divided by its root mean square and weighted
+        before it turns. A gamma has head_dim values (stride 0) or a row a head;
+        None: ones."""
+        norm = _HeadNorm(None if d_q_gamma is None else d_q_gamma.ptr, None if d_k_gamma is None else d_k_gamma.ptr,
+                         q_gamma_stride, k_gamma_stride, eps)
+        _check(lib().vokra_hip_rope_norm_apply_dev(self._ctx._h, self._h, C.byref(norm), rows, d_positions.ptr,
+                                                   *self._sides(n_head_q, d_q, d_q_out, q_stride, q_out_stride),
+                                                   *self._sides(n_head_k, d_k, d_k_out, k_stride, k_out_stride)))
+
+    def _host_sides(self, n, *xs):
+        args, outs = [], []
+        for x in xs:
+            x = None if x is None else _f32(x)
+            if x is not None and (x.size % (self.head_dim * max(n, 1)) or (n == 0 and x.size)):
+                raise InvalidArgument(f"rope plan: {x.size} values for {n} rows of heads of {self.head_dim}")
+            out = None if x is None else np.empty_like(x)
+            heads = 0 if x is None or n == 0 else x.size // n // self.head_dim
+            args += [heads, _ptr(x, C.c_float), _ptr(out, C.c_float)]
+            outs.append(out)
+        return args, tuple(outs)
 
     def apply(self, positions, q=None, k=None):
         """Host rows [n, heads * head_dim]; returns (q, k), None where none is given."""
         pos = np.ascontiguousarray(positions, np.int32).reshape(-1)
-        args, outs = [], []
-        for x in (q, k):
-            x = None if x is None else _f32(x)
-            if x is not None and (x.size % (self.head_dim * max(pos.size, 1)) or (pos.size == 0 and x.size)):
-                raise InvalidArgument(f"rope plan: {x.size} values for {pos.size} rows of heads of {self.head_dim}")
-            out = None if x is None else np.empty_like(x)
-            heads = 0 if x is None or pos.size == 0 else x.size // pos.size // self.head_dim
-            args += [heads, _ptr(x, C.c_float), _ptr(out, C.c_float)]
-            outs.append(out)
+        args, outs = self._host_sides(pos.size, q, k)
         _check(lib().vokra_hip_rope_apply(self._ctx._h, self._h, pos.size, _ptr(pos, C.c_int32), *args))
-        return tuple(outs)
+        return outs
+
+    def norm_apply(self, positions, eps, q=None, q_gamma=None, k=None, k_gamma=None):
+        """apply with norms of the heads in front; a gamma is [head_dim], [heads, head_dim] or None."""
+        pos = np.ascontiguousarray(positions, np.int32).reshape(-1)
+        args, outs = self._host_sides(pos.size, q, k)
+        norm, keep = _HeadNorm(eps=eps), []
+        for name, gamma, heads in (("q", q_gamma, args[0]), ("k", k_gamma, args[3])):
+            if gamma is None:
+                continue
+            g = _f32(gamma)
+            if g.shape not in ((self.head_dim,), (heads, self.head_dim)):
+                raise InvalidArgument(f"rope plan: {name}_gamma {g.shape} for {heads} heads of {self.head_dim}")
+            keep.append(g)
+            setattr(norm, name + "_gamma", g.ctypes.data)
+            setattr(norm, name + "_gamma_stride", self.head_dim if g.ndim == 2 else 0)
+        _check(lib().vokra_hip_rope_norm_apply(self._ctx._h, self._h, C.byref(norm), pos.size, _ptr(pos, C.c_int32),
+                                               *args))
+        return outs
 
     def __del__(self):
         try:
