@@ -372,6 +372,20 @@ int vokra_hip_kv_status(vokra_hip_ctx_t *ctx, vokra_hip_kv_t *kv, size_t *n_appe
 /* read_step (paged_quant.rs:448-480): dequantized rows, *found = 0 for None. */
 int vokra_hip_kv_read(vokra_hip_ctx_t *ctx, vokra_hip_kv_t *kv, size_t layer, size_t t, size_t s, float *k_out,
                       float *v_out, int *found);
+/* Reordering after a beam search's selection (vokra_hip_beam_select): in group
+ * g the stream of beam b, streams[g * beams + b], takes rows 0 .. lens[g] - 1 of the
+ * stream of beam p = parents[g * beams + b] of the same group, in every layer, as they
+ * were before the call (parents may swap and repeat beams). p = -1 or b: the stream
+ * keeps its rows. Rows from lens[g] on stay as they are, in every stream. Pages do not
+ * change hands. beams <= 32; the streams of a call are distinct. Host arrays,
+ * synchronous. No counterpart in the reference (it decodes greedily). */
+int vokra_hip_kv_reorder(vokra_hip_ctx_t *ctx, vokra_hip_kv_t *kv, size_t groups, size_t beams, const int32_t *streams,
+                         const int32_t *parents, const int32_t *lens);
+/* Device arrays, asynchronous, nothing is allocated; max_len (at most max_time) bounds every lens[g]. A
+ * group whose length is not in 0 .. max_len is passed over, and so is a beam whose
+ * parent names none, or with a stream out of range on either side. */
+int vokra_hip_kv_reorder_dev(vokra_hip_ctx_t *ctx, vokra_hip_kv_t *kv, size_t groups, size_t beams,
+                             const int32_t *d_streams, const int32_t *d_parents, const int32_t *d_lens, size_t max_len);
 /* reset (paged_quant.rs:489-493) and release_layer (:500-515). */
 int vokra_hip_kv_reset(vokra_hip_ctx_t *ctx, vokra_hip_kv_t *kv);
 int vokra_hip_kv_release_layer(vokra_hip_ctx_t *ctx, vokra_hip_kv_t *kv, size_t layer);
@@ -862,6 +876,16 @@ int vokra_hip_decoder_step(vokra_hip_ctx_t *ctx, vokra_hip_decoder_t *dec, size_
 int vokra_hip_decoder_step_dev(vokra_hip_ctx_t *ctx, vokra_hip_decoder_t *dec, size_t n, const int32_t *d_streams,
                                const int32_t *d_tokens, const int32_t *d_positions, int32_t *d_next_tokens,
                                float *d_logits);
+/* Reorders the streams of groups of beams as vokra_hip_kv_reorder does, up to
+ * each group's longest stream; a stream takes its parent's position with its rows (one
+ * stream that has read the prompt can be given to all beams so). Cross K/V stays: the
+ * streams of a group hold the same encoder output. */
+int vokra_hip_decoder_reorder(vokra_hip_ctx_t *ctx, vokra_hip_decoder_t *dec, size_t groups, size_t beams,
+                              const int32_t *streams, const int32_t *parents);
+/* For sessions driven through step_dev: the lengths are the caller's. */
+int vokra_hip_decoder_reorder_dev(vokra_hip_ctx_t *ctx, vokra_hip_decoder_t *dec, size_t groups, size_t beams,
+                                  const int32_t *d_streams, const int32_t *d_parents, const int32_t *d_lens,
+                                  size_t max_len);
 /* Synchronizes and reports the last step's page allocation as
  * vokra_hip_kv_status does (INVALID_ARGUMENT for an item outside the cache,
  * KV_CACHE_EXHAUSTED; *n_appended = (layer, item) appends done, layer-major),
@@ -1001,6 +1025,12 @@ int vokra_hip_text_decoder_step(vokra_hip_ctx_t *ctx, vokra_hip_text_decoder_t *
 int vokra_hip_text_decoder_step_dev(vokra_hip_ctx_t *ctx, vokra_hip_text_decoder_t *dec, size_t n,
                                     const int32_t *d_streams, const int32_t *d_tokens, const int32_t *d_positions,
                                     int32_t *d_next_tokens, float *d_logits);
+/* As vokra_hip_decoder_reorder and _reorder_dev, for the text decoder's streams. */
+int vokra_hip_text_decoder_reorder(vokra_hip_ctx_t *ctx, vokra_hip_text_decoder_t *dec, size_t groups, size_t beams,
+                                   const int32_t *streams, const int32_t *parents);
+int vokra_hip_text_decoder_reorder_dev(vokra_hip_ctx_t *ctx, vokra_hip_text_decoder_t *dec, size_t groups, size_t beams,
+                                       const int32_t *d_streams, const int32_t *d_parents, const int32_t *d_lens,
+                                       size_t max_len);
 int vokra_hip_text_decoder_status(vokra_hip_ctx_t *ctx, vokra_hip_text_decoder_t *dec, size_t *n_appended);
 
 /* VoxtralConfig (crates/vokra-models/src/voxtral/config.rs:60-147), the

@@ -584,6 +584,53 @@ int run_paged_attn(vokra_hip_ctx* c, vokra_hip_kv* kv, size_t layer, size_t n, c
     return VOKRA_HIP_OK;
 }
 
+int check_reorder(const vokra_hip_kv* kv, const char* what, size_t groups, size_t beams) {
+    if (beams == 0 || beams > (size_t)vk::kKvBeams)
+        return fail(VOKRA_HIP_ERROR_INVALID_ARGUMENT, "%s: beams must be in 1..%d, got %zu", what, vk::kKvBeams, beams);
+    if (groups > kv->n_stream / beams)  // streams are distinct
+        return fail(VOKRA_HIP_ERROR_INVALID_ARGUMENT, "%s: %zu groups of %zu beams in a cache of %zu streams", what, groups,
+                    beams, kv->n_stream);
+    if (kv->width * kv->bs > ((size_t)1 << 30))
+        return fail(VOKRA_HIP_ERROR_INVALID_ARGUMENT, "%s: pages of more than 2^30 values a stream", what);
+    return VOKRA_HIP_OK;
+}
+
+// The host-array form: every item checked, then one launch.
+int kv_reorder_host(vokra_hip_ctx* c, vokra_hip_kv* kv, const char* what, size_t groups, size_t beams,
+                    const int32_t* streams, const int32_t* parents, const int32_t* lens) {
+    int st = check_reorder(kv, what, groups, beams);
+    if (st) return st;
+    if (groups == 0) return VOKRA_HIP_OK;
+    if (!streams || !parents || !lens) return fail(VOKRA_HIP_ERROR_INVALID_ARGUMENT, "%s: NULL buffer", what);
+    const size_t n = groups * beams;
+    std::vector<char> seen(kv->n_stream, 0);
+    int32_t most = 0;
+    for (size_t i = 0; i < n; ++i) {
+        if (streams[i] < 0 || (size_t)streams[i] >= kv->n_stream || seen[streams[i]])
+            return fail(VOKRA_HIP_ERROR_INVALID_ARGUMENT, "%s: streams must be distinct and < %zu", what, kv->n_stream);
+        seen[streams[i]] = 1;
+        if (parents[i] < -1 || parents[i] >= (int32_t)beams)
+            return fail(VOKRA_HIP_ERROR_INVALID_ARGUMENT, "%s: parent %d of item %zu is no beam of %zu", what, parents[i], i,
+                        beams);
+    }
+    for (size_t g = 0; g < groups; ++g) {
+        if (lens[g] < 0 || (size_t)lens[g] > kv->max_time)
+            return fail(VOKRA_HIP_ERROR_INVALID_ARGUMENT, "%s: length %d of group %zu is not in 0..%zu", what, lens[g], g,
+                        kv->max_time);
+        most = std::max(most, lens[g]);
+    }
+    VK_TRY(set_dev(c), "hipSetDevice");
+    VK_TRY(kv->items.ensure((2 * n + groups) * sizeof(int)), "hipMalloc");
+    int* d = (int*)kv->items.p;
+    VK_TRY(hipMemcpyAsync(d, streams, n * sizeof(int), hipMemcpyHostToDevice, c->stream), "hipMemcpyAsync");
+    VK_TRY(hipMemcpyAsync(d + n, parents, n * sizeof(int), hipMemcpyHostToDevice, c->stream), "hipMemcpyAsync");
+    VK_TRY(hipMemcpyAsync(d + 2 * n, lens, groups * sizeof(int), hipMemcpyHostToDevice, c->stream), "hipMemcpyAsync");
+    VK_TRY(vk::launch_kv_reorder(c->stream, kv->view(), (int)groups, (int)beams, d, d + n, d + 2 * n, most),
+           "launch(vk_kv_reorder)");
+    VK_TRY(hipStreamSynchronize(c->stream), "hipStreamSynchronize");
+    return VOKRA_HIP_OK;
+}
+
 int check_paged_attn(const vokra_hip_kv* kv, size_t layer, size_t n, size_t hq) {
     if (layer >= kv->n_layer)
         return fail(VOKRA_HIP_ERROR_INVALID_ARGUMENT, "layer %zu >= n_layer %zu", layer, kv->n_layer);
@@ -620,6 +667,23 @@ static int clean_part(vokra_hip_ctx* c, DevBuf& b, size_t bytes, hipError_t (*cl
 }
 int ctx_bkv_part(vokra_hip_ctx* c, void** p) {
     return clean_part(c, c->bk_part, kBkvPartBytes, launch_bkv_part_clear, p);
+}
+int kv_reorder_at(vokra_hip_ctx* c, vokra_hip_kv* kv, const char* what, size_t groups, size_t beams,
+                  const int32_t* streams, const int32_t* parents, int32_t* pos) {
+    int st = check_reorder(kv, what, groups, beams);
+    if (st) return st;
+    if (groups && (!streams || !parents)) return fail(VOKRA_HIP_ERROR_INVALID_ARGUMENT, "%s: NULL buffer", what);
+    // a group's length: its longest beam's (rows behind a shorter one's position are never read)
+    std::vector<int32_t> lens(groups, 0), to(groups * beams);
+    for (size_t i = 0; i < groups * beams; ++i)
+        if (streams[i] >= 0 && (size_t)streams[i] < kv->n_stream)
+            lens[i / beams] = std::max(lens[i / beams], pos[streams[i]]);
+    st = kv_reorder_host(c, kv, what, groups, beams, streams, parents, lens.data());
+    if (st) return st;
+    for (size_t i = 0; i < groups * beams; ++i)
+        to[i] = pos[streams[parents[i] < 0 ? i : i / beams * beams + (size_t)parents[i]]];
+    for (size_t i = 0; i < groups * beams; ++i) pos[streams[i]] = to[i];
+    return VOKRA_HIP_OK;
 }
 int ctx_rules_part(vokra_hip_ctx* c, void** p) {
     return clean_part(c, c->ru_part, kRulesPartBytes, launch_rules_clear, p);
@@ -1193,6 +1257,29 @@ int vokra_hip_kv_append(vokra_hip_ctx_t* c, vokra_hip_kv_t* kv, size_t layer, si
                                 (const float*)((char*)d_rows + rb)),
            "launch(vk_kv_append)");
     return kv_append_status(kv, n, streams, times, nullptr);
+}
+
+int vokra_hip_kv_reorder_dev(vokra_hip_ctx_t* c, vokra_hip_kv_t* kv, size_t groups, size_t beams,
+                             const int32_t* d_streams, const int32_t* d_parents, const int32_t* d_lens,
+                             size_t max_len) {
+    if (!c || !kv || kv->ctx != c) return fail(VOKRA_HIP_ERROR_INVALID_ARGUMENT, "kv_reorder: bad context or cache");
+    int st = check_reorder(kv, "kv_reorder", groups, beams);
+    if (st) return st;
+    if (max_len > kv->max_time)
+        return fail(VOKRA_HIP_ERROR_INVALID_ARGUMENT, "kv_reorder: max_len %zu > max_time %zu", max_len, kv->max_time);
+    if (groups == 0) return VOKRA_HIP_OK;
+    if (!d_streams || !d_parents || !d_lens) return fail(VOKRA_HIP_ERROR_INVALID_ARGUMENT, "kv_reorder: NULL buffer");
+    VK_TRY(set_dev(c), "hipSetDevice");
+    VK_TRY(vk::launch_kv_reorder(c->stream, kv->view(), (int)groups, (int)beams, d_streams, d_parents, d_lens,
+                                 (int)max_len),
+           "launch(vk_kv_reorder)");
+    return VOKRA_HIP_OK;
+}
+
+int vokra_hip_kv_reorder(vokra_hip_ctx_t* c, vokra_hip_kv_t* kv, size_t groups, size_t beams, const int32_t* streams,
+                         const int32_t* parents, const int32_t* lens) {
+    if (!c || !kv || kv->ctx != c) return fail(VOKRA_HIP_ERROR_INVALID_ARGUMENT, "kv_reorder: bad context or cache");
+    return kv_reorder_host(c, kv, "kv_reorder", groups, beams, streams, parents, lens);
 }
 
 int vokra_hip_kv_read(vokra_hip_ctx_t* c, vokra_hip_kv_t* kv, size_t layer, size_t t, size_t s, float* k_out,

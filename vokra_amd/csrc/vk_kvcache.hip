@@ -1570,6 +1570,79 @@ __global__ void vk_paged_attn_combine(int n_split, int hq, const int* __restrict
 
 namespace vk {
 
+// ---------------------------------------------------------------------------
+// Reordering after a beam search's selection: in group g the stream of beam b takes
+// rows 0 .. lens[g] - 1 of the stream of beam parents[b], in every layer, as all of
+// them were before. A page holds its bs time steps of every stream, one stream's quants
+// and scales in one run each, so no page changes hands: the runs' bytes move.
+// A thread holds one place of the runs, 16 bytes of quants or 4 of scales, for all of
+// the group's beams that change: it reads all sources before it writes any, and no
+// other thread touches that place, so permutations and repeats need no second copy.
+// Beams that keep their rows, or name no beam, cost nothing. Bound by memory: each
+// source once (a stream that several beams take comes from cache), each changed
+// stream once.
+// NB: at least the beams of a group.
+template <int NB>
+__global__ __launch_bounds__(256) void vk_kv_reorder(KvDev c, int beams, const int* __restrict__ streams,
+                                                     const int* __restrict__ parents, const int* __restrict__ lens,
+                                                     int max_len, int chunks, int layer0, int block0) {
+    __shared__ int s_src[NB], s_dst[NB], s_n;
+    const int g = blockIdx.z, layer = layer0 + (int)blockIdx.y, bx = blockIdx.x / chunks;
+    const int block = block0 + bx, chunk = blockIdx.x - bx * chunks;
+    const int len = lens[g], pid = c.table[layer * c.ppl + block];
+    const int rows = min(len - block * c.bs, c.bs);
+    if (len > max_len || rows <= 0 || (unsigned)pid >= (unsigned)c.cap) return;
+    if (threadIdx.x < 64) {
+        const int b = threadIdx.x;
+        const int p = b < beams ? parents[(size_t)g * beams + b] : -1;
+        const bool named = b < beams && (unsigned)p < (unsigned)beams && p != b;
+        const int dst = named ? streams[(size_t)g * beams + b] : -1;
+        const int src = named ? streams[(size_t)g * beams + p] : -1;
+        const bool moves = (unsigned)dst < (unsigned)c.n_stream && (unsigned)src < (unsigned)c.n_stream;
+        const uint64_t m = __ballot(moves);
+        if (moves) {
+            const int at = __popcll(m & ((1ull << b) - 1));
+            s_src[at] = src;
+            s_dst[at] = dst;
+        }
+        if (b == 0) s_n = __popcll(m);
+    }
+    __syncthreads();
+    const int n = s_n;
+    if (n == 0) return;
+    const int run = c.nh * c.bs * c.hd, q16 = run >> 4;          // quants of a stream in a page, 16-byte pieces
+    const int drun = c.nh * c.bs * c.hb, d4 = drun >> 1;         // its scales, 4-byte pieces
+    const size_t page = (size_t)pid * c.n_stream;
+    int i = chunk * 256 + (int)threadIdx.x;
+    if (i < 2 * q16) {
+        const bool v_side = i >= q16;
+        if (v_side) i -= q16;
+        if ((i * 16 / c.hd) % c.bs >= rows) return;  // a row behind the sequence
+        int8_t* base = (v_side ? c.vq : c.kq) + page * run + (size_t)i * 16;
+        uint4 x[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            if (j < n) x[j] = *(const uint4*)(base + (size_t)s_src[j] * run);
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            if (j < n) *(uint4*)(base + (size_t)s_dst[j] * run) = x[j];
+    } else {
+        i -= 2 * q16;
+        if (i >= 2 * d4) return;
+        const bool v_side = i >= d4;
+        if (v_side) i -= d4;
+        if ((i * 2 / c.hb) % c.bs >= rows) return;
+        uint16_t* base = (v_side ? c.vd : c.kd) + page * drun + (size_t)i * 2;
+        uint32_t x[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            if (j < n) x[j] = *(const uint32_t*)(base + (size_t)s_src[j] * drun);
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            if (j < n) *(uint32_t*)(base + (size_t)s_dst[j] * drun) = x[j];
+    }
+}
+
 static KvDev kv_view(const KvView& v) {
     KvDev c;
     c.kq = (int8_t*)v.kq;
@@ -1641,6 +1714,35 @@ hipError_t launch_kv_alloc_layers(hipStream_t s, const KvView& v, int layer0, in
 hipError_t launch_kv_read(hipStream_t s, const KvView& v, int layer, int t, int st, float* out, int* found) {
     hipLaunchKernelGGL(vk_kv_read, dim3((unsigned)((v.width + 255) / 256)), dim3(256), 0, s, kv_view(v), layer, t, st,
                        out, found);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_reorder(hipStream_t s, const KvView& v, int groups, int beams, const int* streams,
+                             const int* parents, const int* lens, int max_len) {
+    const KvDev c = kv_view(v);
+    const int blocks = (std::min(max_len, c.max_time) + c.bs - 1) / c.bs;
+    if (groups == 0 || blocks == 0) return hipSuccess;
+    const size_t run = (size_t)c.nh * c.bs * c.hd;
+    const int chunks = (int)((2 * (run / 16) + 2 * ((size_t)c.nh * c.bs * c.hb / 2) + 255) / 256);
+    // a grid holds fewer than 2^32 threads: parts of the blocks, layers and groups
+    constexpr size_t kMost = 1 << 23;
+    const int nb = (int)std::min<size_t>(blocks, std::max<size_t>(1, kMost / chunks));
+    const int nl = (int)std::min<size_t>(c.n_layer, std::max<size_t>(1, kMost / ((size_t)nb * chunks)));
+    const int ng = (int)std::min<size_t>(groups, std::max<size_t>(1, kMost / ((size_t)nb * chunks * nl)));
+    for (int g = 0; g < groups; g += ng)
+        for (int l = 0; l < c.n_layer; l += nl)
+            for (int b = 0; b < blocks; b += nb) {
+                const dim3 grid((unsigned)(std::min(nb, blocks - b) * chunks), (unsigned)std::min(nl, c.n_layer - l),
+                                (unsigned)std::min(ng, groups - g));
+                auto go = [&](auto kernel) {
+                    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, c, beams, streams + (size_t)g * beams,
+                                       parents + (size_t)g * beams, lens + g, max_len, chunks, l, b);
+                };
+                if (beams <= 4) go(vk_kv_reorder<4>);
+                else if (beams <= 8) go(vk_kv_reorder<8>);
+                else if (beams <= 16) go(vk_kv_reorder<16>);
+                else go(vk_kv_reorder<32>);
+            }
     return hipGetLastError();
 }
 

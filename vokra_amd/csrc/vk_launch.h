@@ -243,6 +243,10 @@ struct KvView {
 hipError_t launch_kv_append(hipStream_t s, const KvView& v, int layer, int n, const int* streams, const int* times,
                             const float* k, const float* vv);
 hipError_t launch_kv_read(hipStream_t s, const KvView& v, int layer, int t, int st, float* out, int* found);
+// Streams of groups of beams (at most kKvBeams each) take their parents' rows, every layer.
+constexpr int kKvBeams = 32;
+hipError_t launch_kv_reorder(hipStream_t s, const KvView& v, int groups, int beams, const int* streams,
+                             const int* parents, const int* lens, int max_len);
 hipError_t launch_kv_release(hipStream_t s, const KvView& v, int layer);
 hipError_t launch_kv_reset(hipStream_t s, const KvView& v, const int* order, size_t pool_bytes, size_t scale_bytes);
 hipError_t launch_kv_page_of(hipStream_t s, const KvView& v, int layer, int t, int* out);
@@ -332,6 +336,10 @@ struct vokra_hip_kv;
 namespace vk {
 hipStream_t ctx_stream(const vokra_hip_ctx* c);
 int ctx_device(const vokra_hip_ctx* c);
+// The host form of the paged cache's reordering for a session, whose streams' positions are pos
+// (n_stream of them): checks, moves the rows and the positions.
+int kv_reorder_at(vokra_hip_ctx* c, vokra_hip_kv* kv, const char* what, size_t groups, size_t beams,
+                  const int32_t* streams, const int32_t* parents, int32_t* pos);
 // The context's workspace of the logits rules: allocated at the first call, never replaced.
 int ctx_rules_part(vokra_hip_ctx* c, void** p);
 // The same for the partial results of the block caches' attention (first cache).

@@ -708,6 +708,19 @@ int vokra_hip_decoder_kv_pages(vokra_hip_ctx_t* c, vokra_hip_decoder_t* m, size_
     return vokra_hip_kv_pages(c, m->kv, free_pages, pages_in_use);
 }
 
+int vokra_hip_decoder_reorder(vokra_hip_ctx_t* c, vokra_hip_decoder_t* m, size_t groups, size_t beams,
+                              const int32_t* streams, const int32_t* parents) {
+    if (!c || !m || m->ctx != c) return vk::ctx_fail(VOKRA_HIP_ERROR_INVALID_ARGUMENT, "decoder_reorder: bad context");
+    return vk::kv_reorder_at(c, m->kv, "decoder_reorder", groups, beams, streams, parents, m->length.data());
+}
+
+int vokra_hip_decoder_reorder_dev(vokra_hip_ctx_t* c, vokra_hip_decoder_t* m, size_t groups, size_t beams,
+                                  const int32_t* d_streams, const int32_t* d_parents, const int32_t* d_lens,
+                                  size_t max_len) {
+    if (!c || !m || m->ctx != c) return vk::ctx_fail(VOKRA_HIP_ERROR_INVALID_ARGUMENT, "decoder_reorder: bad context");
+    return vokra_hip_kv_reorder_dev(c, m->kv, groups, beams, d_streams, d_parents, d_lens, max_len);
+}
+
 int vokra_hip_decoder_status(vokra_hip_ctx_t* c, vokra_hip_decoder_t* m, size_t* n_appended) {
     if (!c || !m || m->ctx != c) return vk::ctx_fail(VOKRA_HIP_ERROR_INVALID_ARGUMENT, "decoder_status: bad argument");
     size_t a = 0;
@@ -1143,6 +1156,19 @@ int vokra_hip_text_decoder_step(vokra_hip_ctx_t* c, vokra_hip_text_decoder_t* m,
     SS_TRY(vokra_hip_memcpy_dtoh(c, next_tokens, m->next.p, n * 4));
     if (logits) SS_TRY(vokra_hip_memcpy_dtoh(c, logits, m->logits.p, n * m->vocab * sizeof(float)));
     return vk::range_check(c);
+}
+
+int vokra_hip_text_decoder_reorder(vokra_hip_ctx_t* c, vokra_hip_text_decoder_t* m, size_t groups, size_t beams,
+                              const int32_t* streams, const int32_t* parents) {
+    if (!c || !m || m->ctx != c) return vk::ctx_fail(VOKRA_HIP_ERROR_INVALID_ARGUMENT, "text_decoder_reorder: bad context");
+    return vk::kv_reorder_at(c, m->kv, "text_decoder_reorder", groups, beams, streams, parents, m->position.data());
+}
+
+int vokra_hip_text_decoder_reorder_dev(vokra_hip_ctx_t* c, vokra_hip_text_decoder_t* m, size_t groups, size_t beams,
+                                  const int32_t* d_streams, const int32_t* d_parents, const int32_t* d_lens,
+                                  size_t max_len) {
+    if (!c || !m || m->ctx != c) return vk::ctx_fail(VOKRA_HIP_ERROR_INVALID_ARGUMENT, "text_decoder_reorder: bad context");
+    return vokra_hip_kv_reorder_dev(c, m->kv, groups, beams, d_streams, d_parents, d_lens, max_len);
 }
 
 int vokra_hip_text_decoder_status(vokra_hip_ctx_t* c, vokra_hip_text_decoder_t* m, size_t* n_appended) {

@@ -259,6 +259,11 @@ def _declare(L):
     L.vokra_hip_kv_set_free_order.argtypes = [P, P, i32p, sz]
     L.vokra_hip_paged_attn.argtypes = [P, P, sz, sz, i32p, i32p, sz, f32p, C.c_float, f32p]
     L.vokra_hip_paged_attn_dev.argtypes = [P, P, sz, sz, P, P, sz, sz, P, C.c_float, P]
+    L.vokra_hip_kv_reorder.argtypes = [P, P, sz, sz, i32p, i32p, i32p]
+    for name in ("kv", "decoder", "text_decoder"):
+        getattr(L, f"vokra_hip_{name}_reorder_dev").argtypes = [P, P, sz, sz, P, P, P, sz]
+    for name in ("decoder", "text_decoder"):
+        getattr(L, f"vokra_hip_{name}_reorder").argtypes = [P, P, sz, sz, i32p, i32p]
     L.vokra_hip_bkv_create.argtypes = [P, sz, sz, sz, sz, sz, sz, sz, sz, C.c_int, C.POINTER(P)]
     L.vokra_hip_bkv_destroy.argtypes = [P]
     L.vokra_hip_bkv_destroy.restype = None
@@ -657,6 +662,14 @@ class QAct:
             pass
 
 
+def _beam_ids(streams, parents):
+    """(groups, beams, streams, parents) of arrays [groups, beams]."""
+    st, pa = (np.ascontiguousarray(a, np.int32) for a in (streams, parents))
+    if st.ndim != 2 or st.shape != pa.shape:
+        raise InvalidArgument(f"reorder: streams {st.shape} and parents {pa.shape} are not both [groups, beams]")
+    return (*st.shape, st, pa)
+
+
 class KvCache:
     """QuantizedPagedKvCache (paged_quant.rs:240-545) resident on the device."""
 
@@ -695,6 +708,20 @@ class KvCache:
         _check(lib().vokra_hip_kv_read(self._ctx._h, self._h, layer, t, s, _ptr(k, C.c_float),
                                        _ptr(v, C.c_float), C.byref(f)))
         return (k, v) if f.value else None
+
+    def reorder(self, streams, parents, lens):
+        """Stream streams[g, b] takes the first lens[g] rows of streams[g, parents[g, b]]
+        (-1: keeps its own), every layer, all as they were before."""
+        groups, beams, st, pa = _beam_ids(streams, parents)
+        ln = np.ascontiguousarray(lens, np.int32).reshape(-1)
+        if ln.size != groups:
+            raise InvalidArgument(f"reorder: {ln.size} lengths for {groups} groups")
+        _check(lib().vokra_hip_kv_reorder(self._ctx._h, self._h, groups, beams, _ptr(st, C.c_int32),
+                                          _ptr(pa, C.c_int32), _ptr(ln, C.c_int32)))
+
+    def reorder_dev(self, groups, beams, d_streams, d_parents, d_lens, max_len):
+        _check(lib().vokra_hip_kv_reorder_dev(self._ctx._h, self._h, groups, beams, d_streams.ptr, d_parents.ptr,
+                                              d_lens.ptr, max_len))
 
     def reset(self):
         _check(lib().vokra_hip_kv_reset(self._ctx._h, self._h))
@@ -1119,6 +1146,16 @@ class Decoder:
                                                 d_positions.ptr, d_next.ptr,
                                                 None if d_logits is None else d_logits.ptr))
 
+    def reorder(self, streams, parents):
+        """Stream streams[g, b] goes on from what streams[g, parents[g, b]] has read (-1: from its own)."""
+        groups, beams, st, pa = _beam_ids(streams, parents)
+        _check(lib().vokra_hip_decoder_reorder(self._ctx._h, self._h, groups, beams, _ptr(st, C.c_int32),
+                                             _ptr(pa, C.c_int32)))
+
+    def reorder_dev(self, groups, beams, d_streams, d_parents, d_lens, max_len):
+        _check(lib().vokra_hip_decoder_reorder_dev(self._ctx._h, self._h, groups, beams, d_streams.ptr, d_parents.ptr,
+                                                 d_lens.ptr, max_len))
+
     def status(self) -> int:
         """Synchronizes; raises for a failed page allocation of the last
         step, returns the (layer, item) appends done."""
@@ -1213,6 +1250,16 @@ class TextDecoder:
         _check(lib().vokra_hip_text_decoder_step_dev(self._ctx._h, self._h, n, d_streams.ptr, d_tokens.ptr,
                                                      d_positions.ptr, d_next.ptr,
                                                      None if d_logits is None else d_logits.ptr))
+
+    def reorder(self, streams, parents):
+        """Stream streams[g, b] goes on from what streams[g, parents[g, b]] has read (-1: from its own)."""
+        groups, beams, st, pa = _beam_ids(streams, parents)
+        _check(lib().vokra_hip_text_decoder_reorder(self._ctx._h, self._h, groups, beams, _ptr(st, C.c_int32),
+                                             _ptr(pa, C.c_int32)))
+
+    def reorder_dev(self, groups, beams, d_streams, d_parents, d_lens, max_len):
+        _check(lib().vokra_hip_text_decoder_reorder_dev(self._ctx._h, self._h, groups, beams, d_streams.ptr, d_parents.ptr,
+                                                 d_lens.ptr, max_len))
 
     def status(self) -> int:
         n = C.c_size_t(0)
