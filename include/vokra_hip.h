@@ -674,6 +674,41 @@ int vokra_hip_logits_rules_dev(vokra_hip_ctx_t *ctx, size_t rows, size_t vocab, 
 int vokra_hip_logits_rules(vokra_hip_ctx_t *ctx, size_t rows, size_t vocab, const float *logits,
                            const vokra_hip_logits_rules_t *rules, float *out, int32_t *next);
 
+/* Beam search's selection over beams and vocabulary. No counterpart in the
+ * reference (it decodes greedily). Row g * beams + b of logits is beam b of group g:
+ *   a live beam goes on with token v at score + (x_v - ln sum_w exp(x_w));
+ *   an ended beam (ended != 0; NULL: none) with end_token alone, at its own score;
+ *   a beam whose score is -inf or NaN has no continuation (on a first step all beams
+ *   but one), nor has a token at -inf or NaN (which counts as -inf in the sum),
+ *   nor a row that holds +inf.
+ * A group's n_out best go out, the largest first: out_scores, out_parents (beam in the
+ * group), out_tokens and out_ended (0 or 1: the parent had ended, or the token is
+ * end_token), all [groups][n_out]. Totals are formed and compared in 64 bits (the
+ * exponentials in f32); of equal ones the lower beam stands first, in a beam the
+ * larger logit, then the lower token. Where there are fewer than n_out: score -inf,
+ * parent and token -1, ended 1. With n_out = beams the outputs are the next step's
+ * scores and ended, and parents what vokra_hip_kv_reorder takes.
+ * A plan holds the workspace of calls of up to max_groups groups, max_beams <= 32 beams
+ * (max_groups * max_beams <= 65535), max_vocab <= 2^24 tokens and max_out <= 64
+ * continuations; calls on one plan run in the order in which they are made. */
+typedef struct vokra_hip_beam vokra_hip_beam_t;
+int vokra_hip_beam_create(vokra_hip_ctx_t *ctx, size_t max_groups, size_t max_beams, size_t max_vocab, size_t max_out,
+                          vokra_hip_beam_t **out);
+void vokra_hip_beam_destroy(vokra_hip_beam_t *beam);
+/* Device pointers, asynchronous, nothing is allocated; rows of logits `stride` floats
+ * apart. end_token -1: none (ended is then NULL). out_ended may be NULL. Outputs
+ * overlap nothing, except that with n_out = beams out_scores may be scores and
+ * out_ended may be ended. */
+int vokra_hip_beam_select_dev(vokra_hip_ctx_t *ctx, vokra_hip_beam_t *beam, size_t groups, size_t beams, size_t vocab,
+                              size_t n_out, size_t stride, const float *d_logits, const float *d_scores,
+                              const int32_t *d_ended, int32_t end_token, float *d_out_scores, int32_t *d_out_parents,
+                              int32_t *d_out_tokens, int32_t *d_out_ended);
+/* Host arrays (rows side by side), synchronous. */
+int vokra_hip_beam_select(vokra_hip_ctx_t *ctx, vokra_hip_beam_t *beam, size_t groups, size_t beams, size_t vocab,
+                          size_t n_out, const float *logits, const float *scores, const int32_t *ended,
+                          int32_t end_token, float *out_scores, int32_t *out_parents, int32_t *out_tokens,
+                          int32_t *out_ended);
+
 /* out = a + b on device (residual connections; add_assign in the reference's
  * model code, crates/vokra-models/src/whisper/nn.rs). */
 int vokra_hip_add_f32_dev(vokra_hip_ctx_t *ctx, const float *d_a, const float *d_b, float *d_out, size_t n);

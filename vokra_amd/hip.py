@@ -294,6 +294,11 @@ def _declare(L):
     L.vokra_hip_rope_apply.argtypes = [P, P, sz, i32p, sz, f32p, f32p, sz, f32p, f32p]
     L.vokra_hip_rope_norm_apply_dev.argtypes = [P, P, C.POINTER(_HeadNorm), sz, P, sz, P, sz, P, sz, sz, P, sz, P, sz]
     L.vokra_hip_rope_norm_apply.argtypes = [P, P, C.POINTER(_HeadNorm), sz, i32p, sz, f32p, f32p, sz, f32p, f32p]
+    L.vokra_hip_beam_create.argtypes = [P, sz, sz, sz, sz, C.POINTER(P)]
+    L.vokra_hip_beam_destroy.argtypes = [P]
+    L.vokra_hip_beam_destroy.restype = None
+    L.vokra_hip_beam_select_dev.argtypes = [P, P, sz, sz, sz, sz, sz, P, P, P, C.c_int32, P, P, P, P]
+    L.vokra_hip_beam_select.argtypes = [P, P, sz, sz, sz, sz, f32p, f32p, i32p, C.c_int32, f32p, i32p, i32p, i32p]
     L.vokra_hip_logits_rules_dev.argtypes = [P, sz, sz, sz, P, C.POINTER(_LogitsRules), P, P]
     L.vokra_hip_logits_rules.argtypes = [P, sz, sz, f32p, C.POINTER(_LogitsRules), f32p, i32p]
     L.vokra_hip_gemm_f32.argtypes = [P, sz, sz, sz, f32p, sz, f32p, sz, f32p, f32p, sz]
@@ -995,6 +1000,49 @@ class RopePlan:
             pass
 
 
+class BeamSelect:
+    """Beam search's selection (vokra_hip_beam_*): the best continuations of every
+    group's beams, for calls of up to the sizes it is made for."""
+
+    def __init__(self, ctx: "HipContext", max_groups, max_beams, max_vocab, max_out):
+        self._ctx = ctx
+        h = C.c_void_p()
+        _check(lib().vokra_hip_beam_create(ctx._h, max_groups, max_beams, max_vocab, max_out, C.byref(h)))
+        self._h = h
+
+    def select_dev(self, groups, beams, vocab, n_out, d_logits, d_scores, d_out_scores, d_out_parents, d_out_tokens,
+                   d_ended=None, end_token=-1, d_out_ended=None, stride=None):
+        """Rows group * beams + beam of logits, `stride` floats apart; outputs [groups, n_out]."""
+        _check(lib().vokra_hip_beam_select_dev(
+            self._ctx._h, self._h, groups, beams, vocab, n_out, vocab if stride is None else stride, d_logits.ptr,
+            d_scores.ptr, None if d_ended is None else d_ended.ptr, end_token, d_out_scores.ptr, d_out_parents.ptr,
+            d_out_tokens.ptr, None if d_out_ended is None else d_out_ended.ptr))
+
+    def select(self, logits, scores, n_out, ended=None, end_token=-1):
+        """Host form: logits [groups, beams, vocab], scores and ended [groups, beams].
+        Returns (scores, parents, tokens, ended), each [groups, n_out]."""
+        x, sc = _f32(logits), _f32(scores)
+        if x.ndim != 3 or sc.shape != x.shape[:2]:
+            raise InvalidArgument(f"beam select: logits {x.shape} and scores {sc.shape}")
+        en = None if ended is None else np.ascontiguousarray(ended, np.int32)
+        if en is not None and en.shape != sc.shape:
+            raise InvalidArgument(f"beam select: ended {en.shape} for scores {sc.shape}")
+        g, b, v = x.shape
+        out = [np.empty((g, max(n_out, 0)), t) for t in (np.float32, np.int32, np.int32, np.int32)]
+        _check(lib().vokra_hip_beam_select(self._ctx._h, self._h, g, b, v, n_out, _ptr(x, C.c_float),
+                                           _ptr(sc, C.c_float), _ptr(en, C.c_int32), end_token, _ptr(out[0], C.c_float),
+                                           *(_ptr(o, C.c_int32) for o in out[1:])))
+        return tuple(out)
+
+    def __del__(self):
+        try:
+            if getattr(self, "_h", None) and self._h.value and _ctx_alive(self):
+                lib().vokra_hip_beam_destroy(self._h)
+                self._h = C.c_void_p()
+        except Exception:
+            pass
+
+
 class LogitsRules:
     """vokra_hip_logits_rules_t over device buffers, which it keeps."""
 
@@ -1598,6 +1646,9 @@ class HipContext:
     def rope_plan(self, head_dim, rot_dim, layout=RopeLayout.HALF, base=10000.0, scaling=RopeScaling.NONE, factor=1.0,
                   orig_ctx=0, **more) -> RopePlan:
         return RopePlan(self, head_dim, rot_dim, layout, base, scaling, factor, orig_ctx, **more)
+
+    def beam_select(self, max_groups, max_beams, max_vocab, max_out) -> BeamSelect:
+        return BeamSelect(self, max_groups, max_beams, max_vocab, max_out)
 
     # ---- attention ----------------------------------------------------------
     def attn_f32(self, q, k, v, n_head_q: int, n_head_kv: int = None, scale: float = None,
