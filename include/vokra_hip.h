@@ -339,6 +339,48 @@ int vokra_hip_attn_f32_dev(vokra_hip_ctx_t *ctx, size_t batch, size_t t_q, size_
                            size_t n_head_kv, size_t head_dim, const float *d_q, const float *d_k,
                            const float *d_v, float scale, int causal, size_t q_offset, float *d_out);
 
+/* The same over sequences of different lengths, packed one after another (prompts as
+ * a decoder takes them in, utterances against themselves or against the rows of
+ * candidates). The reference attends one sequence at a time
+ * (crates/vokra-models/src/whisper/nn.rs:209-325, voxtral/text_decoder.rs:1302-1360).
+ * Sequence s has query rows q_offsets[s] .. q_offsets[s + 1] - 1 and key rows by
+ * k_offsets likewise (NULL: the queries'). Of n query rows and m keys, row i stands at
+ * position p = m - n + i (the last row at the last key) and sees every key, or (causal)
+ * the keys j <= p, or with a window > 0 those with p - window < j <= p:
+ *   out = softmax((q * scale) . K^T) . V over the keys that it sees, zeros where it
+ * sees none. Query head h reads kv head h / (n_head_q / n_head_kv). f32 in and out: each
+ * product runs as three fp16 products of two parts of both operands (22 bits), each
+ * operand under a power of two (a query row's, a tile of 64 keys' for a kv head), so
+ * results do not depend on the values' size; sums in f32. How a row's keys are split
+ * depends on the whole call, and its last f32 bits may with it. A key row or query
+ * row with a value that is not finite makes rows that see it NaN; a value of V that is
+ * not finite makes its column of those rows not finite; rows that do not see it are not
+ * touched by it.
+ * A plan holds the workspace of calls of up to max_seq (<= 1024) sequences of up to
+ * max_q_rows and max_k_rows (<= 2^20) rows in all: (max_k_rows + 64 max_seq) * n_head_kv *
+ * 8 * head_dim bytes and 2 * 512 * 512 * (head_dim + 4) for partial results.
+ * head_dim 64 or 128 (else UNSUPPORTED_OP); calls on one plan run in the order in which
+ * they are made. */
+typedef struct vokra_hip_pattn vokra_hip_packed_attn_t;
+int vokra_hip_packed_attn_create(vokra_hip_ctx_t *ctx, size_t max_seq, size_t max_q_rows, size_t max_k_rows,
+                                 size_t n_head_q, size_t n_head_kv, size_t head_dim, vokra_hip_packed_attn_t **out);
+void vokra_hip_packed_attn_destroy(vokra_hip_packed_attn_t *attn);
+/* Device pointers, asynchronous, nothing is allocated. n_q_rows and n_k_rows bound the
+ * offsets, max_q and max_k the rows of any sequence. Rows lie q_stride (and so on)
+ * floats apart, so q, k and v may be parts of one projection's rows; all are 16-byte
+ * aligned, out overlaps none. The first sequence whose offsets are out of order, range
+ * or bounds, and those behind it, are passed over: their rows of out stay as they are, as
+ * do rows that no sequence has. */
+int vokra_hip_packed_attn_dev(vokra_hip_ctx_t *ctx, vokra_hip_packed_attn_t *attn, size_t n_seq, size_t n_q_rows,
+                              size_t n_k_rows, size_t max_q, size_t max_k, const int32_t *d_q_offsets,
+                              const int32_t *d_k_offsets, const float *d_q, size_t q_stride, const float *d_k,
+                              size_t k_stride, const float *d_v, size_t v_stride, float scale, int causal,
+                              size_t window, float *d_out, size_t out_stride);
+/* Host arrays (rows side by side), synchronous; offsets out of order are INVALID_ARGUMENT. */
+int vokra_hip_packed_attn(vokra_hip_ctx_t *ctx, vokra_hip_packed_attn_t *attn, size_t n_seq, const int32_t *q_offsets,
+                          const int32_t *k_offsets, const float *q, const float *k, const float *v, float scale,
+                          int causal, size_t window, float *out);
+
 /* ---- paged quantized KV cache in HBM ------------------------------------- */
 
 /* QuantizedPagedKvCache (crates/vokra-core/src/cache/paged_quant.rs:240-545)

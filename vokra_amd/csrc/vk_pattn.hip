@@ -1,0 +1,667 @@
+// vk_pattn.hip — attention over packed sequences of different lengths.
+//
+// Sequence s has n_s query rows and m_s keys, rows of q, k, v from q_off[s], k_off[s]
+// on. Row i of it stands at position p = m_s - n_s + i; query head h reads kv head
+// h / G, G = hq / hkv:
+//   s_j = scale q . k_j, out = sum_j exp(s_j - max) v_j / sum_j exp(s_j - max)
+// over the keys j that the row sees: all, or j <= p (causal), or p - window < j <= p. A row
+// that sees none gives zeros.
+//
+// Work: the n_s G query rows of a (sequence, kv head), row R being query R / G of head
+// hk G + R % G, in tiles of 128 (32 a wave), against tiles of 64 keys.
+//
+// Packing (vk_pattn_pack): every K and V value as two fp16 parts, hi + lo, of the value
+// times a power of two that puts its tile's largest at 2^13, in the order in which the
+// matrix instructions take their operands: a tile is 64 KB (hd 128) that goes to LDS
+// and registers without a shuffle. Three products for one of f32 then hold 22 bits
+// whatever the values' size: hi hi + hi lo + lo hi, sums in f32.
+//   S^T [keys][rows] = K q^T (q split likewise, a power of two a row);
+//   its accumulators are, without leaving the lane, the operand of
+//   O^T [d][rows] = V^T W^T, as V's tiles hold keys in the accumulators' order.
+// Weights w = 2^(14 + s - M), s in units of log2, M the running maximum of s rounded up:
+// a whole number, so what was summed is brought under a new one exactly, and seldom.
+// Where a V tile's power of two is below the largest so far the weights take the
+// difference, for the product alone.
+//
+// Even shares: the tiles' units (64 keys each, and two more for a tile's start and
+// end) lie on one line, which 512 workgroups share evenly whatever the lengths are; a
+// share holds whole tiles and at most two pieces, whose results vk_pattn_join brings
+// together.
+#include <algorithm>
+
+#include "vk_common.h"
+#include "vk_pattn.h"
+
+namespace vk {
+
+typedef _Float16 pa_h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 pa_h2 __attribute__((ext_vector_type(2)));
+typedef uint32_t pa_u4 __attribute__((ext_vector_type(4)));
+
+constexpr int kTileCost = 2;   // a tile's start and end, in units
+constexpr int kLeast = 4;      // the least share
+constexpr float kNoMax = -0x1.fffffep127f;
+
+// halves of one tile's K hi (K lo, V hi, V lo): 64 keys
+constexpr int pa_part(int hd) { return kPaKeys * hd; }
+
+// ---- sequences ---------------------------------------------------------------------
+
+// How many sequences, from the first on, have offsets in order and range; a sequence
+// from there on is passed over. All threads of the workgroup, after a barrier; scratch:
+// one int of LDS.
+__device__ __forceinline__ int pa_in_order(const PaArgs& a, int* s_first) {
+    if (threadIdx.x == 0) *s_first = a.n_seq;
+    __syncthreads();
+    for (int s = threadIdx.x; s < a.n_seq; s += (int)blockDim.x) {
+        const int q0 = a.q_off[s], q1 = a.q_off[s + 1], k0 = a.k_off[s], k1 = a.k_off[s + 1];
+        if (q0 < 0 || q1 < q0 || q1 > a.q_rows || q1 - q0 > a.max_q || k0 < 0 || k1 < k0 || k1 > a.k_rows ||
+            k1 - k0 > a.max_k)
+            atomicMin(s_first, s);
+    }
+    __syncthreads();
+    return *s_first;
+}
+
+// Places of tiles: sequence s has those from rows-before / size + s on, which never meet
+// the next one's.
+__device__ __forceinline__ int pa_q_slot(const PaArgs& a, int q0, int s) {
+    return (int)((long long)q0 * a.g / kPaRows) + s;
+}
+__device__ __forceinline__ int pa_k_slot(int k0, int s) { return k0 / kPaKeys + s; }
+
+// The keys that a tile's rows see lie in `units` tiles from `lo` on (one where there are
+// none).
+__device__ __forceinline__ void pa_span(const PaArgs& a, int n, int m, int row0, int* lo, int* units) {
+    const int last = min(row0 + kPaRows, n * a.g) - 1;
+    int k0 = 0, k1 = m;
+    if (a.causal) {
+        k1 = min(m, last / a.g + (m - n) + 1);
+        if (a.window) k0 = max(0, row0 / a.g + (m - n) - a.window + 1);
+    }
+    *lo = k1 > k0 ? k0 / kPaKeys : 0;
+    *units = k1 > k0 ? (k1 + kPaKeys - 1) / kPaKeys - *lo : 1;
+}
+
+// ---- packing -----------------------------------------------------------------------
+
+// 2^e as f32, e within -126 .. 127
+__device__ __forceinline__ float pa_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// The exponent that puts a largest magnitude a (finite) at 2^13 .. 2^14 when values are
+// multiplied by 2^-e; kPaNoValue for 0.
+__device__ __forceinline__ int pa_exponent(float a) {
+    const int b = (int)(__float_as_uint(a) >> 23);
+    return a == 0.0f ? kPaNoValue : max(b - 127, -126) - 13;
+}
+// x 2^-e for e of pa_exponent: two factors, as the power may be beyond f32's
+__device__ __forceinline__ float pa_scale(float x, int e) {
+    const int h = e >> 1;
+    return e == kPaNoValue ? x : x * pa_pow2(-h) * pa_pow2(h - e);
+}
+
+__device__ __forceinline__ void pa_split(const float (&x)[8], pa_u4& hi, pa_u4& lo) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const pa_h2 h = {(_Float16)x[2 * j], (_Float16)x[2 * j + 1]};
+        const pa_h2 l = {(_Float16)(x[2 * j] - (float)h.x), (_Float16)(x[2 * j + 1] - (float)h.y)};
+        hi[j] = __builtin_bit_cast(uint32_t, h);
+        lo[j] = __builtin_bit_cast(uint32_t, l);
+    }
+}
+
+__device__ __forceinline__ bool pa_finite(float x) { return fabsf(x) < INFINITY; }
+
+// One workgroup: 64 keys of one kv head (blockIdx.y); the last places of x plan instead.
+// Operand order, 16 bytes a lane and place:
+//   K: [half of 32 keys][16 dims][lane]: key lane % 32, dims 8 (lane / 32) ..
+//   V: [16 keys][32 dims][lane]: dim lane % 32, keys 4 (lane / 32) + 0 .. 3 and + 8 .. 11
+template <int HD>
+__device__ void pa_pack(const PaArgs& a, int slot, int head) {
+    __shared__ int s_first;
+    __shared__ float s_k[4], s_v[4];
+    __shared__ unsigned long long s_odd;
+    __shared__ int s_seq;
+    constexpr int N = kPaKeys * HD / 8 / 256;  // pieces of 16 bytes a thread, of K and of V
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, h = lane >> 5, l = lane & 31;
+    const int n = pa_in_order(a, &s_first);
+    if (t == 0) {
+        s_seq = -1;
+        s_odd = 0;
+    }
+    __syncthreads();
+    for (int s = t; s < n; s += 256)
+        if (pa_k_slot(a.k_off[s], s) <= slot) atomicMax(&s_seq, s);
+    __syncthreads();
+    const int seq = s_seq;
+    if (seq < 0) return;
+    const int k0 = a.k_off[seq], m = a.k_off[seq + 1] - k0, first = (slot - pa_k_slot(k0, seq)) * kPaKeys;
+    if (first >= m) return;
+    const float* kp = a.k + (size_t)(k0 + first) * a.k_stride + (size_t)head * HD;
+    const float* vp = a.v + (size_t)(k0 + first) * a.v_stride + (size_t)head * HD;
+    const int keys = min(kPaKeys, m - first);
+    float x[N][8], y[N][8];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int f = wave + 4 * i, key = 32 * (f / (HD / 16)) + l, d = 16 * (f % (HD / 16)) + 8 * h;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[i][j] = 0.0f;
+        if (key < keys) {
+            const float4 u = *(const float4*)(kp + (size_t)key * a.k_stride + d);
+            const float4 w = *(const float4*)(kp + (size_t)key * a.k_stride + d + 4);
+            x[i][0] = u.x, x[i][1] = u.y, x[i][2] = u.z, x[i][3] = u.w;
+            x[i][4] = w.x, x[i][5] = w.y, x[i][6] = w.z, x[i][7] = w.w;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int f = wave + 4 * i, d = 32 * (f % (HD / 32)) + l, key0 = 16 * (f / (HD / 32)) + 4 * h;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int key = key0 + (j & 3) + 8 * (j >> 2);
+            y[i][j] = key < keys ? vp[(size_t)key * a.v_stride + d] : 0.0f;
+        }
+    }
+    float ka = 0.0f, va = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (pa_finite(x[i][j])) ka = fmaxf(ka, fabsf(x[i][j]));
+            if (!pa_finite(y[i][j])) {
+                const int f = wave + 4 * i, key = 16 * (f / (HD / 32)) + 4 * h + (j & 3) + 8 * (j >> 2);
+                atomicOr(&s_odd, 1ull << key);
+                y[i][j] = 0.0f;
+            }
+            va = fmaxf(va, fabsf(y[i][j]));
+        }
+    ka = vk_group_max<64>(ka);
+    va = vk_group_max<64>(va);
+    if (lane == 0) {
+        s_k[wave] = ka;
+        s_v[wave] = va;
+    }
+    __syncthreads();
+    const int ke = pa_exponent(fmaxf(fmaxf(s_k[0], s_k[1]), fmaxf(s_k[2], s_k[3])));
+    const int ve = pa_exponent(fmaxf(fmaxf(s_v[0], s_v[1]), fmaxf(s_v[2], s_v[3])));
+    const size_t place = (size_t)slot * a.hkv + head;
+    pa_u4* out = (pa_u4*)(a.tiles + place * 4 * pa_part(HD));
+    constexpr int P = pa_part(HD) / 8;  // 16-byte pieces of a part
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int at = (wave + 4 * i) * 64 + lane;
+        pa_u4 hi, lo;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[i][j] = pa_scale(x[i][j], ke);
+        pa_split(x[i], hi, lo);
+        out[at] = hi;
+        out[P + at] = lo;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[i][j] = pa_scale(y[i][j], ve);
+        pa_split(y[i], hi, lo);
+        out[2 * P + at] = hi;
+        out[3 * P + at] = lo;
+    }
+    if (t == 0) a.meta[place] = PaTileMeta{ke == kPaNoValue ? 0 : ke, ve, s_odd};
+}
+
+// ---- planning ----------------------------------------------------------------------
+
+// One workgroup: the tiles' costs in order, and where each share begins.
+__device__ void pa_plan(const PaArgs& a) {
+    __shared__ int s_first, s_q[kPaSeqs + 1], s_k[kPaSeqs + 1];
+    __shared__ long long s_wave[4];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int n = pa_in_order(a, &s_first);
+    for (int s = t; s <= n; s += 256) {
+        s_q[s] = n ? a.q_off[s] : 0;
+        s_k[s] = n ? a.k_off[s] : 0;
+    }
+    __syncthreads();
+    const int slots = n ? pa_q_slot(a, s_q[n], n) : 0;  // beyond the last tile
+    auto find = [&](int slot) {  // the last sequence whose places begin at or before it
+        int lo = 0, hi = n - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (pa_q_slot(a, s_q[mid], mid) <= slot) lo = mid;
+            else hi = mid - 1;
+        }
+        return lo;
+    };
+    long long before = 0;
+    for (int base = 0; base < slots; base += 256) {
+        const int slot = base + t;
+        long long cost = 0;
+        if (slot < slots) {
+            const int s = find(slot), len = s_q[s + 1] - s_q[s], row0 = (slot - pa_q_slot(a, s_q[s], s)) * kPaRows;
+            if (row0 < len * a.g) {
+                int lo, units;
+                pa_span(a, len, s_k[s + 1] - s_k[s], row0, &lo, &units);
+                cost = units + kTileCost;
+            }
+        }
+        long long x = cost;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const long long y = __shfl_up(x, o, VK_WAVE);
+            if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 63) s_wave[wave] = x;
+        __syncthreads();
+        long long all = 0, mine = before;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            if (w < wave) mine += s_wave[w];
+            all += s_wave[w];
+        }
+        if (slot < slots) a.line[slot] = mine + x - cost;
+        before += all;
+    }
+    if (t == 0) a.line[slots] = before;
+    const long long total = before * a.hkv;
+    const long long shares = total ? min((long long)kPaShares, max(1ll, total / kLeast)) : 0;
+    const long long size = shares ? (total + shares - 1) / shares : 0;
+    if (t == 0) {
+        a.plan[0] = size;
+        a.plan[1] = total;
+        a.plan[2] = shares ? (total + size - 1) / size : 0;
+        a.plan[3] = n;
+    }
+    __syncthreads();  // line is written (and read by this workgroup alone)
+    __threadfence_block();
+    for (int i = t; i < kPaShares; i += 256) {
+        const long long x = i * size;
+        if (!size || x >= total) continue;
+        // the sequence: lines of sequence s begin at hkv line[its first place]
+        int lo = 0, hi = n - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (a.line[pa_q_slot(a, s_q[mid], mid)] * a.hkv <= x) lo = mid;
+            else hi = mid - 1;
+        }
+        const int s = lo, b = pa_q_slot(a, s_q[s], s);
+        const int tiles = (int)(((long long)(s_q[s + 1] - s_q[s]) * a.g + kPaRows - 1) / kPaRows);
+        const long long l0 = a.line[b], len = a.line[b + tiles] - l0;  // (empty places behind cost nothing)
+        const long long rest = x - l0 * a.hkv;
+        const int head = (int)(rest / len);
+        const long long in = rest - head * len;
+        int tl = 0, th = tiles - 1;
+        while (tl < th) {
+            const int mid = (tl + th + 1) >> 1;
+            if (a.line[b + mid] - l0 <= in) tl = mid;
+            else th = mid - 1;
+        }
+        a.start[i] = PaStart{s, head, b + tl, 0, l0 * a.hkv + head * len + (a.line[b + tl] - l0)};
+    }
+}
+
+template <int HD>
+__global__ __launch_bounds__(256) void vk_pattn_pack(PaArgs a) {
+    // planning first: it takes longest
+    if (blockIdx.x == 0) {
+        if (blockIdx.y == 0) pa_plan(a);
+        return;
+    }
+    pa_pack<HD>(a, (int)blockIdx.x - 1, blockIdx.y);
+}
+
+// ---- products ----------------------------------------------------------------------
+
+// A row's results so far, the same in the lanes l and l + 32 once the halves are summed
+struct PaState {
+    float m, sum;  // M; sum of w
+    int e;         // O is held times 2^-e
+};
+
+// A tile's exponents by a scalar load: a vector load's wait would wait for the tiles on
+// their way to LDS as well. What packing wrote is in memory since its launch ended.
+__device__ __forceinline__ PaTileMeta pa_meta(const PaTileMeta* p) {
+    typedef int i4 __attribute__((ext_vector_type(4)));
+    const uintptr_t x = (uintptr_t)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+    const i4 y = *(const __attribute__((address_space(4))) i4*)(((uintptr_t)hi << 32) | lo);
+    return __builtin_bit_cast(PaTileMeta, y);
+}
+
+// Sum or maximum of a row's two lanes
+__device__ __forceinline__ float pa_row_max(float v) {
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
+__device__ __forceinline__ float pa_row_sum(float v) {
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
+
+// A share's piece of partial results: O in register order [wave][16 bytes' place][lane],
+// then (M, sum, e) of each row.
+constexpr size_t pa_piece_floats(int hd) { return (size_t)kPaRows * hd + kPaRows * 4; }
+
+template <int HD>
+__device__ __forceinline__ void pa_store_rows(const PaArgs& a, int q0, int head, int rows, int row0,
+                                              const vk_f32x16 (&o)[HD / 32], float sum, int e) {
+    const int lane = threadIdx.x & 63, h = lane >> 5, r = row0 + (int)(threadIdx.x >> 6) * 32 + (lane & 31);
+    if (r >= rows) return;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // (NaN stays)
+    const int i = r / a.g, gh = r - i * a.g;
+    float* out = a.out + (size_t)(q0 + i) * a.out_stride + (size_t)(head * a.g + gh) * HD + 4 * h;
+    const int eh = max(min(e, 254), -252) >> 1;
+    const float f0 = e == kPaNoValue ? 0.0f : pa_pow2(eh), f1 = e == kPaNoValue ? 0.0f : pa_pow2(max(min(e, 254), -252) - eh);
+#pragma unroll
+    for (int b = 0; b < HD / 32; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            vk_f32x4 y;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) y[c] = o[b][4 * j + c] * inv * f0 * f1;
+            *(vk_f32x4*)(out + 32 * b + 8 * j) = y;
+        }
+}
+
+template <int HD>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void vk_pattn(PaArgs a) {
+    constexpr int KS = HD / 16, DB = HD / 32, P = pa_part(HD);
+    constexpr int DMA = 2 * P * 2 / 1024 / 4;  // 1 KB loads of K (hi and lo) a wave, and of V
+    __shared__ __align__(16) _Float16 s_k[2 * P], s_v[2 * P];
+    const int share = vk_xcd_tile(blockIdx.x, gridDim.x);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int h = lane >> 5, l = lane & 31;
+    const long long size = a.plan[0], total = a.plan[1];
+    const int n_seq = (int)a.plan[3];
+    const long long x0 = share * size, x1 = min(x0 + size, total);
+    if (threadIdx.x == 0) a.open[share] = PaOpen{0, 0, 0, 0};
+    if (x0 >= x1) return;
+    PaStart st = a.start[share];
+    st.seq = __builtin_amdgcn_readfirstlane(st.seq);
+    st.head = __builtin_amdgcn_readfirstlane(st.head);
+    st.slot = __builtin_amdgcn_readfirstlane(st.slot);
+    const uint32_t lds_k = vk_lds_addr(s_k) + wave * DMA * 1024, lds_v = vk_lds_addr(s_v) + wave * DMA * 1024;
+    int seq = st.seq, head = st.head, slot = st.slot;
+    long long line = st.line;
+    while (line < x1) {
+        const int q0 = __builtin_amdgcn_readfirstlane(a.q_off[seq]), n = __builtin_amdgcn_readfirstlane(a.q_off[seq + 1]) - q0;
+        const int k0 = __builtin_amdgcn_readfirstlane(a.k_off[seq]), m = __builtin_amdgcn_readfirstlane(a.k_off[seq + 1]) - k0;
+        const int rows = n * a.g, base = pa_q_slot(a, q0, seq), row0 = (slot - base) * kPaRows;
+        if (row0 >= rows) {  // the next head, or sequence
+            if (rows > 0 && ++head < a.hkv) {
+                slot = base;
+            } else {
+                head = 0;
+                if (++seq >= n_seq) break;
+                slot = pa_q_slot(a, a.q_off[seq], seq);
+            }
+            slot = __builtin_amdgcn_readfirstlane(slot);
+            continue;
+        }
+        int lo, units;
+        pa_span(a, n, m, row0, &lo, &units);
+        const long long u_first = line + kTileCost;
+        const int u0 = (int)max(min(x0 - u_first, (long long)units), 0ll), u1 = (int)max(min(x1 - u_first, (long long)units), 0ll);
+        line += units + kTileCost;
+        const int this_slot = slot++;
+        if (u0 >= u1) continue;
+
+        // ---- the tile's piece: units u0 .. u1 - 1
+        const size_t first_tile = (size_t)(pa_k_slot(k0, seq) + lo) * a.hkv + head;
+        const char* tiles = (const char*)a.tiles + first_tile * 8 * P + (wave * DMA) * 1024 + lane * 16;
+        const size_t tile_step = (size_t)a.hkv * 8 * P;
+        auto load_k = [&](int u) __attribute__((always_inline)) {
+            const char* g = tiles + u * tile_step;
+#pragma unroll
+            for (int i = 0; i < DMA; ++i) vk_dma_b128(g + i * 1024, lds_k + i * 1024);
+        };
+        auto load_v = [&](int u) __attribute__((always_inline)) {
+            const char* g = tiles + u * tile_step + 4 * P;
+#pragma unroll
+            for (int i = 0; i < DMA; ++i) vk_dma_b128(g + i * 1024, lds_v + i * 1024);
+        };
+        // q of this lane's row: dims 16 ks + 8 h .., as two parts of q 2^-qe
+        const int wrow0 = row0 + wave * 32, r = min(wrow0 + l, rows - 1), qi = r / a.g;
+        const float* qp = a.q + (size_t)(q0 + qi) * a.q_stride + (size_t)(head * a.g + r - qi * a.g) * HD + 8 * h;
+        pa_u4 qh[KS], ql[KS];
+        int qe;
+        {
+            float x[KS][8], most = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const float4 u = *(const float4*)(qp + 16 * s), w = *(const float4*)(qp + 16 * s + 4);
+                x[s][0] = u.x, x[s][1] = u.y, x[s][2] = u.z, x[s][3] = u.w;
+                x[s][4] = w.x, x[s][5] = w.y, x[s][6] = w.z, x[s][7] = w.w;
+            }
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    x[s][j] *= a.sign;
+                    if (pa_finite(x[s][j])) most = fmaxf(most, fabsf(x[s][j]));
+                }
+            const int e = pa_exponent(pa_row_max(most));
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[s][j] = pa_scale(x[s][j], e);
+                pa_split(x[s], qh[s], ql[s]);
+            }
+            qe = e == kPaNoValue ? 0 : e;
+        }
+        // every wave is through with LDS, and the row's loads have come, before the first tile's
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        VK_LDS_BARRIER();
+        load_k(u0);
+        load_v(u0);
+        const int pos = qi + (m - n);  // this lane's row
+        const int wpos0 = wrow0 / a.g + (m - n), wpos1 = min(wrow0 + 31, rows - 1) / a.g + (m - n);  // the wave's
+        vk_f32x16 o[DB];
+#pragma unroll
+        for (int b = 0; b < DB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
+        PaState s = {kNoMax, 0.0f, kPaNoValue};
+        for (int u = u0; u < u1; ++u) {
+            const PaTileMeta mt = pa_meta(a.meta + first_tile + (size_t)u * a.hkv);
+            const int ke = mt.k_exp, ve = mt.v_exp;
+            const unsigned long long odd = mt.odd;
+            const int kk = (lo + u) * kPaKeys;  // its first key
+            // keys of this unit that no row of the wave sees, that some do not
+            const bool none = wrow0 >= rows || kk >= m || (a.causal && (kk > wpos1 || (a.window && kk + kPaKeys - 1 <= wpos0 - a.window)));
+            const bool some = kk + kPaKeys > m || (a.causal && (kk + kPaKeys - 1 > wpos0 || (a.window && kk <= wpos1 - a.window)));
+            vk_wait_vm<DMA>();  // K has come, V may be on its way
+            VK_LDS_BARRIER();
+            vk_f32x16 t[2];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) t[0][i] = t[1][i] = 0.0f;
+            if (!none) {
+                const pa_h8* kh = (const pa_h8*)s_k + lane;
+                const pa_h8* kl = kh + P / 8;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const pa_h8 qhv = __builtin_bit_cast(pa_h8, qh[ks]), qlv = __builtin_bit_cast(pa_h8, ql[ks]);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const pa_h8 ah = kh[(x * KS + ks) * 64], al = kl[(x * KS + ks) * 64];
+                        t[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, qhv, t[x], 0, 0, 0);
+                        t[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, qlv, t[x], 0, 0, 0);
+                        t[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, qhv, t[x], 0, 0, 0);
+                    }
+                }
+            }
+            VK_LDS_BARRIER();  // all waves have read K
+            if (u + 1 < u1) load_k(u + 1);
+            if (!none) {
+                // (kept above 0 and below infinity, which would make NaN of -inf and of 0)
+                const float c = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.c, qe + ke), 0x1p-126f), 0x1.fffffep127f);
+                float most = -INFINITY;
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) t[x][i] *= c;
+                if (some) {
+                    const int end = min(m, a.causal ? pos + 1 : m) - kk;                       // keys below this,
+                    const int begin = a.causal && a.window ? pos - a.window + 1 - kk : 0;      // from this on
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int key = 32 * x + 8 * (i >> 2) + 4 * h + (i & 3);
+                            t[x][i] = key < end && key >= begin ? t[x][i] : -INFINITY;
+                        }
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) most = fmaxf(fmaxf(t[x][i], t[x][i + 1]), most);
+                const float top = fmaxf(ceilf(pa_row_max(most)), s.m);
+                const bool up = ve > s.e;  // the same for all
+                if (__any(top > s.m) || up) {
+                    const float f = __builtin_amdgcn_exp2f(s.m - top);
+                    const float fo = up ? f * __builtin_amdgcn_ldexpf(1.0f, max(s.e - ve, -200)) : f;
+                    s.sum *= f;
+                    s.m = top;
+                    if (up) s.e = ve;
+#pragma unroll
+                    for (int b = 0; b < DB; ++b)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[b][i] *= fo;
+                }
+                const float sub = s.m - 14.0f;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) t[x][i] = __builtin_amdgcn_exp2f(t[x][i] - sub);
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) s.sum += (t[x][i] + t[x][i + 1]) + (t[x][i + 2] + t[x][i + 3]);
+                }
+                if (ve < s.e) {
+                    const float f = __builtin_amdgcn_ldexpf(1.0f, max(ve - s.e, -200));
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) t[x][i] *= f;
+                }
+            }
+            if (u + 1 < u1) vk_wait_vm<DMA>();  // V has come, the next K may be on its way
+            else vk_wait_vm<0>();
+            VK_LDS_BARRIER();
+            if (!none) {
+                const pa_h8* vh = (const pa_h8*)s_v + lane;
+                const pa_h8* vl = vh + P / 8;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    float w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w[j] = t[x >> 1][8 * (x & 1) + j];
+                    pa_u4 wh, wl;
+                    pa_split(w, wh, wl);
+                    const pa_h8 whv = __builtin_bit_cast(pa_h8, wh), wlv = __builtin_bit_cast(pa_h8, wl);
+#pragma unroll
+                    for (int b = 0; b < DB; ++b) {
+                        const pa_h8 ah = vh[(x * DB + b) * 64], al = vl[(x * DB + b) * 64];
+                        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, whv, o[b], 0, 0, 0);
+                        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, wlv, o[b], 0, 0, 0);
+                        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, whv, o[b], 0, 0, 0);
+                    }
+                }
+                if (odd) {  // values that are not finite go to the rows that see them
+                    const int end = min(m, a.causal ? pos + 1 : m) - kk;
+                    const int begin = a.causal && a.window ? pos - a.window + 1 - kk : 0;
+                    for (unsigned long long rest = odd; rest; rest &= rest - 1) {
+                        const int key = __ffsll((unsigned long long)rest) - 1;
+                        const float* vp = a.v + (size_t)(k0 + kk + key) * a.v_stride + (size_t)head * HD + 4 * h;
+                        if (key >= end || key < begin) continue;
+#pragma unroll
+                        for (int b = 0; b < DB; ++b)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float4 y = *(const float4*)(vp + 32 * b + 8 * j);
+                                const float z[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    if (!pa_finite(z[i])) o[b][4 * j + i] += z[i];
+                            }
+                    }
+                }
+            }
+            VK_LDS_BARRIER();  // all waves have read V
+            if (u + 1 < u1) load_v(u + 1);
+        }
+        s.sum = pa_row_sum(s.sum);
+        if (u0 == 0 && u1 == units) {
+            pa_store_rows<HD>(a, q0, head, rows, row0, o, s.sum, s.e);
+            continue;
+        }
+        float* part = a.part + (size_t)(2 * share + (u0 == 0 ? 1 : 0)) * pa_piece_floats(HD);
+        vk_f32x4* po = (vk_f32x4*)part + wave * (HD / 8) * 64 + lane;
+#pragma unroll
+        for (int b = 0; b < DB; ++b)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                po[(b * 4 + j) * 64] = vk_f32x4{o[b][4 * j], o[b][4 * j + 1], o[b][4 * j + 2], o[b][4 * j + 3]};
+        if (h == 0)
+            ((vk_f32x4*)(part + (size_t)kPaRows * HD))[wave * 32 + l] =
+                vk_f32x4{s.m, s.sum, __int_as_float(s.e), 0.0f};
+        if (u0 == 0 && threadIdx.x == 0) {
+            const int last = (int)((u_first + units - 1) / size);  // the share with the last unit
+            a.open[share] = PaOpen{seq, head, this_slot, last - share + 1};
+        }
+    }
+}
+
+// A tile's pieces brought together, in their order: one workgroup for each share with a
+// tile's first piece.
+template <int HD>
+__global__ __launch_bounds__(256) void vk_pattn_join(PaArgs a) {
+    constexpr int DB = HD / 32;
+    const int share = blockIdx.x;
+    if (share >= (int)a.plan[2]) return;
+    const PaOpen open = a.open[share];
+    if (open.pieces < 2) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 31;
+    const int q0 = a.q_off[open.seq], rows = (a.q_off[open.seq + 1] - q0) * a.g;
+    const int row0 = (open.slot - pa_q_slot(a, q0, open.seq)) * kPaRows;
+    vk_f32x16 o[DB];
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
+    PaState s = {kNoMax, 0.0f, kPaNoValue};
+    for (int p = 0; p < open.pieces; ++p) {
+        const float* part = a.part + (size_t)(2 * (share + p) + (p == 0 ? 1 : 0)) * pa_piece_floats(HD);
+        const vk_f32x4* po = (const vk_f32x4*)part + wave * (HD / 8) * 64 + lane;
+        const vk_f32x4 ml = ((const vk_f32x4*)(part + (size_t)kPaRows * HD))[wave * 32 + l];
+        vk_f32x4 y[DB * 4];
+#pragma unroll
+        for (int j = 0; j < DB * 4; ++j) y[j] = po[j * 64];
+        const float m = fmaxf(s.m, ml[0]);
+        const int pe = __float_as_int(ml[2]), e = max(s.e, pe);
+        const float f0 = __builtin_amdgcn_exp2f(s.m - m), f1 = __builtin_amdgcn_exp2f(ml[0] - m);
+        const float g0 = f0 * __builtin_amdgcn_ldexpf(1.0f, max(s.e - e, -200));
+        const float g1 = f1 * __builtin_amdgcn_ldexpf(1.0f, max(pe - e, -200));
+        s.sum = s.sum * f0 + ml[1] * f1;
+        s.m = m;
+        s.e = e;
+#pragma unroll
+        for (int j = 0; j < DB * 4; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[j >> 2][4 * (j & 3) + c] = o[j >> 2][4 * (j & 3) + c] * g0 + y[j][c] * g1;
+    }
+    pa_store_rows<HD>(a, q0, open.head, rows, row0, o, s.sum, s.e);
+}
+
+// ---- launchers ---------------------------------------------------------------------
+
+size_t pattn_part_floats(int hd) { return 2 * (size_t)kPaShares * pa_piece_floats(hd); }
+
+template <int HD>
+static hipError_t go_pattn(hipStream_t s, const PaArgs& a) {
+    hipLaunchKernelGGL(vk_pattn_pack<HD>, dim3((unsigned)a.k_slots + 1, (unsigned)a.hkv), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(vk_pattn<HD>, dim3(kPaShares), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(vk_pattn_join<HD>, dim3(kPaShares), dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_pattn(hipStream_t s, int hd, const PaArgs& a) {
+    return hd == 64 ? go_pattn<64>(s, a) : go_pattn<128>(s, a);
+}
+
+}  // namespace vk

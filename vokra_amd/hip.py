@@ -294,6 +294,12 @@ def _declare(L):
     L.vokra_hip_rope_apply.argtypes = [P, P, sz, i32p, sz, f32p, f32p, sz, f32p, f32p]
     L.vokra_hip_rope_norm_apply_dev.argtypes = [P, P, C.POINTER(_HeadNorm), sz, P, sz, P, sz, P, sz, sz, P, sz, P, sz]
     L.vokra_hip_rope_norm_apply.argtypes = [P, P, C.POINTER(_HeadNorm), sz, i32p, sz, f32p, f32p, sz, f32p, f32p]
+    L.vokra_hip_packed_attn_create.argtypes = [P, sz, sz, sz, sz, sz, sz, C.POINTER(P)]
+    L.vokra_hip_packed_attn_destroy.argtypes = [P]
+    L.vokra_hip_packed_attn_destroy.restype = None
+    L.vokra_hip_packed_attn_dev.argtypes = [P, P, sz, sz, sz, sz, sz, P, P, P, sz, P, sz, P, sz, C.c_float, C.c_int, sz, P,
+                                            sz]
+    L.vokra_hip_packed_attn.argtypes = [P, P, sz, i32p, i32p, f32p, f32p, f32p, C.c_float, C.c_int, sz, f32p]
     L.vokra_hip_beam_create.argtypes = [P, sz, sz, sz, sz, C.POINTER(P)]
     L.vokra_hip_beam_destroy.argtypes = [P]
     L.vokra_hip_beam_destroy.restype = None
@@ -1000,6 +1006,58 @@ class RopePlan:
             pass
 
 
+class PackedAttention:
+    """Attention over packed sequences of different lengths (vokra_hip_packed_attn_*),
+    for calls of up to the sizes it is made for."""
+
+    def __init__(self, ctx: "HipContext", max_seq, max_q_rows, max_k_rows, n_head_q, n_head_kv, head_dim):
+        self._ctx = ctx
+        self._wq, self._wk = n_head_q * head_dim, n_head_kv * head_dim
+        self.head_dim = head_dim
+        h = C.c_void_p()
+        _check(lib().vokra_hip_packed_attn_create(ctx._h, max_seq, max_q_rows, max_k_rows, n_head_q, n_head_kv, head_dim,
+                                                  C.byref(h)))
+        self._h = h
+
+    def attn_dev(self, n_seq, n_q_rows, n_k_rows, max_q, max_k, d_q_offsets, d_k_offsets, d_q, d_k, d_v, scale, d_out,
+                 causal=False, window=0, q_stride=None, k_stride=None, v_stride=None, out_stride=None):
+        """Rows of q, k, v and out at their strides (in floats; the heads' width where not
+        given); d_k_offsets None: the queries'."""
+        wq, wk = self._wq, self._wk
+        _check(lib().vokra_hip_packed_attn_dev(
+            self._ctx._h, self._h, n_seq, n_q_rows, n_k_rows, max_q, max_k, d_q_offsets.ptr,
+            None if d_k_offsets is None else d_k_offsets.ptr, d_q.ptr, wq if q_stride is None else q_stride, d_k.ptr,
+            wk if k_stride is None else k_stride, d_v.ptr, wk if v_stride is None else v_stride, scale,
+            int(bool(causal)), window, d_out.ptr, wq if out_stride is None else out_stride))
+
+    def attn(self, q, k, v, q_lens, k_lens=None, scale=None, causal=False, window=0):
+        """Host rows q [sum(q_lens), n_head_q * head_dim], k and v [sum(k_lens), n_head_kv *
+        head_dim] of sequences of q_lens and k_lens (None: q_lens) rows. Returns q's shape."""
+        qv, kv, vv = _f32(q), _f32(k), _f32(v)
+        ql = np.asarray(q_lens, np.int64).reshape(-1)
+        kl = ql if k_lens is None else np.asarray(k_lens, np.int64).reshape(-1)
+        if ql.size != kl.size or (ql < 0).any() or (kl < 0).any():
+            raise InvalidArgument(f"packed attention: lengths of {ql.size} and {kl.size} sequences")
+        if qv.size != ql.sum() * self._wq or kv.size != kl.sum() * self._wk or vv.size != kv.size:
+            raise InvalidArgument(f"packed attention: {qv.size}, {kv.size} and {vv.size} values for {ql.sum()} and "
+                                  f"{kl.sum()} rows of {self._wq} and {self._wk}")
+        qo, ko = (np.concatenate([[0], np.cumsum(x)]).astype(np.int32) for x in (ql, kl))
+        out = np.zeros_like(qv)
+        _check(lib().vokra_hip_packed_attn(
+            self._ctx._h, self._h, ql.size, _ptr(qo, C.c_int32), _ptr(ko, C.c_int32), _ptr(qv, C.c_float),
+            _ptr(kv, C.c_float), _ptr(vv, C.c_float), self.head_dim ** -0.5 if scale is None else scale,
+            int(bool(causal)), window, _ptr(out, C.c_float)))
+        return out
+
+    def __del__(self):
+        try:
+            if getattr(self, "_h", None) and self._h.value and _ctx_alive(self):
+                lib().vokra_hip_packed_attn_destroy(self._h)
+                self._h = C.c_void_p()
+        except Exception:
+            pass
+
+
 class BeamSelect:
     """Beam search's selection (vokra_hip_beam_*): the best continuations of every
     group's beams, for calls of up to the sizes it is made for."""
@@ -1651,6 +1709,9 @@ class HipContext:
         return BeamSelect(self, max_groups, max_beams, max_vocab, max_out)
 
     # ---- attention ----------------------------------------------------------
+    def packed_attn(self, max_seq, max_q_rows, max_k_rows, n_head_q, n_head_kv, head_dim) -> PackedAttention:
+        return PackedAttention(self, max_seq, max_q_rows, max_k_rows, n_head_q, n_head_kv, head_dim)
+
     def attn_f32(self, q, k, v, n_head_q: int, n_head_kv: int = None, scale: float = None,
                  causal: bool = False, q_offset: int = 0) -> np.ndarray:
         """Fused SDPA (compute.rs:2703 attn_f32 core; nn.rs:209-325, text_decoder.rs:1302-1360).
