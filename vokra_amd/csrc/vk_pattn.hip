@@ -648,6 +648,258 @@ __global__ __launch_bounds__(256) void vk_pattn_join(PaArgs a) {
     pa_store_rows<HD>(a, q0, open.head, rows, row0, o, s.sum, s.e);
 }
 
+// ---- few rows ----------------------------------------------------------------------
+
+// Tokens, or candidates against rows of their own: at most 16 NT query rows of a kv head,
+// which all see the same keys. K and V are read once as they are, f32, straight into the
+// operands of the f32 matrix instruction (16 x 16 x 4): nothing is packed.
+//   S^T [16 keys][16 rows]: a lane's 16 bytes of K are one operand of four products
+//     (key lane % 16, dims 16 c + 4 (lane / 16) + j; q likewise);
+//   its accumulators (keys 4 (lane / 16) + i of row lane % 16) are the operand of
+//   O^T [16 dims][16 rows], step i, whose other one are 16 bytes of V row 4 (lane / 16) + i:
+//     dims 4 (lane % 16) + j, four products.
+// A wave takes KU keys at a time of its workgroup's range, with an online softmax of its
+// own; the four merge through LDS, ranges by vk_pattn_few_join. A step's K goes on its way
+// when the products of the step before have taken theirs, V likewise.
+constexpr int kFewMost = 4096;  // workgroups that leave partial results
+constexpr int few_keys(int hd, int nt) { return 64 * 64 / hd / nt; }  // KU: 128 registers of K and V at most
+
+__device__ __forceinline__ float pa_row4_max(float v) {  // over the lanes l % 16 alike
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    return pa_row_max(v);
+}
+__device__ __forceinline__ float pa_row4_sum(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return pa_row_sum(__uint_as_float(a[0]) + __uint_as_float(a[1]));
+}
+
+// The keys of sequence lengths n, m that its rows see: few rows are all at one place.
+__device__ __forceinline__ int pa_few_begin(const PaArgs& a, int m) {
+    return a.causal && a.window ? max(0, m - a.window) : 0;
+}
+
+template <int HD, int NT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void vk_pattn_few(PaArgs a, int per) {
+    constexpr int KU = few_keys(HD, NT), CH = KU / 16, QC = HD / 16, DD = HD / 64;
+    __shared__ int s_first;
+    __shared__ float s_m[4][16 * NT], s_l[4][16 * NT];
+    __shared__ vk_f32x4 s_o[4][16 * NT][HD / 4];
+    const int seq = blockIdx.z, head = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6, g = lane >> 4,
+              l = lane & 15;
+    const int n_ok = pa_in_order(a, &s_first);
+    if (seq >= n_ok) return;
+    const int q0 = a.q_off[seq], n = a.q_off[seq + 1] - q0, k0 = a.k_off[seq], m = a.k_off[seq + 1] - k0;
+    const int rows = n * a.g;
+    if (rows == 0 || rows > 16 * NT) return;
+    const int begin = pa_few_begin(a, m) + (int)blockIdx.x * per, end = min(begin + per, m);
+    if (blockIdx.x && begin >= m) return;
+    vk_f32x4 q[NT][QC];
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+        const int r = min(16 * x + l, rows - 1), i = r / a.g;
+        const float* qp = a.q + (size_t)(q0 + i) * a.q_stride + (size_t)(head * a.g + r - i * a.g) * HD + 4 * g;
+#pragma unroll
+        for (int c = 0; c < QC; ++c) q[x][c] = *(const vk_f32x4*)(qp + 16 * c) * (a.c * a.sign);
+    }
+    vk_f32x4 o[NT][DD][4];
+    float mx[NT], sum[NT];
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+        mx[x] = kNoMax;
+        sum[x] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DD; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[x][d][j] = vk_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const float* kp = a.k + (size_t)k0 * a.k_stride + (size_t)head * HD + 4 * g;
+    const float* vp = a.v + (size_t)k0 * a.v_stride + (size_t)head * HD + 4 * l;
+    vk_f32x4 k[CH][QC], v[CH][4][DD];
+    auto load_k = [&](int key) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const float* p = kp + (size_t)min(key + 16 * c + l, m - 1) * a.k_stride;
+#pragma unroll
+            for (int x = 0; x < QC; ++x) k[c][x] = __builtin_nontemporal_load((const vk_f32x4*)(p + 16 * x));
+        }
+    };
+    auto load_v = [&](int key) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float* p = vp + (size_t)min(key + 16 * c + 4 * g + i, m - 1) * a.v_stride;
+#pragma unroll
+                for (int d = 0; d < DD; ++d) v[c][i][d] = __builtin_nontemporal_load((const vk_f32x4*)(p + 64 * d));
+            }
+    };
+    int key = begin + wave * KU;
+    if (key < end) {
+        load_k(key);
+        load_v(key);
+    }
+    for (; key < end; key += 4 * KU) {
+        const int next = key + 4 * KU;
+        vk_f32x4 s[NT][CH];
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+            for (int c = 0; c < CH; ++c) s[x][c] = vk_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int y = 0; y < QC; ++y)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int c = 0; c < CH; ++c)
+#pragma unroll
+                    for (int x = 0; x < NT; ++x)
+                        s[x][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c][y][j], q[x][y][j], s[x][c], 0, 0, 0);
+        if (next < end) load_k(next);
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+            float most = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float y = s[x][c][i];
+                    y = y > -INFINITY ? y : __builtin_nanf("");  // of a key that is not finite
+                    y = key + 16 * c + 4 * g + i < end ? y : -INFINITY;
+                    s[x][c][i] = y;
+                    most = fmaxf(most, y);
+                }
+            const float top = fmaxf(pa_row4_max(most), mx[x]);
+            const float f = __builtin_amdgcn_exp2f(mx[x] - top);
+            mx[x] = top;
+            float add = 0.0f;
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[x][c][i] = __builtin_amdgcn_exp2f(s[x][c][i] - top);
+                    add += s[x][c][i];
+                }
+            sum[x] = sum[x] * f + add;
+#pragma unroll
+            for (int d = 0; d < DD; ++d)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[x][d][j] *= f;
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int d = 0; d < DD; ++d)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int x = 0; x < NT; ++x)
+                            o[x][d][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[c][i][d][j], s[x][c][i], o[x][d][j], 0, 0, 0);
+        if (next < end) load_v(next);
+    }
+    // o[x][d][j][i]: row 16 x + l, dim 64 d + 4 (4 g + i) + j
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+        const float all = pa_row4_sum(sum[x]);
+        if (g == 0) {
+            s_m[wave][16 * x + l] = mx[x];
+            s_l[wave][16 * x + l] = all;
+        }
+#pragma unroll
+        for (int d = 0; d < DD; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                s_o[wave][16 * x + l][16 * d + 4 * g + i] =
+                    vk_f32x4{o[x][d][0][i], o[x][d][1][i], o[x][d][2][i], o[x][d][3][i]};
+    }
+    __syncthreads();
+    const int ranges = max(1, (m - pa_few_begin(a, m) + per - 1) / per);
+    float* part = a.part + (((size_t)seq * a.hkv + head) * gridDim.x + blockIdx.x) * (16 * NT) * (HD + 4);
+    for (int y = t; y < rows * (HD / 4); y += 256) {
+        const int r = y / (HD / 4), d = y % (HD / 4);
+        float top = s_m[0][r];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w][r]);
+        vk_f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+        float all = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = __builtin_amdgcn_exp2f(s_m[w][r] - top);
+            all += s_l[w][r] * f;
+            z += s_o[w][r][d] * f;
+        }
+        if (ranges == 1) {
+            const int i = r / a.g;
+            const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+            *(vk_f32x4*)(a.out + (size_t)(q0 + i) * a.out_stride + (size_t)(head * a.g + r - i * a.g) * HD + 4 * d) = z * inv;
+        } else {
+            *(vk_f32x4*)(part + (size_t)r * (HD + 4) + 4 * d) = z;
+            if (d == 0) *(float2*)(part + (size_t)r * (HD + 4) + HD) = make_float2(top, all);
+        }
+    }
+}
+
+// A sequence's ranges of a kv head brought together.
+template <int HD, int NT>
+__global__ __launch_bounds__(256) void vk_pattn_few_join(PaArgs a, int per, int splits) {
+    __shared__ int s_first;
+    const int seq = blockIdx.y, head = blockIdx.x;
+    const int n_ok = pa_in_order(a, &s_first);
+    if (seq >= n_ok) return;
+    const int q0 = a.q_off[seq], n = a.q_off[seq + 1] - q0, m = a.k_off[seq + 1] - a.k_off[seq], rows = n * a.g;
+    const int ranges = (m - pa_few_begin(a, m) + per - 1) / per;
+    if (ranges < 2 || rows > 16 * NT) return;
+    const float* part = a.part + ((size_t)seq * a.hkv + head) * splits * (16 * NT) * (HD + 4);
+    for (int y = threadIdx.x; y < rows * (HD / 4); y += 256) {
+        const int r = y / (HD / 4), d = y % (HD / 4);
+        const float* p = part + (size_t)r * (HD + 4);
+        float top = kNoMax, all = 0.0f;
+        vk_f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s0 = 0; s0 < ranges; s0 += 8) {
+            float2 ml[8];
+            vk_f32x4 w[8];
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                const float* x = p + (size_t)min(s0 + s, ranges - 1) * (16 * NT) * (HD + 4);
+                ml[s] = *(const float2*)(x + HD);
+                w[s] = *(const vk_f32x4*)(x + 4 * d);
+            }
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                if (s0 + s >= ranges) break;
+                const float now = fmaxf(top, ml[s].x);
+                const float f = __builtin_amdgcn_exp2f(top - now), h = __builtin_amdgcn_exp2f(ml[s].x - now);
+                top = now;
+                all = all * f + ml[s].y * h;
+                z = z * f + w[s] * h;
+            }
+        }
+        const int i = r / a.g;
+        const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+        *(vk_f32x4*)(a.out + (size_t)(q0 + i) * a.out_stride + (size_t)(head * a.g + r - i * a.g) * HD + 4 * d) = z * inv;
+    }
+}
+
+template <int HD, int NT>
+static hipError_t go_few(hipStream_t s, const PaArgs& a) {
+    // ranges of a step of all four waves at least, for up to 2048 workgroups if all sequences
+    // were the longest
+    constexpr int step = 4 * few_keys(HD, NT);
+    const long long pairs = (long long)a.n_seq * a.hkv;
+    const int keys = a.causal && a.window ? std::min(a.max_k, a.window) : a.max_k;
+    const long long most = std::max<long long>(1, std::min<long long>(kFewMost, 2048) / pairs);
+    const int per = (int)std::max<long long>(step, ((keys + most - 1) / most + step - 1) / step * step);
+    const int splits = keys ? (keys + per - 1) / per : 1;
+    hipLaunchKernelGGL((vk_pattn_few<HD, NT>), dim3((unsigned)splits, (unsigned)a.hkv, (unsigned)a.n_seq), dim3(256), 0, s, a,
+                       per);
+    if (splits > 1)
+        hipLaunchKernelGGL((vk_pattn_few_join<HD, NT>), dim3((unsigned)a.hkv, (unsigned)a.n_seq), dim3(256), 0, s, a, per,
+                           splits);
+    return hipGetLastError();
+}
+
 // ---- launchers ---------------------------------------------------------------------
 
 size_t pattn_part_floats(int hd) { return 2 * (size_t)kPaShares * pa_piece_floats(hd); }
@@ -661,6 +913,13 @@ static hipError_t go_pattn(hipStream_t s, const PaArgs& a) {
 }
 
 hipError_t launch_pattn(hipStream_t s, int hd, const PaArgs& a) {
+    // few rows that all see the same keys: each key is read by few products, packing it
+    // would move three times its bytes
+    const long long rows = (long long)a.max_q * a.g;
+    if (rows <= kPaFewRows && (!a.causal || a.max_q == 1)) {
+        if (hd == 64) return rows <= 16 ? go_few<64, 1>(s, a) : go_few<64, 2>(s, a);
+        return rows <= 16 ? go_few<128, 1>(s, a) : go_few<128, 2>(s, a);
+    }
     return hd == 64 ? go_pattn<64>(s, a) : go_pattn<128>(s, a);
 }
 
