@@ -7,8 +7,9 @@
 #include <stdint.h>
 
 constexpr int kPaSeqs = 1024;    // sequences of a call at most
-constexpr int kPaShares = 512;   // workgroups that share a call's work: two a CU
-constexpr int kPaRows = 128;     // query rows of a tile: 32 a wave
+constexpr int kPaShares = 512;   // workgroups that share a call's work at most
+// query rows of a tile, 32 a wave
+constexpr int pa_tile_rows(int hd) { return hd == 64 ? 128 : 256; }
 constexpr int kPaKeys = 64;      // keys of a tile
 constexpr int kPaFewRows = 32;   // query rows of a kv head that the kernel without packing takes
 
@@ -43,7 +44,7 @@ struct PaArgs {
     // workspace
     _Float16* tiles;         // [slot of 64 keys][kv head]: K hi, K lo, V hi, V lo in operand order
     PaTileMeta* meta;        // [slot of 64 keys][kv head]
-    long long* line;         // [slot of 128 rows + 1] cost of the tiles before, of one kv head
+    long long* line;         // [slot of a tile of rows + 1] cost of the tiles before, of one kv head
     PaStart* start;          // [kPaShares]
     PaOpen* open;            // [kPaShares]
     long long* plan;         // [0] a share's length, [1] the line's, [2] shares, [3] sequences in order

@@ -8,7 +8,7 @@
 // that sees none gives zeros.
 //
 // Work: the n_s G query rows of a (sequence, kv head), row R being query R / G of head
-// hk G + R % G, in tiles of 128 (32 a wave), against tiles of 64 keys.
+// hk G + R % G, in tiles of 128 (hd 64) or 256 (hd 128), 32 a wave, against tiles of 64 keys.
 //
 // Packing (vk_pattn_pack): every K and V value as two fp16 parts, hi + lo, of the value
 // times a power of two that puts its tile's largest at 2^13, in the order in which the
@@ -24,9 +24,9 @@
 // difference, for the product alone.
 //
 // Even shares: the tiles' units (64 keys each, and two more for a tile's start and
-// end) lie on one line, which 512 workgroups share evenly whatever the lengths are; a
-// share holds whole tiles and at most two pieces, whose results vk_pattn_join brings
-// together.
+// end) lie on one line, which the workgroups that the chip holds at once (two waves a
+// SIMD) share evenly whatever the lengths are; a share holds whole tiles and at most two
+// pieces, whose results vk_pattn_join brings together.
 #include <algorithm>
 
 #include "vk_common.h"
@@ -42,6 +42,7 @@ constexpr int kTileCost = 2;   // a tile's start and end, in units
 constexpr int kLeast = 4;      // the least share
 constexpr float kNoMax = -0x1.fffffep127f;
 
+constexpr int pa_shares(int hd) { return hd == 64 ? 512 : 256; }  // two waves a SIMD
 // halves of one tile's K hi (K lo, V hi, V lo): 64 keys
 constexpr int pa_part(int hd) { return kPaKeys * hd; }
 
@@ -65,15 +66,17 @@ __device__ __forceinline__ int pa_in_order(const PaArgs& a, int* s_first) {
 
 // Places of tiles: sequence s has those from rows-before / size + s on, which never meet
 // the next one's.
+template <int HD>
 __device__ __forceinline__ int pa_q_slot(const PaArgs& a, int q0, int s) {
-    return (int)((long long)q0 * a.g / kPaRows) + s;
+    return (int)((unsigned)(q0 * a.g) / pa_tile_rows(HD)) + s;  // q0 g < 2^31
 }
 __device__ __forceinline__ int pa_k_slot(int k0, int s) { return k0 / kPaKeys + s; }
 
 // The keys that a tile's rows see lie in `units` tiles from `lo` on (one where there are
 // none).
+template <int HD>
 __device__ __forceinline__ void pa_span(const PaArgs& a, int n, int m, int row0, int* lo, int* units) {
-    const int last = min(row0 + kPaRows, n * a.g) - 1;
+    const int last = min(row0 + pa_tile_rows(HD), n * a.g) - 1;
     int k0 = 0, k1 = m;
     if (a.causal) {
         k1 = min(m, last / a.g + (m - n) + 1);
@@ -100,11 +103,20 @@ __device__ __forceinline__ float pa_scale(float x, int e) {
     return e == kPaNoValue ? x : x * pa_pow2(-h) * pa_pow2(h - e);
 }
 
-__device__ __forceinline__ void pa_split(const float (&x)[8], pa_u4& hi, pa_u4& lo) {
+// Eight values as two fp16 parts. x - hi as an fma of hi, widened on the way (one
+// instruction; minus_one is -1, kept from the compiler, which would make a conversion and a
+// subtraction of it): exact.
+__device__ __forceinline__ float pa_minus_one() {
+    float m = -1.0f;
+    asm("" : "+s"(m));
+    return m;
+}
+__device__ __forceinline__ void pa_split(const float (&x)[8], pa_u4& hi, pa_u4& lo, float minus_one) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const pa_h2 h = {(_Float16)x[2 * j], (_Float16)x[2 * j + 1]};
-        const pa_h2 l = {(_Float16)(x[2 * j] - (float)h.x), (_Float16)(x[2 * j + 1] - (float)h.y)};
+        pa_h2 h = {(_Float16)x[2 * j], (_Float16)x[2 * j + 1]};
+        asm("" : "+v"(h));  // the pair itself is what the fmas read
+        const pa_h2 l = {(_Float16)fmaf((float)h.x, minus_one, x[2 * j]), (_Float16)fmaf((float)h.y, minus_one, x[2 * j + 1])};
         hi[j] = __builtin_bit_cast(uint32_t, h);
         lo[j] = __builtin_bit_cast(uint32_t, l);
     }
@@ -187,18 +199,19 @@ __device__ void pa_pack(const PaArgs& a, int slot, int head) {
     const size_t place = (size_t)slot * a.hkv + head;
     pa_u4* out = (pa_u4*)(a.tiles + place * 4 * pa_part(HD));
     constexpr int P = pa_part(HD) / 8;  // 16-byte pieces of a part
+    const float minus_one = pa_minus_one();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int at = (wave + 4 * i) * 64 + lane;
         pa_u4 hi, lo;
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[i][j] = pa_scale(x[i][j], ke);
-        pa_split(x[i], hi, lo);
+        pa_split(x[i], hi, lo, minus_one);
         out[at] = hi;
         out[P + at] = lo;
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[i][j] = pa_scale(y[i][j], ve);
-        pa_split(y[i], hi, lo);
+        pa_split(y[i], hi, lo, minus_one);
         out[2 * P + at] = hi;
         out[3 * P + at] = lo;
     }
@@ -208,6 +221,7 @@ __device__ void pa_pack(const PaArgs& a, int slot, int head) {
 // ---- planning ----------------------------------------------------------------------
 
 // One workgroup: the tiles' costs in order, and where each share begins.
+template <int HD>
 __device__ void pa_plan(const PaArgs& a) {
     __shared__ int s_first, s_q[kPaSeqs + 1], s_k[kPaSeqs + 1];
     __shared__ long long s_wave[4];
@@ -218,12 +232,12 @@ __device__ void pa_plan(const PaArgs& a) {
         s_k[s] = n ? a.k_off[s] : 0;
     }
     __syncthreads();
-    const int slots = n ? pa_q_slot(a, s_q[n], n) : 0;  // beyond the last tile
+    const int slots = n ? pa_q_slot<HD>(a, s_q[n], n) : 0;  // beyond the last tile
     auto find = [&](int slot) {  // the last sequence whose places begin at or before it
         int lo = 0, hi = n - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (pa_q_slot(a, s_q[mid], mid) <= slot) lo = mid;
+            if (pa_q_slot<HD>(a, s_q[mid], mid) <= slot) lo = mid;
             else hi = mid - 1;
         }
         return lo;
@@ -233,10 +247,10 @@ __device__ void pa_plan(const PaArgs& a) {
         const int slot = base + t;
         long long cost = 0;
         if (slot < slots) {
-            const int s = find(slot), len = s_q[s + 1] - s_q[s], row0 = (slot - pa_q_slot(a, s_q[s], s)) * kPaRows;
+            const int s = find(slot), len = s_q[s + 1] - s_q[s], row0 = (slot - pa_q_slot<HD>(a, s_q[s], s)) * pa_tile_rows(HD);
             if (row0 < len * a.g) {
                 int lo, units;
-                pa_span(a, len, s_k[s + 1] - s_k[s], row0, &lo, &units);
+                pa_span<HD>(a, len, s_k[s + 1] - s_k[s], row0, &lo, &units);
                 cost = units + kTileCost;
             }
         }
@@ -260,7 +274,7 @@ __device__ void pa_plan(const PaArgs& a) {
     }
     if (t == 0) a.line[slots] = before;
     const long long total = before * a.hkv;
-    const long long shares = total ? min((long long)kPaShares, max(1ll, total / kLeast)) : 0;
+    const long long shares = total ? min((long long)pa_shares(HD), max(1ll, total / kLeast)) : 0;
     const long long size = shares ? (total + shares - 1) / shares : 0;
     if (t == 0) {
         a.plan[0] = size;
@@ -270,18 +284,18 @@ __device__ void pa_plan(const PaArgs& a) {
     }
     __syncthreads();  // line is written (and read by this workgroup alone)
     __threadfence_block();
-    for (int i = t; i < kPaShares; i += 256) {
+    for (int i = t; i < pa_shares(HD); i += 256) {
         const long long x = i * size;
         if (!size || x >= total) continue;
         // the sequence: lines of sequence s begin at hkv line[its first place]
         int lo = 0, hi = n - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (a.line[pa_q_slot(a, s_q[mid], mid)] * a.hkv <= x) lo = mid;
+            if (a.line[pa_q_slot<HD>(a, s_q[mid], mid)] * a.hkv <= x) lo = mid;
             else hi = mid - 1;
         }
-        const int s = lo, b = pa_q_slot(a, s_q[s], s);
-        const int tiles = (int)(((long long)(s_q[s + 1] - s_q[s]) * a.g + kPaRows - 1) / kPaRows);
+        const int s = lo, b = pa_q_slot<HD>(a, s_q[s], s);
+        const int tiles = (int)(((long long)(s_q[s + 1] - s_q[s]) * a.g + pa_tile_rows(HD) - 1) / pa_tile_rows(HD));
         const long long l0 = a.line[b], len = a.line[b + tiles] - l0;  // (empty places behind cost nothing)
         const long long rest = x - l0 * a.hkv;
         const int head = (int)(rest / len);
@@ -300,7 +314,7 @@ template <int HD>
 __global__ __launch_bounds__(256) void vk_pattn_pack(PaArgs a) {
     // planning first: it takes longest
     if (blockIdx.x == 0) {
-        if (blockIdx.y == 0) pa_plan(a);
+        if (blockIdx.y == 0) pa_plan<HD>(a);
         return;
     }
     pa_pack<HD>(a, (int)blockIdx.x - 1, blockIdx.y);
@@ -336,7 +350,7 @@ __device__ __forceinline__ float pa_row_sum(float v) {
 
 // A share's piece of partial results: O in register order [wave][16 bytes' place][lane],
 // then (M, sum, e) of each row.
-constexpr size_t pa_piece_floats(int hd) { return (size_t)kPaRows * hd + kPaRows * 4; }
+constexpr size_t pa_piece_floats(int hd) { return (size_t)pa_tile_rows(hd) * (hd + 4); }
 
 template <int HD>
 __device__ __forceinline__ void pa_store_rows(const PaArgs& a, int q0, int head, int rows, int row0,
@@ -359,66 +373,85 @@ __device__ __forceinline__ void pa_store_rows(const PaArgs& a, int q0, int head,
         }
 }
 
+// A piece of a tile: its units u0 .. u1 - 1.
+struct PaPiece {
+    int seq, head, slot;    // of the tile
+    long long line;         // its place on the line
+    int q0, n, k0, m;       // the sequence's rows and keys
+    int row0, lo, units;    // the tile's first row, its first tile of keys, its units
+    int u0, u1;
+};
+
+// The first piece of the share x0 .. x1 - 1 of the line from the tile at (seq, head,
+// slot, line) on; false: none. Everything is the same for all threads.
 template <int HD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void vk_pattn(PaArgs a) {
-    constexpr int KS = HD / 16, DB = HD / 32, P = pa_part(HD);
-    constexpr int DMA = 2 * P * 2 / 1024 / 4;  // 1 KB loads of K (hi and lo) a wave, and of V
-    __shared__ __align__(16) _Float16 s_k[2 * P], s_v[2 * P];
+__device__ __forceinline__ bool pa_next(const PaArgs& a, int n_seq, long long x0, long long x1, PaPiece& p) {
+    while (p.line < x1) {
+        p.q0 = __builtin_amdgcn_readfirstlane(a.q_off[p.seq]);
+        p.n = __builtin_amdgcn_readfirstlane(a.q_off[p.seq + 1]) - p.q0;
+        p.k0 = __builtin_amdgcn_readfirstlane(a.k_off[p.seq]);
+        p.m = __builtin_amdgcn_readfirstlane(a.k_off[p.seq + 1]) - p.k0;
+        const int rows = p.n * a.g, base = pa_q_slot<HD>(a, p.q0, p.seq);
+        p.row0 = (p.slot - base) * pa_tile_rows(HD);
+        if (p.row0 >= rows) {  // the next head, or sequence
+            if (rows > 0 && ++p.head < a.hkv) {
+                p.slot = base;
+                continue;
+            }
+            p.head = 0;
+            if (++p.seq >= n_seq) return false;
+            p.slot = pa_q_slot<HD>(a, __builtin_amdgcn_readfirstlane(a.q_off[p.seq]), p.seq);
+            continue;
+        }
+        pa_span<HD>(a, p.n, p.m, p.row0, &p.lo, &p.units);
+        const long long first = p.line + kTileCost;
+        p.u0 = (int)max(min(x0 - first, (long long)p.units), 0ll);
+        p.u1 = (int)max(min(x1 - first, (long long)p.units), 0ll);
+        if (p.u0 < p.u1) return true;
+        p.line += p.units + kTileCost;
+        ++p.slot;
+    }
+    return false;
+}
+
+// Tiles go global -> LDS directly, the next one (of the next piece, too) while this one
+// is worked on: two buffers, one barrier a unit, between which the two waves of a SIMD
+// run as they come, one's products beside the other's weights.
+template <int HD>
+__global__ __launch_bounds__(pa_tile_rows(HD) * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void vk_pattn(PaArgs a) {
+    constexpr int NW = pa_tile_rows(HD) / 32, KS = HD / 16, DB = HD / 32, P = pa_part(HD);
+    constexpr int DMA = 8 * P / 1024 / NW;  // 1 KB loads of a tile a wave
+    __shared__ __align__(16) _Float16 s_t[2][4 * P];  // K hi, K lo, V hi, V lo
     const int share = vk_xcd_tile(blockIdx.x, gridDim.x);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int h = lane >> 5, l = lane & 31;
+    const PaStart st = a.start[share];
     const long long size = a.plan[0], total = a.plan[1];
     const int n_seq = (int)a.plan[3];
     const long long x0 = share * size, x1 = min(x0 + size, total);
     if (threadIdx.x == 0) a.open[share] = PaOpen{0, 0, 0, 0};
     if (x0 >= x1) return;
-    PaStart st = a.start[share];
-    st.seq = __builtin_amdgcn_readfirstlane(st.seq);
-    st.head = __builtin_amdgcn_readfirstlane(st.head);
-    st.slot = __builtin_amdgcn_readfirstlane(st.slot);
-    const uint32_t lds_k = vk_lds_addr(s_k) + wave * DMA * 1024, lds_v = vk_lds_addr(s_v) + wave * DMA * 1024;
-    int seq = st.seq, head = st.head, slot = st.slot;
-    long long line = st.line;
-    while (line < x1) {
-        const int q0 = __builtin_amdgcn_readfirstlane(a.q_off[seq]), n = __builtin_amdgcn_readfirstlane(a.q_off[seq + 1]) - q0;
-        const int k0 = __builtin_amdgcn_readfirstlane(a.k_off[seq]), m = __builtin_amdgcn_readfirstlane(a.k_off[seq + 1]) - k0;
-        const int rows = n * a.g, base = pa_q_slot(a, q0, seq), row0 = (slot - base) * kPaRows;
-        if (row0 >= rows) {  // the next head, or sequence
-            if (rows > 0 && ++head < a.hkv) {
-                slot = base;
-            } else {
-                head = 0;
-                if (++seq >= n_seq) break;
-                slot = pa_q_slot(a, a.q_off[seq], seq);
-            }
-            slot = __builtin_amdgcn_readfirstlane(slot);
-            continue;
-        }
-        int lo, units;
-        pa_span(a, n, m, row0, &lo, &units);
-        const long long u_first = line + kTileCost;
-        const int u0 = (int)max(min(x0 - u_first, (long long)units), 0ll), u1 = (int)max(min(x1 - u_first, (long long)units), 0ll);
-        line += units + kTileCost;
-        const int this_slot = slot++;
-        if (u0 >= u1) continue;
-
-        // ---- the tile's piece: units u0 .. u1 - 1
-        const size_t first_tile = (size_t)(pa_k_slot(k0, seq) + lo) * a.hkv + head;
-        const char* tiles = (const char*)a.tiles + first_tile * 8 * P + (wave * DMA) * 1024 + lane * 16;
-        const size_t tile_step = (size_t)a.hkv * 8 * P;
-        auto load_k = [&](int u) __attribute__((always_inline)) {
-            const char* g = tiles + u * tile_step;
+    PaPiece p;
+    p.seq = __builtin_amdgcn_readfirstlane(st.seq);
+    p.head = __builtin_amdgcn_readfirstlane(st.head);
+    p.slot = __builtin_amdgcn_readfirstlane(st.slot);
+    p.line = st.line;
+    const float minus_one = pa_minus_one();
+    auto load = [&](const PaPiece& x, int u, int buffer) __attribute__((always_inline)) {
+        const size_t tile = (size_t)(pa_k_slot(x.k0, x.seq) + x.lo + u) * a.hkv + x.head;
+        const char* g = (const char*)a.tiles + tile * (8 * P) + wave * (DMA * 1024) + lane * 16;
+        const uint32_t to = vk_lds_addr(s_t) + buffer * (8 * P) + wave * (DMA * 1024);
 #pragma unroll
-            for (int i = 0; i < DMA; ++i) vk_dma_b128(g + i * 1024, lds_k + i * 1024);
-        };
-        auto load_v = [&](int u) __attribute__((always_inline)) {
-            const char* g = tiles + u * tile_step + 4 * P;
-#pragma unroll
-            for (int i = 0; i < DMA; ++i) vk_dma_b128(g + i * 1024, lds_v + i * 1024);
-        };
+        for (int i = 0; i < DMA; ++i) vk_dma_b128(g + i * 1024, to + i * 1024);
+    };
+    if (!pa_next<HD>(a, n_seq, x0, x1, p)) return;
+    load(p, p.u0, 0);
+    int buffer = 0;
+    for (bool more = true; more;) {
+        const int rows = p.n * a.g;
         // q of this lane's row: dims 16 ks + 8 h .., as two parts of q 2^-qe
-        const int wrow0 = row0 + wave * 32, r = min(wrow0 + l, rows - 1), qi = r / a.g;
-        const float* qp = a.q + (size_t)(q0 + qi) * a.q_stride + (size_t)(head * a.g + r - qi * a.g) * HD + 8 * h;
+        const int wrow0 = p.row0 + wave * 32, r = min(wrow0 + l, rows - 1), qi = r / a.g;
+        const float* qp = a.q + (size_t)(p.q0 + qi) * a.q_stride + (size_t)(p.head * a.g + r - qi * a.g) * HD + 8 * h;
         pa_u4 qh[KS], ql[KS];
         int qe;
         {
@@ -441,64 +474,62 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             for (int s = 0; s < KS; ++s) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[s][j] = pa_scale(x[s][j], e);
-                pa_split(x[s], qh[s], ql[s]);
+                pa_split(x[s], qh[s], ql[s], minus_one);
             }
             qe = e == kPaNoValue ? 0 : e;
         }
-        // every wave is through with LDS, and the row's loads have come, before the first tile's
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        VK_LDS_BARRIER();
-        load_k(u0);
-        load_v(u0);
-        const int pos = qi + (m - n);  // this lane's row
-        const int wpos0 = wrow0 / a.g + (m - n), wpos1 = min(wrow0 + 31, rows - 1) / a.g + (m - n);  // the wave's
+        const int pos = qi + (p.m - p.n);  // this lane's row
+        const int wpos0 = wrow0 / a.g + (p.m - p.n), wpos1 = min(wrow0 + 31, rows - 1) / a.g + (p.m - p.n);  // the wave's
         vk_f32x16 o[DB];
 #pragma unroll
         for (int b = 0; b < DB; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
         PaState s = {kNoMax, 0.0f, kPaNoValue};
-        for (int u = u0; u < u1; ++u) {
-            const PaTileMeta mt = pa_meta(a.meta + first_tile + (size_t)u * a.hkv);
+        PaPiece next = p;
+        for (int u = p.u0; u < p.u1; ++u) {
+            const PaTileMeta mt = pa_meta(a.meta + (size_t)(pa_k_slot(p.k0, p.seq) + p.lo + u) * a.hkv + p.head);
             const int ke = mt.k_exp, ve = mt.v_exp;
             const unsigned long long odd = mt.odd;
-            const int kk = (lo + u) * kPaKeys;  // its first key
-            // keys of this unit that no row of the wave sees, that some do not
-            const bool none = wrow0 >= rows || kk >= m || (a.causal && (kk > wpos1 || (a.window && kk + kPaKeys - 1 <= wpos0 - a.window)));
-            const bool some = kk + kPaKeys > m || (a.causal && (kk + kPaKeys - 1 > wpos0 || (a.window && kk <= wpos1 - a.window)));
-            vk_wait_vm<DMA>();  // K has come, V may be on its way
-            VK_LDS_BARRIER();
-            vk_f32x16 t[2];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) t[0][i] = t[1][i] = 0.0f;
+            const int kk = (p.lo + u) * kPaKeys;  // its first key
+            // no row of the wave sees a key of this unit; some see not all
+            const bool none = wrow0 >= rows || kk >= p.m ||
+                              (a.causal && (kk > wpos1 || (a.window && kk + kPaKeys - 1 <= wpos0 - a.window)));
+            const bool some = kk + kPaKeys > p.m ||
+                              (a.causal && (kk + kPaKeys - 1 > wpos0 || (a.window && kk <= wpos1 - a.window)));
+            vk_wait_vm<0>();
+            VK_LDS_BARRIER();  // this tile has come, the one before has been read by all
+            if (u + 1 < p.u1) {
+                load(p, u + 1, buffer ^ 1);
+            } else {
+                next.line += next.units + kTileCost;
+                ++next.slot;
+                more = pa_next<HD>(a, n_seq, x0, x1, next);
+                if (more) load(next, next.u0, buffer ^ 1);
+            }
             if (!none) {
-                const pa_h8* kh = (const pa_h8*)s_k + lane;
+                const pa_h8* kh = (const pa_h8*)s_t[buffer] + lane;
                 const pa_h8* kl = kh + P / 8;
+                const pa_h8* vh = kl + P / 8;
+                const pa_h8* vl = vh + P / 8;
+                constexpr vk_f32x16 zero = {};
+                vk_f32x16 t[2];
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     const pa_h8 qhv = __builtin_bit_cast(pa_h8, qh[ks]), qlv = __builtin_bit_cast(pa_h8, ql[ks]);
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const pa_h8 ah = kh[(x * KS + ks) * 64], al = kl[(x * KS + ks) * 64];
-                        t[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, qhv, t[x], 0, 0, 0);
+                        t[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, qhv, ks ? t[x] : zero, 0, 0, 0);
                         t[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, qlv, t[x], 0, 0, 0);
                         t[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, qhv, t[x], 0, 0, 0);
                     }
                 }
-            }
-            VK_LDS_BARRIER();  // all waves have read K
-            if (u + 1 < u1) load_k(u + 1);
-            if (!none) {
+                const int end = min(p.m, a.causal ? pos + 1 : p.m) - kk;               // the row sees keys below this,
+                const int begin = a.causal && a.window ? pos - a.window + 1 - kk : 0;  // from this on
                 // (kept above 0 and below infinity, which would make NaN of -inf and of 0)
                 const float c = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.c, qe + ke), 0x1p-126f), 0x1.fffffep127f);
-                float most = -INFINITY;
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) t[x][i] *= c;
                 if (some) {
-                    const int end = min(m, a.causal ? pos + 1 : m) - kk;                       // keys below this,
-                    const int begin = a.causal && a.window ? pos - a.window + 1 - kk : 0;      // from this on
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -507,11 +538,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                             t[x][i] = key < end && key >= begin ? t[x][i] : -INFINITY;
                         }
                 }
+                // (a median with infinity, kept from the compiler, is a maximum that takes the
+                // products' results as they come, where fmaxf would first quiet each)
+                float inf = INFINITY;
+                asm("" : "+s"(inf));
+                float most = -INFINITY;
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) most = fmaxf(fmaxf(t[x][i], t[x][i + 1]), most);
-                const float top = fmaxf(ceilf(pa_row_max(most)), s.m);
+                    for (int i = 0; i < 16; i += 4)
+                        most = fmaxf(fmaxf(__builtin_amdgcn_fmed3f(t[x][i], t[x][i + 1], inf),
+                                           __builtin_amdgcn_fmed3f(t[x][i + 2], t[x][i + 3], inf)),
+                                     most);
+                const float top = fmaxf(ceilf(pa_row_max(most) * c), s.m);
                 const bool up = ve > s.e;  // the same for all
                 if (__any(top > s.m) || up) {
                     const float f = __builtin_amdgcn_exp2f(s.m - top);
@@ -528,7 +567,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) t[x][i] = __builtin_amdgcn_exp2f(t[x][i] - sub);
+                    for (int i = 0; i < 16; ++i) t[x][i] = __builtin_amdgcn_exp2f(fmaf(t[x][i], c, -sub));
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) s.sum += (t[x][i] + t[x][i + 1]) + (t[x][i + 2] + t[x][i + 3]);
                 }
@@ -539,20 +578,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
                         for (int i = 0; i < 16; ++i) t[x][i] *= f;
                 }
-            }
-            if (u + 1 < u1) vk_wait_vm<DMA>();  // V has come, the next K may be on its way
-            else vk_wait_vm<0>();
-            VK_LDS_BARRIER();
-            if (!none) {
-                const pa_h8* vh = (const pa_h8*)s_v + lane;
-                const pa_h8* vl = vh + P / 8;
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     float w[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) w[j] = t[x >> 1][8 * (x & 1) + j];
                     pa_u4 wh, wl;
-                    pa_split(w, wh, wl);
+                    pa_split(w, wh, wl, minus_one);
                     const pa_h8 whv = __builtin_bit_cast(pa_h8, wh), wlv = __builtin_bit_cast(pa_h8, wl);
 #pragma unroll
                     for (int b = 0; b < DB; ++b) {
@@ -563,11 +595,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                     }
                 }
                 if (odd) {  // values that are not finite go to the rows that see them
-                    const int end = min(m, a.causal ? pos + 1 : m) - kk;
-                    const int begin = a.causal && a.window ? pos - a.window + 1 - kk : 0;
                     for (unsigned long long rest = odd; rest; rest &= rest - 1) {
                         const int key = __ffsll((unsigned long long)rest) - 1;
-                        const float* vp = a.v + (size_t)(k0 + kk + key) * a.v_stride + (size_t)head * HD + 4 * h;
+                        const float* vp = a.v + (size_t)(p.k0 + kk + key) * a.v_stride + (size_t)p.head * HD + 4 * h;
                         if (key >= end || key < begin) continue;
 #pragma unroll
                         for (int b = 0; b < DB; ++b)
@@ -582,35 +612,35 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                     }
                 }
             }
-            VK_LDS_BARRIER();  // all waves have read V
-            if (u + 1 < u1) load_v(u + 1);
+            buffer ^= 1;
         }
         s.sum = pa_row_sum(s.sum);
-        if (u0 == 0 && u1 == units) {
-            pa_store_rows<HD>(a, q0, head, rows, row0, o, s.sum, s.e);
-            continue;
-        }
-        float* part = a.part + (size_t)(2 * share + (u0 == 0 ? 1 : 0)) * pa_piece_floats(HD);
-        vk_f32x4* po = (vk_f32x4*)part + wave * (HD / 8) * 64 + lane;
+        if (p.u0 == 0 && p.u1 == p.units) {
+            pa_store_rows<HD>(a, p.q0, p.head, rows, p.row0, o, s.sum, s.e);
+        } else {
+            float* part = a.part + (size_t)(2 * share + (p.u0 == 0 ? 1 : 0)) * pa_piece_floats(HD);
+            vk_f32x4* po = (vk_f32x4*)part + wave * (HD / 8) * 64 + lane;
 #pragma unroll
-        for (int b = 0; b < DB; ++b)
+            for (int b = 0; b < DB; ++b)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                po[(b * 4 + j) * 64] = vk_f32x4{o[b][4 * j], o[b][4 * j + 1], o[b][4 * j + 2], o[b][4 * j + 3]};
-        if (h == 0)
-            ((vk_f32x4*)(part + (size_t)kPaRows * HD))[wave * 32 + l] =
-                vk_f32x4{s.m, s.sum, __int_as_float(s.e), 0.0f};
-        if (u0 == 0 && threadIdx.x == 0) {
-            const int last = (int)((u_first + units - 1) / size);  // the share with the last unit
-            a.open[share] = PaOpen{seq, head, this_slot, last - share + 1};
+                for (int j = 0; j < 4; ++j)
+                    po[(b * 4 + j) * 64] = vk_f32x4{o[b][4 * j], o[b][4 * j + 1], o[b][4 * j + 2], o[b][4 * j + 3]};
+            if (h == 0)
+                ((vk_f32x4*)(part + (size_t)pa_tile_rows(HD) * HD))[wave * 32 + l] =
+                    vk_f32x4{s.m, s.sum, __int_as_float(s.e), 0.0f};
+            if (p.u0 == 0 && threadIdx.x == 0) {
+                const int last = (int)((p.line + kTileCost + p.units - 1) / size);  // the share with the last unit
+                a.open[share] = PaOpen{p.seq, p.head, p.slot, last - share + 1};
+            }
         }
+        p = next;
     }
 }
 
 // A tile's pieces brought together, in their order: one workgroup for each share with a
 // tile's first piece.
 template <int HD>
-__global__ __launch_bounds__(256) void vk_pattn_join(PaArgs a) {
+__global__ __launch_bounds__(pa_tile_rows(HD) * 2) void vk_pattn_join(PaArgs a) {
     constexpr int DB = HD / 32;
     const int share = blockIdx.x;
     if (share >= (int)a.plan[2]) return;
@@ -618,7 +648,7 @@ __global__ __launch_bounds__(256) void vk_pattn_join(PaArgs a) {
     if (open.pieces < 2) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 31;
     const int q0 = a.q_off[open.seq], rows = (a.q_off[open.seq + 1] - q0) * a.g;
-    const int row0 = (open.slot - pa_q_slot(a, q0, open.seq)) * kPaRows;
+    const int row0 = (open.slot - pa_q_slot<HD>(a, q0, open.seq)) * pa_tile_rows(HD);
     vk_f32x16 o[DB];
 #pragma unroll
     for (int b = 0; b < DB; ++b)
@@ -628,7 +658,7 @@ __global__ __launch_bounds__(256) void vk_pattn_join(PaArgs a) {
     for (int p = 0; p < open.pieces; ++p) {
         const float* part = a.part + (size_t)(2 * (share + p) + (p == 0 ? 1 : 0)) * pa_piece_floats(HD);
         const vk_f32x4* po = (const vk_f32x4*)part + wave * (HD / 8) * 64 + lane;
-        const vk_f32x4 ml = ((const vk_f32x4*)(part + (size_t)kPaRows * HD))[wave * 32 + l];
+        const vk_f32x4 ml = ((const vk_f32x4*)(part + (size_t)pa_tile_rows(HD) * HD))[wave * 32 + l];
         vk_f32x4 y[DB * 4];
 #pragma unroll
         for (int j = 0; j < DB * 4; ++j) y[j] = po[j * 64];
@@ -902,13 +932,13 @@ static hipError_t go_few(hipStream_t s, const PaArgs& a) {
 
 // ---- launchers ---------------------------------------------------------------------
 
-size_t pattn_part_floats(int hd) { return 2 * (size_t)kPaShares * pa_piece_floats(hd); }
+size_t pattn_part_floats(int hd) { return 2 * (size_t)pa_shares(hd) * pa_piece_floats(hd); }
 
 template <int HD>
 static hipError_t go_pattn(hipStream_t s, const PaArgs& a) {
     hipLaunchKernelGGL(vk_pattn_pack<HD>, dim3((unsigned)a.k_slots + 1, (unsigned)a.hkv), dim3(256), 0, s, a);
-    hipLaunchKernelGGL(vk_pattn<HD>, dim3(kPaShares), dim3(256), 0, s, a);
-    hipLaunchKernelGGL(vk_pattn_join<HD>, dim3(kPaShares), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(vk_pattn<HD>, dim3(pa_shares(HD)), dim3(2 * pa_tile_rows(HD)), 0, s, a);
+    hipLaunchKernelGGL(vk_pattn_join<HD>, dim3(pa_shares(HD)), dim3(2 * pa_tile_rows(HD)), 0, s, a);
     return hipGetLastError();
 }
 
