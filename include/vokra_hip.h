@@ -367,8 +367,8 @@ int vokra_hip_packed_attn_create(vokra_hip_ctx_t *ctx, size_t max_seq, size_t ma
 void vokra_hip_packed_attn_destroy(vokra_hip_packed_attn_t *attn);
 /* Device pointers, asynchronous, nothing is allocated. n_q_rows and n_k_rows bound the
  * offsets, max_q and max_k the rows of any sequence. Rows lie q_stride (and so on)
- * floats apart, so q, k and v may be parts of one projection's rows; all are 16-byte
- * aligned, out overlaps none. The first sequence whose offsets are out of order, range
+ * floats apart (at most 2^23), so q, k and v may be parts of one projection's rows; all are
+ * 16-byte aligned, out overlaps none. The first sequence whose offsets are out of order, range
  * or bounds, and those behind it, are passed over: their rows of out stay as they are, as
  * do rows that no sequence has. */
 int vokra_hip_packed_attn_dev(vokra_hip_ctx_t *ctx, vokra_hip_packed_attn_t *attn, size_t n_seq, size_t n_q_rows,

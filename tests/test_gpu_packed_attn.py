@@ -107,7 +107,10 @@ def test_lengths_heads_and_masks(ctx, hq, hkv, hd, case):
     (8, 2, 128, [1111], None, True, 300),
     (2, 2, 64, [300] * 20, [1500] * 20, False, 0),
     (16, 2, 128, [1] * 40 + [600], [900] * 40 + [800], True, 0),
-    (1, 1, 128, [4100], None, True, 0)])
+    (1, 1, 128, [4100], None, True, 0),
+    (4, 2, 64, [90, 400, 0, 513], None, True, 0),  # packed, with sequences of no rows and of few
+    (8, 1, 128, [33, 385, 1, 64], None, True, 70),
+    (2, 1, 128, [40] * 300, None, True, 0)])  # short ones beyond two rounds of workgroups
 def test_keys_split_over_workgroups(ctx, hq, hkv, hd, ql, kl, causal, window):
     print("[case] packed split", hq, hkv, hd, ql[:3], causal, window, flush=True)
     kl = ql if kl is None else kl
@@ -334,7 +337,7 @@ def test_refusals(ctx):
     bad(*ok, q_stride=124)
     bad(*ok, q_stride=130)
     bad(*ok, k_stride=60)
-    bad(*ok, v_stride=2 ** 33)
+    bad(*ok, v_stride=2 ** 23 + 4)
     bad(*ok, out_stride=127)
     bad(*ok[:7], At(q, 1), *ok[8:])
     bad(*ok[:8], At(k, 2), *ok[9:])

@@ -38,8 +38,10 @@ typedef _Float16 pa_h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 pa_h2 __attribute__((ext_vector_type(2)));
 typedef uint32_t pa_u4 __attribute__((ext_vector_type(4)));
 
-constexpr int kTileCost = 2;   // a tile's start and end, in units
-constexpr int kLeast = 4;      // the least share
+// A tile's start and end, in units: two documents of 5001 and 8192 rows, 32 heads over 8 of
+// 128, 2.11 ms with 2, 2.07 with 3, 2.08 with 4; eight utterances of up to 1500 rows, 20 heads
+// of 64, 153 us with 2, 159 with 3
+constexpr int pa_cost(int hd) { return hd == 64 ? 2 : 3; }
 constexpr float kNoMax = -0x1.fffffep127f;
 
 constexpr int pa_shares(int hd) { return hd == 64 ? 512 : 256; }  // two waves a SIMD
@@ -47,6 +49,11 @@ constexpr int pa_shares(int hd) { return hd == 64 ? 512 : 256; }  // two waves a
 constexpr int pa_part(int hd) { return kPaKeys * hd; }
 
 // ---- sequences ---------------------------------------------------------------------
+
+__device__ __forceinline__ bool pa_wrong(const PaArgs& a, int q0, int q1, int k0, int k1) {
+    return q0 < 0 || q1 < q0 || q1 > a.q_rows || q1 - q0 > a.max_q || k0 < 0 || k1 < k0 || k1 > a.k_rows ||
+           k1 - k0 > a.max_k;
+}
 
 // How many sequences, from the first on, have offsets in order and range; a sequence
 // from there on is passed over. All threads of the workgroup, after a barrier; scratch:
@@ -56,27 +63,34 @@ __device__ __forceinline__ int pa_in_order(const PaArgs& a, int* s_first) {
     __syncthreads();
     for (int s = threadIdx.x; s < a.n_seq; s += (int)blockDim.x) {
         const int q0 = a.q_off[s], q1 = a.q_off[s + 1], k0 = a.k_off[s], k1 = a.k_off[s + 1];
-        if (q0 < 0 || q1 < q0 || q1 > a.q_rows || q1 - q0 > a.max_q || k0 < 0 || k1 < k0 || k1 > a.k_rows ||
-            k1 - k0 > a.max_k)
-            atomicMin(s_first, s);
+        if (pa_wrong(a, q0, q1, k0, k1)) atomicMin(s_first, s);
     }
     __syncthreads();
     return *s_first;
 }
 
+// A piece of a tile: its units u0 .. u1 - 1.
+struct PaPiece {
+    int seq, head, slot;    // of the tile
+    long long line;         // its place on the line
+    int q0, n, k0, m;       // the sequence's rows and keys
+    int row0, lo, units;    // the tile's first row, its first tile of keys, its units
+    int u0, u1;
+};
+
 // Places of tiles: sequence s has those from rows-before / size + s on, which never meet
 // the next one's.
-template <int HD>
+template <int ROWS>
 __device__ __forceinline__ int pa_q_slot(const PaArgs& a, int q0, int s) {
-    return (int)((unsigned)(q0 * a.g) / pa_tile_rows(HD)) + s;  // q0 g < 2^31
+    return (int)((unsigned)(q0 * a.g) / ROWS) + s;  // q0 g < 2^31
 }
 __device__ __forceinline__ int pa_k_slot(int k0, int s) { return k0 / kPaKeys + s; }
 
 // The keys that a tile's rows see lie in `units` tiles from `lo` on (one where there are
 // none).
-template <int HD>
+template <int ROWS>
 __device__ __forceinline__ void pa_span(const PaArgs& a, int n, int m, int row0, int* lo, int* units) {
-    const int last = min(row0 + pa_tile_rows(HD), n * a.g) - 1;
+    const int last = min(row0 + ROWS, n * a.g) - 1;
     int k0 = 0, k1 = m;
     if (a.causal) {
         k1 = min(m, last / a.g + (m - n) + 1);
@@ -91,16 +105,32 @@ __device__ __forceinline__ void pa_span(const PaArgs& a, int n, int m, int row0,
 // 2^e as f32, e within -126 .. 127
 __device__ __forceinline__ float pa_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// The exponent that puts a largest magnitude a (finite) at 2^13 .. 2^14 when values are
-// multiplied by 2^-e; kPaNoValue for 0.
+// The exponent that puts a largest magnitude a at 2^13 .. 2^14 when values are multiplied by
+// 2^-e, which is a normal number (an a below 2^-113 is put lower); kPaNoValue for 0.
 __device__ __forceinline__ int pa_exponent(float a) {
-    const int b = (int)(__float_as_uint(a) >> 23);
-    return a == 0.0f ? kPaNoValue : max(b - 127, -126) - 13;
+    return a == 0.0f ? kPaNoValue : max((int)(__float_as_uint(a) >> 23) - 127 - 13, -127);
 }
-// x 2^-e for e of pa_exponent: two factors, as the power may be beyond f32's
-__device__ __forceinline__ float pa_scale(float x, int e) {
-    const int h = e >> 1;
-    return e == kPaNoValue ? x : x * pa_pow2(-h) * pa_pow2(h - e);
+// 2^-e for e of pa_exponent (1 for none)
+__device__ __forceinline__ float pa_factor(int e) { return pa_pow2(e == kPaNoValue ? 0 : -e); }
+
+__device__ __forceinline__ bool pa_finite(float x) { return fabsf(x) < INFINITY; }
+
+// The largest finite magnitude of a lane's values
+template <int N>
+__device__ __forceinline__ float pa_most(const float (&x)[N][8]) {
+    float y = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) y = fmaxf(fmaxf(fabsf(x[i][j]), fabsf(x[i][j + 1])), y);  // (passes over NaN)
+    if (!(y < INFINITY)) {
+        y = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y = fmaxf(y, pa_finite(x[i][j]) ? fabsf(x[i][j]) : 0.0f);
+    }
+    return y;
 }
 
 // Eight values as two fp16 parts. x - hi as an fma of hi, widened on the way (one
@@ -122,100 +152,163 @@ __device__ __forceinline__ void pa_split(const float (&x)[8], pa_u4& hi, pa_u4& 
     }
 }
 
-__device__ __forceinline__ bool pa_finite(float x) { return fabsf(x) < INFINITY; }
-
-// One workgroup: 64 keys of one kv head (blockIdx.y); the last places of x plan instead.
-// Operand order, 16 bytes a lane and place:
+// 64 keys of a kv head, `keys` of them there, from rows kp and vp on, by 256 threads:
+// taken into registers (load), then written as a tile in operand order (store), 16 bytes
+// a lane and place:
 //   K: [half of 32 keys][16 dims][lane]: key lane % 32, dims 8 (lane / 32) ..
 //   V: [16 keys][32 dims][lane]: dim lane % 32, keys 4 (lane / 32) + 0 .. 3 and + 8 .. 11
+struct PaPackLds {
+    float k[4], v[4];
+    unsigned long long odd[4];
+};
 template <int HD>
-__device__ void pa_pack(const PaArgs& a, int slot, int head) {
-    __shared__ int s_first;
-    __shared__ float s_k[4], s_v[4];
-    __shared__ unsigned long long s_odd;
-    __shared__ int s_seq;
-    constexpr int N = kPaKeys * HD / 8 / 256;  // pieces of 16 bytes a thread, of K and of V
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, h = lane >> 5, l = lane & 31;
-    const int n = pa_in_order(a, &s_first);
-    if (t == 0) {
-        s_seq = -1;
-        s_odd = 0;
-    }
-    __syncthreads();
-    for (int s = t; s < n; s += 256)
-        if (pa_k_slot(a.k_off[s], s) <= slot) atomicMax(&s_seq, s);
-    __syncthreads();
-    const int seq = s_seq;
-    if (seq < 0) return;
-    const int k0 = a.k_off[seq], m = a.k_off[seq + 1] - k0, first = (slot - pa_k_slot(k0, seq)) * kPaKeys;
-    if (first >= m) return;
-    const float* kp = a.k + (size_t)(k0 + first) * a.k_stride + (size_t)head * HD;
-    const float* vp = a.v + (size_t)(k0 + first) * a.v_stride + (size_t)head * HD;
-    const int keys = min(kPaKeys, m - first);
+struct PaPack {
+    static constexpr int N = kPaKeys * HD / 8 / 256;  // pieces of 16 bytes a thread, of K and of V
     float x[N][8], y[N][8];
+
+    // Buffer loads: rows behind the last key read as zero, with no branch (strides are at
+    // most 2^23, so 64 rows are less than 2^31 bytes).
+    __device__ __forceinline__ void load(const float* kp, size_t k_stride, const float* vp, size_t v_stride, int keys) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), h = lane >> 5,
+                  l = lane & 31, ks = (int)k_stride * 4, vs = (int)v_stride * 4;
+        const auto rk = __builtin_amdgcn_make_buffer_rsrc((void*)kp, 0, (keys - 1) * ks + HD * 4, 0x20000);
+        const auto rv = __builtin_amdgcn_make_buffer_rsrc((void*)vp, 0, (keys - 1) * vs + HD * 4, 0x20000);
+        const int kl = l * ks + 32 * h, vl = 4 * h * vs + 4 * l;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int f = wave + 4 * i, key = 32 * (f / (HD / 16)) + l, d = 16 * (f % (HD / 16)) + 8 * h;
+        for (int i = 0; i < N; ++i) {
+            const int f = wave + 4 * i, at = kl + 32 * (f / (HD / 16)) * ks + 64 * (f % (HD / 16));
+            const vk_f32x4 u = __builtin_bit_cast(vk_f32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, at, 0, 0));
+            const vk_f32x4 w = __builtin_bit_cast(vk_f32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, at + 16, 0, 0));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[i][j] = 0.0f;
-        if (key < keys) {
-            const float4 u = *(const float4*)(kp + (size_t)key * a.k_stride + d);
-            const float4 w = *(const float4*)(kp + (size_t)key * a.k_stride + d + 4);
-            x[i][0] = u.x, x[i][1] = u.y, x[i][2] = u.z, x[i][3] = u.w;
-            x[i][4] = w.x, x[i][5] = w.y, x[i][6] = w.z, x[i][7] = w.w;
+            for (int j = 0; j < 4; ++j) {
+                x[i][j] = u[j];
+                x[i][4 + j] = w[j];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int f = wave + 4 * i, at = vl + 16 * (f / (HD / 32)) * vs + 128 * (f % (HD / 32));
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                y[i][j] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rv, at + ((j & 3) + 8 * (j >> 2)) * vs, 0, 0));
         }
     }
+
+    // out: the tile; the four waves meet once
+    __device__ __forceinline__ PaTileMeta store(pa_u4* out, PaPackLds& lds) {
+        constexpr int P = pa_part(HD) / 8;  // 16-byte pieces of a part
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+        float ka = pa_most<N>(x), va = pa_most<N>(y);
+        unsigned long long odd = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float sum = 0.0f;  // not finite if a value is not (or, harmlessly, at values near f32's end)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += fabsf(y[i][j]);
+            if (!pa_finite(sum))
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (!pa_finite(y[i][j])) {
+                        const int f = wave + 4 * i, key = 16 * (f / (HD / 32)) + 4 * h + (j & 3) + 8 * (j >> 2);
+                        odd |= 1ull << key;
+                        y[i][j] = 0.0f;
+                    }
+        }
+        ka = vk_group_max<64>(ka);
+        va = vk_group_max<64>(va);
+        if (__any(odd != 0))
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) odd |= __shfl_xor(odd, o, VK_WAVE);
+        if (lane == 0) {
+            lds.k[wave] = ka;
+            lds.v[wave] = va;
+            lds.odd[wave] = odd;
+        }
+        VK_LDS_BARRIER();
+        const int ke = pa_exponent(fmaxf(fmaxf(lds.k[0], lds.k[1]), fmaxf(lds.k[2], lds.k[3])));
+        const int ve = pa_exponent(fmaxf(fmaxf(lds.v[0], lds.v[1]), fmaxf(lds.v[2], lds.v[3])));
+        const PaTileMeta m = {ke == kPaNoValue ? 0 : ke, ve, (lds.odd[0] | lds.odd[1]) | (lds.odd[2] | lds.odd[3])};
+        const float minus_one = pa_minus_one(), kf = pa_factor(ke), vf = pa_factor(ve);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int at = (wave + 4 * i) * 64 + lane;
+            pa_u4 hi, lo;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[i][j] *= kf;
+            pa_split(x[i], hi, lo, minus_one);
+            out[at] = hi;
+            out[P + at] = lo;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[i][j] *= vf;
+            pa_split(y[i], hi, lo, minus_one);
+            out[2 * P + at] = hi;
+            out[3 * P + at] = lo;
+        }
+        return m;
+    }
+};
+
+// The sequence whose tiles' places `slot` is among, and its rows and keys: the last of those in
+// order (see pa_in_order) that begin there or before; false: none. 256 threads, one round of
+// memory.
+struct PaSeqLds {
+    int first, seq, at[4];
+};
+template <class Slot>
+__device__ __forceinline__ bool pa_find(const PaArgs& a, int slot, PaSeqLds& lds, PaPiece& p, Slot begins) {
+    constexpr int N = kPaSeqs / 256;
+    int q0[N], q1[N], k0[N], k1[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const int f = wave + 4 * i, d = 32 * (f % (HD / 32)) + l, key0 = 16 * (f / (HD / 32)) + 4 * h;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int key = key0 + (j & 3) + 8 * (j >> 2);
-            y[i][j] = key < keys ? vp[(size_t)key * a.v_stride + d] : 0.0f;
-        }
+        const int s = threadIdx.x + 256 * i;
+        if (s < a.n_seq) q0[i] = a.q_off[s], q1[i] = a.q_off[s + 1], k0[i] = a.k_off[s], k1[i] = a.k_off[s + 1];
     }
-    float ka = 0.0f, va = 0.0f;
+    if (threadIdx.x == 0) {
+        lds.first = a.n_seq;
+        lds.seq = -1;
+    }
+    VK_LDS_BARRIER();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int s = threadIdx.x + 256 * i;
+        if (s < a.n_seq && pa_wrong(a, q0[i], q1[i], k0[i], k1[i])) atomicMin(&lds.first, s);
+    }
+    VK_LDS_BARRIER();
+    const int n = lds.first;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int s = threadIdx.x + 256 * i;
+        if (s < n && begins(q0[i], k0[i], s) <= slot) atomicMax(&lds.seq, s);
+    }
+    VK_LDS_BARRIER();
+    p.seq = __builtin_amdgcn_readfirstlane(lds.seq);
 #pragma unroll
     for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (pa_finite(x[i][j])) ka = fmaxf(ka, fabsf(x[i][j]));
-            if (!pa_finite(y[i][j])) {
-                const int f = wave + 4 * i, key = 16 * (f / (HD / 32)) + 4 * h + (j & 3) + 8 * (j >> 2);
-                atomicOr(&s_odd, 1ull << key);
-                y[i][j] = 0.0f;
-            }
-            va = fmaxf(va, fabsf(y[i][j]));
-        }
-    ka = vk_group_max<64>(ka);
-    va = vk_group_max<64>(va);
-    if (lane == 0) {
-        s_k[wave] = ka;
-        s_v[wave] = va;
-    }
-    __syncthreads();
-    const int ke = pa_exponent(fmaxf(fmaxf(s_k[0], s_k[1]), fmaxf(s_k[2], s_k[3])));
-    const int ve = pa_exponent(fmaxf(fmaxf(s_v[0], s_v[1]), fmaxf(s_v[2], s_v[3])));
+        if ((int)threadIdx.x + 256 * i == p.seq) lds.at[0] = q0[i], lds.at[1] = q1[i], lds.at[2] = k0[i], lds.at[3] = k1[i];
+    VK_LDS_BARRIER();
+    if (p.seq < 0) return false;
+    p.q0 = __builtin_amdgcn_readfirstlane(lds.at[0]);
+    p.n = __builtin_amdgcn_readfirstlane(lds.at[1]) - p.q0;
+    p.k0 = __builtin_amdgcn_readfirstlane(lds.at[2]);
+    p.m = __builtin_amdgcn_readfirstlane(lds.at[3]) - p.k0;
+    return true;
+}
+
+// One workgroup: a tile of 64 keys of one kv head.
+template <int HD>
+__device__ void pa_pack(const PaArgs& a, int slot, int head) {
+    __shared__ PaSeqLds s_seq;
+    __shared__ PaPackLds s_lds;
+    PaPiece p;
+    if (!pa_find(a, slot, s_seq, p, [](int, int k0, int s) { return pa_k_slot(k0, s); })) return;
+    const int first = (slot - pa_k_slot(p.k0, p.seq)) * kPaKeys;
+    if (first >= p.m) return;
+    PaPack<HD> t;
+    t.load(a.k + (size_t)(p.k0 + first) * a.k_stride + (size_t)head * HD, a.k_stride,
+           a.v + (size_t)(p.k0 + first) * a.v_stride + (size_t)head * HD, a.v_stride, min(kPaKeys, p.m - first));
     const size_t place = (size_t)slot * a.hkv + head;
-    pa_u4* out = (pa_u4*)(a.tiles + place * 4 * pa_part(HD));
-    constexpr int P = pa_part(HD) / 8;  // 16-byte pieces of a part
-    const float minus_one = pa_minus_one();
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int at = (wave + 4 * i) * 64 + lane;
-        pa_u4 hi, lo;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[i][j] = pa_scale(x[i][j], ke);
-        pa_split(x[i], hi, lo, minus_one);
-        out[at] = hi;
-        out[P + at] = lo;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[i][j] = pa_scale(y[i][j], ve);
-        pa_split(y[i], hi, lo, minus_one);
-        out[2 * P + at] = hi;
-        out[3 * P + at] = lo;
-    }
-    if (t == 0) a.meta[place] = PaTileMeta{ke == kPaNoValue ? 0 : ke, ve, s_odd};
+    const PaTileMeta meta = t.store((pa_u4*)(a.tiles + place * 4 * pa_part(HD)), s_lds);
+    if (threadIdx.x == 0) a.meta[place] = meta;
 }
 
 // ---- planning ----------------------------------------------------------------------
@@ -232,12 +325,12 @@ __device__ void pa_plan(const PaArgs& a) {
         s_k[s] = n ? a.k_off[s] : 0;
     }
     __syncthreads();
-    const int slots = n ? pa_q_slot<HD>(a, s_q[n], n) : 0;  // beyond the last tile
+    const int slots = n ? pa_q_slot<pa_tile_rows(HD)>(a, s_q[n], n) : 0;  // beyond the last tile
     auto find = [&](int slot) {  // the last sequence whose places begin at or before it
         int lo = 0, hi = n - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (pa_q_slot<HD>(a, s_q[mid], mid) <= slot) lo = mid;
+            if (pa_q_slot<pa_tile_rows(HD)>(a, s_q[mid], mid) <= slot) lo = mid;
             else hi = mid - 1;
         }
         return lo;
@@ -247,11 +340,11 @@ __device__ void pa_plan(const PaArgs& a) {
         const int slot = base + t;
         long long cost = 0;
         if (slot < slots) {
-            const int s = find(slot), len = s_q[s + 1] - s_q[s], row0 = (slot - pa_q_slot<HD>(a, s_q[s], s)) * pa_tile_rows(HD);
+            const int s = find(slot), len = s_q[s + 1] - s_q[s], row0 = (slot - pa_q_slot<pa_tile_rows(HD)>(a, s_q[s], s)) * pa_tile_rows(HD);
             if (row0 < len * a.g) {
                 int lo, units;
-                pa_span<HD>(a, len, s_k[s + 1] - s_k[s], row0, &lo, &units);
-                cost = units + kTileCost;
+                pa_span<pa_tile_rows(HD)>(a, len, s_k[s + 1] - s_k[s], row0, &lo, &units);
+                cost = units + pa_cost(HD);
             }
         }
         long long x = cost;
@@ -274,7 +367,7 @@ __device__ void pa_plan(const PaArgs& a) {
     }
     if (t == 0) a.line[slots] = before;
     const long long total = before * a.hkv;
-    const long long shares = total ? min((long long)pa_shares(HD), max(1ll, total / kLeast)) : 0;
+    const long long shares = total ? min((long long)pa_shares(HD), max(1ll, total / (pa_cost(HD) + 1))) : 0;
     const long long size = shares ? (total + shares - 1) / shares : 0;
     if (t == 0) {
         a.plan[0] = size;
@@ -291,10 +384,10 @@ __device__ void pa_plan(const PaArgs& a) {
         int lo = 0, hi = n - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (a.line[pa_q_slot<HD>(a, s_q[mid], mid)] * a.hkv <= x) lo = mid;
+            if (a.line[pa_q_slot<pa_tile_rows(HD)>(a, s_q[mid], mid)] * a.hkv <= x) lo = mid;
             else hi = mid - 1;
         }
-        const int s = lo, b = pa_q_slot<HD>(a, s_q[s], s);
+        const int s = lo, b = pa_q_slot<pa_tile_rows(HD)>(a, s_q[s], s);
         const int tiles = (int)(((long long)(s_q[s + 1] - s_q[s]) * a.g + pa_tile_rows(HD) - 1) / pa_tile_rows(HD));
         const long long l0 = a.line[b], len = a.line[b + tiles] - l0;  // (empty places behind cost nothing)
         const long long rest = x - l0 * a.hkv;
@@ -373,25 +466,25 @@ __device__ __forceinline__ void pa_store_rows(const PaArgs& a, int q0, int head,
         }
 }
 
-// A piece of a tile: its units u0 .. u1 - 1.
-struct PaPiece {
-    int seq, head, slot;    // of the tile
-    long long line;         // its place on the line
-    int q0, n, k0, m;       // the sequence's rows and keys
-    int row0, lo, units;    // the tile's first row, its first tile of keys, its units
-    int u0, u1;
-};
+// A sequence's offsets by scalar loads (see pa_meta; the caller wrote them before the
+// launch).
+__device__ __forceinline__ void pa_lengths(const PaArgs& a, PaPiece& p) {
+    typedef __attribute__((address_space(4))) const int* sp;
+    const sp q = (sp)(uintptr_t)a.q_off + p.seq, k = (sp)(uintptr_t)a.k_off + p.seq;
+    const int q0 = q[0], q1 = q[1], k0 = k[0], k1 = k[1];
+    p.q0 = q0;
+    p.n = q1 - q0;
+    p.k0 = k0;
+    p.m = k1 - k0;
+}
 
 // The first piece of the share x0 .. x1 - 1 of the line from the tile at (seq, head,
-// slot, line) on; false: none. Everything is the same for all threads.
+// slot, line) on, whose sequence's lengths are there; false: none. Everything is the same
+// for all threads.
 template <int HD>
 __device__ __forceinline__ bool pa_next(const PaArgs& a, int n_seq, long long x0, long long x1, PaPiece& p) {
     while (p.line < x1) {
-        p.q0 = __builtin_amdgcn_readfirstlane(a.q_off[p.seq]);
-        p.n = __builtin_amdgcn_readfirstlane(a.q_off[p.seq + 1]) - p.q0;
-        p.k0 = __builtin_amdgcn_readfirstlane(a.k_off[p.seq]);
-        p.m = __builtin_amdgcn_readfirstlane(a.k_off[p.seq + 1]) - p.k0;
-        const int rows = p.n * a.g, base = pa_q_slot<HD>(a, p.q0, p.seq);
+        const int rows = p.n * a.g, base = pa_q_slot<pa_tile_rows(HD)>(a, p.q0, p.seq);
         p.row0 = (p.slot - base) * pa_tile_rows(HD);
         if (p.row0 >= rows) {  // the next head, or sequence
             if (rows > 0 && ++p.head < a.hkv) {
@@ -400,18 +493,193 @@ __device__ __forceinline__ bool pa_next(const PaArgs& a, int n_seq, long long x0
             }
             p.head = 0;
             if (++p.seq >= n_seq) return false;
-            p.slot = pa_q_slot<HD>(a, __builtin_amdgcn_readfirstlane(a.q_off[p.seq]), p.seq);
+            pa_lengths(a, p);
+            p.slot = pa_q_slot<pa_tile_rows(HD)>(a, p.q0, p.seq);
             continue;
         }
-        pa_span<HD>(a, p.n, p.m, p.row0, &p.lo, &p.units);
-        const long long first = p.line + kTileCost;
+        pa_span<pa_tile_rows(HD)>(a, p.n, p.m, p.row0, &p.lo, &p.units);
+        const long long first = p.line + pa_cost(HD);
         p.u0 = (int)max(min(x0 - first, (long long)p.units), 0ll);
         p.u1 = (int)max(min(x1 - first, (long long)p.units), 0ll);
         if (p.u0 < p.u1) return true;
-        p.line += p.units + kTileCost;
+        p.line += p.units + pa_cost(HD);
         ++p.slot;
     }
     return false;
+}
+
+// A wave's 32 rows of a tile: q, as two parts of q 2^-qe in the operand order (dims 16 ks +
+// 8 h .. of row l), and where they stand.
+template <int HD>
+struct PaWave {
+    pa_u4 qh[HD / 16], ql[HD / 16];
+    int qe, from, to;          // this lane's row, which sees the keys from .. to - 1
+    int some_from, some_to;    // keys that a row of the wave sees,
+    int all_from, all_to;      // that all of them see
+
+    __device__ __forceinline__ void load(const PaArgs& a, const PaPiece& p, int wave) {
+        constexpr int KS = HD / 16;
+        const int lane = threadIdx.x & 63, h = lane >> 5, l = lane & 31, rows = p.n * a.g;
+        const int first = p.row0 + wave * 32, r = min(first + l, rows - 1), qi = r / a.g;
+        const int off = p.m - p.n, pos0 = first / a.g + off, pos1 = min(first + 31, rows - 1) / a.g + off, pos = qi + off;
+        from = some_from = all_from = 0;
+        to = some_to = all_to = p.m;
+        if (a.causal) {
+            to = min(p.m, pos + 1);
+            some_to = min(p.m, pos1 + 1);
+            all_to = min(p.m, pos0 + 1);
+            if (a.window) {
+                from = pos - a.window + 1;
+                some_from = pos0 - a.window + 1;
+                all_from = pos1 - a.window + 1;
+            }
+        }
+        if (first >= rows) some_to = 0;  // no rows
+        const float* qp = a.q + (size_t)(p.q0 + qi) * a.q_stride + (size_t)(p.head * a.g + r - qi * a.g) * HD + 8 * h;
+        float x[KS][8];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const float4 u = *(const float4*)(qp + 16 * s), w = *(const float4*)(qp + 16 * s + 4);
+            x[s][0] = u.x, x[s][1] = u.y, x[s][2] = u.z, x[s][3] = u.w;
+            x[s][4] = w.x, x[s][5] = w.y, x[s][6] = w.z, x[s][7] = w.w;
+        }
+        if (a.sign != 1.0f)
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[s][j] *= a.sign;
+        float most = 0.0f;  // (a row with a value that is not finite is NaN under any power of two)
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) most = fmaxf(fmaxf(fabsf(x[s][j]), fabsf(x[s][j + 1])), most);
+        const int e = pa_exponent(pa_row_max(most));
+        const float minus_one = pa_minus_one(), factor = pa_factor(e);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[s][j] *= factor;
+            pa_split(x[s], qh[s], ql[s], minus_one);
+        }
+        qe = e == kPaNoValue ? 0 : e;
+    }
+    // Whether a row of the wave sees a key of the unit that begins at key kk
+    __device__ __forceinline__ bool sees(int kk) const { return kk < some_to && kk + kPaKeys > some_from; }
+};
+
+// One unit: the wave's rows against the tile in LDS (K hi, K lo, V hi, V lo), whose first
+// key is kk.
+template <int HD>
+__device__ __forceinline__ void pa_unit(const PaArgs& a, const PaPiece& x, const PaWave<HD>& w, const _Float16* tile,
+                                        const PaTileMeta& meta, int kk, vk_f32x16 (&o)[HD / 32], PaState& s,
+                                        float minus_one) {
+    constexpr int KS = HD / 16, DB = HD / 32, P = pa_part(HD);
+    const int lane = threadIdx.x & 63, h = lane >> 5, ve = meta.v_exp;
+    const pa_h8* kh = (const pa_h8*)tile + lane;
+    const pa_h8* kl = kh + P / 8;
+    const pa_h8* vh = kl + P / 8;
+    const pa_h8* vl = vh + P / 8;
+    constexpr vk_f32x16 zero = {};
+    vk_f32x16 t[2];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        const pa_h8 qhv = __builtin_bit_cast(pa_h8, w.qh[ks]), qlv = __builtin_bit_cast(pa_h8, w.ql[ks]);
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            const pa_h8 ah = kh[(y * KS + ks) * 64], al = kl[(y * KS + ks) * 64];
+            t[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, qhv, ks ? t[y] : zero, 0, 0, 0);
+            t[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, qlv, t[y], 0, 0, 0);
+            t[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, qhv, t[y], 0, 0, 0);
+        }
+    }
+    const int begin = w.from - kk, end = w.to - kk;  // keys of the unit that the row sees
+    // (kept above 0 and below infinity, which would make NaN of -inf and of 0)
+    const float c = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.c, w.qe + meta.k_exp), 0x1p-126f), 0x1.fffffep127f);
+    if (kk + kPaKeys > w.all_to || kk < w.all_from) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = 32 * y + 8 * (i >> 2) + 4 * h + (i & 3);
+                t[y][i] = key < end && key >= begin ? t[y][i] : -INFINITY;
+            }
+    }
+    // (a median with infinity, kept from the compiler, is a maximum that takes the
+    // products' results as they come, where fmaxf would first quiet each)
+    float inf = INFINITY;
+    asm("" : "+s"(inf));
+    float most = -INFINITY;
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+            most = fmaxf(fmaxf(__builtin_amdgcn_fmed3f(t[y][i], t[y][i + 1], inf),
+                               __builtin_amdgcn_fmed3f(t[y][i + 2], t[y][i + 3], inf)),
+                         most);
+    const float top = fmaxf(ceilf(pa_row_max(most) * c), s.m);
+    const bool up = ve > s.e;  // the same for all
+    if (__any(top > s.m) || up) {
+        const float f = __builtin_amdgcn_exp2f(s.m - top);
+        const float fo = up ? f * __builtin_amdgcn_ldexpf(1.0f, max(s.e - ve, -200)) : f;
+        s.sum *= f;
+        s.m = top;
+        if (up) s.e = ve;
+#pragma unroll
+        for (int b = 0; b < DB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[b][i] *= fo;
+    }
+    const float sub = s.m - 14.0f;
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t[y][i] = __builtin_amdgcn_exp2f(fmaf(t[y][i], c, -sub));
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) s.sum += (t[y][i] + t[y][i + 1]) + (t[y][i + 2] + t[y][i + 3]);
+    }
+    if (ve < s.e) {
+        const float f = __builtin_amdgcn_ldexpf(1.0f, max(ve - s.e, -200));
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) t[y][i] *= f;
+    }
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+        float z[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = t[y >> 1][8 * (y & 1) + j];
+        // (ahead of the other wave of the SIMD, which is at its weights: utterances 157 -> 153 us)
+        if (y == 0) __builtin_amdgcn_s_setprio(1);
+        pa_u4 wh, wl;
+        pa_split(z, wh, wl, minus_one);
+        const pa_h8 whv = __builtin_bit_cast(pa_h8, wh), wlv = __builtin_bit_cast(pa_h8, wl);
+#pragma unroll
+        for (int b = 0; b < DB; ++b) {
+            const pa_h8 ah = vh[(y * DB + b) * 64], al = vl[(y * DB + b) * 64];
+            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, whv, o[b], 0, 0, 0);
+            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, wlv, o[b], 0, 0, 0);
+            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, whv, o[b], 0, 0, 0);
+        }
+    }
+    __builtin_amdgcn_s_setprio(0);
+    if (meta.odd) {  // values that are not finite go to the rows that see them
+        for (unsigned long long rest = meta.odd; rest; rest &= rest - 1) {
+            const int key = __ffsll((unsigned long long)rest) - 1;
+            const float* vp = a.v + (size_t)(x.k0 + kk + key) * a.v_stride + (size_t)x.head * HD + 4 * h;
+            if (key >= end || key < begin) continue;
+#pragma unroll
+            for (int b = 0; b < DB; ++b)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float4 f = *(const float4*)(vp + 32 * b + 8 * j);
+                    const float z[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!pa_finite(z[i])) o[b][4 * j + i] += z[i];
+                }
+        }
+    }
 }
 
 // Tiles go global -> LDS directly, the next one (of the next piece, too) while this one
@@ -419,7 +687,7 @@ __device__ __forceinline__ bool pa_next(const PaArgs& a, int n_seq, long long x0
 // run as they come, one's products beside the other's weights.
 template <int HD>
 __global__ __launch_bounds__(pa_tile_rows(HD) * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void vk_pattn(PaArgs a) {
-    constexpr int NW = pa_tile_rows(HD) / 32, KS = HD / 16, DB = HD / 32, P = pa_part(HD);
+    constexpr int NW = pa_tile_rows(HD) / 32, DB = HD / 32, P = pa_part(HD);
     constexpr int DMA = 8 * P / 1024 / NW;  // 1 KB loads of a tile a wave
     __shared__ __align__(16) _Float16 s_t[2][4 * P];  // K hi, K lo, V hi, V lo
     const int share = vk_xcd_tile(blockIdx.x, gridDim.x);
@@ -436,6 +704,7 @@ __global__ __launch_bounds__(pa_tile_rows(HD) * 2) __attribute__((amdgpu_waves_p
     p.head = __builtin_amdgcn_readfirstlane(st.head);
     p.slot = __builtin_amdgcn_readfirstlane(st.slot);
     p.line = st.line;
+    pa_lengths(a, p);
     const float minus_one = pa_minus_one();
     auto load = [&](const PaPiece& x, int u, int buffer) __attribute__((always_inline)) {
         const size_t tile = (size_t)(pa_k_slot(x.k0, x.seq) + x.lo + u) * a.hkv + x.head;
@@ -449,37 +718,8 @@ __global__ __launch_bounds__(pa_tile_rows(HD) * 2) __attribute__((amdgpu_waves_p
     int buffer = 0;
     for (bool more = true; more;) {
         const int rows = p.n * a.g;
-        // q of this lane's row: dims 16 ks + 8 h .., as two parts of q 2^-qe
-        const int wrow0 = p.row0 + wave * 32, r = min(wrow0 + l, rows - 1), qi = r / a.g;
-        const float* qp = a.q + (size_t)(p.q0 + qi) * a.q_stride + (size_t)(p.head * a.g + r - qi * a.g) * HD + 8 * h;
-        pa_u4 qh[KS], ql[KS];
-        int qe;
-        {
-            float x[KS][8], most = 0.0f;
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const float4 u = *(const float4*)(qp + 16 * s), w = *(const float4*)(qp + 16 * s + 4);
-                x[s][0] = u.x, x[s][1] = u.y, x[s][2] = u.z, x[s][3] = u.w;
-                x[s][4] = w.x, x[s][5] = w.y, x[s][6] = w.z, x[s][7] = w.w;
-            }
-#pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    x[s][j] *= a.sign;
-                    if (pa_finite(x[s][j])) most = fmaxf(most, fabsf(x[s][j]));
-                }
-            const int e = pa_exponent(pa_row_max(most));
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[s][j] = pa_scale(x[s][j], e);
-                pa_split(x[s], qh[s], ql[s], minus_one);
-            }
-            qe = e == kPaNoValue ? 0 : e;
-        }
-        const int pos = qi + (p.m - p.n);  // this lane's row
-        const int wpos0 = wrow0 / a.g + (p.m - p.n), wpos1 = min(wrow0 + 31, rows - 1) / a.g + (p.m - p.n);  // the wave's
+        PaWave<HD> w;
+        w.load(a, p, wave);
         vk_f32x16 o[DB];
 #pragma unroll
         for (int b = 0; b < DB; ++b)
@@ -489,129 +729,18 @@ __global__ __launch_bounds__(pa_tile_rows(HD) * 2) __attribute__((amdgpu_waves_p
         PaPiece next = p;
         for (int u = p.u0; u < p.u1; ++u) {
             const PaTileMeta mt = pa_meta(a.meta + (size_t)(pa_k_slot(p.k0, p.seq) + p.lo + u) * a.hkv + p.head);
-            const int ke = mt.k_exp, ve = mt.v_exp;
-            const unsigned long long odd = mt.odd;
             const int kk = (p.lo + u) * kPaKeys;  // its first key
-            // no row of the wave sees a key of this unit; some see not all
-            const bool none = wrow0 >= rows || kk >= p.m ||
-                              (a.causal && (kk > wpos1 || (a.window && kk + kPaKeys - 1 <= wpos0 - a.window)));
-            const bool some = kk + kPaKeys > p.m ||
-                              (a.causal && (kk + kPaKeys - 1 > wpos0 || (a.window && kk <= wpos1 - a.window)));
             vk_wait_vm<0>();
             VK_LDS_BARRIER();  // this tile has come, the one before has been read by all
             if (u + 1 < p.u1) {
                 load(p, u + 1, buffer ^ 1);
             } else {
-                next.line += next.units + kTileCost;
+                next.line += next.units + pa_cost(HD);
                 ++next.slot;
                 more = pa_next<HD>(a, n_seq, x0, x1, next);
                 if (more) load(next, next.u0, buffer ^ 1);
             }
-            if (!none) {
-                const pa_h8* kh = (const pa_h8*)s_t[buffer] + lane;
-                const pa_h8* kl = kh + P / 8;
-                const pa_h8* vh = kl + P / 8;
-                const pa_h8* vl = vh + P / 8;
-                constexpr vk_f32x16 zero = {};
-                vk_f32x16 t[2];
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    const pa_h8 qhv = __builtin_bit_cast(pa_h8, qh[ks]), qlv = __builtin_bit_cast(pa_h8, ql[ks]);
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const pa_h8 ah = kh[(x * KS + ks) * 64], al = kl[(x * KS + ks) * 64];
-                        t[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, qhv, ks ? t[x] : zero, 0, 0, 0);
-                        t[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, qlv, t[x], 0, 0, 0);
-                        t[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, qhv, t[x], 0, 0, 0);
-                    }
-                }
-                const int end = min(p.m, a.causal ? pos + 1 : p.m) - kk;               // the row sees keys below this,
-                const int begin = a.causal && a.window ? pos - a.window + 1 - kk : 0;  // from this on
-                // (kept above 0 and below infinity, which would make NaN of -inf and of 0)
-                const float c = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.c, qe + ke), 0x1p-126f), 0x1.fffffep127f);
-                if (some) {
-#pragma unroll
-                    for (int x = 0; x < 2; ++x)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int key = 32 * x + 8 * (i >> 2) + 4 * h + (i & 3);
-                            t[x][i] = key < end && key >= begin ? t[x][i] : -INFINITY;
-                        }
-                }
-                // (a median with infinity, kept from the compiler, is a maximum that takes the
-                // products' results as they come, where fmaxf would first quiet each)
-                float inf = INFINITY;
-                asm("" : "+s"(inf));
-                float most = -INFINITY;
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4)
-                        most = fmaxf(fmaxf(__builtin_amdgcn_fmed3f(t[x][i], t[x][i + 1], inf),
-                                           __builtin_amdgcn_fmed3f(t[x][i + 2], t[x][i + 3], inf)),
-                                     most);
-                const float top = fmaxf(ceilf(pa_row_max(most) * c), s.m);
-                const bool up = ve > s.e;  // the same for all
-                if (__any(top > s.m) || up) {
-                    const float f = __builtin_amdgcn_exp2f(s.m - top);
-                    const float fo = up ? f * __builtin_amdgcn_ldexpf(1.0f, max(s.e - ve, -200)) : f;
-                    s.sum *= f;
-                    s.m = top;
-                    if (up) s.e = ve;
-#pragma unroll
-                    for (int b = 0; b < DB; ++b)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[b][i] *= fo;
-                }
-                const float sub = s.m - 14.0f;
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) t[x][i] = __builtin_amdgcn_exp2f(fmaf(t[x][i], c, -sub));
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4) s.sum += (t[x][i] + t[x][i + 1]) + (t[x][i + 2] + t[x][i + 3]);
-                }
-                if (ve < s.e) {
-                    const float f = __builtin_amdgcn_ldexpf(1.0f, max(ve - s.e, -200));
-#pragma unroll
-                    for (int x = 0; x < 2; ++x)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) t[x][i] *= f;
-                }
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    float w[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) w[j] = t[x >> 1][8 * (x & 1) + j];
-                    pa_u4 wh, wl;
-                    pa_split(w, wh, wl, minus_one);
-                    const pa_h8 whv = __builtin_bit_cast(pa_h8, wh), wlv = __builtin_bit_cast(pa_h8, wl);
-#pragma unroll
-                    for (int b = 0; b < DB; ++b) {
-                        const pa_h8 ah = vh[(x * DB + b) * 64], al = vl[(x * DB + b) * 64];
-                        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, whv, o[b], 0, 0, 0);
-                        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, wlv, o[b], 0, 0, 0);
-                        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, whv, o[b], 0, 0, 0);
-                    }
-                }
-                if (odd) {  // values that are not finite go to the rows that see them
-                    for (unsigned long long rest = odd; rest; rest &= rest - 1) {
-                        const int key = __ffsll((unsigned long long)rest) - 1;
-                        const float* vp = a.v + (size_t)(p.k0 + kk + key) * a.v_stride + (size_t)p.head * HD + 4 * h;
-                        if (key >= end || key < begin) continue;
-#pragma unroll
-                        for (int b = 0; b < DB; ++b)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const float4 y = *(const float4*)(vp + 32 * b + 8 * j);
-                                const float z[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    if (!pa_finite(z[i])) o[b][4 * j + i] += z[i];
-                            }
-                    }
-                }
-            }
+            if (w.sees(kk)) pa_unit<HD>(a, p, w, s_t[buffer], mt, kk, o, s, minus_one);
             buffer ^= 1;
         }
         s.sum = pa_row_sum(s.sum);
@@ -629,7 +758,7 @@ __global__ __launch_bounds__(pa_tile_rows(HD) * 2) __attribute__((amdgpu_waves_p
                 ((vk_f32x4*)(part + (size_t)pa_tile_rows(HD) * HD))[wave * 32 + l] =
                     vk_f32x4{s.m, s.sum, __int_as_float(s.e), 0.0f};
             if (p.u0 == 0 && threadIdx.x == 0) {
-                const int last = (int)((p.line + kTileCost + p.units - 1) / size);  // the share with the last unit
+                const int last = (int)((p.line + pa_cost(HD) + p.units - 1) / size);  // the share with the last unit
                 a.open[share] = PaOpen{p.seq, p.head, p.slot, last - share + 1};
             }
         }
@@ -648,7 +777,7 @@ __global__ __launch_bounds__(pa_tile_rows(HD) * 2) void vk_pattn_join(PaArgs a) 
     if (open.pieces < 2) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 31;
     const int q0 = a.q_off[open.seq], rows = (a.q_off[open.seq + 1] - q0) * a.g;
-    const int row0 = (open.slot - pa_q_slot<HD>(a, q0, open.seq)) * pa_tile_rows(HD);
+    const int row0 = (open.slot - pa_q_slot<pa_tile_rows(HD)>(a, q0, open.seq)) * pa_tile_rows(HD);
     vk_f32x16 o[DB];
 #pragma unroll
     for (int b = 0; b < DB; ++b)
@@ -676,6 +805,53 @@ __global__ __launch_bounds__(pa_tile_rows(HD) * 2) void vk_pattn_join(PaArgs a) 
             for (int c = 0; c < 4; ++c) o[j >> 2][4 * (j & 3) + c] = o[j >> 2][4 * (j & 3) + c] * g0 + y[j][c] * g1;
     }
     pa_store_rows<HD>(a, q0, open.head, rows, row0, o, s.sum, s.e);
+}
+
+// ---- short sequences ----------------------------------------------------------------
+
+// Few units a tile: one launch, a workgroup a tile of 128 rows, whose threads pack each
+// tile of keys into LDS themselves. Nothing is planned, split or joined.
+constexpr int kShortRows = 128;
+
+template <int HD>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 2 : 1, HD == 64 ? 2 : 1))) void vk_pattn_short(PaArgs a) {
+    constexpr int DB = HD / 32;
+    __shared__ __align__(16) _Float16 s_t[4 * pa_part(HD)];
+    __shared__ PaSeqLds s_seq;
+    __shared__ PaPackLds s_lds;
+    const int slot = blockIdx.x;
+    PaPiece p;
+    p.head = blockIdx.y;
+    if (!pa_find(a, slot, s_seq, p, [&](int q0, int, int s) { return pa_q_slot<kShortRows>(a, q0, s); })) return;
+    const int rows = p.n * a.g;
+    p.row0 = (slot - pa_q_slot<kShortRows>(a, p.q0, p.seq)) * kShortRows;
+    if (p.row0 >= rows) return;
+    pa_span<kShortRows>(a, p.n, p.m, p.row0, &p.lo, &p.units);
+    const float minus_one = pa_minus_one();
+    PaPack<HD> t;
+    auto load = [&](int kk) __attribute__((always_inline)) {
+        t.load(a.k + (size_t)(p.k0 + kk) * a.k_stride + (size_t)p.head * HD, a.k_stride,
+               a.v + (size_t)(p.k0 + kk) * a.v_stride + (size_t)p.head * HD, a.v_stride, min(kPaKeys, p.m - kk));
+    };
+    int kk = p.lo * kPaKeys;
+    const int end = min(p.m, (p.lo + p.units) * kPaKeys);
+    if (kk < end) load(kk);
+    PaWave<HD> w;
+    w.load(a, p, threadIdx.x >> 6);
+    vk_f32x16 o[DB];
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
+    PaState s = {kNoMax, 0.0f, kPaNoValue};
+    while (kk < end) {
+        const PaTileMeta meta = t.store((pa_u4*)s_t, s_lds);  // (once all waves are through with the tile before)
+        VK_LDS_BARRIER();
+        if (w.sees(kk)) pa_unit<HD>(a, p, w, s_t, meta, kk, o, s, minus_one);
+        kk += kPaKeys;
+        if (kk < end) load(kk);
+    }
+    pa_store_rows<HD>(a, p.q0, p.head, rows, p.row0, o, pa_row_sum(s.sum), s.e);
 }
 
 // ---- few rows ----------------------------------------------------------------------
@@ -949,6 +1125,17 @@ hipError_t launch_pattn(hipStream_t s, int hd, const PaArgs& a) {
     if (rows <= kPaFewRows && (!a.causal || a.max_q == 1)) {
         if (hd == 64) return rows <= 16 ? go_few<64, 1>(s, a) : go_few<64, 2>(s, a);
         return rows <= 16 ? go_few<128, 1>(s, a) : go_few<128, 2>(s, a);
+    }
+    // short sequences, by one launch: at head size 64 up to 512 keys (16 of 512 keys, 20 heads:
+    // 83 us, 98 packed; 16 heads over 2: 68 and 61; three of up to 61: 8 and 17), at 128, where
+    // a workgroup has a CU to itself, up to 384 keys and two rounds of workgroups (four of up
+    // to 400, 16 heads over 2: 48 and 51; 16 of up to 400: 90 and 65; three of up to 61: 13 and 24)
+    const long long tiles = ((long long)a.q_rows * a.g / kShortRows + a.n_seq) * a.hkv;
+    if (hd == 64 ? a.max_k <= 512 : a.max_k <= 384 && tiles <= 512) {
+        const dim3 grid((unsigned)(tiles / a.hkv), (unsigned)a.hkv);
+        if (hd == 64) hipLaunchKernelGGL(vk_pattn_short<64>, grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL(vk_pattn_short<128>, grid, dim3(256), 0, s, a);
+        return hipGetLastError();
     }
     return hd == 64 ? go_pattn<64>(s, a) : go_pattn<128>(s, a);
 }

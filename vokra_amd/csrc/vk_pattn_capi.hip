@@ -70,7 +70,7 @@ int check_rows(const char* name, const float* x, size_t rows, size_t width, size
     if (!x) return ctx_fail(BAD, "packed_attn: %s is NULL", name);
     if (reinterpret_cast<uintptr_t>(x) % 16 != 0 || stride % 4 != 0)
         return ctx_fail(BAD, "packed_attn: rows of %s must be 16-byte aligned", name);
-    if (stride < width || stride > ((size_t)1 << 32))
+    if (stride < width || stride > ((size_t)1 << 23))
         return ctx_fail(BAD, "packed_attn: a row stride of %s is below its %zu values or too large", name, width);
     return VOKRA_HIP_OK;
 }
