@@ -24,10 +24,11 @@ struct BeamArgs {
     int *out_parents, *out_tokens, *out_ended;  // out_ended NULL: not written
     unsigned long long* keys;  // [row][slice][n_out]
     BeamStat* stats;           // [row][slice]
-    int groups, beams, vocab, n_out, end_token, slices;
+    int groups, beams, vocab, n_out, end_token;
+    int slices, group;  // set by the launcher: slices of a row, threads of a group
 };
 
 namespace vk {
-// slices is filled in here
+// slices and group are filled in here
 hipError_t launch_beam_select(hipStream_t s, BeamArgs a);
 }  // namespace vk

@@ -12,10 +12,10 @@
 // different beams are compared, and near ones have to fall in order), takes each
 // beam's best from its slices' lists and the group's from its beams'.
 //
-// The best of a slice without a sort of it: the n_out-th largest of the 256 threads' own
-// maxima bounds the n_out-th largest column from below, and hardly more than n_out columns
-// reach it. They are put into LDS and ranked by counting. Where too many do (ties), they
-// are taken one after the other.
+// The best of a slice without a sort of it: the threads fall into at least n_out groups,
+// and the least of the groups' maxima bounds the n_out-th largest column from below; a few
+// times as many columns as there are groups reach it. They are put into LDS and ranked by
+// counting. Where too many do (ties), they are taken one after the other.
 //
 // A logit that is NaN counts as -inf; a row with +inf has no continuations (its
 // log-softmax has no value). Sums do not depend on where a row lies in memory, so
@@ -26,7 +26,7 @@
 namespace vk {
 
 constexpr int BM_T = 256;     // threads of a slice
-constexpr int BM_CAND = 256;  // candidates that are ranked at once
+constexpr int BM_CAND = 512;  // candidates that are ranked at once
 constexpr int BM_MT = 512;    // threads of a merge: eight waves, a beam each in turn
 constexpr int BM_LIST = 1024; // entries of a beam's lists that a wave holds in LDS
 
@@ -42,13 +42,48 @@ __device__ __forceinline__ float bm_value(unsigned long long key) {
 }
 __device__ __forceinline__ int bm_column(unsigned long long key) { return (int)(0xffffffffu - (uint32_t)key); }
 
-__device__ __forceinline__ unsigned long long bm_wave_max(unsigned long long k) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const unsigned long long y = __shfl_xor(k, o, VK_WAVE);
-        k = y > k ? y : k;
+// The largest of the wave's keys, in every lane: partners by lane permutations in the VALU
+// (see vk_bfly_partner; the last two steps swap rows and halves), 6 steps of some 30 cycles
+// where ds_bpermute's take 150.
+template <int O>
+__device__ __forceinline__ unsigned long long bm_max_step(unsigned long long k) {
+    const uint32_t lo = (uint32_t)k, hi = (uint32_t)(k >> 32);
+    unsigned long long y;
+    if constexpr (O < 16) {
+        y = ((unsigned long long)(uint32_t)vk_bfly_partner<O>((int)hi) << 32) | (uint32_t)vk_bfly_partner<O>((int)lo);
+    } else if constexpr (O == 16) {
+        const auto a = __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
+        const auto b = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+        k = ((unsigned long long)b[0] << 32) | a[0];
+        y = ((unsigned long long)b[1] << 32) | a[1];
+    } else {
+        const auto a = __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+        const auto b = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+        k = ((unsigned long long)b[0] << 32) | a[0];
+        y = ((unsigned long long)b[1] << 32) | a[1];
     }
-    return k;
+    return y > k ? y : k;
+}
+__device__ __forceinline__ unsigned long long bm_wave_max(unsigned long long k) {
+    k = bm_max_step<1>(k);
+    k = bm_max_step<2>(k);
+    k = bm_max_step<4>(k);
+    k = bm_max_step<8>(k);
+    k = bm_max_step<16>(k);
+    return bm_max_step<32>(k);
+}
+
+// Doubles in the order of their bits, above 0 (0: none)
+__device__ __forceinline__ unsigned long long bm_order(double x) {
+    const unsigned long long b = (unsigned long long)__double_as_longlong(x);
+    return b >> 63 ? ~b : b | 0x8000000000000000ull;
+}
+
+// One step of the least of the groups' maxima: maxima within a group of `lanes`, least beyond
+template <int O>
+__device__ __forceinline__ float bm_bound_step(float v, int lanes) {
+    const float w = __int_as_float(vk_bfly_partner<O>(__float_as_int(v)));
+    return O < lanes ? fmaxf(v, w) : fminf(v, w);
 }
 
 // A row that goes on: not ended, with a score above -inf.
@@ -62,7 +97,7 @@ typedef float bm_f4 __attribute__((ext_vector_type(4), aligned(4)));
 template <int E>
 __global__ __launch_bounds__(BM_T) void vk_beam_slices(BeamArgs a) {
     constexpr int SLICE = BM_T * E;
-    __shared__ float s_max[4], s_sorted[4][64], s_bound;
+    __shared__ float s_max[4], s_bound[4];
     __shared__ double s_sum[4];
     __shared__ unsigned long long s_key[BM_CAND];
     __shared__ int s_n;
@@ -90,36 +125,20 @@ __global__ __launch_bounds__(BM_T) void vk_beam_slices(BeamArgs a) {
         if (y[j] == 0.0f) y[j] = 0.0f;  // one zero
         most = fmaxf(most, y[j]);
     }
-    // the wave's maxima in falling order over its lanes
-    float v = most;
-#pragma unroll
-    for (int k = 2; k <= 64; k <<= 1)
-#pragma unroll
-        for (int o = k >> 1; o > 0; o >>= 1) {
-            const float w = __shfl_xor(v, o, VK_WAVE);
-            const bool keeps_max = ((lane & o) == 0) == ((lane & k) == 0);
-            v = keeps_max ? fmaxf(v, w) : fminf(v, w);
-        }
-    s_sorted[wave][lane] = v;
-    if (lane == 0) s_max[wave] = v;
+    float v = bm_bound_step<1>(most, a.group);
+    v = bm_bound_step<2>(v, a.group);
+    v = bm_bound_step<4>(v, a.group);
+    v = bm_bound_step<8>(v, a.group);
+    v = bm_bound_step<16>(v, a.group);
+    v = bm_bound_step<32>(v, a.group);
+    const float top = vk_group_maxf<64>(most);
+    if (lane == 0) {
+        s_max[wave] = top;
+        s_bound[wave] = v;
+    }
     __syncthreads();
     const float m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-    // where v stands among all 256: of equal ones the lower wave's first
-    int rank = lane;
-#pragma unroll
-    for (int o = 1; o < 4; ++o) {
-        const int w = (wave + o) & 3;
-        int n = 0;  // of wave w stand before v
-#pragma unroll
-        for (int step = 32; step > 0; step >>= 1) {
-            const float u = s_sorted[w][n + step - 1];
-            if (u > v || (u == v && w < wave)) n += step;
-        }
-        const float u = s_sorted[w][n];  // n <= 63 here
-        if (u > v || (u == v && w < wave)) ++n;
-        rank += n;
-    }
-    if (rank == a.n_out - 1) s_bound = v;
+    const float bound = fminf(fminf(s_bound[0], s_bound[1]), fminf(s_bound[2], s_bound[3]));
     float sum = 0.0f;
     if (m > -INFINITY)
 #pragma unroll
@@ -128,8 +147,6 @@ __global__ __launch_bounds__(BM_T) void vk_beam_slices(BeamArgs a) {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o, VK_WAVE);
     if (lane == 0) s_sum[wave] = total;
-    __syncthreads();
-    const float bound = s_bound;
     if (most >= bound && most > -INFINITY) {
         int n = 0;
 #pragma unroll
@@ -146,8 +163,8 @@ __global__ __launch_bounds__(BM_T) void vk_beam_slices(BeamArgs a) {
     unsigned long long* out = a.keys + part * a.n_out;
     int count = s_n;
     if (count <= BM_CAND) {
-        if (t < count) {
-            const unsigned long long k = s_key[t];
+        for (int i = t; i < count; i += BM_T) {
+            const unsigned long long k = s_key[i];
             int before = 0;
             for (int j = 0; j < count; ++j) before += s_key[j] > k ? 1 : 0;
             if (before < a.n_out) out[before] = k;
@@ -176,8 +193,9 @@ __global__ __launch_bounds__(BM_T) void vk_beam_slices(BeamArgs a) {
     if (t == 0) a.stats[part] = BeamStat{(s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]), m, count};
 }
 
-// The n_out best of a beam's slices, by a wave: lists fall, so a lane looks at the heads
-// of its slices (s, s + 64, ..) and the wave takes the best head, n_out times.
+// The n_out best of a beam's slices, by a wave: lists fall, so a lane looks at the head
+// of its slices' lists (s, s + 64, ..) and the wave takes the best head, n_out times. The
+// beams' own lists fall too: the first wave takes the group's best from their heads likewise.
 __global__ __launch_bounds__(BM_MT) void vk_beam_merge(BeamArgs a) {
     constexpr int WAVES = BM_MT / 64;
     __shared__ unsigned long long s_list[WAVES][BM_LIST];
@@ -186,8 +204,16 @@ __global__ __launch_bounds__(BM_MT) void vk_beam_merge(BeamArgs a) {
     const int g = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = a.n_out;
     for (int b = wave; b < a.beams; b += WAVES) {
         const int row = g * a.beams + b;
+        const BeamStat* st = a.stats + (size_t)row * a.slices;
+        const unsigned long long* keys = a.keys + (size_t)row * a.slices * n;
+        // all that the beam may need, on its way at once (of a beam that has ended it is not read)
+        BeamStat first = {0.0, -INFINITY, 0};
+        if (lane < a.slices) first = st[lane];
+        const bool staged = a.slices * n <= BM_LIST;
+        if (staged)
+            for (int i = lane; i < a.slices * n; i += 64) s_list[wave][i] = keys[i];
         const float score = a.scores[row];
-        const bool ended = a.ended && a.ended[row], live = bm_live(a, row);
+        const bool ended = a.ended && a.ended[row], live = !ended && score > -INFINITY;
         if (lane == 0) s_ended[b] = ended;
         if (!live) {
             if (lane == 0) {
@@ -197,19 +223,13 @@ __global__ __launch_bounds__(BM_MT) void vk_beam_merge(BeamArgs a) {
             }
             continue;
         }
-        const BeamStat* st = a.stats + (size_t)row * a.slices;
-        const unsigned long long* keys = a.keys + (size_t)row * a.slices * n;
-        const bool staged = a.slices * n <= BM_LIST;
-        if (staged) {
-            for (int i = lane; i < a.slices * n; i += 64) s_list[wave][i] = keys[i];
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own list: no barrier
-        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own list: no barrier
         auto key = [&](int s, int i) { return staged ? s_list[wave][s * n + i] : keys[(size_t)s * n + i]; };
-        float m = -INFINITY;
-        for (int s = lane; s < a.slices; s += 64) m = fmaxf(m, st[s].max);
+        float m = first.max;
+        for (int s = lane + 64; s < a.slices; s += 64) m = fmaxf(m, st[s].max);
         m = vk_group_maxf<64>(m);
-        double sum = 0.0;
-        for (int s = lane; s < a.slices; s += 64)
+        double sum = first.max > -INFINITY ? first.sum * exp((double)first.max - (double)m) : 0.0;
+        for (int s = lane + 64; s < a.slices; s += 64)
             if (st[s].max > -INFINITY) sum += st[s].sum * exp((double)st[s].max - (double)m);
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, VK_WAVE);
@@ -220,7 +240,7 @@ __global__ __launch_bounds__(BM_MT) void vk_beam_merge(BeamArgs a) {
         auto next = [&]() {
             mine = 0;
             if (a.slices <= 64) {  // one list a lane
-                if (lane < a.slices && place < st[lane].count) mine = key(lane, place++);
+                if (place < first.count) mine = key(lane, place++);
                 return;
             }
             for (int s = lane; s < a.slices; s += 64) {
@@ -234,45 +254,39 @@ __global__ __launch_bounds__(BM_MT) void vk_beam_merge(BeamArgs a) {
             }
         };
         next();
+        unsigned long long got = 0;  // lane i: the i-th best
         for (; taken < n; ++taken) {
             const unsigned long long k = bm_wave_max(mine);
             if (!k) break;
-            const double total = (double)score + ((double)bm_value(k) - lse);
-            if (!(total > -INFINITY)) break;  // NaN: the row holds +inf
-            if (lane == 0) {
-                s_total[b][taken] = total;
-                s_token[b][taken] = bm_column(k);
-            }
+            if (lane == taken) got = k;
             last = k;
             if (mine == k) next();
         }
-        if (lane == 0) s_count[b] = taken;
+        const double total = (double)score + ((double)bm_value(got) - lse);
+        const bool there = lane < taken && total > -INFINITY;  // NaN: the row holds +inf
+        if (there) {
+            s_total[b][lane] = total;
+            s_token[b][lane] = bm_column(got);
+        }
+        if (lane == 0) s_count[b] = there ? taken : 0;
     }
     __syncthreads();
     if (wave != 0) return;
-    int at = 0;
     const int count = lane < a.beams ? s_count[lane] : 0;
+    int at = 0;
+    double total = count ? s_total[lane][0] : 0.0;
     for (int i = 0; i < n; ++i) {
-        double best = at < count ? s_total[lane][at] : -INFINITY;
-        int from = lane;
-#pragma unroll
-        for (int o = 1; o < kBeamMost; o <<= 1) {
-            const double w = __shfl_xor(best, o, VK_WAVE);
-            const int f = __shfl_xor(from, o, VK_WAVE);
-            if (w > best || (w == best && f < from)) {
-                best = w;
-                from = f;
-            }
-        }
-        const size_t o = (size_t)g * n + i;
-        if (lane == from && lane < kBeamMost) {  // (from is the same in lanes 0 .. 31)
+        const unsigned long long mine = at < count ? bm_order(total) : 0, best = bm_wave_max(mine);
+        const int from = __ffsll((unsigned long long)__ballot(mine == best)) - 1;  // the lowest beam
+        if (lane == from) {
+            const size_t o = (size_t)g * n + i;
             const bool any = at < count;
             const int token = any ? s_token[lane][at] : -1;
-            a.out_scores[o] = any ? (float)best : -INFINITY;
+            a.out_scores[o] = any ? (float)total : -INFINITY;
             a.out_parents[o] = any ? lane : -1;
             a.out_tokens[o] = token;
             if (a.out_ended) a.out_ended[o] = !any || s_ended[lane] || token == a.end_token ? 1 : 0;
-            ++at;
+            if (++at < count) total = s_total[lane][at];
         }
     }
 }
@@ -282,6 +296,9 @@ hipError_t launch_beam_select(hipStream_t s, BeamArgs a) {
     const bool small = (size_t)rows * a.vocab <= (size_t)512 * 4096;
     const int slice = small ? kBeamSlice : 2 * kBeamSlice;
     a.slices = (a.vocab + slice - 1) / slice;
+    int groups = 4;  // of threads of a slice
+    while (groups < a.n_out) groups *= 2;
+    a.group = BM_T / groups;
     const dim3 grid((unsigned)a.slices, (unsigned)rows);
     if (small) hipLaunchKernelGGL(vk_beam_slices<16>, grid, dim3(BM_T), 0, s, a);
     else hipLaunchKernelGGL(vk_beam_slices<32>, grid, dim3(BM_T), 0, s, a);
