@@ -33,7 +33,8 @@ constexpr int BM_LIST = 1024; // entries of a beam's lists that a wave holds in 
 // Values in the order of their bits, a column index that falls with it behind: the larger
 // key is the better column. Key 0: none.
 __device__ __forceinline__ unsigned long long bm_key(float x, int column) {
-    const uint32_t b = __float_as_uint(x), ord = b & 0x80000000u ? ~b : b | 0x80000000u;
+    const uint32_t b = __float_as_uint(x + 0.0f);  // one zero
+    const uint32_t ord = b & 0x80000000u ? ~b : b | 0x80000000u;
     return ((unsigned long long)ord << 32) | (0xffffffffu - (uint32_t)column);
 }
 __device__ __forceinline__ float bm_value(unsigned long long key) {
@@ -86,6 +87,9 @@ __device__ __forceinline__ float bm_bound_step(float v, int lanes) {
     return O < lanes ? fmaxf(v, w) : fminf(v, w);
 }
 
+// x, -inf for NaN (a maximum passes over NaN)
+__device__ __forceinline__ float bm_number(float x) { return fmaxf(x, -INFINITY); }
+
 // A row that goes on: not ended, with a score above -inf.
 __device__ __forceinline__ bool bm_live(const BeamArgs& a, int row) {
     return !(a.ended && a.ended[row]) && a.scores[row] > -INFINITY;
@@ -110,7 +114,7 @@ __global__ __launch_bounds__(BM_T) void vk_beam_slices(BeamArgs a) {
     for (int j = 0; j < E / 4; ++j) {
         const int c = c0 + 4 * (t + BM_T * j);
         if (c + 3 < a.vocab) {
-            const bm_f4 v = __builtin_nontemporal_load((const bm_f4*)(x + c));
+            const bm_f4 v = *(const bm_f4*)(x + c);
             y[4 * j] = v.x, y[4 * j + 1] = v.y, y[4 * j + 2] = v.z, y[4 * j + 3] = v.w;
         } else {
 #pragma unroll
@@ -118,12 +122,13 @@ __global__ __launch_bounds__(BM_T) void vk_beam_slices(BeamArgs a) {
         }
     }
     if (t == 0) s_n = 0;
-    float most = -INFINITY;
+    float most = -INFINITY, four[E / 4];  // and of each run of four
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-        if (!(y[j] == y[j])) y[j] = -INFINITY;
-        if (y[j] == 0.0f) y[j] = 0.0f;  // one zero
-        most = fmaxf(most, y[j]);
+    for (int j = 0; j < E / 4; ++j) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[4 * j + i] = bm_number(y[4 * j + i]);
+        four[j] = fmaxf(fmaxf(y[4 * j], y[4 * j + 1]), fmaxf(y[4 * j + 2], y[4 * j + 3]));
+        most = fmaxf(most, four[j]);
     }
     float v = bm_bound_step<1>(most, a.group);
     v = bm_bound_step<2>(v, a.group);
@@ -139,25 +144,34 @@ __global__ __launch_bounds__(BM_T) void vk_beam_slices(BeamArgs a) {
     __syncthreads();
     const float m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
     const float bound = fminf(fminf(s_bound[0], s_bound[1]), fminf(s_bound[2], s_bound[3]));
+    // e^(x - m) = 2^(x l - m l), l = log2 e: one fma and one exponential a column. m l is rounded,
+    // by r, the same for all: the sum is multiplied by 2^-r at the end
+    constexpr float l = 1.44269504088896340736f;
+    const bool near = fabsf(m) < 16384.0f;
+    const float ml = near ? m * l : 0.0f, r = near ? fmaf(m, l, -ml) : 0.0f;
     float sum = 0.0f;
-    if (m > -INFINITY)
+    if (near) {
 #pragma unroll
-        for (int j = 0; j < E; ++j) sum += __builtin_amdgcn_exp2f((y[j] - m) * 1.44269504088896340736f);
+        for (int j = 0; j < E; ++j) sum += __builtin_amdgcn_exp2f(fmaf(y[j], l, -ml));
+    } else if (m > -INFINITY) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) sum += __builtin_amdgcn_exp2f((y[j] - m) * l);
+    }
     double total = (double)sum;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o, VK_WAVE);
     if (lane == 0) s_sum[wave] = total;
-    if (most >= bound && most > -INFINITY) {
-        int n = 0;
+    const float from = fmaxf(bound, -0x1.fffffep127f);  // (what is -inf is none)
+    if (__any(most >= from))
 #pragma unroll
-        for (int j = 0; j < E; ++j) n += y[j] >= bound && y[j] > -INFINITY ? 1 : 0;
-        int at = atomicAdd(&s_n, n);
-        if (at + n <= BM_CAND)
+        for (int j = 0; j < E / 4; ++j)
+            if (four[j] >= from)
 #pragma unroll
-            for (int j = 0; j < E; ++j)
-                if (y[j] >= bound && y[j] > -INFINITY)
-                    s_key[at++] = bm_key(y[j], c0 + 4 * (t + BM_T * (j >> 2)) + (j & 3));
-    }
+                for (int i = 0; i < 4; ++i)
+                    if (y[4 * j + i] >= from) {
+                        const int at = atomicAdd(&s_n, 1);
+                        if (at < BM_CAND) s_key[at] = bm_key(y[4 * j + i], c0 + 4 * (t + BM_T * j) + i);
+                    }
     __syncthreads();
     const size_t part = (size_t)row * a.slices + blockIdx.x;
     unsigned long long* out = a.keys + part * a.n_out;
@@ -166,6 +180,7 @@ __global__ __launch_bounds__(BM_T) void vk_beam_slices(BeamArgs a) {
         for (int i = t; i < count; i += BM_T) {
             const unsigned long long k = s_key[i];
             int before = 0;
+#pragma unroll 8
             for (int j = 0; j < count; ++j) before += s_key[j] > k ? 1 : 0;
             if (before < a.n_out) out[before] = k;
         }
@@ -190,7 +205,11 @@ __global__ __launch_bounds__(BM_T) void vk_beam_slices(BeamArgs a) {
             last = k;
         }
     }
-    if (t == 0) a.stats[part] = BeamStat{(s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]), m, count};
+    if (t == 0) {
+        const double x = -0.69314718055994530942 * (double)r;  // below 2^-9: three terms are 2^-40
+        const double all = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+        a.stats[part] = BeamStat{all * (1.0 + x * (1.0 + x * (0.5 + x * 0.16666666666666667))), m, count};
+    }
 }
 
 // The n_out best of a beam's slices, by a wave: lists fall, so a lane looks at the head
@@ -199,8 +218,9 @@ __global__ __launch_bounds__(BM_T) void vk_beam_slices(BeamArgs a) {
 __global__ __launch_bounds__(BM_MT) void vk_beam_merge(BeamArgs a) {
     constexpr int WAVES = BM_MT / 64;
     __shared__ unsigned long long s_list[WAVES][BM_LIST];
+    __shared__ unsigned long long s_some[WAVES][128], s_best[WAVES][64], s_order[BM_MT];
     __shared__ double s_total[kBeamMost][kBeamOut];
-    __shared__ int s_token[kBeamMost][kBeamOut], s_count[kBeamMost], s_ended[kBeamMost];
+    __shared__ int s_rank[BM_MT], s_token[kBeamMost][kBeamOut], s_count[kBeamMost], s_ended[kBeamMost];
     const int g = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = a.n_out;
     for (int b = wave; b < a.beams; b += WAVES) {
         const int row = g * a.beams + b;
@@ -234,8 +254,46 @@ __global__ __launch_bounds__(BM_MT) void vk_beam_merge(BeamArgs a) {
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, VK_WAVE);
         const double lse = (double)m + log(sum);
-        // the best key of a lane's slices that is not taken yet
-        int taken = 0, place = 0;
+        int taken = 0;
+        unsigned long long got = 0;  // lane i: the i-th best
+        bool few = false;
+        if (staged && a.slices <= 64) {
+            // the c-th entries of all lists, c n_out / slices: at least n_out entries reach the least of
+            // them, and seldom more than 128: each of those is ranked by counting
+            const int c = (n + a.slices - 1) / a.slices - 1;
+            unsigned long long bound = lane < a.slices ? (c < first.count ? s_list[wave][lane * n + c] : 0) : ~0ull;
+            bound = ~bm_wave_max(~bound);
+            int found = 0;
+            for (int i = lane; i < (a.slices * n + 63) / 64 * 64; i += 64) {
+                const int s = i / n;
+                const unsigned long long k =
+                    i < a.slices * n && i - s * n < __shfl(first.count, s & 63, VK_WAVE) ? s_list[wave][i] : 0;
+                const uint64_t m1 = __ballot(k && k >= bound);
+                const int at = found + __popcll(m1 & ((1ull << lane) - 1));
+                if (k && k >= bound && at < 128) s_some[wave][at] = k;
+                found += __popcll(m1);
+            }
+            few = found <= 128;
+            if (few) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                const unsigned long long k0 = lane < found ? s_some[wave][lane] : 0,
+                                         k1 = lane + 64 < found ? s_some[wave][lane + 64] : 0;
+                int b0 = 0, b1 = 0;
+#pragma unroll 8
+                for (int i = 0; i < found; ++i) {
+                    const unsigned long long y = s_some[wave][i];
+                    b0 += (int)(y > k0);
+                    b1 += (int)(y > k1);
+                }
+                taken = min(found, n);
+                if (k0 && b0 < n) s_best[wave][b0] = k0;
+                if (k1 && b1 < n) s_best[wave][b1] = k1;
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                got = lane < taken ? s_best[wave][lane] : 0;
+            }
+        }
+        // else the best key of a lane's slices that is not taken yet, again and again
+        int place = 0;
         unsigned long long last = ~0ull, mine = 0;
         auto next = [&]() {
             mine = 0;
@@ -253,14 +311,14 @@ __global__ __launch_bounds__(BM_MT) void vk_beam_merge(BeamArgs a) {
                 }
             }
         };
-        next();
-        unsigned long long got = 0;  // lane i: the i-th best
-        for (; taken < n; ++taken) {
+        if (!few) next();
+        while (!few && taken < n) {
             const unsigned long long k = bm_wave_max(mine);
             if (!k) break;
             if (lane == taken) got = k;
             last = k;
             if (mine == k) next();
+            ++taken;
         }
         const double total = (double)score + ((double)bm_value(got) - lse);
         const bool there = lane < taken && total > -INFINITY;  // NaN: the row holds +inf
@@ -271,6 +329,40 @@ __global__ __launch_bounds__(BM_MT) void vk_beam_merge(BeamArgs a) {
         if (lane == 0) s_count[b] = there ? taken : 0;
     }
     __syncthreads();
+    auto put = [&](int i, int b, int at, bool any) {
+        const size_t o = (size_t)g * n + i;
+        const int token = any ? s_token[b][at] : -1;
+        a.out_scores[o] = any ? (float)s_total[b][at] : -INFINITY;
+        a.out_parents[o] = any ? b : -1;
+        a.out_tokens[o] = token;
+        if (a.out_ended) a.out_ended[o] = !any || s_ended[b] || token == a.end_token ? 1 : 0;
+    };
+    if (a.beams * n <= BM_MT) {
+        // every entry ranked by counting, of equal totals the lower place first; as many threads
+        // an entry as there are, a share of the others each
+        const int t = threadIdx.x, entries = a.beams * n, parts = BM_MT / entries, e = t % entries, part = t / entries;
+        const int b = e / n, at = e - b * n;
+        const bool any = at < s_count[b];
+        const unsigned long long mine = any ? bm_order(s_total[b][at]) : 0;
+        if (part == 0) {
+            s_order[e] = mine;
+            s_rank[e] = 0;
+        }
+        const int all = __syncthreads_count(any && part == 0);
+        int before = 0;
+        if (part < parts && any)
+#pragma unroll 4
+            for (int i = part; i < entries; i += parts) {
+                const unsigned long long y = s_order[i];
+                before += (int)(y > mine) + (int)((y == mine) & (i < e));
+            }
+        if (before) atomicAdd(&s_rank[e], before);
+        __syncthreads();
+        before = s_rank[e];
+        if (part == 0 && any && before < n) put(before, b, at, true);
+        if (t >= all && t < n) put(t, 0, 0, false);
+        return;
+    }
     if (wave != 0) return;
     const int count = lane < a.beams ? s_count[lane] : 0;
     int at = 0;
@@ -279,13 +371,7 @@ __global__ __launch_bounds__(BM_MT) void vk_beam_merge(BeamArgs a) {
         const unsigned long long mine = at < count ? bm_order(total) : 0, best = bm_wave_max(mine);
         const int from = __ffsll((unsigned long long)__ballot(mine == best)) - 1;  // the lowest beam
         if (lane == from) {
-            const size_t o = (size_t)g * n + i;
-            const bool any = at < count;
-            const int token = any ? s_token[lane][at] : -1;
-            a.out_scores[o] = any ? (float)total : -INFINITY;
-            a.out_parents[o] = any ? lane : -1;
-            a.out_tokens[o] = token;
-            if (a.out_ended) a.out_ended[o] = !any || s_ended[lane] || token == a.end_token ? 1 : 0;
+            put(i, lane, at, at < count);
             if (++at < count) total = s_total[lane][at];
         }
     }
