@@ -1581,8 +1581,8 @@ namespace vk {
 // Beams that keep their rows, or name no beam, cost nothing. Bound by memory: each
 // source once (a stream that several beams take comes from cache), each changed
 // stream once, past the caches: two of five streams of twelve groups of 100 .. 447 rows,
-// 20 heads of 64, eight layers (143 MB read and written each) take 40 us, 88 through the
-// caches; four pages a workgroup, two in flight, 43. Five streams of 301 rows of 2 heads
+// 20 heads of 64, eight layers (143 MB read and written each) take 49 us, 88 through the
+// caches; four pages a workgroup, two in flight, 52. Five streams of 301 rows of 2 heads
 // of 128 in four layers take 3 us.
 // NB: at least the beams of a group.
 template <int NB>

@@ -864,11 +864,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
 //   its accumulators (keys 4 (lane / 16) + i of row lane % 16) are the operand of
 //   O^T [16 dims][16 rows], step i, whose other one are 16 bytes of V row 4 (lane / 16) + i:
 //     dims 4 (lane % 16) + j, four products.
-// A wave takes KU keys at a time of its workgroup's range, with an online softmax of its
+// A wave takes 16 keys at a time of its workgroup's range, with an online softmax of its
 // own; the four merge through LDS, ranges by vk_pattn_few_join. A step's K goes on its way
-// when the products of the step before have taken theirs, V likewise.
-constexpr int kFewMost = 4096;  // workgroups that leave partial results
-constexpr int few_keys(int hd, int nt) { return 64 * 64 / hd / nt; }  // KU: 128 registers of K and V at most
+// when the products of the step before have taken theirs, V likewise; steps of 16 keys
+// leave room for four waves a SIMD (of 64 and 32, with two and three waves: 44 and 39 us).
+// Bound by the reads of K and V: five rows each against 16 sequences of 97 to 1500 keys, 20
+// heads of 64, 131 MB, take 39 us with the join from memory (3.4 TB/s). Neighbouring
+// workgroups are the heads of the same keys, so that whole rows of K and V are on their
+// way (ranges of one head: 44 against 41 us), and the reads go through the caches: K and V
+// that stay in the last one from step to step take 31 us, 36 past them (from memory 39
+// and 38).
+constexpr int kFewMost = 2048;  // workgroups that leave partial results
+constexpr int kFewKeys = 16;  // of a wave's step
 
 __device__ __forceinline__ float pa_row4_max(float v) {  // over the lanes l % 16 alike
     const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -885,21 +892,23 @@ __device__ __forceinline__ int pa_few_begin(const PaArgs& a, int m) {
     return a.causal && a.window ? max(0, m - a.window) : 0;
 }
 
+constexpr int few_waves(int hd, int nt) { return hd * nt == 64 ? 4 : hd * nt == 128 ? 3 : 2; }  // what K, V, q and o leave
+
 template <int HD, int NT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void vk_pattn_few(PaArgs a, int per) {
-    constexpr int KU = few_keys(HD, NT), CH = KU / 16, QC = HD / 16, DD = HD / 64;
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_waves(HD, NT)))) void vk_pattn_few(PaArgs a, int per) {
+    constexpr int KU = kFewKeys, QC = HD / 16, DD = HD / 64;
     __shared__ int s_first;
     __shared__ float s_m[4][16 * NT], s_l[4][16 * NT];
     __shared__ vk_f32x4 s_o[4][16 * NT][HD / 4];
-    const int seq = blockIdx.z, head = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6, g = lane >> 4,
+    const int seq = blockIdx.z, head = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6, g = lane >> 4,
               l = lane & 15;
     const int n_ok = pa_in_order(a, &s_first);
     if (seq >= n_ok) return;
     const int q0 = a.q_off[seq], n = a.q_off[seq + 1] - q0, k0 = a.k_off[seq], m = a.k_off[seq + 1] - k0;
     const int rows = n * a.g;
     if (rows == 0 || rows > 16 * NT) return;
-    const int begin = pa_few_begin(a, m) + (int)blockIdx.x * per, end = min(begin + per, m);
-    if (blockIdx.x && begin >= m) return;
+    const int begin = pa_few_begin(a, m) + (int)blockIdx.y * per, end = min(begin + per, m);
+    if (blockIdx.y && begin >= m) return;
     vk_f32x4 q[NT][QC];
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
@@ -921,24 +930,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void v
     }
     const float* kp = a.k + (size_t)k0 * a.k_stride + (size_t)head * HD + 4 * g;
     const float* vp = a.v + (size_t)k0 * a.v_stride + (size_t)head * HD + 4 * l;
-    vk_f32x4 k[CH][QC], v[CH][4][DD];
+    vk_f32x4 k[QC], v[4][DD];
     auto load_k = [&](int key) __attribute__((always_inline)) {
+        const float* p = kp + (size_t)min(key + l, m - 1) * a.k_stride;
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const float* p = kp + (size_t)min(key + 16 * c + l, m - 1) * a.k_stride;
-#pragma unroll
-            for (int x = 0; x < QC; ++x) k[c][x] = __builtin_nontemporal_load((const vk_f32x4*)(p + 16 * x));
-        }
+        for (int x = 0; x < QC; ++x) k[x] = *(const vk_f32x4*)(p + 16 * x);
     };
     auto load_v = [&](int key) __attribute__((always_inline)) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
+        for (int i = 0; i < 4; ++i) {
+            const float* p = vp + (size_t)min(key + 4 * g + i, m - 1) * a.v_stride;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float* p = vp + (size_t)min(key + 16 * c + 4 * g + i, m - 1) * a.v_stride;
-#pragma unroll
-                for (int d = 0; d < DD; ++d) v[c][i][d] = __builtin_nontemporal_load((const vk_f32x4*)(p + 64 * d));
-            }
+            for (int d = 0; d < DD; ++d) v[i][d] = *(const vk_f32x4*)(p + 64 * d);
+        }
     };
     int key = begin + wave * KU;
     if (key < end) {
@@ -947,45 +951,37 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void v
     }
     for (; key < end; key += 4 * KU) {
         const int next = key + 4 * KU;
-        vk_f32x4 s[NT][CH];
+        vk_f32x4 s[NT];
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
-#pragma unroll
-            for (int c = 0; c < CH; ++c) s[x][c] = vk_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int x = 0; x < NT; ++x) s[x] = vk_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int y = 0; y < QC; ++y)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int c = 0; c < CH; ++c)
-#pragma unroll
-                    for (int x = 0; x < NT; ++x)
-                        s[x][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c][y][j], q[x][y][j], s[x][c], 0, 0, 0);
+                for (int x = 0; x < NT; ++x)
+                    s[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[y][j], q[x][y][j], s[x], 0, 0, 0);
         if (next < end) load_k(next);
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
             float most = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < CH; ++c)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float y = s[x][c][i];
-                    y = y > -INFINITY ? y : __builtin_nanf("");  // of a key that is not finite
-                    y = key + 16 * c + 4 * g + i < end ? y : -INFINITY;
-                    s[x][c][i] = y;
-                    most = fmaxf(most, y);
-                }
+            for (int i = 0; i < 4; ++i) {
+                float y = s[x][i];
+                y = y > -INFINITY ? y : __builtin_nanf("");  // of a key that is not finite
+                y = key + 4 * g + i < end ? y : -INFINITY;
+                s[x][i] = y;
+                most = fmaxf(most, y);
+            }
             const float top = fmaxf(pa_row4_max(most), mx[x]);
             const float f = __builtin_amdgcn_exp2f(mx[x] - top);
             mx[x] = top;
             float add = 0.0f;
 #pragma unroll
-            for (int c = 0; c < CH; ++c)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[x][c][i] = __builtin_amdgcn_exp2f(s[x][c][i] - top);
-                    add += s[x][c][i];
-                }
+            for (int i = 0; i < 4; ++i) {
+                s[x][i] = __builtin_amdgcn_exp2f(s[x][i] - top);
+                add += s[x][i];
+            }
             sum[x] = sum[x] * f + add;
 #pragma unroll
             for (int d = 0; d < DD; ++d)
@@ -993,16 +989,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void v
                 for (int j = 0; j < 4; ++j) o[x][d][j] *= f;
         }
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int d = 0; d < DD; ++d)
 #pragma unroll
-                for (int d = 0; d < DD; ++d)
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int x = 0; x < NT; ++x)
-                            o[x][d][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[c][i][d][j], s[x][c][i], o[x][d][j], 0, 0, 0);
+                    for (int x = 0; x < NT; ++x)
+                        o[x][d][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][d][j], s[x][i], o[x][d][j], 0, 0, 0);
         if (next < end) load_v(next);
     }
     // o[x][d][j][i]: row 16 x + l, dim 64 d + 4 (4 g + i) + j
@@ -1022,7 +1016,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void v
     }
     __syncthreads();
     const int ranges = max(1, (m - pa_few_begin(a, m) + per - 1) / per);
-    float* part = a.part + (((size_t)seq * a.hkv + head) * gridDim.x + blockIdx.x) * (16 * NT) * (HD + 4);
+    float* part = a.part + (((size_t)seq * a.hkv + head) * gridDim.y + blockIdx.y) * (16 * NT) * (HD + 4);
     for (int y = t; y < rows * (HD / 4); y += 256) {
         const int r = y / (HD / 4), d = y % (HD / 4);
         float top = s_m[0][r];
@@ -1090,15 +1084,15 @@ __global__ __launch_bounds__(256) void vk_pattn_few_join(PaArgs a, int per, int 
 
 template <int HD, int NT>
 static hipError_t go_few(hipStream_t s, const PaArgs& a) {
-    // ranges of a step of all four waves at least, for up to 2048 workgroups if all sequences
+    // ranges of a step of all four waves at least, for up to kFewMost workgroups if all sequences
     // were the longest
-    constexpr int step = 4 * few_keys(HD, NT);
+    constexpr int step = 4 * kFewKeys;
     const long long pairs = (long long)a.n_seq * a.hkv;
     const int keys = a.causal && a.window ? std::min(a.max_k, a.window) : a.max_k;
-    const long long most = std::max<long long>(1, std::min<long long>(kFewMost, 2048) / pairs);
+    const long long most = std::max<long long>(1, kFewMost / pairs);
     const int per = (int)std::max<long long>(step, ((keys + most - 1) / most + step - 1) / step * step);
     const int splits = keys ? (keys + per - 1) / per : 1;
-    hipLaunchKernelGGL((vk_pattn_few<HD, NT>), dim3((unsigned)splits, (unsigned)a.hkv, (unsigned)a.n_seq), dim3(256), 0, s, a,
+    hipLaunchKernelGGL((vk_pattn_few<HD, NT>), dim3((unsigned)a.hkv, (unsigned)splits, (unsigned)a.n_seq), dim3(256), 0, s, a,
                        per);
     if (splits > 1)
         hipLaunchKernelGGL((vk_pattn_few_join<HD, NT>), dim3((unsigned)a.hkv, (unsigned)a.n_seq), dim3(256), 0, s, a, per,
