@@ -127,6 +127,10 @@ def test_device_items_that_name_nothing_are_passed_over_and_graphs(ctx):
     kv.reorder_dev(3, 3, d_ids, d_par, d_len, t)
     ctx.synchronize()
     assert np.array_equal(held(kv, 2, n, t), want)
+    put(ids, [[1, 2, 0], [1, 0, 0], [2, 0, 1]], [-2 ** 31, -2 ** 31 + 8, -1])  # below zero by as much as there is
+    kv.reorder_dev(3, 3, d_ids, d_par, d_len, t)
+    ctx.synchronize()
+    assert np.array_equal(held(kv, 2, n, t), want)
     graph = ctx.capture(lambda: kv.reorder_dev(3, 3, d_ids, d_par, d_len, t))
     for _ in range(3):
         par, lens = g.integers(-1, 3, (3, 3)), g.integers(0, t + 1, 3)

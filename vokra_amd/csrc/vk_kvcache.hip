@@ -1593,8 +1593,9 @@ __global__ __launch_bounds__(256) void vk_kv_reorder(KvDev c, int beams, const i
     const int g = blockIdx.z, layer = layer0 + (int)blockIdx.y, bx = blockIdx.x / chunks;
     const int block = block0 + bx, chunk = blockIdx.x - bx * chunks;
     const int len = lens[g], pid = c.table[layer * c.ppl + block];
+    if ((unsigned)len > (unsigned)max_len || (unsigned)pid >= (unsigned)c.cap) return;
     const int rows = min(len - block * c.bs, c.bs);
-    if (len > max_len || rows <= 0 || (unsigned)pid >= (unsigned)c.cap) return;
+    if (rows <= 0) return;
     if (threadIdx.x < 64) {
         const int b = threadIdx.x;
         const int p = b < beams ? parents[(size_t)g * beams + b] : -1;
