@@ -351,7 +351,8 @@ int vokra_hip_attn_f32_dev(vokra_hip_ctx_t *ctx, size_t batch, size_t t_q, size_
  * sees none. Query head h reads kv head h / (n_head_q / n_head_kv). f32 in and out: each
  * product runs as three fp16 products of two parts of both operands (22 bits), each
  * operand under a power of two (a query row's, a tile of 64 keys' for a kv head), so
- * results do not depend on the values' size; sums in f32. How a row's keys are split
+ * results do not depend on the values' size; of few rows (max_q * n_head_q / n_head_kv <=
+ * 32, max_q 1 if causal) in f32 as they are. Sums in f32. How a row's keys are split
  * depends on the whole call, and its last f32 bits may with it. A key row or query
  * row with a value that is not finite makes rows that see it NaN; a value of V that is
  * not finite makes its column of those rows not finite; rows that do not see it are not
