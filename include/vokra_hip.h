@@ -351,8 +351,9 @@ int vokra_hip_attn_f32_dev(vokra_hip_ctx_t *ctx, size_t batch, size_t t_q, size_
  * sees none. Query head h reads kv head h / (n_head_q / n_head_kv). f32 in and out: each
  * product runs as three fp16 products of two parts of both operands (22 bits), each
  * operand under a power of two (a query row's, a tile of 64 keys' for a kv head), so
- * results do not depend on the values' size; of few rows (max_q * n_head_q / n_head_kv <=
- * 32, max_q 1 if causal) in f32 as they are. Sums in f32. How a row's keys are split
+ * results do not depend on the values' size (a value is held to 2^-37 of its row's or
+ * tile's largest at least); of few rows (max_q * n_head_q / n_head_kv <= 32, max_q 1 if
+ * causal) in f32 as they are. Sums in f32. How a row's keys are split
  * depends on the whole call, and its last f32 bits may with it. A key row or query
  * row with a value that is not finite makes rows that see it NaN; a value of V that is
  * not finite makes its column of those rows not finite; rows that do not see it are not
@@ -660,7 +661,7 @@ int vokra_hip_rope_apply(vokra_hip_ctx_t *ctx, const vokra_hip_rope_t *rope, siz
  * turned; the values beyond rot_dim are normed too. gamma: head_dim values for all
  * heads of a side (stride 0), or a row for each head, stride floats apart (at least
  * head_dim); NULL: ones. No counterpart in the reference (its heads have no norms).
- * Everything else as in rope_apply; gammas overlap no output. */
+ * All in f32, the squares too. Everything else as in rope_apply; gammas overlap no output. */
 typedef struct vokra_hip_head_norm {
     const float *q_gamma, *k_gamma;
     size_t q_gamma_stride, k_gamma_stride;

@@ -121,6 +121,23 @@ def test_keys_split_over_workgroups(ctx, hq, hkv, hd, ql, kl, causal, window):
     check(got, *attend(q, k, v, ql, kl, hq, hkv, hd ** -0.5, causal, window))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,hd,ql,kl,causal,window", [
+    (1024, 1, 64, [2, 0, 1], [70, 5, 9], True, 0), (1024, 1024, 64, [2, 1], [65, 1], False, 0),
+    (512, 2, 128, [5], [66], True, 3), (1024, 4, 128, [1, 2], [900, 1], True, 0),
+    (2, 2, 128, [1] * 1023 + [300], [3] * 1023 + [300], True, 0), (2, 1, 64, [0] * 1000 + [40] * 24, None, True, 0),
+    (2, 1, 64, [1, 0] * 512, [0, 3] * 512, False, 0)])
+def test_the_ends_of_the_ranges(ctx, hq, hkv, hd, ql, kl, causal, window):
+    """As many heads and sequences as a plan takes."""
+    print("[case] packed ends", hq, hkv, hd, len(ql), causal, window, flush=True)
+    kl = ql if kl is None else kl
+    g = np.random.default_rng(hq)
+    q, k, v = rows(g, sum(ql), sum(kl), hq, hkv, hd)
+    plan = ctx.packed_attn(len(ql), sum(ql), sum(kl), hq, hkv, hd)
+    got = plan.attn(q, k, v, ql, kl, hd ** -0.5, causal, window)
+    check(got, *attend(q, k, v, ql, kl, hq, hkv, hd ** -0.5, causal, window))
+
+
 FEW = [(1, 1, 64, [1], [1]), (8, 1, 128, [1, 1, 1], [3, 900, 64]), (20, 20, 64, [5] * 6, [97, 1, 1500, 0, 16, 333]),
        (2, 2, 128, [7, 0, 16, 3], [40, 9, 2000, 17]), (6, 2, 64, [10, 1], [5000, 15]), (32, 1, 64, [1], [70]),
        (4, 2, 128, [16, 2], [33, 3000])]

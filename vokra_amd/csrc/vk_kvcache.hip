@@ -1733,7 +1733,7 @@ hipError_t launch_kv_reorder(hipStream_t s, const KvView& v, int groups, int bea
     // a grid holds fewer than 2^32 threads: parts of the blocks, layers and groups
     constexpr size_t kMost = 1 << 23;
     const int nb = (int)std::min<size_t>(blocks, std::max<size_t>(1, kMost / chunks));
-    const int nl = (int)std::min<size_t>(c.n_layer, std::max<size_t>(1, kMost / ((size_t)nb * chunks)));
+    const int nl = (int)std::min<size_t>(std::min(c.n_layer, 65535), std::max<size_t>(1, kMost / ((size_t)nb * chunks)));
     const int ng = (int)std::min<size_t>(groups, std::max<size_t>(1, kMost / ((size_t)nb * chunks * nl)));
     for (int g = 0; g < groups; g += ng)
         for (int l = 0; l < c.n_layer; l += nl)
