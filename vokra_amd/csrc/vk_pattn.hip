@@ -445,25 +445,58 @@ __device__ __forceinline__ float pa_row_sum(float v) {
 // then (M, sum, e) of each row.
 constexpr size_t pa_piece_floats(int hd) { return (size_t)pa_tile_rows(hd) * (hd + 4); }
 
+// Rows of q and out go through LDS, 32 rows of 32 values a wave at a time: the matrix
+// instruction wants a row a lane, a load or store of whole lines eight lanes a row. Row r's
+// 16-byte piece c lies at r, c ^ (r % 8): neither way meets a bank twice. (Three sequences of
+// up to 61 rows 13.4 -> 12.6 us, 16 of up to 400 in tiles 65 -> 61; long ones as before.)
+constexpr int kPaTurn = 256;  // pieces a wave
+struct PaTurn {
+    vk_f32x4* lds;  // the wave's
+    int lane_at, row_at, sw;  // pieces of 8 rows a lane, 8 j rows on; of this lane's row
+    __device__ __forceinline__ PaTurn(vk_f32x4* of_waves) {
+        const int lane = threadIdx.x & 63, l = lane & 31;
+        lds = of_waves + (threadIdx.x >> 6) * kPaTurn;
+        lane_at = (lane & ~7) + ((lane & 7) ^ (lane >> 3));
+        row_at = 8 * l;
+        sw = l & 7;
+    }
+    __device__ __forceinline__ vk_f32x4& line(int j) { return lds[64 * j + lane_at]; }
+    __device__ __forceinline__ vk_f32x4& row(int c) { return lds[row_at + (c ^ sw)]; }
+    // Between the two: a wave's LDS accesses run in order, so it is the compiler's alone.
+    static __device__ __forceinline__ void turn() { asm volatile("" ::: "memory"); }
+};
+
 template <int HD>
 __device__ __forceinline__ void pa_store_rows(const PaArgs& a, int q0, int head, int rows, int row0,
-                                              const vk_f32x16 (&o)[HD / 32], float sum, int e) {
-    const int lane = threadIdx.x & 63, h = lane >> 5, r = row0 + (int)(threadIdx.x >> 6) * 32 + (lane & 31);
-    if (r >= rows) return;
+                                              const vk_f32x16 (&o)[HD / 32], float sum, int e, PaTurn t) {
+    const int lane = threadIdx.x & 63, h = lane >> 5, first = row0 + (int)(threadIdx.x >> 6) * 32;
+    if (first >= rows) return;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // (NaN stays)
-    const int i = r / a.g, gh = r - i * a.g;
-    float* out = a.out + (size_t)(q0 + i) * a.out_stride + (size_t)(head * a.g + gh) * HD + 4 * h;
+    float* out[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int r = min(first + 8 * j + (lane >> 3), rows - 1), i = r / a.g;
+        out[j] = a.out + (size_t)(q0 + i) * a.out_stride + (size_t)(head * a.g + r - i * a.g) * HD + 4 * (lane & 7);
+    }
     const int eh = max(min(e, 254), -252) >> 1;
     const float f0 = e == kPaNoValue ? 0.0f : pa_pow2(eh), f1 = e == kPaNoValue ? 0.0f : pa_pow2(max(min(e, 254), -252) - eh);
 #pragma unroll
-    for (int b = 0; b < HD / 32; ++b)
+    for (int b = 0; b < HD / 32; ++b) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             vk_f32x4 y;
 #pragma unroll
             for (int c = 0; c < 4; ++c) y[c] = o[b][4 * j + c] * inv * f0 * f1;
-            *(vk_f32x4*)(out + 32 * b + 8 * j) = y;
+            t.row(2 * j + h) = y;
         }
+        t.turn();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const vk_f32x4 y = t.line(j);
+            if (first + 8 * j + (lane >> 3) < rows) *(vk_f32x4*)(out[j] + 32 * b) = y;
+        }
+        t.turn();
+    }
 }
 
 // A sequence's offsets by scalar loads (see pa_meta; the caller wrote them before the
@@ -517,7 +550,7 @@ struct PaWave {
     int some_from, some_to;    // keys that a row of the wave sees,
     int all_from, all_to;      // that all of them see
 
-    __device__ __forceinline__ void load(const PaArgs& a, const PaPiece& p, int wave) {
+    __device__ __forceinline__ void load(const PaArgs& a, const PaPiece& p, int wave, PaTurn t) {
         constexpr int KS = HD / 16;
         const int lane = threadIdx.x & 63, h = lane >> 5, l = lane & 31, rows = p.n * a.g;
         const int first = p.row0 + wave * 32, r = min(first + l, rows - 1), qi = r / a.g;
@@ -535,13 +568,27 @@ struct PaWave {
             }
         }
         if (first >= rows) some_to = 0;  // no rows
-        const float* qp = a.q + (size_t)(p.q0 + qi) * a.q_stride + (size_t)(p.head * a.g + r - qi * a.g) * HD + 8 * h;
+        vk_f32x4 y[HD / 32][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = min(first + 8 * j + (lane >> 3), rows - 1), i = r / a.g;
+            const float* qp = a.q + (size_t)(p.q0 + i) * a.q_stride + (size_t)(p.head * a.g + r - i * a.g) * HD + 4 * (lane & 7);
+#pragma unroll
+            for (int b = 0; b < HD / 32; ++b) y[b][j] = *(const vk_f32x4*)(qp + 32 * b);
+        }
         float x[KS][8];
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const float4 u = *(const float4*)(qp + 16 * s), w = *(const float4*)(qp + 16 * s + 4);
-            x[s][0] = u.x, x[s][1] = u.y, x[s][2] = u.z, x[s][3] = u.w;
-            x[s][4] = w.x, x[s][5] = w.y, x[s][6] = w.z, x[s][7] = w.w;
+        for (int b = 0; b < HD / 32; ++b) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t.line(j) = y[b][j];
+            t.turn();
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const vk_f32x4 z = t.row(4 * (c >> 1) + 2 * h + (c & 1));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[2 * b + (c >> 1)][4 * (c & 1) + j] = z[j];
+            }
+            t.turn();
         }
         if (a.sign != 1.0f)
 #pragma unroll
@@ -690,6 +737,8 @@ __global__ __launch_bounds__(pa_tile_rows(HD) * 2) __attribute__((amdgpu_waves_p
     constexpr int NW = pa_tile_rows(HD) / 32, DB = HD / 32, P = pa_part(HD);
     constexpr int DMA = 8 * P / 1024 / NW;  // 1 KB loads of a tile a wave
     __shared__ __align__(16) _Float16 s_t[2][4 * P];  // K hi, K lo, V hi, V lo
+    __shared__ vk_f32x4 s_turn[NW * kPaTurn];
+    const PaTurn turn(s_turn);
     const int share = vk_xcd_tile(blockIdx.x, gridDim.x);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int h = lane >> 5, l = lane & 31;
@@ -719,7 +768,7 @@ __global__ __launch_bounds__(pa_tile_rows(HD) * 2) __attribute__((amdgpu_waves_p
     for (bool more = true; more;) {
         const int rows = p.n * a.g;
         PaWave<HD> w;
-        w.load(a, p, wave);
+        w.load(a, p, wave, turn);
         vk_f32x16 o[DB];
 #pragma unroll
         for (int b = 0; b < DB; ++b)
@@ -745,7 +794,7 @@ __global__ __launch_bounds__(pa_tile_rows(HD) * 2) __attribute__((amdgpu_waves_p
         }
         s.sum = pa_row_sum(s.sum);
         if (p.u0 == 0 && p.u1 == p.units) {
-            pa_store_rows<HD>(a, p.q0, p.head, rows, p.row0, o, s.sum, s.e);
+            pa_store_rows<HD>(a, p.q0, p.head, rows, p.row0, o, s.sum, s.e, turn);
         } else {
             float* part = a.part + (size_t)(2 * share + (p.u0 == 0 ? 1 : 0)) * pa_piece_floats(HD);
             vk_f32x4* po = (vk_f32x4*)part + wave * (HD / 8) * 64 + lane;
@@ -771,6 +820,7 @@ __global__ __launch_bounds__(pa_tile_rows(HD) * 2) __attribute__((amdgpu_waves_p
 template <int HD>
 __global__ __launch_bounds__(pa_tile_rows(HD) * 2) void vk_pattn_join(PaArgs a) {
     constexpr int DB = HD / 32;
+    __shared__ vk_f32x4 s_turn[pa_tile_rows(HD) / 32 * kPaTurn];
     const int share = blockIdx.x;
     if (share >= (int)a.plan[2]) return;
     const PaOpen open = a.open[share];
@@ -804,7 +854,7 @@ __global__ __launch_bounds__(pa_tile_rows(HD) * 2) void vk_pattn_join(PaArgs a) 
 #pragma unroll
             for (int c = 0; c < 4; ++c) o[j >> 2][4 * (j & 3) + c] = o[j >> 2][4 * (j & 3) + c] * g0 + y[j][c] * g1;
     }
-    pa_store_rows<HD>(a, q0, open.head, rows, row0, o, s.sum, s.e);
+    pa_store_rows<HD>(a, q0, open.head, rows, row0, o, s.sum, s.e, PaTurn(s_turn));
 }
 
 // ---- short sequences ----------------------------------------------------------------
@@ -817,8 +867,10 @@ template <int HD>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 2 : 1, HD == 64 ? 2 : 1))) void vk_pattn_short(PaArgs a) {
     constexpr int DB = HD / 32;
     __shared__ __align__(16) _Float16 s_t[4 * pa_part(HD)];
+    __shared__ vk_f32x4 s_turn[kShortRows / 32 * kPaTurn];
     __shared__ PaSeqLds s_seq;
     __shared__ PaPackLds s_lds;
+    const PaTurn turn(s_turn);
     const int slot = blockIdx.x;
     PaPiece p;
     p.head = blockIdx.y;
@@ -837,7 +889,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
     const int end = min(p.m, (p.lo + p.units) * kPaKeys);
     if (kk < end) load(kk);
     PaWave<HD> w;
-    w.load(a, p, threadIdx.x >> 6);
+    w.load(a, p, threadIdx.x >> 6, turn);
     vk_f32x16 o[DB];
 #pragma unroll
     for (int b = 0; b < DB; ++b)
@@ -851,7 +903,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
         kk += kPaKeys;
         if (kk < end) load(kk);
     }
-    pa_store_rows<HD>(a, p.q0, p.head, rows, p.row0, o, pa_row_sum(s.sum), s.e);
+    pa_store_rows<HD>(a, p.q0, p.head, rows, p.row0, o, pa_row_sum(s.sum), s.e, turn);
 }
 
 // ---- few rows ----------------------------------------------------------------------
@@ -1121,11 +1173,12 @@ hipError_t launch_pattn(hipStream_t s, int hd, const PaArgs& a) {
         return rows <= 16 ? go_few<128, 1>(s, a) : go_few<128, 2>(s, a);
     }
     // short sequences, by one launch: at head size 64 up to 512 keys (16 of 512 keys, 20 heads:
-    // 83 us, 98 packed; 16 heads over 2: 68 and 61; three of up to 61: 8 and 17), at 128, where
-    // a workgroup has a CU to itself, up to 384 keys and two rounds of workgroups (four of up
-    // to 400, 16 heads over 2: 48 and 51; 16 of up to 400: 90 and 65; three of up to 61: 13 and 24)
+    // 82 us, 96 packed; 16 heads over 2: 67 and 61; three of up to 61: 8 and 17), at 128, where
+    // a workgroup has a CU to itself, up to 448 keys (four of up to 400, 8 heads: 42 and 46, 16
+    // over 2: 47 and 50; of 512: 55 and 49) and two rounds of workgroups (16 of up to 400, 16
+    // over 2: 88 and 61); three of up to 61: 13 and 21
     const long long tiles = ((long long)a.q_rows * a.g / kShortRows + a.n_seq) * a.hkv;
-    if (hd == 64 ? a.max_k <= 512 : a.max_k <= 384 && tiles <= 512) {
+    if (hd == 64 ? a.max_k <= 512 : a.max_k <= 448 && tiles <= 512) {
         const dim3 grid((unsigned)(tiles / a.hkv), (unsigned)a.hkv);
         if (hd == 64) hipLaunchKernelGGL(vk_pattn_short<64>, grid, dim3(256), 0, s, a);
         else hipLaunchKernelGGL(vk_pattn_short<128>, grid, dim3(256), 0, s, a);
