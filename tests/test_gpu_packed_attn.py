@@ -140,7 +140,7 @@ def test_the_ends_of_the_ranges(ctx, hq, hkv, hd, ql, kl, causal, window):
 
 FEW = [(1, 1, 64, [1], [1]), (8, 1, 128, [1, 1, 1], [3, 900, 64]), (20, 20, 64, [5] * 6, [97, 1, 1500, 0, 16, 333]),
        (2, 2, 128, [7, 0, 16, 3], [40, 9, 2000, 17]), (6, 2, 64, [10, 1], [5000, 15]), (32, 1, 64, [1], [70]),
-       (4, 2, 128, [16, 2], [33, 3000])]
+       (4, 2, 128, [16, 2], [33, 3000]), (16, 1, 128, [1], [20000]), (3, 3, 64, [32, 1], [9001, 70])]
 
 
 @pytest.mark.gpu

@@ -6,6 +6,11 @@
 // the larger total first; of equal totals the lower beam, in one beam the larger logit
 // and then the lower token.
 //
+// Bound by reading the logits once, and by two launches: 256 rows of 128259 columns (131
+// MB), 16 continuations, take 32 us for the slices (4.1 TB/s) and 12 for the merge, 320 of
+// 51866, five, 17 and 6; five rows of 51865, ten, 7 and 7, which is dependent rounds of
+// memory, LDS and lane permutations.
+//
 // Two launches. Slices: a workgroup reads 4096 or 8192 columns of a row once, into
 // registers, and leaves their maximum, the sum of their exponentials and their n_out best
 // columns. Merge: a workgroup a group joins the slices' sums (64 bits: totals of
@@ -379,7 +384,10 @@ __global__ __launch_bounds__(BM_MT) void vk_beam_merge(BeamArgs a) {
 
 hipError_t launch_beam_select(hipStream_t s, BeamArgs a) {
     const int rows = a.groups * a.beams;
-    const bool small = (size_t)rows * a.vocab <= (size_t)512 * 4096;
+    // up to 16 lists a beam, smaller slices end earlier (16 groups of four beams of 8192 tokens:
+    // 11.1 us against 12.5; 64 of five of 51866: 23.8 against 24.3); above that, half the
+    // lists to merge (one group of eight of 128259: 14.1 against 15.0, eight: 17.4 against 19.9)
+    const bool small = a.vocab <= 16 * kBeamSlice;
     const int slice = small ? kBeamSlice : 2 * kBeamSlice;
     a.slices = (a.vocab + slice - 1) / slice;
     int groups = 4;  // of threads of a slice

@@ -294,7 +294,9 @@ __device__ __forceinline__ bool pa_find(const PaArgs& a, int slot, PaSeqLds& lds
     return true;
 }
 
-// One workgroup: a tile of 64 keys of one kv head.
+// One workgroup: a tile of 64 keys of one kv head. Bound by memory, which it moves twice:
+// 13193 rows of 8 heads of 128 (216 MB read and written) 44 us, 6400 of 20 heads of 64 (131
+// MB) 22 us.
 template <int HD>
 __device__ void pa_pack(const PaArgs& a, int slot, int head) {
     __shared__ PaSeqLds s_seq;
@@ -729,6 +731,12 @@ __device__ __forceinline__ void pa_unit(const PaArgs& a, const PaPiece& x, const
     }
 }
 
+// Bound by the matrix instructions and the clock that they leave: two documents of 5001 and
+// 8192 rows, causal, 32 heads over 8 of 128, take 2.05 ms (0.37 PFLOP/s at f32 level, 1.1 in
+// fp16 products, 87% of what a large library product of fp16 reaches), 16 prompts of up
+// to 2048 rows, 16 heads over 2, 322 us (0.9), eight utterances of up to 1500 rows, 20 heads
+// of 64, 127 us (0.82). Loads of q ahead of a tile's end and stores that nothing waits for
+// changed none of them.
 // Tiles go global -> LDS directly, the next one (of the next piece, too) while this one
 // is worked on: two buffers, one barrier a unit, between which the two waves of a SIMD
 // run as they come, one's products beside the other's weights.
@@ -816,7 +824,8 @@ __global__ __launch_bounds__(pa_tile_rows(HD) * 2) __attribute__((amdgpu_waves_p
 }
 
 // A tile's pieces brought together, in their order: one workgroup for each share with a
-// tile's first piece.
+// tile's first piece. Bound by reading them (up to two a share, 135 KB each at 128): 16 - 20 us
+// at 128, 8 at 64.
 template <int HD>
 __global__ __launch_bounds__(pa_tile_rows(HD) * 2) void vk_pattn_join(PaArgs a) {
     constexpr int DB = HD / 32;
@@ -927,6 +936,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
 // that stay in the last one from step to step take 31 us, 36 past them (from memory 39
 // and 38).
 constexpr int kFewMost = 2048;  // workgroups that leave partial results
+constexpr int kFewRanges = 64;   // of a sequence (32 rows against 8000 keys, 8 heads of 128: 29 us, 43 with 128, 27 with 32;
+                                 // one of 100000 keys, 16 heads over 2: 49, 46 and 78)
 constexpr int kFewKeys = 16;  // of a wave's step
 
 __device__ __forceinline__ float pa_row4_max(float v) {  // over the lanes l % 16 alike
@@ -1093,62 +1104,78 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_waves(H
     }
 }
 
-// A sequence's ranges of a kv head brought together.
+// A sequence's ranges of a kv head brought together: a workgroup has 64 pieces of four
+// values, its waves every fourth range, eight on their way at once. (16 rows against 8000
+// keys, 8 heads of 128, 24 us in all; one workgroup a sequence and kv head, all ranges in
+// turn, 99.)
 template <int HD, int NT>
 __global__ __launch_bounds__(256) void vk_pattn_few_join(PaArgs a, int per, int splits) {
     __shared__ int s_first;
-    const int seq = blockIdx.y, head = blockIdx.x;
+    __shared__ float2 s_ml[4][64];
+    __shared__ vk_f32x4 s_o[4][64];
+    const int seq = blockIdx.z, head = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n_ok = pa_in_order(a, &s_first);
     if (seq >= n_ok) return;
     const int q0 = a.q_off[seq], n = a.q_off[seq + 1] - q0, m = a.k_off[seq + 1] - a.k_off[seq], rows = n * a.g;
-    const int ranges = (m - pa_few_begin(a, m) + per - 1) / per;
-    if (ranges < 2 || rows > 16 * NT) return;
-    const float* part = a.part + ((size_t)seq * a.hkv + head) * splits * (16 * NT) * (HD + 4);
-    for (int y = threadIdx.x; y < rows * (HD / 4); y += 256) {
-        const int r = y / (HD / 4), d = y % (HD / 4);
-        const float* p = part + (size_t)r * (HD + 4);
-        float top = kNoMax, all = 0.0f;
-        vk_f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s0 = 0; s0 < ranges; s0 += 8) {
-            float2 ml[8];
-            vk_f32x4 w[8];
+    const int ranges = (m - pa_few_begin(a, m) + per - 1) / per, y = (int)blockIdx.x * 64 + lane;
+    if (ranges < 2 || rows > 16 * NT || (int)blockIdx.x * 64 >= rows * (HD / 4)) return;
+    const int r = min(y / (HD / 4), rows - 1), d = y % (HD / 4);
+    const float* p = a.part + ((size_t)seq * a.hkv + head) * splits * (16 * NT) * (HD + 4) + (size_t)r * (HD + 4);
+    float top = kNoMax, all = 0.0f;
+    vk_f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s0 = wave; s0 < ranges; s0 += 32) {
+        float2 ml[8];
+        vk_f32x4 w[8];
 #pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                const float* x = p + (size_t)min(s0 + s, ranges - 1) * (16 * NT) * (HD + 4);
-                ml[s] = *(const float2*)(x + HD);
-                w[s] = *(const vk_f32x4*)(x + 4 * d);
-            }
-#pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                if (s0 + s >= ranges) break;
-                const float now = fmaxf(top, ml[s].x);
-                const float f = __builtin_amdgcn_exp2f(top - now), h = __builtin_amdgcn_exp2f(ml[s].x - now);
-                top = now;
-                all = all * f + ml[s].y * h;
-                z = z * f + w[s] * h;
-            }
+        for (int s = 0; s < 8; ++s) {
+            const float* x = p + (size_t)min(s0 + 4 * s, ranges - 1) * (16 * NT) * (HD + 4);
+            ml[s] = *(const float2*)(x + HD);
+            w[s] = *(const vk_f32x4*)(x + 4 * d);
         }
-        const int i = r / a.g;
-        const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-        *(vk_f32x4*)(a.out + (size_t)(q0 + i) * a.out_stride + (size_t)(head * a.g + r - i * a.g) * HD + 4 * d) = z * inv;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            if (s0 + 4 * s >= ranges) break;
+            const float now = fmaxf(top, ml[s].x);
+            const float f = __builtin_amdgcn_exp2f(top - now), h = __builtin_amdgcn_exp2f(ml[s].x - now);
+            top = now;
+            all = all * f + ml[s].y * h;
+            z = z * f + w[s] * h;
+        }
     }
+    s_ml[wave][lane] = make_float2(top, all);
+    s_o[wave][lane] = z;
+    __syncthreads();
+    if (wave != 0 || y >= rows * (HD / 4)) return;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, s_ml[w][lane].x);
+    all = 0.0f;
+    z = vk_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float f = __builtin_amdgcn_exp2f(s_ml[w][lane].x - top);
+        all += s_ml[w][lane].y * f;
+        z += s_o[w][lane] * f;
+    }
+    const int i = r / a.g;
+    const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+    *(vk_f32x4*)(a.out + (size_t)(q0 + i) * a.out_stride + (size_t)(head * a.g + r - i * a.g) * HD + 4 * d) = z * inv;
 }
 
 template <int HD, int NT>
 static hipError_t go_few(hipStream_t s, const PaArgs& a) {
-    // ranges of a step of all four waves at least, for up to kFewMost workgroups if all sequences
-    // were the longest
+    // ranges of a step of all four waves at least, up to kFewRanges of them a sequence and
+    // kFewMost in all if all sequences were the longest
     constexpr int step = 4 * kFewKeys;
     const long long pairs = (long long)a.n_seq * a.hkv;
     const int keys = a.causal && a.window ? std::min(a.max_k, a.window) : a.max_k;
-    const long long most = std::max<long long>(1, kFewMost / pairs);
+    const long long most = std::max<long long>(1, std::min<long long>(kFewRanges, kFewMost / pairs));
     const int per = (int)std::max<long long>(step, ((keys + most - 1) / most + step - 1) / step * step);
     const int splits = keys ? (keys + per - 1) / per : 1;
     hipLaunchKernelGGL((vk_pattn_few<HD, NT>), dim3((unsigned)a.hkv, (unsigned)splits, (unsigned)a.n_seq), dim3(256), 0, s, a,
                        per);
     if (splits > 1)
-        hipLaunchKernelGGL((vk_pattn_few_join<HD, NT>), dim3((unsigned)a.hkv, (unsigned)a.n_seq), dim3(256), 0, s, a, per,
-                           splits);
+        hipLaunchKernelGGL((vk_pattn_few_join<HD, NT>), dim3((unsigned)(a.max_q * a.g * (HD / 4) + 63) / 64, (unsigned)a.hkv, (unsigned)a.n_seq),
+                           dim3(256), 0, s, a, per, splits);
     return hipGetLastError();
 }
 
@@ -1166,7 +1193,8 @@ static hipError_t go_pattn(hipStream_t s, const PaArgs& a) {
 
 hipError_t launch_pattn(hipStream_t s, int hd, const PaArgs& a) {
     // few rows that all see the same keys: each key is read by few products, packing it
-    // would move three times its bytes
+    // would move three times its bytes (16 sequences of 1000 keys, 20 heads of 64, of 5 rows: 33
+    // us, 104 packed; of 32: 49 and 105; 32 rows of 8 heads of 128 against 8000 keys: 29 and 90)
     const long long rows = (long long)a.max_q * a.g;
     if (rows <= kPaFewRows && (!a.causal || a.max_q == 1)) {
         if (hd == 64) return rows <= 16 ? go_few<64, 1>(s, a) : go_few<64, 2>(s, a);
