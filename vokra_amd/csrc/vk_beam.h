@@ -7,7 +7,7 @@
 
 constexpr int kBeamMost = 32;      // beams of a group
 constexpr int kBeamOut = 64;       // continuations of a group
-constexpr int kBeamSlice = 4096;   // columns of the smaller slices (the workspace is sized by them)
+constexpr int kBeamSlice = 4096;   // columns of the smaller slices at most (the workspace is sized by them)
 
 struct BeamStat {
     double sum;  // of e^(x - max) over the slice
@@ -25,10 +25,10 @@ struct BeamArgs {
     unsigned long long* keys;  // [row][slice][n_out]
     BeamStat* stats;           // [row][slice]
     int groups, beams, vocab, n_out, end_token;
-    int slices, group;  // set by the launcher: slices of a row, threads of a group
+    int slices, width, group;  // set by the launcher: slices of a row, their columns, threads of a group
 };
 
 namespace vk {
-// slices and group are filled in here
+// slices, width and group are filled in here
 hipError_t launch_beam_select(hipStream_t s, BeamArgs a);
 }  // namespace vk

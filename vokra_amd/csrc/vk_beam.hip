@@ -11,7 +11,7 @@
 // 51866, five, 17 and 6; five rows of 51865, ten, 7 and 7, which is dependent rounds of
 // memory, LDS and lane permutations.
 //
-// Two launches. Slices: a workgroup reads 4096 or 8192 columns of a row once, into
+// Two launches. Slices: a workgroup reads up to 4096 or 8192 columns of a row once, into
 // registers, and leaves their maximum, the sum of their exponentials and their n_out best
 // columns. Merge: a workgroup a group joins the slices' sums (64 bits: totals of
 // different beams are compared, and near ones have to fall in order), takes each
@@ -105,7 +105,6 @@ typedef float bm_f4 __attribute__((ext_vector_type(4), aligned(4)));
 // E columns a thread, in runs of four
 template <int E>
 __global__ __launch_bounds__(BM_T) void vk_beam_slices(BeamArgs a) {
-    constexpr int SLICE = BM_T * E;
     __shared__ float s_max[4], s_bound[4];
     __shared__ double s_sum[4];
     __shared__ unsigned long long s_key[BM_CAND];
@@ -113,17 +112,17 @@ __global__ __launch_bounds__(BM_T) void vk_beam_slices(BeamArgs a) {
     const int row = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
     if (!bm_live(a, row)) return;
     const float* x = a.logits + (size_t)row * a.stride;
-    const int c0 = (int)blockIdx.x * SLICE;
+    const int c0 = (int)blockIdx.x * a.width, c1 = min(c0 + a.width, a.vocab);
     float y[E];
 #pragma unroll
     for (int j = 0; j < E / 4; ++j) {
         const int c = c0 + 4 * (t + BM_T * j);
-        if (c + 3 < a.vocab) {
+        if (c + 3 < c1) {
             const bm_f4 v = *(const bm_f4*)(x + c);
             y[4 * j] = v.x, y[4 * j + 1] = v.y, y[4 * j + 2] = v.z, y[4 * j + 3] = v.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[4 * j + i] = c + i < a.vocab ? x[c + i] : -INFINITY;
+            for (int i = 0; i < 4; ++i) y[4 * j + i] = c + i < c1 ? x[c + i] : -INFINITY;
         }
     }
     if (t == 0) s_n = 0;
@@ -390,6 +389,9 @@ hipError_t launch_beam_select(hipStream_t s, BeamArgs a) {
     const bool small = a.vocab <= 16 * kBeamSlice;
     const int slice = small ? kBeamSlice : 2 * kBeamSlice;
     a.slices = (a.vocab + slice - 1) / slice;
+    // slices of one width: all threads of each have columns (with a narrow last one its empty
+    // threads bound nothing, and all of its columns are ranked: four beams of 12749 tokens 21 -> 11 us)
+    a.width = ((a.vocab + a.slices - 1) / a.slices + 3) / 4 * 4;
     int groups = 4;  // of threads of a slice
     while (groups < a.n_out) groups *= 2;
     a.group = BM_T / groups;
