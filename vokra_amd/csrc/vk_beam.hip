@@ -34,6 +34,7 @@ constexpr int BM_T = 256;     // threads of a slice
 constexpr int BM_CAND = 512;  // candidates that are ranked at once
 constexpr int BM_MT = 512;    // threads of a merge: eight waves, a beam each in turn
 constexpr int BM_LIST = 1024; // entries of a beam's lists that a wave holds in LDS
+constexpr int BM_FEW = 64;    // entries of a group that are all ranked
 
 // Values in the order of their bits, a column index that falls with it behind: the larger
 // key is the better column. Key 0: none.
@@ -224,8 +225,9 @@ __global__ __launch_bounds__(BM_MT) void vk_beam_merge(BeamArgs a) {
     __shared__ unsigned long long s_list[WAVES][BM_LIST];
     __shared__ unsigned long long s_some[WAVES][128], s_best[WAVES][64], s_order[BM_MT];
     __shared__ double s_total[kBeamMost][kBeamOut];
-    __shared__ int s_rank[BM_MT], s_token[kBeamMost][kBeamOut], s_count[kBeamMost], s_ended[kBeamMost];
+    __shared__ int s_rank[BM_MT], s_place[BM_MT], s_found, s_token[kBeamMost][kBeamOut], s_count[kBeamMost], s_ended[kBeamMost];
     const int g = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = a.n_out;
+    if (threadIdx.x == 0) s_found = 0;
     for (int b = wave; b < a.beams; b += WAVES) {
         const int row = g * a.beams + b;
         const BeamStat* st = a.stats + (size_t)row * a.slices;
@@ -342,29 +344,51 @@ __global__ __launch_bounds__(BM_MT) void vk_beam_merge(BeamArgs a) {
         if (a.out_ended) a.out_ended[o] = !any || s_ended[b] || token == a.end_token ? 1 : 0;
     };
     if (a.beams * n <= BM_MT) {
-        // every entry ranked by counting, of equal totals the lower place first; as many threads
-        // an entry as there are, a share of the others each
-        const int t = threadIdx.x, entries = a.beams * n, parts = BM_MT / entries, e = t % entries, part = t / entries;
-        const int b = e / n, at = e - b * n;
-        const bool any = at < s_count[b];
-        const unsigned long long mine = any ? bm_order(s_total[b][at]) : 0;
-        if (part == 0) {
-            s_order[e] = mine;
-            s_rank[e] = 0;
+        // ranked by counting, of equal totals the lower place first; as many threads an entry as
+        // there are, a share of the others each. Of many entries those alone that reach the least
+        // of the c-th ones of the F lists that are full, F c n_out or more: at least n_out
+        // (twelve beams, 24 continuations: 20 -> 11.5 us; few entries are ranked sooner than
+        // bounded, five of five 6.6 and 7.9)
+        const int t = threadIdx.x, entries = a.beams * n;
+        int found = entries;
+        if (entries > BM_FEW) {
+            const int count = lane < a.beams ? s_count[lane] : 0, full = __popcll(__ballot(count == n));
+            const int c = full ? (n + full - 1) / full - 1 : 0;
+            const unsigned long long bound = full ? ~bm_wave_max(count == n ? ~bm_order(s_total[lane][c]) : 0) : 0;
+            const int b = t / n, at = t - b * n;
+            const unsigned long long own = t < entries && at < s_count[b] ? bm_order(s_total[b][at]) : 0;
+            if (own && own >= bound) {
+                const int i = atomicAdd(&s_found, 1);
+                s_order[i] = own;
+                s_place[i] = t;
+                s_rank[i] = 0;
+            }
+            __syncthreads();
+            found = s_found;
+        } else {
+            if (t < entries) {
+                const int b = t / n, at = t - b * n;
+                s_order[t] = at < s_count[b] ? bm_order(s_total[b][at]) : 0;
+                s_place[t] = t;
+                s_rank[t] = 0;
+            }
+            __syncthreads();
         }
-        const int all = __syncthreads_count(any && part == 0);
+        const int parts = found ? BM_MT / found : 0, e = found ? t % found : 0, part = found ? t / found : 0;
+        const unsigned long long mine = found ? s_order[e] : 0;
+        const int place = found ? s_place[e] : 0;
         int before = 0;
-        if (part < parts && any)
+        if (part < parts)
 #pragma unroll 4
-            for (int i = part; i < entries; i += parts) {
+            for (int i = part; i < found; i += parts) {
                 const unsigned long long y = s_order[i];
-                before += (int)(y > mine) + (int)((y == mine) & (i < e));
+                before += (int)(y > mine) + (int)((y == mine) & (s_place[i] < place));
             }
         if (before) atomicAdd(&s_rank[e], before);
         __syncthreads();
-        before = s_rank[e];
-        if (part == 0 && any && before < n) put(before, b, at, true);
-        if (t >= all && t < n) put(t, 0, 0, false);
+        // (entries that are none come last, in the order of their places)
+        if (t < found && s_rank[t] < n) put(s_rank[t], place / n, place % n, mine != 0);
+        if (t >= found && t < n) put(t, 0, 0, false);
         return;
     }
     if (wave != 0) return;
