@@ -110,6 +110,8 @@ def test_lengths_heads_and_masks(ctx, hq, hkv, hd, case):
     (1, 1, 128, [4100], None, True, 0),
     (4, 2, 64, [90, 400, 0, 513], None, True, 0),  # packed, with sequences of no rows and of few
     (8, 1, 128, [33, 385, 1, 64], None, True, 70),
+    (2, 2, 64, [700, 3], [900, 5], True, 191), (2, 1, 64, [700, 3], [900, 5], True, 257), (4, 2, 128, [1000], None, True, 1),
+    (1, 1, 128, [80, 600], [1600, 600], True, 130),  # long ones, each row of few keys
     (2, 1, 128, [40] * 300, None, True, 0)])  # short ones beyond two rounds of workgroups
 def test_keys_split_over_workgroups(ctx, hq, hkv, hd, ql, kl, causal, window):
     print("[case] packed split", hq, hkv, hd, ql[:3], causal, window, flush=True)

@@ -1206,7 +1206,10 @@ hipError_t launch_pattn(hipStream_t s, int hd, const PaArgs& a) {
     // over 2: 47 and 50; of 512: 55 and 49) and two rounds of workgroups (16 of up to 400, 16
     // over 2: 88 and 61); three of up to 61: 13 and 21
     const long long tiles = ((long long)a.q_rows * a.g / kShortRows + a.n_seq) * a.hkv;
-    if (hd == 64 ? a.max_k <= 512 : a.max_k <= 448 && tiles <= 512) {
+    // and long ones of which a tile's rows see up to 320 (20 heads of 64, four of up to 1500, a
+    // window of 100: 47 and 60, of 400: 80 and 76; 8 heads of 128, one of 1000, of 128: 29 and 45)
+    const int most = a.causal && a.window && a.window + kShortRows / a.g <= 320 ? 320 : a.max_k;
+    if (hd == 64 ? most <= 512 : most <= 448 && tiles <= 512) {
         const dim3 grid((unsigned)(tiles / a.hkv), (unsigned)a.hkv);
         if (hd == 64) hipLaunchKernelGGL(vk_pattn_short<64>, grid, dim3(256), 0, s, a);
         else hipLaunchKernelGGL(vk_pattn_short<128>, grid, dim3(256), 0, s, a);
