@@ -352,8 +352,8 @@ int vokra_hip_attn_f32_dev(vokra_hip_ctx_t *ctx, size_t batch, size_t t_q, size_
  * product runs as three fp16 products of two parts of both operands (22 bits), each
  * operand under a power of two (a query row's, a tile of 64 keys' for a kv head), so
  * results do not depend on the values' size (a value is held to 2^-37 of its row's or
- * tile's largest at least); of few rows (max_q * n_head_q / n_head_kv <= 32, max_q 1 if
- * causal) in f32 as they are. Sums in f32. How a row's keys are split
+ * tile's largest at least); of few rows (max_q * n_head_q / n_head_kv <= 32) in f32 as
+ * they are. Sums in f32. How a row's keys are split
  * depends on the whole call, and its last f32 bits may with it. A key row or query
  * row with a value that is not finite makes rows that see it NaN; a value of V that is
  * not finite makes its column of those rows not finite; rows that do not see it are not

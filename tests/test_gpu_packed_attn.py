@@ -142,7 +142,8 @@ def test_the_ends_of_the_ranges(ctx, hq, hkv, hd, ql, kl, causal, window):
 
 FEW = [(1, 1, 64, [1], [1]), (8, 1, 128, [1, 1, 1], [3, 900, 64]), (20, 20, 64, [5] * 6, [97, 1, 1500, 0, 16, 333]),
        (2, 2, 128, [7, 0, 16, 3], [40, 9, 2000, 17]), (6, 2, 64, [10, 1], [5000, 15]), (32, 1, 64, [1], [70]),
-       (4, 2, 128, [16, 2], [33, 3000]), (16, 1, 128, [1], [20000]), (3, 3, 64, [32, 1], [9001, 70])]
+       (4, 2, 128, [16, 2], [33, 3000]), (16, 1, 128, [1], [20000]), (3, 3, 64, [32, 1], [9001, 70]),
+       (4, 1, 128, [4, 8, 2], [700, 3, 1]), (2, 1, 64, [9, 0, 5], [4, 0, 300])]
 
 
 @pytest.mark.gpu
@@ -187,7 +188,9 @@ def test_values_of_any_size(ctx, ql, kl, causal):
 @pytest.mark.gpu
 @pytest.mark.parametrize("hq,hkv,hd,ql,kl,causal,window", [
     (2, 1, 64, [100, 90], [100, 90], True, 0), (2, 2, 128, [100, 90], [100, 90], True, 20),
-    (3, 1, 64, [5, 4], [100, 90], True, 0), (2, 1, 64, [5, 4], [100, 90], False, 0), (2, 2, 128, [1, 1], [100, 90], True, 30)])
+    (3, 1, 64, [5, 4], [100, 90], True, 0), (2, 1, 64, [5, 4], [100, 90], False, 0), (2, 2, 128, [1, 1], [100, 90], True, 30),
+    (2, 1, 64, [5, 4], [100, 90], True, 20), (2, 2, 128, [7, 13], [100, 90], True, 9), (4, 1, 64, [8, 6], [100, 90], True, 70),
+    (2, 1, 128, [16, 9], [100, 90], True, 0)])
 def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(ctx, hq, hkv, hd, ql, kl, causal, window):
     print("[case] packed nan", hq, hkv, hd, ql, causal, window, flush=True)
     g = np.random.default_rng(9)

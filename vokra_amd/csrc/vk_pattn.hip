@@ -917,9 +917,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
 
 // ---- few rows ----------------------------------------------------------------------
 
-// Tokens, or candidates against rows of their own: at most 16 NT query rows of a kv head,
-// which all see the same keys. K and V are read once as they are, f32, straight into the
-// operands of the f32 matrix instruction (16 x 16 x 4): nothing is packed.
+// Tokens and drafts, or candidates against rows of their own: at most 16 NT query rows of a kv
+// head, which see the same keys but for some at the ends. K and V are read once as they
+// are, f32, straight into the operands of the f32 matrix instruction (16 x 16 x 4): nothing
+// is packed.
 //   S^T [16 keys][16 rows]: a lane's 16 bytes of K are one operand of four products
 //     (key lane % 16, dims 16 c + 4 (lane / 16) + j; q likewise);
 //   its accumulators (keys 4 (lane / 16) + i of row lane % 16) are the operand of
@@ -930,7 +931,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
 // when the products of the step before have taken theirs, V likewise; steps of 16 keys
 // leave room for four waves a SIMD (of 64 and 32, with two and three waves: 44 and 39 us).
 // Bound by the reads of K and V: five rows each against 16 sequences of 97 to 1500 keys, 20
-// heads of 64, 131 MB, take 39 us with the join from memory (3.4 TB/s). Neighbouring
+// heads of 64, 131 MB, take 38 us with the join from memory (3.5 TB/s). Neighbouring
 // workgroups are the heads of the same keys, so that whole rows of K and V are on their
 // way (ranges of one head: 44 against 41 us), and the reads go through the caches: K and V
 // that stay in the last one from step to step take 31 us, 36 past them (from memory 39
@@ -950,15 +951,18 @@ __device__ __forceinline__ float pa_row4_sum(float v) {
     return pa_row_sum(__uint_as_float(a[0]) + __uint_as_float(a[1]));
 }
 
-// The keys of sequence lengths n, m that its rows see: few rows are all at one place.
-__device__ __forceinline__ int pa_few_begin(const PaArgs& a, int m) {
-    return a.causal && a.window ? max(0, m - a.window) : 0;
+// The first key that a row of n, of m keys, sees
+__device__ __forceinline__ int pa_few_begin(const PaArgs& a, int n, int m) {
+    return a.causal && a.window ? max(0, m - n - a.window + 1) : 0;
 }
 
-constexpr int few_waves(int hd, int nt) { return hd * nt == 64 ? 4 : hd * nt == 128 ? 3 : 2; }  // what K, V, q and o leave
+// what K, V, q and o leave, and the masks of ENDS
+constexpr int few_waves(int hd, int nt, bool ends) { return hd * nt == 64 ? 4 : hd * nt == 128 && !ends ? 3 : 2; }
 
-template <int HD, int NT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_waves(HD, NT)))) void vk_pattn_few(PaArgs a, int per) {
+// ENDS: rows of one sequence see different keys (causal, more than one row a sequence). Their
+// masks cost a token of 32 heads over 2 of 128 against 2000 keys 42 us for 38.
+template <int HD, int NT, bool ENDS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_waves(HD, NT, ENDS)))) void vk_pattn_few(PaArgs a, int per) {
     constexpr int KU = kFewKeys, QC = HD / 16, DD = HD / 64;
     __shared__ int s_first;
     __shared__ float s_m[4][16 * NT], s_l[4][16 * NT];
@@ -970,12 +974,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_waves(H
     const int q0 = a.q_off[seq], n = a.q_off[seq + 1] - q0, k0 = a.k_off[seq], m = a.k_off[seq + 1] - k0;
     const int rows = n * a.g;
     if (rows == 0 || rows > 16 * NT) return;
-    const int begin = pa_few_begin(a, m) + (int)blockIdx.y * per, end = min(begin + per, m);
+    const int begin = pa_few_begin(a, n, m) + (int)blockIdx.y * per, end = min(begin + per, m);
     if (blockIdx.y && begin >= m) return;
+    // this lane's rows see the keys from .. to - 1, all rows those of all_from .. all_to - 1
+    int from[NT], to[NT];
+    const int all_from = a.window ? m - a.window : 0, all_to = m - n + 1;
     vk_f32x4 q[NT][QC];
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
         const int r = min(16 * x + l, rows - 1), i = r / a.g;
+        from[x] = ENDS && a.window ? m - n + i - a.window + 1 : 0;
+        to[x] = ENDS ? min(end, m - n + i + 1) : end;
         const float* qp = a.q + (size_t)(q0 + i) * a.q_stride + (size_t)(head * a.g + r - i * a.g) * HD + 4 * g;
 #pragma unroll
         for (int c = 0; c < QC; ++c) q[x][c] = *(const vk_f32x4*)(qp + 16 * c) * (a.c * a.sign);
@@ -1007,6 +1016,40 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_waves(H
             for (int d = 0; d < DD; ++d) v[i][d] = *(const vk_f32x4*)(p + 64 * d);
         }
     };
+    // Where rows see different keys, values of V that are not finite are taken out of the
+    // product and added to the rows that see them
+    auto few_odd = [&](int key) __attribute__((always_inline)) {
+        uint32_t odd = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int d = 0; d < DD; ++d)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (!pa_finite(v[i][d][j])) {
+                        odd |= 1u << (4 * g + i);
+                        v[i][d][j] = 0.0f;
+                    }
+        if (!__any(odd != 0)) return;
+#pragma unroll
+        for (int b = 1; b < 64; b <<= 1) odd |= __shfl_xor(odd, b, VK_WAVE);
+        for (; odd; odd &= odd - 1) {
+            const int at = key + __ffs(odd) - 1;
+            if (at >= end) break;
+            const float* p = a.v + (size_t)(k0 + at) * a.v_stride + (size_t)head * HD + 16 * g;
+#pragma unroll
+            for (int d = 0; d < DD; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const vk_f32x4 f = *(const vk_f32x4*)(p + 64 * d + 4 * i);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int x = 0; x < NT; ++x)
+                            if (!pa_finite(f[j]) && at >= from[x] && at < to[x]) o[x][d][j][i] += f[j];
+                }
+        }
+    };
     int key = begin + wave * KU;
     if (key < end) {
         load_k(key);
@@ -1032,7 +1075,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_waves(H
             for (int i = 0; i < 4; ++i) {
                 float y = s[x][i];
                 y = y > -INFINITY ? y : __builtin_nanf("");  // of a key that is not finite
-                y = key + 4 * g + i < end ? y : -INFINITY;
+                const int at = key + 4 * g + i;
+                y = (!ENDS || at >= from[x]) && at < to[x] ? y : -INFINITY;
                 s[x][i] = y;
                 most = fmaxf(most, y);
             }
@@ -1051,6 +1095,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_waves(H
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[x][d][j] *= f;
         }
+        if (ENDS && (key < all_from || key + KU > all_to)) few_odd(key);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -1078,7 +1123,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_waves(H
                     vk_f32x4{o[x][d][0][i], o[x][d][1][i], o[x][d][2][i], o[x][d][3][i]};
     }
     __syncthreads();
-    const int ranges = max(1, (m - pa_few_begin(a, m) + per - 1) / per);
+    const int ranges = max(1, (m - pa_few_begin(a, n, m) + per - 1) / per);
     float* part = a.part + (((size_t)seq * a.hkv + head) * gridDim.y + blockIdx.y) * (16 * NT) * (HD + 4);
     for (int y = t; y < rows * (HD / 4); y += 256) {
         const int r = y / (HD / 4), d = y % (HD / 4);
@@ -1117,7 +1162,7 @@ __global__ __launch_bounds__(256) void vk_pattn_few_join(PaArgs a, int per, int 
     const int n_ok = pa_in_order(a, &s_first);
     if (seq >= n_ok) return;
     const int q0 = a.q_off[seq], n = a.q_off[seq + 1] - q0, m = a.k_off[seq + 1] - a.k_off[seq], rows = n * a.g;
-    const int ranges = (m - pa_few_begin(a, m) + per - 1) / per, y = (int)blockIdx.x * 64 + lane;
+    const int ranges = (m - pa_few_begin(a, n, m) + per - 1) / per, y = (int)blockIdx.x * 64 + lane;
     if (ranges < 2 || rows > 16 * NT || (int)blockIdx.x * 64 >= rows * (HD / 4)) return;
     const int r = min(y / (HD / 4), rows - 1), d = y % (HD / 4);
     const float* p = a.part + ((size_t)seq * a.hkv + head) * splits * (16 * NT) * (HD + 4) + (size_t)r * (HD + 4);
@@ -1161,22 +1206,27 @@ __global__ __launch_bounds__(256) void vk_pattn_few_join(PaArgs a, int per, int 
     *(vk_f32x4*)(a.out + (size_t)(q0 + i) * a.out_stride + (size_t)(head * a.g + r - i * a.g) * HD + 4 * d) = z * inv;
 }
 
-template <int HD, int NT>
-static hipError_t go_few(hipStream_t s, const PaArgs& a) {
+template <int HD, int NT, bool ENDS>
+static hipError_t go_few_as(hipStream_t s, const PaArgs& a) {
     // ranges of a step of all four waves at least, up to kFewRanges of them a sequence and
     // kFewMost in all if all sequences were the longest
     constexpr int step = 4 * kFewKeys;
     const long long pairs = (long long)a.n_seq * a.hkv;
-    const int keys = a.causal && a.window ? std::min(a.max_k, a.window) : a.max_k;
+    const int keys = a.causal && a.window ? std::min(a.max_k, a.window + a.max_q - 1) : a.max_k;
     const long long most = std::max<long long>(1, std::min<long long>(kFewRanges, kFewMost / pairs));
     const int per = (int)std::max<long long>(step, ((keys + most - 1) / most + step - 1) / step * step);
     const int splits = keys ? (keys + per - 1) / per : 1;
-    hipLaunchKernelGGL((vk_pattn_few<HD, NT>), dim3((unsigned)a.hkv, (unsigned)splits, (unsigned)a.n_seq), dim3(256), 0, s, a,
+    hipLaunchKernelGGL((vk_pattn_few<HD, NT, ENDS>), dim3((unsigned)a.hkv, (unsigned)splits, (unsigned)a.n_seq), dim3(256), 0, s, a,
                        per);
     if (splits > 1)
         hipLaunchKernelGGL((vk_pattn_few_join<HD, NT>), dim3((unsigned)(a.max_q * a.g * (HD / 4) + 63) / 64, (unsigned)a.hkv, (unsigned)a.n_seq),
                            dim3(256), 0, s, a, per, splits);
     return hipGetLastError();
+}
+
+template <int HD, int NT>
+static hipError_t go_few(hipStream_t s, const PaArgs& a) {
+    return a.causal && a.max_q > 1 ? go_few_as<HD, NT, true>(s, a) : go_few_as<HD, NT, false>(s, a);
 }
 
 // ---- launchers ---------------------------------------------------------------------
@@ -1192,11 +1242,12 @@ static hipError_t go_pattn(hipStream_t s, const PaArgs& a) {
 }
 
 hipError_t launch_pattn(hipStream_t s, int hd, const PaArgs& a) {
-    // few rows that all see the same keys: each key is read by few products, packing it
-    // would move three times its bytes (16 sequences of 1000 keys, 20 heads of 64, of 5 rows: 33
-    // us, 104 packed; of 32: 49 and 105; 32 rows of 8 heads of 128 against 8000 keys: 29 and 90)
+    // few rows: each key is read by few products, packing it would move three times its bytes (16
+    // sequences of 1000 keys, 20 heads of 64, of 5 rows: 33 us, 104 packed; of 32: 49 and 105; of
+    // 2000 keys and four causal rows: 69 and 209; 32 rows of 8 heads of 128 against 8000 keys: 29
+    // and 90; against 32 keys, in one launch either way: 10 and 12)
     const long long rows = (long long)a.max_q * a.g;
-    if (rows <= kPaFewRows && (!a.causal || a.max_q == 1)) {
+    if (rows <= kPaFewRows) {
         if (hd == 64) return rows <= 16 ? go_few<64, 1>(s, a) : go_few<64, 2>(s, a);
         return rows <= 16 ? go_few<128, 1>(s, a) : go_few<128, 2>(s, a);
     }
