@@ -369,7 +369,9 @@ __device__ void pa_plan(const PaArgs& a) {
     }
     if (t == 0) a.line[slots] = before;
     const long long total = before * a.hkv;
-    const long long shares = total ? min((long long)pa_shares(HD), max(1ll, total / (pa_cost(HD) + 1))) : 0;
+    // two units at least: of a small call more workgroups (two sequences of up to 714 rows, 2 heads
+    // of 128: 39 us, 46 with four; of 800 rows, 16 over 2: 43 and 47)
+    const long long shares = total ? min((long long)pa_shares(HD), max(1ll, total / 2)) : 0;
     const long long size = shares ? (total + shares - 1) / shares : 0;
     if (t == 0) {
         a.plan[0] = size;
