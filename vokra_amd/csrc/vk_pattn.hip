@@ -452,7 +452,7 @@ constexpr size_t pa_piece_floats(int hd) { return (size_t)pa_tile_rows(hd) * (hd
 // Rows of q and out go through LDS, 32 rows of 32 values a wave at a time: the matrix
 // instruction wants a row a lane, a load or store of whole lines eight lanes a row. Row r's
 // 16-byte piece c lies at r, c ^ (r % 8): neither way meets a bank twice. (Three sequences of
-// up to 61 rows 13.4 -> 12.6 us, 16 of up to 400 in tiles 65 -> 61; long ones as before.)
+// up to 61 rows, in tiles of 128, 13.4 -> 12.6 us, 16 of up to 400 in tiles 65 -> 61; long ones as before.)
 constexpr int kPaTurn = 256;  // pieces a wave
 struct PaTurn {
     vk_f32x4* lds;  // the wave's
@@ -619,24 +619,24 @@ struct PaWave {
 };
 
 // One unit: the wave's rows against the tile in LDS (K hi, K lo, V hi, V lo), whose first
-// key is kk.
-template <int HD>
+// key is kk, or (NY 1) the half y0 of its keys.
+template <int HD, int NY = 2>
 __device__ __forceinline__ void pa_unit(const PaArgs& a, const PaPiece& x, const PaWave<HD>& w, const _Float16* tile,
                                         const PaTileMeta& meta, int kk, vk_f32x16 (&o)[HD / 32], PaState& s,
-                                        float minus_one) {
+                                        float minus_one, int y0 = 0) {
     constexpr int KS = HD / 16, DB = HD / 32, P = pa_part(HD);
     const int lane = threadIdx.x & 63, h = lane >> 5, ve = meta.v_exp;
-    const pa_h8* kh = (const pa_h8*)tile + lane;
+    const pa_h8* kh = (const pa_h8*)tile + lane + y0 * (KS * 64);
     const pa_h8* kl = kh + P / 8;
-    const pa_h8* vh = kl + P / 8;
+    const pa_h8* vh = (const pa_h8*)tile + lane + 2 * (P / 8) + y0 * (2 * DB * 64);
     const pa_h8* vl = vh + P / 8;
     constexpr vk_f32x16 zero = {};
-    vk_f32x16 t[2];
+    vk_f32x16 t[NY];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
         const pa_h8 qhv = __builtin_bit_cast(pa_h8, w.qh[ks]), qlv = __builtin_bit_cast(pa_h8, w.ql[ks]);
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
+        for (int y = 0; y < NY; ++y) {
             const pa_h8 ah = kh[(y * KS + ks) * 64], al = kl[(y * KS + ks) * 64];
             t[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, qhv, ks ? t[y] : zero, 0, 0, 0);
             t[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, qlv, t[y], 0, 0, 0);
@@ -648,10 +648,10 @@ __device__ __forceinline__ void pa_unit(const PaArgs& a, const PaPiece& x, const
     const float c = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.c, w.qe + meta.k_exp), 0x1p-126f), 0x1.fffffep127f);
     if (kk + kPaKeys > w.all_to || kk < w.all_from) {
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
+        for (int y = 0; y < NY; ++y)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int key = 32 * y + 8 * (i >> 2) + 4 * h + (i & 3);
+                const int key = 32 * (y0 + y) + 8 * (i >> 2) + 4 * h + (i & 3);
                 t[y][i] = key < end && key >= begin ? t[y][i] : -INFINITY;
             }
     }
@@ -661,7 +661,7 @@ __device__ __forceinline__ void pa_unit(const PaArgs& a, const PaPiece& x, const
     asm("" : "+s"(inf));
     float most = -INFINITY;
 #pragma unroll
-    for (int y = 0; y < 2; ++y)
+    for (int y = 0; y < NY; ++y)
 #pragma unroll
         for (int i = 0; i < 16; i += 4)
             most = fmaxf(fmaxf(__builtin_amdgcn_fmed3f(t[y][i], t[y][i + 1], inf),
@@ -682,7 +682,7 @@ __device__ __forceinline__ void pa_unit(const PaArgs& a, const PaPiece& x, const
     }
     const float sub = s.m - 14.0f;
 #pragma unroll
-    for (int y = 0; y < 2; ++y) {
+    for (int y = 0; y < NY; ++y) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) t[y][i] = __builtin_amdgcn_exp2f(fmaf(t[y][i], c, -sub));
 #pragma unroll
@@ -691,12 +691,12 @@ __device__ __forceinline__ void pa_unit(const PaArgs& a, const PaPiece& x, const
     if (ve < s.e) {
         const float f = __builtin_amdgcn_ldexpf(1.0f, max(ve - s.e, -200));
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
+        for (int y = 0; y < NY; ++y)
 #pragma unroll
             for (int i = 0; i < 16; ++i) t[y][i] *= f;
     }
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
+    for (int y = 0; y < 2 * NY; ++y) {
         float z[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) z[j] = t[y >> 1][8 * (y & 1) + j];
@@ -718,7 +718,7 @@ __device__ __forceinline__ void pa_unit(const PaArgs& a, const PaPiece& x, const
         for (unsigned long long rest = meta.odd; rest; rest &= rest - 1) {
             const int key = __ffsll((unsigned long long)rest) - 1;
             const float* vp = a.v + (size_t)(x.k0 + kk + key) * a.v_stride + (size_t)x.head * HD + 4 * h;
-            if (key >= end || key < begin) continue;
+            if (key >= end || key < begin || (NY == 1 && key >> 5 != y0)) continue;
 #pragma unroll
             for (int b = 0; b < DB; ++b)
 #pragma unroll
@@ -825,6 +825,23 @@ __global__ __launch_bounds__(pa_tile_rows(HD) * 2) __attribute__((amdgpu_waves_p
     }
 }
 
+// Results so far and those of other keys of the same rows: y, and (M, sum, e) in ml.
+template <int DB>
+__device__ __forceinline__ void pa_add(vk_f32x16 (&o)[DB], PaState& s, const vk_f32x4 (&y)[4 * DB], const vk_f32x4& ml) {
+    const float m = fmaxf(s.m, ml[0]);
+    const int pe = __float_as_int(ml[2]), e = max(s.e, pe);
+    const float f0 = __builtin_amdgcn_exp2f(s.m - m), f1 = __builtin_amdgcn_exp2f(ml[0] - m);
+    const float g0 = f0 * __builtin_amdgcn_ldexpf(1.0f, max(s.e - e, -200));
+    const float g1 = f1 * __builtin_amdgcn_ldexpf(1.0f, max(pe - e, -200));
+    s.sum = s.sum * f0 + ml[1] * f1;
+    s.m = m;
+    s.e = e;
+#pragma unroll
+    for (int j = 0; j < DB * 4; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[j >> 2][4 * (j & 3) + c] = o[j >> 2][4 * (j & 3) + c] * g0 + y[j][c] * g1;
+}
+
 // A tile's pieces brought together, in their order: one workgroup for each share with a
 // tile's first piece. Bound by reading them (up to two a share, 135 KB each at 128): 16 - 20 us
 // at 128, 8 at 64.
@@ -852,44 +869,41 @@ __global__ __launch_bounds__(pa_tile_rows(HD) * 2) void vk_pattn_join(PaArgs a) 
         vk_f32x4 y[DB * 4];
 #pragma unroll
         for (int j = 0; j < DB * 4; ++j) y[j] = po[j * 64];
-        const float m = fmaxf(s.m, ml[0]);
-        const int pe = __float_as_int(ml[2]), e = max(s.e, pe);
-        const float f0 = __builtin_amdgcn_exp2f(s.m - m), f1 = __builtin_amdgcn_exp2f(ml[0] - m);
-        const float g0 = f0 * __builtin_amdgcn_ldexpf(1.0f, max(s.e - e, -200));
-        const float g1 = f1 * __builtin_amdgcn_ldexpf(1.0f, max(pe - e, -200));
-        s.sum = s.sum * f0 + ml[1] * f1;
-        s.m = m;
-        s.e = e;
-#pragma unroll
-        for (int j = 0; j < DB * 4; ++j)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[j >> 2][4 * (j & 3) + c] = o[j >> 2][4 * (j & 3) + c] * g0 + y[j][c] * g1;
+        pa_add(o, s, y, ml);
     }
     pa_store_rows<HD>(a, q0, open.head, rows, row0, o, s.sum, s.e, PaTurn(s_turn));
 }
 
 // ---- short sequences ----------------------------------------------------------------
 
-// Few units a tile: one launch, a workgroup a tile of 128 rows, whose threads pack each
-// tile of keys into LDS themselves. Nothing is planned, split or joined.
-constexpr int kShortRows = 128;
+// Few units a tile: one launch, a workgroup a tile of 128 or 64 rows, whose threads pack
+// each tile of keys into LDS themselves. Nothing is planned, split over workgroups or joined.
+// ROWS 128: a wave has 32 rows. 64: two waves have 32, each half of every tile's keys.
+// Bound by a wave's own steps, one after the other: loads, packing, products, weights (5.5
+// us a tile of 64 keys at head size 128 and 128 rows, 4 at 64).
 
-template <int HD>
+// Tiles of 64 rows where the chip holds them all at once (16 heads over 2 of 128, one sequence
+// of 256: 24.7 us, 28.2 with 128; of 400: 36.6 and 42.9; eleven of 8 heads of up to 300, more
+// than that: 51 and 34; 20 heads of 64, four of up to 226: 15.4 and 18.0)
+constexpr int short_few(int hd) { return hd == 64 ? 512 : 256; }
+
+template <int HD, int ROWS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 2 : 1, HD == 64 ? 2 : 1))) void vk_pattn_short(PaArgs a) {
-    constexpr int DB = HD / 32;
+    constexpr int DB = HD / 32, RG = ROWS / 32;
     __shared__ __align__(16) _Float16 s_t[4 * pa_part(HD)];
-    __shared__ vk_f32x4 s_turn[kShortRows / 32 * kPaTurn];
+    __shared__ vk_f32x4 s_turn[4 * kPaTurn];
     __shared__ PaSeqLds s_seq;
     __shared__ PaPackLds s_lds;
     const PaTurn turn(s_turn);
-    const int slot = blockIdx.x;
+    const int slot = blockIdx.x, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), rw = wave % RG, half = wave / RG;
     PaPiece p;
     p.head = blockIdx.y;
-    if (!pa_find(a, slot, s_seq, p, [&](int q0, int, int s) { return pa_q_slot<kShortRows>(a, q0, s); })) return;
+    if (!pa_find(a, slot, s_seq, p, [&](int q0, int, int s) { return pa_q_slot<ROWS>(a, q0, s); })) return;
     const int rows = p.n * a.g;
-    p.row0 = (slot - pa_q_slot<kShortRows>(a, p.q0, p.seq)) * kShortRows;
+    p.row0 = (slot - pa_q_slot<ROWS>(a, p.q0, p.seq)) * ROWS;
     if (p.row0 >= rows) return;
-    pa_span<kShortRows>(a, p.n, p.m, p.row0, &p.lo, &p.units);
+    pa_span<ROWS>(a, p.n, p.m, p.row0, &p.lo, &p.units);
     const float minus_one = pa_minus_one();
     PaPack<HD> t;
     auto load = [&](int kk) __attribute__((always_inline)) {
@@ -900,7 +914,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
     const int end = min(p.m, (p.lo + p.units) * kPaKeys);
     if (kk < end) load(kk);
     PaWave<HD> w;
-    w.load(a, p, threadIdx.x >> 6, turn);
+    w.load(a, p, rw, turn);
     vk_f32x16 o[DB];
 #pragma unroll
     for (int b = 0; b < DB; ++b)
@@ -910,9 +924,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
     while (kk < end) {
         const PaTileMeta meta = t.store((pa_u4*)s_t, s_lds);  // (once all waves are through with the tile before)
         VK_LDS_BARRIER();
-        if (w.sees(kk)) pa_unit<HD>(a, p, w, s_t, meta, kk, o, s, minus_one);
+        if (w.sees(kk)) pa_unit<HD, RG / 2>(a, p, w, s_t, meta, kk, o, s, minus_one, half);
         kk += kPaKeys;
         if (kk < end) load(kk);
+    }
+    if constexpr (RG == 2) {
+        VK_LDS_BARRIER();  // all are through with the tile
+        vk_f32x4* po = (vk_f32x4*)s_t + rw * (HD / 8) * 64 + lane;
+        if (half) {
+#pragma unroll
+            for (int b = 0; b < DB; ++b)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    po[(b * 4 + j) * 64] = vk_f32x4{o[b][4 * j], o[b][4 * j + 1], o[b][4 * j + 2], o[b][4 * j + 3]};
+            s_turn[wave * kPaTurn + lane] = vk_f32x4{s.m, s.sum, __int_as_float(s.e), 0.0f};
+        }
+        VK_LDS_BARRIER();
+        if (half) return;
+        vk_f32x4 y[DB * 4];
+#pragma unroll
+        for (int j = 0; j < DB * 4; ++j) y[j] = po[j * 64];
+        pa_add(o, s, y, s_turn[(wave + RG) * kPaTurn + lane]);
     }
     pa_store_rows<HD>(a, p.q0, p.head, rows, p.row0, o, pa_row_sum(s.sum), s.e, turn);
 }
@@ -1257,15 +1289,18 @@ hipError_t launch_pattn(hipStream_t s, int hd, const PaArgs& a) {
     // 82 us, 96 packed; 16 heads over 2: 67 and 61; three of up to 61: 8 and 17), at 128, where
     // a workgroup has a CU to itself, up to 448 keys (four of up to 400, 8 heads: 42 and 46, 16
     // over 2: 47 and 50; of 512: 55 and 49) and two rounds of workgroups (16 of up to 400, 16
-    // over 2: 88 and 61); three of up to 61: 13 and 21
-    const long long tiles = ((long long)a.q_rows * a.g / kShortRows + a.n_seq) * a.hkv;
+    // over 2: 88 and 61); three of up to 61: 12 and 21
+    auto tiles = [&](int rows) { return ((long long)a.q_rows * a.g / rows + a.n_seq) * a.hkv; };
     // and long ones of which a tile's rows see up to 320 (20 heads of 64, four of up to 1500, a
     // window of 100: 47 and 60, of 400: 80 and 76; 8 heads of 128, one of 1000, of 128: 29 and 45)
-    const int most = a.causal && a.window && a.window + kShortRows / a.g <= 320 ? 320 : a.max_k;
-    if (hd == 64 ? most <= 512 : most <= 448 && tiles <= 512) {
-        const dim3 grid((unsigned)(tiles / a.hkv), (unsigned)a.hkv);
-        if (hd == 64) hipLaunchKernelGGL(vk_pattn_short<64>, grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL(vk_pattn_short<128>, grid, dim3(256), 0, s, a);
+    const int most = a.causal && a.window && a.window + 128 / a.g <= 320 ? 320 : a.max_k;
+    if (hd == 64 ? most <= 512 : most <= 448 && tiles(128) <= 512) {
+        const bool few = tiles(64) <= short_few(hd);
+        const dim3 grid((unsigned)(tiles(few ? 64 : 128) / a.hkv), (unsigned)a.hkv);
+        if (hd == 64 && few) hipLaunchKernelGGL((vk_pattn_short<64, 64>), grid, dim3(256), 0, s, a);
+        else if (hd == 64) hipLaunchKernelGGL((vk_pattn_short<64, 128>), grid, dim3(256), 0, s, a);
+        else if (few) hipLaunchKernelGGL((vk_pattn_short<128, 64>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((vk_pattn_short<128, 128>), grid, dim3(256), 0, s, a);
         return hipGetLastError();
     }
     return hd == 64 ? go_pattn<64>(s, a) : go_pattn<128>(s, a);
