@@ -112,6 +112,8 @@ def test_lengths_heads_and_masks(ctx, hq, hkv, hd, case):
     (8, 1, 128, [33, 385, 1, 64], None, True, 70),
     (2, 2, 64, [700, 3], [900, 5], True, 191), (2, 1, 64, [700, 3], [900, 5], True, 257), (4, 2, 128, [1000], None, True, 1),
     (1, 1, 128, [80, 600], [1600, 600], True, 130),  # long ones, each row of few keys
+    (8, 8, 128, [200, 300, 250, 100, 33, 299, 128, 64, 1, 0, 257], None, True, 0),  # short ones, many tiles
+    (4, 2, 64, [250] * 39 + [17], None, True, 90),
     (2, 1, 128, [40] * 300, None, True, 0)])  # short ones beyond two rounds of workgroups
 def test_keys_split_over_workgroups(ctx, hq, hkv, hd, ql, kl, causal, window):
     print("[case] packed split", hq, hkv, hd, ql[:3], causal, window, flush=True)
@@ -190,7 +192,8 @@ def test_values_of_any_size(ctx, ql, kl, causal):
     (2, 1, 64, [100, 90], [100, 90], True, 0), (2, 2, 128, [100, 90], [100, 90], True, 20),
     (3, 1, 64, [5, 4], [100, 90], True, 0), (2, 1, 64, [5, 4], [100, 90], False, 0), (2, 2, 128, [1, 1], [100, 90], True, 30),
     (2, 1, 64, [5, 4], [100, 90], True, 20), (2, 2, 128, [7, 13], [100, 90], True, 9), (4, 1, 64, [8, 6], [100, 90], True, 70),
-    (2, 1, 128, [16, 9], [100, 90], True, 0)])
+    (2, 1, 128, [16, 9], [100, 90], True, 0), (2, 1, 64, [600, 90], [600, 90], True, 0), (2, 2, 128, [600, 90], [600, 90], True, 99),
+    (64, 64, 128, [100, 90], [100, 90], True, 0), (160, 160, 64, [100, 90], [100, 90], True, 33)])  # in each way
 def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(ctx, hq, hkv, hd, ql, kl, causal, window):
     print("[case] packed nan", hq, hkv, hd, ql, causal, window, flush=True)
     g = np.random.default_rng(9)
