@@ -13,7 +13,7 @@
 //
 // Two launches. Slices: a workgroup reads up to 4096 or 8192 columns of a row once, into
 // registers, and leaves their maximum, the sum of their exponentials and their n_out best
-// columns. Merge: a workgroup a group joins the slices' sums (64 bits: totals of
+// columns. Merge: a workgroup a group joins the slices' sums (in 64 bits: totals of
 // different beams are compared, and near ones have to fall in order), takes each
 // beam's best from its slices' lists and the group's from its beams'.
 //
@@ -254,9 +254,11 @@ __global__ __launch_bounds__(BM_MT) void vk_beam_merge(BeamArgs a) {
         float m = first.max;
         for (int s = lane + 64; s < a.slices; s += 64) m = fmaxf(m, st[s].max);
         m = vk_group_maxf<64>(m);
-        double sum = first.max > -INFINITY ? first.sum * exp((double)first.max - (double)m) : 0.0;
+        // e^(max - m) in f32, as the slices' exponentials (in 64 bits 0.7 us more, by its instructions alone)
+        auto under = [m](float max) { return (double)__builtin_amdgcn_exp2f((max - m) * 1.44269504088896340736f); };
+        double sum = first.max > -INFINITY ? first.sum * under(first.max) : 0.0;
         for (int s = lane + 64; s < a.slices; s += 64)
-            if (st[s].max > -INFINITY) sum += st[s].sum * exp((double)st[s].max - (double)m);
+            if (st[s].max > -INFINITY) sum += st[s].sum * under(st[s].max);
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, VK_WAVE);
         const double lse = (double)m + log(sum);
