@@ -53,23 +53,28 @@ __device__ __forceinline__ int bm_column(unsigned long long key) { return (int)(
 // (see vk_bfly_partner; the last two steps swap rows and halves), 6 steps of some 30 cycles
 // where ds_bpermute's take 150.
 template <int O>
-__device__ __forceinline__ unsigned long long bm_max_step(unsigned long long k) {
+__device__ __forceinline__ void bm_partners(unsigned long long k, unsigned long long& x, unsigned long long& y) {
     const uint32_t lo = (uint32_t)k, hi = (uint32_t)(k >> 32);
-    unsigned long long y;
+    x = k;
     if constexpr (O < 16) {
         y = ((unsigned long long)(uint32_t)vk_bfly_partner<O>((int)hi) << 32) | (uint32_t)vk_bfly_partner<O>((int)lo);
     } else if constexpr (O == 16) {
         const auto a = __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
         const auto b = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
-        k = ((unsigned long long)b[0] << 32) | a[0];
+        x = ((unsigned long long)b[0] << 32) | a[0];
         y = ((unsigned long long)b[1] << 32) | a[1];
     } else {
         const auto a = __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
         const auto b = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
-        k = ((unsigned long long)b[0] << 32) | a[0];
+        x = ((unsigned long long)b[0] << 32) | a[0];
         y = ((unsigned long long)b[1] << 32) | a[1];
     }
-    return y > k ? y : k;
+}
+template <int O>
+__device__ __forceinline__ unsigned long long bm_max_step(unsigned long long k) {
+    unsigned long long x, y;
+    bm_partners<O>(k, x, y);
+    return y > x ? y : x;
 }
 __device__ __forceinline__ unsigned long long bm_wave_max(unsigned long long k) {
     k = bm_max_step<1>(k);
@@ -78,6 +83,22 @@ __device__ __forceinline__ unsigned long long bm_wave_max(unsigned long long k) 
     k = bm_max_step<8>(k);
     k = bm_max_step<16>(k);
     return bm_max_step<32>(k);
+}
+
+// The sum over the wave likewise, in a fixed order
+template <int O>
+__device__ __forceinline__ double bm_sum_step(double v) {
+    unsigned long long x, y;
+    bm_partners<O>((unsigned long long)__double_as_longlong(v), x, y);
+    return __longlong_as_double((long long)x) + __longlong_as_double((long long)y);
+}
+__device__ __forceinline__ double bm_wave_sum(double v) {
+    v = bm_sum_step<1>(v);
+    v = bm_sum_step<2>(v);
+    v = bm_sum_step<4>(v);
+    v = bm_sum_step<8>(v);
+    v = bm_sum_step<16>(v);
+    return bm_sum_step<32>(v);
 }
 
 // Doubles in the order of their bits, above 0 (0: none)
@@ -162,9 +183,7 @@ __global__ __launch_bounds__(BM_T) void vk_beam_slices(BeamArgs a) {
 #pragma unroll
         for (int j = 0; j < E; ++j) sum += __builtin_amdgcn_exp2f((y[j] - m) * l);
     }
-    double total = (double)sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o, VK_WAVE);
+    const double total = bm_wave_sum((double)sum);
     if (lane == 0) s_sum[wave] = total;
     const float from = fmaxf(bound, -0x1.fffffep127f);  // (what is -inf is none)
     if (__any(most >= from))
@@ -259,8 +278,7 @@ __global__ __launch_bounds__(BM_MT) void vk_beam_merge(BeamArgs a) {
         double sum = first.max > -INFINITY ? first.sum * under(first.max) : 0.0;
         for (int s = lane + 64; s < a.slices; s += 64)
             if (st[s].max > -INFINITY) sum += st[s].sum * under(st[s].max);
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, VK_WAVE);
+        sum = bm_wave_sum(sum);
         const double lse = (double)m + log(sum);
         int taken = 0;
         unsigned long long got = 0;  // lane i: the i-th best
