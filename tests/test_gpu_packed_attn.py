@@ -142,6 +142,28 @@ def test_the_ends_of_the_ranges(ctx, hq, hkv, hd, ql, kl, causal, window):
     check(got, *attend(q, k, v, ql, kl, hq, hkv, hd ** -0.5, causal, window))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,hd,n,causal", [(2, 1, 128, 1500, True), (2, 2, 64, 2100, False), (16, 2, 64, 5000, True),
+                                                (1, 1, 128, 9000, True), (20, 1, 64, 1, False)])
+def test_the_same_bits_every_time(ctx, hq, hkv, hd, n, causal):
+    """Whichever workgroup joins a tile's pieces."""
+    print("[case] packed again", hq, hkv, hd, n, flush=True)
+    g = np.random.default_rng(n)
+    m = max(n, 3000)
+    q, k, v = rows(g, n, m, hq, hkv, hd)
+    plan = ctx.packed_attn(1, n, m, hq, hkv, hd)
+    d_q, d_k, d_v, d_o = (_up(ctx, a) for a in (q, k, v, np.zeros_like(q)))
+    qo, ko = _up(ctx, np.array([0, n], np.int32)), _up(ctx, np.array([0, m], np.int32))
+    first = None
+    for _ in range(25):
+        d_o.upload(np.zeros_like(q))
+        plan.attn_dev(1, n, m, n, m, qo, ko, d_q, d_k, d_v, hd ** -0.5, d_o, causal=causal)
+        ctx.synchronize()
+        got = d_o.download(F, q.size)
+        assert first is None or np.array_equal(got, first)
+        first = got
+
+
 FEW = [(1, 1, 64, [1], [1]), (8, 1, 128, [1, 1, 1], [3, 900, 64]), (20, 20, 64, [5] * 6, [97, 1, 1500, 0, 16, 333]),
        (2, 2, 128, [7, 0, 16, 3], [40, 9, 2000, 17]), (6, 2, 64, [10, 1], [5000, 15]), (32, 1, 64, [1], [70]),
        (4, 2, 128, [16, 2], [33, 3000]), (16, 1, 128, [1], [20000]), (3, 3, 64, [32, 1], [9001, 70]),

@@ -27,11 +27,6 @@ struct alignas(16) PaStart {
     long long line;       // that tile's place on the line
 };
 
-// A tile that several shares have: written by the share with its first unit.
-struct alignas(16) PaOpen {
-    int seq, head, slot, pieces;  // pieces 0: none
-};
-
 struct PaArgs {
     const float *q, *k, *v;
     float* out;
@@ -46,8 +41,8 @@ struct PaArgs {
     PaTileMeta* meta;        // [slot of 64 keys][kv head]
     long long* line;         // [slot of a tile of rows + 1] cost of the tiles before, of one kv head
     PaStart* start;          // [kPaShares]
-    PaOpen* open;            // [kPaShares]
-    long long* plan;         // [0] a share's length, [1] the line's, [2] shares, [3] sequences in order
+    int* ended;              // [kPaShares] pieces of the tile whose first unit a share has that have ended
+    long long* plan;         // [0] a share's length, [1] the line's, [2] sequences in order
     float* part;             // partial results: [share][2] pieces
     int q_slots, k_slots;    // places of tiles
 };

@@ -26,7 +26,7 @@
 // Even shares: the tiles' units (64 keys each, and two more for a tile's start and
 // end) lie on one line, which the workgroups that the chip holds at once (two waves a
 // SIMD) share evenly whatever the lengths are; a share holds whole tiles and at most two
-// pieces, whose results vk_pattn_join brings together.
+// pieces, whose results the last share of a tile to end brings together.
 #include <algorithm>
 
 #include "vk_common.h"
@@ -376,12 +376,12 @@ __device__ void pa_plan(const PaArgs& a) {
     if (t == 0) {
         a.plan[0] = size;
         a.plan[1] = total;
-        a.plan[2] = shares ? (total + size - 1) / size : 0;
-        a.plan[3] = n;
+        a.plan[2] = n;
     }
     __syncthreads();  // line is written (and read by this workgroup alone)
     __threadfence_block();
     for (int i = t; i < pa_shares(HD); i += 256) {
+        a.ended[i] = 0;
         const long long x = i * size;
         if (!size || x >= total) continue;
         // the sequence: lines of sequence s begin at hkv line[its first place]
@@ -733,11 +733,67 @@ __device__ __forceinline__ void pa_unit(const PaArgs& a, const PaPiece& x, const
     }
 }
 
+// Results so far and those of other keys of the same rows: y, and (M, sum, e) in ml.
+template <int DB>
+__device__ __forceinline__ void pa_add(vk_f32x16 (&o)[DB], PaState& s, const vk_f32x4 (&y)[4 * DB], const vk_f32x4& ml) {
+    const float m = fmaxf(s.m, ml[0]);
+    const int pe = __float_as_int(ml[2]), e = max(s.e, pe);
+    const float f0 = __builtin_amdgcn_exp2f(s.m - m), f1 = __builtin_amdgcn_exp2f(ml[0] - m);
+    const float g0 = f0 * __builtin_amdgcn_ldexpf(1.0f, max(s.e - e, -200));
+    const float g1 = f1 * __builtin_amdgcn_ldexpf(1.0f, max(pe - e, -200));
+    s.sum = s.sum * f0 + ml[1] * f1;
+    s.m = m;
+    s.e = e;
+#pragma unroll
+    for (int j = 0; j < DB * 4; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[j >> 2][4 * (j & 3) + c] = o[j >> 2][4 * (j & 3) + c] * g0 + y[j][c] * g1;
+}
+
+// A piece's results in memory: of this share's pieces, or of another's that has ended, which may
+// be on another XCD. Past the caches that are an XCD's own (policy bit 4, sc1, as an access of
+// the device's scope carries).
+template <int HD>
+struct PaParts {
+    __amdgpu_buffer_rsrc_t r;
+    int at;  // this lane's first 16 bytes of a piece
+    __device__ __forceinline__ PaParts(const PaArgs& a)
+        : r(__builtin_amdgcn_make_buffer_rsrc((void*)a.part, 0, (int)(2 * pa_shares(HD) * pa_piece_floats(HD) * 4), 0x20000)) {
+        at = ((int)(threadIdx.x >> 6) * (HD / 8) * 64 + (int)(threadIdx.x & 63)) * 16;
+    }
+    __device__ __forceinline__ int state(int piece) const {
+        return (int)(piece * pa_piece_floats(HD) * 4) + pa_tile_rows(HD) * HD * 4 +
+               ((int)(threadIdx.x >> 6) * 32 + (int)(threadIdx.x & 31)) * 16;
+    }
+    __device__ __forceinline__ void put(int piece, const vk_f32x16 (&o)[HD / 32], const PaState& s) const {
+        const int base = (int)(piece * pa_piece_floats(HD) * 4) + at;
+#pragma unroll
+        for (int b = 0; b < HD / 32; ++b)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const vk_f32x4 y = {o[b][4 * j], o[b][4 * j + 1], o[b][4 * j + 2], o[b][4 * j + 3]};
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(pa_u4, y), r, base + (b * 4 + j) * 1024, 0, 16);
+            }
+        if ((threadIdx.x & 32) == 0)
+            __builtin_amdgcn_raw_buffer_store_b128(
+                __builtin_bit_cast(pa_u4, vk_f32x4{s.m, s.sum, __int_as_float(s.e), 0.0f}), r, state(piece), 0, 16);
+    }
+    __device__ __forceinline__ void add(int piece, vk_f32x16 (&o)[HD / 32], PaState& s) const {
+        const int base = (int)(piece * pa_piece_floats(HD) * 4) + at;
+        const vk_f32x4 ml = __builtin_bit_cast(vk_f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, state(piece), 0, 16));
+        vk_f32x4 y[HD / 8];
+#pragma unroll
+        for (int j = 0; j < HD / 8; ++j)
+            y[j] = __builtin_bit_cast(vk_f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, base + j * 1024, 0, 16));
+        pa_add(o, s, y, ml);
+    }
+};
+
 // Bound by the matrix instructions and the clock that they leave: two documents of 5001 and
-// 8192 rows, causal, 32 heads over 8 of 128, take 2.05 ms (0.37 PFLOP/s at f32 level, 1.1 in
-// fp16 products, 87% of what a large library product of fp16 reaches), 16 prompts of up
-// to 2048 rows, 16 heads over 2, 322 us (0.9), eight utterances of up to 1500 rows, 20 heads
-// of 64, 127 us (0.82). Loads of q ahead of a tile's end and stores that nothing waits for
+// 8192 rows, causal, 32 heads over 8 of 128, take 2.04 ms (0.37 PFLOP/s at f32 level, 1.1 in
+// fp16 products, 88% of what a large library product of fp16 reaches), 16 prompts of up
+// to 2048 rows, 16 heads over 2, 315 us (0.92), eight utterances of up to 1500 rows, 20 heads
+// of 64, 125 us (0.83). Loads of q ahead of a tile's end and stores that nothing waits for
 // changed none of them.
 // Tiles go global -> LDS directly, the next one (of the next piece, too) while this one
 // is worked on: two buffers, one barrier a unit, between which the two waves of a SIMD
@@ -749,14 +805,14 @@ __global__ __launch_bounds__(pa_tile_rows(HD) * 2) __attribute__((amdgpu_waves_p
     __shared__ __align__(16) _Float16 s_t[2][4 * P];  // K hi, K lo, V hi, V lo
     __shared__ vk_f32x4 s_turn[NW * kPaTurn];
     const PaTurn turn(s_turn);
+    const PaParts<HD> parts(a);
     const int share = vk_xcd_tile(blockIdx.x, gridDim.x);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int h = lane >> 5, l = lane & 31;
     const PaStart st = a.start[share];
     const long long size = a.plan[0], total = a.plan[1];
-    const int n_seq = (int)a.plan[3];
+    const int n_seq = (int)a.plan[2];
     const long long x0 = share * size, x1 = min(x0 + size, total);
-    if (threadIdx.x == 0) a.open[share] = PaOpen{0, 0, 0, 0};
     if (x0 >= x1) return;
     PaPiece p;
     p.seq = __builtin_amdgcn_readfirstlane(st.seq);
@@ -806,72 +862,45 @@ __global__ __launch_bounds__(pa_tile_rows(HD) * 2) __attribute__((amdgpu_waves_p
         if (p.u0 == 0 && p.u1 == p.units) {
             pa_store_rows<HD>(a, p.q0, p.head, rows, p.row0, o, s.sum, s.e, turn);
         } else {
-            float* part = a.part + (size_t)(2 * share + (p.u0 == 0 ? 1 : 0)) * pa_piece_floats(HD);
-            vk_f32x4* po = (vk_f32x4*)part + wave * (HD / 8) * 64 + lane;
+            // shares owner .. owner + pieces - 1 have pieces of this tile. The last of them to end
+            // joins all, in their order (of two, either order gives the same sums, so the one held
+            // here need not pass through memory). All write before any counts itself, nothing
+            // spins. (By a launch of its own: prompts 345 us for 335, utterances 151 for 146.)
+            const long long first = p.line + pa_cost(HD);
+            const int owner = (int)(first / size), pieces = (int)((first + p.units - 1) / size) - owner + 1;
+            const bool two = pieces == 2;
+            int* const ended = (int*)s_turn;  // (where no row of q or out is now)
+            bool last = false;
+            if (two) {
+                if (threadIdx.x == 0) *ended = __hip_atomic_load(&a.ended[owner], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                VK_LDS_BARRIER();
+                last = *ended == 1;
+                VK_LDS_BARRIER();
+            }
+            if (!last) {
+                parts.put(2 * share + (p.u0 == 0 ? 1 : 0), o, s);
+                vk_wait_vm<0>();
+                VK_LDS_BARRIER();
+                if (threadIdx.x == 0) *ended = atomicAdd(&a.ended[owner], 1);
+                VK_LDS_BARRIER();
+                last = *ended == pieces - 1;
+                VK_LDS_BARRIER();
+            }
+            if (last) {
+                if (!two) {
 #pragma unroll
-            for (int b = 0; b < DB; ++b)
+                    for (int b = 0; b < DB; ++b)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    po[(b * 4 + j) * 64] = vk_f32x4{o[b][4 * j], o[b][4 * j + 1], o[b][4 * j + 2], o[b][4 * j + 3]};
-            if (h == 0)
-                ((vk_f32x4*)(part + (size_t)pa_tile_rows(HD) * HD))[wave * 32 + l] =
-                    vk_f32x4{s.m, s.sum, __int_as_float(s.e), 0.0f};
-            if (p.u0 == 0 && threadIdx.x == 0) {
-                const int last = (int)((p.line + pa_cost(HD) + p.units - 1) / size);  // the share with the last unit
-                a.open[share] = PaOpen{p.seq, p.head, p.slot, last - share + 1};
+                        for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
+                    s = PaState{kNoMax, 0.0f, kPaNoValue};
+                }
+                for (int i = 0; i < pieces; ++i)
+                    if (!two || i != share - owner) parts.add(2 * (owner + i) + (i == 0 ? 1 : 0), o, s);
+                pa_store_rows<HD>(a, p.q0, p.head, rows, p.row0, o, s.sum, s.e, turn);
             }
         }
         p = next;
     }
-}
-
-// Results so far and those of other keys of the same rows: y, and (M, sum, e) in ml.
-template <int DB>
-__device__ __forceinline__ void pa_add(vk_f32x16 (&o)[DB], PaState& s, const vk_f32x4 (&y)[4 * DB], const vk_f32x4& ml) {
-    const float m = fmaxf(s.m, ml[0]);
-    const int pe = __float_as_int(ml[2]), e = max(s.e, pe);
-    const float f0 = __builtin_amdgcn_exp2f(s.m - m), f1 = __builtin_amdgcn_exp2f(ml[0] - m);
-    const float g0 = f0 * __builtin_amdgcn_ldexpf(1.0f, max(s.e - e, -200));
-    const float g1 = f1 * __builtin_amdgcn_ldexpf(1.0f, max(pe - e, -200));
-    s.sum = s.sum * f0 + ml[1] * f1;
-    s.m = m;
-    s.e = e;
-#pragma unroll
-    for (int j = 0; j < DB * 4; ++j)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[j >> 2][4 * (j & 3) + c] = o[j >> 2][4 * (j & 3) + c] * g0 + y[j][c] * g1;
-}
-
-// A tile's pieces brought together, in their order: one workgroup for each share with a
-// tile's first piece. Bound by reading them (up to two a share, 135 KB each at 128): 16 - 20 us
-// at 128, 8 at 64.
-template <int HD>
-__global__ __launch_bounds__(pa_tile_rows(HD) * 2) void vk_pattn_join(PaArgs a) {
-    constexpr int DB = HD / 32;
-    __shared__ vk_f32x4 s_turn[pa_tile_rows(HD) / 32 * kPaTurn];
-    const int share = blockIdx.x;
-    if (share >= (int)a.plan[2]) return;
-    const PaOpen open = a.open[share];
-    if (open.pieces < 2) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 31;
-    const int q0 = a.q_off[open.seq], rows = (a.q_off[open.seq + 1] - q0) * a.g;
-    const int row0 = (open.slot - pa_q_slot<pa_tile_rows(HD)>(a, q0, open.seq)) * pa_tile_rows(HD);
-    vk_f32x16 o[DB];
-#pragma unroll
-    for (int b = 0; b < DB; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
-    PaState s = {kNoMax, 0.0f, kPaNoValue};
-    for (int p = 0; p < open.pieces; ++p) {
-        const float* part = a.part + (size_t)(2 * (share + p) + (p == 0 ? 1 : 0)) * pa_piece_floats(HD);
-        const vk_f32x4* po = (const vk_f32x4*)part + wave * (HD / 8) * 64 + lane;
-        const vk_f32x4 ml = ((const vk_f32x4*)(part + (size_t)pa_tile_rows(HD) * HD))[wave * 32 + l];
-        vk_f32x4 y[DB * 4];
-#pragma unroll
-        for (int j = 0; j < DB * 4; ++j) y[j] = po[j * 64];
-        pa_add(o, s, y, ml);
-    }
-    pa_store_rows<HD>(a, q0, open.head, rows, row0, o, s.sum, s.e, PaTurn(s_turn));
 }
 
 // ---- short sequences ----------------------------------------------------------------
@@ -1271,7 +1300,6 @@ template <int HD>
 static hipError_t go_pattn(hipStream_t s, const PaArgs& a) {
     hipLaunchKernelGGL(vk_pattn_pack<HD>, dim3((unsigned)a.k_slots + 1, (unsigned)a.hkv), dim3(256), 0, s, a);
     hipLaunchKernelGGL(vk_pattn<HD>, dim3(pa_shares(HD)), dim3(2 * pa_tile_rows(HD)), 0, s, a);
-    hipLaunchKernelGGL(vk_pattn_join<HD>, dim3(pa_shares(HD)), dim3(2 * pa_tile_rows(HD)), 0, s, a);
     return hipGetLastError();
 }
 

@@ -109,7 +109,7 @@ int vokra_hip_packed_attn_create(vokra_hip_ctx_t* c, size_t max_seq, size_t max_
     } all[] = {{&p->tiles, ks * n_head_kv * 4 * kPaKeys * head_dim * 2},
                {&p->meta, ks * n_head_kv * sizeof(PaTileMeta)},
                {&p->line, (qs + 1) * sizeof(long long)},
-               {&p->shares, kPaShares * (sizeof(PaStart) + sizeof(PaOpen)) + 4 * sizeof(long long)},
+               {&p->shares, kPaShares * (sizeof(PaStart) + sizeof(int)) + 3 * sizeof(long long)},
                {&p->part, vk::pattn_part_floats((int)head_dim) * sizeof(float)}};
     hipError_t e = hipSuccess;
     for (auto& x : all)
@@ -180,8 +180,8 @@ int vokra_hip_packed_attn_dev(vokra_hip_ctx_t* c, vokra_hip_packed_attn_t* p, si
     a.meta = (PaTileMeta*)p->meta;
     a.line = (long long*)p->line;
     a.start = (PaStart*)p->shares;
-    a.open = (PaOpen*)(a.start + kPaShares);
-    a.plan = (long long*)(a.open + kPaShares);
+    a.ended = (int*)(a.start + kPaShares);
+    a.plan = (long long*)(a.ended + kPaShares);
     a.part = (float*)p->part;
     a.q_slots = (int)places(n_q_rows * (size_t)a.g, (size_t)pa_tile_rows((int)p->hd), n_seq);
     a.k_slots = (int)places(n_k_rows, kPaKeys, n_seq);
