@@ -186,6 +186,25 @@ def test_strides_in_place_and_in_a_graph(ctx):
 
 
 @pytest.mark.gpu
+def test_rows_far_apart(ctx):
+    """Rows of logits more than 2^32 bytes apart."""
+    print("[case] beam far", flush=True)
+    g = np.random.default_rng(4)
+    x, stride = logits(g, 1, 2, 5000), (1 << 30) + 3
+    wide = hip.DeviceBuffer(ctx, (stride + 5000) * 4)
+    for b in (0, 1):
+        hip._check(hip.lib().vokra_hip_memcpy_htod(ctx._h, C.c_void_p(wide.ptr.value + b * stride * 4),
+                                                   x[0, b].ctypes.data_as(C.c_void_p), x[0, b].nbytes))
+    scores = np.array([[-1.0, -2.0]], F)
+    d_s = hip.DeviceBuffer.from_array(ctx, scores)
+    out = [hip.DeviceBuffer.from_array(ctx, np.zeros((1, 7), t)) for t in (F, np.int32, np.int32, np.int32)]
+    ctx.beam_select(1, 2, 5000, 7).select_dev(1, 2, 5000, 7, wide, d_s, *out[:3], d_out_ended=out[3], stride=stride)
+    ctx.synchronize()
+    got = [b.download(t, 7).reshape(1, 7) for b, t in zip(out, (F, np.int32, np.int32, np.int32))]
+    check(got, select(x, scores, 7))
+
+
+@pytest.mark.gpu
 def test_refusals(ctx):
     print("[case] beam refusals", flush=True)
     for a in ((0, 1, 1, 1), (1, 0, 1, 1), (1, 33, 1, 1), (1, 1, 2 ** 24 + 1, 1), (1, 1, 1, 65), (1, 1, 0, 1), (1, 1, 1, 0),

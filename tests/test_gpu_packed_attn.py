@@ -164,6 +164,41 @@ def test_the_same_bits_every_time(ctx, hq, hkv, hd, n, causal):
         first = got
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,stride", [(140, 1 << 23), (600, 1 << 21)])
+def test_rows_far_apart(ctx, n, stride):
+    """Rows of a projection more than 2^32 bytes apart, and of outputs."""
+    print("[case] packed far", n, stride, flush=True)
+    g = np.random.default_rng(n)
+    hq, hkv, hd = 2, 1, 64
+    q, k, v = rows(g, n, n, hq, hkv, hd)
+    wide = hip.DeviceBuffer(ctx, ((n - 1) * stride + 4 * hd) * 4)
+    x = np.concatenate([q, k, v], 1)
+    at = lambda row, col=0: C.c_void_p(wide.ptr.value + (row * stride + col) * 4)  # noqa: E731
+    for r in range(n):
+        hip._check(hip.lib().vokra_hip_memcpy_htod(ctx._h, at(r), np.ascontiguousarray(x[r]).ctypes.data_as(C.c_void_p),
+                                                   x[r].nbytes))
+    d_q, d_k, d_v = (At(wide, c) for c in (0, 2 * hd, 3 * hd))
+    d_o, d_small = _up(ctx, np.zeros_like(q)), [_up(ctx, a) for a in (q, k, v)]
+    off = _up(ctx, np.array([0, n], np.int32))
+    plan = ctx.packed_attn(1, n, n, hq, hkv, hd)
+    want, tol = attend(q, k, v, [n], [n], hq, hkv, hd ** -0.5, True)
+    plan.attn_dev(1, n, n, n, n, off, None, d_q, d_k, d_v, hd ** -0.5, d_o, causal=True, q_stride=stride, k_stride=stride,
+                  v_stride=stride)
+    ctx.synchronize()
+    check(d_o.download(F, q.size), want, tol)
+    few = _up(ctx, np.array([0, 3], np.int32))
+    plan.attn_dev(1, 3, n, 3, n, few, off, d_small[0], d_k, d_v, hd ** -0.5, d_o, k_stride=stride, v_stride=stride)
+    ctx.synchronize()
+    check(d_o.download(F, 3 * hq * hd), *attend(q[:3], k, v, [3], [n], hq, hkv, hd ** -0.5))
+    plan.attn_dev(1, n, n, n, n, off, None, *d_small, hd ** -0.5, wide, causal=True, out_stride=stride)
+    ctx.synchronize()
+    got = np.empty((n, hq * hd), F)
+    for r in range(n):
+        hip._check(hip.lib().vokra_hip_memcpy_dtoh(ctx._h, got[r].ctypes.data_as(C.c_void_p), at(r), got[r].nbytes))
+    check(got, want, tol)
+
+
 FEW = [(1, 1, 64, [1], [1]), (8, 1, 128, [1, 1, 1], [3, 900, 64]), (20, 20, 64, [5] * 6, [97, 1, 1500, 0, 16, 333]),
        (2, 2, 128, [7, 0, 16, 3], [40, 9, 2000, 17]), (6, 2, 64, [10, 1], [5000, 15]), (32, 1, 64, [1], [70]),
        (4, 2, 128, [16, 2], [33, 3000]), (16, 1, 128, [1], [20000]), (3, 3, 64, [32, 1], [9001, 70]),
