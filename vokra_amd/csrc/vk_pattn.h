@@ -44,7 +44,7 @@ struct PaArgs {
     int* ended;              // [kPaShares] pieces of the tile whose first unit a share has that have ended
     long long* plan;         // [0] a share's length, [1] the line's, [2] sequences in order
     float* part;             // partial results: [share][2] pieces
-    int q_slots, k_slots;    // places of tiles
+    int k_slots;             // places of tiles of keys
 };
 
 namespace vk {

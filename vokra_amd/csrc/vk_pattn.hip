@@ -342,7 +342,8 @@ __device__ void pa_plan(const PaArgs& a) {
         const int slot = base + t;
         long long cost = 0;
         if (slot < slots) {
-            const int s = find(slot), len = s_q[s + 1] - s_q[s], row0 = (slot - pa_q_slot<pa_tile_rows(HD)>(a, s_q[s], s)) * pa_tile_rows(HD);
+            const int s = find(slot), len = s_q[s + 1] - s_q[s];
+            const int row0 = (slot - pa_q_slot<pa_tile_rows(HD)>(a, s_q[s], s)) * pa_tile_rows(HD);
             if (row0 < len * a.g) {
                 int lo, units;
                 pa_span<pa_tile_rows(HD)>(a, len, s_k[s + 1] - s_k[s], row0, &lo, &units);
@@ -872,7 +873,8 @@ __global__ __launch_bounds__(pa_tile_rows(HD) * 2) __attribute__((amdgpu_waves_p
             int* const ended = (int*)s_turn;  // (where no row of q or out is now)
             bool last = false;
             if (two) {
-                if (threadIdx.x == 0) *ended = __hip_atomic_load(&a.ended[owner], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (threadIdx.x == 0)
+                    *ended = __hip_atomic_load(&a.ended[owner], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 VK_LDS_BARRIER();
                 last = *ended == 1;
                 VK_LDS_BARRIER();
@@ -1279,11 +1281,12 @@ static hipError_t go_few_as(hipStream_t s, const PaArgs& a) {
     const long long most = std::max<long long>(1, std::min<long long>(kFewRanges, kFewMost / pairs));
     const int per = (int)std::max<long long>(step, ((keys + most - 1) / most + step - 1) / step * step);
     const int splits = keys ? (keys + per - 1) / per : 1;
-    hipLaunchKernelGGL((vk_pattn_few<HD, NT, ENDS>), dim3((unsigned)a.hkv, (unsigned)splits, (unsigned)a.n_seq), dim3(256), 0, s, a,
-                       per);
-    if (splits > 1)
-        hipLaunchKernelGGL((vk_pattn_few_join<HD, NT>), dim3((unsigned)(a.max_q * a.g * (HD / 4) + 63) / 64, (unsigned)a.hkv, (unsigned)a.n_seq),
-                           dim3(256), 0, s, a, per, splits);
+    const dim3 grid((unsigned)a.hkv, (unsigned)splits, (unsigned)a.n_seq);
+    hipLaunchKernelGGL((vk_pattn_few<HD, NT, ENDS>), grid, dim3(256), 0, s, a, per);
+    if (splits > 1) {
+        const dim3 join((unsigned)(a.max_q * a.g * (HD / 4) + 63) / 64, (unsigned)a.hkv, (unsigned)a.n_seq);
+        hipLaunchKernelGGL((vk_pattn_few_join<HD, NT>), join, dim3(256), 0, s, a, per, splits);
+    }
     return hipGetLastError();
 }
 

@@ -102,7 +102,8 @@ int vokra_hip_packed_attn_create(vokra_hip_ctx_t* c, size_t max_seq, size_t max_
     p->hq = n_head_q;
     p->hkv = n_head_kv;
     p->hd = head_dim;
-    const size_t ks = places(max_k_rows, kPaKeys, max_seq), qs = places(max_q_rows * (n_head_q / n_head_kv), (size_t)pa_tile_rows((int)head_dim), max_seq);
+    const size_t ks = places(max_k_rows, kPaKeys, max_seq);
+    const size_t qs = places(max_q_rows * (n_head_q / n_head_kv), (size_t)pa_tile_rows((int)head_dim), max_seq);
     struct {
         void** p;
         size_t bytes;
@@ -183,7 +184,6 @@ int vokra_hip_packed_attn_dev(vokra_hip_ctx_t* c, vokra_hip_packed_attn_t* p, si
     a.ended = (int*)(a.start + kPaShares);
     a.plan = (long long*)(a.ended + kPaShares);
     a.part = (float*)p->part;
-    a.q_slots = (int)places(n_q_rows * (size_t)a.g, (size_t)pa_tile_rows((int)p->hd), n_seq);
     a.k_slots = (int)places(n_k_rows, kPaKeys, n_seq);
     PA_TRY(vk::launch_pattn(vk::ctx_stream(c), (int)p->hd, a), "launch(vk_pattn)");
     return VOKRA_HIP_OK;
